@@ -13,15 +13,31 @@ DYNCONV_ERR_TIMEOUT).  Call it once per training step (or set DYNCONV_SYNC_CHECK
 """
 from ._lib import DynconvError, check_device, set_sync_checks
 from .headwise import headwise_dynamic_convolution
+from .linear_attention import decay_linear_attention, decay_linear_attention_fused, decay_linear_attention_step
 from .lowrank import lowrank_dynamic_convolution, lowrank_dynamic_convolution_grouped
 from .modules import LowRankDynamicShortConvolution, QKVLowRankDynamicShortConvolution
 from .parallel import data_parallel, shard_rows
 from .sequence_parallel import headwise_dynamic_convolution_sp, lowrank_dynamic_convolution_sp
+from .step import (
+    convolution_cache,
+    headwise_dynamic_convolution_step,
+    lowrank_dynamic_convolution_grouped_step,
+    lowrank_dynamic_convolution_step,
+)
+from .vocab_loss import linear_cross_entropy
 
 __all__ = [
     "headwise_dynamic_convolution",
     "lowrank_dynamic_convolution",
     "lowrank_dynamic_convolution_grouped",
+    "headwise_dynamic_convolution_step",
+    "lowrank_dynamic_convolution_step",
+    "lowrank_dynamic_convolution_grouped_step",
+    "convolution_cache",
+    "decay_linear_attention",
+    "decay_linear_attention_fused",
+    "decay_linear_attention_step",
+    "linear_cross_entropy",
     "LowRankDynamicShortConvolution",
     "QKVLowRankDynamicShortConvolution",
     "data_parallel",

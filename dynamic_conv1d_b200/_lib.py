@@ -6,6 +6,7 @@ cannot be loaded, every op raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -49,6 +50,16 @@ _SIGNATURES = {
     "dynconv_comm_destroy": (_c_int, [_c_vp]),
     "dynconv_lr_bwd_grouped_dp": (_c_int, [_c_vp] * 10 + [_c_vp, _c_size] + [_c_i64] * 6
                                   + [_c_int, _c_int, _c_vp, _c_vp, _c_vp]),
+    "dynconv_lr_step": (_c_int, [_c_vp] * 7 + [_c_int] + [_c_i64] * 6 + [_c_int, _c_int, _c_vp]),
+    "dynconv_hw_step": (_c_int, [_c_vp] * 6 + [_c_int] + [_c_i64] * 5 + [_c_int, _c_int, _c_vp]),
+    "dynconv_la_workspace_bytes": (_c_size, [_c_i64] * 5 + [_c_int, _c_int]),
+    "dynconv_la_fwd": (_c_int, [_c_vp] * 8 + [_c_vp, _c_size] + [_c_i64] * 5 + [ctypes.c_float, _c_int, _c_vp]),
+    "dynconv_la_bwd": (_c_int, [_c_vp] * 12 + [_c_vp, _c_size] + [_c_i64] * 5 + [ctypes.c_float, _c_int, _c_vp]),
+    "dynconv_la_step": (_c_int, [_c_vp] * 7 + [_c_int, _c_vp] + [_c_i64] * 5 + [ctypes.c_float, _c_int, _c_vp]),
+    "dynconv_vocab_loss_fwd_workspace_bytes": (_c_size, [_c_i64] * 3 + [_c_int]),
+    "dynconv_vocab_loss_fwd": (_c_int, [_c_vp] * 7 + [_c_size] + [_c_i64] * 4 + [_c_int, _c_int, _c_vp]),
+    "dynconv_vocab_loss_bwd_workspace_bytes": (_c_size, [_c_i64] * 3 + [_c_int] * 3),
+    "dynconv_vocab_loss_bwd": (_c_int, [_c_vp] * 9 + [_c_size] + [_c_i64] * 4 + [_c_int, _c_int, _c_vp]),
     "dynconv_cast_f32": (_c_int, [_c_vp, _c_vp, _c_i64, _c_int, _c_vp]),
     "dynconv_umma_selftest": (_c_int, [_c_vp, _c_vp, _c_vp] + [_c_int] * 12 + [_c_vp]),
     "dynconv_wait_selftest": (_c_int, [ctypes.c_uint64, _c_vp, _c_vp]),
@@ -116,6 +127,22 @@ def on_device(fn):
             return fn(ctx, first, *args)
 
     return wrapper
+
+
+_same_device = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """Context in which t's device is current (free when it already is)."""
+    if t.device.index == torch.cuda.current_device():
+        return _same_device
+    return torch.cuda.device(t.device)
+
+
+def raw_stream(t: torch.Tensor) -> int:
+    """The current stream of t's device as an address (``stream_of`` without the Stream object,
+    for calls whose kernels take a few microseconds)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def ptr(t: torch.Tensor | None):

@@ -138,17 +138,17 @@ int lr_tm_bwd_launch(const void* x, const void* z, const void* U, const void* sw
 bool comm_peers(const void* comm, lrtc::DpPeers* out);
 int comm_device(const void* comm);
 
-namespace {
-
-constexpr size_t kAlign = 256;
-constexpr int kMaxGroups = 16;
-size_t align_up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
-
 int check_dtype(int dtype) {
   if (dtype != DYNCONV_DTYPE_BF16 && dtype != DYNCONV_DTYPE_F32)
     return set_error(DYNCONV_ERR_UNSUPPORTED, "dtype %d (expected bf16=0 or f32=1)", dtype);
   return DYNCONV_OK;
 }
+
+namespace {
+
+constexpr size_t kAlign = 256;
+constexpr int kMaxGroups = 16;
+size_t align_up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
 
 int check_common(int64_t B, int64_t T, int64_t D, int64_t W) {
   if (B < 0 || T < 0 || D <= 0) return set_error(DYNCONV_ERR_SHAPE, "bad sizes B=%lld T=%lld D=%lld", (long long)B, (long long)T, (long long)D);
@@ -238,12 +238,6 @@ int report_earlier_timeout(cudaStream_t st) {
                    dev, site);
 }
 
-// First step of every kernel-launching entry point.
-int op_entry(cudaStream_t st) {
-  wire_host_error_word(st);
-  return report_earlier_timeout(st);
-}
-
 int log2_exact(int64_t v) {
   int l = 0;
   while ((int64_t(1) << l) < v) ++l;
@@ -251,6 +245,12 @@ int log2_exact(int64_t v) {
 }
 
 }  // namespace
+
+int op_entry(cudaStream_t st) {
+  wire_host_error_word(st);
+  return report_earlier_timeout(st);
+}
+
 }  // namespace dynconv
 
 using namespace dynconv;

@@ -48,6 +48,12 @@ int ensure_context();
 int encode_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
                            const cuuint64_t* strides_bytes, const cuuint32_t* box);
 
+// First step of every kernel-launching entry point: wires the host-visible error word on
+// a device's first call and reports a kernel that gave up a wait earlier.
+int op_entry(cudaStream_t st);
+// DYNCONV_OK for a known dynconv_dtype.
+int check_dtype(int dtype);
+
 // Counts kernel launches (dynconv_launch_count) -- call once per launch.
 void note_launch(int n = 1);
 

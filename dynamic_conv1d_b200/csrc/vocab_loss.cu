@@ -1,0 +1,310 @@
+// vocab_loss.cu -- the vocabulary loss on the CUDA cores: tiled fp32 products for fp32
+// tensors and for bf16 shapes outside the tensor-core envelope, and the kernel that merges
+// the forward's tiles.  The formulas stand in vocab_loss.cuh.
+#include "vocab_loss.cuh"
+
+namespace dynconv {
+namespace vl {
+
+namespace {
+
+constexpr int kTile = 64;   // rows and columns of a tile
+constexpr int kK = 16;      // inner steps staged at once
+constexpr int kThreads = 256;
+constexpr int kLd = kTile + 4;
+
+enum Mode { kForward, kGrad, kAccumulate, kStore };
+
+// out(m, n) = sum_k A[m*am + k*ak] * B[n*bn + k*bk] over one CTA's 64 x 64 tile and its
+// share blockIdx.z of the inner dimension; 4 x 4 outputs per thread, fp32 throughout.
+struct Gemm {
+  const void *A, *B;
+  int64_t am, ak, bn, bk;
+  int64_t M, N, K, k_share;
+  int64_t col0;       // kForward, kGrad: first vocabulary column of the product
+  void* out;          // kGrad: piece buffer, kStore: tensor, kAccumulate: fp32 [z][M][N]
+  int64_t out_ld;
+  int add;            // kAccumulate: add to what is there
+};
+
+// Stages kTile rows x kK inner steps, transposed to [k][row].  The thread order follows the
+// dense dimension, so that loads coalesce either way.
+template <typename T>
+__device__ __forceinline__ void stage(float* s, const T* src, int64_t rs, int64_t ks, int64_t r0, int64_t rows,
+                                      int64_t k0, int64_t k_end) {
+  for (int i = threadIdx.x; i < kTile * kK; i += kThreads) {
+    int r, k;
+    if (ks == 1) {
+      k = i % kK;
+      r = i / kK;
+    } else {
+      r = i % kTile;
+      k = i / kTile;
+    }
+    const bool in = r0 + r < rows && k0 + k < k_end;
+    s[k * kLd + r] = in ? Elem<T>::to_f(src[(r0 + r) * rs + (k0 + k) * ks]) : 0.f;
+  }
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kThreads) vl_gemm_kernel(const Gemm g, const Problem p) {
+  __shared__ __align__(16) float as[kK * kLd], bs[kK * kLd];
+  const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
+  const int64_t k_begin = blockIdx.z * g.k_share, k_end = min(g.K, k_begin + g.k_share);
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  float acc[4][4] = {};
+  for (int64_t k0 = k_begin; k0 < k_end; k0 += kK) {
+    stage((float*)as, (const T*)g.A, g.am, g.ak, m0, g.M, k0, k_end);
+    stage((float*)bs, (const T*)g.B, g.bn, g.bk, n0, g.N, k0, k_end);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kK; ++k) {
+      const float4 a = *reinterpret_cast<const float4*>(as + k * kLd + ty * 4);
+      const float4 b = *reinterpret_cast<const float4*>(bs + k * kLd + tx * 4);
+      const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = m0 + ty * 4 + i;
+    const bool row = m < g.M;
+    if constexpr (MODE == kForward) {
+      // 16 threads (one half warp) share a row: its maximum, then its sum of exponentials
+      const int64_t t = row ? p.target[m] : -1;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t n = n0 + tx * 4 + j;
+        if (n < g.N) mx = fmaxf(mx, acc[i][j]);
+        if (row && n < g.N && n == t) p.tgt[m] = acc[i][j];
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + tx * 4 + j < g.N) sum += expf(acc[i][j] - mx);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (row && tx == 0) p.part[(int64_t)blockIdx.y * p.N + m] = make_float2(mx, sum);
+    } else if constexpr (MODE == kGrad) {
+      if (!row) continue;
+      const int64_t t = p.target[m];
+      const float f = row_factor(p, m, t), lse = p.lse[m];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t n = n0 + tx * 4 + j;
+        if (n >= g.N) continue;
+        const float pr = expf(acc[i][j] - lse) - (g.col0 + n == t ? 1.f : 0.f);
+        ((T*)g.out)[m * g.out_ld + n] = Elem<T>::from_f(f == 0.f ? 0.f : pr * f);
+      }
+    } else {
+      if (!row) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t n = n0 + tx * 4 + j;
+        if (n >= g.N) continue;
+        if constexpr (MODE == kAccumulate) {
+          float* o = (float*)g.out + ((int64_t)blockIdx.z * g.M + m) * g.out_ld + n;
+          *o = g.add ? *o + acc[i][j] : acc[i][j];
+        } else {
+          ((T*)g.out)[m * g.out_ld + n] = Elem<T>::from_f(acc[i][j]);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int MODE>
+int gemm(Gemm g, const Problem& p, int z, const char* what) {
+  g.k_share = ((g.K + z - 1) / z + kK - 1) / kK * kK;
+  const int64_t gx = (g.M + kTile - 1) / kTile, gy = (g.N + kTile - 1) / kTile;
+  if (gx > INT32_MAX || gy > 65535) return set_error(DYNCONV_ERR_SHAPE, "%s: too many tiles", what);
+  vl_gemm_kernel<T, MODE><<<dim3((unsigned)gx, (unsigned)gy, (unsigned)z), kThreads, 0, p.st>>>(g, p);
+  DYNCONV_CHECK_LAUNCH(what);
+  return DYNCONV_OK;
+}
+
+// Merges the tiles' (maximum, sum) of 32 rows per CTA: lane = row, warps take every eighth
+// tile; then the rows' losses.
+__global__ void __launch_bounds__(256) vl_merge_kernel(const Problem p, int64_t tiles) {
+  __shared__ float2 part[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t n = (int64_t)blockIdx.x * 32 + lane;
+  float mx = -INFINITY, sum = 0.f;
+  if (n < p.N) {
+    for (int64_t i = w; i < tiles; i += 8) {
+      const float2 v = p.part[i * p.N + n];
+      const float m2 = fmaxf(mx, v.x);
+      if (m2 == -INFINITY) continue;  // nothing finite so far: exp(-inf) adds nothing
+      sum = sum * expf(mx - m2) + v.y * expf(v.x - m2);
+      mx = m2;
+    }
+  }
+  part[w][lane] = make_float2(mx, sum);
+  __syncthreads();
+  if (w != 0 || n >= p.N) return;
+  for (int i = 1; i < 8; ++i) {
+    const float2 v = part[i][lane];
+    const float m2 = fmaxf(mx, v.x);
+    if (m2 == -INFINITY) continue;
+    sum = sum * expf(mx - m2) + v.y * expf(v.x - m2);
+    mx = m2;
+  }
+  const float lse = mx + logf(sum);
+  p.lse[n] = lse;
+  const int64_t t = p.target[n];
+  // an ignored row adds nothing; a target outside the vocabulary makes the loss NaN
+  float row = 0.f;
+  if (t != p.ignore) row = (t >= 0 && t < p.V) ? lse - p.tgt[n] : __int_as_float(0x7fc00000);
+  if (p.reduction == kNone)
+    p.loss[n] = row;
+  else
+    p.tgt[n] = row;
+}
+
+// Sums the rows' losses in a fixed order (one CTA) and counts the rows that take part.
+__global__ void __launch_bounds__(1024) vl_total_kernel(const Problem p) {
+  __shared__ double ssum[32];
+  __shared__ long long scnt[32];
+  double sum = 0.0;
+  long long cnt = 0;
+  for (int64_t n = threadIdx.x; n < p.N; n += 1024) {
+    if (p.reduction != kNone) sum += (double)p.tgt[n];
+    cnt += p.target[n] != p.ignore;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    ssum[threadIdx.x >> 5] = sum;
+    scnt[threadIdx.x >> 5] = cnt;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  sum = 0.0;
+  cnt = 0;
+  for (int i = 0; i < 32; ++i) {
+    sum += ssum[i];
+    cnt += scnt[i];
+  }
+  p.stats[0] = (float)sum;
+  p.stats[1] = (float)cnt;
+  if (p.reduction == kSum) p.loss[0] = (float)sum;
+  if (p.reduction == kMean) p.loss[0] = (float)(sum / (double)cnt);  // no row left: 0/0, NaN
+}
+
+template <typename T>
+int fwd(const Problem& p) {
+  Gemm g{};
+  g.A = p.hidden, g.am = p.D, g.ak = 1;
+  g.B = p.weight, g.bn = p.D, g.bk = 1;
+  g.M = p.N, g.N = p.V, g.K = p.D;
+  int s = gemm<T, kForward>(g, p, 1, "vl_gemm_kernel (forward)");
+  return s ? s : merge_launch(p, (p.V + kTile - 1) / kTile);
+}
+
+template <typename T>
+int bwd(const Problem& p, const Plan& pl, int dtype) {
+  int s;
+  for (int64_t v0 = 0; v0 < p.V; v0 += pl.piece) {
+    const int64_t vp = p.V - v0 < pl.piece ? p.V - v0 : pl.piece;
+    const T* w = (const T*)p.weight + v0 * p.D;
+    Gemm g{};
+    g.A = p.hidden, g.am = p.D, g.ak = 1;
+    g.B = w, g.bn = p.D, g.bk = 1;
+    g.M = p.N, g.N = vp, g.K = p.D, g.col0 = v0;
+    g.out = p.piece, g.out_ld = pl.pitch;
+    if ((s = gemm<T, kGrad>(g, p, 1, "vl_gemm_kernel (logits' gradient)"))) return s;
+    if (p.dweight) {
+      Gemm gw{};
+      gw.A = p.piece, gw.am = 1, gw.ak = pl.pitch;
+      gw.B = p.hidden, gw.bn = 1, gw.bk = p.D;
+      gw.M = vp, gw.N = p.D, gw.K = p.N;
+      gw.out_ld = p.D;
+      if (pl.z_w == 1) {
+        gw.out = (T*)p.dweight + v0 * p.D;
+        if ((s = gemm<T, kStore>(gw, p, 1, "vl_gemm_kernel (weight gradient)"))) return s;
+      } else {
+        gw.out = p.acc_w;
+        if ((s = gemm<T, kAccumulate>(gw, p, pl.z_w, "vl_gemm_kernel (weight gradient)"))) return s;
+        if ((s = reduce_partials_launch(p.acc_w, pl.z_w, vp * p.D, nullptr, (T*)p.dweight + v0 * p.D, dtype, p.st)))
+          return s;
+      }
+    }
+    if (p.dhidden) {
+      Gemm gh{};
+      gh.A = p.piece, gh.am = pl.pitch, gh.ak = 1;
+      gh.B = w, gh.bn = 1, gh.bk = p.D;
+      gh.M = p.N, gh.N = p.D, gh.K = vp;
+      gh.out = p.acc_h, gh.out_ld = p.D, gh.add = v0 > 0;
+      if ((s = gemm<T, kAccumulate>(gh, p, pl.z_h, "vl_gemm_kernel (hidden gradient)"))) return s;
+    }
+  }
+  return finish_hidden(p, pl, dtype);
+}
+
+}  // namespace
+
+int finish_hidden(const Problem& p, const Plan& pl, int dtype) {
+  if (!p.dhidden) return DYNCONV_OK;
+  return reduce_partials_launch(p.acc_h, pl.z_h, p.N * p.D, nullptr, p.dhidden, dtype, p.st);
+}
+
+int merge_launch(const Problem& p, int64_t tiles) {
+  if (p.N > 0) {
+    vl_merge_kernel<<<(unsigned)((p.N + 31) / 32), 256, 0, p.st>>>(p, tiles);
+    DYNCONV_CHECK_LAUNCH("vl_merge_kernel");
+  }
+  vl_total_kernel<<<1, 1024, 0, p.st>>>(p);
+  DYNCONV_CHECK_LAUNCH("vl_total_kernel");
+  return DYNCONV_OK;
+}
+
+int tile_cols(bool tc) { return tc ? 256 : kTile; }
+
+// A piece is as wide as keeps its buffer near 256 MB (twice the L2: wide enough that the
+// products' tiles fill the GPU many times over, small beside the weight and its gradient)
+// and at least 4096 columns.  Inner dimensions are spread over several CTAs per tile while
+// the tiles of a product are fewer than two per SM and each share keeps 512 steps.
+Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc) {
+  const int64_t elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4;
+  Plan pl;
+  const int64_t cols = ((int64_t)256 << 20) / (elem * (N > 0 ? N : 1)) / 1024 * 1024;
+  pl.piece = cols < 4096 ? 4096 : cols;
+  if (pl.piece > V) pl.piece = V;
+  // equal pieces, whole tiles
+  const int64_t n = (V + pl.piece - 1) / pl.piece;
+  pl.piece = ((V + n - 1) / n + 255) / 256 * 256;
+  if (pl.piece > V) pl.piece = V;
+  pl.pitch = (pl.piece + 63) / 64 * 64;
+  const int64_t tm = tc ? 128 : kTile, tn = tc ? 256 : kTile;
+  auto share = [&](int64_t rows, int64_t cols_, int64_t inner) {
+    const int64_t tiles = ((rows + tm - 1) / tm) * ((cols_ + tn - 1) / tn);
+    int64_t z = 2 * (int64_t)sm_count() / (tiles > 0 ? tiles : 1);
+    if (z > inner / 512) z = inner / 512;
+    if (z > 16) z = 16;
+    return (int)(z < 1 ? 1 : z);
+  };
+  pl.z_h = share(N, D, pl.piece);
+  pl.z_w = share(pl.piece, D, N);
+  return pl;
+}
+
+int simple_fwd(const Problem& p, int dtype) {
+  return dtype == DYNCONV_DTYPE_BF16 ? fwd<__nv_bfloat16>(p) : fwd<float>(p);
+}
+
+int simple_bwd(const Problem& p, const Plan& pl, int dtype) {
+  return dtype == DYNCONV_DTYPE_BF16 ? bwd<__nv_bfloat16>(p, pl, dtype) : bwd<float>(p, pl, dtype);
+}
+
+}  // namespace vl
+}  // namespace dynconv

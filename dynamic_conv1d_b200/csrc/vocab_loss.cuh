@@ -1,0 +1,73 @@
+// vocab_loss.cuh -- what the vocabulary-loss kernels share.
+//
+// Softmax cross entropy of hidden [N, D] against a vocabulary weight [V, D] without the
+// logits [N, V] in memory.  With l = hidden weight^T:
+//     lse_n = log sum_v exp(l_nv),  loss_n = lse_n - l_{n,t_n}
+//     dl_nv = (exp(l_nv - lse_n) - [v = t_n]) * g_n
+//     dhidden = dl weight,  dweight = dl^T hidden
+// Forward: one matrix product whose epilogue keeps, of each tile, every row's maximum and
+// sum of exponentials (fp32); a second kernel merges the tiles.  Backward, piece of the
+// vocabulary by piece: the product again, with dl rounded to the tensors' type into a
+// piece buffer, then its two products.  dhidden accumulates in fp32 over the pieces.
+#pragma once
+
+#include "common.cuh"
+
+namespace dynconv {
+namespace vl {
+
+enum Reduction { kNone = 0, kSum = 1, kMean = 2 };
+
+struct Problem {
+  const void* hidden;       // [N, D]
+  const void* weight;       // [V, D]
+  const int64_t* target;    // [N]
+  int64_t N, D, V;
+  int64_t ignore;
+  int reduction;
+  // forward
+  float* lse;               // [N]
+  float* loss;              // [N] (kNone) or [1]
+  float* stats;             // [2]: sum of the rows' losses, number of rows that count
+  float2* part;             // [tiles][N]: maximum and sum of exponentials of a tile's row
+  float* tgt;               // [N]: the target's logit
+  // backward
+  const float* dloss;       // [N] (kNone) or [1]
+  void* dhidden;            // [N, D] or null
+  void* dweight;            // [V, D] or null
+  void* piece;              // [N, pitch]: dl of one piece of the vocabulary
+  float* acc_h;             // [z_h][N][D] fp32
+  float* acc_w;             // [z_w][piece rows][D] fp32, z_w > 1
+  cudaStream_t st;
+};
+
+// How the backward is cut: columns of a piece, its row pitch, and over how many CTAs a
+// tile's inner dimension is spread where there are few tiles.
+struct Plan {
+  int64_t piece, pitch;
+  int z_h, z_w;
+};
+
+// A row's factor: 0 where the target is ignored or outside the vocabulary.
+__device__ __forceinline__ float row_factor(const Problem& p, int64_t n, int64_t t) {
+  if (t == p.ignore || t < 0 || t >= p.V) return 0.f;
+  if (p.reduction == kNone) return p.dloss[n];
+  return p.reduction == kSum ? p.dloss[0] : p.dloss[0] / p.stats[1];
+}
+
+int tile_cols(bool tc);  // columns of the vocabulary in one forward tile
+bool tc_supported(const Problem& p, int dtype);
+Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc);
+int merge_launch(const Problem& p, int64_t tiles);
+// cast of acc_h's z_h parts into dhidden
+int finish_hidden(const Problem& p, const Plan& pl, int dtype);
+
+int simple_fwd(const Problem& p, int dtype);
+int simple_bwd(const Problem& p, const Plan& pl, int dtype);
+int tc_fwd(const Problem& p);
+int tc_bwd(const Problem& p, const Plan& pl);
+
+}  // namespace vl
+
+int reduce_partials_launch(const float* part, int P, int64_t n, float* out_f32, void* out, int dtype, cudaStream_t st);
+}  // namespace dynconv

@@ -247,6 +247,89 @@ int dynconv_lr_bwd_grouped_dp(const void* x, const void* z, const void* U, const
  * dU_fp32.to(U.dtype), lowrank.py:294, and dstatic_accum.to(...), headwise.py:305). */
 int dynconv_cast_f32(const float* src, void* dst, int64_t n, int dtype, void* stream);
 
+/* ------------------------------------------------------- steps of one token */
+
+/* One token of the convolutions for B sequences, on a cache of each sequence's last
+ * W-1 inputs, for generating text (no reference counterpart: the reference runs whole
+ * sequences only).
+ *   x, y      : [B, C], C = G*D channels (hw_step: C = D)
+ *   cache     : [n_rows, W-1, C], oldest input first: x[:, T-(W-1):] after a prompt of T
+ *               tokens (zeros where T < W-1).  Updated in place: the oldest input leaves,
+ *               x enters.  May be NULL when W = 1.
+ *   slots     : NULL (batch row b uses cache row b; n_rows >= B) or [B] indices of
+ *               slot_bytes = 4 or 8 bytes into a pool of n_rows cache rows.  No index may
+ *               occur twice.  A row whose index lies outside the pool touches no cache
+ *               and its output is zero (padding rows of a captured batch).
+ * Other arguments as for dynconv_lr_fwd_grouped (z [B, G*R], U [G, R, W*D],
+ * static_w [G, W, D]; R <= 64) and dynconv_hw_fwd (weight [B, H, W]; any H that divides D).
+ * B <= 65535. */
+int dynconv_lr_step(const void* x, const void* z, const void* U, const void* static_w, void* cache, void* y,
+                    const void* slots, int slot_bytes,
+                    int64_t B, int64_t n_rows, int64_t D, int64_t R, int64_t W, int64_t G,
+                    int dtype, int residual, void* stream);
+int dynconv_hw_step(const void* x, const void* weight, const void* static_w, void* cache, void* y,
+                    const void* slots, int slot_bytes,
+                    int64_t B, int64_t n_rows, int64_t D, int64_t H, int64_t W,
+                    int dtype, int residual, void* stream);
+
+/* ---------------------------------------------- linear attention with decay */
+
+/* Linear attention whose state decays by exp(log_decay[h]) per token in head h:
+ *     S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t
+ * (no reference counterpart; it consumes the convolved queries, keys and values).
+ *   q, k [B,T,H,dk], v, o [B,T,H,dv] in `dtype`, dense in the last dimension, any other
+ *   strides: `strides` holds the element strides of batch, time and head for q, k, v, o
+ *   (12 numbers), so the thirds of a fused [B,T,3*H*d] buffer are read in place.
+ *   log_decay [H] float32, <= 0 (a factor of at most one; -inf forgets at once).
+ *   initial_state (NULL = zero), final_state (NULL = not wanted): [B,H,dk,dv] float32.
+ * dk, dv in 1..256, B*H <= 65535.  T = 0 copies the state. */
+size_t dynconv_la_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype, int backward);
+int dynconv_la_fwd(const void* q, const void* k, const void* v, const float* log_decay, const float* initial_state,
+                   void* o, float* final_state, const int64_t* strides,
+                   void* workspace, size_t workspace_bytes,
+                   int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, float scale, int dtype, void* stream);
+/* Gradients for upstream d_o and d_final_state (NULL = zero).  `strides`: batch, time and
+ * head for q, k, v, d_o, dq, d_k, d_v (21 numbers).  d_initial_state may be NULL.  The decay
+ * is a constant of the model: it has no gradient. */
+int dynconv_la_bwd(const void* q, const void* k, const void* v, const float* log_decay, const float* initial_state,
+                   const void* d_o, const float* d_final_state, void* dq, void* d_k, void* d_v,
+                   float* d_initial_state, const int64_t* strides, void* workspace, size_t workspace_bytes,
+                   int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, float scale, int dtype, void* stream);
+/* One token for B sequences: q, k [B,H,dk], v [B,H,dv] (`strides`: batch and head of q, k, v,
+ * 6 numbers), o [B,H,dv] dense, state [n_rows,H,dk,dv] float32 updated in place; slots as for
+ * dynconv_lr_step. */
+int dynconv_la_step(const void* q, const void* k, const void* v, float* state, const float* log_decay, void* o,
+                    const void* slots, int slot_bytes, const int64_t* strides,
+                    int64_t B, int64_t n_rows, int64_t H, int64_t dk, int64_t dv, float scale,
+                    int dtype, void* stream);
+
+/* ------------------------------------------------------------ vocabulary loss */
+
+/* Softmax cross entropy of hidden [N,D] against weight [V,D] (logits = hidden weight^T),
+ * computed in pieces of the vocabulary without the [N,V] logits in memory (no reference
+ * counterpart; the loss of a language model built on the convolutions).
+ *   target [N] int64.  A row whose target is ignore_index counts for nothing; any other
+ *   target outside [0,V) makes the loss NaN and contributes no gradient.
+ *   reduction: 0 none (loss [N]), 1 sum, 2 mean over the rows that count (loss [1]; NaN
+ *   when none does).  loss, lse [N] and stats [2] are float32; lse and stats are kept for
+ *   the backward (stats: sum of the rows' losses, number of rows that count).
+ * V <= 4194304. */
+size_t dynconv_vocab_loss_fwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype);
+int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t* target,
+                           float* loss, float* lse, float* stats, void* workspace, size_t workspace_bytes,
+                           int64_t N, int64_t D, int64_t V, int64_t ignore_index, int reduction,
+                           int dtype, void* stream);
+/* Gradients for dloss ([N] or [1] float32, as loss).  dhidden [N,D] or dweight [V,D] may be
+ * NULL (not wanted).  The logits' gradient is rounded to `dtype` before its two products
+ * (bf16 tensor-core operands), which accumulate in float32; no atomics. */
+size_t dynconv_vocab_loss_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype,
+                                              int want_dhidden, int want_dweight);
+int dynconv_vocab_loss_bwd(const void* hidden, const void* weight, const int64_t* target,
+                           const float* lse, const float* stats, const float* dloss,
+                           void* dhidden, void* dweight, void* workspace, size_t workspace_bytes,
+                           int64_t N, int64_t D, int64_t V, int64_t ignore_index, int reduction,
+                           int dtype, void* stream);
+
 /* ------------------------------------------------------------- diagnostics */
 
 /* One tcgen05.mma (kind::f16, bf16 in, fp32 accumulate) sequence on operands

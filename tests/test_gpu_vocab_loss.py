@@ -1,0 +1,235 @@
+"""GPU: the vocabulary loss and its gradients against the definition in 64 bits.
+
+Tolerances (relative 2-norm):
+  loss : fp32 from fp32 logits whose terms are exact products; a logit's sum of D <= 512
+         terms is off by at most 512 * 2^-24 of their absolute sum, which the tests keep
+         below 16: 16 * 512 * 2^-24 = 4.9e-4 absolute at the worst, 1e-5 relative in the
+         loss's own size at the usual square root of it;
+  bf16 gradients: the logits' gradient rounded once and the result once, each by less than
+         2^-9 of the values in the root mean square: 2 * 2^-9;
+  fp32 gradients: sums of up to 512 terms at 2^-24, and exp() of logits off by the same
+         relative amount: 1024 * 2^-24.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from dynamic_conv1d_b200 import check_device, linear_cross_entropy
+
+pytestmark = pytest.mark.gpu
+
+GRAD = {torch.bfloat16: 2.0**-8, torch.float32: 1024 * 2.0**-24}
+LOSS = 1e-5
+BOTH = [torch.bfloat16, torch.float32]
+IGNORE = -100
+
+
+def rel(a, b):
+    a, b = a.detach().double(), b.detach().double()
+    n, d = torch.linalg.vector_norm(b), torch.linalg.vector_norm(a - b)
+    return (d / n if n > 0 else d).item()
+
+
+def make(N, D, V, dtype, seed=0, scale=1.5, ignored=0.2):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    h = torch.randn(N, D, device="cuda", generator=g).to(dtype)
+    w = (torch.randn(V, D, device="cuda", generator=g) * scale * D**-0.5).to(dtype)
+    t = torch.randint(0, V, (N,), device="cuda", generator=g)
+    drop = torch.rand(N, device="cuda", generator=g) < ignored
+    if N:
+        drop[0] = False
+    return h, w, torch.where(drop, torch.full_like(t, IGNORE), t)
+
+
+def definition(h, w, t, up, reduction):
+    """(loss, dhidden, dweight) in 64 bits for upstream gradient `up`."""
+    h, w = h.double(), w.double()
+    keep = t != IGNORE
+    l = h @ w.T
+    lse = torch.logsumexp(l, 1)
+    rows = torch.where(keep, lse - l.gather(1, t.clamp(min=0)[:, None])[:, 0], 0.0)
+    n = keep.sum()
+    loss = {"none": rows, "sum": rows.sum(), "mean": rows.sum() / n}[reduction]
+    f = (up.double() if reduction != "mean" else up.double() / n).expand(len(t)) * keep
+    d = torch.exp(l - lse[:, None])
+    d.scatter_add_(1, t.clamp(min=0)[:, None], -torch.ones_like(d[:, :1]))
+    d *= f[:, None]
+    return loss, d @ w, d.T @ h
+
+
+def check(h, w, t, reduction="mean", up=None, loss_tol=LOSS):
+    if up is None:
+        up = torch.tensor(1.0, device="cuda")
+    own = [x.detach().requires_grad_() for x in (h, w)]
+    loss = linear_cross_entropy(*own, t, reduction=reduction)
+    loss.backward(up)
+    check_device(loss)
+    rl, rh, rw = definition(h, w, t, up, reduction)
+    assert loss.dtype == torch.float32 and loss.shape == rl.shape
+    got = (rel(loss, rl), rel(own[0].grad, rh), rel(own[1].grad, rw))
+    assert got[0] <= loss_tol and got[1] <= GRAD[h.dtype] and got[2] <= GRAD[h.dtype], got
+    return loss.detach(), own[0].grad, own[1].grad
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("N,D,V", [(1, 8, 2), (1, 64, 1), (3, 16, 7), (5, 13, 30), (64, 64, 64), (65, 64, 65), (127, 72, 300), (128, 128, 256),
+                                   (129, 136, 257), (200, 256, 1000), (257, 512, 511), (300, 33, 513), (2, 512, 5000), (1000, 8, 300)])
+def test_sizes(dtype, N, D, V):
+    check(*make(N, D, V, dtype, seed=N + V))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_reductions(dtype, reduction):
+    h, w, t = make(150, 64, 500, dtype)
+    up = torch.randn(150, device="cuda") if reduction == "none" else torch.tensor(0.37, device="cuda")
+    check(h, w, t, reduction, up)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_shapes_and_expanded_upstream(dtype):
+    h, w, t = make(60, 64, 200, dtype)
+    h3, t3 = h.view(4, 15, 64).requires_grad_(), t.view(4, 15)
+    rows = linear_cross_entropy(h3, w, t3, reduction="none")
+    assert rows.shape == (4, 15)
+    rows.sum().backward()  # an expanded scalar as upstream gradient
+    _, rh, _ = definition(h, w, t, torch.tensor(1.0, device="cuda"), "sum")
+    assert rel(h3.grad.view(60, 64), rh) <= GRAD[dtype]
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_several_pieces(dtype):
+    """More rows and words than one piece of the vocabulary holds."""
+    N, V = (33000, 9001) if dtype == torch.bfloat16 else (17000, 9001)
+    check(*make(N, 16, V, dtype))
+
+
+def test_long_inner_dimensions():
+    """Few tiles, long sums: the inner dimension is spread over several CTAs."""
+    check(*make(20, 128, 30000, torch.bfloat16))
+    check(*make(20, 64, 9000, torch.float32))
+    check(*make(6000, 64, 100, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_gradient_of_one_side(dtype):
+    h, w, t = make(100, 64, 300, dtype)
+    _, rh, rw = check(h, w, t)
+    a = h.detach().requires_grad_()
+    linear_cross_entropy(a, w, t).backward()
+    assert torch.equal(a.grad, rh)
+    b = w.detach().requires_grad_()
+    linear_cross_entropy(h, b, t).backward()
+    assert torch.equal(b.grad, rw)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_all_rows_ignored(dtype):
+    h, w, t = make(70, 64, 100, dtype)
+    t = torch.full_like(t, IGNORE)
+    for reduction, want in (("mean", float("nan")), ("sum", 0.0)):
+        own = [x.detach().requires_grad_() for x in (h, w)]
+        loss = linear_cross_entropy(*own, t, reduction=reduction)
+        loss.backward()
+        assert (loss.isnan() if want != want else loss == want).item()
+        assert own[0].grad.count_nonzero() == 0 and own[1].grad.count_nonzero() == 0
+    assert linear_cross_entropy(h, w, t, reduction="none").count_nonzero() == 0
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_target_outside_the_vocabulary(dtype):
+    h, w, t = make(70, 64, 100, dtype, ignored=0.0)
+    t[3], t[4] = 100, -1
+    rows = linear_cross_entropy(h, w, t, reduction="none")
+    assert rows[3].isnan() and rows[4].isnan() and rows.isnan().sum() == 2
+    own = [x.detach().requires_grad_() for x in (h, w)]
+    linear_cross_entropy(*own, t).backward()
+    assert own[0].grad[3].count_nonzero() == 0 and own[0].grad.isfinite().all() and own[1].grad.isfinite().all()
+    # another index to ignore: -1 is then an ignored row, -100 is outside
+    t2 = t.clone()
+    t2[3] = 5
+    assert linear_cross_entropy(h, w, t2, ignore_index=-1).isfinite()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_large_logits(dtype):
+    """Logits of several hundred: nothing overflows, and a row dominated by one word is exact
+    there.  The loss is then a difference of logits of about 400 computed with 2^-24 * 64 each."""
+    h, w, t = make(90, 64, 400, dtype, scale=100.0)
+    own = [x.detach().requires_grad_() for x in (h, w)]
+    loss = linear_cross_entropy(*own, t)
+    loss.backward()
+    rl, rh, rw = definition(h, w, t, torch.tensor(1.0, device="cuda"), "mean")
+    assert rel(loss, rl) <= 1e-4
+    # exp() of logits off by 400 * 64 * 2^-24 = 1.5e-3
+    tol = GRAD[dtype] + 1.5e-3
+    assert rel(own[0].grad, rh) <= tol and rel(own[1].grad, rw) <= tol
+
+
+def test_infinite_and_nan_rows():
+    h, w, t = make(80, 64, 300, torch.bfloat16, ignored=0.0)
+    h = h.clone()
+    h[7, 3] = float("nan")
+    rows = linear_cross_entropy(h, w, t, reduction="none")
+    assert rows[7].isnan() and rows.isnan().sum() == 1
+
+
+def test_gradient_against_differences():
+    """Central difference in fp32 along a direction: step 1e-2, error of the third order
+    (1e-4 of the derivative's size, measured on the definition in 64 bits) plus the fp32
+    loss's own rounding 1e-6 / 1e-2."""
+    h, w, t = make(40, 32, 60, torch.float32)
+    for i in range(2):
+        x = [h, w]
+        a = x[i].detach().requires_grad_()
+        x[i] = a
+        linear_cross_entropy(x[0], x[1], t).backward()
+        e = torch.randn(a.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+        e /= torch.linalg.vector_norm(e)
+        with torch.no_grad():
+            f = lambda s: linear_cross_entropy(*[y + s * e if j == i else y for j, y in enumerate((h, w))], t).double()  # noqa: E731
+            dif = (f(1e-2) - f(-1e-2)) / 2e-2
+        ana = (a.grad.double() * e.double()).sum()
+        assert abs(dif - ana) <= 1e-4 * torch.linalg.vector_norm(a.grad) + 1e-4
+
+
+def test_empty_batch():
+    h, w, t = make(0, 64, 100, torch.bfloat16)
+    w.requires_grad_()
+    loss = linear_cross_entropy(h, w, t, reduction="sum")
+    loss.backward()
+    assert loss == 0 and w.grad.count_nonzero() == 0
+    assert linear_cross_entropy(h, w, t).isnan()
+    assert linear_cross_entropy(h, w, t, reduction="none").shape == (0,)
+
+
+def test_weight_of_another_type():
+    h, w, t = make(50, 64, 100, torch.bfloat16)
+    w32 = w.float().requires_grad_()
+    linear_cross_entropy(h, w32, t).backward()
+    _, _, rw = definition(h, w, t, torch.tensor(1.0, device="cuda"), "mean")
+    assert w32.grad.dtype == torch.float32 and rel(w32.grad, rw) <= GRAD[torch.bfloat16]
+
+
+def test_same_bits_again_and_other_stream():
+    h, w, t = make(300, 128, 3000, torch.bfloat16)
+    one = check(h, w, t)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        own = [x.detach().requires_grad_() for x in (h, w)]
+        loss = linear_cross_entropy(*own, t)
+        loss.backward()
+    torch.cuda.current_stream().wait_stream(st)
+    for a, b in zip(one, (loss.detach(), own[0].grad, own[1].grad)):
+        assert torch.equal(a, b)
+
+
+def test_refusals():
+    h, w, t = make(10, 64, 50, torch.bfloat16)
+    good = dict(hidden=h, weight=w, target=t)
+    for bad in (dict(hidden=h.cpu()), dict(hidden=h.half(), weight=w.half()), dict(hidden=h[:, ::2]), dict(weight=w[:, :32]), dict(weight=w.T),
+                dict(target=t[:5]), dict(target=t.int()), dict(target=t.cpu()), dict(reduction="max")):
+        with pytest.raises((AssertionError, TypeError, RuntimeError)):
+            linear_cross_entropy(**(good | bad))
