@@ -53,7 +53,7 @@ int ensure_context() {
 }
 
 int encode_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
-                           const cuuint64_t* strides_bytes, const cuuint32_t* box) {
+                           const cuuint64_t* strides_bytes, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
   int s = ensure_context();
   if (s) return s;
   using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -71,8 +71,7 @@ int encode_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const c
   if (!fn) return set_error(DYNCONV_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides_bytes,
-                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(DYNCONV_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return DYNCONV_OK;
 }
@@ -93,10 +92,12 @@ unsigned int lr_tc_error_word();
 unsigned int lr_bwd_tm_error_word();
 unsigned int hw_tma_error_word();
 unsigned int selftest_error_word();
+unsigned int vl_tc_error_word();
 int lr_tc_error_word_wire(unsigned int* host_word);
 int lr_bwd_tm_error_word_wire(unsigned int* host_word);
 int hw_tma_error_word_wire(unsigned int* host_word);
 int selftest_error_word_wire(unsigned int* host_word);
+int vl_tc_error_word_wire(unsigned int* host_word);
 bool hw_tma_supported(int64_t D, int64_t H, int W, int log2hs, int dtype, const void* const* ptrs, int nptrs);
 int hw_tma_partial_rows(int64_t B, int64_t T, int64_t D, int log2hs);
 int hw_tma_fwd_launch(const void* x, const void* w, const void* sw, void* y, int64_t B, int64_t T, int64_t D, int64_t H,
@@ -208,7 +209,7 @@ void wire_host_error_word(cudaStream_t st) {
   }
   unsigned int* mine = static_cast<unsigned int*>(dp) + dev;
   if (lr_tc_error_word_wire(mine) || lr_bwd_tm_error_word_wire(mine) || hw_tma_error_word_wire(mine) ||
-      selftest_error_word_wire(mine)) {
+      selftest_error_word_wire(mine) || vl_tc_error_word_wire(mine)) {
     cudaGetLastError();
     return;
   }
@@ -231,6 +232,7 @@ int report_earlier_timeout(cudaStream_t st) {
     (void)lr_bwd_tm_error_word();
     (void)selftest_error_word();
     (void)hw_tma_error_word();
+    (void)vl_tc_error_word();
   }
   return set_error(DYNCONV_ERR_TIMEOUT,
                    "a kernel launched earlier on device %d gave up a bounded wait (site %u): the outputs of that "
@@ -289,12 +291,13 @@ int dynconv_check_device(void* stream) {
       __atomic_exchange_n(words + dev, 0u, __ATOMIC_ACQ_REL);
   }
   // every word is read (and so cleared) before the first non-zero one is reported
-  const unsigned int words[4] = {lr_tc_error_word(), lr_bwd_tm_error_word(), selftest_error_word(),
-                                 hw_tma_error_word()};
-  static const char* const kFile[4] = {"lowrank forward", "lowrank backward", "self-test", "headwise"};
+  const unsigned int words[] = {lr_tc_error_word(), lr_bwd_tm_error_word(), selftest_error_word(),
+                                hw_tma_error_word(), vl_tc_error_word()};
+  static const char* const kFile[] = {"lowrank forward", "lowrank backward", "self-test", "headwise",
+                                      "vocabulary loss"};
   for (unsigned int v : words)
     if (v == 0xFFFFFFFFu) return set_error(DYNCONV_ERR_CUDA, "could not read the device error word");
-  for (int i = 0; i < 4; ++i)
+  for (size_t i = 0; i < sizeof(words) / sizeof(words[0]); ++i)
     if (words[i] != 0)
       return set_error(DYNCONV_ERR_TIMEOUT, "a device-side bounded wait gave up (%s kernel, site %u)", kFile[i],
                        words[i]);

@@ -224,7 +224,8 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
 
 size_t dynconv_vocab_loss_fwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype) {
   if (check_loss(N, D, V, 0, dtype)) return 0;
-  const int64_t tiles = (V + vl::tile_cols(false) - 1) / vl::tile_cols(false);
+  // the CUDA-core tiles are the narrower ones: enough for either path
+  const int64_t tiles = (V + vl::tile_cols(false) - 1) / vl::tile_cols(false) + 2;
   return align_up((size_t)tiles * N * sizeof(float2)) + align_up((size_t)N * sizeof(float));
 }
 
@@ -248,13 +249,16 @@ int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t
     return set_error(DYNCONV_ERR_WORKSPACE, "vocab_loss_fwd: workspace %zu < %zu bytes", workspace_bytes, need);
   p.tgt = (float*)workspace;
   p.part = (float2*)((char*)workspace + align_up((size_t)N * sizeof(float)));
-  return vl::simple_fwd(p, dtype);
+  return vl::tc_supported(p, dtype) ? vl::tc_fwd(p) : vl::simple_fwd(p, dtype);
 }
 
 size_t dynconv_vocab_loss_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int want_dhidden,
                                               int want_dweight) {
   if (check_loss(N, D, V, 0, dtype) || N == 0) return 0;
-  return loss_backward_bytes(vl::plan(N, D, V, dtype, false), N, D, dtype, want_dhidden, want_dweight).total();
+  // alignment can move a call to the CUDA-core path: enough for either
+  const size_t a = loss_backward_bytes(vl::plan(N, D, V, dtype, false), N, D, dtype, want_dhidden, want_dweight).total();
+  const size_t b = loss_backward_bytes(vl::plan(N, D, V, dtype, true), N, D, dtype, want_dhidden, want_dweight).total();
+  return a > b ? a : b;
 }
 
 int dynconv_vocab_loss_bwd(const void* hidden, const void* weight, const int64_t* target, const float* lse,
@@ -273,19 +277,20 @@ int dynconv_vocab_loss_bwd(const void* hidden, const void* weight, const int64_t
   }
   if (!hidden || !weight || !target || !lse || !stats || !dloss)
     return set_error(DYNCONV_ERR_ARGUMENT, "vocab_loss_bwd: null tensor");
-  const vl::Plan pl = vl::plan(N, D, V, dtype, false);
-  const LossBackwardBytes b = loss_backward_bytes(pl, N, D, dtype, dhidden != nullptr, dweight != nullptr);
-  if (!workspace || workspace_bytes < b.total())
-    return set_error(DYNCONV_ERR_WORKSPACE, "vocab_loss_bwd: workspace %zu < %zu bytes", workspace_bytes, b.total());
   vl::Problem p{};
   p.hidden = hidden, p.weight = weight, p.target = target;
   p.N = N, p.D = D, p.V = V, p.ignore = ignore_index, p.reduction = reduction;
   p.lse = const_cast<float*>(lse), p.stats = const_cast<float*>(stats), p.dloss = dloss;
   p.dhidden = dhidden, p.dweight = dweight, p.st = st;
   p.piece = workspace;
+  const bool tc = vl::tc_supported(p, dtype);
+  const vl::Plan pl = vl::plan(N, D, V, dtype, tc);
+  const LossBackwardBytes b = loss_backward_bytes(pl, N, D, dtype, dhidden != nullptr, dweight != nullptr);
+  if (!workspace || workspace_bytes < b.total())
+    return set_error(DYNCONV_ERR_WORKSPACE, "vocab_loss_bwd: workspace %zu < %zu bytes", workspace_bytes, b.total());
   p.acc_h = (float*)((char*)workspace + b.piece);
   p.acc_w = (float*)((char*)workspace + b.piece + b.acc_h);
-  return vl::simple_bwd(p, pl, dtype);
+  return tc ? vl::tc_bwd(p, pl) : vl::simple_bwd(p, pl, dtype);
 }
 
 }  // extern "C"

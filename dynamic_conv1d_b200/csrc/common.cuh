@@ -42,11 +42,12 @@ int sm_count();
 // has made no runtime call yet -- autograd's backward worker, say -- has none.
 int ensure_context();
 
-// Encodes a tiled, no-swizzle, zero-fill bf16 TMA descriptor (cuTensorMapEncodeTiled,
-// reached through the runtime's driver entry point).  `strides_bytes` has rank-1
-// entries (dimension 0 is dense).  DYNCONV_OK or DYNCONV_ERR_CUDA.
+// Encodes a tiled, zero-fill bf16 TMA descriptor (cuTensorMapEncodeTiled, reached through
+// the runtime's driver entry point).  `strides_bytes` has rank-1 entries (dimension 0 is
+// dense).  DYNCONV_OK or DYNCONV_ERR_CUDA.
 int encode_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
-                           const cuuint64_t* strides_bytes, const cuuint32_t* box);
+                           const cuuint64_t* strides_bytes, const cuuint32_t* box,
+                           CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_NONE);
 
 // First step of every kernel-launching entry point: wires the host-visible error word on
 // a device's first call and reports a kernel that gave up a wait earlier.
@@ -330,6 +331,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
   return mbar_wait_slow(bar, parity, site, abort_flag);
 }
 
+// After a wait gave up: waits, again for a limited time, for a phase that copies or products
+// already in flight will complete.
+static __device__ __noinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait_suspend(bar, parity, kWaitSuspendNs))
+    if (globaltimer_ns() - t0 > 100000000ull) break;  // 0.1 s
+}
+
 // TMA tiled 3-D load into shared memory, completion counted on `bar`.
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0,
                                             int c1, int c2, uint64_t policy) {
@@ -357,6 +366,15 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
       "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group.L2::cache_hint [%0, {%2, %3, %4}], [%1], %5;" ::"l"(
           reinterpret_cast<uint64_t>(map)),
       "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+      : "memory");
+}
+
+// TMA tiled 2-D load into shared memory, completion counted on `bar`.
+__device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::
+          "r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
       : "memory");
 }
 
@@ -507,6 +525,22 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// 32 lanes x 32 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // 32 lanes x 8 consecutive 32-bit columns.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
   uint32_t r[8];
@@ -573,6 +607,19 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
+}
+
+// 128-byte-swizzled K-major operand (TMA box of 64 K elements, so rows of 128 bytes and
+// 8-row groups of 1024): a K step of 16 elements advances the start address by 32 bytes.
+__device__ __forceinline__ uint64_t make_smem_desc_sw128_k(uint32_t smem_addr) {
+  return make_smem_desc_sw128(smem_addr, 16, 1024);
+}
+
+// 2^x, at most 2 units in the last place off.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Instruction descriptor for kind::f16 with bf16 A/B and fp32 D.

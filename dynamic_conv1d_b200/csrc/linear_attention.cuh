@@ -60,7 +60,8 @@ struct Params {
 
 // log2 of the decay factor.  A factor of zero is kept finite, so that 0 * log stays 0.
 __device__ __forceinline__ double log2_decay(const float* log_decay, int h) {
-  return fmax((double)log_decay[h] * 1.4426950408889634, -16384.0);
+  const double l2 = (double)log_decay[h] * 1.4426950408889634;
+  return l2 < -16384.0 ? -16384.0 : l2;  // (a NaN stays one)
 }
 
 // A state's factor over n tokens as a sum of two floats.  The same factor multiplies the

@@ -85,10 +85,11 @@ __global__ void __launch_bounds__(kThreads) vl_gemm_kernel(const Gemm g, const P
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mx *= kLog2e;
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (n0 + tx * 4 + j < g.N) sum += expf(acc[i][j] - mx);
+        if (n0 + tx * 4 + j < g.N) sum += exp2f(fmaf(acc[i][j], kLog2e, -mx));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (row && tx == 0) p.part[(int64_t)blockIdx.y * p.N + m] = make_float2(mx, sum);
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(256) vl_merge_kernel(const Problem p, int64_t 
       const float2 v = p.part[i * p.N + n];
       const float m2 = fmaxf(mx, v.x);
       if (m2 == -INFINITY) continue;  // nothing finite so far: exp(-inf) adds nothing
-      sum = sum * expf(mx - m2) + v.y * expf(v.x - m2);
+      sum = sum * exp2f(mx - m2) + v.y * exp2f(v.x - m2);
       mx = m2;
     }
   }
@@ -153,10 +154,10 @@ __global__ void __launch_bounds__(256) vl_merge_kernel(const Problem p, int64_t 
     const float2 v = part[i][lane];
     const float m2 = fmaxf(mx, v.x);
     if (m2 == -INFINITY) continue;
-    sum = sum * expf(mx - m2) + v.y * expf(v.x - m2);
+    sum = sum * exp2f(mx - m2) + v.y * exp2f(v.x - m2);
     mx = m2;
   }
-  const float lse = mx + logf(sum);
+  const float lse = (float)(((double)mx + (double)log2f(sum)) * 0.6931471805599453);
   p.lse[n] = lse;
   const int64_t t = p.target[n];
   // an ignored row adds nothing; a target outside the vocabulary makes the loss NaN
@@ -268,7 +269,7 @@ int merge_launch(const Problem& p, int64_t tiles) {
   return DYNCONV_OK;
 }
 
-int tile_cols(bool tc) { return tc ? 256 : kTile; }
+int tile_cols(bool tc) { return tc ? 128 : kTile; }
 
 // A piece is as wide as keeps its buffer near 256 MB (twice the L2: wide enough that the
 // products' tiles fill the GPU many times over, small beside the weight and its gradient)

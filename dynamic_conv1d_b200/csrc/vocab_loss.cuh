@@ -16,6 +16,8 @@
 namespace dynconv {
 namespace vl {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 enum Reduction { kNone = 0, kSum = 1, kMean = 2 };
 
 struct Problem {
@@ -29,7 +31,8 @@ struct Problem {
   float* lse;               // [N]
   float* loss;              // [N] (kNone) or [1]
   float* stats;             // [2]: sum of the rows' losses, number of rows that count
-  float2* part;             // [tiles][N]: maximum and sum of exponentials of a tile's row
+  float2* part;             // [tiles][N]: of a tile's row, m = max * log2(e) rounded, and
+                            // sum of 2^(l * log2(e) - m)
   float* tgt;               // [N]: the target's logit
   // backward
   const float* dloss;       // [N] (kNone) or [1]

@@ -1,0 +1,406 @@
+// vocab_loss_tc.cu -- the vocabulary loss on the tensor cores (bf16).
+//
+// One persistent kernel computes out(m, n) = sum_k A(m, k) B(n, k) for all four products;
+// only the operands' majors and the epilogue differ:
+//     forward       A = hidden [N][D],      B = weight [V][D]      -> row maxima and sums
+//     logits' grad  A = hidden,             B = weight piece       -> dl (bf16, piece buffer)
+//     dhidden       A = dl [N][piece],      B = weight piece^T     -> fp32, added up over pieces
+//     dweight       A = dl^T,               B = hidden^T           -> bf16
+// K-major operands are TMA boxes of 64 K elements x rows, the transposed ones boxes of 64
+// rows x 64 K steps; both land in 128-byte-swizzled tiles that tcgen05.mma reads as they
+// are, so nothing is ever transposed in memory.
+//
+// A CTA runs one producer warp (TMA ring of kStages), one MMA warp and eight epilogue warps
+// (two per TMEM lane quarter, half of the columns each) on 128 x 256 tiles; two
+// accumulators of 256 TMEM columns let a tile's epilogue run under the next tile's products.
+#include "vocab_loss.cuh"
+
+namespace dynconv {
+namespace vl {
+
+namespace {
+
+constexpr int kM = 128, kN = 256, kKB = 64;  // tile, and inner elements per stage
+constexpr int kStages = 4;
+constexpr int kEpiWarps = 8;
+constexpr int kTcThreads = 64 + 32 * kEpiWarps;
+constexpr uint32_t kABytes = kM * kKB * 2, kBBytes = kN * kKB * 2, kStageBytes = kABytes + kBBytes;
+constexpr uint32_t kAtom = 64 * kKB * 2;  // one 64 x 64 box
+constexpr int kSmem = kStages * (int)kStageBytes + 1024;
+constexpr int kHalf = kN / 2;  // columns of one epilogue warp; a forward tile's partials are per half
+
+enum TcMode { kTcForward, kTcGrad, kTcAdd, kTcStore };
+
+struct TcGemm {
+  int64_t M, N;        // extents of the output
+  int k_blocks;        // 64-element blocks of the inner dimension
+  int m_tiles, n_tiles, z;
+  int group;           // m tiles that share a sweep over n: consecutive tiles walk a group's rows first
+  int64_t col0;        // kTcGrad: first vocabulary column
+  void* out;
+  int64_t out_ld;
+  int add;             // kTcAdd: add to what is there
+};
+
+struct Tile {
+  int m, n, z, kb0, kb1;
+};
+
+__device__ __forceinline__ Tile tile_at(const TcGemm& g, int t) {
+  Tile r;
+  const int plane = g.m_tiles * g.n_tiles;
+  r.z = t / plane;
+  t -= r.z * plane;
+  const int grp = t / (g.group * g.n_tiles);
+  t -= grp * g.group * g.n_tiles;
+  const int rows = min(g.group, g.m_tiles - grp * g.group);
+  r.n = t / rows;
+  r.m = grp * g.group + (t - r.n * rows);
+  r.kb0 = (int)((int64_t)g.k_blocks * r.z / g.z);
+  r.kb1 = (int)((int64_t)g.k_blocks * (r.z + 1) / g.z);
+  return r;
+}
+
+template <int MODE>
+__device__ __forceinline__ void epilogue_columns(const TcGemm& g, const Problem& p, const float (&v)[32], int64_t row,
+                                                 int64_t col, bool row_in, float f, float lse2, int64_t t, int z) {
+  // col: first of the 32 columns; dimensions of the outputs are multiples of 8 (kTcGrad: the
+  // piece buffer's pitch is), so whole groups of 8 are in or out
+  if constexpr (MODE == kTcGrad) {
+    float d[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) d[j] = f != 0.f ? ex2(fmaf(v[j], kLog2e, -lse2)) * f : 0.f;  // (an ignored row's NaN stays out)
+    const int64_t at = t - g.col0 - col;
+    if (at >= 0 && at < 32) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j == at) d[j] -= f;
+    }
+    if (!row_in) return;
+    __nv_bfloat16* o = (__nv_bfloat16*)g.out + row * g.out_ld + col;
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      if (col + j >= g.N) break;
+      uint4 u;
+      u.x = pack_bf16x2(d[j], d[j + 1]), u.y = pack_bf16x2(d[j + 2], d[j + 3]);
+      u.z = pack_bf16x2(d[j + 4], d[j + 5]), u.w = pack_bf16x2(d[j + 6], d[j + 7]);
+      *reinterpret_cast<uint4*>(o + j) = u;
+    }
+  } else if constexpr (MODE == kTcAdd) {
+    if (!row_in) return;
+    float* o = (float*)g.out + ((int64_t)z * g.M + row) * g.out_ld + col;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      if (col + j >= g.N) break;
+      float4 u = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      if (g.add) {
+        const float4 w = *reinterpret_cast<const float4*>(o + j);
+        u.x += w.x, u.y += w.y, u.z += w.z, u.w += w.w;
+      }
+      *reinterpret_cast<float4*>(o + j) = u;
+    }
+  } else if constexpr (MODE == kTcStore) {
+    if (!row_in) return;
+    __nv_bfloat16* o = (__nv_bfloat16*)g.out + row * g.out_ld + col;
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      if (col + j >= g.N) break;
+      uint4 u;
+      u.x = pack_bf16x2(v[j], v[j + 1]), u.y = pack_bf16x2(v[j + 2], v[j + 3]);
+      u.z = pack_bf16x2(v[j + 4], v[j + 5]), u.w = pack_bf16x2(v[j + 6], v[j + 7]);
+      *reinterpret_cast<uint4*>(o + j) = u;
+    }
+  }
+}
+
+template <int MODE, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    vl_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                 const __grid_constant__ TcGemm g, const __grid_constant__ Problem p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem_1024(smem_raw);
+  __shared__ uint64_t full_bar[kStages], empty_bar[kStages], accf_bar[2], acce_bar[2], drain_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_tiles = g.m_tiles * g.n_tiles * g.z;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&accf_bar[a], 1);
+      mbar_init(&acce_bar[a], kEpiWarps);
+    }
+    mbar_init(&drain_bar, 1);
+    abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tensormap(&amap);
+    prefetch_tensormap(&bmap);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool dead = false;
+      for (int i = blockIdx.x; i < n_tiles && !dead; i += gridDim.x) {
+        const Tile t = tile_at(g, i);
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&empty_bar[s], ((it / kStages) & 1) ^ 1, kErrWaitProducer, &abort_flag)) {
+            dead = true;
+            break;
+          }
+          uint8_t* a = smem + s * kStageBytes;
+          uint8_t* b = a + kABytes;
+          mbar_arrive_expect_tx(&full_bar[s], kStageBytes);
+          if constexpr (A_MN) {
+#pragma unroll
+            for (int j = 0; j < kM / 64; ++j)
+              tma_load_2d(a + j * kAtom, &amap, &full_bar[s], t.m * kM + j * 64, kb * kKB);
+          } else {
+            tma_load_2d(a, &amap, &full_bar[s], kb * kKB, t.m * kM);
+          }
+          if constexpr (B_MN) {
+#pragma unroll
+            for (int j = 0; j < kN / 64; ++j)
+              tma_load_2d(b + j * kAtom, &bmap, &full_bar[s], t.n * kN + j * 64, kb * kKB);
+          } else {
+            tma_load_2d(b, &bmap, &full_bar[s], kb * kKB, t.n * kN);
+          }
+        }
+      }
+      // a wait gave up: let the copies in flight land before the shared memory is given back
+      if (abort_flag)
+        for (int j = max(0, it - kStages); j < it; ++j)
+          mbar_drain(&full_bar[j % kStages], (j / kStages) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = make_idesc_bf16(kM, kN, A_MN, B_MN);
+    int it = 0, n = 0;
+    bool dead = false;
+    for (int i = blockIdx.x; i < n_tiles && !dead; i += gridDim.x, ++n) {
+      const Tile t = tile_at(g, i);
+      const int a = n & 1;
+      if (!mbar_wait(&acce_bar[a], ((n >> 1) & 1) ^ 1, kErrWaitMma, &abort_flag)) break;
+      tc_fence_after();
+      for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+        const int s = it % kStages;
+        if (!mbar_wait(&full_bar[s], (it / kStages) & 1, kErrWaitMma, &abort_flag)) {
+          dead = true;
+          break;
+        }
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t as = smem_u32(smem + s * kStageBytes), bs = as + kABytes;
+#pragma unroll
+          for (int k = 0; k < kKB / 16; ++k) {
+            const uint64_t ad = A_MN ? make_smem_desc_sw128(as + k * 2048, kAtom, 1024) : make_smem_desc_sw128_k(as + k * 32);
+            const uint64_t bd = B_MN ? make_smem_desc_sw128(bs + k * 2048, kAtom, 1024) : make_smem_desc_sw128_k(bs + k * 32);
+            umma_f16(tmem + a * kN, ad, bd, idesc, (kb > t.kb0 || k > 0) ? 1u : 0u);
+          }
+          umma_commit(&empty_bar[s]);
+          if (kb == t.kb1 - 1) umma_commit(&accf_bar[a]);
+        }
+        __syncwarp();
+      }
+    }
+    if (abort_flag) {  // the products in flight, before their accumulators are given back
+      if (lane == 0) {
+        umma_commit(&drain_bar);
+        mbar_drain(&drain_bar, 0);
+      }
+      __syncwarp();
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    bool dead = false;
+    int n = 0;
+    for (int i = blockIdx.x; i < n_tiles; i += gridDim.x, ++n) {
+      const Tile t = tile_at(g, i);
+      const int a = n & 1;
+      const int64_t row = (int64_t)t.m * kM + q * 32 + lane;
+      const int64_t col0 = (int64_t)t.n * kN + half * kHalf;
+      const bool row_in = row < g.M;
+      float f = 0.f, lse2 = 0.f;
+      int64_t target = -1;
+      if constexpr (MODE == kTcForward || MODE == kTcGrad) {
+        if (row_in) target = p.target[row];
+        if constexpr (MODE == kTcGrad) {
+          if (row_in) {
+            f = row_factor(p, row, target);
+            lse2 = p.lse[row] * kLog2e;
+          }
+        }
+      }
+      if (!dead) dead = !mbar_wait(&accf_bar[a], (n >> 1) & 1, kErrWaitEpilogue, &abort_flag);
+      tc_fence_after();
+      if (!dead) {
+        const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + a * kN + half * kHalf;
+        float m2 = -INFINITY, sum = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < kHalf; c += 32) {
+          float v[32];
+          tmem_ld32(base + c, v);
+          tmem_ld_wait();
+          if constexpr (MODE == kTcForward) {
+            const int64_t left = g.N - (col0 + c);  // columns that are there
+            float mx = -INFINITY;
+            if (left >= 32) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (j >= left) v[j] = -INFINITY;
+                mx = fmaxf(mx, v[j]);
+              }
+            }
+            const float m_new = fmaxf(m2, mx * kLog2e);
+            if (m_new > -INFINITY) {
+              float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                s0 += ex2(fmaf(v[j], kLog2e, -m_new));
+                s1 += ex2(fmaf(v[j + 1], kLog2e, -m_new));
+              }
+              sum = fmaf(sum, ex2(m2 - m_new), s0 + s1);
+              m2 = m_new;
+            }
+            const int64_t at = target - (col0 + c);
+            if (row_in && at >= 0 && at < 32 && at < left) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j == at) p.tgt[row] = v[j];
+            }
+          } else {
+            epilogue_columns<MODE>(g, p, v, row, col0 + c, row_in, f, lse2, target, t.z);
+          }
+        }
+        if constexpr (MODE == kTcForward) {
+          if (row_in) p.part[((int64_t)t.n * 2 + half) * g.M + row] = make_float2(m2, sum);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acce_bar[a]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// A row-major [rows][cols] bf16 matrix as boxes of 64 columns x box_rows rows, 128-byte swizzle.
+int matrix_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  return encode_tensor_map_bf16(map, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int MODE, bool A_MN, bool B_MN>
+int launch(const CUtensorMap& a, const CUtensorMap& b, TcGemm g, const Problem& p, const char* what) {
+  const int64_t mt = (g.M + kM - 1) / kM, nt = (g.N + kN - 1) / kN;
+  if (mt * nt * g.z > INT32_MAX) return set_error(DYNCONV_ERR_SHAPE, "%s: too many tiles", what);
+  g.m_tiles = (int)mt, g.n_tiles = (int)nt;
+  if (g.group > g.m_tiles) g.group = g.m_tiles;
+  const int tiles = g.m_tiles * g.n_tiles * g.z;
+  const int grid = tiles < sm_count() ? tiles : sm_count();
+  cudaError_t e = cudaFuncSetAttribute(vl_tc_kernel<MODE, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_status(e, "cudaFuncSetAttribute(vl_tc)");
+  }
+  vl_tc_kernel<MODE, A_MN, B_MN><<<grid, kTcThreads, kSmem, p.st>>>(a, b, g, p);
+  DYNCONV_CHECK_LAUNCH(what);
+  return DYNCONV_OK;
+}
+
+// Rows of hidden (a group) that stay in L2 while the vocabulary is swept over them: half of it.
+int row_group(int64_t D) {
+  const int64_t g = ((int64_t)64 << 20) / (kM * D * 2);
+  return g < 1 ? 1 : (int)(g < 4096 ? g : 4096);
+}
+
+}  // namespace
+
+bool tc_supported(const Problem& p, int dtype) {
+  if (dtype != DYNCONV_DTYPE_BF16 || p.D % 8 != 0) return false;
+  const void* ptrs[] = {p.hidden, p.weight, p.dhidden, p.dweight, p.piece};
+  for (const void* q : ptrs)
+    if (reinterpret_cast<uintptr_t>(q) & 15) return false;
+  return true;
+}
+
+int tc_fwd(const Problem& p) {
+  CUtensorMap a, b;
+  int s;
+  if ((s = matrix_map(&a, p.hidden, p.D, p.N, p.D, kM))) return s;
+  if ((s = matrix_map(&b, p.weight, p.D, p.V, p.D, kN))) return s;
+  TcGemm g{};
+  g.M = p.N, g.N = p.V, g.k_blocks = (int)((p.D + kKB - 1) / kKB), g.z = 1, g.group = row_group(p.D);
+  if ((s = launch<kTcForward, false, false>(a, b, g, p, "vl_tc_kernel (forward)"))) return s;
+  return merge_launch(p, (p.V + kN - 1) / kN * 2);
+}
+
+int tc_bwd(const Problem& p, const Plan& pl) {
+  int s;
+  CUtensorMap hk, hm;
+  if ((s = matrix_map(&hk, p.hidden, p.D, p.N, p.D, kM))) return s;
+  if ((s = matrix_map(&hm, p.hidden, p.D, p.N, p.D, 64))) return s;
+  const int d_blocks = (int)((p.D + kKB - 1) / kKB);
+  for (int64_t v0 = 0; v0 < p.V; v0 += pl.piece) {
+    const int64_t vp = p.V - v0 < pl.piece ? p.V - v0 : pl.piece;
+    const __nv_bfloat16* w = (const __nv_bfloat16*)p.weight + v0 * p.D;
+    // maps of exactly this piece: what lies beyond it reads as zero
+    CUtensorMap wk, wm, pk, pm;
+    if ((s = matrix_map(&wk, w, p.D, vp, p.D, kN))) return s;
+    if ((s = matrix_map(&wm, w, p.D, vp, p.D, 64))) return s;
+    if ((s = matrix_map(&pk, p.piece, vp, p.N, pl.pitch, kM))) return s;
+    if ((s = matrix_map(&pm, p.piece, vp, p.N, pl.pitch, 64))) return s;
+    TcGemm g{};
+    g.M = p.N, g.N = vp, g.k_blocks = d_blocks, g.z = 1, g.group = row_group(p.D);
+    g.col0 = v0, g.out = p.piece, g.out_ld = pl.pitch;
+    if ((s = launch<kTcGrad, false, false>(hk, wk, g, p, "vl_tc_kernel (logits' gradient)"))) return s;
+    if (p.dweight) {
+      __nv_bfloat16* dw = (__nv_bfloat16*)p.dweight + v0 * p.D;
+      TcGemm gw{};
+      gw.M = vp, gw.N = p.D, gw.k_blocks = (int)((p.N + kKB - 1) / kKB), gw.z = pl.z_w, gw.group = 1, gw.out_ld = p.D;
+      if (pl.z_w == 1) {
+        gw.out = dw;
+        if ((s = launch<kTcStore, true, true>(pm, hm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
+      } else {
+        gw.out = p.acc_w;
+        if ((s = launch<kTcAdd, true, true>(pm, hm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
+        if ((s = reduce_partials_launch(p.acc_w, pl.z_w, vp * p.D, nullptr, dw, DYNCONV_DTYPE_BF16, p.st))) return s;
+      }
+    }
+    if (p.dhidden) {
+      TcGemm gh{};
+      gh.M = p.N, gh.N = p.D, gh.k_blocks = (int)((vp + kKB - 1) / kKB), gh.group = 1;
+      // the first piece fills every share; a short last one may have fewer blocks than shares
+      gh.z = pl.z_h < gh.k_blocks ? pl.z_h : gh.k_blocks;
+      gh.out = p.acc_h, gh.out_ld = p.D, gh.add = v0 > 0;
+      if ((s = launch<kTcAdd, false, true>(pk, wm, gh, p, "vl_tc_kernel (hidden gradient)"))) return s;
+    }
+  }
+  return finish_hidden(p, pl, DYNCONV_DTYPE_BF16);
+}
+
+}  // namespace vl
+
+DYNCONV_DEFINE_ERROR_ACCESSOR(vl_tc_error_word)
+
+}  // namespace dynconv
