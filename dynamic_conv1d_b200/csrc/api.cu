@@ -93,11 +93,13 @@ unsigned int lr_bwd_tm_error_word();
 unsigned int hw_tma_error_word();
 unsigned int selftest_error_word();
 unsigned int vl_tc_error_word();
+unsigned int la_tc_error_word();
 int lr_tc_error_word_wire(unsigned int* host_word);
 int lr_bwd_tm_error_word_wire(unsigned int* host_word);
 int hw_tma_error_word_wire(unsigned int* host_word);
 int selftest_error_word_wire(unsigned int* host_word);
 int vl_tc_error_word_wire(unsigned int* host_word);
+int la_tc_error_word_wire(unsigned int* host_word);
 bool hw_tma_supported(int64_t D, int64_t H, int W, int log2hs, int dtype, const void* const* ptrs, int nptrs);
 int hw_tma_partial_rows(int64_t B, int64_t T, int64_t D, int log2hs);
 int hw_tma_fwd_launch(const void* x, const void* w, const void* sw, void* y, int64_t B, int64_t T, int64_t D, int64_t H,
@@ -209,7 +211,8 @@ void wire_host_error_word(cudaStream_t st) {
   }
   unsigned int* mine = static_cast<unsigned int*>(dp) + dev;
   if (lr_tc_error_word_wire(mine) || lr_bwd_tm_error_word_wire(mine) || hw_tma_error_word_wire(mine) ||
-      selftest_error_word_wire(mine) || vl_tc_error_word_wire(mine)) {
+      selftest_error_word_wire(mine) || vl_tc_error_word_wire(mine) ||
+      la_tc_error_word_wire(mine)) {
     cudaGetLastError();
     return;
   }
@@ -233,6 +236,7 @@ int report_earlier_timeout(cudaStream_t st) {
     (void)selftest_error_word();
     (void)hw_tma_error_word();
     (void)vl_tc_error_word();
+    (void)la_tc_error_word();
   }
   return set_error(DYNCONV_ERR_TIMEOUT,
                    "a kernel launched earlier on device %d gave up a bounded wait (site %u): the outputs of that "
@@ -292,9 +296,9 @@ int dynconv_check_device(void* stream) {
   }
   // every word is read (and so cleared) before the first non-zero one is reported
   const unsigned int words[] = {lr_tc_error_word(), lr_bwd_tm_error_word(), selftest_error_word(),
-                                hw_tma_error_word(), vl_tc_error_word()};
+                                hw_tma_error_word(), vl_tc_error_word(), la_tc_error_word()};
   static const char* const kFile[] = {"lowrank forward", "lowrank backward", "self-test", "headwise",
-                                      "vocabulary loss"};
+                                      "vocabulary loss", "linear attention"};
   for (unsigned int v : words)
     if (v == 0xFFFFFFFFu) return set_error(DYNCONV_ERR_CUDA, "could not read the device error word");
   for (size_t i = 0; i < sizeof(words) / sizeof(words[0]); ++i)

@@ -38,7 +38,7 @@ int check_step(int64_t B, int64_t n_rows, int64_t D, int64_t W, const void* slot
 int check_attention(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype) {
   int s;
   if ((s = check_dtype(dtype))) return s;
-  if (B < 0 || T < 0 || H <= 0 || B * H > kMaxRows || T > INT32_MAX)
+  if (B < 0 || T < 0 || H <= 0 || B * H > kMaxRows || T > (1 << 30))
     return set_error(DYNCONV_ERR_SHAPE, "linear attention: bad sizes B=%lld T=%lld H=%lld", (long long)B, (long long)T,
                      (long long)H);
   if (dk < 1 || dk > la::kMaxDim || dv < 1 || dv > la::kMaxDim)
@@ -90,12 +90,13 @@ size_t la_seg_bytes(const la::Params& p) {
 }
 
 int la_run(la::Params& p, int dtype, void* ws, size_t ws_bytes, cudaStream_t st) {
-  la::simple_plan(&p);
+  const bool tc = la::tc_supported(p, dtype);
+  tc ? la::tc_plan(&p) : la::simple_plan(&p);
   const size_t need = la_seg_bytes(p);
   if (need && (!ws || ws_bytes < need))
     return set_error(DYNCONV_ERR_WORKSPACE, "linear attention: workspace %zu < %zu bytes", ws_bytes, need);
   p.seg = (float*)ws;
-  return la::simple_launch(p, dtype, st);
+  return tc ? la::tc_launch(p, st) : la::simple_launch(p, dtype, st);
 }
 
 int check_loss(int64_t N, int64_t D, int64_t V, int reduction, int dtype) {
@@ -162,8 +163,12 @@ int dynconv_hw_step(const void* x, const void* weight, const void* static_w, voi
 size_t dynconv_la_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype, int backward) {
   if (check_attention(B, T, H, dk, dv, dtype) || B * T == 0) return 0;
   la::Params p = backward ? la_backward_params(B, T, H, dk, dv, 1.f) : la_forward_params(B, T, H, dk, dv, 1.f);
+  // strides and alignment decide the path at the call: enough for either
   la::simple_plan(&p);
-  return la_seg_bytes(p);
+  const size_t simple = la_seg_bytes(p);
+  la::tc_plan(&p);
+  const size_t tc = la_seg_bytes(p);
+  return simple > tc ? simple : tc;
 }
 
 int dynconv_la_fwd(const void* q, const void* k, const void* v, const float* log_decay, const float* initial_state,

@@ -112,10 +112,14 @@ __global__ void __launch_bounds__(kThreads) la_simple_kernel(const __grid_consta
       for (int j = 0; j < kC; ++j) {
         const float a_0 = as[ty * (kC + 1) + j], a_1 = as[(ty + 16) * (kC + 1) + j];
         const float w_0 = ws[j * (kC + 1) + tx], w_1 = ws[j * (kC + 1) + tx + 16];
-        o1[0][0] = fmaf(a_0, w_0, o1[0][0]);
-        o1[0][1] = fmaf(a_0, w_1, o1[0][1]);
-        o1[1][0] = fmaf(a_1, w_0, o1[1][0]);
-        o1[1][1] = fmaf(a_1, w_1, o1[1][1]);
+        if (j <= ty) {  // a later token's w may be inf or NaN: not even times zero
+          o1[0][0] = fmaf(a_0, w_0, o1[0][0]);
+          o1[0][1] = fmaf(a_0, w_1, o1[0][1]);
+        }
+        if (j <= ty + 16) {
+          o1[1][0] = fmaf(a_1, w_0, o1[1][0]);
+          o1[1][1] = fmaf(a_1, w_1, o1[1][1]);
+        }
       }
       for (int d = 0; d < dx; ++d) {
         const float x0 = xs[ty * (dx + 1) + d], x1 = xs[(ty + 16) * (dx + 1) + d];
@@ -313,7 +317,7 @@ int scan_launch(const Params& p, int chunk, cudaStream_t st) {
 }
 
 // Cuts chains until there are about four CTAs for each SM, with eight chunks at least in a segment.
-int simple_plan(Params* p) {
+void simple_plan(Params* p) {
   const int64_t chunks = (p->T + kC - 1) / kC;
   int64_t chains = 0;
   for (int r = 0; r < p->n_roles; ++r) chains += (int64_t)p->B * p->H * ((p->role[r].dw + kSlice - 1) / kSlice);
@@ -322,7 +326,6 @@ int simple_plan(Params* p) {
   if (seg < 1) seg = 1;
   p->chunks_per_seg = (int)((chunks + seg - 1) / seg);
   p->n_seg = (int)((chunks + p->chunks_per_seg - 1) / p->chunks_per_seg);
-  return kC;
 }
 
 namespace {

@@ -85,11 +85,11 @@ __device__ __forceinline__ float* seg_state(const Params& p, int role, int seg, 
 // Launches the scan over segment states (role.s_in -> p.seg in place; chunk = tokens per chunk).
 int scan_launch(const Params& p, int chunk, cudaStream_t st);
 // CUDA-core kernels: any type, strides and widths up to kMaxDim.
-int simple_plan(Params* p);  // chooses n_seg / chunks_per_seg; returns the chunk length
+void simple_plan(Params* p);  // chooses n_seg and chunks_per_seg
 int simple_launch(const Params& p, int dtype, cudaStream_t st);
 // tcgen05 kernels: see tc_supported for their envelope.
 bool tc_supported(const Params& p, int dtype);
-int tc_plan(Params* p);
+void tc_plan(Params* p);
 int tc_launch(const Params& p, cudaStream_t st);
 
 int step_launch(const View& q, const View& k, const View& v, float* state, const float* log_decay, void* o,

@@ -1,0 +1,569 @@
+// linear_attention_tc.cu -- linear attention with a decay for each head on the tensor cores
+// (bf16, widths up to 128).  The formulas stand in linear_attention.cuh.
+//
+// A CTA runs one segment of one chain: a role, a batch row and head, and 64 columns of w.
+// Chunks have 128 tokens.  Per chunk four products (tcgen05, fp32 accumulators in TMEM):
+//     Sc = X Y^T            128 x 128   both operands as TMA laid them down (K-major)
+//     O1 = A W              A = Sc under the decay mask, bf16, written back to TMEM
+//     O2 = X S              S = the state before the chunk, bf16 in shared memory
+//     KV = Y^T W'           W' = W weighted by the decays to the chunk's end
+// and out = a_scale O1 + (row factor) O2.  The state itself stays in registers in fp32 (lane
+// = row of S, 64 columns): S <- g^L S + KV.  W' is a product of a bf16 value and a weight, so
+// its rounding to bf16 would cost the state its precision: it is split into NS bf16 parts
+// (two: 2^-17 of each term, three: 2^-25, when the state goes back to the caller).
+//
+// Warps: a producer (TMA rings: x and y two deep, w NW deep), an MMA issuer, and three groups of
+// four: masks (Sc -> A), state (KV -> S), and edge (W -> W', and the outputs).  The issuer runs
+//     A(i-1) ready: O1(i-1);  Sc(i);  S(i) ready: O2(i);  W'(i) ready: KV(i)
+// so that while the mask group works on chunk i, the pipe has O2 and KV of the same chunk.
+//
+// A masked score is zero whatever its value was, but 0 * inf in O1 is NaN: a value of w that is
+// not finite is taken out of the tile and marks the rows that may see it (the slow path
+// of the edge group), so rows before it stay clean.
+#include "linear_attention.cuh"
+
+namespace dynconv {
+namespace la {
+
+namespace {
+
+constexpr int kC = 128;     // tokens of a chunk
+constexpr int kSlice = 64;  // columns of w per CTA
+constexpr int kTcThreads = 64 + 3 * 128;
+constexpr uint32_t kBox = 64 * kC * 2;  // one TMA box: 128 rows of 64 bf16
+constexpr int kMaxMaps = kMaxRoles * 3;
+
+// TMEM columns
+constexpr uint32_t kColSc = 0, kColA = 128, kColKv = 192, kColO1 = 320, kColO2 = 384, kTmemCols = 512;
+
+struct TcMaps {
+  CUtensorMap m[kMaxMaps];  // [role][x, y, w]
+};
+
+template <int DX, int NS>
+struct Smem {
+  static constexpr int kNW = NS == 3 ? 2 : 3;  // depth of the w ring (shared-memory bound at DX = 128)
+  static constexpr uint32_t kX = DX / 64 * kBox;
+  static constexpr uint32_t kOffX = 0;
+  static constexpr uint32_t kOffY = kOffX + 2 * kX;
+  static constexpr uint32_t kOffW = kOffY + 2 * kX;
+  static constexpr uint32_t kOffH = kOffW + kNW * kBox;  // W': NS boxes
+  static constexpr uint32_t kOffS = kOffH + NS * kBox;
+  static constexpr uint32_t kTotal = kOffS + DX * 128 + 1024;
+};
+
+struct Bars {
+  uint64_t xy_full[2], xy_empty[2], w_full[3], w_empty[3];
+  uint64_t sc_full, a_ready, o_full, o_free, h_ready, kv_full, s_ready, drain;
+};
+
+// 16-byte chunk c of row r in a 128-byte-swizzled tile of 128-byte rows.
+__device__ __forceinline__ uint32_t sw_off(int r, int c) { return (uint32_t)r * 128u + (uint32_t)((c ^ (r & 7)) << 4); }
+
+__device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
+
+template <int DX, int NS, bool STATE_ONLY>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    la_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ TcMaps maps, int total_slices) {
+  using L = Smem<DX, NS>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem_1024(smem_raw);
+  __shared__ Bars bars;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  // Not-finite values of w in chunk i: bad_any[i % 3] = i + 1, and for each column the first
+  // one's scan position a as (i + 1) * 256 + 255 - a (the largest wins, so nothing is ever
+  // reset).  A warp may be two chunks ahead of another here, not three.
+  __shared__ unsigned bad_any[3], bad_row[3][kSlice];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // consecutive CTAs: the roles and slices of one batch row and head, which read the same tensors
+  int ss = blockIdx.x % total_slices;
+  const int64_t rest = blockIdx.x / total_slices;
+  const int bh = (int)(rest % ((int64_t)p.B * p.H));
+  const int seg = (int)(rest / ((int64_t)p.B * p.H));
+  int ri = 0;
+  while (ri + 1 < p.n_roles && ss >= (p.role[ri].dw + kSlice - 1) / kSlice) {
+    ss -= (p.role[ri].dw + kSlice - 1) / kSlice;
+    ++ri;
+  }
+  if (STATE_ONLY && seg == p.n_seg - 1) return;
+  const Role& ro = p.role[ri];
+  const int c0 = ss * kSlice;
+  const int b = bh / p.H, h = bh % p.H;
+  const int64_t n_chunks = (p.T + kC - 1) / kC;
+  const int64_t first = (int64_t)seg * p.chunks_per_seg;
+  const int n = (int)(min(n_chunks, first + p.chunks_per_seg) - first);
+  const int e = ro.reverse ? 0 : 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars.xy_full[s], 1);
+      mbar_init(&bars.xy_empty[s], 1);
+    }
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(&bars.w_full[s], 1);
+      mbar_init(&bars.w_empty[s], 1);
+    }
+    mbar_init(&bars.sc_full, 1);
+    mbar_init(&bars.a_ready, 4);
+    mbar_init(&bars.o_full, 1);
+    mbar_init(&bars.o_free, 4);
+    mbar_init(&bars.h_ready, 4);
+    mbar_init(&bars.kv_full, 1);
+    mbar_init(&bars.s_ready, 4);
+    mbar_init(&bars.drain, 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (threadIdx.x < 3 * kSlice) bad_row[threadIdx.x / kSlice][threadIdx.x % kSlice] = 0;
+  if (threadIdx.x < 3) bad_any[threadIdx.x] = 0;
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  auto start_of = [&](int i) -> int {  // first token of chunk i's tile (negative: before the sequence)
+    const int64_t ch = first + i;
+    return (int)(ro.reverse ? p.T - (ch + 1) * kC : ch * kC);
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer
+    if (lane == 0) {
+      const CUtensorMap *mx = &maps.m[ri * 3], *my = mx + 1, *mw = mx + 2;
+      int issued = 0;
+      for (int i = 0; i < n; ++i) {
+        const int t0 = start_of(i), s = i & 1, sw = i % L::kNW;
+        if (!mbar_wait(&bars.xy_empty[s], ((i >> 1) & 1) ^ 1, kErrWaitProducer, &abort_flag)) break;
+        mbar_arrive_expect_tx(&bars.xy_full[s], STATE_ONLY ? L::kX : 2 * L::kX);
+#pragma unroll
+        for (int d = 0; d < DX / 64; ++d) {
+          if (!STATE_ONLY) tma_load_4d(smem + L::kOffX + s * L::kX + d * kBox, mx, &bars.xy_full[s], d * 64, h, t0, b, policy_evict_normal());
+          tma_load_4d(smem + L::kOffY + s * L::kX + d * kBox, my, &bars.xy_full[s], d * 64, h, t0, b, policy_evict_normal());
+        }
+        issued = 2 * i + 1;
+        if (!mbar_wait(&bars.w_empty[sw], ((i / L::kNW) & 1) ^ 1, kErrWaitProducer, &abort_flag)) break;
+        mbar_arrive_expect_tx(&bars.w_full[sw], kBox);
+        tma_load_4d(smem + L::kOffW + sw * kBox, mw, &bars.w_full[sw], c0, h, t0, b, policy_evict_normal());
+        issued = 2 * i + 2;
+      }
+      if (abort_flag) {  // a wait gave up: the copies in flight land before the shared memory is given back
+        for (int j = max(0, issued - 2 * 3); j < issued; ++j) {
+          const int i = j >> 1;
+          if (j & 1)
+            mbar_drain(&bars.w_full[i % L::kNW], (i / L::kNW) & 1);
+          else
+            mbar_drain(&bars.xy_full[i & 1], (i >> 1) & 1);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    constexpr uint32_t id_sc = make_idesc_bf16(kC, kC, 0, 0);
+    constexpr uint32_t id_o = make_idesc_bf16(kC, kSlice, 0, 1);
+    constexpr uint32_t id_kv = make_idesc_bf16(kC, 2 * kSlice, 1, 1);
+    constexpr uint32_t id_kv1 = make_idesc_bf16(kC, kSlice, 1, 1);
+    const uint32_t sb = smem_u32(smem);
+    auto issue_o1 = [&](int j) -> bool {
+      if (j > 0 && !mbar_wait(&bars.o_free, (j - 1) & 1, kErrWaitMma, &abort_flag)) return false;
+      if (!mbar_wait(&bars.a_ready, j & 1, kErrWaitMma, &abort_flag)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t w = sb + L::kOffW + (j % L::kNW) * kBox;
+#pragma unroll
+        for (int k = 0; k < kC / 16; ++k)
+          umma_f16_ts(tmem + kColO1, tmem + kColA + k * 8, make_smem_desc_sw128(w + k * 2048, kBox, 1024), id_o, k > 0);
+        umma_commit(&bars.w_empty[j % L::kNW]);
+        umma_commit(&bars.o_full);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool dead = false;
+    for (int i = 0; i < n; ++i) {
+      const int s = i & 1;
+      const uint32_t x = sb + L::kOffX + s * L::kX, y = sb + L::kOffY + s * L::kX;
+      if (!STATE_ONLY && i > 0 && !issue_o1(i - 1)) {
+        dead = true;
+        break;
+      }
+      if (!mbar_wait(&bars.xy_full[s], (i >> 1) & 1, kErrWaitMma, &abort_flag)) break;
+      tc_fence_after();
+      if (!STATE_ONLY) {
+        if (lane == 0) {
+#pragma unroll
+          for (int k = 0; k < DX / 16; ++k) {
+            const uint32_t at = (k / 4) * kBox + (k % 4) * 32;
+            umma_f16(tmem + kColSc, make_smem_desc_sw128_k(x + at), make_smem_desc_sw128_k(y + at), id_sc, k > 0);
+          }
+          umma_commit(&bars.sc_full);
+        }
+        __syncwarp();
+      }
+      // (the state group has read KV of the chunk before)
+      if (!mbar_wait(&bars.s_ready, i & 1, kErrWaitMma, &abort_flag)) break;
+      tc_fence_after();
+      if (!STATE_ONLY) {
+        if (lane == 0) {
+#pragma unroll
+          for (int k = 0; k < DX / 16; ++k)
+            umma_f16(tmem + kColO2 + s * kSlice, make_smem_desc_sw128_k(x + (k / 4) * kBox + (k % 4) * 32),
+                     make_smem_desc_sw128(sb + L::kOffS + k * 2048, kBox, 1024), id_o, k > 0);
+        }
+        __syncwarp();
+      }
+      if (!mbar_wait(&bars.h_ready, i & 1, kErrWaitMma, &abort_flag)) break;
+      tc_fence_after();
+      if (lane == 0) {
+        // rows of Y^T beyond DX = 64 read the next tile: lanes of KV that nobody looks at
+#pragma unroll
+        for (int k = 0; k < kC / 16; ++k)
+          umma_f16(tmem + kColKv, make_smem_desc_sw128(y + k * 2048, kBox, 1024),
+                   make_smem_desc_sw128(sb + L::kOffH + k * 2048, kBox, 1024), id_kv, k > 0);
+        if (NS == 3) {
+#pragma unroll
+          for (int k = 0; k < kC / 16; ++k)
+            umma_f16(tmem + kColKv + kSlice, make_smem_desc_sw128(y + k * 2048, kBox, 1024),
+                     make_smem_desc_sw128(sb + L::kOffH + 2 * kBox + k * 2048, kBox, 1024), id_kv1, 1);
+        }
+        if (STATE_ONLY) umma_commit(&bars.w_empty[i % L::kNW]);
+        umma_commit(&bars.xy_empty[s]);
+        umma_commit(&bars.kv_full);
+      }
+      __syncwarp();
+    }
+    if (!STATE_ONLY && !dead && !abort_flag) issue_o1(n - 1);
+    if (abort_flag) {  // the products in flight, before their accumulators are given back
+      if (lane == 0) {
+        umma_commit(&bars.drain);
+        mbar_drain(&bars.drain, 0);
+      }
+      __syncwarp();
+    }
+  } else {
+    const double l2d = log2_decay(p.log_decay, h);
+    const int q = warp & 3;
+    const int row = q * 32 + lane;  // token of the chunk's tile, or row of the state
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    const int a = ro.reverse ? kC - 1 - row : row;  // scan position of token `row`
+    const int group = (warp - 2) >> 2;
+    if (group == 0) {
+      // ---------------------------------------------------------------- masks
+      if (!STATE_ONLY) {
+        const float l2 = (float)l2d, sign = ro.reverse ? -1.f : 1.f;
+        for (int i = 0; i < n; ++i) {
+          if (!mbar_wait(&bars.sc_full, i & 1, kErrWaitEpilogue, &abort_flag)) break;
+          if (i > 0 && !mbar_wait(&bars.o_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < kC; c += 32) {
+            uint32_t w[16];
+            const bool none = ro.reverse ? c + 31 < q * 32 : c > q * 32 + 31;  // (uniform in the warp)
+            if (none) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[j] = 0u;
+            } else {
+              const float dist = sign * (float)(row - c);  // tokens from column c to this row
+              float v[32];
+              tmem_ld32(tmem + lanes + kColSc + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float m = ex2(l2 * (dist - sign * (float)j));
+                const bool in = ro.reverse ? c + j >= row : c + j <= row;
+                v[j] = in ? v[j] * m : 0.f;
+              }
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+            }
+            const uint32_t at = tmem + lanes + kColA + c / 2;
+            tmem_st8(at, {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]});
+            tmem_st8(at + 8, {w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]});
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.a_ready);
+        }
+      }
+    } else if (group == 1) {
+      // ---------------------------------------------------------------- state
+      const int64_t n_state = (int64_t)ro.dx * ro.dw;
+      const bool live = row < ro.dx;
+      float S[kSlice];
+      {
+        const float* src = nullptr;
+        int64_t sj = 1;
+        if (!STATE_ONLY && live) {
+          if (p.n_seg > 1)
+            src = seg_state(p, ri, seg, bh, n_state) + (int64_t)row * ro.dw + c0;
+          else if (ro.s_in)
+            src = ro.s_in + (int64_t)bh * n_state + (int64_t)row * ro.si + (int64_t)c0 * ro.sj, sj = ro.sj;
+        }
+#pragma unroll
+        for (int j = 0; j < kSlice; ++j) S[j] = src && c0 + j < ro.dw ? src[j * sj] : 0.f;
+      }
+      const Factor f_full = decay_factor(l2d, kC);
+      bool dead = false;
+      for (int i = 0; i <= n; ++i) {
+        if (i > 0) {
+          if (!mbar_wait(&bars.kv_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)) {
+            dead = true;
+            break;
+          }
+          tc_fence_after();
+          const int64_t left = p.T - (first + i - 1) * kC;
+          const Factor f = left >= kC ? f_full : decay_factor(l2d, (double)left);
+#pragma unroll
+          for (int c = 0; c < kSlice; c += 16) {
+            float v[16], u[16];
+            tmem_ld16(tmem + lanes + kColKv + c, v);
+            tmem_ld16(tmem + lanes + kColKv + kSlice + c, u);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) S[c + j] = decay_add(f, S[c + j], v[j] + u[j]);
+          }
+          tc_fence_before();
+        }
+        if (i == n) break;
+        if (!STATE_ONLY) {
+          // the products that read the previous S were committed with kv_full
+          if (row < DX) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint4 w;
+              w.x = pack_bf16x2(S[8 * c], S[8 * c + 1]), w.y = pack_bf16x2(S[8 * c + 2], S[8 * c + 3]);
+              w.z = pack_bf16x2(S[8 * c + 4], S[8 * c + 5]), w.w = pack_bf16x2(S[8 * c + 6], S[8 * c + 7]);
+              *reinterpret_cast<uint4*>(smem + L::kOffS + sw_off(row, c)) = w;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.s_ready);
+        } else {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.s_ready);
+        }
+      }
+      if (!dead && live) {
+        float* dst = nullptr;
+        int64_t sj = 1;
+        if (STATE_ONLY)
+          dst = seg_state(p, ri, seg, bh, n_state) + (int64_t)row * ro.dw + c0;
+        else if (seg == p.n_seg - 1 && ro.s_out)
+          dst = ro.s_out + (int64_t)bh * n_state + (int64_t)row * ro.si + (int64_t)c0 * ro.sj, sj = ro.sj;
+        if (dst) {
+#pragma unroll
+          for (int j = 0; j < kSlice; ++j)
+            if (c0 + j < ro.dw) dst[j * sj] = S[j];
+        }
+      }
+    } else {
+      // ----------------------------------------------------------------- edge
+      // one chunk's outputs are written while the next chunk's W' is already made
+      const float fo = ro.i_scale * (float)exp2(l2d * (a + e));
+      const float fw = ro.w_scale * (float)exp2(l2d * (kC - e - a));
+      __nv_bfloat16* out = (__nv_bfloat16*)ro.out.p + (int64_t)b * ro.out.sb + (int64_t)h * ro.out.sh + c0;
+      auto outputs = [&](int i) -> bool {
+        if (!mbar_wait(&bars.o_full, i & 1, kErrWaitEpilogue, &abort_flag)) return false;
+        tc_fence_after();
+        const int t = start_of(i) + row;
+        const bool in = t >= 0 && t < p.T;
+        const bool bad = bad_any[i % 3] == (unsigned)i + 1;
+        uint4 o[8];
+#pragma unroll
+        for (int c = 0; c < kSlice; c += 16) {
+          float v[16], u[16];
+          tmem_ld16(tmem + lanes + kColO1 + c, v);
+          tmem_ld16(tmem + lanes + kColO2 + (i & 1) * kSlice + c, u);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = fmaf(fo, u[j], ro.a_scale * v[j]);
+          if (bad) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+            {
+              const unsigned key = bad_row[i % 3][c + j];
+              if (key >> 8 == (unsigned)i + 1 && 255 - (int)(key & 255) <= a) v[j] = __int_as_float(0x7fc00000);
+            }
+          }
+          uint32_t* w = reinterpret_cast<uint32_t*>(&o[c / 8]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.o_free);
+        if (in) {
+          __nv_bfloat16* dst = out + (int64_t)t * ro.out.st;
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (c0 + 8 * c < ro.dw) *reinterpret_cast<uint4*>(dst + 8 * c) = o[c];
+        }
+        return true;
+      };
+      bool dead = false;
+      for (int i = 0; i < n; ++i) {
+        const int sw = i % L::kNW;
+        if (!mbar_wait(&bars.w_full[sw], (i / L::kNW) & 1, kErrWaitEpilogue, &abort_flag) ||
+            (i > 0 && !mbar_wait(&bars.kv_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag))) {
+          dead = true;
+          break;
+        }
+        const int64_t left = p.T - (first + i) * kC;
+        float f = fw;
+        if (left < kC) f = a < left ? ro.w_scale * (float)exp2(l2d * (double)(left - e - a)) : 0.f;
+        uint8_t* src = smem + L::kOffW + sw * kBox;
+        uint8_t* dst = smem + L::kOffH;
+        uint32_t odd = 0;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t at = sw_off(row, c);
+          const uint4 u = *reinterpret_cast<const uint4*>(src + at);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          uint32_t part[NS][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            odd |= (w[j] & 0x7F807F80u) + 0x00800080u;  // an exponent of all ones carries into the sign
+            float lo = bf_lo(w[j]) * f, hi = bf_hi(w[j]) * f;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+              part[s][j] = pack_bf16x2(lo, hi);
+              if (s + 1 < NS) {
+                lo -= bf_lo(part[s][j]);
+                hi -= bf_hi(part[s][j]);
+              }
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+            *reinterpret_cast<uint4*>(dst + s * kBox + at) = make_uint4(part[s][0], part[s][1], part[s][2], part[s][3]);
+        }
+        if (!STATE_ONLY && (odd & 0x80008000u)) {
+          // the tile keeps zeros where a value was not finite; rows that may see it become NaN
+          __nv_bfloat16* wr = reinterpret_cast<__nv_bfloat16*>(src);
+          for (int c = 0; c < kSlice; ++c) {
+            __nv_bfloat16* at = wr + (sw_off(row, c >> 3) >> 1) + (c & 7);
+            if (!isfinite(__bfloat162float(*at))) {
+              *at = __float2bfloat16_rn(0.f);
+              atomicMax(&bad_row[i % 3][c], ((unsigned)i + 1) * 256 + 255 - a);
+              bad_any[i % 3] = (unsigned)i + 1;
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.h_ready);
+        if (!STATE_ONLY && i > 0 && !outputs(i - 1)) {
+          dead = true;
+          break;
+        }
+      }
+      if (!STATE_ONLY && !dead) outputs(n - 1);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+bool mappable(const View& v, int64_t B, int64_t T, int H) {
+  if (reinterpret_cast<uintptr_t>(v.p) & 15) return false;
+  const int64_t s[3] = {v.sb, v.st, v.sh}, n[3] = {B, T, H};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 != 0 || s[i] * 2 >= ((int64_t)1 << 40))) return false;
+  return true;
+}
+
+int view_map(CUtensorMap* map, const View& v, int64_t B, int64_t T, int H, int d) {
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
+  const cuuint64_t strides[3] = {(cuuint64_t)(H > 1 ? v.sh * 2 : 16), (cuuint64_t)(T > 1 ? v.st * 2 : 16),
+                                 (cuuint64_t)(B > 1 ? v.sb * 2 : 16)};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)kC, 1};
+  return encode_tensor_map_bf16(map, v.p, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int DX, int NS, bool STATE_ONLY>
+int go(const Params& p, const TcMaps& maps, cudaStream_t st) {
+  using L = Smem<DX, NS>;
+  static_assert(L::kTotal <= 232448 - 1024, "shared memory of one CTA");
+  int slices = 0;
+  for (int r = 0; r < p.n_roles; ++r) slices += (p.role[r].dw + kSlice - 1) / kSlice;
+  const int64_t blocks = (int64_t)p.n_seg * p.B * p.H * slices;
+  if (blocks > INT32_MAX) return set_error(DYNCONV_ERR_SHAPE, "linear attention: B*H too large");
+  cudaError_t e =
+      cudaFuncSetAttribute(la_tc_kernel<DX, NS, STATE_ONLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kTotal);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_status(e, "cudaFuncSetAttribute(la_tc)");
+  }
+  la_tc_kernel<DX, NS, STATE_ONLY><<<(unsigned)blocks, kTcThreads, L::kTotal, st>>>(p, maps, slices);
+  DYNCONV_CHECK_LAUNCH("la_tc_kernel");
+  return DYNCONV_OK;
+}
+
+template <int DX, int NS>
+int passes(const Params& p, const TcMaps& maps, cudaStream_t st) {
+  int s;
+  if (p.n_seg > 1) {
+    if ((s = go<DX, NS, true>(p, maps, st))) return s;
+    if ((s = scan_launch(p, kC, st))) return s;
+  }
+  return go<DX, NS, false>(p, maps, st);
+}
+
+}  // namespace
+
+// bf16, widths that are multiples of 8 up to 128, and tensors that TMA can address: 16-byte
+// aligned, strides positive multiples of 16 bytes.
+bool tc_supported(const Params& p, int dtype) {
+  if (dtype != DYNCONV_DTYPE_BF16) return false;
+  for (int r = 0; r < p.n_roles; ++r) {
+    const Role& ro = p.role[r];
+    if (ro.dx % 8 || ro.dw % 8 || ro.dx > 128 || ro.dw > 128) return false;
+    for (const View* v : {&ro.x, &ro.y, &ro.w, &ro.out})
+      if (!mappable(*v, p.B, p.T, p.H)) return false;
+  }
+  return true;
+}
+
+// Cuts chains while there are fewer than one per SM: each cut costs its segment a second
+// read of y and w, so segments keep eight chunks at least.
+void tc_plan(Params* p) {
+  const int64_t chunks = (p->T + kC - 1) / kC;
+  int64_t chains = 0;
+  for (int r = 0; r < p->n_roles; ++r) chains += (int64_t)p->B * p->H * ((p->role[r].dw + kSlice - 1) / kSlice);
+  int64_t seg = sm_count() / chains;
+  if (seg > chunks / 8) seg = chunks / 8;
+  if (seg < 1) seg = 1;
+  p->chunks_per_seg = (int)((chunks + seg - 1) / seg);
+  p->n_seg = (int)((chunks + p->chunks_per_seg - 1) / p->chunks_per_seg);
+}
+
+int tc_launch(const Params& p, cudaStream_t st) {
+  TcMaps maps;
+  int s, dx = 0;
+  bool states = false;
+  for (int r = 0; r < p.n_roles; ++r) {
+    const Role& ro = p.role[r];
+    if ((s = view_map(&maps.m[3 * r], ro.x, p.B, p.T, p.H, ro.dx))) return s;
+    if ((s = view_map(&maps.m[3 * r + 1], ro.y, p.B, p.T, p.H, ro.dx))) return s;
+    if ((s = view_map(&maps.m[3 * r + 2], ro.w, p.B, p.T, p.H, ro.dw))) return s;
+    dx = ro.dx > dx ? ro.dx : dx;
+    states = states || ro.s_out;
+  }
+  if (dx <= 64) return states ? passes<64, 3>(p, maps, st) : passes<64, 2>(p, maps, st);
+  return states ? passes<128, 3>(p, maps, st) : passes<128, 2>(p, maps, st);
+}
+
+}  // namespace la
+
+DYNCONV_DEFINE_ERROR_ACCESSOR(la_tc_error_word)
+
+}  // namespace dynconv

@@ -282,7 +282,7 @@ int dynconv_hw_step(const void* x, const void* weight, const void* static_w, voi
  *   (12 numbers), so the thirds of a fused [B,T,3*H*d] buffer are read in place.
  *   log_decay [H] float32, <= 0 (a factor of at most one; -inf forgets at once).
  *   initial_state (NULL = zero), final_state (NULL = not wanted): [B,H,dk,dv] float32.
- * dk, dv in 1..256, B*H <= 65535.  T = 0 copies the state. */
+ * dk, dv in 1..256, B*H <= 65535, T <= 2^30.  T = 0 copies the state. */
 size_t dynconv_la_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype, int backward);
 int dynconv_la_fwd(const void* q, const void* k, const void* v, const float* log_decay, const float* initial_state,
                    void* o, float* final_state, const int64_t* strides,

@@ -264,6 +264,33 @@ def test_nan_stays_in_its_row_and_head():
     assert got[1, 200:, 1].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("t", [0, 1, 130, 255, 299])
+def test_later_tokens_stay_masked(dtype, bad, t):
+    """What is not finite in one token's q, k or v reaches no earlier token (a prompt's padding may
+    hold anything), and the gradients of a padded batch's own tokens stay finite."""
+    q, k, v, do, S0, _, ld = inputs(1, 300, 2, 64, 64, dtype)
+    want = decay_linear_attention(q, k, v, ld, S0)
+    for x in (q, k, v):
+        keep = x[0, t:, 1].clone()
+        x[0, t:, 1] = bad
+        got = decay_linear_attention(q, k, v, ld, S0)
+        assert torch.equal(got[0, :t, 1], want[0, :t, 1]) and torch.equal(got[0, :, 0], want[0, :, 0])
+        assert not got[0, t:, 1].isfinite().any()
+        x[0, t:, 1] = keep
+    # backwards in time: an upstream gradient that is not finite reaches no later token's dk, dv
+    own = [x.detach().requires_grad_() for x in (q, k, v)]
+    ref = torch.autograd.grad(decay_linear_attention(*own, ld, S0), own, do)
+    do = do.clone()
+    do[0, t, 0, 3] = bad
+    got = torch.autograd.grad(decay_linear_attention(*own, ld, S0), own, do)
+    for i, (g, r) in enumerate(zip(got, ref)):
+        assert torch.equal(g[0, t + 1:, 0], r[0, t + 1:, 0]) and torch.equal(g[0, :, 1], r[0, :, 1])
+        if i == 0:
+            assert torch.equal(g[0, :t, 0], r[0, :t, 0])
+
+
 # ------------------------------------------------------------------------------ steps
 
 
