@@ -13,9 +13,9 @@
 // (two: 2^-17 of each term, three: 2^-25, when the state goes back to the caller).
 //
 // Warps: a producer (TMA rings: x and y two deep, w NW deep), an MMA issuer, and three groups of
-// four: masks (Sc -> A), state (KV -> S), and edge (W -> W', and the outputs).  The issuer runs
+// four: scores (Sc -> A, and the outputs), state (KV -> S), and weights (W -> W').  The issuer runs
 //     A(i-1) ready: O1(i-1);  Sc(i);  S(i) ready: O2(i);  W'(i) ready: KV(i)
-// so that while the mask group works on chunk i, the pipe has O2 and KV of the same chunk.
+// so that while the scores group works on chunk i, the pipe has O2 and KV of the same chunk.
 //
 // A masked score is zero whatever its value was, but 0 * inf in O1 is NaN: a value of w that is
 // not finite is taken out of the tile and marks the rows that may see it (the slow path
@@ -31,18 +31,21 @@ constexpr int kC = 128;     // tokens of a chunk
 constexpr int kSlice = 64;  // columns of w per CTA
 constexpr int kTcThreads = 64 + 3 * 128;
 constexpr uint32_t kBox = 64 * kC * 2;  // one TMA box: 128 rows of 64 bf16
-constexpr int kMaxMaps = kMaxRoles * 3;
+constexpr int kMaxMaps = kMaxRoles * 4;
 
 // TMEM columns
 constexpr uint32_t kColSc = 0, kColA = 128, kColKv = 192, kColO1 = 320, kColO2 = 384, kTmemCols = 512;
 
 struct TcMaps {
-  CUtensorMap m[kMaxMaps];  // [role][x, y, w]
+  CUtensorMap m[kMaxMaps];  // [role][x, y, w, out]
 };
 
 template <int DX, int NS>
 struct Smem {
   static constexpr int kNW = NS == 3 ? 2 : 3;  // depth of the w ring (shared-memory bound at DX = 128)
+  // With three w tiles, outputs leave through the w tile that their chunk no longer needs (TMA
+  // store); with two that would hold up the next load, and rows are stored directly.
+  static constexpr bool kStage = kNW == 3;
   static constexpr uint32_t kX = DX / 64 * kBox;
   static constexpr uint32_t kOffX = 0;
   static constexpr uint32_t kOffY = kOffX + 2 * kX;
@@ -76,8 +79,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // one's scan position a as (i + 1) * 256 + 255 - a (the largest wins, so nothing is ever
   // reset).  A warp may be two chunks ahead of another here, not three.
   __shared__ unsigned bad_any[3], bad_row[3][kSlice];
+  __shared__ __align__(16) float far_of[32];  // decays from a column to its 32-column block's far edge
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // consecutive CTAs: the roles and slices of one batch row and head, which read the same tensors
   int ss = blockIdx.x % total_slices;
   const int64_t rest = blockIdx.x / total_slices;
@@ -104,7 +108,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int s = 0; s < 3; ++s) {
       mbar_init(&bars.w_full[s], 1);
-      mbar_init(&bars.w_empty[s], 1);
+      mbar_init(&bars.w_empty[s], !STATE_ONLY && L::kStage ? 4 : 1);
     }
     mbar_init(&bars.sc_full, 1);
     mbar_init(&bars.a_ready, 4);
@@ -119,6 +123,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   if (threadIdx.x < 3 * kSlice) bad_row[threadIdx.x / kSlice][threadIdx.x % kSlice] = 0;
   if (threadIdx.x < 3) bad_any[threadIdx.x] = 0;
+  if (threadIdx.x < 32)
+    far_of[threadIdx.x] = (float)exp2(log2_decay(p.log_decay, h) * (ro.reverse ? threadIdx.x : 31 - threadIdx.x));
   if (warp == 1) {
     tmem_alloc(&tmem_slot, kTmemCols);
     tmem_relinquish();
@@ -135,7 +141,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
-      const CUtensorMap *mx = &maps.m[ri * 3], *my = mx + 1, *mw = mx + 2;
+      const CUtensorMap *mx = &maps.m[ri * 4], *my = mx + 1, *mw = mx + 2;
       int issued = 0;
       for (int i = 0; i < n; ++i) {
         const int t0 = start_of(i), s = i & 1, sw = i % L::kNW;
@@ -170,25 +176,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     constexpr uint32_t id_kv = make_idesc_bf16(kC, 2 * kSlice, 1, 1);
     constexpr uint32_t id_kv1 = make_idesc_bf16(kC, kSlice, 1, 1);
     const uint32_t sb = smem_u32(smem);
+    const uint32_t el = elect_lane();
     auto issue_o1 = [&](int j) -> bool {
       if (j > 0 && !mbar_wait(&bars.o_free, (j - 1) & 1, kErrWaitMma, &abort_flag)) return false;
       if (!mbar_wait(&bars.a_ready, j & 1, kErrWaitMma, &abort_flag)) return false;
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t w = sb + L::kOffW + (j % L::kNW) * kBox;
+      const uint32_t w = desc_lo(sb + L::kOffW + (j % L::kNW) * kBox, kBox);
 #pragma unroll
-        for (int k = 0; k < kC / 16; ++k)
-          umma_f16_ts(tmem + kColO1, tmem + kColA + k * 8, make_smem_desc_sw128(w + k * 2048, kBox, 1024), id_o, k > 0);
-        umma_commit(&bars.w_empty[j % L::kNW]);
-        umma_commit(&bars.o_full);
-      }
+      for (int k = 0; k < kC / 16; ++k)
+        umma_f16_ts_e(el, tmem + kColO1, tmem + kColA + k * 8, w + k * (2048 / 16), id_o, k > 0);
+      if (!L::kStage) umma_commit_e(el, &bars.w_empty[j % L::kNW]);
+      umma_commit_e(el, &bars.o_full);
       __syncwarp();
       return true;
     };
     bool dead = false;
     for (int i = 0; i < n; ++i) {
       const int s = i & 1;
-      const uint32_t x = sb + L::kOffX + s * L::kX, y = sb + L::kOffY + s * L::kX;
+      const uint32_t x = desc_lo(sb + L::kOffX + s * L::kX), yk = desc_lo(sb + L::kOffY + s * L::kX),
+                     ym = desc_lo(sb + L::kOffY + s * L::kX, kBox);
       if (!STATE_ONLY && i > 0 && !issue_o1(i - 1)) {
         dead = true;
         break;
@@ -196,55 +202,48 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!mbar_wait(&bars.xy_full[s], (i >> 1) & 1, kErrWaitMma, &abort_flag)) break;
       tc_fence_after();
       if (!STATE_ONLY) {
-        if (lane == 0) {
 #pragma unroll
-          for (int k = 0; k < DX / 16; ++k) {
-            const uint32_t at = (k / 4) * kBox + (k % 4) * 32;
-            umma_f16(tmem + kColSc, make_smem_desc_sw128_k(x + at), make_smem_desc_sw128_k(y + at), id_sc, k > 0);
-          }
-          umma_commit(&bars.sc_full);
+        for (int k = 0; k < DX / 16; ++k) {
+          const uint32_t at = ((k / 4) * kBox + (k % 4) * 32) / 16;
+          umma_f16_e(el, tmem + kColSc, x + at, yk + at, id_sc, k > 0);
         }
+        umma_commit_e(el, &bars.sc_full);
         __syncwarp();
       }
       // (the state group has read KV of the chunk before)
       if (!mbar_wait(&bars.s_ready, i & 1, kErrWaitMma, &abort_flag)) break;
       tc_fence_after();
       if (!STATE_ONLY) {
-        if (lane == 0) {
+        const uint32_t st = desc_lo(sb + L::kOffS, kBox);
 #pragma unroll
-          for (int k = 0; k < DX / 16; ++k)
-            umma_f16(tmem + kColO2 + s * kSlice, make_smem_desc_sw128_k(x + (k / 4) * kBox + (k % 4) * 32),
-                     make_smem_desc_sw128(sb + L::kOffS + k * 2048, kBox, 1024), id_o, k > 0);
-        }
+        for (int k = 0; k < DX / 16; ++k)
+          umma_f16_e(el, tmem + kColO2 + s * kSlice, x + ((k / 4) * kBox + (k % 4) * 32) / 16, st + k * (2048 / 16),
+                     id_o, k > 0);
         __syncwarp();
       }
       if (!mbar_wait(&bars.h_ready, i & 1, kErrWaitMma, &abort_flag)) break;
       tc_fence_after();
-      if (lane == 0) {
+      {
         // rows of Y^T beyond DX = 64 read the next tile: lanes of KV that nobody looks at
+        const uint32_t hw = desc_lo(sb + L::kOffH, kBox), hw2 = desc_lo(sb + L::kOffH + 2 * kBox, kBox);
 #pragma unroll
         for (int k = 0; k < kC / 16; ++k)
-          umma_f16(tmem + kColKv, make_smem_desc_sw128(y + k * 2048, kBox, 1024),
-                   make_smem_desc_sw128(sb + L::kOffH + k * 2048, kBox, 1024), id_kv, k > 0);
+          umma_f16_e(el, tmem + kColKv, ym + k * (2048 / 16), hw + k * (2048 / 16), id_kv, k > 0);
         if (NS == 3) {
 #pragma unroll
           for (int k = 0; k < kC / 16; ++k)
-            umma_f16(tmem + kColKv + kSlice, make_smem_desc_sw128(y + k * 2048, kBox, 1024),
-                     make_smem_desc_sw128(sb + L::kOffH + 2 * kBox + k * 2048, kBox, 1024), id_kv1, 1);
+            umma_f16_e(el, tmem + kColKv + kSlice, ym + k * (2048 / 16), hw2 + k * (2048 / 16), id_kv1, 1);
         }
-        if (STATE_ONLY) umma_commit(&bars.w_empty[i % L::kNW]);
-        umma_commit(&bars.xy_empty[s]);
-        umma_commit(&bars.kv_full);
+        if (STATE_ONLY) umma_commit_e(el, &bars.w_empty[i % L::kNW]);
+        umma_commit_e(el, &bars.xy_empty[s]);
+        umma_commit_e(el, &bars.kv_full);
       }
       __syncwarp();
     }
     if (!STATE_ONLY && !dead && !abort_flag) issue_o1(n - 1);
     if (abort_flag) {  // the products in flight, before their accumulators are given back
-      if (lane == 0) {
-        umma_commit(&bars.drain);
-        mbar_drain(&bars.drain, 0);
-      }
-      __syncwarp();
+      umma_commit_e(el, &bars.drain);
+      mbar_drain(&bars.drain, 0);
     }
   } else {
     const double l2d = log2_decay(p.log_decay, h);
@@ -254,33 +253,121 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int a = ro.reverse ? kC - 1 - row : row;  // scan position of token `row`
     const int group = (warp - 2) >> 2;
     if (group == 0) {
-      // ---------------------------------------------------------------- masks
+      // ----------------------------------------------------- outputs and masks
       if (!STATE_ONLY) {
-        const float l2 = (float)l2d, sign = ro.reverse ? -1.f : 1.f;
-        for (int i = 0; i < n; ++i) {
-          if (!mbar_wait(&bars.sc_full, i & 1, kErrWaitEpilogue, &abort_flag)) break;
-          if (i > 0 && !mbar_wait(&bars.o_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)) break;
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < kC; c += 32) {
-            uint32_t w[16];
-            const bool none = ro.reverse ? c + 31 < q * 32 : c > q * 32 + 31;  // (uniform in the warp)
-            if (none) {
+        const bool rev = ro.reverse;
+        const int slot_rows = q * 32 * 128;  // this warp's rows in a w tile
+        const float fo = ro.i_scale * (float)exp2(l2d * (a + e));
+        __nv_bfloat16* out = (__nv_bfloat16*)ro.out.p + (int64_t)b * ro.out.sb + (int64_t)h * ro.out.sh + c0;
+        // Decays of the scores.  On the diagonal 32 x 32 block: g^|row - column|, kept per thread.
+        // d blocks away from it: g^(distance) = near * g^(32 (d - 1)) * far[column], near <= 1 from
+        // the row to its block's edge, far from the column's edge to the column (shared memory).
+        float diag[32];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] = 0u;
-            } else {
-              const float dist = sign * (float)(row - c);  // tokens from column c to this row
-              float v[32];
-              tmem_ld32(tmem + lanes + kColSc + c, v);
-              tmem_ld_wait();
+        for (int j = 0; j < 32; ++j) {
+          const int dist = rev ? j - lane : lane - j;
+          diag[j] = dist >= 0 ? (float)exp2(l2d * dist) : 0.f;
+        }
+        const float near = (float)exp2(l2d * (rev ? 32 - lane : lane + 1)), g32 = (float)exp2(l2d * 32);
+        const int blocks = rev ? 4 - q : q + 1;  // 32-column blocks that are not masked
+        {  // the masked blocks of A are zero once and for all
+          const uint32_t z[8] = {};
+          for (int c = 0; c < 4; ++c)
+            if (rev ? c < q : c > q) {
+              tmem_st8(tmem + lanes + kColA + c * 16, z);
+              tmem_st8(tmem + lanes + kColA + c * 16 + 8, z);
+            }
+        }
+        auto outputs = [&](int i) {
+          const int t = start_of(i) + row;
+          const bool bad = bad_any[i % 3] == (unsigned)i + 1;
+          uint4 o[8];
 #pragma unroll
+          for (int c = 0; c < kSlice; c += 32) {
+            float v[32], u[32];
+            tmem_ld32(tmem + lanes + kColO1 + c, v);
+            tmem_ld32(tmem + lanes + kColO2 + (i & 1) * kSlice + c, u);
+            tmem_ld_wait();
+            if (bad) {
               for (int j = 0; j < 32; ++j) {
-                const float m = ex2(l2 * (dist - sign * (float)j));
-                const bool in = ro.reverse ? c + j >= row : c + j <= row;
-                v[j] = in ? v[j] * m : 0.f;
-              }
+                const unsigned key = bad_row[i % 3][c + j];
+                if (key >> 8 == (unsigned)i + 1 && 255 - (int)(key & 255) <= a) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+                  for (int k = 0; k < 32; ++k)
+                    if (k == j) v[k] = __int_as_float(0x7fc00000);
+                }
+              }
+            }
+            uint32_t* w = reinterpret_cast<uint32_t*>(&o[c / 8]);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 r = fma2(make_float2(fo, fo), make_float2(u[2 * j], u[2 * j + 1]),
+                                    mul2(make_float2(ro.a_scale, ro.a_scale), make_float2(v[2 * j], v[2 * j + 1])));
+              w[j] = pack_bf16x2(r.x, r.y);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.o_free);
+          if (L::kStage && p.T - (first + i) * kC >= kC) {  // a whole chunk: TMA store of the warp's 32 rows
+            uint8_t* tile = smem + L::kOffW + (i % L::kNW) * kBox;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + sw_off(row, c)) = o[c];
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_4d(&maps.m[ri * 4 + 3], tile + slot_rows, c0, h, start_of(i) + q * 32, b);
+              bulk_commit_group();
+            }
+          } else if (t >= 0 && t < p.T) {
+            __nv_bfloat16* dst = out + (int64_t)t * ro.out.st;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              if (c0 + 8 * c < ro.dw) *reinterpret_cast<uint4*>(dst + 8 * c) = o[c];
+          }
+        };
+        bool dead = false;
+        for (int i = 0; i <= n; ++i) {
+          if (i > 0) {
+            if (!mbar_wait(&bars.o_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)) {
+              dead = true;
+              break;
+            }
+            tc_fence_after();
+            outputs(i - 1);
+          }
+          if (i == n) break;
+          if (!mbar_wait(&bars.sc_full, i & 1, kErrWaitEpilogue, &abort_flag)) {
+            dead = true;
+            break;
+          }
+          tc_fence_after();
+          float f = near;
+#pragma unroll 1
+          for (int k = 0; k < blocks; ++k) {
+            const int c = (rev ? q + k : q - k) * 32;
+            float v[32];
+            uint32_t w[16];
+            tmem_ld32(tmem + lanes + kColSc + c, v);
+            tmem_ld_wait();
+            if (k == 0) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const bool in0 = rev ? 2 * j >= lane : 2 * j <= lane, in1 = rev ? 2 * j + 1 >= lane : 2 * j + 1 <= lane;
+                const float2 m = mul2(make_float2(v[2 * j], v[2 * j + 1]), make_float2(diag[2 * j], diag[2 * j + 1]));
+                w[j] = pack_bf16x2(in0 ? m.x : 0.f, in1 ? m.y : 0.f);  // (whatever a masked score was)
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) {
+                const float4 t4 = *reinterpret_cast<const float4*>(&far_of[2 * j]);
+                const float2 f2 = make_float2(f, f);
+                const float2 m0 = mul2(mul2(f2, make_float2(t4.x, t4.y)), make_float2(v[2 * j], v[2 * j + 1]));
+                const float2 m1 = mul2(mul2(f2, make_float2(t4.z, t4.w)), make_float2(v[2 * j + 2], v[2 * j + 3]));
+                w[j] = pack_bf16x2(m0.x, m0.y);
+                w[j + 1] = pack_bf16x2(m1.x, m1.y);
+              }
+              f *= g32;
             }
             const uint32_t at = tmem + lanes + kColA + c / 2;
             tmem_st8(at, {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]});
@@ -288,9 +375,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           tmem_st_wait();
           tc_fence_before();
+          if (L::kStage && i > 0 && lane == 0) {  // the stores of chunk i-1 have read their tile by now
+            bulk_wait_group_read<0>();
+            mbar_arrive(&bars.w_empty[(i - 1) % L::kNW]);
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars.a_ready);
         }
+        if (lane == 0) bulk_wait_group<0>();
       }
     } else if (group == 1) {
       // ---------------------------------------------------------------- state
@@ -327,7 +419,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tmem_ld16(tmem + lanes + kColKv + kSlice + c, u);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) S[c + j] = decay_add(f, S[c + j], v[j] + u[j]);
+            for (int j = 0; j < 16; j += 2) {  // decay_add of pairs
+              const float2 s2 = make_float2(S[c + j], S[c + j + 1]);
+              float2 r = add2(make_float2(v[j], v[j + 1]), make_float2(u[j], u[j + 1]));
+              r = fma2(make_float2(f.hi, f.hi), s2, fma2(make_float2(f.lo, f.lo), s2, r));
+              S[c + j] = r.x, S[c + j + 1] = r.y;
+            }
           }
           tc_fence_before();
         }
@@ -365,57 +462,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
     } else {
-      // ----------------------------------------------------------------- edge
-      // one chunk's outputs are written while the next chunk's W' is already made
-      const float fo = ro.i_scale * (float)exp2(l2d * (a + e));
+      // -------------------------------------------------------------- weights
       const float fw = ro.w_scale * (float)exp2(l2d * (kC - e - a));
-      __nv_bfloat16* out = (__nv_bfloat16*)ro.out.p + (int64_t)b * ro.out.sb + (int64_t)h * ro.out.sh + c0;
-      auto outputs = [&](int i) -> bool {
-        if (!mbar_wait(&bars.o_full, i & 1, kErrWaitEpilogue, &abort_flag)) return false;
-        tc_fence_after();
-        const int t = start_of(i) + row;
-        const bool in = t >= 0 && t < p.T;
-        const bool bad = bad_any[i % 3] == (unsigned)i + 1;
-        uint4 o[8];
-#pragma unroll
-        for (int c = 0; c < kSlice; c += 16) {
-          float v[16], u[16];
-          tmem_ld16(tmem + lanes + kColO1 + c, v);
-          tmem_ld16(tmem + lanes + kColO2 + (i & 1) * kSlice + c, u);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = fmaf(fo, u[j], ro.a_scale * v[j]);
-          if (bad) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-            {
-              const unsigned key = bad_row[i % 3][c + j];
-              if (key >> 8 == (unsigned)i + 1 && 255 - (int)(key & 255) <= a) v[j] = __int_as_float(0x7fc00000);
-            }
-          }
-          uint32_t* w = reinterpret_cast<uint32_t*>(&o[c / 8]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.o_free);
-        if (in) {
-          __nv_bfloat16* dst = out + (int64_t)t * ro.out.st;
-#pragma unroll
-          for (int c = 0; c < 8; ++c)
-            if (c0 + 8 * c < ro.dw) *reinterpret_cast<uint4*>(dst + 8 * c) = o[c];
-        }
-        return true;
-      };
-      bool dead = false;
       for (int i = 0; i < n; ++i) {
         const int sw = i % L::kNW;
         if (!mbar_wait(&bars.w_full[sw], (i / L::kNW) & 1, kErrWaitEpilogue, &abort_flag) ||
-            (i > 0 && !mbar_wait(&bars.kv_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag))) {
-          dead = true;
+            (i > 0 && !mbar_wait(&bars.kv_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)))
           break;
-        }
         const int64_t left = p.T - (first + i) * kC;
         float f = fw;
         if (left < kC) f = a < left ? ro.w_scale * (float)exp2(l2d * (double)(left - e - a)) : 0.f;
@@ -431,14 +484,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             odd |= (w[j] & 0x7F807F80u) + 0x00800080u;  // an exponent of all ones carries into the sign
-            float lo = bf_lo(w[j]) * f, hi = bf_hi(w[j]) * f;
+            float2 x = mul2(make_float2(bf_lo(w[j]), bf_hi(w[j])), make_float2(f, f));
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-              part[s][j] = pack_bf16x2(lo, hi);
-              if (s + 1 < NS) {
-                lo -= bf_lo(part[s][j]);
-                hi -= bf_hi(part[s][j]);
-              }
+              part[s][j] = pack_bf16x2(x.x, x.y);
+              if (s + 1 < NS) x = add2(x, make_float2(-bf_lo(part[s][j]), -bf_hi(part[s][j])));
             }
           }
 #pragma unroll
@@ -460,12 +510,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.h_ready);
-        if (!STATE_ONLY && i > 0 && !outputs(i - 1)) {
-          dead = true;
-          break;
-        }
       }
-      if (!STATE_ONLY && !dead) outputs(n - 1);
     }
   }
   tc_fence_before();
@@ -481,11 +526,11 @@ bool mappable(const View& v, int64_t B, int64_t T, int H) {
   return true;
 }
 
-int view_map(CUtensorMap* map, const View& v, int64_t B, int64_t T, int H, int d) {
+int view_map(CUtensorMap* map, const View& v, int64_t B, int64_t T, int H, int d, int rows) {
   const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
   const cuuint64_t strides[3] = {(cuuint64_t)(H > 1 ? v.sh * 2 : 16), (cuuint64_t)(T > 1 ? v.st * 2 : 16),
                                  (cuuint64_t)(B > 1 ? v.sb * 2 : 16)};
-  const cuuint32_t box[4] = {64, 1, (cuuint32_t)kC, 1};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
   return encode_tensor_map_bf16(map, v.p, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
@@ -552,9 +597,10 @@ int tc_launch(const Params& p, cudaStream_t st) {
   bool states = false;
   for (int r = 0; r < p.n_roles; ++r) {
     const Role& ro = p.role[r];
-    if ((s = view_map(&maps.m[3 * r], ro.x, p.B, p.T, p.H, ro.dx))) return s;
-    if ((s = view_map(&maps.m[3 * r + 1], ro.y, p.B, p.T, p.H, ro.dx))) return s;
-    if ((s = view_map(&maps.m[3 * r + 2], ro.w, p.B, p.T, p.H, ro.dw))) return s;
+    if ((s = view_map(&maps.m[4 * r], ro.x, p.B, p.T, p.H, ro.dx, kC))) return s;
+    if ((s = view_map(&maps.m[4 * r + 1], ro.y, p.B, p.T, p.H, ro.dx, kC))) return s;
+    if ((s = view_map(&maps.m[4 * r + 2], ro.w, p.B, p.T, p.H, ro.dw, kC))) return s;
+    if ((s = view_map(&maps.m[4 * r + 3], ro.out, p.B, p.T, p.H, ro.dw, 32))) return s;
     dx = ro.dx > dx ? ro.dx : dx;
     states = states || ro.s_out;
   }
