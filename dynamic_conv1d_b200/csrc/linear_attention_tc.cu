@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // one's scan position a as (i + 1) * 256 + 255 - a (the largest wins, so nothing is ever
   // reset).  A warp may be two chunks ahead of another here, not three.
   __shared__ unsigned bad_any[3], bad_row[3][kSlice];
+  __shared__ float pw[kC + 1];                // decay^0 .. decay^kC
   __shared__ __align__(16) float far_of[32];  // decays from a column to its 32-column block's far edge
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -123,8 +124,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   if (threadIdx.x < 3 * kSlice) bad_row[threadIdx.x / kSlice][threadIdx.x % kSlice] = 0;
   if (threadIdx.x < 3) bad_any[threadIdx.x] = 0;
-  if (threadIdx.x < 32)
-    far_of[threadIdx.x] = (float)exp2(log2_decay(p.log_decay, h) * (ro.reverse ? threadIdx.x : 31 - threadIdx.x));
+  if (threadIdx.x <= kC) {
+    const float f = (float)exp2(log2_decay(p.log_decay, h) * threadIdx.x);
+    pw[threadIdx.x] = f;
+    if (threadIdx.x < 32) far_of[ro.reverse ? threadIdx.x : 31 - threadIdx.x] = f;
+  }
   if (warp == 1) {
     tmem_alloc(&tmem_slot, kTmemCols);
     tmem_relinquish();
@@ -246,7 +250,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_drain(&bars.drain, 0);
     }
   } else {
-    const double l2d = log2_decay(p.log_decay, h);
     const int q = warp & 3;
     const int row = q * 32 + lane;  // token of the chunk's tile, or row of the state
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!STATE_ONLY) {
         const bool rev = ro.reverse;
         const int slot_rows = q * 32 * 128;  // this warp's rows in a w tile
-        const float fo = ro.i_scale * (float)exp2(l2d * (a + e));
+        const float fo = ro.i_scale * pw[a + e];
         __nv_bfloat16* out = (__nv_bfloat16*)ro.out.p + (int64_t)b * ro.out.sb + (int64_t)h * ro.out.sh + c0;
         // Decays of the scores.  On the diagonal 32 x 32 block: g^|row - column|, kept per thread.
         // d blocks away from it: g^(distance) = near * g^(32 (d - 1)) * far[column], near <= 1 from
@@ -266,9 +269,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
           const int dist = rev ? j - lane : lane - j;
-          diag[j] = dist >= 0 ? (float)exp2(l2d * dist) : 0.f;
+          diag[j] = dist >= 0 ? pw[dist] : 0.f;
         }
-        const float near = (float)exp2(l2d * (rev ? 32 - lane : lane + 1)), g32 = (float)exp2(l2d * 32);
+        const float near = pw[rev ? 32 - lane : lane + 1], g32 = pw[32];
         const int blocks = rev ? 4 - q : q + 1;  // 32-column blocks that are not masked
         {  // the masked blocks of A are zero once and for all
           const uint32_t z[8] = {};
@@ -280,50 +283,54 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         auto outputs = [&](int i) {
           const int t = start_of(i) + row;
+          // a whole chunk leaves through its w tile and a TMA store of each warp's 32 rows
+          const bool staged = L::kStage && p.T - (first + i) * kC >= kC;
+          uint8_t* tile = smem + L::kOffW + (i % L::kNW) * kBox;
+          __nv_bfloat16* dst = out + (int64_t)t * ro.out.st;
+          const bool in = t >= 0 && t < p.T;
           const bool bad = bad_any[i % 3] == (unsigned)i + 1;
-          uint4 o[8];
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < kSlice; c += 32) {
             float v[32], u[32];
             tmem_ld32(tmem + lanes + kColO1 + c, v);
             tmem_ld32(tmem + lanes + kColO2 + (i & 1) * kSlice + c, u);
             tmem_ld_wait();
-            if (bad) {
-              for (int j = 0; j < 32; ++j) {
-                const unsigned key = bad_row[i % 3][c + j];
-                if (key >> 8 == (unsigned)i + 1 && 255 - (int)(key & 255) <= a) {
-#pragma unroll
-                  for (int k = 0; k < 32; ++k)
-                    if (k == j) v[k] = __int_as_float(0x7fc00000);
-                }
-              }
-            }
-            uint32_t* w = reinterpret_cast<uint32_t*>(&o[c / 8]);
+            uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const float2 r = fma2(make_float2(fo, fo), make_float2(u[2 * j], u[2 * j + 1]),
                                     mul2(make_float2(ro.a_scale, ro.a_scale), make_float2(v[2 * j], v[2 * j + 1])));
               w[j] = pack_bf16x2(r.x, r.y);
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint4 o = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+              if (staged)
+                *reinterpret_cast<uint4*>(tile + sw_off(row, c / 8 + j)) = o;
+              else if (in && c0 + c + 8 * j < ro.dw)
+                *reinterpret_cast<uint4*>(dst + c + 8 * j) = o;
+            }
           }
           tc_fence_before();
+          if (bad) {
+#pragma unroll 1
+            for (int c = 0; c < kSlice; ++c) {
+              const unsigned key = bad_row[i % 3][c];
+              if (key >> 8 != (unsigned)i + 1 || 255 - (int)(key & 255) > a) continue;
+              if (staged)
+                *reinterpret_cast<uint16_t*>(tile + sw_off(row, c / 8) + (c & 7) * 2) = 0x7FC0;
+              else if (in && c0 + c < ro.dw)
+                *reinterpret_cast<uint16_t*>(dst + c) = 0x7FC0;
+            }
+          }
+          if (staged) fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.o_free);
-          if (L::kStage && p.T - (first + i) * kC >= kC) {  // a whole chunk: TMA store of the warp's 32 rows
-            uint8_t* tile = smem + L::kOffW + (i % L::kNW) * kBox;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + sw_off(row, c)) = o[c];
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
+          if (lane == 0) {
+            mbar_arrive(&bars.o_free);
+            if (staged) {
               tma_store_4d(&maps.m[ri * 4 + 3], tile + slot_rows, c0, h, start_of(i) + q * 32, b);
               bulk_commit_group();
             }
-          } else if (t >= 0 && t < p.T) {
-            __nv_bfloat16* dst = out + (int64_t)t * ro.out.st;
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              if (c0 + 8 * c < ro.dw) *reinterpret_cast<uint4*>(dst + 8 * c) = o[c];
           }
         };
         bool dead = false;
@@ -401,6 +408,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int j = 0; j < kSlice; ++j) S[j] = src && c0 + j < ro.dw ? src[j * sj] : 0.f;
       }
+      const double l2d = log2_decay(p.log_decay, h);
       const Factor f_full = decay_factor(l2d, kC);
       bool dead = false;
       for (int i = 0; i <= n; ++i) {
@@ -463,7 +471,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     } else {
       // -------------------------------------------------------------- weights
-      const float fw = ro.w_scale * (float)exp2(l2d * (kC - e - a));
+      const float fw = ro.w_scale * pw[kC - e - a];
       for (int i = 0; i < n; ++i) {
         const int sw = i % L::kNW;
         if (!mbar_wait(&bars.w_full[sw], (i / L::kNW) & 1, kErrWaitEpilogue, &abort_flag) ||
@@ -471,11 +479,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           break;
         const int64_t left = p.T - (first + i) * kC;
         float f = fw;
-        if (left < kC) f = a < left ? ro.w_scale * (float)exp2(l2d * (double)(left - e - a)) : 0.f;
+        if (left < kC) f = a < left ? ro.w_scale * pw[left - e - a] : 0.f;
         uint8_t* src = smem + L::kOffW + sw * kBox;
         uint8_t* dst = smem + L::kOffH;
         uint32_t odd = 0;
-#pragma unroll
+#pragma unroll 4
         for (int c = 0; c < 8; ++c) {
           const uint32_t at = sw_off(row, c);
           const uint4 u = *reinterpret_cast<const uint4*>(src + at);
