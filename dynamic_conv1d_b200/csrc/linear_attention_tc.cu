@@ -12,10 +12,11 @@
 // its rounding to bf16 would cost the state its precision: it is split into NS bf16 parts
 // (two: 2^-17 of each term, three: 2^-25, when the state goes back to the caller).
 //
-// Warps: a producer (TMA rings: x and y two deep, w NW deep), an MMA issuer, and three groups of
+// Warps: a producer (TMA rings two deep), an MMA issuer, and three groups of
 // four: scores (Sc -> A, and the outputs), state (KV -> S), and weights (W -> W').  The issuer runs
-//     A(i-1) ready: O1(i-1);  Sc(i);  S(i) ready: O2(i);  W'(i) ready: KV(i)
-// so that while the scores group works on chunk i, the pipe has O2 and KV of the same chunk.
+//     A(i-1) ready: O1(i-1);  Sc(i);  W'(i) ready: KV(i);  S(i) ready: O2(i)
+// so that while the scores group masks chunk i and writes the outputs of chunk i-1, the pipe has
+// KV and O2 of chunk i and O1 and Sc of the next.
 //
 // A masked score is zero whatever its value was, but 0 * inf in O1 is NaN: a value of w that is
 // not finite is taken out of the tile and marks the rows that may see it (the slow path
@@ -31,10 +32,13 @@ constexpr int kC = 128;     // tokens of a chunk
 constexpr int kSlice = 64;  // columns of w per CTA
 constexpr int kTcThreads = 64 + 3 * 128;
 constexpr uint32_t kBox = 64 * kC * 2;  // one TMA box: 128 rows of 64 bf16
+// Chunks brought into L2 ahead of their loads: a tile from HBM takes about 2000 cycles, half a
+// chunk's time, and the w ring asks for its next tile late.
+constexpr int kAhead = 3;
 constexpr int kMaxMaps = kMaxRoles * 4;
 
 // TMEM columns
-constexpr uint32_t kColSc = 0, kColA = 128, kColKv = 192, kColO1 = 320, kColO2 = 384, kTmemCols = 512;
+constexpr uint32_t kColSc = 0, kColA = 128, kColKv = 192, kColO1 = 256, kColO2 = 384, kTmemCols = 512;  // O1, O2: two each
 
 struct TcMaps {
   CUtensorMap m[kMaxMaps];  // [role][x, y, w, out]
@@ -42,22 +46,22 @@ struct TcMaps {
 
 template <int DX, int NS>
 struct Smem {
-  static constexpr int kNW = NS == 3 ? 2 : 3;  // depth of the w ring (shared-memory bound at DX = 128)
-  // With three w tiles, outputs leave through the w tile that their chunk no longer needs (TMA
-  // store); with two that would hold up the next load, and rows are stored directly.
-  static constexpr bool kStage = kNW == 3;
+  // The third part of W' takes the room in which outputs are staged for TMA stores: their rows are
+  // then stored directly.
+  static constexpr bool kStage = NS == 2;
   static constexpr uint32_t kX = DX / 64 * kBox;
   static constexpr uint32_t kOffX = 0;
   static constexpr uint32_t kOffY = kOffX + 2 * kX;
   static constexpr uint32_t kOffW = kOffY + 2 * kX;
-  static constexpr uint32_t kOffH = kOffW + kNW * kBox;  // W': NS boxes
-  static constexpr uint32_t kOffS = kOffH + NS * kBox;
+  static constexpr uint32_t kOffH = kOffW + 2 * kBox;  // W': NS boxes, or two and the staged outputs
+  static constexpr uint32_t kOffO = kOffH + 2 * kBox;
+  static constexpr uint32_t kOffS = kOffH + 3 * kBox;
   static constexpr uint32_t kTotal = kOffS + DX * 128 + 1024;
 };
 
 struct Bars {
-  uint64_t xy_full[2], xy_empty[2], w_full[3], w_empty[3];
-  uint64_t sc_full, a_ready, o_full, o_free, h_ready, kv_full, s_ready, drain;
+  uint64_t xy_full[2], xy_empty[2], w_full[2], w_empty[2];
+  uint64_t sc_full, a_ready, o_full, o_free[2], o2_full, h_ready, kv_full, s_ready, drain;
 };
 
 // 16-byte chunk c of row r in a 128-byte-swizzled tile of 128-byte rows.
@@ -75,11 +79,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  // Not-finite values of w in chunk i: bad_any[i % 3] = i + 1, and for each column the first
+  // Not-finite values of w in chunk i: bad_any[i % 4] = i + 1, and for each column the first
   // one's scan position a as (i + 1) * 256 + 255 - a (the largest wins, so nothing is ever
-  // reset).  A warp may be two chunks ahead of another here, not three.
-  __shared__ unsigned bad_any[3], bad_row[3][kSlice];
-  __shared__ float pw[kC + 1];                // decay^0 .. decay^kC
+  // reset).  The writers may be three chunks ahead of the readers, not four.
+  __shared__ unsigned bad_any[4], bad_row[4][kSlice];
+  __shared__ float decays[31 + kC + 1];       // 31 zeros, then decay^0 .. decay^kC
+  const float* pw = decays + 31;
   __shared__ __align__(16) float far_of[32];  // decays from a column to its 32-column block's far edge
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -106,15 +111,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars.xy_full[s], 1);
       mbar_init(&bars.xy_empty[s], 1);
-    }
-    for (int s = 0; s < 3; ++s) {
       mbar_init(&bars.w_full[s], 1);
-      mbar_init(&bars.w_empty[s], !STATE_ONLY && L::kStage ? 4 : 1);
+      mbar_init(&bars.w_empty[s], 1);
     }
     mbar_init(&bars.sc_full, 1);
     mbar_init(&bars.a_ready, 4);
     mbar_init(&bars.o_full, 1);
-    mbar_init(&bars.o_free, 4);
+    mbar_init(&bars.o_free[0], 4);
+    mbar_init(&bars.o_free[1], 4);
+    mbar_init(&bars.o2_full, 1);
     mbar_init(&bars.h_ready, 4);
     mbar_init(&bars.kv_full, 1);
     mbar_init(&bars.s_ready, 4);
@@ -122,12 +127,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     abort_flag = 0;
     fence_barrier_init();
   }
-  if (threadIdx.x < 3 * kSlice) bad_row[threadIdx.x / kSlice][threadIdx.x % kSlice] = 0;
-  if (threadIdx.x < 3) bad_any[threadIdx.x] = 0;
+  if (threadIdx.x < 4 * kSlice) bad_row[threadIdx.x / kSlice][threadIdx.x % kSlice] = 0;
+  if (threadIdx.x < 4) bad_any[threadIdx.x] = 0;
   if (threadIdx.x <= kC) {
     const float f = (float)exp2(log2_decay(p.log_decay, h) * threadIdx.x);
-    pw[threadIdx.x] = f;
-    if (threadIdx.x < 32) far_of[ro.reverse ? threadIdx.x : 31 - threadIdx.x] = f;
+    decays[31 + threadIdx.x] = f;
+    if (threadIdx.x < 32) {
+      far_of[ro.reverse ? threadIdx.x : 31 - threadIdx.x] = f;
+      if (threadIdx.x < 31) decays[threadIdx.x] = 0.f;
+    }
   }
   if (warp == 1) {
     tmem_alloc(&tmem_slot, kTmemCols);
@@ -148,7 +156,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const CUtensorMap *mx = &maps.m[ri * 4], *my = mx + 1, *mw = mx + 2;
       int issued = 0;
       for (int i = 0; i < n; ++i) {
-        const int t0 = start_of(i), s = i & 1, sw = i % L::kNW;
+        const int t0 = start_of(i), s = i & 1;
+        if (i + kAhead < n) {
+          const int t1 = start_of(i + kAhead);
+#pragma unroll
+          for (int d = 0; d < DX / 64; ++d) {
+            if (!STATE_ONLY) tma_prefetch_4d(mx, d * 64, h, t1, b);
+            tma_prefetch_4d(my, d * 64, h, t1, b);
+          }
+          tma_prefetch_4d(mw, c0, h, t1, b);
+        }
         if (!mbar_wait(&bars.xy_empty[s], ((i >> 1) & 1) ^ 1, kErrWaitProducer, &abort_flag)) break;
         mbar_arrive_expect_tx(&bars.xy_full[s], STATE_ONLY ? L::kX : 2 * L::kX);
 #pragma unroll
@@ -157,16 +174,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tma_load_4d(smem + L::kOffY + s * L::kX + d * kBox, my, &bars.xy_full[s], d * 64, h, t0, b, policy_evict_normal());
         }
         issued = 2 * i + 1;
-        if (!mbar_wait(&bars.w_empty[sw], ((i / L::kNW) & 1) ^ 1, kErrWaitProducer, &abort_flag)) break;
-        mbar_arrive_expect_tx(&bars.w_full[sw], kBox);
-        tma_load_4d(smem + L::kOffW + sw * kBox, mw, &bars.w_full[sw], c0, h, t0, b, policy_evict_normal());
+        if (!mbar_wait(&bars.w_empty[s], ((i >> 1) & 1) ^ 1, kErrWaitProducer, &abort_flag)) break;
+        mbar_arrive_expect_tx(&bars.w_full[s], kBox);
+        tma_load_4d(smem + L::kOffW + s * kBox, mw, &bars.w_full[s], c0, h, t0, b, policy_evict_normal());
         issued = 2 * i + 2;
       }
       if (abort_flag) {  // a wait gave up: the copies in flight land before the shared memory is given back
-        for (int j = max(0, issued - 2 * 3); j < issued; ++j) {
+        for (int j = max(0, issued - 4); j < issued; ++j) {
           const int i = j >> 1;
           if (j & 1)
-            mbar_drain(&bars.w_full[i % L::kNW], (i / L::kNW) & 1);
+            mbar_drain(&bars.w_full[i & 1], (i >> 1) & 1);
           else
             mbar_drain(&bars.xy_full[i & 1], (i >> 1) & 1);
         }
@@ -177,19 +194,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---------------------------------------------------------------- MMA issuer
     constexpr uint32_t id_sc = make_idesc_bf16(kC, kC, 0, 0);
     constexpr uint32_t id_o = make_idesc_bf16(kC, kSlice, 0, 1);
-    constexpr uint32_t id_kv = make_idesc_bf16(kC, 2 * kSlice, 1, 1);
-    constexpr uint32_t id_kv1 = make_idesc_bf16(kC, kSlice, 1, 1);
+    constexpr uint32_t id_kv = make_idesc_bf16(kC, kSlice, 1, 1);
     const uint32_t sb = smem_u32(smem);
     const uint32_t el = elect_lane();
     auto issue_o1 = [&](int j) -> bool {
-      if (j > 0 && !mbar_wait(&bars.o_free, (j - 1) & 1, kErrWaitMma, &abort_flag)) return false;
       if (!mbar_wait(&bars.a_ready, j & 1, kErrWaitMma, &abort_flag)) return false;
       tc_fence_after();
-      const uint32_t w = desc_lo(sb + L::kOffW + (j % L::kNW) * kBox, kBox);
+      const uint32_t w = desc_lo(sb + L::kOffW + (j & 1) * kBox, kBox);
 #pragma unroll
       for (int k = 0; k < kC / 16; ++k)
-        umma_f16_ts_e(el, tmem + kColO1, tmem + kColA + k * 8, w + k * (2048 / 16), id_o, k > 0);
-      if (!L::kStage) umma_commit_e(el, &bars.w_empty[j % L::kNW]);
+        umma_f16_ts_e(el, tmem + kColO1 + (j & 1) * kSlice, tmem + kColA + k * 8, w + k * (2048 / 16), id_o, k > 0);
+      umma_commit_e(el, &bars.w_empty[j & 1]);
       umma_commit_e(el, &bars.o_full);
       __syncwarp();
       return true;
@@ -214,34 +229,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         umma_commit_e(el, &bars.sc_full);
         __syncwarp();
       }
-      // (the state group has read KV of the chunk before)
-      if (!mbar_wait(&bars.s_ready, i & 1, kErrWaitMma, &abort_flag)) break;
+      // s_ready: the state group has read KV of the chunk before
+      if (!mbar_wait(&bars.h_ready, i & 1, kErrWaitMma, &abort_flag) ||
+          !mbar_wait(&bars.s_ready, i & 1, kErrWaitMma, &abort_flag))
+        break;
       tc_fence_after();
-      if (!STATE_ONLY) {
+      // W' part by part into one accumulator; rows of Y^T beyond DX = 64 read the next tile:
+      // lanes of KV that nobody looks at
+#pragma unroll
+      for (int part = 0; part < NS; ++part) {
+        const uint32_t hw = desc_lo(sb + L::kOffH + part * kBox, kBox);
+#pragma unroll
+        for (int k = 0; k < kC / 16; ++k)
+          umma_f16_e(el, tmem + kColKv, ym + k * (2048 / 16), hw + k * (2048 / 16), id_kv, part > 0 || k > 0);
+      }
+      umma_commit_e(el, &bars.kv_full);
+      if (STATE_ONLY) {
+        umma_commit_e(el, &bars.w_empty[i & 1]);
+      } else {
+        // the outputs of chunk i-2 have left this O2 (and the O1 that O1(i) will write)
+        if (i > 1 && !mbar_wait(&bars.o_free[s], ((i >> 1) - 1) & 1, kErrWaitMma, &abort_flag)) break;
+        tc_fence_after();
         const uint32_t st = desc_lo(sb + L::kOffS, kBox);
 #pragma unroll
         for (int k = 0; k < DX / 16; ++k)
           umma_f16_e(el, tmem + kColO2 + s * kSlice, x + ((k / 4) * kBox + (k % 4) * 32) / 16, st + k * (2048 / 16),
                      id_o, k > 0);
-        __syncwarp();
+        umma_commit_e(el, &bars.o2_full);
       }
-      if (!mbar_wait(&bars.h_ready, i & 1, kErrWaitMma, &abort_flag)) break;
-      tc_fence_after();
-      {
-        // rows of Y^T beyond DX = 64 read the next tile: lanes of KV that nobody looks at
-        const uint32_t hw = desc_lo(sb + L::kOffH, kBox), hw2 = desc_lo(sb + L::kOffH + 2 * kBox, kBox);
-#pragma unroll
-        for (int k = 0; k < kC / 16; ++k)
-          umma_f16_e(el, tmem + kColKv, ym + k * (2048 / 16), hw + k * (2048 / 16), id_kv, k > 0);
-        if (NS == 3) {
-#pragma unroll
-          for (int k = 0; k < kC / 16; ++k)
-            umma_f16_e(el, tmem + kColKv + kSlice, ym + k * (2048 / 16), hw2 + k * (2048 / 16), id_kv1, 1);
-        }
-        if (STATE_ONLY) umma_commit_e(el, &bars.w_empty[i % L::kNW]);
-        umma_commit_e(el, &bars.xy_empty[s]);
-        umma_commit_e(el, &bars.kv_full);
-      }
+      umma_commit_e(el, &bars.xy_empty[s]);
       __syncwarp();
     }
     if (!STATE_ONLY && !dead && !abort_flag) issue_o1(n - 1);
@@ -262,15 +278,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int slot_rows = q * 32 * 128;  // this warp's rows in a w tile
         const float fo = ro.i_scale * pw[a + e];
         __nv_bfloat16* out = (__nv_bfloat16*)ro.out.p + (int64_t)b * ro.out.sb + (int64_t)h * ro.out.sh + c0;
-        // Decays of the scores.  On the diagonal 32 x 32 block: g^|row - column|, kept per thread.
-        // d blocks away from it: g^(distance) = near * g^(32 (d - 1)) * far[column], near <= 1 from
-        // the row to its block's edge, far from the column's edge to the column (shared memory).
-        float diag[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const int dist = rev ? j - lane : lane - j;
-          diag[j] = dist >= 0 ? pw[dist] : 0.f;
-        }
+        // Decays of the scores.  On the diagonal 32 x 32 block: g^|row - column|, read along the
+        // diagonals of the table.  d blocks away from it: g^(distance) = near * g^(32 (d - 1)) *
+        // far[column], near from the row to its block's edge, far from the column's edge to the
+        // column (both at most one, so nothing overflows on the way).
+        const float* diag = pw + (rev ? -lane : lane);
+        const int step = rev ? 1 : -1;
+        const uint32_t seen = rev ? 0xFFFFFFFFu << lane : 0xFFFFFFFFu >> (31 - lane);  // columns of the diagonal block
         const float near = pw[rev ? 32 - lane : lane + 1], g32 = pw[32];
         const int blocks = rev ? 4 - q : q + 1;  // 32-column blocks that are not masked
         {  // the masked blocks of A are zero once and for all
@@ -283,16 +297,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         auto outputs = [&](int i) {
           const int t = start_of(i) + row;
-          // a whole chunk leaves through its w tile and a TMA store of each warp's 32 rows
+          // a whole chunk leaves through shared memory and a TMA store of each warp's 32 rows
           const bool staged = L::kStage && p.T - (first + i) * kC >= kC;
-          uint8_t* tile = smem + L::kOffW + (i % L::kNW) * kBox;
+          uint8_t* tile = smem + L::kOffO;
+          if (lane == 0) bulk_wait_group_read<0>();  // the store of the chunk before has read it
+          __syncwarp();
           __nv_bfloat16* dst = out + (int64_t)t * ro.out.st;
           const bool in = t >= 0 && t < p.T;
-          const bool bad = bad_any[i % 3] == (unsigned)i + 1;
+          const bool bad = bad_any[i & 3] == (unsigned)i + 1;
 #pragma unroll 1
           for (int c = 0; c < kSlice; c += 32) {
             float v[32], u[32];
-            tmem_ld32(tmem + lanes + kColO1 + c, v);
+            tmem_ld32(tmem + lanes + kColO1 + (i & 1) * kSlice + c, v);
             tmem_ld32(tmem + lanes + kColO2 + (i & 1) * kSlice + c, u);
             tmem_ld_wait();
             uint32_t w[16];
@@ -315,7 +331,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (bad) {
 #pragma unroll 1
             for (int c = 0; c < kSlice; ++c) {
-              const unsigned key = bad_row[i % 3][c];
+              const unsigned key = bad_row[i & 3][c];
               if (key >> 8 != (unsigned)i + 1 || 255 - (int)(key & 255) > a) continue;
               if (staged)
                 *reinterpret_cast<uint16_t*>(tile + sw_off(row, c / 8) + (c & 7) * 2) = 0x7FC0;
@@ -326,29 +342,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (staged) fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&bars.o_free);
+            mbar_arrive(&bars.o_free[i & 1]);
             if (staged) {
               tma_store_4d(&maps.m[ri * 4 + 3], tile + slot_rows, c0, h, start_of(i) + q * 32, b);
               bulk_commit_group();
             }
           }
         };
-        bool dead = false;
         for (int i = 0; i <= n; ++i) {
-          if (i > 0) {
-            if (!mbar_wait(&bars.o_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)) {
-              dead = true;
-              break;
-            }
-            tc_fence_after();
-            outputs(i - 1);
-          }
-          if (i == n) break;
-          if (!mbar_wait(&bars.sc_full, i & 1, kErrWaitEpilogue, &abort_flag)) {
-            dead = true;
+          // A's reader, O1(i-1), is done (as is O2(i-1), issued before it)
+          if ((i > 0 && !mbar_wait(&bars.o_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)) ||
+              (i < n && !mbar_wait(&bars.sc_full, i & 1, kErrWaitEpilogue, &abort_flag)))
+            break;
+          tc_fence_after();
+          if (i == n) {
+            outputs(n - 1);
             break;
           }
-          tc_fence_after();
           float f = near;
 #pragma unroll 1
           for (int k = 0; k < blocks; ++k) {
@@ -360,9 +370,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (k == 0) {
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                const bool in0 = rev ? 2 * j >= lane : 2 * j <= lane, in1 = rev ? 2 * j + 1 >= lane : 2 * j + 1 <= lane;
-                const float2 m = mul2(make_float2(v[2 * j], v[2 * j + 1]), make_float2(diag[2 * j], diag[2 * j + 1]));
-                w[j] = pack_bf16x2(in0 ? m.x : 0.f, in1 ? m.y : 0.f);  // (whatever a masked score was)
+                const float2 m = mul2(make_float2(v[2 * j], v[2 * j + 1]), make_float2(diag[step * 2 * j], diag[step * (2 * j + 1)]));
+                // (zero whatever a masked score was)
+                w[j] = pack_bf16x2(seen & (1u << (2 * j)) ? m.x : 0.f, seen & (2u << (2 * j)) ? m.y : 0.f);
               }
             } else {
 #pragma unroll
@@ -382,12 +392,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           tmem_st_wait();
           tc_fence_before();
-          if (L::kStage && i > 0 && lane == 0) {  // the stores of chunk i-1 have read their tile by now
-            bulk_wait_group_read<0>();
-            mbar_arrive(&bars.w_empty[(i - 1) % L::kNW]);
-          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars.a_ready);
+          if (i > 0) outputs(i - 1);
         }
         if (lane == 0) bulk_wait_group<0>();
       }
@@ -421,16 +428,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int64_t left = p.T - (first + i - 1) * kC;
           const Factor f = left >= kC ? f_full : decay_factor(l2d, (double)left);
 #pragma unroll
-          for (int c = 0; c < kSlice; c += 16) {
-            float v[16], u[16];
-            tmem_ld16(tmem + lanes + kColKv + c, v);
-            tmem_ld16(tmem + lanes + kColKv + kSlice + c, u);
+          for (int c = 0; c < kSlice; c += 32) {
+            float v[32];
+            tmem_ld32(tmem + lanes + kColKv + c, v);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) {  // decay_add of pairs
+            for (int j = 0; j < 32; j += 2) {  // decay_add of pairs
               const float2 s2 = make_float2(S[c + j], S[c + j + 1]);
-              float2 r = add2(make_float2(v[j], v[j + 1]), make_float2(u[j], u[j + 1]));
-              r = fma2(make_float2(f.hi, f.hi), s2, fma2(make_float2(f.lo, f.lo), s2, r));
+              const float2 r = fma2(make_float2(f.hi, f.hi), s2, fma2(make_float2(f.lo, f.lo), s2, make_float2(v[j], v[j + 1])));
               S[c + j] = r.x, S[c + j + 1] = r.y;
             }
           }
@@ -438,7 +443,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (i == n) break;
         if (!STATE_ONLY) {
-          // the products that read the previous S were committed with kv_full
+          if (i > 0 && !mbar_wait(&bars.o2_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)) {  // S's reader
+            dead = true;
+            break;
+          }
           if (row < DX) {
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
@@ -473,8 +481,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // -------------------------------------------------------------- weights
       const float fw = ro.w_scale * pw[kC - e - a];
       for (int i = 0; i < n; ++i) {
-        const int sw = i % L::kNW;
-        if (!mbar_wait(&bars.w_full[sw], (i / L::kNW) & 1, kErrWaitEpilogue, &abort_flag) ||
+        const int sw = i & 1;
+        if (!mbar_wait(&bars.w_full[sw], (i >> 1) & 1, kErrWaitEpilogue, &abort_flag) ||
             (i > 0 && !mbar_wait(&bars.kv_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)))
           break;
         const int64_t left = p.T - (first + i) * kC;
@@ -510,8 +518,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __nv_bfloat16* at = wr + (sw_off(row, c >> 3) >> 1) + (c & 7);
             if (!isfinite(__bfloat162float(*at))) {
               *at = __float2bfloat16_rn(0.f);
-              atomicMax(&bad_row[i % 3][c], ((unsigned)i + 1) * 256 + 255 - a);
-              bad_any[i % 3] = (unsigned)i + 1;
+              atomicMax(&bad_row[i & 3][c], ((unsigned)i + 1) * 256 + 255 - a);
+              bad_any[i & 3] = (unsigned)i + 1;
             }
           }
         }
@@ -586,17 +594,26 @@ bool tc_supported(const Params& p, int dtype) {
   return true;
 }
 
-// Cuts chains while there are fewer than one per SM: each cut costs its segment a second
-// read of y and w, so segments keep eight chunks at least.
+// Cuts chains into the number of segments with the lowest estimated time, counted in chunks of
+// one CTA: both passes run in rounds of one CTA per SM, the state pass costs kStatePass of a
+// chunk's time per chunk, and a round's start kStart chunks (measured at 128 x 128: a chunk 2.2
+// us, of the state pass 1.0 us, about 5 us to start).
 void tc_plan(Params* p) {
-  const int64_t chunks = (p->T + kC - 1) / kC;
+  constexpr double kStatePass = 0.45, kStart = 2.0;
+  const int64_t chunks = (p->T + kC - 1) / kC, sms = sm_count();
   int64_t chains = 0;
   for (int r = 0; r < p->n_roles; ++r) chains += (int64_t)p->B * p->H * ((p->role[r].dw + kSlice - 1) / kSlice);
-  int64_t seg = sm_count() / chains;
-  if (seg > chunks / 8) seg = chunks / 8;
-  if (seg < 1) seg = 1;
-  p->chunks_per_seg = (int)((chunks + seg - 1) / seg);
-  p->n_seg = (int)((chunks + p->chunks_per_seg - 1) / p->chunks_per_seg);
+  double best = 1e300;
+  p->n_seg = 1, p->chunks_per_seg = (int)chunks;
+  for (int64_t want = 1; want <= 64 && want <= chunks; ++want) {
+    const int64_t per = (chunks + want - 1) / want, seg = (chunks + per - 1) / per;
+    double cost = (double)((chains * seg + sms - 1) / sms) * ((double)per + kStart);
+    if (seg > 1) cost += (double)((chains * (seg - 1) + sms - 1) / sms) * ((double)per * kStatePass + kStart) + kStart;
+    if (cost < best) {
+      best = cost;
+      p->n_seg = (int)seg, p->chunks_per_seg = (int)per;
+    }
+  }
 }
 
 int tc_launch(const Params& p, cudaStream_t st) {
