@@ -19,6 +19,9 @@ namespace dynconv {
 namespace {
 
 constexpr int kThreads = 128;
+// Below this many rows the CUDA-core path runs a block per row with its taps in parallel: 2.5 to 3
+// us for 1 to 6 rows of 3 x 2048 channels in fp32, where blocks of eight rows take 7.7 us up to 32.
+constexpr int kFewRows = 32;
 
 __device__ __forceinline__ int64_t slot_of(const void* slots, int slot_bytes, int b) {
   if (!slots) return b;
@@ -134,6 +137,203 @@ __global__ void __launch_bounds__(kThreads) lr_step_kernel(const T* __restrict__
                             residual);
 }
 
+// Few rows: the time is the latency of the loads, so each warp takes one tap and all its ranks'
+// loads are in flight at once; the taps' products meet in shared memory.  Block: W warps of 32
+// channel vectors, one batch row.
+template <typename T, int W, int VEC>
+__global__ void __launch_bounds__(32 * W) lr_step_few_kernel(const T* __restrict__ x, const T* __restrict__ z,
+                                                             const T* __restrict__ U, const T* __restrict__ sw, T* cache,
+                                                             T* __restrict__ y, const void* __restrict__ slots,
+                                                             int slot_bytes, int64_t n_rows, int64_t D, int R, int G,
+                                                             int residual) {
+  __shared__ float part[W][32 * VEC];
+  __shared__ float zs[64];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t C = (int64_t)G * D, b = blockIdx.y;
+  const int64_t per = (D / VEC + 31) / 32;  // blocks of a group
+  const int64_t g = blockIdx.x / per;
+  const int64_t d = ((blockIdx.x - g * per) * 32 + lane) * VEC, c = g * D + d;
+  const int64_t row = slot_of(slots, slot_bytes, (int)b);
+  const bool in = d < D, live = row >= 0 && row < n_rows;
+  const T* Ug = U + (g * R * W + w) * D + d;
+  constexpr int kFly = 16;
+  float u[kFly][VEC];
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < kFly; ++i)
+      if (in && r0 + i < R) load_vec<T, VEC>(Ug + (int64_t)(r0 + i) * W * D, u[i]);
+  };
+  fetch(0);
+  float past[VEC], next[VEC], tap[VEC];  // this tap's input, and the one that takes its place
+  T* cr = cache + (live ? row : 0) * (int64_t)(W - 1) * C + c;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) past[e] = next[e] = tap[e] = 0.f;
+  if (in && live) {
+    const T* xr = x + b * C + c;
+    load_vec<T, VEC>(w == 0 ? xr : cr + (int64_t)(W - 1 - w) * C, past);
+    if (w > 0) load_vec<T, VEC>(w == 1 ? xr : cr + (int64_t)(W - w) * C, next);
+  }
+  if (in && sw) load_vec<T, VEC>(sw + (g * W + w) * D + d, tap);
+  for (int r = threadIdx.x; r < R; r += 32 * W) zs[r] = Elem<T>::to_f(z[(b * G + g) * R + r]);
+  __syncthreads();  // (also: every cache row has been read before one is written)
+  for (int r0 = 0; r0 < R; r0 += kFly) {
+    if (r0 > 0) fetch(r0);
+#pragma unroll
+    for (int i = 0; i < kFly; ++i)
+      if (in && r0 + i < R) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) tap[e] = fmaf(zs[r0 + i], u[i][e], tap[e]);
+      }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) part[w][lane * VEC + e] = tap[e] * past[e];
+  if (in && live && w > 0) store_vec<T, VEC>(cr + (int64_t)(W - 1 - w) * C, next);
+  __syncthreads();
+  if (w != 0 || !in) return;
+  float out[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    out[e] = residual ? past[e] : 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) out[e] += part[k][lane * VEC + e];
+  }
+  store_vec<T, VEC>(y + b * C + c, out);
+}
+
+// bf16, many rows: the taps are a small matrix product (rows x ranks by ranks x channels), 2 R
+// operations for each byte of the batch: on the CUDA cores 53 us for 256 rows of 3 x 4096
+// channels at R = 31, so it goes to the tensor cores.  mma.sync is the fitting form here: a
+// warp's 16 x 32 outputs are consumed in registers by the convolution itself, K is R <= 64, and
+// the kernel is bound by the batch's bytes, not by the product.
+//
+// Block: 32 channels of one group, four warps with 16 rows each, U's tile staged once for 64
+// rows.  Channels are staged permuted, so that a thread's four column pairs are eight
+// neighbouring channels: one 16-byte access per row and tensor.
+constexpr int kMmaRows = 64, kMmaCh = 32;
+
+__device__ __forceinline__ void mma_16n8k16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+
+template <int W>
+__global__ void __launch_bounds__(128) lr_step_mma_kernel(const __nv_bfloat16* __restrict__ x,
+                                                          const __nv_bfloat16* __restrict__ z,
+                                                          const __nv_bfloat16* __restrict__ U,
+                                                          const __nv_bfloat16* __restrict__ sw, __nv_bfloat16* cache,
+                                                          __nv_bfloat16* __restrict__ y, const void* __restrict__ slots,
+                                                          int slot_bytes, int64_t B, int64_t n_rows, int64_t D, int R,
+                                                          int RP, int G, int residual) {
+  // us[w][k / 2][position] = channels' (U[k], U[k + 1]) pairs: B fragments are single words.
+  // Row pitch 40 words: the four k rows that a fragment load touches lie 8 banks apart.
+  extern __shared__ uint32_t us[];
+  constexpr int kPitch = 40;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t C = (int64_t)G * D;
+  const int64_t per = (D + kMmaCh - 1) / kMmaCh;
+  const int64_t g = blockIdx.x / per, d0 = (blockIdx.x - g * per) * kMmaCh;
+  const int K2 = RP / 2;
+  const int r0 = lane >> 2, q = lane & 3;
+  const int64_t d = d0 + q * 8, c = g * D + d;
+  const int64_t b0 = (int64_t)blockIdx.y * kMmaRows + warp * 16;
+  // stage U: a thread takes 8 channels of a rank pair; position of channel c in the tile:
+  // column pair j = (c % 8) / 2 of thread c / 8 is column 2 (c / 8) + c % 2 of product j
+  for (int i = threadIdx.x; i < W * K2 * 4; i += 128) {
+    const int oct = i & 3, rest = i >> 2, k2 = rest % K2, w = rest / K2;
+    const int64_t d = d0 + oct * 8;
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+    const __nv_bfloat16* src = U + ((g * R + 2 * k2) * W + w) * D + d;
+    if (d < D && 2 * k2 < R) lo = *reinterpret_cast<const uint4*>(src);
+    if (d < D && 2 * k2 + 1 < R) hi = *reinterpret_cast<const uint4*>(src + (int64_t)W * D);
+    uint32_t* dst = us + (w * K2 + k2) * kPitch + oct * 2;
+    const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      dst[j * 8] = __byte_perm(l[j], h[j], 0x5410);
+      dst[j * 8 + 1] = __byte_perm(l[j], h[j], 0x7632);
+    }
+  }
+  __syncthreads();
+  if (b0 >= B) return;
+  float acc[4][W][4];  // column pair, tap, (row r0: two channels, row r0 + 8: two channels)
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][w][e] = 0.f;
+  for (int k0 = 0; k0 < RP; k0 += 16) {
+    uint32_t a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t b = b0 + r0 + (i & 1) * 8;
+      const int k = k0 + q * 2 + (i >> 1) * 8;
+      const uint16_t* zr = reinterpret_cast<const uint16_t*>(z) + (b * G + g) * R + k;
+      const uint32_t lo = b < B && k < R ? zr[0] : 0, hi = b < B && k + 1 < R ? zr[1] : 0;
+      a[i] = lo | (hi << 16);
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const uint32_t* f = us + (w * K2 + k0 / 2 + q) * kPitch + r0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mma_16n8k16(acc[j][w], a, f[j * 8], f[4 * kPitch + j * 8]);
+    }
+  }
+  if (d >= D) return;
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    const int64_t b = b0 + r0 + hf * 8;
+    if (b >= B) continue;
+    uint4* yr = reinterpret_cast<uint4*>(y + b * C + c);
+    const int64_t row = slot_of(slots, slot_bytes, (int)b);
+    if (row < 0 || row >= n_rows) {
+      *yr = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    // (loaded ahead of the products they would take 32 registers more: 18.1 instead of 14.5 us
+    // for 256 rows of 3 x 4096 channels)
+    __nv_bfloat16* cr = cache + row * (int64_t)(W - 1) * C + c;
+    uint4 past[W];
+    past[0] = *reinterpret_cast<const uint4*>(x + b * C + c);
+#pragma unroll
+    for (int w = 1; w < W; ++w) past[w] = *reinterpret_cast<const uint4*>(cr + (int64_t)(W - 1 - w) * C);
+    float out[8], v[8], s[8];
+    unpack8(past[0], v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = residual ? v[e] : 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      unpack8(past[w], v);
+      if (sw) {
+        unpack8(*reinterpret_cast<const uint4*>(sw + (g * W + w) * D + d), s);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = fmaf(acc[e >> 1][w][hf * 2 + (e & 1)] + s[e], v[e], out[e]);
+    }
+    uint4 o;
+    o.x = pack_bf16x2(out[0], out[1]), o.y = pack_bf16x2(out[2], out[3]);
+    o.z = pack_bf16x2(out[4], out[5]), o.w = pack_bf16x2(out[6], out[7]);
+    *yr = o;
+#pragma unroll
+    for (int w = 1; w < W; ++w) *reinterpret_cast<uint4*>(cr + (int64_t)(W - 1 - w) * C) = past[w - 1];
+  }
+}
+
 // One batch row per blockIdx.y; the head's W weights are read by all its channels' threads
 // (the same few cache lines).
 template <typename T, int W, int VEC>
@@ -168,9 +368,10 @@ struct StepArgs {
   cudaStream_t st;
 };
 
-template <typename T, int W, int VEC, int RB>
-int lr_launch(const StepArgs& a) {
+template <typename T, int W, int VEC>
+int lr_many(const StepArgs& a) {
   const int64_t C = a.G * a.D;
+  constexpr int RB = 8;
   const dim3 grid((unsigned)((C / VEC + kThreads - 1) / kThreads), (unsigned)((a.B + RB - 1) / RB));
   const size_t smem = (size_t)a.G * a.R * RB * sizeof(float);
   lr_step_kernel<T, W, VEC, RB><<<grid, kThreads, smem, a.st>>>(
@@ -180,11 +381,43 @@ int lr_launch(const StepArgs& a) {
   return DYNCONV_OK;
 }
 
+template <typename T, int W, int VEC>
+int lr_few(const StepArgs& a) {
+  const int64_t blocks = a.G * ((a.D / VEC + 31) / 32);
+  lr_step_few_kernel<T, W, VEC><<<dim3((unsigned)blocks, (unsigned)a.B), 32 * W, 0, a.st>>>(
+      (const T*)a.x, (const T*)a.z, (const T*)a.U, (const T*)a.sw, (T*)a.cache, (T*)a.y, a.slots, a.slot_bytes,
+      a.n_rows, a.D, a.R, a.G, a.residual);
+  DYNCONV_CHECK_LAUNCH("lr_step_few_kernel");
+  return DYNCONV_OK;
+}
+
+template <int W>
+int lr_mma(const StepArgs& a) {
+  const int rp = (a.R + 15) / 16 * 16;
+  const dim3 grid((unsigned)(a.G * ((a.D + kMmaCh - 1) / kMmaCh)), (unsigned)((a.B + kMmaRows - 1) / kMmaRows));
+  const size_t smem = (size_t)W * (rp / 2) * 40 * sizeof(uint32_t);  // at most 20 KB
+  using bf = __nv_bfloat16;
+  lr_step_mma_kernel<W><<<grid, 128, smem, a.st>>>((const bf*)a.x, (const bf*)a.z, (const bf*)a.U, (const bf*)a.sw,
+                                                   (bf*)a.cache, (bf*)a.y, a.slots, a.slot_bytes, a.B, a.n_rows, a.D,
+                                                   a.R, rp, a.G, a.residual);
+  DYNCONV_CHECK_LAUNCH("lr_step_mma_kernel");
+  return DYNCONV_OK;
+}
+
+bool aligned_octets(const StepArgs& a) {
+  if (a.D % 8 != 0) return false;
+  const void* ptrs[] = {a.x, a.U, a.sw, a.cache, a.y};
+  for (const void* q : ptrs)
+    if (reinterpret_cast<uintptr_t>(q) & 15) return false;
+  return true;
+}
+
 template <typename T, int W>
 int lr_pick(const StepArgs& a, bool pairs) {
-  const bool many = a.B >= 4;
-  if (pairs) return many ? lr_launch<T, W, 2, 8>(a) : lr_launch<T, W, 2, 1>(a);
-  return many ? lr_launch<T, W, 1, 8>(a) : lr_launch<T, W, 1, 1>(a);
+  if constexpr (sizeof(T) == 2 && W <= 4)
+    if (aligned_octets(a)) return lr_mma<W>(a);
+  if (a.B < kFewRows) return pairs ? lr_few<T, W, 2>(a) : lr_few<T, W, 1>(a);
+  return pairs ? lr_many<T, W, 2>(a) : lr_many<T, W, 1>(a);
 }
 
 template <typename T, int W>
