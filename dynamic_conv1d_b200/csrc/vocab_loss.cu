@@ -271,32 +271,48 @@ int merge_launch(const Problem& p, int64_t tiles) {
 
 int tile_cols(bool tc) { return tc ? 128 : kTile; }
 
-// A piece is as wide as keeps its buffer near 256 MB (twice the L2: wide enough that the
-// products' tiles fill the GPU many times over, small beside the weight and its gradient)
-// and at least 4096 columns.  Inner dimensions are spread over several CTAs per tile while
-// the tiles of a product are fewer than two per SM and each share keeps 512 steps.
+// The piece's width is the one with the lowest estimated time among those whose buffer stays
+// within 512 MB: each product runs in rounds of one tile per SM (weight-gradient tiles are few and
+// long: at 16384 x 2048 a width of 7168 columns makes 448 of them, three rounds and four
+// tiles), each piece costs three launches and one pass over the fp32 sums of dhidden.  Times are
+// counted in blocks of 64 inner elements of a tile, 0.46 us each on the tensor cores.
+// Where a product has few tiles its inner dimension is spread over several CTAs, each share at
+// least 512 elements.
 Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc) {
-  const int64_t elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4;
-  Plan pl;
-  const int64_t cols = ((int64_t)256 << 20) / (elem * (N > 0 ? N : 1)) / 1024 * 1024;
-  pl.piece = cols < 4096 ? 4096 : cols;
-  if (pl.piece > V) pl.piece = V;
-  // equal pieces, whole tiles
-  const int64_t n = (V + pl.piece - 1) / pl.piece;
-  pl.piece = ((V + n - 1) / n + 255) / 256 * 256;
-  if (pl.piece > V) pl.piece = V;
-  pl.pitch = (pl.piece + 63) / 64 * 64;
+  const int64_t elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4, sms = sm_count();
   const int64_t tm = tc ? 128 : kTile, tn = tc ? 256 : kTile;
-  auto share = [&](int64_t rows, int64_t cols_, int64_t inner) {
-    const int64_t tiles = ((rows + tm - 1) / tm) * ((cols_ + tn - 1) / tn);
-    int64_t z = 2 * (int64_t)sm_count() / (tiles > 0 ? tiles : 1);
+  const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const auto share = [&](int64_t tiles, int64_t inner) {
+    int64_t z = 2 * sms / tiles;
     if (z > inner / 512) z = inner / 512;
     if (z > 16) z = 16;
     return (int)(z < 1 ? 1 : z);
   };
-  pl.z_h = share(N, D, pl.piece);
-  pl.z_w = share(pl.piece, D, N);
-  return pl;
+  const double launch = 10, sums = 0.5 * (double)(N * D) * 8 / 6.5e12 / 0.46e-6;
+  const int64_t n_tiles = up(N, tm), d_tiles = up(D, tn);
+  const auto cost = [&](int64_t cols, int z_h, int z_w) {
+    const double logits = (double)(up(n_tiles * up(cols, tn), sms) * up(D, 64));
+    const double dw = (double)(up(up(cols, tm) * d_tiles * z_w, sms) * up(up(N, 64), z_w));
+    const double dh = (double)(up(n_tiles * d_tiles * z_h, sms) * up(up(cols, 64), z_h));
+    return logits + dw + dh + 3 * launch + sums * z_h;
+  };
+  int64_t most = ((int64_t)512 << 20) / (elem * (N > 0 ? N : 1)) / 256 * 256;
+  if (most < 1024) most = 1024;
+  Plan best{};
+  double best_cost = 1e300;
+  for (int64_t cols = most < V ? most : up(V, 256) * 256;; cols -= 256) {
+    const int64_t full = V / cols, rest = V - full * cols;
+    const int z_h = share(n_tiles * d_tiles, cols < V ? cols : V), z_w = share(up(cols < V ? cols : V, tm) * d_tiles, N);
+    const double c = (double)full * cost(cols, z_h, z_w) + (rest ? cost(rest, z_h, z_w) : 0.0);
+    if (c < best_cost) {
+      best_cost = c;
+      best.piece = cols < V ? cols : V;
+      best.z_h = z_h, best.z_w = z_w;
+    }
+    if (cols <= 1024 || up(V, cols) > 64) break;
+  }
+  best.pitch = up(best.piece, 64) * 64;
+  return best;
 }
 
 int simple_fwd(const Problem& p, int dtype) {
