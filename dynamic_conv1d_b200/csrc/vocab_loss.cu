@@ -272,15 +272,15 @@ int merge_launch(const Problem& p, int64_t tiles) {
 int tile_cols(bool tc) { return tc ? 128 : kTile; }
 
 // The piece's width is the one with the lowest estimated time among those whose buffer stays
-// within 512 MB: each product runs in rounds of one tile per SM (weight-gradient tiles are few and
-// long: at 16384 x 2048 a width of 7168 columns makes 448 of them, three rounds and four
-// tiles), each piece costs three launches and one pass over the fp32 sums of dhidden.  Times are
+// within 512 MB: each product runs in rounds of one tile per SM or SM pair (weight-gradient tiles
+// are few and long: at 16384 x 2048 a width of 7168 columns makes 224 of them, three rounds of 74
+// and two tiles), each piece costs three launches and one pass over the fp32 sums of dhidden.  Times are
 // counted in blocks of 64 inner elements of a tile, 0.46 us each on the tensor cores.
 // Where a product has few tiles its inner dimension is spread over several CTAs, each share at
 // least 512 elements.
 Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc) {
-  const int64_t elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4, sms = sm_count();
-  const int64_t tm = tc ? 128 : kTile, tn = tc ? 256 : kTile;
+  const int64_t elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4, sms = tc ? sm_count() / 2 : sm_count();
+  const int64_t tm = tc ? 256 : kTile, tn = tc ? 256 : kTile;
   const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const auto share = [&](int64_t tiles, int64_t inner) {
     int64_t z = 2 * sms / tiles;

@@ -10,8 +10,13 @@
 // rows x 64 K steps; both land in 128-byte-swizzled tiles that tcgen05.mma reads as they
 // are, so nothing is ever transposed in memory.
 //
-// A CTA runs one producer warp (TMA ring of kStages), one MMA warp and eight epilogue warps
-// (two per TMEM lane quarter, half of the columns each) on 128 x 256 tiles; two
+// Two CTAs of a cluster (the two SMs of a TPC) work on one 256 x 256 tile with cta_group::2
+// products: each holds its 128 rows of A and half of B's 256 rows, and its 128 rows of the
+// accumulator.  A CTA by itself on 128 x 256 would move 24 KB through shared memory for each
+// product of 16 inner elements (12 KB written by TMA, 12 KB read by the product), 192 cycles at
+// 128 bytes each for 128 cycles of tensor work; a pair moves 16 KB per SM.
+// Each CTA runs one producer warp (TMA ring of kStages) and eight epilogue warps (two per TMEM
+// lane quarter, half of the columns each); the pair's first CTA issues the products.  Two
 // accumulators of 256 TMEM columns let a tile's epilogue run under the next tile's products.
 #include "vocab_loss.cuh"
 
@@ -20,11 +25,12 @@ namespace vl {
 
 namespace {
 
-constexpr int kM = 128, kN = 256, kKB = 64;  // tile, and inner elements per stage
-constexpr int kStages = 4;
+constexpr int kM = 256, kN = 256, kKB = 64;  // a pair's tile, and inner elements per stage
+constexpr int kHalfM = 128, kHalfB = 128;    // rows of A and of B in one CTA
+constexpr int kStages = 6;
 constexpr int kEpiWarps = 8;
 constexpr int kTcThreads = 64 + 32 * kEpiWarps;
-constexpr uint32_t kABytes = kM * kKB * 2, kBBytes = kN * kKB * 2, kStageBytes = kABytes + kBBytes;
+constexpr uint32_t kABytes = kHalfM * kKB * 2, kBBytes = kHalfB * kKB * 2, kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kAtom = 64 * kKB * 2;  // one 64 x 64 box
 constexpr int kSmem = kStages * (int)kStageBytes + 1024;
 constexpr int kHalf = kN / 2;  // columns of one epilogue warp; a forward tile's partials are per half
@@ -59,6 +65,68 @@ __device__ __forceinline__ Tile tile_at(const TcGemm& g, int t) {
   r.kb0 = (int)((int64_t)g.k_blocks * r.z / g.z);
   r.kb1 = (int)((int64_t)g.k_blocks * (r.z + 1) / g.z);
   return r;
+}
+
+// ---- a CTA pair: addresses in the first CTA, products over both
+
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t in_first_cta(const void* p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void arrive_in_first_cta(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Into this CTA's shared memory, counted on the first CTA's barrier.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_pair(uint32_t elected, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "n"(kDescHiSw128), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+
+// Arrives on the barrier at this place in both CTAs when the products issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(uint32_t elected, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(
+          smem_u32(bar)),
+      "r"(elected), "h"((uint16_t)3)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
 template <int MODE>
@@ -114,16 +182,18 @@ __device__ __forceinline__ void epilogue_columns(const TcGemm& g, const Problem&
 }
 
 template <int MODE, bool A_MN, bool B_MN>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     vl_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                  const __grid_constant__ TcGemm g, const __grid_constant__ Problem p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
+  // full and acce are used in the first CTA only; empty and accf in both
   __shared__ uint64_t full_bar[kStages], empty_bar[kStages], accf_bar[2], acce_bar[2], drain_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int n_tiles = g.m_tiles * g.n_tiles * g.z;
+  const int rank = (int)cta_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -132,7 +202,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&accf_bar[a], 1);
-      mbar_init(&acce_bar[a], kEpiWarps);
+      mbar_init(&acce_bar[a], 2 * kEpiWarps);
     }
     mbar_init(&drain_bar, 1);
     abort_flag = 0;
@@ -140,12 +210,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     prefetch_tensormap(&amap);
     prefetch_tensormap(&bmap);
   }
-  if (warp == 1) {
-    tmem_alloc(&tmem_slot, 512);
-    tmem_relinquish();
-  }
+  if (warp == 1) tmem_alloc_pair(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
@@ -153,8 +221,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (lane == 0) {
       int it = 0;
       bool dead = false;
-      for (int i = blockIdx.x; i < n_tiles && !dead; i += gridDim.x) {
+      for (int i = pair; i < n_tiles && !dead; i += pairs) {
         const Tile t = tile_at(g, i);
+        const int m0 = t.m * kM + rank * kHalfM, n0 = t.n * kN + rank * kHalfB;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
           const int s = it % kStages;
           if (!mbar_wait(&empty_bar[s], ((it / kStages) & 1) ^ 1, kErrWaitProducer, &abort_flag)) {
@@ -163,74 +232,76 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           uint8_t* a = smem + s * kStageBytes;
           uint8_t* b = a + kABytes;
-          mbar_arrive_expect_tx(&full_bar[s], kStageBytes);
+          const uint32_t full = in_first_cta(&full_bar[s]);
+          // the first CTA announces both CTAs' bytes (the other's may land before: the phase
+          // still waits for this arrival)
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * kStageBytes);
           if constexpr (A_MN) {
 #pragma unroll
-            for (int j = 0; j < kM / 64; ++j)
-              tma_load_2d(a + j * kAtom, &amap, &full_bar[s], t.m * kM + j * 64, kb * kKB);
+            for (int j = 0; j < kHalfM / 64; ++j) tma_load_pair(a + j * kAtom, &amap, full, m0 + j * 64, kb * kKB);
           } else {
-            tma_load_2d(a, &amap, &full_bar[s], kb * kKB, t.m * kM);
+            tma_load_pair(a, &amap, full, kb * kKB, m0);
           }
           if constexpr (B_MN) {
 #pragma unroll
-            for (int j = 0; j < kN / 64; ++j)
-              tma_load_2d(b + j * kAtom, &bmap, &full_bar[s], t.n * kN + j * 64, kb * kKB);
+            for (int j = 0; j < kHalfB / 64; ++j) tma_load_pair(b + j * kAtom, &bmap, full, n0 + j * 64, kb * kKB);
           } else {
-            tma_load_2d(b, &bmap, &full_bar[s], kb * kKB, t.n * kN);
+            tma_load_pair(b, &bmap, full, kb * kKB, n0);
           }
         }
       }
-      // a wait gave up: let the copies in flight land before the shared memory is given back
-      if (abort_flag)
+      // a wait gave up: let the copies in flight land before the shared memory is given back (the
+      // pair leaves together)
+      if (abort_flag && rank == 0)
         for (int j = max(0, it - kStages); j < it; ++j)
           mbar_drain(&full_bar[j % kStages], (j / kStages) & 1);
     }
     __syncwarp();
   } else if (warp == 1) {
-    constexpr uint32_t idesc = make_idesc_bf16(kM, kN, A_MN, B_MN);
-    int it = 0, n = 0;
-    bool dead = false;
-    for (int i = blockIdx.x; i < n_tiles && !dead; i += gridDim.x, ++n) {
-      const Tile t = tile_at(g, i);
-      const int a = n & 1;
-      if (!mbar_wait(&acce_bar[a], ((n >> 1) & 1) ^ 1, kErrWaitMma, &abort_flag)) break;
-      tc_fence_after();
-      for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-        const int s = it % kStages;
-        if (!mbar_wait(&full_bar[s], (it / kStages) & 1, kErrWaitMma, &abort_flag)) {
-          dead = true;
-          break;
-        }
+    if (rank == 0) {
+      constexpr uint32_t idesc = make_idesc_bf16(kM, kN, A_MN, B_MN);
+      const uint32_t el = elect_lane();
+      const uint32_t sb = smem_u32(smem);
+      int it = 0, n = 0;
+      bool dead = false;
+      for (int i = pair; i < n_tiles && !dead; i += pairs, ++n) {
+        const Tile t = tile_at(g, i);
+        const int a = n & 1;
+        if (!mbar_wait(&acce_bar[a], ((n >> 1) & 1) ^ 1, kErrWaitMma, &abort_flag)) break;
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");  // (half of the arrivals came from the other CTA)
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t as = smem_u32(smem + s * kStageBytes), bs = as + kABytes;
-#pragma unroll
-          for (int k = 0; k < kKB / 16; ++k) {
-            const uint64_t ad = A_MN ? make_smem_desc_sw128(as + k * 2048, kAtom, 1024) : make_smem_desc_sw128_k(as + k * 32);
-            const uint64_t bd = B_MN ? make_smem_desc_sw128(bs + k * 2048, kAtom, 1024) : make_smem_desc_sw128_k(bs + k * 32);
-            umma_f16(tmem + a * kN, ad, bd, idesc, (kb > t.kb0 || k > 0) ? 1u : 0u);
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&full_bar[s], (it / kStages) & 1, kErrWaitMma, &abort_flag)) {
+            dead = true;
+            break;
           }
-          umma_commit(&empty_bar[s]);
-          if (kb == t.kb1 - 1) umma_commit(&accf_bar[a]);
+          tc_fence_after();
+          const uint32_t as = sb + s * kStageBytes;
+          const uint32_t ad = desc_lo(as, A_MN ? kAtom : 16), bd = desc_lo(as + kABytes, B_MN ? kAtom : 16);
+#pragma unroll
+          for (int k = 0; k < kKB / 16; ++k)
+            umma_pair(el, tmem + a * kN, ad + k * (A_MN ? 2048 : 32) / 16, bd + k * (B_MN ? 2048 : 32) / 16, idesc,
+                      (kb > t.kb0 || k > 0) ? 1u : 0u);
+          umma_commit_pair(el, &empty_bar[s]);
+          if (kb == t.kb1 - 1) umma_commit_pair(el, &accf_bar[a]);
+          __syncwarp();
         }
-        __syncwarp();
       }
-    }
-    if (abort_flag) {  // the products in flight, before their accumulators are given back
-      if (lane == 0) {
-        umma_commit(&drain_bar);
+      if (abort_flag) {  // the products in flight, before their accumulators are given back
+        umma_commit_pair(el, &drain_bar);
         mbar_drain(&drain_bar, 0);
       }
-      __syncwarp();
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
     bool dead = false;
     int n = 0;
-    for (int i = blockIdx.x; i < n_tiles; i += gridDim.x, ++n) {
+    const uint32_t freed[2] = {in_first_cta(&acce_bar[0]), in_first_cta(&acce_bar[1])};
+    for (int i = pair; i < n_tiles; i += pairs, ++n) {
       const Tile t = tile_at(g, i);
       const int a = n & 1;
-      const int64_t row = (int64_t)t.m * kM + q * 32 + lane;
+      const int64_t row = (int64_t)t.m * kM + rank * kHalfM + q * 32 + lane;
       const int64_t col0 = (int64_t)t.n * kN + half * kHalf;
       const bool row_in = row < g.M;
       float f = 0.f, lse2 = 0.f;
@@ -294,12 +365,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acce_bar[a]);
+      if (lane == 0) arrive_in_first_cta(freed[a]);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  cluster_sync();  // neither CTA leaves while the other may still use its shared memory
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
 // A row-major [rows][cols] bf16 matrix as boxes of 64 columns x box_rows rows, 128-byte swizzle.
@@ -316,8 +388,8 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, TcGemm g, const Problem& 
   if (mt * nt * g.z > INT32_MAX) return set_error(DYNCONV_ERR_SHAPE, "%s: too many tiles", what);
   g.m_tiles = (int)mt, g.n_tiles = (int)nt;
   if (g.group > g.m_tiles) g.group = g.m_tiles;
-  const int tiles = g.m_tiles * g.n_tiles * g.z;
-  const int grid = tiles < sm_count() ? tiles : sm_count();
+  const int tiles = g.m_tiles * g.n_tiles * g.z, most = sm_count() / 2;
+  const int grid = 2 * (tiles < most ? tiles : most);
   cudaError_t e = cudaFuncSetAttribute(vl_tc_kernel<MODE, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -347,8 +419,8 @@ bool tc_supported(const Problem& p, int dtype) {
 int tc_fwd(const Problem& p) {
   CUtensorMap a, b;
   int s;
-  if ((s = matrix_map(&a, p.hidden, p.D, p.N, p.D, kM))) return s;
-  if ((s = matrix_map(&b, p.weight, p.D, p.V, p.D, kN))) return s;
+  if ((s = matrix_map(&a, p.hidden, p.D, p.N, p.D, kHalfM))) return s;
+  if ((s = matrix_map(&b, p.weight, p.D, p.V, p.D, kHalfB))) return s;
   TcGemm g{};
   g.M = p.N, g.N = p.V, g.k_blocks = (int)((p.D + kKB - 1) / kKB), g.z = 1, g.group = row_group(p.D);
   if ((s = launch<kTcForward, false, false>(a, b, g, p, "vl_tc_kernel (forward)"))) return s;
@@ -358,7 +430,7 @@ int tc_fwd(const Problem& p) {
 int tc_bwd(const Problem& p, const Plan& pl) {
   int s;
   CUtensorMap hk, hm;
-  if ((s = matrix_map(&hk, p.hidden, p.D, p.N, p.D, kM))) return s;
+  if ((s = matrix_map(&hk, p.hidden, p.D, p.N, p.D, kHalfM))) return s;
   if ((s = matrix_map(&hm, p.hidden, p.D, p.N, p.D, 64))) return s;
   const int d_blocks = (int)((p.D + kKB - 1) / kKB);
   for (int64_t v0 = 0; v0 < p.V; v0 += pl.piece) {
@@ -366,9 +438,9 @@ int tc_bwd(const Problem& p, const Plan& pl) {
     const __nv_bfloat16* w = (const __nv_bfloat16*)p.weight + v0 * p.D;
     // maps of exactly this piece: what lies beyond it reads as zero
     CUtensorMap wk, wm, pk, pm;
-    if ((s = matrix_map(&wk, w, p.D, vp, p.D, kN))) return s;
+    if ((s = matrix_map(&wk, w, p.D, vp, p.D, kHalfB))) return s;
     if ((s = matrix_map(&wm, w, p.D, vp, p.D, 64))) return s;
-    if ((s = matrix_map(&pk, p.piece, vp, p.N, pl.pitch, kM))) return s;
+    if ((s = matrix_map(&pk, p.piece, vp, p.N, pl.pitch, kHalfM))) return s;
     if ((s = matrix_map(&pm, p.piece, vp, p.N, pl.pitch, 64))) return s;
     TcGemm g{};
     g.M = p.N, g.N = vp, g.k_blocks = d_blocks, g.z = 1, g.group = row_group(p.D);
