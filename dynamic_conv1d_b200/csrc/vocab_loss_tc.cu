@@ -32,7 +32,9 @@ constexpr int kEpiWarps = 8;
 constexpr int kTcThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kABytes = kHalfM * kKB * 2, kBBytes = kHalfB * kKB * 2, kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kAtom = 64 * kKB * 2;  // one 64 x 64 box
-constexpr int kSmem = kStages * (int)kStageBytes + 1024;
+constexpr uint32_t kStageOut = 32 * 128;  // an epilogue warp's 32 rows x 64 columns of bf16, staged for a TMA store
+constexpr int kSmem = kStages * (int)kStageBytes + kEpiWarps * (int)kStageOut + 1024;
+static_assert(kSmem <= 232448 - 1024, "shared memory of one CTA");
 constexpr int kHalf = kN / 2;  // columns of one epilogue warp; a forward tile's partials are per half
 
 enum TcMode { kTcForward, kTcGrad, kTcAdd, kTcStore };
@@ -43,9 +45,10 @@ struct TcGemm {
   int m_tiles, n_tiles, z;
   int group;           // m tiles that share a sweep over n: consecutive tiles walk a group's rows first
   int64_t col0;        // kTcGrad: first vocabulary column
-  void* out;
+  void* out;           // kTcAdd: fp32 [z][M][N] (the bf16 outputs go through a tensor map)
   int64_t out_ld;
   int add;             // kTcAdd: add to what is there
+  void* result;        // kTcAdd: not null: the last sums, rounded to bf16
 };
 
 struct Tile {
@@ -129,62 +132,55 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
-template <int MODE>
-__device__ __forceinline__ void epilogue_columns(const TcGemm& g, const Problem& p, const float (&v)[32], int64_t row,
-                                                 int64_t col, bool row_in, float f, float lse2, int64_t t, int z) {
-  // col: first of the 32 columns; dimensions of the outputs are multiples of 8 (kTcGrad: the
-  // piece buffer's pitch is), so whole groups of 8 are in or out
-  if constexpr (MODE == kTcGrad) {
-    float d[32];
+// dl of 32 columns, in place.  f: the row's factor, at: the target's column among the 32.
+__device__ __forceinline__ void logits_gradient(float (&v)[32], float f, float lse2, int64_t at) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) d[j] = f != 0.f ? ex2(fmaf(v[j], kLog2e, -lse2)) * f : 0.f;  // (an ignored row's NaN stays out)
-    const int64_t at = t - g.col0 - col;
-    if (at >= 0 && at < 32) {
+  for (int j = 0; j < 32; ++j) v[j] = f != 0.f ? ex2(fmaf(v[j], kLog2e, -lse2)) * f : 0.f;  // (an ignored row's NaN stays out)
+  if (at >= 0 && at < 32) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j == at) d[j] -= f;
+    for (int j = 0; j < 32; ++j)
+      if (j == at) v[j] -= f;
+  }
+}
+
+// 32 columns of a row of the fp32 sums, added up over pieces; the last piece rounds them into
+// the result itself.  Widths are multiples of 8.
+__device__ __forceinline__ void add_columns(const TcGemm& g, const float (&v)[32], int64_t row, int64_t col, int z) {
+  float* o = (float*)g.out + ((int64_t)z * g.M + row) * g.out_ld + col;
+  __nv_bfloat16* r = (__nv_bfloat16*)g.result + row * g.out_ld + col;
+#pragma unroll
+  for (int j = 0; j < 32; j += 8) {
+    if (col + j >= g.N) break;
+    float4 u0 = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]), u1 = make_float4(v[j + 4], v[j + 5], v[j + 6], v[j + 7]);
+    if (g.add) {
+      const float4 w0 = *reinterpret_cast<const float4*>(o + j), w1 = *reinterpret_cast<const float4*>(o + j + 4);
+      u0.x += w0.x, u0.y += w0.y, u0.z += w0.z, u0.w += w0.w;
+      u1.x += w1.x, u1.y += w1.y, u1.z += w1.z, u1.w += w1.w;
     }
-    if (!row_in) return;
-    __nv_bfloat16* o = (__nv_bfloat16*)g.out + row * g.out_ld + col;
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      if (col + j >= g.N) break;
-      uint4 u;
-      u.x = pack_bf16x2(d[j], d[j + 1]), u.y = pack_bf16x2(d[j + 2], d[j + 3]);
-      u.z = pack_bf16x2(d[j + 4], d[j + 5]), u.w = pack_bf16x2(d[j + 6], d[j + 7]);
-      *reinterpret_cast<uint4*>(o + j) = u;
+    if (g.result) {
+      *reinterpret_cast<uint4*>(r + j) =
+          make_uint4(pack_bf16x2(u0.x, u0.y), pack_bf16x2(u0.z, u0.w), pack_bf16x2(u1.x, u1.y), pack_bf16x2(u1.z, u1.w));
+    } else {
+      *reinterpret_cast<float4*>(o + j) = u0;
+      *reinterpret_cast<float4*>(o + j + 4) = u1;
     }
-  } else if constexpr (MODE == kTcAdd) {
-    if (!row_in) return;
-    float* o = (float*)g.out + ((int64_t)z * g.M + row) * g.out_ld + col;
+  }
+}
+
+// 32 columns of a row, rounded into half of the warp's staged tile (128-byte swizzle).
+__device__ __forceinline__ void stage_columns(uint8_t* tile, int row, int half, const float (&v)[32]) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      if (col + j >= g.N) break;
-      float4 u = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-      if (g.add) {
-        const float4 w = *reinterpret_cast<const float4*>(o + j);
-        u.x += w.x, u.y += w.y, u.z += w.z, u.w += w.w;
-      }
-      *reinterpret_cast<float4*>(o + j) = u;
-    }
-  } else if constexpr (MODE == kTcStore) {
-    if (!row_in) return;
-    __nv_bfloat16* o = (__nv_bfloat16*)g.out + row * g.out_ld + col;
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      if (col + j >= g.N) break;
-      uint4 u;
-      u.x = pack_bf16x2(v[j], v[j + 1]), u.y = pack_bf16x2(v[j + 2], v[j + 3]);
-      u.z = pack_bf16x2(v[j + 4], v[j + 5]), u.w = pack_bf16x2(v[j + 6], v[j + 7]);
-      *reinterpret_cast<uint4*>(o + j) = u;
-    }
+  for (int j = 0; j < 4; ++j) {
+    const uint4 u = make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                               pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+    *reinterpret_cast<uint4*>(tile + row * 128 + (((half * 4 + j) ^ (row & 7)) << 4)) = u;
   }
 }
 
 template <int MODE, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     vl_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
-                 const __grid_constant__ TcGemm g, const __grid_constant__ Problem p) {
+                 const __grid_constant__ CUtensorMap omap, const __grid_constant__ TcGemm g, const __grid_constant__ Problem p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
   // full and acce are used in the first CTA only; empty and accf in both
@@ -355,8 +351,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
               for (int j = 0; j < 32; ++j)
                 if (j == at) p.tgt[row] = v[j];
             }
+          } else if constexpr (MODE == kTcAdd) {
+            if (row_in) add_columns(g, v, row, col0 + c, t.z);
           } else {
-            epilogue_columns<MODE>(g, p, v, row, col0 + c, row_in, f, lse2, target, t.z);
+            // bf16: 64 columns at a time through the warp's staged tile and a TMA store, which
+            // leaves out what lies beyond the matrix
+            uint8_t* tile = smem + kStages * kStageBytes + (warp - 2) * kStageOut;
+            if ((c & 32) == 0) {
+              if (lane == 0) bulk_wait_group_read<0>();
+              __syncwarp();
+            }
+            if constexpr (MODE == kTcGrad) logits_gradient(v, f, lse2, target - g.col0 - (col0 + c));
+            stage_columns(tile, lane, (c >> 5) & 1, v);
+            if (c & 32) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&omap, tile, (int)(col0 + c - 32), t.m * kM + rank * kHalfM + q * 32);
+                bulk_commit_group();
+              }
+            }
           }
         }
         if constexpr (MODE == kTcForward) {
@@ -366,6 +380,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_in_first_cta(freed[a]);
+    }
+    if constexpr (MODE == kTcGrad || MODE == kTcStore) {
+      if (lane == 0) bulk_wait_group<0>();
     }
   }
   tc_fence_before();
@@ -383,7 +400,7 @@ int matrix_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, i
 }
 
 template <int MODE, bool A_MN, bool B_MN>
-int launch(const CUtensorMap& a, const CUtensorMap& b, TcGemm g, const Problem& p, const char* what) {
+int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, TcGemm g, const Problem& p, const char* what) {
   const int64_t mt = (g.M + kM - 1) / kM, nt = (g.N + kN - 1) / kN;
   if (mt * nt * g.z > INT32_MAX) return set_error(DYNCONV_ERR_SHAPE, "%s: too many tiles", what);
   g.m_tiles = (int)mt, g.n_tiles = (int)nt;
@@ -395,7 +412,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, TcGemm g, const Problem& 
     cudaGetLastError();
     return cuda_status(e, "cudaFuncSetAttribute(vl_tc)");
   }
-  vl_tc_kernel<MODE, A_MN, B_MN><<<grid, kTcThreads, kSmem, p.st>>>(a, b, g, p);
+  vl_tc_kernel<MODE, A_MN, B_MN><<<grid, kTcThreads, kSmem, p.st>>>(a, b, o, g, p);
   DYNCONV_CHECK_LAUNCH(what);
   return DYNCONV_OK;
 }
@@ -423,7 +440,7 @@ int tc_fwd(const Problem& p) {
   if ((s = matrix_map(&b, p.weight, p.D, p.V, p.D, kHalfB))) return s;
   TcGemm g{};
   g.M = p.N, g.N = p.V, g.k_blocks = (int)((p.D + kKB - 1) / kKB), g.z = 1, g.group = row_group(p.D);
-  if ((s = launch<kTcForward, false, false>(a, b, g, p, "vl_tc_kernel (forward)"))) return s;
+  if ((s = launch<kTcForward, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)"))) return s;
   return merge_launch(p, (p.V + kN - 1) / kN * 2);
 }
 
@@ -437,25 +454,27 @@ int tc_bwd(const Problem& p, const Plan& pl) {
     const int64_t vp = p.V - v0 < pl.piece ? p.V - v0 : pl.piece;
     const __nv_bfloat16* w = (const __nv_bfloat16*)p.weight + v0 * p.D;
     // maps of exactly this piece: what lies beyond it reads as zero
-    CUtensorMap wk, wm, pk, pm;
+    CUtensorMap wk, wm, pk, pm, po;
     if ((s = matrix_map(&wk, w, p.D, vp, p.D, kHalfB))) return s;
     if ((s = matrix_map(&wm, w, p.D, vp, p.D, 64))) return s;
     if ((s = matrix_map(&pk, p.piece, vp, p.N, pl.pitch, kHalfM))) return s;
     if ((s = matrix_map(&pm, p.piece, vp, p.N, pl.pitch, 64))) return s;
+    if ((s = matrix_map(&po, p.piece, vp, p.N, pl.pitch, 32))) return s;
     TcGemm g{};
     g.M = p.N, g.N = vp, g.k_blocks = d_blocks, g.z = 1, g.group = row_group(p.D);
-    g.col0 = v0, g.out = p.piece, g.out_ld = pl.pitch;
-    if ((s = launch<kTcGrad, false, false>(hk, wk, g, p, "vl_tc_kernel (logits' gradient)"))) return s;
+    g.col0 = v0;
+    if ((s = launch<kTcGrad, false, false>(hk, wk, po, g, p, "vl_tc_kernel (logits' gradient)"))) return s;
     if (p.dweight) {
       __nv_bfloat16* dw = (__nv_bfloat16*)p.dweight + v0 * p.D;
       TcGemm gw{};
       gw.M = vp, gw.N = p.D, gw.k_blocks = (int)((p.N + kKB - 1) / kKB), gw.z = pl.z_w, gw.group = 1, gw.out_ld = p.D;
       if (pl.z_w == 1) {
-        gw.out = dw;
-        if ((s = launch<kTcStore, true, true>(pm, hm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
+        CUtensorMap wo;
+        if ((s = matrix_map(&wo, dw, p.D, vp, p.D, 32))) return s;
+        if ((s = launch<kTcStore, true, true>(pm, hm, wo, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
       } else {
         gw.out = p.acc_w;
-        if ((s = launch<kTcAdd, true, true>(pm, hm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
+        if ((s = launch<kTcAdd, true, true>(pm, hm, pm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
         if ((s = reduce_partials_launch(p.acc_w, pl.z_w, vp * p.D, nullptr, dw, DYNCONV_DTYPE_BF16, p.st))) return s;
       }
     }
@@ -465,10 +484,11 @@ int tc_bwd(const Problem& p, const Plan& pl) {
       // the first piece fills every share; a short last one may have fewer blocks than shares
       gh.z = pl.z_h < gh.k_blocks ? pl.z_h : gh.k_blocks;
       gh.out = p.acc_h, gh.out_ld = p.D, gh.add = v0 > 0;
-      if ((s = launch<kTcAdd, false, true>(pk, wm, gh, p, "vl_tc_kernel (hidden gradient)"))) return s;
+      gh.result = pl.z_h == 1 && v0 + vp == p.V ? p.dhidden : nullptr;
+      if ((s = launch<kTcAdd, false, true>(pk, wm, pk, gh, p, "vl_tc_kernel (hidden gradient)"))) return s;
     }
   }
-  return finish_hidden(p, pl, DYNCONV_DTYPE_BF16);
+  return pl.z_h > 1 ? finish_hidden(p, pl, DYNCONV_DTYPE_BF16) : DYNCONV_OK;
 }
 
 }  // namespace vl
