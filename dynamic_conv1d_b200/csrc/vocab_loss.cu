@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads) vl_gemm_kernel(const Gemm g, const P
           float* o = (float*)g.out + ((int64_t)blockIdx.z * g.M + m) * g.out_ld + n;
           *o = g.add ? *o + acc[i][j] : acc[i][j];
         } else {
-          ((T*)g.out)[m * g.out_ld + n] = Elem<T>::from_f(acc[i][j]);
+          ((T*)g.out)[m * g.out_ld + n] = Elem<T>::from_f(acc[i][j] * result_factor(p));
         }
       }
     }
@@ -236,8 +236,7 @@ int bwd(const Problem& p, const Plan& pl, int dtype) {
       } else {
         gw.out = p.acc_w;
         if ((s = gemm<T, kAccumulate>(gw, p, pl.z_w, "vl_gemm_kernel (weight gradient)"))) return s;
-        if ((s = reduce_partials_launch(p.acc_w, pl.z_w, vp * p.D, nullptr, (T*)p.dweight + v0 * p.D, dtype, p.st)))
-          return s;
+        if ((s = finish_launch(p, p.acc_w, pl.z_w, vp * p.D, (T*)p.dweight + v0 * p.D, dtype))) return s;
       }
     }
     if (p.dhidden) {
@@ -249,14 +248,47 @@ int bwd(const Problem& p, const Plan& pl, int dtype) {
       if ((s = gemm<T, kAccumulate>(gh, p, pl.z_h, "vl_gemm_kernel (hidden gradient)"))) return s;
     }
   }
-  return finish_hidden(p, pl, dtype);
+  return p.dhidden ? finish_launch(p, p.acc_h, pl.z_h, p.N * p.D, p.dhidden, dtype) : DYNCONV_OK;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) vl_finish_kernel(const Problem p, const float* __restrict__ parts, int n_parts,
+                                                        int64_t n, T* __restrict__ out) {
+  const float f = result_factor(p);
+  const int64_t step = (int64_t)gridDim.x * blockDim.x;
+  int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (n % 4 == 0) {  // (the parts are 256-byte aligned; the output's rows may start anywhere)
+    for (; i < n / 4; i += step) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int z = 0; z < n_parts; ++z) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(parts + z * n) + i);
+        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+      }
+      const float r[4] = {a.x * f, a.y * f, a.z * f, a.w * f};
+      store_span(out + 4 * i, r);
+    }
+    return;
+  }
+  for (; i < n; i += step) {
+    float a = 0.f;
+    for (int z = 0; z < n_parts; ++z) a += __ldg(parts + z * n + i);
+    out[i] = Elem<T>::from_f(a * f);
+  }
 }
 
 }  // namespace
 
-int finish_hidden(const Problem& p, const Plan& pl, int dtype) {
-  if (!p.dhidden) return DYNCONV_OK;
-  return reduce_partials_launch(p.acc_h, pl.z_h, p.N * p.D, nullptr, p.dhidden, dtype, p.st);
+int finish_launch(const Problem& p, const float* parts, int n_parts, int64_t n, void* out, int dtype) {
+  if (n <= 0) return DYNCONV_OK;
+  int64_t grid = (n / 4 + 255) / 256 + 1;
+  if (grid > 16 * (int64_t)sm_count()) grid = 16 * (int64_t)sm_count();
+  if (dtype == DYNCONV_DTYPE_BF16)
+    vl_finish_kernel<<<(unsigned)grid, 256, 0, p.st>>>(p, parts, n_parts, n, (__nv_bfloat16*)out);
+  else
+    vl_finish_kernel<<<(unsigned)grid, 256, 0, p.st>>>(p, parts, n_parts, n, (float*)out);
+  DYNCONV_CHECK_LAUNCH("vl_finish_kernel");
+  return DYNCONV_OK;
 }
 
 int merge_launch(const Problem& p, int64_t tiles) {

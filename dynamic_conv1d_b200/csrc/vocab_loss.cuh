@@ -5,6 +5,11 @@
 //     lse_n = log sum_v exp(l_nv),  loss_n = lse_n - l_{n,t_n}
 //     dl_nv = (exp(l_nv - lse_n) - [v = t_n]) * g_n
 //     dhidden = dl weight,  dweight = dl^T hidden
+// The factors g_n are dloss (sum) or dloss / count (mean) of every row that counts: they multiply
+// the finished products in fp32, and the operand dl is exp(l - lse) - [v = t] alone, so that
+// its largest entry, near -1, is not rounded together with a factor that is the same for every
+// row (one bf16 rounding of the factor moved both gradients by up to 2^-8).  With one dloss
+// per row (no reduction) the factors differ and are part of dl.
 // Forward: one matrix product whose epilogue keeps, of each tile, every row's maximum and
 // sum of exponentials (fp32); a second kernel merges the tiles.  Backward, piece of the
 // vocabulary by piece: the product again, with dl rounded to the tensors' type into a
@@ -51,19 +56,25 @@ struct Plan {
   int z_h, z_w;
 };
 
-// A row's factor: 0 where the target is ignored or outside the vocabulary.
+// A row's factor within dl: 0 where the target is ignored or outside the vocabulary.
 __device__ __forceinline__ float row_factor(const Problem& p, int64_t n, int64_t t) {
   if (t == p.ignore || t < 0 || t >= p.V) return 0.f;
-  if (p.reduction == kNone) return p.dloss[n];
-  return p.reduction == kSum ? p.dloss[0] : p.dloss[0] / p.stats[1];
+  return p.reduction == kNone ? p.dloss[n] : 1.f;
+}
+
+// The factor of both finished gradients.  (No row that counts: dl is zero, and so are they.)
+__device__ __forceinline__ float result_factor(const Problem& p) {
+  if (p.reduction == kNone) return 1.f;
+  if (p.reduction == kSum) return p.dloss[0];
+  return p.stats[1] > 0.f ? p.dloss[0] / p.stats[1] : 0.f;
 }
 
 int tile_cols(bool tc);  // columns of the vocabulary in one forward tile
 bool tc_supported(const Problem& p, int dtype);
 Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc);
 int merge_launch(const Problem& p, int64_t tiles);
-// cast of acc_h's z_h parts into dhidden
-int finish_hidden(const Problem& p, const Plan& pl, int dtype);
+// out[i] = result_factor * the sum of n-element parts, in part order, rounded to dtype
+int finish_launch(const Problem& p, const float* parts, int n_parts, int64_t n, void* out, int dtype);
 
 int simple_fwd(const Problem& p, int dtype);
 int simple_bwd(const Problem& p, const Plan& pl, int dtype);
@@ -71,6 +82,4 @@ int tc_fwd(const Problem& p);
 int tc_bwd(const Problem& p, const Plan& pl);
 
 }  // namespace vl
-
-int reduce_partials_launch(const float* part, int P, int64_t n, float* out_f32, void* out, int dtype, cudaStream_t st);
 }  // namespace dynconv

@@ -35,9 +35,14 @@ constexpr uint32_t kAtom = 64 * kKB * 2;  // one 64 x 64 box
 constexpr uint32_t kStageOut = 32 * 128;  // an epilogue warp's 32 rows x 64 columns of bf16, staged for a TMA store
 constexpr int kSmem = kStages * (int)kStageBytes + kEpiWarps * (int)kStageOut + 1024;
 static_assert(kSmem <= 232448 - 1024, "shared memory of one CTA");
+// The tensor core's accumulation truncates: a sum of 4096 products came out 3.8e-6 of itself too
+// small, which the loss's 32 bits would show (1.1e-6 of it).  Where the inner dimension is longer
+// than kChain blocks (2048 products), the forward sums that many at a time and adds those sums
+// up in registers (kTcForwardLong; a form of its own, as it needs 128 registers more).
+constexpr int kChain = 32;
 constexpr int kHalf = kN / 2;  // columns of one epilogue warp; a forward tile's partials are per half
 
-enum TcMode { kTcForward, kTcGrad, kTcAdd, kTcStore };
+enum TcMode { kTcForward, kTcForwardLong, kTcGrad, kTcAdd, kTcStore };
 
 struct TcGemm {
   int64_t M, N;        // extents of the output
@@ -145,7 +150,8 @@ __device__ __forceinline__ void logits_gradient(float (&v)[32], float f, float l
 
 // 32 columns of a row of the fp32 sums, added up over pieces; the last piece rounds them into
 // the result itself.  Widths are multiples of 8.
-__device__ __forceinline__ void add_columns(const TcGemm& g, const float (&v)[32], int64_t row, int64_t col, int z) {
+__device__ __forceinline__ void add_columns(const TcGemm& g, const float (&v)[32], int64_t row, int64_t col, int z,
+                                            float factor) {
   float* o = (float*)g.out + ((int64_t)z * g.M + row) * g.out_ld + col;
   __nv_bfloat16* r = (__nv_bfloat16*)g.result + row * g.out_ld + col;
 #pragma unroll
@@ -158,6 +164,8 @@ __device__ __forceinline__ void add_columns(const TcGemm& g, const float (&v)[32
       u1.x += w1.x, u1.y += w1.y, u1.z += w1.z, u1.w += w1.w;
     }
     if (g.result) {
+      u0.x *= factor, u0.y *= factor, u0.z *= factor, u0.w *= factor;
+      u1.x *= factor, u1.y *= factor, u1.z *= factor, u1.w *= factor;
       *reinterpret_cast<uint4*>(r + j) =
           make_uint4(pack_bf16x2(u0.x, u0.y), pack_bf16x2(u0.z, u0.w), pack_bf16x2(u1.x, u1.y), pack_bf16x2(u1.z, u1.w));
     } else {
@@ -181,6 +189,7 @@ template <int MODE, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     vl_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                  const __grid_constant__ CUtensorMap omap, const __grid_constant__ TcGemm g, const __grid_constant__ Problem p) {
+  constexpr bool kForward = MODE == kTcForward || MODE == kTcForwardLong;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
   // full and acce are used in the first CTA only; empty and accf in both
@@ -262,11 +271,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       bool dead = false;
       for (int i = pair; i < n_tiles && !dead; i += pairs, ++n) {
         const Tile t = tile_at(g, i);
-        const int a = n & 1;
-        if (!mbar_wait(&acce_bar[a], ((n >> 1) & 1) ^ 1, kErrWaitMma, &abort_flag)) break;
-        asm volatile("fence.acq_rel.cluster;" ::: "memory");  // (half of the arrivals came from the other CTA)
-        tc_fence_after();
+        int a = n & 1, first = t.kb0;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+          if (kb == t.kb0 || (MODE == kTcForwardLong && kb - first == kChain)) {
+            if (kb > t.kb0) ++n;
+            a = n & 1, first = kb;
+            if (!mbar_wait(&acce_bar[a], ((n >> 1) & 1) ^ 1, kErrWaitMma, &abort_flag)) {
+              dead = true;
+              break;
+            }
+            asm volatile("fence.acq_rel.cluster;" ::: "memory");  // (half of the arrivals came from the other CTA)
+            tc_fence_after();
+          }
           const int s = it % kStages;
           if (!mbar_wait(&full_bar[s], (it / kStages) & 1, kErrWaitMma, &abort_flag)) {
             dead = true;
@@ -278,9 +294,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int k = 0; k < kKB / 16; ++k)
             umma_pair(el, tmem + a * kN, ad + k * (A_MN ? 2048 : 32) / 16, bd + k * (B_MN ? 2048 : 32) / 16, idesc,
-                      (kb > t.kb0 || k > 0) ? 1u : 0u);
+                      (kb > first || k > 0) ? 1u : 0u);
           umma_commit_pair(el, &empty_bar[s]);
-          if (kb == t.kb1 - 1) umma_commit_pair(el, &accf_bar[a]);
+          if (kb == t.kb1 - 1 || (MODE == kTcForwardLong && kb - first == kChain - 1)) umma_commit_pair(el, &accf_bar[a]);
           __syncwarp();
         }
       }
@@ -293,16 +309,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     const int q = warp & 3, half = (warp - 2) >> 2;
     bool dead = false;
     int n = 0;
+    const float factor = MODE == kTcAdd || MODE == kTcStore ? result_factor(p) : 1.f;
     const uint32_t freed[2] = {in_first_cta(&acce_bar[0]), in_first_cta(&acce_bar[1])};
     for (int i = pair; i < n_tiles; i += pairs, ++n) {
       const Tile t = tile_at(g, i);
-      const int a = n & 1;
+      int a = n & 1;
       const int64_t row = (int64_t)t.m * kM + rank * kHalfM + q * 32 + lane;
       const int64_t col0 = (int64_t)t.n * kN + half * kHalf;
       const bool row_in = row < g.M;
       float f = 0.f, lse2 = 0.f;
       int64_t target = -1;
-      if constexpr (MODE == kTcForward || MODE == kTcGrad) {
+      if constexpr (kForward || MODE == kTcGrad) {
         if (row_in) target = p.target[row];
         if constexpr (MODE == kTcGrad) {
           if (row_in) {
@@ -311,25 +328,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           }
         }
       }
+      float chained[MODE == kTcForwardLong ? kHalf : 1];  // the sums of the chains before the last
+      if constexpr (MODE == kTcForwardLong) {
+        const int chains = (g.k_blocks + kChain - 1) / kChain;
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) chained[j] = 0.f;
+#pragma unroll 1
+        for (int k = 0; k + 1 < chains; ++k, ++n) {
+          a = n & 1;
+          if (!dead) dead = !mbar_wait(&accf_bar[a], (n >> 1) & 1, kErrWaitEpilogue, &abort_flag);
+          tc_fence_after();
+          if (!dead) {
+            const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + a * kN + half * kHalf;
+#pragma unroll
+            for (int c = 0; c < kHalf; c += 8) {
+              float v[8];
+              tmem_ld8(base + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 8; ++j) chained[c + j] += v[j];
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_in_first_cta(freed[a]);
+        }
+        a = n & 1;
+      }
       if (!dead) dead = !mbar_wait(&accf_bar[a], (n >> 1) & 1, kErrWaitEpilogue, &abort_flag);
       tc_fence_after();
       if (!dead) {
         const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + a * kN + half * kHalf;
         float m2 = -INFINITY, sum = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < kHalf; c += 32) {
-          float v[32];
-          tmem_ld32(base + c, v);
+        const int there = (int)max((int64_t)0, min((int64_t)kHalf, g.N - col0));  // columns that are there
+        const int64_t t_col = target - col0;
+        const int mine = row_in && t_col >= 0 && t_col < there ? (int)t_col : -1;  // the target's column
+        constexpr int kStep = MODE == kTcForwardLong ? 16 : 32;  // columns at a time (registers)
+#pragma unroll (MODE == kTcForwardLong ? kHalf / kStep : 1)
+        for (int c = 0; c < kHalf; c += kStep) {
+          float v[kStep];
+          if constexpr (MODE == kTcForwardLong)
+            tmem_ld16(base + c, v);
+          else
+            tmem_ld32(base + c, v);
           tmem_ld_wait();
-          if constexpr (MODE == kTcForward) {
-            const int64_t left = g.N - (col0 + c);  // columns that are there
-            float mx = -INFINITY;
-            if (left >= 32) {
+          if constexpr (MODE == kTcForwardLong) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
+            for (int j = 0; j < kStep; ++j) v[j] += chained[c + j];
+          }
+          if constexpr (kForward) {
+            const int left = there - c;
+            float mx = -INFINITY;
+            if (left >= kStep) {
+#pragma unroll
+              for (int j = 0; j < kStep; ++j) mx = fmaxf(mx, v[j]);
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
+              for (int j = 0; j < kStep; ++j) {
                 if (j >= left) v[j] = -INFINITY;
                 mx = fmaxf(mx, v[j]);
               }
@@ -338,21 +393,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             if (m_new > -INFINITY) {
               float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) {
+              for (int j = 0; j < kStep; j += 2) {
                 s0 += ex2(fmaf(v[j], kLog2e, -m_new));
                 s1 += ex2(fmaf(v[j + 1], kLog2e, -m_new));
               }
               sum = fmaf(sum, ex2(m2 - m_new), s0 + s1);
               m2 = m_new;
             }
-            const int64_t at = target - (col0 + c);
-            if (row_in && at >= 0 && at < 32 && at < left) {
+            if (mine >= c && mine < c + kStep) {
+              uint32_t bits = 0;  // (selected by masks: an indexed read would put v into local memory)
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j == at) p.tgt[row] = v[j];
+              for (int j = 0; j < kStep; ++j) bits |= __float_as_uint(v[j]) & -(uint32_t)(j == mine - c);
+              p.tgt[row] = __uint_as_float(bits);
             }
           } else if constexpr (MODE == kTcAdd) {
-            if (row_in) add_columns(g, v, row, col0 + c, t.z);
+            if (row_in) add_columns(g, v, row, col0 + c, t.z, factor);
           } else {
             // bf16: 64 columns at a time through the warp's staged tile and a TMA store, which
             // leaves out what lies beyond the matrix
@@ -361,7 +416,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
               if (lane == 0) bulk_wait_group_read<0>();
               __syncwarp();
             }
-            if constexpr (MODE == kTcGrad) logits_gradient(v, f, lse2, target - g.col0 - (col0 + c));
+            if constexpr (MODE == kTcGrad) {
+              logits_gradient(v, f, lse2, target - g.col0 - (col0 + c));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= factor;
+            }
             stage_columns(tile, lane, (c >> 5) & 1, v);
             if (c & 32) {
               fence_proxy_async_smem();
@@ -373,7 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             }
           }
         }
-        if constexpr (MODE == kTcForward) {
+        if constexpr (kForward) {
           if (row_in) p.part[((int64_t)t.n * 2 + half) * g.M + row] = make_float2(m2, sum);
         }
       }
@@ -440,7 +500,9 @@ int tc_fwd(const Problem& p) {
   if ((s = matrix_map(&b, p.weight, p.D, p.V, p.D, kHalfB))) return s;
   TcGemm g{};
   g.M = p.N, g.N = p.V, g.k_blocks = (int)((p.D + kKB - 1) / kKB), g.z = 1, g.group = row_group(p.D);
-  if ((s = launch<kTcForward, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)"))) return s;
+  s = g.k_blocks <= kChain ? launch<kTcForward, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)")
+                           : launch<kTcForwardLong, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)");
+  if (s) return s;
   return merge_launch(p, (p.V + kN - 1) / kN * 2);
 }
 
@@ -475,7 +537,7 @@ int tc_bwd(const Problem& p, const Plan& pl) {
       } else {
         gw.out = p.acc_w;
         if ((s = launch<kTcAdd, true, true>(pm, hm, pm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
-        if ((s = reduce_partials_launch(p.acc_w, pl.z_w, vp * p.D, nullptr, dw, DYNCONV_DTYPE_BF16, p.st))) return s;
+        if ((s = finish_launch(p, p.acc_w, pl.z_w, vp * p.D, dw, DYNCONV_DTYPE_BF16))) return s;
       }
     }
     if (p.dhidden) {
@@ -488,7 +550,8 @@ int tc_bwd(const Problem& p, const Plan& pl) {
       if ((s = launch<kTcAdd, false, true>(pk, wm, pk, gh, p, "vl_tc_kernel (hidden gradient)"))) return s;
     }
   }
-  return pl.z_h > 1 ? finish_hidden(p, pl, DYNCONV_DTYPE_BF16) : DYNCONV_OK;
+  if (!p.dhidden || pl.z_h == 1) return DYNCONV_OK;
+  return finish_launch(p, p.acc_h, pl.z_h, p.N * p.D, p.dhidden, DYNCONV_DTYPE_BF16);
 }
 
 }  // namespace vl
