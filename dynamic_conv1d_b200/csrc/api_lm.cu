@@ -229,8 +229,7 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
 
 size_t dynconv_vocab_loss_fwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype) {
   if (check_loss(N, D, V, 0, dtype)) return 0;
-  // the CUDA-core tiles are the narrower ones: enough for either path
-  const int64_t tiles = (V + vl::tile_cols(false) - 1) / vl::tile_cols(false) + 2;
+  const int64_t tiles = (V + vl::kNarrowestTile - 1) / vl::kNarrowestTile + 2;  // enough for either path
   return align_up((size_t)tiles * N * sizeof(float2)) + align_up((size_t)N * sizeof(float));
 }
 

@@ -8,15 +8,13 @@ namespace vl {
 
 namespace {
 
-constexpr int kTile = 64;   // rows and columns of a tile
 constexpr int kK = 16;      // inner steps staged at once
 constexpr int kThreads = 256;
-constexpr int kLd = kTile + 4;
 
 enum Mode { kForward, kGrad, kAccumulate, kStore };
 
-// out(m, n) = sum_k A[m*am + k*ak] * B[n*bn + k*bk] over one CTA's 64 x 64 tile and its
-// share blockIdx.z of the inner dimension; 4 x 4 outputs per thread, fp32 throughout.
+// out(m, n) = sum_k A[m*am + k*ak] * B[n*bn + k*bk] over one CTA's tile and its share
+// blockIdx.z of the inner dimension, fp32 throughout.
 struct Gemm {
   const void *A, *B;
   int64_t am, ak, bn, bk;
@@ -27,69 +25,117 @@ struct Gemm {
   int add;            // kAccumulate: add to what is there
 };
 
-// Stages kTile rows x kK inner steps, transposed to [k][row].  The thread order follows the
-// dense dimension, so that loads coalesce either way.
-template <typename T>
-__device__ __forceinline__ void stage(float* s, const T* src, int64_t rs, int64_t ks, int64_t r0, int64_t rows,
-                                      int64_t k0, int64_t k_end) {
-  for (int i = threadIdx.x; i < kTile * kK; i += kThreads) {
-    int r, k;
-    if (ks == 1) {
-      k = i % kK;
-      r = i / kK;
+// One thread's share of TILE rows x kK inner steps: fetched into registers while the stage
+// before is multiplied, then put down transposed, [k][row].  Threads follow the dense
+// dimension, so that loads coalesce either way.
+template <typename T, int TILE>
+struct Stage {
+  static constexpr int kPer = TILE * kK / kThreads;
+  float v[kPer];
+  __device__ __forceinline__ static void place(int i, bool k_dense, int& r, int& k) {
+    const int t = threadIdx.x + i * kThreads;
+    if (k_dense) {
+      k = t % kK;
+      r = t / kK;
     } else {
-      r = i % kTile;
-      k = i / kTile;
+      r = t % TILE;
+      k = t / TILE;
     }
-    const bool in = r0 + r < rows && k0 + k < k_end;
-    s[k * kLd + r] = in ? Elem<T>::to_f(src[(r0 + r) * rs + (k0 + k) * ks]) : 0.f;
   }
-}
+  __device__ __forceinline__ void fetch(const T* src, int64_t rs, int64_t ks, int64_t r0, int64_t rows, int64_t k0,
+                                        int64_t k_end) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      int r, k;
+      place(i, ks == 1, r, k);
+      v[i] = r0 + r < rows && k0 + k < k_end ? Elem<T>::to_f(src[(r0 + r) * rs + (k0 + k) * ks]) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void put(float* s, bool k_dense) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      int r, k;
+      place(i, k_dense, r, k);
+      s[k * (TILE + 4) + r] = v[i];
+    }
+  }
+};
 
-template <typename T, int MODE>
-__global__ void __launch_bounds__(kThreads) vl_gemm_kernel(const Gemm g, const Problem p) {
-  __shared__ __align__(16) float as[kK * kLd], bs[kK * kLd];
-  const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
+// R x R outputs per thread in groups of four rows and columns, products in packed pairs.
+// R = 8: 128 x 128 tiles, 4 bytes of shared memory read for each two multiply-adds; R = 4: 64 x 64
+// tiles, for few rows or too few tiles.
+template <typename T, int MODE, int R>
+__global__ void __launch_bounds__(kThreads, 2) vl_gemm_kernel(const Gemm g, const Problem p) {
+  constexpr int TILE = 16 * R, LD = TILE + 4, Q = R / 4;
+  __shared__ __align__(16) float as[2][kK * LD], bs[2][kK * LD];
+  const int64_t m0 = (int64_t)blockIdx.x * TILE, n0 = (int64_t)blockIdx.y * TILE;
   const int64_t k_begin = blockIdx.z * g.k_share, k_end = min(g.K, k_begin + g.k_share);
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  float acc[4][4] = {};
-  for (int64_t k0 = k_begin; k0 < k_end; k0 += kK) {
-    stage((float*)as, (const T*)g.A, g.am, g.ak, m0, g.M, k0, k_end);
-    stage((float*)bs, (const T*)g.B, g.bn, g.bk, n0, g.N, k0, k_end);
-    __syncthreads();
+  const bool ad = g.ak == 1, bd = g.bk == 1;
+  float2 acc2[R][R / 2] = {};
+  Stage<T, TILE> a_next, b_next;
+  if (k_begin < k_end) {
+    a_next.fetch((const T*)g.A, g.am, g.ak, m0, g.M, k_begin, k_end);
+    b_next.fetch((const T*)g.B, g.bn, g.bk, n0, g.N, k_begin, k_end);
+  }
+  int buf = 0;
+  for (int64_t k0 = k_begin; k0 < k_end; k0 += kK, buf ^= 1) {
+    a_next.put(as[buf], ad);
+    b_next.put(bs[buf], bd);
+    __syncthreads();  // (the other buffer's readers passed the barrier before this one)
+    if (k0 + kK < k_end) {
+      a_next.fetch((const T*)g.A, g.am, g.ak, m0, g.M, k0 + kK, k_end);
+      b_next.fetch((const T*)g.B, g.bn, g.bk, n0, g.N, k0 + kK, k_end);
+    }
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
-      const float4 a = *reinterpret_cast<const float4*>(as + k * kLd + ty * 4);
-      const float4 b = *reinterpret_cast<const float4*>(bs + k * kLd + tx * 4);
-      const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+      float4 a[Q], b[Q];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < Q; ++i) {
+        a[i] = *reinterpret_cast<const float4*>(as[buf] + k * LD + i * 64 + ty * 4);
+        b[i] = *reinterpret_cast<const float4*>(bs[buf] + k * LD + i * 64 + tx * 4);
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+      for (int i = 0; i < R; ++i) {
+        const float4 a4 = a[i >> 2];
+        const float av = (i & 3) == 0 ? a4.x : (i & 3) == 1 ? a4.y : (i & 3) == 2 ? a4.z : a4.w;
+        const float2 aa = make_float2(av, av);
+#pragma unroll
+        for (int j = 0; j < Q; ++j) {
+          acc2[i][2 * j] = fma2(aa, make_float2(b[j].x, b[j].y), acc2[i][2 * j]);
+          acc2[i][2 * j + 1] = fma2(aa, make_float2(b[j].z, b[j].w), acc2[i][2 * j + 1]);
+        }
+      }
     }
-    __syncthreads();
   }
+  const float factor = MODE == kStore ? result_factor(p) : 1.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty * 4 + i;
+  for (int i = 0; i < R; ++i) {
+    const int64_t m = m0 + (i >> 2) * 64 + ty * 4 + (i & 3);
     const bool row = m < g.M;
+    float acc[R];
+    int64_t col[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      acc[j] = j & 1 ? acc2[i][j >> 1].y : acc2[i][j >> 1].x;
+      col[j] = n0 + (j >> 2) * 64 + tx * 4 + (j & 3);
+    }
     if constexpr (MODE == kForward) {
       // 16 threads (one half warp) share a row: its maximum, then its sum of exponentials
       const int64_t t = row ? p.target[m] : -1;
       float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t n = n0 + tx * 4 + j;
-        if (n < g.N) mx = fmaxf(mx, acc[i][j]);
-        if (row && n < g.N && n == t) p.tgt[m] = acc[i][j];
+      for (int j = 0; j < R; ++j) {
+        if (col[j] < g.N) mx = fmaxf(mx, acc[j]);
+        if (row && col[j] < g.N && col[j] == t) p.tgt[m] = acc[j];
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       mx *= kLog2e;
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n0 + tx * 4 + j < g.N) sum += exp2f(fmaf(acc[i][j], kLog2e, -mx));
+      for (int j = 0; j < R; ++j)
+        if (col[j] < g.N) sum += exp2f(fmaf(acc[j], kLog2e, -mx));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (row && tx == 0) p.part[(int64_t)blockIdx.y * p.N + m] = make_float2(mx, sum);
@@ -98,37 +144,46 @@ __global__ void __launch_bounds__(kThreads) vl_gemm_kernel(const Gemm g, const P
       const int64_t t = p.target[m];
       const float f = row_factor(p, m, t), lse = p.lse[m];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t n = n0 + tx * 4 + j;
-        if (n >= g.N) continue;
-        const float pr = expf(acc[i][j] - lse) - (g.col0 + n == t ? 1.f : 0.f);
-        ((T*)g.out)[m * g.out_ld + n] = Elem<T>::from_f(f == 0.f ? 0.f : pr * f);
+      for (int j = 0; j < R; ++j) {
+        if (col[j] >= g.N) continue;
+        const float pr = expf(acc[j] - lse) - (g.col0 + col[j] == t ? 1.f : 0.f);
+        ((T*)g.out)[m * g.out_ld + col[j]] = Elem<T>::from_f(f == 0.f ? 0.f : pr * f);
       }
     } else {
       if (!row) continue;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t n = n0 + tx * 4 + j;
-        if (n >= g.N) continue;
+      for (int j = 0; j < R; ++j) {
+        if (col[j] >= g.N) continue;
         if constexpr (MODE == kAccumulate) {
-          float* o = (float*)g.out + ((int64_t)blockIdx.z * g.M + m) * g.out_ld + n;
-          *o = g.add ? *o + acc[i][j] : acc[i][j];
+          float* o = (float*)g.out + ((int64_t)blockIdx.z * g.M + m) * g.out_ld + col[j];
+          *o = g.add ? *o + acc[j] : acc[j];
         } else {
-          ((T*)g.out)[m * g.out_ld + n] = Elem<T>::from_f(acc[i][j] * result_factor(p));
+          ((T*)g.out)[m * g.out_ld + col[j]] = Elem<T>::from_f(acc[j] * factor);
         }
       }
     }
   }
 }
 
+// 128 x 128 tiles where both sides fill them and there are enough for the SMs.
+bool large_tiles(int64_t M, int64_t N, int64_t z) {
+  return M >= 96 && N >= 96 && ((M + 127) / 128) * ((N + 127) / 128) * z >= sm_count() / 2;
+}
+
+template <typename T, int MODE, int R>
+int gemm_tiles(const Gemm& g, const Problem& p, int z, const char* what) {
+  constexpr int TILE = 16 * R;
+  const int64_t gx = (g.M + TILE - 1) / TILE, gy = (g.N + TILE - 1) / TILE;
+  if (gx > INT32_MAX || gy > 65535) return set_error(DYNCONV_ERR_SHAPE, "%s: too many tiles", what);
+  vl_gemm_kernel<T, MODE, R><<<dim3((unsigned)gx, (unsigned)gy, (unsigned)z), kThreads, 0, p.st>>>(g, p);
+  DYNCONV_CHECK_LAUNCH(what);
+  return DYNCONV_OK;
+}
+
 template <typename T, int MODE>
 int gemm(Gemm g, const Problem& p, int z, const char* what) {
   g.k_share = ((g.K + z - 1) / z + kK - 1) / kK * kK;
-  const int64_t gx = (g.M + kTile - 1) / kTile, gy = (g.N + kTile - 1) / kTile;
-  if (gx > INT32_MAX || gy > 65535) return set_error(DYNCONV_ERR_SHAPE, "%s: too many tiles", what);
-  vl_gemm_kernel<T, MODE><<<dim3((unsigned)gx, (unsigned)gy, (unsigned)z), kThreads, 0, p.st>>>(g, p);
-  DYNCONV_CHECK_LAUNCH(what);
-  return DYNCONV_OK;
+  return large_tiles(g.M, g.N, z) ? gemm_tiles<T, MODE, 8>(g, p, z, what) : gemm_tiles<T, MODE, 4>(g, p, z, what);
 }
 
 // Merges the tiles' (maximum, sum) of 32 rows per CTA: lane = row, warps take every eighth
@@ -209,7 +264,8 @@ int fwd(const Problem& p) {
   g.B = p.weight, g.bn = p.D, g.bk = 1;
   g.M = p.N, g.N = p.V, g.K = p.D;
   int s = gemm<T, kForward>(g, p, 1, "vl_gemm_kernel (forward)");
-  return s ? s : merge_launch(p, (p.V + kTile - 1) / kTile);
+  const int64_t tile = large_tiles(p.N, p.V, 1) ? 128 : 64;
+  return s ? s : merge_launch(p, (p.V + tile - 1) / tile);
 }
 
 template <typename T>
@@ -301,22 +357,21 @@ int merge_launch(const Problem& p, int64_t tiles) {
   return DYNCONV_OK;
 }
 
-int tile_cols(bool tc) { return tc ? 128 : kTile; }
-
 // The piece's width is the one with the lowest estimated time among those whose buffer stays
 // within 512 MB: each product runs in rounds of one tile per SM or SM pair (weight-gradient tiles
 // are few and long: at 16384 x 2048 a width of 7168 columns makes 224 of them, three rounds of 74
 // and two tiles), each piece costs three launches and one pass over the fp32 sums of dhidden.  Times are
 // counted in blocks of 64 inner elements of a tile, 0.46 us each on the tensor cores.
 // Where a product has few tiles its inner dimension is spread over several CTAs, each share at
-// least 512 elements.
+// least 512 elements (128 on the CUDA cores, where they take as long).
 Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc) {
   const int64_t elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4, sms = tc ? sm_count() / 2 : sm_count();
-  const int64_t tm = tc ? 256 : kTile, tn = tc ? 256 : kTile;
+  const int64_t tm = tc ? 256 : 128, tn = tc ? 256 : 128;
   const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const int64_t least = tc ? 512 : 128;
   const auto share = [&](int64_t tiles, int64_t inner) {
     int64_t z = 2 * sms / tiles;
-    if (z > inner / 512) z = inner / 512;
+    if (z > inner / least) z = inner / least;
     if (z > 16) z = 16;
     return (int)(z < 1 ? 1 : z);
   };

@@ -69,7 +69,7 @@ __device__ __forceinline__ float result_factor(const Problem& p) {
   return p.stats[1] > 0.f ? p.dloss[0] / p.stats[1] : 0.f;
 }
 
-int tile_cols(bool tc);  // columns of the vocabulary in one forward tile
+constexpr int kNarrowestTile = 64;  // columns of the vocabulary in one forward tile, at least
 bool tc_supported(const Problem& p, int dtype);
 Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc);
 int merge_launch(const Problem& p, int64_t tiles);
