@@ -31,33 +31,36 @@ struct Gemm {
 template <typename T, int TILE>
 struct Stage {
   static constexpr int kPer = TILE * kK / kThreads;
+  const T* at;        // this thread's first element of the current step
+  int64_t next, step; // to its next element, to the next step's
+  uint32_t rows;      // which of its elements lie in rows that are there
+  int k, dk, to, dto; // its first inner index and place in shared memory, and how they go on
   float v[kPer];
-  __device__ __forceinline__ static void place(int i, bool k_dense, int& r, int& k) {
-    const int t = threadIdx.x + i * kThreads;
-    if (k_dense) {
-      k = t % kK;
-      r = t / kK;
-    } else {
-      r = t % TILE;
-      k = t / TILE;
-    }
-  }
-  __device__ __forceinline__ void fetch(const T* src, int64_t rs, int64_t ks, int64_t r0, int64_t rows, int64_t k0,
-                                        int64_t k_end) {
+  __device__ __forceinline__ Stage(const T* src, int64_t rs, int64_t ks, int64_t r0, int64_t n_rows, int64_t k0) {
+    const int t = threadIdx.x;
+    const bool k_dense = ks == 1;
+    const int r = k_dense ? t / kK : t % TILE, dr = k_dense ? kThreads / kK : 0;
+    k = k_dense ? t % kK : t / TILE;
+    dk = k_dense ? 0 : kThreads / TILE;
+    to = k * (TILE + 4) + r;
+    dto = dk * (TILE + 4) + dr;
+    at = src + (r0 + r) * rs + (k0 + k) * ks;
+    next = dr * rs + dk * ks;
+    step = kK * ks;
+    rows = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      int r, k;
-      place(i, ks == 1, r, k);
-      v[i] = r0 + r < rows && k0 + k < k_end ? Elem<T>::to_f(src[(r0 + r) * rs + (k0 + k) * ks]) : 0.f;
-    }
+    for (int i = 0; i < kPer; ++i) rows |= (uint32_t)(r0 + r + i * dr < n_rows) << i;
   }
-  __device__ __forceinline__ void put(float* s, bool k_dense) const {
+  __device__ __forceinline__ void fetch(int k_left) {  // k_left: inner elements from this step on
+    const T* q = at;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      int r, k;
-      place(i, k_dense, r, k);
-      s[k * (TILE + 4) + r] = v[i];
-    }
+    for (int i = 0; i < kPer; ++i, q += next)
+      v[i] = (rows >> i & 1) && k + i * dk < k_left ? Elem<T>::to_f(*q) : 0.f;
+    at += step;
+  }
+  __device__ __forceinline__ void put(float* s) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s[to + i * dto] = v[i];
   }
 };
 
@@ -71,22 +74,17 @@ __global__ void __launch_bounds__(kThreads, 2) vl_gemm_kernel(const Gemm g, cons
   const int64_t m0 = (int64_t)blockIdx.x * TILE, n0 = (int64_t)blockIdx.y * TILE;
   const int64_t k_begin = blockIdx.z * g.k_share, k_end = min(g.K, k_begin + g.k_share);
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  const bool ad = g.ak == 1, bd = g.bk == 1;
   float2 acc2[R][R / 2] = {};
-  Stage<T, TILE> a_next, b_next;
-  if (k_begin < k_end) {
-    a_next.fetch((const T*)g.A, g.am, g.ak, m0, g.M, k_begin, k_end);
-    b_next.fetch((const T*)g.B, g.bn, g.bk, n0, g.N, k_begin, k_end);
-  }
-  int buf = 0;
-  for (int64_t k0 = k_begin; k0 < k_end; k0 += kK, buf ^= 1) {
-    a_next.put(as[buf], ad);
-    b_next.put(bs[buf], bd);
+  Stage<T, TILE> a_next((const T*)g.A, g.am, g.ak, m0, g.M, k_begin), b_next((const T*)g.B, g.bn, g.bk, n0, g.N, k_begin);
+  int left = (int)(k_end - k_begin), buf = 0;  // (a share beyond the end has none)
+  a_next.fetch(left);
+  b_next.fetch(left);
+  for (; left > 0; left -= kK, buf ^= 1) {
+    a_next.put(as[buf]);
+    b_next.put(bs[buf]);
     __syncthreads();  // (the other buffer's readers passed the barrier before this one)
-    if (k0 + kK < k_end) {
-      a_next.fetch((const T*)g.A, g.am, g.ak, m0, g.M, k0 + kK, k_end);
-      b_next.fetch((const T*)g.B, g.bn, g.bk, n0, g.N, k0 + kK, k_end);
-    }
+    a_next.fetch(left - kK);
+    b_next.fetch(left - kK);
 #pragma unroll
     for (int k = 0; k < kK; ++k) {
       float4 a[Q], b[Q];
