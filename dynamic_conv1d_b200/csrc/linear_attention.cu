@@ -9,23 +9,37 @@ namespace la {
 
 namespace {
 
-// ------------------------------------------------------------------ chunked, simple
+// ------------------------------------------------------------------ chunked, CUDA cores
 
 constexpr int kC = 32;        // tokens of a chunk
 constexpr int kSlice = 32;    // columns of w per CTA
 constexpr int kThreads = 256;
+constexpr int kLd = kC + 4;   // pitch of the chunk x chunk and slice x chunk tiles
+
+__host__ __device__ constexpr int row_pitch(int dx) { return (dx + 3) / 4 * 4 + 4; }  // of x, y and the state
 
 __host__ __device__ constexpr size_t simple_smem_floats(int dx) {
-  return (size_t)2 * kC * (dx + 1) + 2 * kC * (kC + 1) + (size_t)dx * (kSlice + 1) + kC + 1;
+  return (size_t)(2 * kC + kSlice) * row_pitch(dx) + 3 * kC * kLd + kC + 4;
+}
+
+__device__ __forceinline__ float4 f4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+
+__device__ __forceinline__ void dot4(float& acc, const float4& a, const float4& b) {
+  acc = fmaf(a.x, b.x, acc);
+  acc = fmaf(a.y, b.y, acc);
+  acc = fmaf(a.z, b.z, acc);
+  acc = fmaf(a.w, b.w, acc);
 }
 
 // One CTA runs one segment of one chain, chunk after chunk, with the state in shared
 // memory.  state_only: the segment's own state from zero, into p.seg.
-// Everything is fp32; each output is rounded once.
+// Everything is fp32; each output is rounded once.  Every product runs along a dense dimension of
+// both operands (w and the state are kept transposed), four elements per shared-memory read, and
+// a thread owns 2 x 2 scores and outputs or 2 x 4 elements of the state.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) la_simple_kernel(const __grid_constant__ Params p, int n_slices,
                                                              int state_only) {
-  extern __shared__ float sm[];
+  extern __shared__ __align__(16) float sm[];
   int64_t id = blockIdx.x;
   const int slice = (int)(id % n_slices);
   id /= n_slices;
@@ -39,95 +53,106 @@ __global__ void __launch_bounds__(kThreads) la_simple_kernel(const __grid_consta
   if (c0 >= dw || (state_only && seg == p.n_seg - 1)) return;
   const int nc = min(kSlice, dw - c0);
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ld = row_pitch(dx), d4 = (ld - 4) / 4;
 
-  float* xs = sm;                    // [kC][dx+1]
-  float* ys = xs + kC * (dx + 1);    // [kC][dx+1]
-  float* ws = ys + kC * (dx + 1);    // [kC][kC+1]
-  float* as = ws + kC * (kC + 1);    // [kC][kC+1]
-  float* S = as + kC * (kC + 1);     // [dx][kSlice+1]
-  float* pw = S + dx * (kSlice + 1); // decay^0 .. decay^kC
+  float* xs = sm;                // [kC][ld]
+  float* ys = xs + kC * ld;      // [kC][ld]
+  float* St = ys + kC * ld;      // [kSlice][ld]: the state, transposed
+  float* wt = St + kSlice * ld;  // [kSlice][kLd]: w, transposed
+  float* ht = wt + kC * kLd;     // [kSlice][kLd]: w weighted by the decays to the chunk's end
+  float* as = ht + kC * kLd;     // [kC][kLd]: scores under the decay mask
+  float* pw = as + kC * kLd;     // decay^0 .. decay^kC
 
   const double l2 = log2_decay(p.log_decay, h);
   if (tid <= kC) pw[tid] = (float)exp2(l2 * tid);
   const Factor f_full = decay_factor(l2, kC);
   const int64_t n_state = (int64_t)dx * dw;
-  for (int i = tid; i < dx * kSlice; i += kThreads) {
-    const int r = i / kSlice, c = i % kSlice;
+  for (int r = warp; r < ld; r += kThreads / 32) {  // (columns beyond dx stay zero, here and in x and y)
     float v = 0.f;
-    if (c < nc && !state_only) {
+    if (r < dx && lane < nc && !state_only) {
       if (p.n_seg > 1)
-        v = seg_state(p, ri, seg, bh, n_state)[(int64_t)r * dw + c0 + c];
+        v = seg_state(p, ri, seg, bh, n_state)[(int64_t)r * dw + c0 + lane];
       else if (ro.s_in)
-        v = ro.s_in[bh * n_state + (int64_t)r * ro.si + (int64_t)(c0 + c) * ro.sj];
+        v = ro.s_in[bh * n_state + (int64_t)r * ro.si + (int64_t)(c0 + lane) * ro.sj];
     }
-    S[r * (kSlice + 1) + c] = v;
+    St[lane * ld + r] = v;
+  }
+  for (int i = tid; i < 2 * kC * 4; i += kThreads) {  // (x and y are adjacent)
+    const int r = i >> 2, c = (dx & ~3) + (i & 3);
+    if (c < ld) xs[r * ld + c] = 0.f;
   }
 
   const T* xp = (const T*)ro.x.p + b * ro.x.sb + h * ro.x.sh;
   const T* yp = (const T*)ro.y.p + b * ro.y.sb + h * ro.y.sh;
-  const T* wp = (const T*)ro.w.p + b * ro.w.sb + h * ro.w.sh;
-  T* op = (T*)ro.out.p + b * ro.out.sb + h * ro.out.sh;
+  const T* wp = (const T*)ro.w.p + b * ro.w.sb + h * ro.w.sh + c0;
+  T* op = (T*)ro.out.p + b * ro.out.sb + h * ro.out.sh + c0;
   const int64_t n_chunks = (p.T + kC - 1) / kC;
   const int64_t first = (int64_t)seg * p.chunks_per_seg;
   const int64_t last = min(n_chunks, first + p.chunks_per_seg);
   const int e = ro.reverse ? 0 : 1;
+  const int ty = tid >> 4, tx = tid & 15;
   for (int64_t ch = first; ch < last; ++ch) {
     const int64_t a0 = ch * kC;  // scan position of the chunk's first token
     const int L = (int)min((int64_t)kC, p.T - a0);
     __syncthreads();
-    for (int i = tid; i < kC * dx; i += kThreads) {
-      const int r = i / dx, d = i - r * dx;
+#pragma unroll
+    for (int i = 0; i < kC / 8; ++i) {
+      const int r = warp + i * 8;
       const int64_t t = ro.reverse ? p.T - 1 - (a0 + r) : a0 + r;
-      xs[r * (dx + 1) + d] = (r < L && !state_only) ? Elem<T>::to_f(xp[t * ro.x.st + d]) : 0.f;
-      ys[r * (dx + 1) + d] = r < L ? Elem<T>::to_f(yp[t * ro.y.st + d]) : 0.f;
-    }
-    for (int i = tid; i < kC * kSlice; i += kThreads) {
-      const int r = i / kSlice, c = i % kSlice;
-      const int64_t t = ro.reverse ? p.T - 1 - (a0 + r) : a0 + r;
-      ws[r * (kC + 1) + c] = (r < L && c < nc) ? Elem<T>::to_f(wp[t * ro.w.st + c0 + c]) : 0.f;
+      for (int d = lane; d < dx; d += 32) {
+        if (!state_only) xs[r * ld + d] = r < L ? Elem<T>::to_f(xp[t * ro.x.st + d]) : 0.f;
+        ys[r * ld + d] = r < L ? Elem<T>::to_f(yp[t * ro.y.st + d]) : 0.f;
+      }
+      const float w = (r < L && lane < nc) ? Elem<T>::to_f(wp[t * ro.w.st + lane]) : 0.f;
+      wt[lane * kLd + r] = w;
+      ht[lane * kLd + r] = r < L ? w * pw[L - e - r] : 0.f;
     }
     __syncthreads();
     if (!state_only) {
-      // scores: thread (ty, tx) owns rows ty, ty+16 and columns tx, tx+16
-      const int ty = tid >> 4, tx = tid & 15;
-      float acc[2][2] = {};
-      for (int d = 0; d < dx; ++d) {
-        const float x0 = xs[ty * (dx + 1) + d], x1 = xs[(ty + 16) * (dx + 1) + d];
-        const float y0 = ys[tx * (dx + 1) + d], y1 = ys[(tx + 16) * (dx + 1) + d];
-        acc[0][0] = fmaf(x0, y0, acc[0][0]);
-        acc[0][1] = fmaf(x0, y1, acc[0][1]);
-        acc[1][0] = fmaf(x1, y0, acc[1][0]);
-        acc[1][1] = fmaf(x1, y1, acc[1][1]);
+      // scores, and the product with the state: thread (ty, tx) owns rows ty, ty+16, columns tx, tx+16
+      float sc[2][2] = {}, o2[2][2] = {};
+#pragma unroll 2
+      for (int d = 0; d < d4; ++d) {
+        const float4 x0 = f4(xs + ty * ld + 4 * d), x1 = f4(xs + (ty + 16) * ld + 4 * d);
+        const float4 y0 = f4(ys + tx * ld + 4 * d), y1 = f4(ys + (tx + 16) * ld + 4 * d);
+        const float4 s0 = f4(St + tx * ld + 4 * d), s1 = f4(St + (tx + 16) * ld + 4 * d);
+        dot4(sc[0][0], x0, y0);
+        dot4(sc[0][1], x0, y1);
+        dot4(sc[1][0], x1, y0);
+        dot4(sc[1][1], x1, y1);
+        dot4(o2[0][0], x0, s0);
+        dot4(o2[0][1], x0, s1);
+        dot4(o2[1][0], x1, s0);
+        dot4(o2[1][1], x1, s1);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int r = ty + 16 * i, c = tx + 16 * j;
-          as[r * (kC + 1) + c] = c <= r ? acc[i][j] * pw[r - c] * ro.a_scale : 0.f;
+          as[r * kLd + c] = c <= r ? sc[i][j] * pw[r - c] * ro.a_scale : 0.f;
         }
       __syncthreads();
-      float o1[2][2] = {}, o2[2][2] = {};
-      for (int j = 0; j < kC; ++j) {
-        const float a_0 = as[ty * (kC + 1) + j], a_1 = as[(ty + 16) * (kC + 1) + j];
-        const float w_0 = ws[j * (kC + 1) + tx], w_1 = ws[j * (kC + 1) + tx + 16];
-        if (j <= ty) {  // a later token's w may be inf or NaN: not even times zero
-          o1[0][0] = fmaf(a_0, w_0, o1[0][0]);
-          o1[0][1] = fmaf(a_0, w_1, o1[0][1]);
+      float o1[2][2] = {};
+      for (int j = 0; j < kC; j += 4) {
+        if (j > ty + 16) break;
+        float4 w[2] = {f4(wt + tx * kLd + j), f4(wt + (tx + 16) * kLd + j)};
+#pragma unroll
+        for (int i = 1; i >= 0; --i) {
+          const int r = ty + 16 * i;
+          // a later token's w may be inf or NaN: not even times zero (row ty+16 first: it sees more)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (j + 0 > r) w[c].x = 0.f;
+            if (j + 1 > r) w[c].y = 0.f;
+            if (j + 2 > r) w[c].z = 0.f;
+            if (j + 3 > r) w[c].w = 0.f;
+          }
+          const float4 a = f4(as + r * kLd + j);
+          dot4(o1[i][0], a, w[0]);
+          dot4(o1[i][1], a, w[1]);
         }
-        if (j <= ty + 16) {
-          o1[1][0] = fmaf(a_1, w_0, o1[1][0]);
-          o1[1][1] = fmaf(a_1, w_1, o1[1][1]);
-        }
-      }
-      for (int d = 0; d < dx; ++d) {
-        const float x0 = xs[ty * (dx + 1) + d], x1 = xs[(ty + 16) * (dx + 1) + d];
-        const float s0 = S[d * (kSlice + 1) + tx], s1 = S[d * (kSlice + 1) + tx + 16];
-        o2[0][0] = fmaf(x0, s0, o2[0][0]);
-        o2[0][1] = fmaf(x0, s1, o2[0][1]);
-        o2[1][0] = fmaf(x1, s0, o2[1][0]);
-        o2[1][1] = fmaf(x1, s1, o2[1][1]);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -138,31 +163,52 @@ __global__ void __launch_bounds__(kThreads) la_simple_kernel(const __grid_consta
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int c = tx + 16 * j;
-          if (c < nc) op[t * ro.out.st + c0 + c] = Elem<T>::from_f(fmaf(f, o2[i][j], o1[i][j]));
+          if (c < nc) op[t * ro.out.st + c] = Elem<T>::from_f(fmaf(f, o2[i][j], o1[i][j]));
         }
       }
-      __syncthreads();  // the state's readers are done
+      // (the state's readers were done before the barrier above)
     }
-    const int c = tid & 31;
     const Factor f = L == kC ? f_full : decay_factor(l2, L);
-    for (int r = tid >> 5; r < dx; r += kThreads / 32) {
-      float acc = 0.f;
-      for (int j = 0; j < L; ++j)
-        acc = fmaf(ys[j * (dx + 1) + r], ws[j * (kC + 1) + c] * pw[L - e - j], acc);
-      S[r * (kSlice + 1) + c] = decay_add(f, S[r * (kSlice + 1) + c], ro.w_scale * acc);
+    for (int i = tid; i < d4 * 16; i += kThreads) {
+      const int c = i & 15, d = (i >> 4) * 4;
+      float4 acc[2] = {};
+#pragma unroll 2
+      for (int j = 0; j < kC; j += 4) {
+        const float4 h0 = f4(ht + c * kLd + j), h1 = f4(ht + (c + 16) * kLd + j);
+        const float hv[2][4] = {{h0.x, h0.y, h0.z, h0.w}, {h1.x, h1.y, h1.z, h1.w}};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 y = f4(ys + (j + k) * ld + d);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            acc[m].x = fmaf(hv[m][k], y.x, acc[m].x);
+            acc[m].y = fmaf(hv[m][k], y.y, acc[m].y);
+            acc[m].z = fmaf(hv[m][k], y.z, acc[m].z);
+            acc[m].w = fmaf(hv[m][k], y.w, acc[m].w);
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float* S = St + (c + 16 * m) * ld + d;
+        float4 v = f4(S);
+        v.x = decay_add(f, v.x, ro.w_scale * acc[m].x);
+        v.y = decay_add(f, v.y, ro.w_scale * acc[m].y);
+        v.z = decay_add(f, v.z, ro.w_scale * acc[m].z);
+        v.w = decay_add(f, v.w, ro.w_scale * acc[m].w);
+        *reinterpret_cast<float4*>(S) = v;
+      }
     }
   }
   __syncthreads();
   const bool to_user = !state_only && seg == p.n_seg - 1 && ro.s_out;
-  if (!state_only && !to_user) return;
-  for (int i = tid; i < dx * kSlice; i += kThreads) {
-    const int r = i / kSlice, c = i % kSlice;
-    if (c >= nc) continue;
-    const float v = S[r * (kSlice + 1) + c];
+  if ((!state_only && !to_user) || lane >= nc) return;
+  for (int r = warp; r < dx; r += kThreads / 32) {
+    const float v = St[lane * ld + r];
     if (state_only)
-      seg_state(p, ri, seg, bh, n_state)[(int64_t)r * dw + c0 + c] = v;
+      seg_state(p, ri, seg, bh, n_state)[(int64_t)r * dw + c0 + lane] = v;
     else
-      ro.s_out[bh * n_state + (int64_t)r * ro.si + (int64_t)(c0 + c) * ro.sj] = v;
+      ro.s_out[bh * n_state + (int64_t)r * ro.si + (int64_t)(c0 + lane) * ro.sj] = v;
   }
 }
 
@@ -316,17 +362,25 @@ int scan_launch(const Params& p, int chunk, cudaStream_t st) {
   return DYNCONV_OK;
 }
 
-// Cuts chains until there are about four CTAs for each SM, with eight chunks at least in a segment.
-void simple_plan(Params* p) {
-  const int64_t chunks = (p->T + kC - 1) / kC;
+void plan_segments(Params* p, int chunk, int slice, int slots, double state_pass, double start, double scan) {
+  const int64_t chunks = (p->T + chunk - 1) / chunk;
   int64_t chains = 0;
-  for (int r = 0; r < p->n_roles; ++r) chains += (int64_t)p->B * p->H * ((p->role[r].dw + kSlice - 1) / kSlice);
-  int64_t seg = (4 * (int64_t)sm_count() + chains - 1) / chains;
-  seg = seg < chunks / 8 ? seg : chunks / 8;
-  if (seg < 1) seg = 1;
-  p->chunks_per_seg = (int)((chunks + seg - 1) / seg);
-  p->n_seg = (int)((chunks + p->chunks_per_seg - 1) / p->chunks_per_seg);
+  for (int r = 0; r < p->n_roles; ++r) chains += (int64_t)p->B * p->H * ((p->role[r].dw + slice - 1) / slice);
+  double best = 1e300;
+  p->n_seg = 1, p->chunks_per_seg = (int)chunks;
+  for (int64_t want = 1; want <= 64 && want <= chunks; ++want) {
+    const int64_t per = (chunks + want - 1) / want, seg = (chunks + per - 1) / per;
+    double cost = (double)((chains * seg + slots - 1) / slots) * ((double)per + start);
+    if (seg > 1) cost += (double)((chains * (seg - 1) + slots - 1) / slots) * ((double)per * state_pass + start) + scan;
+    if (cost < best) {
+      best = cost;
+      p->n_seg = (int)seg, p->chunks_per_seg = (int)per;
+    }
+  }
 }
+
+// Measured at 64 x 64: a chunk 4 us, of the state pass 2.5 us, 4 us to start, 4 us for the scan; four CTAs per SM.
+void simple_plan(Params* p) { plan_segments(p, kC, kSlice, 4 * sm_count(), 0.6, 1.0, 1.0); }
 
 namespace {
 template <typename T>

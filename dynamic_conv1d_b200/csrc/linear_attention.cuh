@@ -82,6 +82,11 @@ __device__ __forceinline__ float* seg_state(const Params& p, int role, int seg, 
   return p.seg + ((int64_t)(role * p.n_seg + seg) * p.B * p.H + bh) * n;
 }
 
+// Cuts chains into the number of segments with the lowest estimated time, counted in chunks of one
+// CTA: both passes run in rounds of `slots` CTAs; the state pass costs `state_pass` of a chunk's
+// time per chunk, a round's start `start` and the scan `scan` chunks.
+void plan_segments(Params* p, int chunk, int slice, int slots, double state_pass, double start, double scan);
+
 // Launches the scan over segment states (role.s_in -> p.seg in place; chunk = tokens per chunk).
 int scan_launch(const Params& p, int chunk, cudaStream_t st);
 // CUDA-core kernels: any type, strides and widths up to kMaxDim.

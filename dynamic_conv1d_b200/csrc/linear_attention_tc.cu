@@ -594,27 +594,8 @@ bool tc_supported(const Params& p, int dtype) {
   return true;
 }
 
-// Cuts chains into the number of segments with the lowest estimated time, counted in chunks of
-// one CTA: both passes run in rounds of one CTA per SM, the state pass costs kStatePass of a
-// chunk's time per chunk, and a round's start kStart chunks (measured at 128 x 128: a chunk 2.2
-// us, of the state pass 1.0 us, about 5 us to start).
-void tc_plan(Params* p) {
-  constexpr double kStatePass = 0.45, kStart = 2.0;
-  const int64_t chunks = (p->T + kC - 1) / kC, sms = sm_count();
-  int64_t chains = 0;
-  for (int r = 0; r < p->n_roles; ++r) chains += (int64_t)p->B * p->H * ((p->role[r].dw + kSlice - 1) / kSlice);
-  double best = 1e300;
-  p->n_seg = 1, p->chunks_per_seg = (int)chunks;
-  for (int64_t want = 1; want <= 64 && want <= chunks; ++want) {
-    const int64_t per = (chunks + want - 1) / want, seg = (chunks + per - 1) / per;
-    double cost = (double)((chains * seg + sms - 1) / sms) * ((double)per + kStart);
-    if (seg > 1) cost += (double)((chains * (seg - 1) + sms - 1) / sms) * ((double)per * kStatePass + kStart) + kStart;
-    if (cost < best) {
-      best = cost;
-      p->n_seg = (int)seg, p->chunks_per_seg = (int)per;
-    }
-  }
-}
+// Measured at 128 x 128: a chunk 2.2 us, of the state pass 1 us, 5 us to start, 7 us for the scan; one CTA per SM.
+void tc_plan(Params* p) { plan_segments(p, kC, kSlice, sm_count(), 0.45, 2.5, 3.0); }
 
 int tc_launch(const Params& p, cudaStream_t st) {
   TcMaps maps;

@@ -32,58 +32,55 @@ def _strides(*tensors):
     return _Strides[len(s)](*s)
 
 
-def _workspace(lib, q, dv, backward):
-    B, T, H, dk = q.shape
-    n = lib.dynconv_la_workspace_bytes(B, T, H, dk, dv, _lib.dtype_code(q.dtype), backward)
-    return torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
-def _fwd(q, k, v, log_decay, s0, o, s1, scale):
+def _workspace(lib, like, sizes, code, backward):
+    n = lib.dynconv_la_workspace_bytes(*sizes, code, backward)
+    return (torch.empty(n, device=like.device, dtype=torch.uint8), n) if n else (None, 0)
+
+
+def _fwd(like, addresses, strides, sizes, log_decay, s0, o, s1, scale):
+    """addresses of q, k, v, o; strides of their batch, time and head; sizes B, T, H, dk, dv."""
     lib = _lib.load()
-    B, T, H, dk = q.shape
-    dv = v.shape[-1]
-    ws = _workspace(lib, q, dv, 0)
-    _lib.check(
-        lib.dynconv_la_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), None if s0 is None else s0.data_ptr(),
-            o.data_ptr(), None if s1 is None else s1.data_ptr(), _strides(q, k, v, o),
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
-            B, T, H, dk, dv, scale, _lib.dtype_code(q.dtype), _lib.raw_stream(q),
-        )
-    )
+    code = _lib.dtype_code(like.dtype)
+    ws, n = _workspace(lib, like, sizes, code, 0)
+    q, k, v = addresses
+    status = lib.dynconv_la_fwd(q, k, v, log_decay.data_ptr(), _ptr(s0), o.data_ptr(), _ptr(s1), strides, _ptr(ws), n,
+                                *sizes, scale, code, _lib.raw_stream(like))
+    if status:
+        _lib.check(status)
     _lib.after_call(o)
 
 
-def _bwd(q, k, v, log_decay, s0, do, ds1, dq, dk_, dv_, ds0, scale):
+def _bwd(like, addresses, strides, sizes, log_decay, s0, ds1, ds0, scale):
+    """addresses of q, k, v, do, dq, dk, dv; strides likewise."""
     lib = _lib.load()
-    B, T, H, dk = q.shape
-    dv = v.shape[-1]
+    code = _lib.dtype_code(like.dtype)
     if ds1 is not None:
         ds1 = ds1.to(torch.float32).contiguous()
-    with _lib.device_of(q):
-        ws = _workspace(lib, q, dv, 1)
-        _lib.check(
-            lib.dynconv_la_bwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), None if s0 is None else s0.data_ptr(),
-                do.data_ptr(), None if ds1 is None else ds1.data_ptr(), dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(),
-                None if ds0 is None else ds0.data_ptr(), _strides(q, k, v, do, dq, dk_, dv_),
-                None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
-                B, T, H, dk, dv, scale, _lib.dtype_code(q.dtype), _lib.raw_stream(q),
-            )
-        )
-        _lib.after_call(dq)
+    q, k, v, do, dq, dk_, dv_ = addresses
+    with _lib.device_of(like):
+        ws, n = _workspace(lib, like, sizes, code, 1)
+        status = lib.dynconv_la_bwd(q, k, v, log_decay.data_ptr(), _ptr(s0), do, _ptr(ds1), dq, dk_, dv_, _ptr(ds0),
+                                    strides, _ptr(ws), n, *sizes, scale, code, _lib.raw_stream(like))
+        if status:
+            _lib.check(status)
+        _lib.after_call(like)
 
 
 class _DecayLinearAttentionFn(torch.autograd.Function):
     @staticmethod
-    @_lib.on_device
     def forward(ctx, q, k, v, log_decay, initial_state, scale, want_state):
         q, k, v = _dense(q), _dense(k), _dense(v)
         B, T, H, dk = q.shape
         dv = v.shape[-1]
-        o = torch.empty((B, T, H, dv), device=q.device, dtype=q.dtype)
-        s1 = torch.empty((B, H, dk, dv), device=q.device, dtype=torch.float32) if want_state else None
-        _fwd(q, k, v, log_decay, initial_state, o, s1, scale)
+        with _lib.device_of(q):
+            o = torch.empty((B, T, H, dv), device=q.device, dtype=q.dtype)
+            s1 = torch.empty((B, H, dk, dv), device=q.device, dtype=torch.float32) if want_state else None
+            _fwd(q, (q.data_ptr(), k.data_ptr(), v.data_ptr()), _strides(q, k, v, o), (B, T, H, dk, dv), log_decay,
+                 initial_state, o, s1, scale)
         ctx.save_for_backward(q, k, v, log_decay, initial_state)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
@@ -92,10 +89,13 @@ class _DecayLinearAttentionFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do, ds1):
         q, k, v, log_decay, s0 = ctx.saved_tensors
+        B, T, H, dk = q.shape
         do = torch.zeros(v.shape, device=v.device, dtype=v.dtype) if do is None else _dense(do.to(v.dtype))
         dq, dk_, dv_ = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
         ds0 = torch.empty_like(s0) if s0 is not None and ctx.needs_input_grad[4] else None
-        _bwd(q, k, v, log_decay, s0, do, ds1, dq, dk_, dv_, ds0, ctx.scale)
+        tensors = (q, k, v, do, dq, dk_, dv_)
+        _bwd(q, [t.data_ptr() for t in tensors], _strides(*tensors), (B, T, H, dk, v.shape[-1]), log_decay, s0, ds1, ds0,
+             ctx.scale)
         return dq, dk_, dv_, None, ds0, None, None
 
 
@@ -103,15 +103,18 @@ class _FusedDecayLinearAttentionFn(torch.autograd.Function):
     """On the thirds of one [B, T, 3*H*d] buffer, its gradient written as one buffer too."""
 
     @staticmethod
-    @_lib.on_device
     def forward(ctx, qkv, log_decay, initial_state, scale, want_state):
         B, T, C = qkv.shape
         H = log_decay.shape[0]
         d = C // (3 * H)
-        q, k, v = qkv.view(B, T, 3, H, d).unbind(2)
-        o = torch.empty((B, T, H * d), device=qkv.device, dtype=qkv.dtype)
-        s1 = torch.empty((B, H, d, d), device=qkv.device, dtype=torch.float32) if want_state else None
-        _fwd(q, k, v, log_decay, initial_state, o.view(B, T, H, d), s1, scale)
+        third = (T * C, C, d)  # strides of q, k and v in the buffer
+        own = (T * H * d, H * d, d)
+        at, step = qkv.data_ptr(), H * d * qkv.element_size()
+        with _lib.device_of(qkv):
+            o = torch.empty((B, T, H * d), device=qkv.device, dtype=qkv.dtype)
+            s1 = torch.empty((B, H, d, d), device=qkv.device, dtype=torch.float32) if want_state else None
+            _fwd(qkv, (at, at + step, at + 2 * step), _Strides[12](*third, *third, *third, *own), (B, T, H, d, d),
+                 log_decay, initial_state, o, s1, scale)
         ctx.save_for_backward(qkv, log_decay, initial_state)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
@@ -123,13 +126,15 @@ class _FusedDecayLinearAttentionFn(torch.autograd.Function):
         B, T, C = qkv.shape
         H = log_decay.shape[0]
         d = C // (3 * H)
-        shape = (B, T, 3, H, d)
         if do is None:
             do = torch.zeros((B, T, H * d), device=qkv.device, dtype=qkv.dtype)
-        do = do.to(qkv.dtype).contiguous().view(B, T, H, d)
+        do = do.to(qkv.dtype).contiguous()
         dqkv = torch.empty_like(qkv)
         ds0 = torch.empty_like(s0) if s0 is not None and ctx.needs_input_grad[2] else None
-        _bwd(*qkv.view(shape).unbind(2), log_decay, s0, do, ds1, *dqkv.view(shape).unbind(2), ds0,
+        third, own = (T * C, C, d), (T * H * d, H * d, d)
+        at, to, step = qkv.data_ptr(), dqkv.data_ptr(), H * d * qkv.element_size()
+        _bwd(qkv, (at, at + step, at + 2 * step, do.data_ptr(), to, to + step, to + 2 * step),
+             _Strides[21](*third, *third, *third, *own, *third, *third, *third), (B, T, H, d, d), log_decay, s0, ds1, ds0,
              ctx.scale)
         return dqkv, None, ds0, None, None
 
@@ -141,9 +146,12 @@ def _check_decay(log_decay, H):
 
 
 def _check_state(state, rows, H, dk, dv):
-    assert state.is_cuda and state.is_contiguous() and state.dtype == torch.float32
-    assert state.dim() == 4 and state.shape[1:] == (H, dk, dv)
-    assert rows is None or state.shape[0] == rows
+    """Rows of a state."""
+    assert state.is_cuda and state.is_contiguous() and state.dtype == torch.float32 and state.dim() == 4
+    n, h, a, b = state.shape
+    assert h == H and a == dk and b == dv, f"state must be [n, {H}, {dk}, {dv}]"
+    assert rows is None or n == rows
+    return n
 
 
 def decay_linear_attention(
@@ -231,20 +239,23 @@ def decay_linear_attention_step(
     B, H, dk = q.shape
     dv = v.shape[-1]
     _check_decay(log_decay, H)
-    _check_state(state, None, H, dk, dv)
-    assert slots is not None or state.shape[0] >= B
-    _no_grad_wanted(q, k, v, state)
+    n = _check_state(state, None, H, dk, dv)
+    assert slots is not None or n >= B
+    if torch.is_grad_enabled():
+        _no_grad_wanted(q, k, v, state)
     code = _lib.dtype_code(q.dtype)
-    q, k, v = _dense(q), _dense(k), _dense(v)
-    sp, sb = _slots(slots, B)
+    (qb, qh, qd), (kb, kh, kd), (vb, vh, vd) = q.stride(), k.stride(), v.stride()
+    if (qd != 1 and dk > 1) or (kd != 1 and dk > 1) or (vd != 1 and dv > 1):
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
+    sp, sb = (None, 0) if slots is None else _slots(slots, B)
     o = torch.empty((B, H, dv), device=q.device, dtype=q.dtype)
     with _lib.device_of(q):
-        _lib.check(
-            _lib.load().dynconv_la_step(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), state.data_ptr(), log_decay.data_ptr(), o.data_ptr(), sp, sb,
-                _Strides[6](*q.stride()[:2], *k.stride()[:2], *v.stride()[:2]), B, state.shape[0], H, dk, dv,
-                dk**-0.5 if scale is None else float(scale), code, _lib.raw_stream(q),
-            )
-        )
+        status = _lib.load().dynconv_la_step(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), state.data_ptr(), log_decay.data_ptr(), o.data_ptr(), sp, sb,
+            _Strides[6](qb, qh, kb, kh, vb, vh), B, n, H, dk, dv, dk**-0.5 if scale is None else float(scale), code,
+            _lib.raw_stream(q))
+        if status:
+            _lib.check(status)
         _lib.after_call(o)
     return o

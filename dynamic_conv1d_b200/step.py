@@ -18,14 +18,14 @@ from . import _lib
 
 
 def _no_grad_wanted(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("a single-token step has no gradient: call it under torch.no_grad()")
+    """Called where gradients are enabled."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError("a single-token step has no gradient: call it under torch.no_grad()")
 
 
 def _slots(slots: torch.Tensor | None, B: int):
     """(pointer, bytes of an index) of a slot table."""
-    if slots is None:
-        return None, 0
     assert slots.is_cuda and slots.is_contiguous() and slots.shape == (B,)
     assert slots.dtype in (torch.int32, torch.int64), "slots must be int32 or int64"
     return slots.data_ptr(), slots.element_size()
@@ -64,15 +64,9 @@ def lowrank_dynamic_convolution_grouped_step(
     Returns:
         y: [B, G*D].
     """
-    assert x.is_cuda and x.is_contiguous() and x.dim() == 2
-    assert z.is_cuda and z.is_contiguous() and z.dim() == 2 and z.shape[0] == x.shape[0]
-    assert U.is_cuda and U.is_contiguous() and U.dim() == 3
-    B, C = x.shape
+    assert U.dim() == 3
     G, R, WD = U.shape
-    assert C % G == 0 and z.shape[1] == G * R
-    D = C // G
-    assert WD % D == 0, "U must be [G, R, W*D]"
-    return _lowrank_step(x, z, U, cache, static_w, residual, slots, B, D, R, WD // D, G)
+    return _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, G)
 
 
 def lowrank_dynamic_convolution_step(
@@ -86,46 +80,52 @@ def lowrank_dynamic_convolution_step(
 ) -> torch.Tensor:
     """One token of ``lowrank_dynamic_convolution``: x [B, D], z [B, R], U [R, W*D],
     static_w [W, D], cache [n, W-1, D].  See ``lowrank_dynamic_convolution_grouped_step``."""
-    assert x.is_cuda and x.is_contiguous() and x.dim() == 2
-    assert z.is_cuda and z.is_contiguous() and z.dim() == 2 and z.shape[0] == x.shape[0]
-    assert U.is_cuda and U.is_contiguous() and U.dim() == 2
-    B, D = x.shape
+    assert U.dim() == 2
     R, WD = U.shape
-    assert z.shape[1] == R
-    assert WD % D == 0, "U must be [R, W*D]"
-    return _lowrank_step(x, z, U, cache, static_w, residual, slots, B, D, R, WD // D, 1)
+    return _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, 1)
 
 
-def _check_cache(x, cache, W, slots):
-    assert cache.is_cuda and cache.is_contiguous() and cache.dtype == x.dtype
-    assert cache.dim() == 3 and cache.shape[1:] == (W - 1, x.shape[1])
-    assert slots is not None or cache.shape[0] >= x.shape[0]
+def _check_cache(cache, dtype, B, W, C, slots):
+    """Rows of the cache."""
+    assert cache.is_cuda and cache.is_contiguous() and cache.dtype == dtype and cache.dim() == 3
+    n, rows, channels = cache.shape
+    assert rows == W - 1 and channels == C, f"cache must be [n, {W - 1}, {C}]"
+    assert slots is not None or n >= B
+    return n
 
 
-def _lowrank_step(x, z, U, cache, static_w, residual, slots, B, D, R, W, G):
-    _check_cache(x, cache, W, slots)
+def _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, G):
+    assert x.is_cuda and x.is_contiguous() and x.dim() == 2
+    assert z.is_cuda and z.is_contiguous()
+    assert U.is_cuda and U.is_contiguous()
+    B, C = x.shape
+    D = C // G
+    assert D * G == C and z.shape == (B, G * R)
+    W = WD // D
+    assert W * D == WD, "U must be [G, R, W*D]"
+    dtype = x.dtype
+    n = _check_cache(cache, dtype, B, W, C, slots)
     if static_w is not None:
         assert static_w.is_cuda and static_w.is_contiguous()
         assert static_w.shape == ((W, D) if U.dim() == 2 else (G, W, D))
-    _no_grad_wanted(x, z, U, static_w)
-    code = _lib.dtype_code(x.dtype)
+        if static_w.dtype != dtype:
+            static_w = static_w.to(dtype)
+    if torch.is_grad_enabled():
+        _no_grad_wanted(x, z, U, static_w)
+    code = _lib.dtype_code(dtype)
     # parameters of another dtype are cast for the call, as by the whole-sequence op
-    if z.dtype != x.dtype:
-        z = z.to(x.dtype)
-    if U.dtype != x.dtype:
-        U = U.to(x.dtype)
-    if static_w is not None and static_w.dtype != x.dtype:
-        static_w = static_w.to(x.dtype)
-    sp, sb = _slots(slots, B)
+    if z.dtype != dtype:
+        z = z.to(dtype)
+    if U.dtype != dtype:
+        U = U.to(dtype)
+    sp, sb = (None, 0) if slots is None else _slots(slots, B)
     y = torch.empty_like(x)
     with _lib.device_of(x):
-        _lib.check(
-            _lib.load().dynconv_lr_step(
-                x.data_ptr(), z.data_ptr(), U.data_ptr(), None if static_w is None else static_w.data_ptr(),
-                cache.data_ptr(), y.data_ptr(), sp, sb, B, cache.shape[0], D, R, W, G, code, int(bool(residual)),
-                _lib.raw_stream(x),
-            )
-        )
+        status = _lib.load().dynconv_lr_step(
+            x.data_ptr(), z.data_ptr(), U.data_ptr(), None if static_w is None else static_w.data_ptr(),
+            cache.data_ptr(), y.data_ptr(), sp, sb, B, n, D, R, W, G, code, 1 if residual else 0, _lib.raw_stream(x))
+        if status:
+            _lib.check(status)
         _lib.after_call(y)
     return y
 
@@ -146,23 +146,24 @@ def headwise_dynamic_convolution_step(
     B, D = x.shape
     H, W = weight.shape[1:]
     assert D % H == 0, f"D={D} must be divisible by H={H}"
-    _check_cache(x, cache, W, slots)
+    dtype = x.dtype
+    n = _check_cache(cache, dtype, B, W, D, slots)
     if static_w is not None:
         assert static_w.is_cuda and static_w.is_contiguous()
-        assert static_w.dtype == x.dtype
+        assert static_w.dtype == dtype
         assert static_w.shape == (W, D)
-    _no_grad_wanted(x, weight, static_w)
-    code = _lib.dtype_code(x.dtype)
-    weight = weight.to(dtype=x.dtype).contiguous()
-    sp, sb = _slots(slots, B)
+    if torch.is_grad_enabled():
+        _no_grad_wanted(x, weight, static_w)
+    code = _lib.dtype_code(dtype)
+    if weight.dtype != dtype or not weight.is_contiguous():
+        weight = weight.to(dtype=dtype).contiguous()
+    sp, sb = (None, 0) if slots is None else _slots(slots, B)
     y = torch.empty_like(x)
     with _lib.device_of(x):
-        _lib.check(
-            _lib.load().dynconv_hw_step(
-                x.data_ptr(), weight.data_ptr(), None if static_w is None else static_w.data_ptr(),
-                cache.data_ptr(), y.data_ptr(), sp, sb, B, cache.shape[0], D, H, W, code, int(bool(residual)),
-                _lib.raw_stream(x),
-            )
-        )
+        status = _lib.load().dynconv_hw_step(
+            x.data_ptr(), weight.data_ptr(), None if static_w is None else static_w.data_ptr(),
+            cache.data_ptr(), y.data_ptr(), sp, sb, B, n, D, H, W, code, 1 if residual else 0, _lib.raw_stream(x))
+        if status:
+            _lib.check(status)
         _lib.after_call(y)
     return y
