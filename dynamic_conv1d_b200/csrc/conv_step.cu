@@ -207,9 +207,9 @@ __global__ void __launch_bounds__(32 * W) lr_step_few_kernel(const T* __restrict
 // the kernel is bound by the batch's bytes, not by the product.
 //
 // Block: 32 channels of one group, four warps with 16 rows each, U's tile staged once for 64
-// rows.  Channels are staged permuted, so that a thread's four column pairs are eight
+// rows, the static filter in it as one more rank whose z is one.  Channels are staged permuted, so that a thread's four column pairs are eight
 // neighbouring channels: one 16-byte access per row and tensor.
-constexpr int kMmaRows = 64, kMmaCh = 32;
+constexpr int kMmaRows = 64, kMmaCh = 32, kMmaThreads = 128;
 
 __device__ __forceinline__ void mma_16n8k16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -228,35 +228,74 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
   }
 }
 
-template <int W>
-__global__ void __launch_bounds__(128) lr_step_mma_kernel(const __nv_bfloat16* __restrict__ x,
+template <int W, int KS>
+__global__ void __launch_bounds__(kMmaThreads, 6) lr_step_mma_kernel(const __nv_bfloat16* __restrict__ x,
                                                           const __nv_bfloat16* __restrict__ z,
                                                           const __nv_bfloat16* __restrict__ U,
                                                           const __nv_bfloat16* __restrict__ sw, __nv_bfloat16* cache,
                                                           __nv_bfloat16* __restrict__ y, const void* __restrict__ slots,
                                                           int slot_bytes, int64_t B, int64_t n_rows, int64_t D, int R,
-                                                          int RP, int G, int residual) {
+                                                          int G, int residual) {
   // us[w][k / 2][position] = channels' (U[k], U[k + 1]) pairs: B fragments are single words.
   // Row pitch 40 words: the four k rows that a fragment load touches lie 8 banks apart.
-  extern __shared__ uint32_t us[];
-  constexpr int kPitch = 40;
+  constexpr int kPitch = 40, K2 = KS * 8;
+  __shared__ uint32_t us[W * K2 * kPitch];  // at most 25 KB
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t C = (int64_t)G * D;
   const int64_t per = (D + kMmaCh - 1) / kMmaCh;
   const int64_t g = blockIdx.x / per, d0 = (blockIdx.x - g * per) * kMmaCh;
-  const int K2 = RP / 2;
   const int r0 = lane >> 2, q = lane & 3;
   const int64_t d = d0 + q * 8, c = g * D + d;
   const int64_t b0 = (int64_t)blockIdx.y * kMmaRows + warp * 16;
+  // this thread's inputs and caches, under way while U is staged and multiplied
+  uint4 past[2][W];
+  int64_t rows[2];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    const int64_t b = b0 + r0 + hf * 8;
+    rows[hf] = -1;
+#pragma unroll
+    for (int w = 0; w < W; ++w) past[hf][w] = make_uint4(0, 0, 0, 0);
+    if (b >= B || d >= D) continue;
+    const int64_t row = slot_of(slots, slot_bytes, (int)b);
+    if (row < 0 || row >= n_rows) continue;
+    rows[hf] = row;
+    const __nv_bfloat16* cr = cache + row * (int64_t)(W - 1) * C + c;
+    past[hf][0] = *reinterpret_cast<const uint4*>(x + b * C + c);
+#pragma unroll
+    for (int w = 1; w < W; ++w) past[hf][w] = *reinterpret_cast<const uint4*>(cr + (int64_t)(W - 1 - w) * C);
+  }
+  // z's fragments; rank R is the static filter's, with a z of one
+  uint32_t a[KS][4];
+  {
+    const uint16_t* zr = reinterpret_cast<const uint16_t*>(z) + ((b0 + r0) * G + g) * R;
+    const int64_t eight = (int64_t)8 * G * R;
+    const bool there[2] = {b0 + r0 < B, b0 + r0 + 8 < B};
+    const uint32_t one = sw ? 0x3F80u : 0u;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = ks * 16 + q * 2 + (i >> 1) * 8;
+        const uint16_t* at = zr + (i & 1) * eight + k;
+        uint32_t lo = k == R ? one : 0u, hi = k + 1 == R ? one : 0u;
+        if (there[i & 1] && k < R) lo = at[0];
+        if (there[i & 1] && k + 1 < R) hi = at[1];
+        a[ks][i] = lo | (hi << 16);
+      }
+  }
   // stage U: a thread takes 8 channels of a rank pair; position of channel c in the tile:
   // column pair j = (c % 8) / 2 of thread c / 8 is column 2 (c / 8) + c % 2 of product j
-  for (int i = threadIdx.x; i < W * K2 * 4; i += 128) {
+  for (int i = threadIdx.x; i < W * K2 * 4; i += kMmaThreads) {
     const int oct = i & 3, rest = i >> 2, k2 = rest % K2, w = rest / K2;
-    const int64_t d = d0 + oct * 8;
+    const int64_t du = d0 + oct * 8;
     uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-    const __nv_bfloat16* src = U + ((g * R + 2 * k2) * W + w) * D + d;
-    if (d < D && 2 * k2 < R) lo = *reinterpret_cast<const uint4*>(src);
-    if (d < D && 2 * k2 + 1 < R) hi = *reinterpret_cast<const uint4*>(src + (int64_t)W * D);
+    const __nv_bfloat16* src = U + ((g * R + 2 * k2) * W + w) * D + du;
+    const __nv_bfloat16* st = sw + (g * W + w) * D + du;
+    if (du < D && 2 * k2 < R) lo = *reinterpret_cast<const uint4*>(src);
+    if (du < D && 2 * k2 + 1 < R) hi = *reinterpret_cast<const uint4*>(src + (int64_t)W * D);
+    if (du < D && sw && 2 * k2 == R) lo = *reinterpret_cast<const uint4*>(st);
+    if (du < D && sw && 2 * k2 + 1 == R) hi = *reinterpret_cast<const uint4*>(st);
     uint32_t* dst = us + (w * K2 + k2) * kPitch + oct * 2;
     const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, h[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -266,71 +305,46 @@ __global__ void __launch_bounds__(128) lr_step_mma_kernel(const __nv_bfloat16* _
     }
   }
   __syncthreads();
-  if (b0 >= B) return;
-  float acc[4][W][4];  // column pair, tap, (row r0: two channels, row r0 + 8: two channels)
+  if (b0 >= B) return;  // (whole warps: all lanes take part in the products, channels there or not)
+  float out[2][8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int hf = 0; hf < 2; ++hf) {
+    float v[8];
+    unpack8(past[hf][0], v);
 #pragma unroll
-    for (int w = 0; w < W; ++w)
+    for (int e = 0; e < 8; ++e) out[hf][e] = residual ? v[e] : 0.f;
+  }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][w][e] = 0.f;
-  for (int k0 = 0; k0 < RP; k0 += 16) {
-    uint32_t a[4];
+  for (int w = 0; w < W; ++w) {  // tap by tap: its 32 weights, then their part of the outputs
+    float acc[4][4] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t b = b0 + r0 + (i & 1) * 8;
-      const int k = k0 + q * 2 + (i >> 1) * 8;
-      const uint16_t* zr = reinterpret_cast<const uint16_t*>(z) + (b * G + g) * R + k;
-      const uint32_t lo = b < B && k < R ? zr[0] : 0, hi = b < B && k + 1 < R ? zr[1] : 0;
-      a[i] = lo | (hi << 16);
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint32_t* f = us + (w * K2 + ks * 8 + q) * kPitch + r0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mma_16n8k16(acc[j], a[ks], f[j * 8], f[4 * kPitch + j * 8]);
     }
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const uint32_t* f = us + (w * K2 + k0 / 2 + q) * kPitch + r0;
+    for (int hf = 0; hf < 2; ++hf) {
+      float v[8];
+      unpack8(past[hf][w], v);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mma_16n8k16(acc[j][w], a, f[j * 8], f[4 * kPitch + j * 8]);
+      for (int e = 0; e < 8; ++e) out[hf][e] = fmaf(acc[e >> 1][hf * 2 + (e & 1)], v[e], out[hf][e]);
     }
   }
-  if (d >= D) return;
 #pragma unroll
   for (int hf = 0; hf < 2; ++hf) {
     const int64_t b = b0 + r0 + hf * 8;
-    if (b >= B) continue;
+    if (b >= B || d >= D) continue;
     uint4* yr = reinterpret_cast<uint4*>(y + b * C + c);
-    const int64_t row = slot_of(slots, slot_bytes, (int)b);
-    if (row < 0 || row >= n_rows) {
+    if (rows[hf] < 0) {
       *yr = make_uint4(0, 0, 0, 0);
       continue;
     }
-    // (loaded ahead of the products they would take 32 registers more: 18.1 instead of 14.5 us
-    // for 256 rows of 3 x 4096 channels)
-    __nv_bfloat16* cr = cache + row * (int64_t)(W - 1) * C + c;
-    uint4 past[W];
-    past[0] = *reinterpret_cast<const uint4*>(x + b * C + c);
+    const float(&o)[8] = out[hf];
+    *yr = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+    __nv_bfloat16* cr = cache + rows[hf] * (int64_t)(W - 1) * C + c;
 #pragma unroll
-    for (int w = 1; w < W; ++w) past[w] = *reinterpret_cast<const uint4*>(cr + (int64_t)(W - 1 - w) * C);
-    float out[8], v[8], s[8];
-    unpack8(past[0], v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = residual ? v[e] : 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      unpack8(past[w], v);
-      if (sw) {
-        unpack8(*reinterpret_cast<const uint4*>(sw + (g * W + w) * D + d), s);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) out[e] = fmaf(acc[e >> 1][w][hf * 2 + (e & 1)] + s[e], v[e], out[e]);
-    }
-    uint4 o;
-    o.x = pack_bf16x2(out[0], out[1]), o.y = pack_bf16x2(out[2], out[3]);
-    o.z = pack_bf16x2(out[4], out[5]), o.w = pack_bf16x2(out[6], out[7]);
-    *yr = o;
-#pragma unroll
-    for (int w = 1; w < W; ++w) *reinterpret_cast<uint4*>(cr + (int64_t)(W - 1 - w) * C) = past[w - 1];
+    for (int w = 1; w < W; ++w) *reinterpret_cast<uint4*>(cr + (int64_t)(W - 1 - w) * C) = past[hf][w - 1];
   }
 }
 
@@ -391,17 +405,26 @@ int lr_few(const StepArgs& a) {
   return DYNCONV_OK;
 }
 
-template <int W>
-int lr_mma(const StepArgs& a) {
-  const int rp = (a.R + 15) / 16 * 16;
+template <int W, int KS>
+int lr_mma_go(const StepArgs& a) {
   const dim3 grid((unsigned)(a.G * ((a.D + kMmaCh - 1) / kMmaCh)), (unsigned)((a.B + kMmaRows - 1) / kMmaRows));
-  const size_t smem = (size_t)W * (rp / 2) * 40 * sizeof(uint32_t);  // at most 20 KB
   using bf = __nv_bfloat16;
-  lr_step_mma_kernel<W><<<grid, 128, smem, a.st>>>((const bf*)a.x, (const bf*)a.z, (const bf*)a.U, (const bf*)a.sw,
-                                                   (bf*)a.cache, (bf*)a.y, a.slots, a.slot_bytes, a.B, a.n_rows, a.D,
-                                                   a.R, rp, a.G, a.residual);
+  lr_step_mma_kernel<W, KS><<<grid, kMmaThreads, 0, a.st>>>((const bf*)a.x, (const bf*)a.z, (const bf*)a.U, (const bf*)a.sw,
+                                                    (bf*)a.cache, (bf*)a.y, a.slots, a.slot_bytes, a.B, a.n_rows, a.D,
+                                                    a.R, a.G, a.residual);
   DYNCONV_CHECK_LAUNCH("lr_step_mma_kernel");
   return DYNCONV_OK;
+}
+
+template <int W>
+int lr_mma(const StepArgs& a) {
+  switch ((a.R + (a.sw ? 1 : 0) + 15) / 16) {  // ranks, the static filter's among them
+    case 1: return lr_mma_go<W, 1>(a);
+    case 2: return lr_mma_go<W, 2>(a);
+    case 3: return lr_mma_go<W, 3>(a);
+    case 4: return lr_mma_go<W, 4>(a);
+    default: return lr_mma_go<W, 5>(a);
+  }
 }
 
 bool aligned_octets(const StepArgs& a) {
