@@ -12,8 +12,8 @@
 // its rounding to bf16 would cost the state its precision: it is split into NS bf16 parts
 // (two: 2^-17 of each term, three: 2^-25, when the state goes back to the caller).
 //
-// Warps: a producer (TMA rings two deep), an MMA issuer, and three groups of
-// four: scores (Sc -> A, and the outputs), state (KV -> S), and weights (W -> W').  The issuer runs
+// Warps: a producer (TMA rings two deep), an MMA issuer, and four groups of four, whose warps
+// own 32 TMEM lanes each: two for the scores (Sc -> A, and the outputs), state (KV -> S), and weights (W -> W').  The issuer runs
 //     A(i-1) ready: O1(i-1);  Sc(i);  W'(i) ready: KV(i);  S(i) ready: O2(i)
 // so that while the scores group masks chunk i and writes the outputs of chunk i-1, the pipe has
 // KV and O2 of chunk i and O1 and Sc of the next.
@@ -30,11 +30,12 @@ namespace {
 
 constexpr int kC = 128;     // tokens of a chunk
 constexpr int kSlice = 64;  // columns of w per CTA
-constexpr int kTcThreads = 64 + 3 * 128;
+constexpr int kTcThreads = 64 + 4 * 128;
 constexpr uint32_t kBox = 64 * kC * 2;  // one TMA box: 128 rows of 64 bf16
 // Chunks brought into L2 ahead of their loads: a tile from HBM takes about 2000 cycles, half a
 // chunk's time, and the w ring asks for its next tile late.
 constexpr int kAhead = 3;
+constexpr uint32_t kStageOut = 32 * 64;  // 32 rows x 32 columns of outputs
 constexpr int kMaxMaps = kMaxRoles * 4;
 
 // TMEM columns
@@ -66,6 +67,11 @@ struct Bars {
 
 // 16-byte chunk c of row r in a 128-byte-swizzled tile of 128-byte rows.
 __device__ __forceinline__ uint32_t sw_off(int r, int c) { return (uint32_t)r * 128u + (uint32_t)((c ^ (r & 7)) << 4); }
+
+// 16-byte chunk c of row r in a 64-byte-swizzled tile of 64-byte rows (a warp's staged outputs).
+__device__ __forceinline__ uint32_t out_off(int r, int c) {
+  return (uint32_t)r * 64u + (uint32_t)((c ^ ((r >> 1) & 3)) << 4);
+}
 
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
@@ -115,10 +121,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&bars.w_empty[s], 1);
     }
     mbar_init(&bars.sc_full, 1);
-    mbar_init(&bars.a_ready, 4);
+    mbar_init(&bars.a_ready, 8);
     mbar_init(&bars.o_full, 1);
-    mbar_init(&bars.o_free[0], 4);
-    mbar_init(&bars.o_free[1], 4);
+    mbar_init(&bars.o_free[0], 8);
+    mbar_init(&bars.o_free[1], 8);
     mbar_init(&bars.o2_full, 1);
     mbar_init(&bars.h_ready, 4);
     mbar_init(&bars.kv_full, 1);
@@ -271,11 +277,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
     const int a = ro.reverse ? kC - 1 - row : row;  // scan position of token `row`
     const int group = (warp - 2) >> 2;
-    if (group == 0) {
+    if (group < 2) {
       // ----------------------------------------------------- outputs and masks
       if (!STATE_ONLY) {
         const bool rev = ro.reverse;
-        const int slot_rows = q * 32 * 128;  // this warp's rows in a w tile
+        const int half = group;  // of the outputs' columns, and every other block of the scores
+        uint8_t* tile = smem + L::kOffO + (half * 4 + q) * kStageOut;
         const float fo = ro.i_scale * pw[a + e];
         __nv_bfloat16* out = (__nv_bfloat16*)ro.out.p + (int64_t)b * ro.out.sb + (int64_t)h * ro.out.sh + c0;
         // Decays of the scores.  On the diagonal 32 x 32 block: g^|row - column|, read along the
@@ -289,7 +296,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int blocks = rev ? 4 - q : q + 1;  // 32-column blocks that are not masked
         {  // the masked blocks of A are zero once and for all
           const uint32_t z[8] = {};
-          for (int c = 0; c < 4; ++c)
+          for (int c = half; c < 4; c += 2)
             if (rev ? c < q : c > q) {
               tmem_st8(tmem + lanes + kColA + c * 16, z);
               tmem_st8(tmem + lanes + kColA + c * 16 + 8, z);
@@ -297,46 +304,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         auto outputs = [&](int i) {
           const int t = start_of(i) + row;
-          // a whole chunk leaves through shared memory and a TMA store of each warp's 32 rows
+          // a whole chunk leaves through shared memory and a TMA store of each warp's 32 x 32
           const bool staged = L::kStage && p.T - (first + i) * kC >= kC;
-          uint8_t* tile = smem + L::kOffO;
-          if (lane == 0) bulk_wait_group_read<0>();  // the store of the chunk before has read it
+          if (lane == 0) bulk_wait_group_read<0>();  // the store of the chunk before has read the tile
           __syncwarp();
           __nv_bfloat16* dst = out + (int64_t)t * ro.out.st;
           const bool in = t >= 0 && t < p.T;
           const bool bad = bad_any[i & 3] == (unsigned)i + 1;
-#pragma unroll 1
-          for (int c = 0; c < kSlice; c += 32) {
-            float v[32], u[32];
-            tmem_ld32(tmem + lanes + kColO1 + (i & 1) * kSlice + c, v);
-            tmem_ld32(tmem + lanes + kColO2 + (i & 1) * kSlice + c, u);
-            tmem_ld_wait();
-            uint32_t w[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+          for (int c = 0; c < 32; c += 16) {
+            float v[16], u[16];
+            tmem_ld16(tmem + lanes + kColO1 + (i & 1) * kSlice + half * 32 + c, v);
+            tmem_ld16(tmem + lanes + kColO2 + (i & 1) * kSlice + half * 32 + c, u);
+            tmem_ld_wait();
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
               const float2 r = fma2(make_float2(fo, fo), make_float2(u[2 * j], u[2 * j + 1]),
                                     mul2(make_float2(ro.a_scale, ro.a_scale), make_float2(v[2 * j], v[2 * j + 1])));
               w[j] = pack_bf16x2(r.x, r.y);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
               const uint4 o = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
               if (staged)
-                *reinterpret_cast<uint4*>(tile + sw_off(row, c / 8 + j)) = o;
-              else if (in && c0 + c + 8 * j < ro.dw)
-                *reinterpret_cast<uint4*>(dst + c + 8 * j) = o;
+                *reinterpret_cast<uint4*>(tile + out_off(lane, c / 8 + j)) = o;
+              else if (in && c0 + half * 32 + c + 8 * j < ro.dw)
+                *reinterpret_cast<uint4*>(dst + half * 32 + c + 8 * j) = o;
             }
           }
           tc_fence_before();
           if (bad) {
 #pragma unroll 1
-            for (int c = 0; c < kSlice; ++c) {
-              const unsigned key = bad_row[i & 3][c];
+            for (int c = 0; c < 32; ++c) {
+              const unsigned key = bad_row[i & 3][half * 32 + c];
               if (key >> 8 != (unsigned)i + 1 || 255 - (int)(key & 255) > a) continue;
               if (staged)
-                *reinterpret_cast<uint16_t*>(tile + sw_off(row, c / 8) + (c & 7) * 2) = 0x7FC0;
-              else if (in && c0 + c < ro.dw)
-                *reinterpret_cast<uint16_t*>(dst + c) = 0x7FC0;
+                *reinterpret_cast<uint16_t*>(tile + out_off(lane, c / 8) + (c & 7) * 2) = 0x7FC0;
+              else if (in && c0 + half * 32 + c < ro.dw)
+                *reinterpret_cast<uint16_t*>(dst + half * 32 + c) = 0x7FC0;
             }
           }
           if (staged) fence_proxy_async_smem();
@@ -344,7 +350,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (lane == 0) {
             mbar_arrive(&bars.o_free[i & 1]);
             if (staged) {
-              tma_store_4d(&maps.m[ri * 4 + 3], tile + slot_rows, c0, h, start_of(i) + q * 32, b);
+              tma_store_4d(&maps.m[ri * 4 + 3], tile, c0 + half * 32, h, start_of(i) + q * 32, b);
               bulk_commit_group();
             }
           }
@@ -359,9 +365,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             outputs(n - 1);
             break;
           }
-          float f = near;
+          float f = half ? near : near * g32;  // of this warp's first block off the diagonal: 1 or 2 away
 #pragma unroll 1
-          for (int k = 0; k < blocks; ++k) {
+          for (int k = half; k < blocks; k += 2) {
             const int c = (rev ? q + k : q - k) * 32;
             float v[32];
             uint32_t w[16];
@@ -384,7 +390,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 w[j] = pack_bf16x2(m0.x, m0.y);
                 w[j + 1] = pack_bf16x2(m1.x, m1.y);
               }
-              f *= g32;
+              f *= g32 * g32;
             }
             const uint32_t at = tmem + lanes + kColA + c / 2;
             tmem_st8(at, {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]});
@@ -398,7 +404,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (lane == 0) bulk_wait_group<0>();
       }
-    } else if (group == 1) {
+    } else if (group == 2) {
       // ---------------------------------------------------------------- state
       const int64_t n_state = (int64_t)ro.dx * ro.dw;
       const bool live = row < ro.dx;
@@ -428,12 +434,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int64_t left = p.T - (first + i - 1) * kC;
           const Factor f = left >= kC ? f_full : decay_factor(l2d, (double)left);
 #pragma unroll
-          for (int c = 0; c < kSlice; c += 32) {
-            float v[32];
-            tmem_ld32(tmem + lanes + kColKv + c, v);
+          for (int c = 0; c < kSlice; c += 16) {
+            float v[16];
+            tmem_ld16(tmem + lanes + kColKv + c, v);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {  // decay_add of pairs
+            for (int j = 0; j < 16; j += 2) {  // decay_add of pairs
               const float2 s2 = make_float2(S[c + j], S[c + j + 1]);
               const float2 r = fma2(make_float2(f.hi, f.hi), s2, fma2(make_float2(f.lo, f.lo), s2, make_float2(v[j], v[j + 1])));
               S[c + j] = r.x, S[c + j + 1] = r.y;
@@ -542,12 +548,13 @@ bool mappable(const View& v, int64_t B, int64_t T, int H) {
   return true;
 }
 
-int view_map(CUtensorMap* map, const View& v, int64_t B, int64_t T, int H, int d, int rows) {
+int view_map(CUtensorMap* map, const View& v, int64_t B, int64_t T, int H, int d, int cols, int rows) {
   const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
   const cuuint64_t strides[3] = {(cuuint64_t)(H > 1 ? v.sh * 2 : 16), (cuuint64_t)(T > 1 ? v.st * 2 : 16),
                                  (cuuint64_t)(B > 1 ? v.sb * 2 : 16)};
-  const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
-  return encode_tensor_map_bf16(map, v.p, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const cuuint32_t box[4] = {(cuuint32_t)cols, 1, (cuuint32_t)rows, 1};
+  return encode_tensor_map_bf16(map, v.p, 4, dims, strides, box,
+                                cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 template <int DX, int NS, bool STATE_ONLY>
@@ -603,10 +610,10 @@ int tc_launch(const Params& p, cudaStream_t st) {
   bool states = false;
   for (int r = 0; r < p.n_roles; ++r) {
     const Role& ro = p.role[r];
-    if ((s = view_map(&maps.m[4 * r], ro.x, p.B, p.T, p.H, ro.dx, kC))) return s;
-    if ((s = view_map(&maps.m[4 * r + 1], ro.y, p.B, p.T, p.H, ro.dx, kC))) return s;
-    if ((s = view_map(&maps.m[4 * r + 2], ro.w, p.B, p.T, p.H, ro.dw, kC))) return s;
-    if ((s = view_map(&maps.m[4 * r + 3], ro.out, p.B, p.T, p.H, ro.dw, 32))) return s;
+    if ((s = view_map(&maps.m[4 * r], ro.x, p.B, p.T, p.H, ro.dx, 64, kC))) return s;
+    if ((s = view_map(&maps.m[4 * r + 1], ro.y, p.B, p.T, p.H, ro.dx, 64, kC))) return s;
+    if ((s = view_map(&maps.m[4 * r + 2], ro.w, p.B, p.T, p.H, ro.dw, 64, kC))) return s;
+    if ((s = view_map(&maps.m[4 * r + 3], ro.out, p.B, p.T, p.H, ro.dw, 32, 32))) return s;
     dx = ro.dx > dx ? ro.dx : dx;
     states = states || ro.s_out;
   }
