@@ -2,6 +2,8 @@
 // one token, linear attention with decay, and the vocabulary loss (declared in
 // include/dynconv.h).  Like api.cu it validates, carves the caller's workspace and
 // dispatches; it allocates nothing and never synchronises.
+#include <algorithm>
+
 #include "common.cuh"
 #include "linear_attention.cuh"
 #include "vocab_loss.cuh"
@@ -91,7 +93,7 @@ size_t la_seg_bytes(const la::Params& p) {
 
 int la_run(la::Params& p, int dtype, void* ws, size_t ws_bytes, cudaStream_t st) {
   const bool tc = la::tc_supported(p, dtype);
-  tc ? la::tc_plan(&p) : la::simple_plan(&p);
+  tc ? la::tc_plan(&p, la::wants_states(p)) : la::simple_plan(&p);
   const size_t need = la_seg_bytes(p);
   if (need && (!ws || ws_bytes < need))
     return set_error(DYNCONV_ERR_WORKSPACE, "linear attention: workspace %zu < %zu bytes", ws_bytes, need);
@@ -163,12 +165,14 @@ int dynconv_hw_step(const void* x, const void* weight, const void* static_w, voi
 size_t dynconv_la_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype, int backward) {
   if (check_attention(B, T, H, dk, dv, dtype) || B * T == 0) return 0;
   la::Params p = backward ? la_backward_params(B, T, H, dk, dv, 1.f) : la_forward_params(B, T, H, dk, dv, 1.f);
-  // strides and alignment decide the path at the call: enough for either
+  // strides, alignment and the states wanted decide the path and the cut at the call: enough for each
   la::simple_plan(&p);
   const size_t simple = la_seg_bytes(p);
-  la::tc_plan(&p);
+  la::tc_plan(&p, false);
   const size_t tc = la_seg_bytes(p);
-  return simple > tc ? simple : tc;
+  la::tc_plan(&p, true);
+  const size_t tc_states = la_seg_bytes(p);
+  return std::max(simple, std::max(tc, tc_states));
 }
 
 int dynconv_la_fwd(const void* q, const void* k, const void* v, const float* log_decay, const float* initial_state,

@@ -215,26 +215,42 @@ __global__ void __launch_bounds__(kThreads) la_simple_kernel(const __grid_consta
 // ----------------------------------------------------------------------------- scan
 
 // In place over the segments of each (role, batch row, head): what segment s added to a
-// state of zero becomes the state at its start.  One thread per state element; the next
-// segment's value is loaded before the current one is used.
+// state of zero becomes the state at its start.  One thread per state element; eight
+// segments' values are under way before the first is used.
 __global__ void __launch_bounds__(256) la_scan_kernel(const __grid_constant__ Params p, int chunk) {
+  __shared__ Factor factor[2];  // over a whole segment, over the last
   const Role& ro = p.role[blockIdx.z];
   const int64_t n_state = (int64_t)ro.dx * ro.dw;
   const int64_t bh = blockIdx.y;
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (threadIdx.x < 2) {
+    const double span = (double)chunk * p.chunks_per_seg;
+    factor[threadIdx.x] = decay_factor(log2_decay(p.log_decay, (int)(bh % p.H)),
+                                       threadIdx.x == 0 ? span : (double)p.T - span * (p.n_seg - 1));
+  }
+  __syncthreads();
   if (i >= n_state) return;
+  const Factor f = factor[0];
   const int r = (int)(i / ro.dw), c = (int)(i % ro.dw);
-  const Factor f = decay_factor(log2_decay(p.log_decay, (int)(bh % p.H)), (double)chunk * p.chunks_per_seg);
-  float S = ro.s_in ? ro.s_in[bh * n_state + (int64_t)r * ro.si + (int64_t)c * ro.sj] : 0.f;
+  const int64_t at = bh * n_state + (int64_t)r * ro.si + (int64_t)c * ro.sj;
+  const int own_segs = p.n_seg - (p.scan_final ? 0 : 1);  // segments that have left their own state
+  float S = ro.s_in ? ro.s_in[at] : 0.f;
   float* s0 = seg_state(p, blockIdx.z, 0, bh, n_state) + i;
   const int64_t step = (int64_t)p.B * p.H * n_state;
-  float own = *s0;
-  for (int s = 0; s < p.n_seg; ++s) {
-    const float next = s + 2 < p.n_seg ? s0[step] : 0.f;
-    *s0 = S;
-    S = decay_add(f, S, own);
-    own = next;
-    s0 += step;
+  constexpr int kFly = 8;
+  for (int s = 0; s < p.n_seg; s += kFly) {
+    float own[kFly];
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) own[k] = s + k < own_segs ? s0[(s + k) * step] : 0.f;
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) {
+      if (s + k >= p.n_seg) break;
+      s0[(s + k) * step] = S;
+      if (s + k + 1 < p.n_seg)
+        S = decay_add(f, S, own[k]);
+      else if (p.scan_final && ro.s_out)
+        ro.s_out[at] = decay_add(factor[1], S, own[k]);
+    }
   }
 }
 
@@ -362,7 +378,8 @@ int scan_launch(const Params& p, int chunk, cudaStream_t st) {
   return DYNCONV_OK;
 }
 
-void plan_segments(Params* p, int chunk, int slice, int slots, double state_pass, double start, double scan) {
+void plan_segments(Params* p, int chunk, int slice, int slots, double whole, double state_pass, double start,
+                   double scan) {
   const int64_t chunks = (p->T + chunk - 1) / chunk;
   int64_t chains = 0;
   for (int r = 0; r < p->n_roles; ++r) chains += (int64_t)p->B * p->H * ((p->role[r].dw + slice - 1) / slice);
@@ -370,8 +387,9 @@ void plan_segments(Params* p, int chunk, int slice, int slots, double state_pass
   p->n_seg = 1, p->chunks_per_seg = (int)chunks;
   for (int64_t want = 1; want <= 64 && want <= chunks; ++want) {
     const int64_t per = (chunks + want - 1) / want, seg = (chunks + per - 1) / per;
-    double cost = (double)((chains * seg + slots - 1) / slots) * ((double)per + start);
-    if (seg > 1) cost += (double)((chains * (seg - 1) + slots - 1) / slots) * ((double)per * state_pass + start) + scan;
+    double cost = (double)((chains * seg + slots - 1) / slots) * ((double)per * (seg > 1 ? 1.0 : whole) + start);
+    const int64_t first = seg - (p->scan_final ? 0 : 1);  // segments of the state pass
+    if (seg > 1) cost += (double)((chains * first + slots - 1) / slots) * ((double)per * state_pass + start) + scan;
     if (cost < best) {
       best = cost;
       p->n_seg = (int)seg, p->chunks_per_seg = (int)per;
@@ -380,7 +398,7 @@ void plan_segments(Params* p, int chunk, int slice, int slots, double state_pass
 }
 
 // Measured at 64 x 64: a chunk 4 us, of the state pass 2.5 us, 4 us to start, 4 us for the scan; four CTAs per SM.
-void simple_plan(Params* p) { plan_segments(p, kC, kSlice, 4 * sm_count(), 0.6, 1.0, 1.0); }
+void simple_plan(Params* p) { plan_segments(p, kC, kSlice, 4 * sm_count(), 1.0, 0.6, 1.0, 1.0); }
 
 namespace {
 template <typename T>

@@ -56,6 +56,7 @@ struct Params {
   int n_seg;               // segments of a chain
   int chunks_per_seg;
   float* seg;              // n_seg > 1: [role][n_seg][B*H][dx*dw] (dx*dw is the same for every role)
+  int scan_final;          // the state pass covers the last segment too, and the scan writes s_out
 };
 
 // log2 of the decay factor.  A factor of zero is kept finite, so that 0 * log stays 0.
@@ -78,14 +79,22 @@ __device__ __forceinline__ Factor decay_factor(double l2, double n) {
 // f * S + a
 __device__ __forceinline__ float decay_add(Factor f, float S, float a) { return fmaf(f.hi, S, fmaf(f.lo, S, a)); }
 
+inline bool wants_states(const Params& p) {
+  for (int r = 0; r < p.n_roles; ++r)
+    if (p.role[r].s_out) return true;
+  return false;
+}
+
 __device__ __forceinline__ float* seg_state(const Params& p, int role, int seg, int64_t bh, int64_t n) {
   return p.seg + ((int64_t)(role * p.n_seg + seg) * p.B * p.H + bh) * n;
 }
 
 // Cuts chains into the number of segments with the lowest estimated time, counted in chunks of one
-// CTA: both passes run in rounds of `slots` CTAs; the state pass costs `state_pass` of a chunk's
-// time per chunk, a round's start `start` and the scan `scan` chunks.
-void plan_segments(Params* p, int chunk, int slice, int slots, double state_pass, double start, double scan);
+// CTA: both passes run in rounds of `slots` CTAs; an uncut chain costs `whole` and the state pass
+// `state_pass` of a chunk's time per chunk, a round's start `start` and the scan `scan` chunks.
+// Sets n_seg and chunks_per_seg; p->scan_final says what the state pass covers.
+void plan_segments(Params* p, int chunk, int slice, int slots, double whole, double state_pass, double start,
+                   double scan);
 
 // Launches the scan over segment states (role.s_in -> p.seg in place; chunk = tokens per chunk).
 int scan_launch(const Params& p, int chunk, cudaStream_t st);
@@ -94,7 +103,7 @@ void simple_plan(Params* p);  // chooses n_seg and chunks_per_seg
 int simple_launch(const Params& p, int dtype, cudaStream_t st);
 // tcgen05 kernels: see tc_supported for their envelope.
 bool tc_supported(const Params& p, int dtype);
-void tc_plan(Params* p);
+void tc_plan(Params* p, bool states);  // states: the state after the last token is wanted
 int tc_launch(const Params& p, cudaStream_t st);
 
 int step_launch(const View& q, const View& k, const View& v, float* state, const float* log_decay, void* o,

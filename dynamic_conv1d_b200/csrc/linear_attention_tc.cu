@@ -57,12 +57,14 @@ struct Smem {
   static constexpr uint32_t kOffH = kOffW + 2 * kBox;  // W': NS boxes, or two and the staged outputs
   static constexpr uint32_t kOffO = kOffH + 2 * kBox;
   static constexpr uint32_t kOffS = kOffH + 3 * kBox;
-  static constexpr uint32_t kTotal = kOffS + DX * 128 + 1024;
+  // The state pass has no x, no S and no outputs: a second W', in x's place where that is wide enough.
+  static constexpr uint32_t kOffH2 = DX == 128 ? kOffX : kOffS + DX * 128;
+  static constexpr uint32_t kTotal = kOffS + DX * 128 + (DX == 128 ? 0 : NS * kBox) + 1024;
 };
 
 struct Bars {
   uint64_t xy_full[2], xy_empty[2], w_full[2], w_empty[2];
-  uint64_t sc_full, a_ready, o_full, o_free[2], o2_full, h_ready, kv_full, s_ready, drain;
+  uint64_t sc_full, a_ready, o_full, o_free[2], o2_full, h_ready[2], kv_full[2], s_ready, kv_free[2], drain;
 };
 
 // 16-byte chunk c of row r in a 128-byte-swizzled tile of 128-byte rows.
@@ -80,6 +82,9 @@ template <int DX, int NS, bool STATE_ONLY>
 __global__ void __launch_bounds__(kTcThreads, 1)
     la_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ TcMaps maps, int total_slices) {
   using L = Smem<DX, NS>;
+  // W' and KV are single in the main pass (their time hides behind the other products) and double in
+  // the state pass, which has nothing else to do.
+  constexpr int kBuf = STATE_ONLY ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
   __shared__ Bars bars;
@@ -104,7 +109,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     ss -= (p.role[ri].dw + kSlice - 1) / kSlice;
     ++ri;
   }
-  if (STATE_ONLY && seg == p.n_seg - 1) return;
+  if (STATE_ONLY && seg == p.n_seg - 1 && !p.scan_final) return;
   const Role& ro = p.role[ri];
   const int c0 = ss * kSlice;
   const int b = bh / p.H, h = bh % p.H;
@@ -126,8 +131,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(&bars.o_free[0], 8);
     mbar_init(&bars.o_free[1], 8);
     mbar_init(&bars.o2_full, 1);
-    mbar_init(&bars.h_ready, 4);
-    mbar_init(&bars.kv_full, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars.h_ready[s], 4);
+      mbar_init(&bars.kv_full[s], 1);
+      mbar_init(&bars.kv_free[s], 4);
+    }
     mbar_init(&bars.s_ready, 4);
     mbar_init(&bars.drain, 1);
     abort_flag = 0;
@@ -235,21 +243,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         umma_commit_e(el, &bars.sc_full);
         __syncwarp();
       }
-      // s_ready: the state group has read KV of the chunk before
-      if (!mbar_wait(&bars.h_ready, i & 1, kErrWaitMma, &abort_flag) ||
-          !mbar_wait(&bars.s_ready, i & 1, kErrWaitMma, &abort_flag))
+      const int hb = i % kBuf;
+      if (!mbar_wait(&bars.h_ready[hb], (i / kBuf) & 1, kErrWaitMma, &abort_flag)) break;
+      // the state group has read what this KV holds (s_ready: and has put down S)
+      if (STATE_ONLY ? i >= kBuf && !mbar_wait(&bars.kv_free[hb], (i / kBuf - 1) & 1, kErrWaitMma, &abort_flag)
+                     : !mbar_wait(&bars.s_ready, i & 1, kErrWaitMma, &abort_flag))
         break;
       tc_fence_after();
       // W' part by part into one accumulator; rows of Y^T beyond DX = 64 read the next tile:
       // lanes of KV that nobody looks at
 #pragma unroll
       for (int part = 0; part < NS; ++part) {
-        const uint32_t hw = desc_lo(sb + L::kOffH + part * kBox, kBox);
+        const uint32_t hw = desc_lo(sb + (hb ? L::kOffH2 : L::kOffH) + part * kBox, kBox);
 #pragma unroll
         for (int k = 0; k < kC / 16; ++k)
-          umma_f16_e(el, tmem + kColKv, ym + k * (2048 / 16), hw + k * (2048 / 16), id_kv, part > 0 || k > 0);
+          umma_f16_e(el, tmem + (hb ? kColO1 : kColKv), ym + k * (2048 / 16), hw + k * (2048 / 16), id_kv, part > 0 || k > 0);
       }
-      umma_commit_e(el, &bars.kv_full);
+      umma_commit_e(el, &bars.kv_full[hb]);
       if (STATE_ONLY) {
         umma_commit_e(el, &bars.w_empty[i & 1]);
       } else {
@@ -277,7 +287,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
     const int a = ro.reverse ? kC - 1 - row : row;  // scan position of token `row`
     const int group = (warp - 2) >> 2;
-    if (group < 2) {
+    if (group == 1 || (group == 0 && !STATE_ONLY)) {
       // ----------------------------------------------------- outputs and masks
       if (!STATE_ONLY) {
         const bool rev = ro.reverse;
@@ -426,7 +436,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       bool dead = false;
       for (int i = 0; i <= n; ++i) {
         if (i > 0) {
-          if (!mbar_wait(&bars.kv_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)) {
+          const int hb = (i - 1) % kBuf;
+          if (!mbar_wait(&bars.kv_full[hb], ((i - 1) / kBuf) & 1, kErrWaitEpilogue, &abort_flag)) {
             dead = true;
             break;
           }
@@ -436,7 +447,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int c = 0; c < kSlice; c += 16) {
             float v[16];
-            tmem_ld16(tmem + lanes + kColKv + c, v);
+            tmem_ld16(tmem + lanes + (hb ? kColO1 : kColKv) + c, v);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {  // decay_add of pairs
@@ -446,6 +457,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
           tc_fence_before();
+          if (STATE_ONLY) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.kv_free[hb]);
+          }
         }
         if (i == n) break;
         if (!STATE_ONLY) {
@@ -465,9 +480,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars.s_ready);
-        } else {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.s_ready);
         }
       }
       if (!dead && live) {
@@ -475,7 +487,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int64_t sj = 1;
         if (STATE_ONLY)
           dst = seg_state(p, ri, seg, bh, n_state) + (int64_t)row * ro.dw + c0;
-        else if (seg == p.n_seg - 1 && ro.s_out)
+        else if (seg == p.n_seg - 1 && ro.s_out && !p.scan_final)
           dst = ro.s_out + (int64_t)bh * n_state + (int64_t)row * ro.si + (int64_t)c0 * ro.sj, sj = ro.sj;
         if (dst) {
 #pragma unroll
@@ -486,16 +498,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else {
       // -------------------------------------------------------------- weights
       const float fw = ro.w_scale * pw[kC - e - a];
-      for (int i = 0; i < n; ++i) {
-        const int sw = i & 1;
+      // (the state pass: two groups, every other chunk each)
+      for (int i = STATE_ONLY && group == 0 ? 1 : 0; i < n; i += kBuf) {
+        const int sw = i & 1, hb = i % kBuf;
         if (!mbar_wait(&bars.w_full[sw], (i >> 1) & 1, kErrWaitEpilogue, &abort_flag) ||
-            (i > 0 && !mbar_wait(&bars.kv_full, (i - 1) & 1, kErrWaitEpilogue, &abort_flag)))
+            (i >= kBuf && !mbar_wait(&bars.kv_full[hb], (i / kBuf - 1) & 1, kErrWaitEpilogue, &abort_flag)))
           break;
         const int64_t left = p.T - (first + i) * kC;
         float f = fw;
         if (left < kC) f = a < left ? ro.w_scale * pw[left - e - a] : 0.f;
         uint8_t* src = smem + L::kOffW + sw * kBox;
-        uint8_t* dst = smem + L::kOffH;
+        uint8_t* dst = smem + (hb ? L::kOffH2 : L::kOffH);
         uint32_t odd = 0;
 #pragma unroll 4
         for (int c = 0; c < 8; ++c) {
@@ -531,7 +544,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.h_ready);
+        if (lane == 0) mbar_arrive(&bars.h_ready[hb]);
       }
     }
   }
@@ -576,14 +589,15 @@ int go(const Params& p, const TcMaps& maps, cudaStream_t st) {
   return DYNCONV_OK;
 }
 
-template <int DX, int NS>
-int passes(const Params& p, const TcMaps& maps, cudaStream_t st) {
+// NS = 3 wherever a state goes back to the caller: in the state pass where there is one.
+template <int DX>
+int passes(const Params& p, const TcMaps& maps, bool states, cudaStream_t st) {
   int s;
   if (p.n_seg > 1) {
-    if ((s = go<DX, NS, true>(p, maps, st))) return s;
+    if ((s = states ? go<DX, 3, true>(p, maps, st) : go<DX, 2, true>(p, maps, st))) return s;
     if ((s = scan_launch(p, kC, st))) return s;
   }
-  return go<DX, NS, false>(p, maps, st);
+  return states && p.n_seg == 1 ? go<DX, 3, false>(p, maps, st) : go<DX, 2, false>(p, maps, st);
 }
 
 }  // namespace
@@ -601,13 +615,18 @@ bool tc_supported(const Params& p, int dtype) {
   return true;
 }
 
-// Measured at 128 x 128: a chunk 2.2 us, of the state pass 1 us, 5 us to start, 7 us for the scan; one CTA per SM.
-void tc_plan(Params* p) { plan_segments(p, kC, kSlice, sm_count(), 0.45, 2.5, 3.0); }
+// Measured at 128 x 128, one CTA per SM: a chunk 2 us, 2.9 with the third part of W'; a chunk of the
+// state pass 1.1 us, 1.4 with it; 9 us to start and end a round, 6 us for the scan.  So a long chain
+// whose last state is wanted is cheaper cut, with the third part in the state pass alone.
+void tc_plan(Params* p, bool states) {
+  p->scan_final = states;
+  plan_segments(p, kC, kSlice, sm_count(), states ? 1.45 : 1.0, states ? 0.7 : 0.55, 4.5, 3.0);
+  if (p->n_seg == 1) p->scan_final = 0;
+}
 
 int tc_launch(const Params& p, cudaStream_t st) {
   TcMaps maps;
   int s, dx = 0;
-  bool states = false;
   for (int r = 0; r < p.n_roles; ++r) {
     const Role& ro = p.role[r];
     if ((s = view_map(&maps.m[4 * r], ro.x, p.B, p.T, p.H, ro.dx, 64, kC))) return s;
@@ -615,10 +634,9 @@ int tc_launch(const Params& p, cudaStream_t st) {
     if ((s = view_map(&maps.m[4 * r + 2], ro.w, p.B, p.T, p.H, ro.dw, 64, kC))) return s;
     if ((s = view_map(&maps.m[4 * r + 3], ro.out, p.B, p.T, p.H, ro.dw, 32, 32))) return s;
     dx = ro.dx > dx ? ro.dx : dx;
-    states = states || ro.s_out;
   }
-  if (dx <= 64) return states ? passes<64, 3>(p, maps, st) : passes<64, 2>(p, maps, st);
-  return states ? passes<128, 3>(p, maps, st) : passes<128, 2>(p, maps, st);
+  const bool states = wants_states(p);
+  return dx <= 64 ? passes<64>(p, maps, states, st) : passes<128>(p, maps, states, st);
 }
 
 }  // namespace la
