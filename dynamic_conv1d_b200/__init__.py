@@ -3,7 +3,12 @@
     from dynamic_conv1d_b200 import headwise_dynamic_convolution, lowrank_dynamic_convolution
 
 Both ops are ``torch.autograd.Function``s over libdynconv.so, a C-ABI library of
-hand-written sm_100a CUDA kernels (see ``include/dynconv.h``).
+hand-written sm_100a CUDA kernels (see ``include/dynconv.h``).  So are the operators around
+them in a language model:
+
+    decay_linear_attention[_fused]        linear attention with a decay for each head
+    linear_cross_entropy                  the loss over a large vocabulary, without logits
+    *_step, convolution_cache             one token at a time, on caches updated in place
 
 Calls never synchronise.  The tensor-core kernels bound every device-side wait
 (1.5 s); a wait that gives up makes its kernel return early and sets a device
@@ -15,7 +20,12 @@ from ._lib import DynconvError, check_device, set_sync_checks
 from .headwise import headwise_dynamic_convolution
 from .linear_attention import decay_linear_attention, decay_linear_attention_fused, decay_linear_attention_step
 from .lowrank import lowrank_dynamic_convolution, lowrank_dynamic_convolution_grouped
-from .modules import LowRankDynamicShortConvolution, QKVLowRankDynamicShortConvolution
+from .modules import (
+    ConvolvedLinearAttention,
+    LayerCache,
+    LowRankDynamicShortConvolution,
+    QKVLowRankDynamicShortConvolution,
+)
 from .parallel import data_parallel, shard_rows
 from .sequence_parallel import headwise_dynamic_convolution_sp, lowrank_dynamic_convolution_sp
 from .step import (
@@ -40,6 +50,8 @@ __all__ = [
     "linear_cross_entropy",
     "LowRankDynamicShortConvolution",
     "QKVLowRankDynamicShortConvolution",
+    "ConvolvedLinearAttention",
+    "LayerCache",
     "data_parallel",
     "lowrank_dynamic_convolution_sp",
     "headwise_dynamic_convolution_sp",
