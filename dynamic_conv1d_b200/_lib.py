@@ -130,19 +130,22 @@ def on_device(fn):
 
 
 _same_device = contextlib.nullcontext()
+# the bindings under torch.cuda.current_device / current_stream, without the Python objects, for
+# calls whose kernels take a few microseconds
+current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+raw_stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
 def device_of(t: torch.Tensor):
     """Context in which t's device is current (free when it already is)."""
-    if t.device.index == torch.cuda.current_device():
+    if t.get_device() == current_device():
         return _same_device
     return torch.cuda.device(t.device)
 
 
 def raw_stream(t: torch.Tensor) -> int:
-    """The current stream of t's device as an address (``stream_of`` without the Stream object,
-    for calls whose kernels take a few microseconds)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    """The current stream of t's device as an address."""
+    return raw_stream_of(t.get_device())
 
 
 def ptr(t: torch.Tensor | None):

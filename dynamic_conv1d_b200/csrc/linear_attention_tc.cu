@@ -118,6 +118,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int n = (int)(min(n_chunks, first + p.chunks_per_seg) - first);
   const int e = ro.reverse ? 0 : 1;
 
+  auto start_of = [&](int i) -> int {  // first token of chunk i's tile (negative: before the sequence)
+    const int64_t ch = first + i;
+    return (int)(ro.reverse ? p.T - (ch + 1) * kC : ch * kC);
+  };
+
+  const CUtensorMap *mx = &maps.m[ri * 4], *my = mx + 1, *mw = mx + 2;
+  auto load_xy = [&](int i) {
+    const int s = i & 1;
+    mbar_arrive_expect_tx(&bars.xy_full[s], STATE_ONLY ? L::kX : 2 * L::kX);
+#pragma unroll
+    for (int d = 0; d < DX / 64; ++d) {
+      if (!STATE_ONLY)
+        tma_load_4d(smem + L::kOffX + s * L::kX + d * kBox, mx, &bars.xy_full[s], d * 64, h, start_of(i), b,
+                    policy_evict_normal());
+      tma_load_4d(smem + L::kOffY + s * L::kX + d * kBox, my, &bars.xy_full[s], d * 64, h, start_of(i), b,
+                  policy_evict_normal());
+    }
+  };
+  auto load_w = [&](int i) {
+    const int s = i & 1;
+    mbar_arrive_expect_tx(&bars.w_full[s], kBox);
+    tma_load_4d(smem + L::kOffW + s * kBox, mw, &bars.w_full[s], c0, h, start_of(i), b, policy_evict_normal());
+  };
+
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars.xy_full[s], 1);
@@ -140,6 +164,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(&bars.drain, 1);
     abort_flag = 0;
     fence_barrier_init();
+    for (int i = 0; i < 2 && i < n; ++i) {  // the first loads, under way while the CTA sets itself up
+      load_xy(i);
+      load_w(i);
+    }
   }
   if (threadIdx.x < 4 * kSlice) bad_row[threadIdx.x / kSlice][threadIdx.x % kSlice] = 0;
   if (threadIdx.x < 4) bad_any[threadIdx.x] = 0;
@@ -159,18 +187,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  auto start_of = [&](int i) -> int {  // first token of chunk i's tile (negative: before the sequence)
-    const int64_t ch = first + i;
-    return (int)(ro.reverse ? p.T - (ch + 1) * kC : ch * kC);
-  };
-
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
-      const CUtensorMap *mx = &maps.m[ri * 4], *my = mx + 1, *mw = mx + 2;
-      int issued = 0;
+      int issued = n < 2 ? 2 * n : 4;
       for (int i = 0; i < n; ++i) {
-        const int t0 = start_of(i), s = i & 1;
+        const int s = i & 1;
         if (i + kAhead < n) {
           const int t1 = start_of(i + kAhead);
 #pragma unroll
@@ -180,17 +202,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           tma_prefetch_4d(mw, c0, h, t1, b);
         }
+        if (i < 2) continue;  // (loaded above)
         if (!mbar_wait(&bars.xy_empty[s], ((i >> 1) & 1) ^ 1, kErrWaitProducer, &abort_flag)) break;
-        mbar_arrive_expect_tx(&bars.xy_full[s], STATE_ONLY ? L::kX : 2 * L::kX);
-#pragma unroll
-        for (int d = 0; d < DX / 64; ++d) {
-          if (!STATE_ONLY) tma_load_4d(smem + L::kOffX + s * L::kX + d * kBox, mx, &bars.xy_full[s], d * 64, h, t0, b, policy_evict_normal());
-          tma_load_4d(smem + L::kOffY + s * L::kX + d * kBox, my, &bars.xy_full[s], d * 64, h, t0, b, policy_evict_normal());
-        }
+        load_xy(i);
         issued = 2 * i + 1;
         if (!mbar_wait(&bars.w_empty[s], ((i >> 1) & 1) ^ 1, kErrWaitProducer, &abort_flag)) break;
-        mbar_arrive_expect_tx(&bars.w_full[s], kBox);
-        tma_load_4d(smem + L::kOffW + s * kBox, mw, &bars.w_full[s], c0, h, t0, b, policy_evict_normal());
+        load_w(i);
         issued = 2 * i + 2;
       }
       if (abort_flag) {  // a wait gave up: the copies in flight land before the shared memory is given back
@@ -412,24 +429,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (lane == 0) mbar_arrive(&bars.a_ready);
           if (i > 0) outputs(i - 1);
         }
-        if (lane == 0) bulk_wait_group<0>();
+        if (lane == 0) bulk_wait_group_read<0>();  // (shared memory may go once it has been read)
       }
     } else if (group == 2) {
       // ---------------------------------------------------------------- state
       const int64_t n_state = (int64_t)ro.dx * ro.dw;
       const bool live = row < ro.dx;
       float S[kSlice];
+      // Rows of 64 floats per thread would touch 32 lines with every load: states whose w-dimension
+      // is dense pass through the warp's part of S's shared memory, a line at a time (rows
+      // and columns of a 32 x 32 tile exchanged, column index ^ row against bank conflicts).
+      float* tile = reinterpret_cast<float*>(smem + L::kOffS) + q * 1024;
+      const int rows_here = min(32, ro.dx - q * 32);  // (none or fewer in the upper warps)
       {
         const float* src = nullptr;
-        int64_t sj = 1;
-        if (!STATE_ONLY && live) {
+        int64_t si = ro.dw, sj = 1;
+        if (!STATE_ONLY) {
           if (p.n_seg > 1)
-            src = seg_state(p, ri, seg, bh, n_state) + (int64_t)row * ro.dw + c0;
+            src = seg_state(p, ri, seg, bh, n_state);
           else if (ro.s_in)
-            src = ro.s_in + (int64_t)bh * n_state + (int64_t)row * ro.si + (int64_t)c0 * ro.sj, sj = ro.sj;
+            src = ro.s_in + (int64_t)bh * n_state, si = ro.si, sj = ro.sj;
         }
+        if (src && sj == 1 && rows_here > 0) {
 #pragma unroll
-        for (int j = 0; j < kSlice; ++j) S[j] = src && c0 + j < ro.dw ? src[j * sj] : 0.f;
+          for (int hf = 0; hf < kSlice; hf += 32) {
+            const bool in = c0 + hf + lane < ro.dw;
+            const float* at = src + (int64_t)q * 32 * si + c0 + hf + lane;
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r) tile[r * 32 + (lane ^ r)] = in && r < rows_here ? at[r * si] : 0.f;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) S[hf + j] = tile[lane * 32 + (j ^ lane)];
+            __syncwarp();
+          }
+        } else {
+          if (!live) src = nullptr;
+          const float* at = src + row * si + c0 * sj;
+#pragma unroll
+          for (int j = 0; j < kSlice; ++j) S[j] = src && c0 + j < ro.dw ? at[j * sj] : 0.f;
+        }
       }
       const double l2d = log2_decay(p.log_decay, h);
       const Factor f_full = decay_factor(l2d, kC);
@@ -482,17 +520,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (lane == 0) mbar_arrive(&bars.s_ready);
         }
       }
-      if (!dead && live) {
+      if (!dead) {
         float* dst = nullptr;
-        int64_t sj = 1;
+        int64_t si = ro.dw, sj = 1;
         if (STATE_ONLY)
-          dst = seg_state(p, ri, seg, bh, n_state) + (int64_t)row * ro.dw + c0;
+          dst = seg_state(p, ri, seg, bh, n_state);
         else if (seg == p.n_seg - 1 && ro.s_out && !p.scan_final)
-          dst = ro.s_out + (int64_t)bh * n_state + (int64_t)row * ro.si + (int64_t)c0 * ro.sj, sj = ro.sj;
-        if (dst) {
+          dst = ro.s_out + (int64_t)bh * n_state, si = ro.si, sj = ro.sj;
+        if (dst && sj == 1 && rows_here > 0) {
+          // S's last reader is O2 of the last chunk
+          if (!STATE_ONLY) dead = !mbar_wait(&bars.o2_full, (n - 1) & 1, kErrWaitEpilogue, &abort_flag);
+          if (!dead) {
+#pragma unroll
+            for (int hf = 0; hf < kSlice; hf += 32) {
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) tile[lane * 32 + (j ^ lane)] = S[hf + j];
+              __syncwarp();
+              float* at = dst + (int64_t)q * 32 * si + c0 + hf + lane;
+              if (c0 + hf + lane < ro.dw) {
+#pragma unroll 8
+                for (int r = 0; r < 32; ++r)
+                  if (r < rows_here) at[r * si] = tile[r * 32 + (lane ^ r)];
+              }
+            }
+          }
+        } else if (dst && sj != 1 && live) {
+          float* at = dst + row * si + c0 * sj;
 #pragma unroll
           for (int j = 0; j < kSlice; ++j)
-            if (c0 + j < ro.dw) dst[j * sj] = S[j];
+            if (c0 + j < ro.dw) at[j * sj] = S[j];
         }
       }
     } else {

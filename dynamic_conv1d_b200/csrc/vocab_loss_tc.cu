@@ -442,7 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       if (lane == 0) arrive_in_first_cta(freed[a]);
     }
     if constexpr (MODE == kTcGrad || MODE == kTcStore) {
-      if (lane == 0) bulk_wait_group<0>();
+      if (lane == 0) bulk_wait_group_read<0>();  // (shared memory may go once it has been read)
     }
   }
   tc_fence_before();

@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .step import _no_grad_wanted, _slots
+from .step import _refuse_gradient, _slots
 
 _Strides = {n: ctypes.c_int64 * n for n in (6, 12, 21)}
 
@@ -241,8 +241,8 @@ def decay_linear_attention_step(
     _check_decay(log_decay, H)
     n = _check_state(state, None, H, dk, dv)
     assert slots is not None or n >= B
-    if torch.is_grad_enabled():
-        _no_grad_wanted(q, k, v, state)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        _refuse_gradient()
     code = _lib.dtype_code(q.dtype)
     (qb, qh, qd), (kb, kh, kd), (vb, vh, vd) = q.stride(), k.stride(), v.stride()
     if (qd != 1 and dk > 1) or (kd != 1 and dk > 1) or (vd != 1 and dv > 1):

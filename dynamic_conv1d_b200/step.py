@@ -17,11 +17,8 @@ import torch
 from . import _lib
 
 
-def _no_grad_wanted(*tensors) -> None:
-    """Called where gradients are enabled."""
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            raise RuntimeError("a single-token step has no gradient: call it under torch.no_grad()")
+def _refuse_gradient():
+    raise RuntimeError("a single-token step has no gradient: call it under torch.no_grad()")
 
 
 def _slots(slots: torch.Tensor | None, B: int):
@@ -110,8 +107,9 @@ def _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, G):
         assert static_w.shape == ((W, D) if U.dim() == 2 else (G, W, D))
         if static_w.dtype != dtype:
             static_w = static_w.to(dtype)
-    if torch.is_grad_enabled():
-        _no_grad_wanted(x, z, U, static_w)
+    if torch.is_grad_enabled() and (x.requires_grad or z.requires_grad or U.requires_grad
+                                    or (static_w is not None and static_w.requires_grad)):
+        _refuse_gradient()
     code = _lib.dtype_code(dtype)
     # parameters of another dtype are cast for the call, as by the whole-sequence op
     if z.dtype != dtype:
@@ -152,8 +150,9 @@ def headwise_dynamic_convolution_step(
         assert static_w.is_cuda and static_w.is_contiguous()
         assert static_w.dtype == dtype
         assert static_w.shape == (W, D)
-    if torch.is_grad_enabled():
-        _no_grad_wanted(x, weight, static_w)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                    or (static_w is not None and static_w.requires_grad)):
+        _refuse_gradient()
     code = _lib.dtype_code(dtype)
     if weight.dtype != dtype or not weight.is_contiguous():
         weight = weight.to(dtype=dtype).contiguous()
