@@ -104,7 +104,7 @@ int la_run(la::Params& p, int dtype, void* ws, size_t ws_bytes, cudaStream_t st)
 int check_loss(int64_t N, int64_t D, int64_t V, int reduction, int dtype) {
   int s;
   if ((s = check_dtype(dtype))) return s;
-  if (N < 0 || D < 1 || V < 1 || N > INT32_MAX || D > INT32_MAX / 16 || V > (int64_t)1 << 22)
+  if (N < 0 || D < 1 || V < 1 || N > (1 << 30) || D > INT32_MAX / 16 || V > (int64_t)1 << 22)
     return set_error(DYNCONV_ERR_SHAPE, "vocabulary loss: bad sizes N=%lld D=%lld V=%lld", (long long)N, (long long)D,
                      (long long)V);
   if (reduction < vl::kNone || reduction > vl::kMean)
@@ -234,7 +234,7 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
 size_t dynconv_vocab_loss_fwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype) {
   if (check_loss(N, D, V, 0, dtype)) return 0;
   const int64_t tiles = (V + vl::kNarrowestTile - 1) / vl::kNarrowestTile + 2;  // enough for either path
-  return align_up((size_t)tiles * N * sizeof(float2)) + align_up((size_t)N * sizeof(float));
+  return align_up((size_t)tiles * std::min(N, vl::kRowsAtOnce) * sizeof(float2)) + align_up((size_t)N * sizeof(float));
 }
 
 int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t* target, float* loss, float* lse,
@@ -250,7 +250,7 @@ int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t
   p.hidden = hidden, p.weight = weight, p.target = target;
   p.N = N, p.D = D, p.V = V, p.ignore = ignore_index, p.reduction = reduction;
   p.lse = lse, p.loss = loss, p.stats = stats, p.st = st;
-  if (N == 0) return vl::merge_launch(p, 0);
+  if (N == 0) return vl::total_launch(p);
   if (!hidden || !weight || !target || !lse) return set_error(DYNCONV_ERR_ARGUMENT, "vocab_loss_fwd: null tensor");
   const size_t need = dynconv_vocab_loss_fwd_workspace_bytes(N, D, V, dtype);
   if (!workspace || workspace_bytes < need)

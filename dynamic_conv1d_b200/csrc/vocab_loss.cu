@@ -8,7 +8,7 @@ namespace vl {
 
 namespace {
 
-constexpr int kK = 16;      // inner steps staged at once
+constexpr int kK = 8;       // inner steps staged at once (16 take more registers and 5% longer)
 constexpr int kThreads = 256;
 
 enum Mode { kForward, kGrad, kAccumulate, kStore };
@@ -256,14 +256,19 @@ __global__ void __launch_bounds__(1024) vl_total_kernel(const Problem p) {
 }
 
 template <typename T>
-int fwd(const Problem& p) {
-  Gemm g{};
-  g.A = p.hidden, g.am = p.D, g.ak = 1;
-  g.B = p.weight, g.bn = p.D, g.bk = 1;
-  g.M = p.N, g.N = p.V, g.K = p.D;
-  int s = gemm<T, kForward>(g, p, 1, "vl_gemm_kernel (forward)");
-  const int64_t tile = large_tiles(p.N, p.V, 1) ? 128 : 64;
-  return s ? s : merge_launch(p, (p.V + tile - 1) / tile);
+int fwd(const Problem& all) {
+  int s;
+  for (int64_t r0 = 0; r0 < all.N; r0 += kRowsAtOnce) {
+    const Problem p = rows_from(all, r0, sizeof(T));
+    Gemm g{};
+    g.A = p.hidden, g.am = p.D, g.ak = 1;
+    g.B = p.weight, g.bn = p.D, g.bk = 1;
+    g.M = p.N, g.N = p.V, g.K = p.D;
+    if ((s = gemm<T, kForward>(g, p, 1, "vl_gemm_kernel (forward)"))) return s;
+    const int64_t tile = large_tiles(p.N, p.V, 1) ? 128 : 64;
+    if ((s = merge_launch(p, (p.V + tile - 1) / tile))) return s;
+  }
+  return total_launch(all);
 }
 
 template <typename T>
@@ -346,10 +351,12 @@ int finish_launch(const Problem& p, const float* parts, int n_parts, int64_t n, 
 }
 
 int merge_launch(const Problem& p, int64_t tiles) {
-  if (p.N > 0) {
-    vl_merge_kernel<<<(unsigned)((p.N + 31) / 32), 256, 0, p.st>>>(p, tiles);
-    DYNCONV_CHECK_LAUNCH("vl_merge_kernel");
-  }
+  vl_merge_kernel<<<(unsigned)((p.N + 31) / 32), 256, 0, p.st>>>(p, tiles);
+  DYNCONV_CHECK_LAUNCH("vl_merge_kernel");
+  return DYNCONV_OK;
+}
+
+int total_launch(const Problem& p) {
   vl_total_kernel<<<1, 1024, 0, p.st>>>(p);
   DYNCONV_CHECK_LAUNCH("vl_total_kernel");
   return DYNCONV_OK;
@@ -385,7 +392,8 @@ Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc) {
   if (most < 1024) most = 1024;
   Plan best{};
   double best_cost = 1e300;
-  for (int64_t cols = most < V ? most : up(V, 256) * 256;; cols -= 256) {
+  const int64_t step = up(up(V, 128), 256) * 256;  // at most about 128 candidates
+  for (int64_t cols = most < V ? most : up(V, 256) * 256; cols > 0; cols -= step) {
     const int64_t full = V / cols, rest = V - full * cols;
     const int z_h = share(n_tiles * d_tiles, cols < V ? cols : V), z_w = share(up(cols < V ? cols : V, tm) * d_tiles, N);
     const double c = (double)full * cost(cols, z_h, z_w) + (rest ? cost(rest, z_h, z_w) : 0.0);
@@ -394,7 +402,7 @@ Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc) {
       best.piece = cols < V ? cols : V;
       best.z_h = z_h, best.z_w = z_w;
     }
-    if (cols <= 1024 || up(V, cols) > 64) break;
+    if (up(V, cols) > 64) break;
   }
   best.pitch = up(best.piece, 64) * 64;
   return best;

@@ -36,7 +36,7 @@ struct Problem {
   float* lse;               // [N]
   float* loss;              // [N] (kNone) or [1]
   float* stats;             // [2]: sum of the rows' losses, number of rows that count
-  float2* part;             // [tiles][N]: of a tile's row, m = max * log2(e) rounded, and
+  float2* part;             // [tiles][rows at once]: of a tile's row, m = max * log2(e) rounded, and
                             // sum of 2^(l * log2(e) - m)
   float* tgt;               // [N]: the target's logit
   // backward
@@ -69,10 +69,23 @@ __device__ __forceinline__ float result_factor(const Problem& p) {
   return p.stats[1] > 0.f ? p.dloss[0] / p.stats[1] : 0.f;
 }
 
+// The forward takes this many rows at a time: it bounds the tiles' partial sums in the workspace
+// (8 bytes for each row and tile), and the weight is read again once per 32768 rows only.
+constexpr int64_t kRowsAtOnce = 32768;
 constexpr int kNarrowestTile = 64;  // columns of the vocabulary in one forward tile, at least
 bool tc_supported(const Problem& p, int dtype);
 Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc);
-int merge_launch(const Problem& p, int64_t tiles);
+int merge_launch(const Problem& rows, int64_t tiles);  // the rows' losses from their tiles
+int total_launch(const Problem& p);                    // their sum and number
+// The part of a forward problem that begins at row r0.
+inline Problem rows_from(const Problem& p, int64_t r0, int64_t elem) {
+  Problem r = p;
+  r.N = p.N - r0 < kRowsAtOnce ? p.N - r0 : kRowsAtOnce;
+  r.hidden = (const char*)p.hidden + r0 * p.D * elem;
+  r.target += r0, r.lse += r0, r.tgt += r0;
+  if (p.reduction == kNone) r.loss += r0;
+  return r;
+}
 // out[i] = result_factor * the sum of n-element parts, in part order, rounded to dtype
 int finish_launch(const Problem& p, const float* parts, int n_parts, int64_t n, void* out, int dtype);
 

@@ -493,17 +493,20 @@ bool tc_supported(const Problem& p, int dtype) {
   return true;
 }
 
-int tc_fwd(const Problem& p) {
+int tc_fwd(const Problem& all) {
   CUtensorMap a, b;
   int s;
-  if ((s = matrix_map(&a, p.hidden, p.D, p.N, p.D, kHalfM))) return s;
-  if ((s = matrix_map(&b, p.weight, p.D, p.V, p.D, kHalfB))) return s;
-  TcGemm g{};
-  g.M = p.N, g.N = p.V, g.k_blocks = (int)((p.D + kKB - 1) / kKB), g.z = 1, g.group = row_group(p.D);
-  s = g.k_blocks <= kChain ? launch<kTcForward, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)")
-                           : launch<kTcForwardLong, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)");
-  if (s) return s;
-  return merge_launch(p, (p.V + kN - 1) / kN * 2);
+  if ((s = matrix_map(&b, all.weight, all.D, all.V, all.D, kHalfB))) return s;
+  for (int64_t r0 = 0; r0 < all.N; r0 += kRowsAtOnce) {
+    const Problem p = rows_from(all, r0, 2);
+    if ((s = matrix_map(&a, p.hidden, p.D, p.N, p.D, kHalfM))) return s;
+    TcGemm g{};
+    g.M = p.N, g.N = p.V, g.k_blocks = (int)((p.D + kKB - 1) / kKB), g.z = 1, g.group = row_group(p.D);
+    s = g.k_blocks <= kChain ? launch<kTcForward, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)")
+                             : launch<kTcForwardLong, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)");
+    if (s || (s = merge_launch(p, (p.V + kN - 1) / kN * 2))) return s;
+  }
+  return total_launch(all);
 }
 
 int tc_bwd(const Problem& p, const Plan& pl) {

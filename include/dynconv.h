@@ -313,7 +313,7 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
  *   reduction: 0 none (loss [N]), 1 sum, 2 mean over the rows that count (loss [1]; NaN
  *   when none does).  loss, lse [N] and stats [2] are float32; lse and stats are kept for
  *   the backward (stats: sum of the rows' losses, number of rows that count).
- * V <= 4194304. */
+ * N <= 2^30, V <= 4194304. */
 size_t dynconv_vocab_loss_fwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype);
 int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t* target,
                            float* loss, float* lse, float* stats, void* workspace, size_t workspace_bytes,

@@ -105,11 +105,27 @@ def test_several_pieces(dtype):
     check(*make(N, 16, V, dtype))
 
 
+@pytest.mark.parametrize("dtype", BOTH)
+def test_more_rows_than_one_launch(dtype):
+    """The forward takes 32768 rows at a time."""
+    h, w, t = make(40001, 16, 200, dtype)
+    rows = linear_cross_entropy(h, w, t, reduction="none")
+    want, _, _ = definition(h, w, t, torch.ones(40001, device="cuda"), "none")
+    assert rel(rows, want) <= LOSS
+    check(h, w, t)
+
+
 def test_long_inner_dimensions():
     """Few tiles, long sums: the inner dimension is spread over several CTAs."""
     check(*make(20, 128, 30000, torch.bfloat16))
     check(*make(20, 64, 9000, torch.float32))
     check(*make(6000, 64, 100, torch.bfloat16))
+
+
+def test_channels_beyond_one_chain():
+    """More than 2048 products in a logit: summed in parts (bf16)."""
+    for D in (2056, 4096, 5000):
+        check(*make(130, D, 300, torch.bfloat16), loss_tol=2 * LOSS)
 
 
 @pytest.mark.parametrize("dtype", BOTH)
