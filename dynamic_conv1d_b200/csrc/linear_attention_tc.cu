@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&bars.xy_full[s], 1);
       mbar_init(&bars.xy_empty[s], 1);
       mbar_init(&bars.w_full[s], 1);
-      mbar_init(&bars.w_empty[s], 1);
+      mbar_init(&bars.w_empty[s], STATE_ONLY ? 4 : 1);  // (the state pass needs w only to weight it)
     }
     mbar_init(&bars.sc_full, 1);
     mbar_init(&bars.a_ready, 8);
@@ -190,9 +190,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
-      int issued = n < 2 ? 2 * n : 4;
+      int xy = min(n, 2), w = xy;  // loads issued
+      auto more_xy = [&](int i) -> bool {
+        if (!mbar_wait(&bars.xy_empty[i & 1], ((i >> 1) & 1) ^ 1, kErrWaitProducer, &abort_flag)) return false;
+        load_xy(i);
+        xy = i + 1;
+        return true;
+      };
+      auto more_w = [&](int i) -> bool {
+        if (!mbar_wait(&bars.w_empty[i & 1], ((i >> 1) & 1) ^ 1, kErrWaitProducer, &abort_flag)) return false;
+        load_w(i);
+        w = i + 1;
+        return true;
+      };
       for (int i = 0; i < n; ++i) {
-        const int s = i & 1;
+        // w's tile is free first in the state pass, last in the main pass
+        if (i >= 2 && !(STATE_ONLY ? more_w(i) && more_xy(i) : more_xy(i) && more_w(i))) break;
         if (i + kAhead < n) {
           const int t1 = start_of(i + kAhead);
 #pragma unroll
@@ -202,22 +215,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           tma_prefetch_4d(mw, c0, h, t1, b);
         }
-        if (i < 2) continue;  // (loaded above)
-        if (!mbar_wait(&bars.xy_empty[s], ((i >> 1) & 1) ^ 1, kErrWaitProducer, &abort_flag)) break;
-        load_xy(i);
-        issued = 2 * i + 1;
-        if (!mbar_wait(&bars.w_empty[s], ((i >> 1) & 1) ^ 1, kErrWaitProducer, &abort_flag)) break;
-        load_w(i);
-        issued = 2 * i + 2;
       }
       if (abort_flag) {  // a wait gave up: the copies in flight land before the shared memory is given back
-        for (int j = max(0, issued - 4); j < issued; ++j) {
-          const int i = j >> 1;
-          if (j & 1)
-            mbar_drain(&bars.w_full[i & 1], (i >> 1) & 1);
-          else
-            mbar_drain(&bars.xy_full[i & 1], (i >> 1) & 1);
-        }
+        for (int i = max(0, xy - 2); i < xy; ++i) mbar_drain(&bars.xy_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, w - 2); i < w; ++i) mbar_drain(&bars.w_full[i & 1], (i >> 1) & 1);
       }
     }
     __syncwarp();
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---------------------------------------------------------------- MMA issuer
     constexpr uint32_t id_sc = make_idesc_bf16(kC, kC, 0, 0);
     constexpr uint32_t id_o = make_idesc_bf16(kC, kSlice, 0, 1);
-    constexpr uint32_t id_kv = make_idesc_bf16(kC, kSlice, 1, 1);
+    constexpr uint32_t id_kv = make_idesc_bf16(kC, kSlice, 1, 1), id_kv2 = make_idesc_bf16(kC, 2 * kSlice, 1, 1);
     const uint32_t sb = smem_u32(smem);
     const uint32_t el = elect_lane();
     auto issue_o1 = [&](int j) -> bool {
@@ -267,19 +268,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      : !mbar_wait(&bars.s_ready, i & 1, kErrWaitMma, &abort_flag))
         break;
       tc_fence_after();
-      // W' part by part into one accumulator; rows of Y^T beyond DX = 64 read the next tile:
-      // lanes of KV that nobody looks at
-#pragma unroll
-      for (int part = 0; part < NS; ++part) {
-        const uint32_t hw = desc_lo(sb + (hb ? L::kOffH2 : L::kOffH) + part * kBox, kBox);
+      // rows of Y^T beyond DX = 64 read the next tile: lanes of KV that nobody looks at
+      const uint32_t hs = sb + (hb ? L::kOffH2 : L::kOffH);
+      if (STATE_ONLY) {
+        // the first two parts of W' side by side, the third on top of the second: half as many
+        // products as part by part, in columns that the main pass does not have
 #pragma unroll
         for (int k = 0; k < kC / 16; ++k)
-          umma_f16_e(el, tmem + (hb ? kColO1 : kColKv), ym + k * (2048 / 16), hw + k * (2048 / 16), id_kv, part > 0 || k > 0);
+          umma_f16_e(el, tmem + hb * 2 * kSlice, ym + k * (2048 / 16), desc_lo(hs, kBox) + k * (2048 / 16), id_kv2, k > 0);
+        if (NS == 3) {
+#pragma unroll
+          for (int k = 0; k < kC / 16; ++k)
+            umma_f16_e(el, tmem + hb * 2 * kSlice + kSlice, ym + k * (2048 / 16),
+                       desc_lo(hs + 2 * kBox, kBox) + k * (2048 / 16), id_kv, 1);
+        }
+      } else {
+#pragma unroll
+        for (int part = 0; part < NS; ++part) {
+          const uint32_t hw = desc_lo(hs + part * kBox, kBox);
+#pragma unroll
+          for (int k = 0; k < kC / 16; ++k)
+            umma_f16_e(el, tmem + kColKv, ym + k * (2048 / 16), hw + k * (2048 / 16), id_kv, part > 0 || k > 0);
+        }
       }
       umma_commit_e(el, &bars.kv_full[hb]);
-      if (STATE_ONLY) {
-        umma_commit_e(el, &bars.w_empty[i & 1]);
-      } else {
+      if (!STATE_ONLY) {
         // the outputs of chunk i-2 have left this O2 (and the O1 that O1(i) will write)
         if (i > 1 && !mbar_wait(&bars.o_free[s], ((i >> 1) - 1) & 1, kErrWaitMma, &abort_flag)) break;
         tc_fence_after();
@@ -485,8 +498,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int c = 0; c < kSlice; c += 16) {
             float v[16];
-            tmem_ld16(tmem + lanes + (hb ? kColO1 : kColKv) + c, v);
-            tmem_ld_wait();
+            if (STATE_ONLY) {
+              float u[16];
+              tmem_ld16(tmem + lanes + hb * 2 * kSlice + c, v);
+              tmem_ld16(tmem + lanes + hb * 2 * kSlice + kSlice + c, u);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] += u[j];
+            } else {
+              tmem_ld16(tmem + lanes + kColKv + c, v);
+              tmem_ld_wait();
+            }
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {  // decay_add of pairs
               const float2 s2 = make_float2(S[c + j], S[c + j + 1]);
@@ -601,7 +623,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.h_ready[hb]);
+        if (lane == 0) {
+          mbar_arrive(&bars.h_ready[hb]);
+          if (STATE_ONLY) mbar_arrive(&bars.w_empty[sw]);
+        }
       }
     }
   }
