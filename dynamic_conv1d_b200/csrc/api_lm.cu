@@ -263,10 +263,7 @@ int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t
 size_t dynconv_vocab_loss_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int want_dhidden,
                                               int want_dweight) {
   if (check_loss(N, D, V, 0, dtype) || N == 0) return 0;
-  // alignment can move a call to the CUDA-core path: enough for either
-  const size_t a = loss_backward_bytes(vl::plan(N, D, V, dtype, false), N, D, dtype, want_dhidden, want_dweight).total();
-  const size_t b = loss_backward_bytes(vl::plan(N, D, V, dtype, true), N, D, dtype, want_dhidden, want_dweight).total();
-  return a > b ? a : b;
+  return loss_backward_bytes(vl::plan(N, D, V, dtype), N, D, dtype, want_dhidden, want_dweight).total();
 }
 
 int dynconv_vocab_loss_bwd(const void* hidden, const void* weight, const int64_t* target, const float* lse,
@@ -292,7 +289,7 @@ int dynconv_vocab_loss_bwd(const void* hidden, const void* weight, const int64_t
   p.dhidden = dhidden, p.dweight = dweight, p.st = st;
   p.piece = workspace;
   const bool tc = vl::tc_supported(p, dtype);
-  const vl::Plan pl = vl::plan(N, D, V, dtype, tc);
+  const vl::Plan pl = vl::plan(N, D, V, dtype);
   const LossBackwardBytes b = loss_backward_bytes(pl, N, D, dtype, dhidden != nullptr, dweight != nullptr);
   if (!workspace || workspace_bytes < b.total())
     return set_error(DYNCONV_ERR_WORKSPACE, "vocab_loss_bwd: workspace %zu < %zu bytes", workspace_bytes, b.total());

@@ -369,7 +369,10 @@ int total_launch(const Problem& p) {
 // counted in blocks of 64 inner elements of a tile, 0.46 us each on the tensor cores.
 // Where a product has few tiles its inner dimension is spread over several CTAs, each share at
 // least 512 elements (128 on the CUDA cores, where they take as long).
-Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc) {
+// The cut rests on sizes and type alone, so that a workspace asked for by size fits every call of
+// that size: tensors whose alignment keeps them from the tensor cores are cut the same way.
+Plan plan(int64_t N, int64_t D, int64_t V, int dtype) {
+  const bool tc = dtype == DYNCONV_DTYPE_BF16 && D % 8 == 0;
   const int64_t elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4, sms = tc ? sm_count() / 2 : sm_count();
   const int64_t tm = tc ? 256 : 128, tn = tc ? 256 : 128;
   const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
@@ -392,7 +395,7 @@ Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc) {
   if (most < 1024) most = 1024;
   Plan best{};
   double best_cost = 1e300;
-  const int64_t step = up(up(V, 128), 256) * 256;  // at most about 128 candidates
+  const int64_t step = up(up(V, 32), 256) * 256;  // at most about 32 candidates (0.4 us of host time each)
   for (int64_t cols = most < V ? most : up(V, 256) * 256; cols > 0; cols -= step) {
     const int64_t full = V / cols, rest = V - full * cols;
     const int z_h = share(n_tiles * d_tiles, cols < V ? cols : V), z_w = share(up(cols < V ? cols : V, tm) * d_tiles, N);

@@ -74,7 +74,7 @@ __device__ __forceinline__ float result_factor(const Problem& p) {
 constexpr int64_t kRowsAtOnce = 32768;
 constexpr int kNarrowestTile = 64;  // columns of the vocabulary in one forward tile, at least
 bool tc_supported(const Problem& p, int dtype);
-Plan plan(int64_t N, int64_t D, int64_t V, int dtype, bool tc);
+Plan plan(int64_t N, int64_t D, int64_t V, int dtype);
 int merge_launch(const Problem& rows, int64_t tiles);  // the rows' losses from their tiles
 int total_launch(const Problem& p);                    // their sum and number
 // The part of a forward problem that begins at row r0.

@@ -122,6 +122,14 @@ def test_long_inner_dimensions():
     check(*make(6000, 64, 100, torch.bfloat16))
 
 
+def test_unaligned_tensors():
+    """Views that TMA cannot address take the CUDA-core products, cut the same way."""
+    N, D, V = 200, 64, 500
+    h, w, t = make(N, D, V, torch.bfloat16)
+    shift = lambda x: torch.cat([x.new_zeros(1), x.flatten()])[1:].view(x.shape)  # noqa: E731
+    check(shift(h), shift(w), t)
+
+
 def test_channels_beyond_one_chain():
     """More than 2048 products in a logit: summed in parts (bf16)."""
     for D in (2056, 4096, 5000):
