@@ -75,6 +75,14 @@ __device__ __forceinline__ uint32_t out_off(int r, int c) {
   return (uint32_t)r * 64u + (uint32_t)((c ^ ((r >> 1) & 3)) << 4);
 }
 
+// Lane by lane max(a, |b|) of two bf16 pairs; NaN if either is.
+__device__ __forceinline__ uint32_t max_abs_nan(uint32_t a, uint32_t b) {
+  uint32_t m, d;
+  asm("abs.bf16x2 %0, %1;" : "=r"(m) : "r"(b));
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(m));
+  return d;
+}
+
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
 
@@ -588,7 +596,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (left < kC) f = a < left ? ro.w_scale * pw[left - e - a] : 0.f;
         uint8_t* src = smem + L::kOffW + sw * kBox;
         uint8_t* dst = smem + (hb ? L::kOffH2 : L::kOffH);
-        uint32_t odd = 0;
+        uint32_t largest = 0;  // magnitudes of the even and the odd columns, NaN above all
 #pragma unroll 4
         for (int c = 0; c < 8; ++c) {
           const uint32_t at = sw_off(row, c);
@@ -597,19 +605,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           uint32_t part[NS][4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            odd |= (w[j] & 0x7F807F80u) + 0x00800080u;  // an exponent of all ones carries into the sign
+            largest = max_abs_nan(largest, w[j]);
             float2 x = mul2(make_float2(bf_lo(w[j]), bf_hi(w[j])), make_float2(f, f));
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
               part[s][j] = pack_bf16x2(x.x, x.y);
-              if (s + 1 < NS) x = add2(x, make_float2(-bf_lo(part[s][j]), -bf_hi(part[s][j])));
+              if (s + 1 < NS) x = fma2(make_float2(bf_lo(part[s][j]), bf_hi(part[s][j])), make_float2(-1.f, -1.f), x);
             }
           }
 #pragma unroll
           for (int s = 0; s < NS; ++s)
             *reinterpret_cast<uint4*>(dst + s * kBox + at) = make_uint4(part[s][0], part[s][1], part[s][2], part[s][3]);
         }
-        if (!STATE_ONLY && (odd & 0x80008000u)) {
+        if (!STATE_ONLY && ((largest & 0x7F80u) == 0x7F80u || (largest & 0x7F800000u) == 0x7F800000u)) {
           // the tile keeps zeros where a value was not finite; rows that may see it become NaN
           __nv_bfloat16* wr = reinterpret_cast<__nv_bfloat16*>(src);
           for (int c = 0; c < kSlice; ++c) {
