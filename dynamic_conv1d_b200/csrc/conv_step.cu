@@ -9,9 +9,14 @@
 // `row` is b, or slots[b] when the rows' caches lie in a pool; a slot outside the pool
 // leaves every cache alone and its output row is zero.
 //
-// A thread owns VEC neighbouring channels of RB batch rows: it alone reads and rewrites
-// their cache, so the update in place needs no barrier.  Everything accumulates in
-// fp32 and each output is rounded once.
+// A thread owns neighbouring channels of its batch rows: it alone reads and rewrites their
+// cache, so the update in place needs no barrier (the few-rows kernel reads all of it before
+// one).  Everything accumulates in fp32 and each output is rounded once.
+//
+// Measured (B200, graph replay): one row of 3 x 2048 channels at rank 15 2.3 us, a launch's time; 512
+// such rows 9.2 us; 256 rows of 3 x 4096 at rank 31 13.9 us with the tensors in L2 and 19.5 us
+// from HBM, where their 53 MB take 8.2 us: bound by the latency of a block's phases (slots, then
+// caches; U's tile; products; stores) at 24 warps per SM.  Headwise, 64 rows of 2048: 2.5 us.
 #include "common.cuh"
 
 namespace dynconv {
@@ -137,8 +142,8 @@ __global__ void __launch_bounds__(kThreads) lr_step_kernel(const T* __restrict__
                             residual);
 }
 
-// Few rows: the time is the latency of the loads, so each warp takes one tap and all its ranks'
-// loads are in flight at once; the taps' products meet in shared memory.  Block: W warps of 32
+// Few rows outside the tensor-core form: the time is the latency of the loads, so each warp takes one
+// tap and all its ranks' loads are in flight at once; the taps' products meet in shared memory.  Block: W warps of 32
 // channel vectors, one batch row.
 template <typename T, int W, int VEC>
 __global__ void __launch_bounds__(32 * W) lr_step_few_kernel(const T* __restrict__ x, const T* __restrict__ z,
@@ -200,15 +205,18 @@ __global__ void __launch_bounds__(32 * W) lr_step_few_kernel(const T* __restrict
   store_vec<T, VEC>(y + b * C + c, out);
 }
 
-// bf16, many rows: the taps are a small matrix product (rows x ranks by ranks x channels), 2 R
-// operations for each byte of the batch: on the CUDA cores 53 us for 256 rows of 3 x 4096
-// channels at R = 31, so it goes to the tensor cores.  mma.sync is the fitting form here: a
-// warp's 16 x 32 outputs are consumed in registers by the convolution itself, K is R <= 64, and
-// the kernel is bound by the batch's bytes, not by the product.
+// bf16, W <= 4, whole 16-byte groups of channels: the taps are a small matrix product (rows x ranks
+// by ranks x channels), 2 R operations for each byte of the batch: on the CUDA cores 53 us for
+// 256 rows of 3 x 4096 channels at R = 31, so it goes to the tensor cores.  mma.sync is the
+// fitting form here: a warp's 16 x 32 outputs are consumed in registers by the convolution
+// itself, K is R <= 64, and the tensor pipe is 10% busy.  One row takes no longer than in the
+// few-rows form (2.3 against 2.5 us), so every batch goes this way.
 //
 // Block: 32 channels of one group, four warps with 16 rows each, U's tile staged once for 64
-// rows, the static filter in it as one more rank whose z is one.  Channels are staged permuted, so that a thread's four column pairs are eight
-// neighbouring channels: one 16-byte access per row and tensor.
+// rows, the static filter in it as one more rank whose z is one.  Channels are staged
+// permuted, so that a thread's four column pairs are eight neighbouring channels: one
+// 16-byte access per row and tensor.  (64 channels and 128 or 256 rows per block measured
+// 10 to 25% longer.)
 constexpr int kMmaRows = 64, kMmaCh = 32, kMmaThreads = 128;
 
 __device__ __forceinline__ void mma_16n8k16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {

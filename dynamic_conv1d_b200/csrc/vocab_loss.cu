@@ -1,6 +1,11 @@
 // vocab_loss.cu -- the vocabulary loss on the CUDA cores: tiled fp32 products for fp32
 // tensors and for bf16 shapes outside the tensor-core envelope, and the kernel that merges
 // the forward's tiles.  The formulas stand in vocab_loss.cuh.
+//
+// What bounds the products: the fp32 units, and tiles that do not divide the SMs.  1021 tokens x 256
+// channels over 4999 words in fp32 (B200): 90 us for each of the two logits' products (320 tiles
+// of 128 x 128, 296 at a time), 80 us for each gradient: 29 to 33 TFLOP/s where the units could
+// do 72.
 #include "vocab_loss.cuh"
 
 namespace dynconv {

@@ -18,6 +18,12 @@
 // Each CTA runs one producer warp (TMA ring of kStages) and eight epilogue warps (two per TMEM
 // lane quarter, half of the columns each); the pair's first CTA issues the products.  Two
 // accumulators of 256 TMEM columns let a tile's epilogue run under the next tile's products.
+//
+// What bounds it: the tensor cores at the clock that the power limit leaves (pipe 88 to 92% active).
+// 16384 tokens x 2048 channels over 50001 words (B200, bf16): forward 2.2 ms, logits again 2.3,
+// weight gradient 2.15, hidden gradient 2.1 ms: 1.5 PFLOP/s each, 94% of a library product's
+// burst rate; back to back under the power limit the pass takes 10.6 ms (1.27 PFLOP/s; that
+// library product sustains 1.38).
 #include "vocab_loss.cuh"
 
 namespace dynconv {

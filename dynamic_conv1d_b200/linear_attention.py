@@ -139,15 +139,15 @@ class _FusedDecayLinearAttentionFn(torch.autograd.Function):
         return dqkv, None, ds0, None, None
 
 
-def _check_decay(log_decay, H):
-    assert log_decay.is_cuda and log_decay.is_contiguous() and log_decay.dtype == torch.float32
+def _check_decay(log_decay, dev, H):
+    assert log_decay.get_device() == dev and log_decay.is_contiguous() and log_decay.dtype == torch.float32
     assert log_decay.shape == (H,)
     assert not log_decay.requires_grad, "the decay is a constant of each head: it has no gradient"
 
 
-def _check_state(state, rows, H, dk, dv):
+def _check_state(state, dev, rows, H, dk, dv):
     """Rows of a state."""
-    assert state.is_cuda and state.is_contiguous() and state.dtype == torch.float32 and state.dim() == 4
+    assert state.get_device() == dev and state.is_contiguous() and state.dtype == torch.float32 and state.dim() == 4
     n, h, a, b = state.shape
     assert h == H and a == dk and b == dv, f"state must be [n, {H}, {dk}, {dv}]"
     assert rows is None or n == rows
@@ -178,13 +178,14 @@ def decay_linear_attention(
     Returns:
         o [B, T, H, dv], or (o, state).  Differentiable in q, k, v and initial_state.
     """
-    assert q.is_cuda and k.is_cuda and v.is_cuda
+    dev = q.get_device()  # (-1 on the CPU)
+    assert dev >= 0 and k.get_device() == dev and v.get_device() == dev
     assert q.dim() == 4 and k.shape == q.shape and v.shape[:3] == q.shape[:3] and v.dim() == 4
     assert q.dtype == k.dtype == v.dtype
     _, _, H, dk = q.shape
-    _check_decay(log_decay, H)
+    _check_decay(log_decay, dev, H)
     if initial_state is not None:
-        _check_state(initial_state, q.shape[0], H, dk, v.shape[-1])
+        _check_state(initial_state, dev, q.shape[0], H, dk, v.shape[-1])
     scale = dk**-0.5 if scale is None else float(scale)
     o, s1 = _DecayLinearAttentionFn.apply(q, k, v, log_decay, initial_state, scale, bool(return_state))
     return (o, s1) if return_state else o
@@ -201,13 +202,14 @@ def decay_linear_attention_fused(
     ``QKVLowRankDynamicShortConvolution.forward_fused`` returns them, with H = len(log_decay).
     Returns o [B, T, H*d] (or (o, state)); the gradient comes back as one [B, T, 3*H*d]
     tensor, with no split or concatenation on either way."""
-    assert qkv.is_cuda and qkv.is_contiguous() and qkv.dim() == 3
+    dev = qkv.get_device()
+    assert dev >= 0 and qkv.is_contiguous() and qkv.dim() == 3
     H = log_decay.shape[0]
     assert qkv.shape[-1] % (3 * H) == 0, "qkv must be [B, T, 3*H*d]"
     d = qkv.shape[-1] // (3 * H)
-    _check_decay(log_decay, H)
+    _check_decay(log_decay, dev, H)
     if initial_state is not None:
-        _check_state(initial_state, qkv.shape[0], H, d, d)
+        _check_state(initial_state, dev, qkv.shape[0], H, d, d)
     scale = d**-0.5 if scale is None else float(scale)
     o, s1 = _FusedDecayLinearAttentionFn.apply(qkv, log_decay, initial_state, scale, bool(return_state))
     return (o, s1) if return_state else o
@@ -233,13 +235,14 @@ def decay_linear_attention_step(
     Returns:
         o: [B, H, dv].  Has no gradient.
     """
-    assert q.is_cuda and k.is_cuda and v.is_cuda
+    dev = q.get_device()
+    assert dev >= 0 and k.get_device() == dev and v.get_device() == dev
     assert q.dim() == 3 and k.shape == q.shape and v.dim() == 3 and v.shape[:2] == q.shape[:2]
     assert q.dtype == k.dtype == v.dtype
     B, H, dk = q.shape
     dv = v.shape[-1]
-    _check_decay(log_decay, H)
-    n = _check_state(state, None, H, dk, dv)
+    _check_decay(log_decay, dev, H)
+    n = _check_state(state, dev, None, H, dk, dv)
     assert slots is not None or n >= B
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         _refuse_gradient()
@@ -248,7 +251,7 @@ def decay_linear_attention_step(
     if (qd != 1 and dk > 1) or (kd != 1 and dk > 1) or (vd != 1 and dv > 1):
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
         (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
-    sp, sb = (None, 0) if slots is None else _slots(slots, B)
+    sp, sb = (None, 0) if slots is None else _slots(slots, B, dev)
     o = torch.empty((B, H, dv), device=q.device, dtype=q.dtype)
     with _lib.device_of(q):
         status = _lib.load().dynconv_la_step(

@@ -21,9 +21,9 @@ def _refuse_gradient():
     raise RuntimeError("a single-token step has no gradient: call it under torch.no_grad()")
 
 
-def _slots(slots: torch.Tensor | None, B: int):
-    """(pointer, bytes of an index) of a slot table."""
-    assert slots.is_cuda and slots.is_contiguous() and slots.shape == (B,)
+def _slots(slots: torch.Tensor, B: int, dev: int):
+    """(pointer, bytes of an index) of a slot table on device `dev`."""
+    assert slots.get_device() == dev and slots.is_contiguous() and slots.shape == (B,)
     assert slots.dtype in (torch.int32, torch.int64), "slots must be int32 or int64"
     return slots.data_ptr(), slots.element_size()
 
@@ -82,9 +82,9 @@ def lowrank_dynamic_convolution_step(
     return _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, 1)
 
 
-def _check_cache(cache, dtype, B, W, C, slots):
+def _check_cache(cache, dev, dtype, B, W, C, slots):
     """Rows of the cache."""
-    assert cache.is_cuda and cache.is_contiguous() and cache.dtype == dtype and cache.dim() == 3
+    assert cache.get_device() == dev and cache.is_contiguous() and cache.dtype == dtype and cache.dim() == 3
     n, rows, channels = cache.shape
     assert rows == W - 1 and channels == C, f"cache must be [n, {W - 1}, {C}]"
     assert slots is not None or n >= B
@@ -92,18 +92,19 @@ def _check_cache(cache, dtype, B, W, C, slots):
 
 
 def _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, G):
-    assert x.is_cuda and x.is_contiguous() and x.dim() == 2
-    assert z.is_cuda and z.is_contiguous()
-    assert U.is_cuda and U.is_contiguous()
+    dev = x.get_device()  # (-1 on the CPU)
+    assert dev >= 0 and x.is_contiguous() and x.dim() == 2
+    assert z.get_device() == dev and z.is_contiguous()
+    assert U.get_device() == dev and U.is_contiguous()
     B, C = x.shape
     D = C // G
     assert D * G == C and z.shape == (B, G * R)
     W = WD // D
     assert W * D == WD, "U must be [G, R, W*D]"
     dtype = x.dtype
-    n = _check_cache(cache, dtype, B, W, C, slots)
+    n = _check_cache(cache, dev, dtype, B, W, C, slots)
     if static_w is not None:
-        assert static_w.is_cuda and static_w.is_contiguous()
+        assert static_w.get_device() == dev and static_w.is_contiguous()
         assert static_w.shape == ((W, D) if U.dim() == 2 else (G, W, D))
         if static_w.dtype != dtype:
             static_w = static_w.to(dtype)
@@ -116,7 +117,7 @@ def _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, G):
         z = z.to(dtype)
     if U.dtype != dtype:
         U = U.to(dtype)
-    sp, sb = (None, 0) if slots is None else _slots(slots, B)
+    sp, sb = (None, 0) if slots is None else _slots(slots, B, dev)
     y = torch.empty_like(x)
     with _lib.device_of(x):
         status = _lib.load().dynconv_lr_step(
@@ -139,15 +140,16 @@ def headwise_dynamic_convolution_step(
     """One token of ``headwise_dynamic_convolution``: x [B, D], weight [B, H, W],
     static_w [W, D], cache [n, W-1, D] (updated in place), slots as for
     ``lowrank_dynamic_convolution_grouped_step``.  Returns y [B, D]."""
-    assert x.is_cuda and x.is_contiguous() and x.dim() == 2
-    assert weight.is_cuda and weight.dim() == 3 and weight.shape[0] == x.shape[0]
+    dev = x.get_device()
+    assert dev >= 0 and x.is_contiguous() and x.dim() == 2
+    assert weight.get_device() == dev and weight.dim() == 3 and weight.shape[0] == x.shape[0]
     B, D = x.shape
     H, W = weight.shape[1:]
     assert D % H == 0, f"D={D} must be divisible by H={H}"
     dtype = x.dtype
-    n = _check_cache(cache, dtype, B, W, D, slots)
+    n = _check_cache(cache, dev, dtype, B, W, D, slots)
     if static_w is not None:
-        assert static_w.is_cuda and static_w.is_contiguous()
+        assert static_w.get_device() == dev and static_w.is_contiguous()
         assert static_w.dtype == dtype
         assert static_w.shape == (W, D)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
@@ -156,7 +158,7 @@ def headwise_dynamic_convolution_step(
     code = _lib.dtype_code(dtype)
     if weight.dtype != dtype or not weight.is_contiguous():
         weight = weight.to(dtype=dtype).contiguous()
-    sp, sb = (None, 0) if slots is None else _slots(slots, B)
+    sp, sb = (None, 0) if slots is None else _slots(slots, B, dev)
     y = torch.empty_like(x)
     with _lib.device_of(x):
         status = _lib.load().dynconv_hw_step(

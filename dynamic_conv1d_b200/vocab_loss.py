@@ -90,9 +90,9 @@ def linear_cross_entropy(
         are this rank's own, as for any other parameter of the model around the ops.
     """
     assert hidden.is_cuda and hidden.is_contiguous()
-    assert weight.is_cuda and weight.is_contiguous() and weight.dim() == 2
+    assert weight.device == hidden.device and weight.is_contiguous() and weight.dim() == 2
     assert weight.shape[1] == hidden.shape[-1]
-    assert target.is_cuda and target.dtype == torch.int64 and target.shape == hidden.shape[:-1]
+    assert target.device == hidden.device and target.dtype == torch.int64 and target.shape == hidden.shape[:-1]
     assert reduction in _REDUCTIONS, f"reduction must be one of {tuple(_REDUCTIONS)}"
     loss = _LinearCrossEntropyFn.apply(
         hidden.view(-1, hidden.shape[-1]), weight, target.reshape(-1).contiguous(), int(ignore_index),
