@@ -237,7 +237,7 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
 }
 
 template <int W, int KS>
-__global__ void __launch_bounds__(kMmaThreads, 6) lr_step_mma_kernel(const __nv_bfloat16* __restrict__ x,
+__global__ void __launch_bounds__(kMmaThreads, KS == 1 ? 6 : 5) lr_step_mma_kernel(const __nv_bfloat16* __restrict__ x,
                                                           const __nv_bfloat16* __restrict__ z,
                                                           const __nv_bfloat16* __restrict__ U,
                                                           const __nv_bfloat16* __restrict__ sw, __nv_bfloat16* cache,
@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(kMmaThreads, 6) lr_step_mma_kernel(const __nv_
   // Row pitch 40 words: the four k rows that a fragment load touches lie 8 banks apart.
   constexpr int kPitch = 40, K2 = KS * 8;
   __shared__ uint32_t us[W * K2 * kPitch];  // at most 25 KB
+  __shared__ uint32_t zs[4][KS == 1 ? 1 : 16][K2 + 4];  // each warp's rows of z (pitch: 8 rows meet no bank twice)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t C = (int64_t)G * D;
   const int64_t per = (D + kMmaCh - 1) / kMmaCh;
@@ -273,28 +274,44 @@ __global__ void __launch_bounds__(kMmaThreads, 6) lr_step_mma_kernel(const __nv_
 #pragma unroll
     for (int w = 1; w < W; ++w) past[hf][w] = *reinterpret_cast<const uint4*>(cr + (int64_t)(W - 1 - w) * C);
   }
-  // z's fragments; rank R is the static filter's, with a z of one
+  // z; rank R is the static filter's, with a z of one.  Up to 16 ranks a thread loads its fragment's
+  // elements itself; above, a lane takes a rank of each of the warp's rows (whole lines) and the
+  // fragments come out of shared memory (256 rows, 3 x 4096 channels, rank 31: 18.7 against
+  // 20.4 us; at rank 15, 3 x 2048 channels, 7.5 against 5.6).
+  constexpr bool kDirect = KS == 1;
+  constexpr int kHalves = (KS + 1) / 2;
+  const uint16_t one = sw ? 0x3F80 : 0;
   uint32_t a[KS][4];
-  {
+  uint16_t zv[kDirect ? 1 : 16][kHalves];
+  if constexpr (kDirect) {
     const uint16_t* zr = reinterpret_cast<const uint16_t*>(z) + ((b0 + r0) * G + g) * R;
     const int64_t eight = (int64_t)8 * G * R;
     const bool there[2] = {b0 + r0 < B, b0 + r0 + 8 < B};
-    const uint32_t one = sw ? 0x3F80u : 0u;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int i = 0; i < 4; ++i) {
+      const int k = q * 2 + (i >> 1) * 8;
+      const uint16_t* at = zr + (i & 1) * eight + k;
+      uint32_t lo = k == R ? one : 0, hi = k + 1 == R ? one : 0;
+      if (there[i & 1] && k < R) lo = at[0];
+      if (there[i & 1] && k + 1 < R) hi = at[1];
+      a[0][i] = lo | (hi << 16);
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = ks * 16 + q * 2 + (i >> 1) * 8;
-        const uint16_t* at = zr + (i & 1) * eight + k;
-        uint32_t lo = k == R ? one : 0u, hi = k + 1 == R ? one : 0u;
-        if (there[i & 1] && k < R) lo = at[0];
-        if (there[i & 1] && k + 1 < R) hi = at[1];
-        a[ks][i] = lo | (hi << 16);
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const int k = h * 32 + lane;
+        zv[r][h] = k == R ? one : 0;
+        if (b0 + r < B && k < R) zv[r][h] = reinterpret_cast<const uint16_t*>(z)[((b0 + r) * G + g) * R + k];
       }
   }
   // stage U: a thread takes 8 channels of a rank pair; position of channel c in the tile:
   // column pair j = (c % 8) / 2 of thread c / 8 is column 2 (c / 8) + c % 2 of product j
-  for (int i = threadIdx.x; i < W * K2 * 4; i += kMmaThreads) {
+#pragma unroll
+  for (int n = 0; n < (W * K2 * 4 + kMmaThreads - 1) / kMmaThreads; ++n) {
+    const int i = threadIdx.x + n * kMmaThreads;
+    if (W * K2 * 4 % kMmaThreads != 0 && i >= W * K2 * 4) break;
     const int oct = i & 3, rest = i >> 2, k2 = rest % K2, w = rest / K2;
     const int64_t du = d0 + oct * 8;
     uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
@@ -312,8 +329,21 @@ __global__ void __launch_bounds__(kMmaThreads, 6) lr_step_mma_kernel(const __nv_
       dst[j * 8 + 1] = __byte_perm(l[j], h[j], 0x7632);
     }
   }
+  if constexpr (!kDirect) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+        if (h * 32 + lane < KS * 16) reinterpret_cast<uint16_t*>(zs[warp][r])[h * 32 + lane] = zv[r][h];
+  }
   __syncthreads();
   if (b0 >= B) return;  // (whole warps: all lanes take part in the products, channels there or not)
+  if constexpr (!kDirect) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[ks][i] = zs[warp][r0 + (i & 1) * 8][ks * 8 + (i >> 1) * 4 + q];
+  }
   float out[2][8];
 #pragma unroll
   for (int hf = 0; hf < 2; ++hf) {
