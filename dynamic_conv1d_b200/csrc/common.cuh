@@ -377,15 +377,6 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
       : "memory");
 }
 
-// TMA tiled 2-D load into shared memory, completion counted on `bar`.
-__device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::
-          "r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
-      : "memory");
-}
-
 // Brings a TMA tile into L2 ahead of its load.
 __device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {
   asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
@@ -634,16 +625,11 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// 128-byte-swizzled K-major operand (TMA box of 64 K elements, so rows of 128 bytes and
-// 8-row groups of 1024): a K step of 16 elements advances the start address by 32 bytes.
-__device__ __forceinline__ uint64_t make_smem_desc_sw128_k(uint32_t smem_addr) {
-  return make_smem_desc_sw128(smem_addr, 16, 1024);
-}
-
-// High word of the two descriptors above (stride between 8-row groups 1024, sm_100 version,
-// 128-byte swizzle); the low word holds the start address and, for MN-major operands, the stride
-// between 64-element atoms, both in units of 16 bytes.  Products of one operand tile differ
-// in the low word only, by a constant.
+// 128-byte-swizzled descriptors in two words.  High word: stride between 8-row groups 1024, sm_100
+// version, 128-byte swizzle.  Low word: the start address and, for MN-major operands, the
+// stride between 64-element atoms (make_smem_desc_sw128), both in units of 16 bytes.  K-major
+// operands (TMA boxes of 64 K elements) advance by 32 bytes for a K step of 16, MN-major ones
+// by 2048: products of one tile differ in the low word only, by a constant.
 constexpr uint32_t kDescHiSw128 = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr, uint32_t lbo = 16) {
   return (smem_addr >> 4) | ((lbo >> 4) << 16);
