@@ -14,9 +14,9 @@
 // one).  Everything accumulates in fp32 and each output is rounded once.
 //
 // Measured (B200, graph replay): one row of 3 x 2048 channels at rank 15 2.3 us, a launch's time; 512
-// such rows 9.2 us; 256 rows of 3 x 4096 at rank 31 13.9 us with the tensors in L2 and 19.5 us
+// such rows 9.2 us; 256 rows of 3 x 4096 at rank 31 13.4 us with the tensors in L2 and 18.5 us
 // from HBM, where their 53 MB take 8.2 us: bound by the latency of a block's phases (slots, then
-// caches; U's tile; products; stores) at 24 warps per SM.  Headwise, 64 rows of 2048: 2.5 us.
+// caches; U's tile; products; stores) at 20 warps per SM.  Headwise, 64 rows of 2048: 2.5 us.
 #include "common.cuh"
 
 namespace dynconv {
