@@ -1,11 +1,12 @@
-// vocab_loss.cu -- the vocabulary loss on the CUDA cores: tiled fp32 products for fp32
-// tensors and for bf16 shapes outside the tensor-core envelope, and the kernel that merges
-// the forward's tiles.  The formulas stand in vocab_loss.cuh.
+// vocab_loss.cu -- the vocabulary loss on the CUDA cores: tiled fp32 products for bf16 tensors that
+// TMA cannot address (a width that is no multiple of 8, a base off 16 bytes), the kernels that
+// merge the forward's tiles and join partial sums, and the cut of both paths' work.  The
+// formulas stand in vocab_loss.cuh.
 //
-// What bounds the products: the fp32 units, and tiles that do not divide the SMs.  1021 tokens x 256
-// channels over 4999 words in fp32 (B200): 90 us for each of the two logits' products (320 tiles
-// of 128 x 128, 296 at a time), 80 us for each gradient: 29 to 33 TFLOP/s where the units could
-// do 72.
+// What bounds the products: the fp32 units, and tiles that do not divide the SMs.  1021 tokens x 257
+// channels over 4999 words in bf16 (B200): 93 and 97 us for the two logits' products (320 tiles
+// of 128 x 128, 296 at a time), 100 and 120 us for the gradients: 22 to 28 TFLOP/s where the units
+// could do 72.
 #include "vocab_loss.cuh"
 
 namespace dynconv {
@@ -15,6 +16,7 @@ namespace {
 
 constexpr int kK = 8;       // inner steps staged at once (16 take more registers and 5% longer)
 constexpr int kThreads = 256;
+using T = __nv_bfloat16;
 
 enum Mode { kForward, kGrad, kAccumulate, kStore };
 
@@ -33,7 +35,7 @@ struct Gemm {
 // One thread's share of TILE rows x kK inner steps: fetched into registers while the stage
 // before is multiplied, then put down transposed, [k][row].  Threads follow the dense
 // dimension, so that loads coalesce either way.
-template <typename T, int TILE>
+template <int TILE>
 struct Stage {
   static constexpr int kPer = TILE * kK / kThreads;
   const T* at;        // this thread's first element of the current step
@@ -72,7 +74,7 @@ struct Stage {
 // R x R outputs per thread in groups of four rows and columns, products in packed pairs.
 // R = 8: 128 x 128 tiles, 4 bytes of shared memory read for each two multiply-adds; R = 4: 64 x 64
 // tiles, for few rows or too few tiles.
-template <typename T, int MODE, int R>
+template <int MODE, int R>
 __global__ void __launch_bounds__(kThreads, 2) vl_gemm_kernel(const Gemm g, const Problem p) {
   constexpr int TILE = 16 * R, LD = TILE + 4, Q = R / 4;
   __shared__ __align__(16) float as[2][kK * LD], bs[2][kK * LD];
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, 2) vl_gemm_kernel(const Gemm g, cons
   const int64_t k_begin = blockIdx.z * g.k_share, k_end = min(g.K, k_begin + g.k_share);
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   float2 acc2[R][R / 2] = {};
-  Stage<T, TILE> a_next((const T*)g.A, g.am, g.ak, m0, g.M, k_begin), b_next((const T*)g.B, g.bn, g.bk, n0, g.N, k_begin);
+  Stage<TILE> a_next((const T*)g.A, g.am, g.ak, m0, g.M, k_begin), b_next((const T*)g.B, g.bn, g.bk, n0, g.N, k_begin);
   int left = (int)(k_end - k_begin), buf = 0;  // (a share beyond the end has none)
   a_next.fetch(left);
   b_next.fetch(left);
@@ -173,20 +175,20 @@ bool large_tiles(int64_t M, int64_t N, int64_t z) {
   return M >= 96 && N >= 96 && ((M + 127) / 128) * ((N + 127) / 128) * z >= sm_count() / 2;
 }
 
-template <typename T, int MODE, int R>
+template <int MODE, int R>
 int gemm_tiles(const Gemm& g, const Problem& p, int z, const char* what) {
   constexpr int TILE = 16 * R;
   const int64_t gx = (g.M + TILE - 1) / TILE, gy = (g.N + TILE - 1) / TILE;
   if (gx > INT32_MAX || gy > 65535) return set_error(DYNCONV_ERR_SHAPE, "%s: too many tiles", what);
-  vl_gemm_kernel<T, MODE, R><<<dim3((unsigned)gx, (unsigned)gy, (unsigned)z), kThreads, 0, p.st>>>(g, p);
+  vl_gemm_kernel<MODE, R><<<dim3((unsigned)gx, (unsigned)gy, (unsigned)z), kThreads, 0, p.st>>>(g, p);
   DYNCONV_CHECK_LAUNCH(what);
   return DYNCONV_OK;
 }
 
-template <typename T, int MODE>
+template <int MODE>
 int gemm(Gemm g, const Problem& p, int z, const char* what) {
   g.k_share = ((g.K + z - 1) / z + kK - 1) / kK * kK;
-  return large_tiles(g.M, g.N, z) ? gemm_tiles<T, MODE, 8>(g, p, z, what) : gemm_tiles<T, MODE, 4>(g, p, z, what);
+  return large_tiles(g.M, g.N, z) ? gemm_tiles<MODE, 8>(g, p, z, what) : gemm_tiles<MODE, 4>(g, p, z, what);
 }
 
 // Merges the tiles' (maximum, sum) of 32 rows per CTA: lane = row, warps take every eighth
@@ -260,64 +262,9 @@ __global__ void __launch_bounds__(1024) vl_total_kernel(const Problem p) {
   if (p.reduction == kMean) p.loss[0] = (float)(sum / (double)cnt);  // no row left: 0/0, NaN
 }
 
-template <typename T>
-int fwd(const Problem& all) {
-  int s;
-  for (int64_t r0 = 0; r0 < all.N; r0 += kRowsAtOnce) {
-    const Problem p = rows_from(all, r0, sizeof(T));
-    Gemm g{};
-    g.A = p.hidden, g.am = p.D, g.ak = 1;
-    g.B = p.weight, g.bn = p.D, g.bk = 1;
-    g.M = p.N, g.N = p.V, g.K = p.D;
-    if ((s = gemm<T, kForward>(g, p, 1, "vl_gemm_kernel (forward)"))) return s;
-    const int64_t tile = large_tiles(p.N, p.V, 1) ? 128 : 64;
-    if ((s = merge_launch(p, (p.V + tile - 1) / tile))) return s;
-  }
-  return total_launch(all);
-}
-
-template <typename T>
-int bwd(const Problem& p, const Plan& pl, int dtype) {
-  int s;
-  for (int64_t v0 = 0; v0 < p.V; v0 += pl.piece) {
-    const int64_t vp = p.V - v0 < pl.piece ? p.V - v0 : pl.piece;
-    const T* w = (const T*)p.weight + v0 * p.D;
-    Gemm g{};
-    g.A = p.hidden, g.am = p.D, g.ak = 1;
-    g.B = w, g.bn = p.D, g.bk = 1;
-    g.M = p.N, g.N = vp, g.K = p.D, g.col0 = v0;
-    g.out = p.piece, g.out_ld = pl.pitch;
-    if ((s = gemm<T, kGrad>(g, p, 1, "vl_gemm_kernel (logits' gradient)"))) return s;
-    if (p.dweight) {
-      Gemm gw{};
-      gw.A = p.piece, gw.am = 1, gw.ak = pl.pitch;
-      gw.B = p.hidden, gw.bn = 1, gw.bk = p.D;
-      gw.M = vp, gw.N = p.D, gw.K = p.N;
-      gw.out_ld = p.D;
-      if (pl.z_w == 1) {
-        gw.out = (T*)p.dweight + v0 * p.D;
-        if ((s = gemm<T, kStore>(gw, p, 1, "vl_gemm_kernel (weight gradient)"))) return s;
-      } else {
-        gw.out = p.acc_w;
-        if ((s = gemm<T, kAccumulate>(gw, p, pl.z_w, "vl_gemm_kernel (weight gradient)"))) return s;
-        if ((s = finish_launch(p, p.acc_w, pl.z_w, vp * p.D, (T*)p.dweight + v0 * p.D, dtype))) return s;
-      }
-    }
-    if (p.dhidden) {
-      Gemm gh{};
-      gh.A = p.piece, gh.am = pl.pitch, gh.ak = 1;
-      gh.B = w, gh.bn = 1, gh.bk = p.D;
-      gh.M = p.N, gh.N = p.D, gh.K = vp;
-      gh.out = p.acc_h, gh.out_ld = p.D, gh.add = v0 > 0;
-      if ((s = gemm<T, kAccumulate>(gh, p, pl.z_h, "vl_gemm_kernel (hidden gradient)"))) return s;
-    }
-  }
-  return p.dhidden ? finish_launch(p, p.acc_h, pl.z_h, p.N * p.D, p.dhidden, dtype) : DYNCONV_OK;
-}
-
-template <typename T>
+template <typename Out>
 __global__ void __launch_bounds__(256) vl_finish_kernel(const Problem p, const float* __restrict__ parts, int n_parts,
-                                                        int64_t n, T* __restrict__ out) {
+                                                        int64_t n, Out* __restrict__ out) {
   const float f = result_factor(p);
   const int64_t step = (int64_t)gridDim.x * blockDim.x;
   int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -337,7 +284,7 @@ __global__ void __launch_bounds__(256) vl_finish_kernel(const Problem p, const f
   for (; i < n; i += step) {
     float a = 0.f;
     for (int z = 0; z < n_parts; ++z) a += __ldg(parts + z * n + i);
-    out[i] = Elem<T>::from_f(a * f);
+    out[i] = Elem<Out>::from_f(a * f);
   }
 }
 
@@ -371,33 +318,40 @@ int total_launch(const Problem& p) {
 // within 512 MB: each product runs in rounds of one tile per SM or SM pair (weight-gradient tiles
 // are few and long: at 16384 x 2048 a width of 7168 columns makes 224 of them, three rounds of 74
 // and two tiles), each piece costs three launches and one pass over the fp32 sums of dhidden.  Times are
-// counted in blocks of 64 inner elements of a tile, 0.46 us each on the tensor cores.
+// counted in blocks of 64 inner elements of a tile, 0.46 us each on the tensor cores; an fp32
+// tensor's parts make six products of each block.
 // Where a product has few tiles its inner dimension is spread over several CTAs, each share at
-// least 512 elements (128 on the CUDA cores, where they take as long).
+// least 512 elements (one chain of 256 for fp32 tensors; 128 on the CUDA cores, where they take as
+// long).
 // The cut rests on sizes and type alone, so that a workspace asked for by size fits every call of
 // that size: tensors whose alignment keeps them from the tensor cores are cut the same way.
 Plan plan(int64_t N, int64_t D, int64_t V, int dtype) {
-  const bool tc = dtype == DYNCONV_DTYPE_BF16 && D % 8 == 0;
-  const int64_t elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4, sms = tc ? sm_count() / 2 : sm_count();
+  const bool split = dtype == DYNCONV_DTYPE_F32, tc = split || D % 8 == 0;
+  const int64_t elem = split ? 2 * kSplitParts : 2, sms = tc ? sm_count() / 2 : sm_count();
   const int64_t tm = tc ? 256 : 128, tn = tc ? 256 : 128;
   const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-  const int64_t least = tc ? 512 : 128;
+  const int64_t least = split ? 64 * kSplitChain : tc ? 512 : 128;
   const auto share = [&](int64_t tiles, int64_t inner) {
     int64_t z = 2 * sms / tiles;
     if (z > inner / least) z = inner / least;
     if (z > 16) z = 16;
     return (int)(z < 1 ? 1 : z);
   };
+  // blocks of a tile's inner dimension that one of z shares has
+  const auto inner = [&](int64_t n, int z) {
+    return split ? up(up(n, 64 * kSplitChain), z) * kSplitChain * kSplitProducts : up(up(n, 64), z);
+  };
   const double launch = 10, sums = 0.5 * (double)(N * D) * 8 / 6.5e12 / 0.46e-6;
   const int64_t n_tiles = up(N, tm), d_tiles = up(D, tn);
   const auto cost = [&](int64_t cols, int z_h, int z_w) {
-    const double logits = (double)(up(n_tiles * up(cols, tn), sms) * up(D, 64));
-    const double dw = (double)(up(up(cols, tm) * d_tiles * z_w, sms) * up(up(N, 64), z_w));
-    const double dh = (double)(up(n_tiles * d_tiles * z_h, sms) * up(up(cols, 64), z_h));
-    return logits + dw + dh + 3 * launch + sums * z_h;
+    const double logits = (double)(up(n_tiles * up(cols, tn), sms) * inner(D, 1));
+    const double dw = (double)(up(up(cols, tm) * d_tiles * z_w, sms) * inner(N, z_w));
+    const double dh = (double)(up(n_tiles * d_tiles * z_h, sms) * inner(cols, z_h));
+    return logits + dw + dh + (split ? 4 : 3) * launch + sums * z_h;
   };
   int64_t most = ((int64_t)512 << 20) / (elem * (N > 0 ? N : 1)) / 256 * 256;
   if (most < 1024) most = 1024;
+  if (split && most > words_at_once(D, V)) most = words_at_once(D, V);
   Plan best{};
   double best_cost = 1e300;
   const int64_t step = up(up(V, 32), 256) * 256;  // at most about 32 candidates (0.4 us of host time each)
@@ -416,12 +370,57 @@ Plan plan(int64_t N, int64_t D, int64_t V, int dtype) {
   return best;
 }
 
-int simple_fwd(const Problem& p, int dtype) {
-  return dtype == DYNCONV_DTYPE_BF16 ? fwd<__nv_bfloat16>(p) : fwd<float>(p);
+int simple_fwd(const Problem& all) {
+  int s;
+  for (int64_t r0 = 0; r0 < all.N; r0 += kRowsAtOnce) {
+    const Problem p = rows_from(all, r0, sizeof(T));
+    Gemm g{};
+    g.A = p.hidden, g.am = p.D, g.ak = 1;
+    g.B = p.weight, g.bn = p.D, g.bk = 1;
+    g.M = p.N, g.N = p.V, g.K = p.D;
+    if ((s = gemm<kForward>(g, p, 1, "vl_gemm_kernel (forward)"))) return s;
+    const int64_t tile = large_tiles(p.N, p.V, 1) ? 128 : 64;
+    if ((s = merge_launch(p, (p.V + tile - 1) / tile))) return s;
+  }
+  return total_launch(all);
 }
 
-int simple_bwd(const Problem& p, const Plan& pl, int dtype) {
-  return dtype == DYNCONV_DTYPE_BF16 ? bwd<__nv_bfloat16>(p, pl, dtype) : bwd<float>(p, pl, dtype);
+int simple_bwd(const Problem& p, const Plan& pl) {
+  int s;
+  for (int64_t v0 = 0; v0 < p.V; v0 += pl.piece) {
+    const int64_t vp = p.V - v0 < pl.piece ? p.V - v0 : pl.piece;
+    const T* w = (const T*)p.weight + v0 * p.D;
+    Gemm g{};
+    g.A = p.hidden, g.am = p.D, g.ak = 1;
+    g.B = w, g.bn = p.D, g.bk = 1;
+    g.M = p.N, g.N = vp, g.K = p.D, g.col0 = v0;
+    g.out = p.piece, g.out_ld = pl.pitch;
+    if ((s = gemm<kGrad>(g, p, 1, "vl_gemm_kernel (logits' gradient)"))) return s;
+    if (p.dweight) {
+      Gemm gw{};
+      gw.A = p.piece, gw.am = 1, gw.ak = pl.pitch;
+      gw.B = p.hidden, gw.bn = 1, gw.bk = p.D;
+      gw.M = vp, gw.N = p.D, gw.K = p.N;
+      gw.out_ld = p.D;
+      if (pl.z_w == 1) {
+        gw.out = (T*)p.dweight + v0 * p.D;
+        if ((s = gemm<kStore>(gw, p, 1, "vl_gemm_kernel (weight gradient)"))) return s;
+      } else {
+        gw.out = p.acc_w;
+        if ((s = gemm<kAccumulate>(gw, p, pl.z_w, "vl_gemm_kernel (weight gradient)"))) return s;
+        if ((s = finish_launch(p, p.acc_w, pl.z_w, vp * p.D, (T*)p.dweight + v0 * p.D, DYNCONV_DTYPE_BF16))) return s;
+      }
+    }
+    if (p.dhidden) {
+      Gemm gh{};
+      gh.A = p.piece, gh.am = pl.pitch, gh.ak = 1;
+      gh.B = w, gh.bn = 1, gh.bk = p.D;
+      gh.M = p.N, gh.N = p.D, gh.K = vp;
+      gh.out = p.acc_h, gh.out_ld = p.D, gh.add = v0 > 0;
+      if ((s = gemm<kAccumulate>(gh, p, pl.z_h, "vl_gemm_kernel (hidden gradient)"))) return s;
+    }
+  }
+  return p.dhidden ? finish_launch(p, p.acc_h, pl.z_h, p.N * p.D, p.dhidden, DYNCONV_DTYPE_BF16) : DYNCONV_OK;
 }
 
 }  // namespace vl

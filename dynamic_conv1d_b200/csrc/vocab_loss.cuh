@@ -46,6 +46,9 @@ struct Problem {
   void* piece;              // [N, pitch]: dl of one piece of the vocabulary
   float* acc_h;             // [z_h][N][D] fp32
   float* acc_w;             // [z_w][piece rows][D] fp32, z_w > 1
+  // fp32 tensors, either way: three bf16 parts of each (pitch part_pitch(D))
+  __nv_bfloat16* hidden_parts;  // [3][N or rows at once][pitch]
+  __nv_bfloat16* weight_parts;  // [3][words at once][pitch]
   cudaStream_t st;
 };
 
@@ -73,6 +76,22 @@ __device__ __forceinline__ float result_factor(const Problem& p) {
 // (8 bytes for each row and tile), and the weight is read again once per 32768 rows only.
 constexpr int64_t kRowsAtOnce = 32768;
 constexpr int kNarrowestTile = 64;  // columns of the vocabulary in one forward tile, at least
+
+// fp32 tensors on the tensor cores: x = x0 + x1 + x2, each part the rest rounded to bf16 (8
+// digits each: the three hold all 24), and a product of two such numbers is the six products of
+// parts whose indices add up to at most two; the three left out are below 2^-23 of it.
+constexpr int kSplitParts = 3, kSplitProducts = 6;
+// The tensor core's accumulation truncates (vocab_loss_tc.cu): 4 blocks of 64 inner elements
+// are summed there, and these sums in fp32 registers.
+constexpr int kSplitChain = 4;
+inline int64_t part_pitch(int64_t D) { return (D + 7) / 8 * 8; }
+inline size_t part_bytes(int64_t rows, int64_t D) { return (size_t)kSplitParts * 2 * rows * part_pitch(D); }
+// Words of the vocabulary whose parts are kept at once: at most 512 MB of them.
+inline int64_t words_at_once(int64_t D, int64_t V) {
+  const int64_t most = ((int64_t)512 << 20) / (2 * kSplitParts * part_pitch(D)) / 256 * 256;
+  return most < 1024 ? (V < 1024 ? V : 1024) : most < V ? most : V;
+}
+
 bool tc_supported(const Problem& p, int dtype);
 Plan plan(int64_t N, int64_t D, int64_t V, int dtype);
 int merge_launch(const Problem& rows, int64_t tiles);  // the rows' losses from their tiles
@@ -89,10 +108,10 @@ inline Problem rows_from(const Problem& p, int64_t r0, int64_t elem) {
 // out[i] = result_factor * the sum of n-element parts, in part order, rounded to dtype
 int finish_launch(const Problem& p, const float* parts, int n_parts, int64_t n, void* out, int dtype);
 
-int simple_fwd(const Problem& p, int dtype);
-int simple_bwd(const Problem& p, const Plan& pl, int dtype);
-int tc_fwd(const Problem& p);
-int tc_bwd(const Problem& p, const Plan& pl);
+int simple_fwd(const Problem& p);
+int simple_bwd(const Problem& p, const Plan& pl);
+int tc_fwd(const Problem& p, int dtype);
+int tc_bwd(const Problem& p, const Plan& pl, int dtype);
 
 }  // namespace vl
 }  // namespace dynconv

@@ -1,4 +1,5 @@
-// vocab_loss_tc.cu -- the vocabulary loss on the tensor cores (bf16).
+// vocab_loss_tc.cu -- the vocabulary loss on the tensor cores: bf16 tensors, and fp32 ones in three
+// bf16 parts.
 //
 // One persistent kernel computes out(m, n) = sum_k A(m, k) B(n, k) for all four products;
 // only the operands' majors and the epilogue differ:
@@ -24,6 +25,18 @@
 // weight gradient 2.15, hidden gradient 2.1 ms: 1.5 PFLOP/s each, 94% of a library product's
 // burst rate; back to back under the power limit the pass takes 10.6 ms (1.27 PFLOP/s; that
 // library product sustains 1.38).
+//
+// fp32 tensors (SPLIT) go through the same kernel: a small kernel writes each tensor as three bf16
+// parts (bound by HBM: 4 bytes read and 6 written for each number), the inner dimension is walked
+// once for each of six products of parts, and dl leaves the epilogue as parts too.  The sums of
+// 256 inner elements' products are added up in registers (the tensor core's sums alone would be
+// off by more than fp32's rounding).  Products at 1/6 of the bf16 rate are 3.5 times what the
+// fp32 units could do at their best.  Whole passes, forward and backward (B200; in brackets the CUDA
+// cores' tiles that did this before): 1021 tokens x 256 channels over 4999 words 35 + 103 us (90 + 233),
+// 1021 x 1024 x 8000 93 + 269 us (400 + 1226), 4096 x 2048 x 65536 5.0 + 16.2 ms (20.8 + 71.1):
+// 1.25 PFLOP/s of bf16 products.  Few rows gain only over large vocabularies, as the tensors are
+// written anew: one row of 256 x 4999 25 + 61 us (19 + 40), of 2048 x 65536 0.83 + 1.27 ms (0.63 +
+// 1.52), 32 rows of the latter 0.59 + 1.12 (0.65 + 1.67).
 #include "vocab_loss.cuh"
 
 namespace dynconv {
@@ -48,24 +61,30 @@ static_assert(kSmem <= 232448 - 1024, "shared memory of one CTA");
 constexpr int kChain = 32;
 constexpr int kHalf = kN / 2;  // columns of one epilogue warp; a forward tile's partials are per half
 
+// fp32 tensors in three bf16 parts (SPLIT): in blocks of 64 inner elements by product, kSplitChain
+// blocks' six products at a time, the smallest products first.
+constexpr int kSplitBlocks = kSplitChain * kSplitProducts;
+
 enum TcMode { kTcForward, kTcForwardLong, kTcGrad, kTcAdd, kTcStore };
 
 struct TcGemm {
   int64_t M, N;        // extents of the output
-  int k_blocks;        // 64-element blocks of the inner dimension
+  int k_blocks;        // 64-element blocks of the inner dimension (SPLIT: of each product)
   int m_tiles, n_tiles, z;
   int group;           // m tiles that share a sweep over n: consecutive tiles walk a group's rows first
   int64_t col0;        // kTcGrad: first vocabulary column
   void* out;           // kTcAdd: fp32 [z][M][N] (the bf16 outputs go through a tensor map)
   int64_t out_ld;
   int add;             // kTcAdd: add to what is there
-  void* result;        // kTcAdd: not null: the last sums, rounded to bf16
+  void* result;        // kTcAdd: not null: the last sums, in the tensors' type
+  int vec;             // SPLIT kTcAdd: rows of out and result may be written 16 bytes at a time
 };
 
 struct Tile {
   int m, n, z, kb0, kb1;
 };
 
+template <bool SPLIT>
 __device__ __forceinline__ Tile tile_at(const TcGemm& g, int t) {
   Tile r;
   const int plane = g.m_tiles * g.n_tiles;
@@ -76,9 +95,27 @@ __device__ __forceinline__ Tile tile_at(const TcGemm& g, int t) {
   const int rows = min(g.group, g.m_tiles - grp * g.group);
   r.n = t / rows;
   r.m = grp * g.group + (t - r.n * rows);
-  r.kb0 = (int)((int64_t)g.k_blocks * r.z / g.z);
-  r.kb1 = (int)((int64_t)g.k_blocks * (r.z + 1) / g.z);
+  if constexpr (SPLIT) {  // whole chains
+    const int64_t chains = (g.k_blocks + kSplitChain - 1) / kSplitChain;
+    r.kb0 = (int)(chains * r.z / g.z) * kSplitBlocks;
+    r.kb1 = min((int)(chains * (r.z + 1) / g.z) * kSplitBlocks, g.k_blocks * kSplitProducts);
+  } else {
+    r.kb0 = (int)((int64_t)g.k_blocks * r.z / g.z);
+    r.kb1 = (int)((int64_t)g.k_blocks * (r.z + 1) / g.z);
+  }
   return r;
+}
+
+// SPLIT: what the kb-th block of products multiplies.
+struct SplitBlock {
+  int block, a, b;  // 64 inner elements, parts of A and B
+};
+
+__device__ __forceinline__ SplitBlock split_block(int k_blocks, int kb) {
+  const int chain = kb / kSplitBlocks, r = kb - chain * kSplitBlocks;
+  const int blocks = min(kSplitChain, k_blocks - chain * kSplitChain), product = r / blocks;
+  // parts (0,2), (1,1), (2,0), (0,1), (1,0), (0,0)
+  return {chain * kSplitChain + r - product * blocks, 0x010210 >> (4 * product) & 3, 0x001012 >> (4 * product) & 3};
 }
 
 // ---- a CTA pair: addresses in the first CTA, products over both
@@ -109,6 +146,15 @@ __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map,
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
       "%4}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+// The same from one of the parts of an fp32 tensor.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int part) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(part)
       : "memory");
 }
 
@@ -143,14 +189,82 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
-// dl of 32 columns, in place.  f: the row's factor, at: the target's column among the 32.
-__device__ __forceinline__ void logits_gradient(float (&v)[32], float f, float lse2, int64_t at) {
+// dl of n columns, in place.  f: the row's factor, at: the target's column among them.
+template <int n>
+__device__ __forceinline__ void logits_gradient(float (&v)[n], float f, float lse2, int64_t at) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = f != 0.f ? ex2(fmaf(v[j], kLog2e, -lse2)) * f : 0.f;  // (an ignored row's NaN stays out)
-  if (at >= 0 && at < 32) {
+  for (int j = 0; j < n; ++j) v[j] = f != 0.f ? ex2(fmaf(v[j], kLog2e, -lse2)) * f : 0.f;  // (an ignored row's NaN stays out)
+  if (at >= 0 && at < n) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < n; ++j)
       if (j == at) v[j] -= f;
+  }
+}
+
+// The next bf16 part of two numbers, packed; the numbers keep the rest (exact).
+__device__ __forceinline__ uint32_t take_part(float2& x) {
+  const uint32_t p = pack_bf16x2(x.x, x.y);
+  x = add2(x, make_float2(-__uint_as_float(p << 16), -__uint_as_float(p & 0xFFFF0000u)));
+  return p;
+}
+
+// An fp32 matrix as its three parts.
+__global__ void __launch_bounds__(256) vl_split_kernel(const float* __restrict__ src, int64_t rows, int64_t D,
+                                                       int64_t pitch, __nv_bfloat16* __restrict__ parts) {
+  const int64_t per = pitch / 8, n = rows * per, plane = rows * pitch;
+  const bool vec = D % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / per, c = (i - row * per) * 8;
+    const float* s = src + row * D + c;
+    float2 v[4];
+    if (vec) {
+      const float4 lo = reinterpret_cast<const float4*>(s)[0], hi = reinterpret_cast<const float4*>(s)[1];
+      v[0] = make_float2(lo.x, lo.y), v[1] = make_float2(lo.z, lo.w);
+      v[2] = make_float2(hi.x, hi.y), v[3] = make_float2(hi.z, hi.w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = make_float2(c + 2 * j < D ? s[2 * j] : 0.f, c + 2 * j + 1 < D ? s[2 * j + 1] : 0.f);
+    }
+    // the first part is cut to bf16's range: a number close to fp32's largest stays finite, an
+    // infinity or a NaN becomes a NaN in the parts that follow
+    constexpr float kLargest = 3.38953139e38f;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float2 cut = make_float2(fminf(fmaxf(v[j].x, -kLargest), kLargest), fminf(fmaxf(v[j].y, -kLargest), kLargest));
+      const float2 over = make_float2(v[j].x - cut.x, v[j].y - cut.y);  // zero, but for those
+      w[j] = take_part(cut);
+      v[j] = add2(cut, over);
+    }
+    __nv_bfloat16* to = parts + row * pitch + c;
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+    for (int k = 1; k < kSplitParts; ++k)
+      *reinterpret_cast<uint4*>(to + k * plane) = make_uint4(take_part(v[0]), take_part(v[1]), take_part(v[2]), take_part(v[3]));
+  }
+}
+
+// 16 columns of a row of fp32 sums, added up over pieces; the last ones are the result in fp32.
+__device__ __forceinline__ void add_columns(const TcGemm& g, const float (&v)[16], int64_t row, int64_t col, int z,
+                                            float factor) {
+  const float* o = (const float*)g.out + ((int64_t)z * g.M + row) * g.out_ld + col;
+  float* to = g.result ? (float*)g.result + row * g.out_ld + col : const_cast<float*>(o);
+  const float f = g.result ? factor : 1.f;
+#pragma unroll
+  for (int j = 0; j < 16; j += 4) {
+    if (g.vec && col + j < g.N) {  // (N is a multiple of four)
+      float4 u = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      if (g.add) {
+        const float4 w = *reinterpret_cast<const float4*>(o + j);
+        u.x += w.x, u.y += w.y, u.z += w.z, u.w += w.w;
+      }
+      *reinterpret_cast<float4*>(to + j) = make_float4(u.x * f, u.y * f, u.z * f, u.w * f);
+    } else {
+#pragma unroll
+      for (int i = j; i < j + 4; ++i)
+        if (col + i < g.N) to[i] = (v[i] + (g.add ? o[i] : 0.f)) * f;
+    }
   }
 }
 
@@ -191,11 +305,13 @@ __device__ __forceinline__ void stage_columns(uint8_t* tile, int row, int half, 
   }
 }
 
-template <int MODE, bool A_MN, bool B_MN>
+template <int MODE, bool A_MN, bool B_MN, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     vl_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                  const __grid_constant__ CUtensorMap omap, const __grid_constant__ TcGemm g, const __grid_constant__ Problem p) {
   constexpr bool kForward = MODE == kTcForward || MODE == kTcForwardLong;
+  constexpr bool kChained = MODE == kTcForwardLong || SPLIT;  // sums of kBlocks blocks are added up in registers
+  constexpr int kBlocks = SPLIT ? kSplitBlocks : kChain;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
   // full and acce are used in the first CTA only; empty and accf in both
@@ -233,7 +349,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       int it = 0;
       bool dead = false;
       for (int i = pair; i < n_tiles && !dead; i += pairs) {
-        const Tile t = tile_at(g, i);
+        const Tile t = tile_at<SPLIT>(g, i);
         const int m0 = t.m * kM + rank * kHalfM, n0 = t.n * kN + rank * kHalfB;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
           const int s = it % kStages;
@@ -247,17 +363,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           // the first CTA announces both CTAs' bytes (the other's may land before: the phase
           // still waits for this arrival)
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * kStageBytes);
+          SplitBlock sp{kb, 0, 0};
+          if constexpr (SPLIT) sp = split_block(g.k_blocks, kb);
+          auto load = [&](uint8_t* dst, const CUtensorMap* map, int c0, int c1, int part) {
+            if constexpr (SPLIT)
+              tma_load_pair(dst, map, full, c0, c1, part);
+            else
+              tma_load_pair(dst, map, full, c0, c1);
+          };
           if constexpr (A_MN) {
 #pragma unroll
-            for (int j = 0; j < kHalfM / 64; ++j) tma_load_pair(a + j * kAtom, &amap, full, m0 + j * 64, kb * kKB);
+            for (int j = 0; j < kHalfM / 64; ++j) load(a + j * kAtom, &amap, m0 + j * 64, sp.block * kKB, sp.a);
           } else {
-            tma_load_pair(a, &amap, full, kb * kKB, m0);
+            load(a, &amap, sp.block * kKB, m0, sp.a);
           }
           if constexpr (B_MN) {
 #pragma unroll
-            for (int j = 0; j < kHalfB / 64; ++j) tma_load_pair(b + j * kAtom, &bmap, full, n0 + j * 64, kb * kKB);
+            for (int j = 0; j < kHalfB / 64; ++j) load(b + j * kAtom, &bmap, n0 + j * 64, sp.block * kKB, sp.b);
           } else {
-            tma_load_pair(b, &bmap, full, kb * kKB, n0);
+            load(b, &bmap, sp.block * kKB, n0, sp.b);
           }
         }
       }
@@ -276,10 +400,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       int it = 0, n = 0;
       bool dead = false;
       for (int i = pair; i < n_tiles && !dead; i += pairs, ++n) {
-        const Tile t = tile_at(g, i);
+        const Tile t = tile_at<SPLIT>(g, i);
         int a = n & 1, first = t.kb0;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-          if (kb == t.kb0 || (MODE == kTcForwardLong && kb - first == kChain)) {
+          if (kb == t.kb0 || (kChained && kb - first == kBlocks)) {
             if (kb > t.kb0) ++n;
             a = n & 1, first = kb;
             if (!mbar_wait(&acce_bar[a], ((n >> 1) & 1) ^ 1, kErrWaitMma, &abort_flag)) {
@@ -302,7 +426,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             umma_pair(el, tmem + a * kN, ad + k * (A_MN ? 2048 : 32) / 16, bd + k * (B_MN ? 2048 : 32) / 16, idesc,
                       (kb > first || k > 0) ? 1u : 0u);
           umma_commit_pair(el, &empty_bar[s]);
-          if (kb == t.kb1 - 1 || (MODE == kTcForwardLong && kb - first == kChain - 1)) umma_commit_pair(el, &accf_bar[a]);
+          if (kb == t.kb1 - 1 || (kChained && kb - first == kBlocks - 1)) umma_commit_pair(el, &accf_bar[a]);
           __syncwarp();
         }
       }
@@ -318,7 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     const float factor = MODE == kTcAdd || MODE == kTcStore ? result_factor(p) : 1.f;
     const uint32_t freed[2] = {in_first_cta(&acce_bar[0]), in_first_cta(&acce_bar[1])};
     for (int i = pair; i < n_tiles; i += pairs, ++n) {
-      const Tile t = tile_at(g, i);
+      const Tile t = tile_at<SPLIT>(g, i);
       int a = n & 1;
       const int64_t row = (int64_t)t.m * kM + rank * kHalfM + q * 32 + lane;
       const int64_t col0 = (int64_t)t.n * kN + half * kHalf;
@@ -334,13 +458,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      float chained[MODE == kTcForwardLong ? kHalf : 1];  // the sums of the chains before the last
-      if constexpr (MODE == kTcForwardLong) {
-        const int chains = (g.k_blocks + kChain - 1) / kChain;
+      float chained[kChained ? kHalf : 1];  // the sums of the chains before the last (SPLIT: of all)
+      if constexpr (kChained) {
+        const int chains = (t.kb1 - t.kb0 + kBlocks - 1) / kBlocks, early = SPLIT ? chains : chains - 1;
 #pragma unroll
         for (int j = 0; j < kHalf; ++j) chained[j] = 0.f;
 #pragma unroll 1
-        for (int k = 0; k + 1 < chains; ++k, ++n) {
+        for (int k = 0; k < early; ++k, ++n) {
           a = n & 1;
           if (!dead) dead = !mbar_wait(&accf_bar[a], (n >> 1) & 1, kErrWaitEpilogue, &abort_flag);
           tc_fence_after();
@@ -359,28 +483,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           __syncwarp();
           if (lane == 0) arrive_in_first_cta(freed[a]);
         }
+        if constexpr (SPLIT) --n;
         a = n & 1;
       }
-      if (!dead) dead = !mbar_wait(&accf_bar[a], (n >> 1) & 1, kErrWaitEpilogue, &abort_flag);
-      tc_fence_after();
+      if constexpr (!SPLIT) {
+        if (!dead) dead = !mbar_wait(&accf_bar[a], (n >> 1) & 1, kErrWaitEpilogue, &abort_flag);
+        tc_fence_after();
+      }
       if (!dead) {
         const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + a * kN + half * kHalf;
         float m2 = -INFINITY, sum = 0.f;
         const int there = (int)max((int64_t)0, min((int64_t)kHalf, g.N - col0));  // columns that are there
-        const int64_t t_col = target - col0;
+        const int64_t t_col = target - g.col0 - col0;
         const int mine = row_in && t_col >= 0 && t_col < there ? (int)t_col : -1;  // the target's column
-        constexpr int kStep = MODE == kTcForwardLong ? 16 : 32;  // columns at a time (registers)
-#pragma unroll (MODE == kTcForwardLong ? kHalf / kStep : 1)
+        constexpr int kStep = kChained ? 16 : 32;  // columns at a time (registers)
+#pragma unroll (kChained ? kHalf / kStep : 1)
         for (int c = 0; c < kHalf; c += kStep) {
           float v[kStep];
-          if constexpr (MODE == kTcForwardLong)
+          if constexpr (SPLIT) {
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) v[j] = chained[c + j];
+          } else if constexpr (kChained) {
             tmem_ld16(base + c, v);
-          else
-            tmem_ld32(base + c, v);
-          tmem_ld_wait();
-          if constexpr (MODE == kTcForwardLong) {
+            tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < kStep; ++j) v[j] += chained[c + j];
+          } else {
+            tmem_ld32(base + c, v);
+            tmem_ld_wait();
           }
           if constexpr (kForward) {
             const int left = there - c;
@@ -414,6 +544,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             }
           } else if constexpr (MODE == kTcAdd) {
             if (row_in) add_columns(g, v, row, col0 + c, t.z, factor);
+          } else if constexpr (SPLIT) {
+            logits_gradient(v, f, lse2, target - g.col0 - (col0 + c));
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) chained[c + j] = v[j];
+            // 64 columns at a time, part by part, through the staged tile (1021 x 256 x 4999: 102 us for the
+            // backward, where 16-byte stores from each row's thread take 114)
+            if ((c + kStep) % 64 == 0) {
+              uint8_t* tile = smem + kStages * kStageBytes + (warp - 2) * kStageOut;
+              const int from = c + kStep - 64;
+              float2 pr[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) pr[j] = make_float2(chained[from + 2 * j], chained[from + 2 * j + 1]);
+#pragma unroll
+              for (int k = 0; k < kSplitParts; ++k) {
+                if (lane == 0) bulk_wait_group_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  *reinterpret_cast<uint4*>(tile + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                      make_uint4(take_part(pr[4 * j]), take_part(pr[4 * j + 1]), take_part(pr[4 * j + 2]), take_part(pr[4 * j + 3]));
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  tma_store_3d(&omap, tile, (int)(col0 + from), t.m * kM + rank * kHalfM + q * 32, k);
+                  bulk_commit_group();
+                }
+              }
+            }
           } else {
             // bf16: 64 columns at a time through the warp's staged tile and a TMA store, which
             // leaves out what lies beyond the matrix
@@ -443,9 +601,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           if (row_in) p.part[((int64_t)t.n * 2 + half) * g.M + row] = make_float2(m2, sum);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_in_first_cta(freed[a]);
+      if constexpr (!SPLIT) {  // (SPLIT has given its accumulators back one by one)
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_in_first_cta(freed[a]);
+      }
     }
     if constexpr (MODE == kTcGrad || MODE == kTcStore) {
       if (lane == 0) bulk_wait_group_read<0>();  // (shared memory may go once it has been read)
@@ -457,15 +617,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
-// A row-major [rows][cols] bf16 matrix as boxes of 64 columns x box_rows rows, 128-byte swizzle.
-int matrix_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows) {
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
-  return encode_tensor_map_bf16(map, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+// A row-major [rows][cols] bf16 matrix as boxes of 64 columns x box_rows rows, 128-byte swizzle; with
+// PARTS, the three parts of an fp32 one.
+template <bool PARTS>
+int matrix_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows, int64_t plane = 0) {
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, kSplitParts};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  return encode_tensor_map_bf16(map, base, PARTS ? 3 : 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int MODE, bool A_MN, bool B_MN>
+template <int MODE, bool A_MN, bool B_MN, bool SPLIT>
 int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, TcGemm g, const Problem& p, const char* what) {
   const int64_t mt = (g.M + kM - 1) / kM, nt = (g.N + kN - 1) / kN;
   if (mt * nt * g.z > INT32_MAX) return set_error(DYNCONV_ERR_SHAPE, "%s: too many tiles", what);
@@ -473,94 +635,142 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, TcG
   if (g.group > g.m_tiles) g.group = g.m_tiles;
   const int tiles = g.m_tiles * g.n_tiles * g.z, most = sm_count() / 2;
   const int grid = 2 * (tiles < most ? tiles : most);
-  cudaError_t e = cudaFuncSetAttribute(vl_tc_kernel<MODE, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  cudaError_t e =
+      cudaFuncSetAttribute(vl_tc_kernel<MODE, A_MN, B_MN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return cuda_status(e, "cudaFuncSetAttribute(vl_tc)");
   }
-  vl_tc_kernel<MODE, A_MN, B_MN><<<grid, kTcThreads, kSmem, p.st>>>(a, b, o, g, p);
+  vl_tc_kernel<MODE, A_MN, B_MN, SPLIT><<<grid, kTcThreads, kSmem, p.st>>>(a, b, o, g, p);
   DYNCONV_CHECK_LAUNCH(what);
   return DYNCONV_OK;
 }
 
+int split_launch(const Problem& p, const float* src, int64_t rows, __nv_bfloat16* parts) {
+  const int64_t pitch = part_pitch(p.D), most = 16 * (int64_t)sm_count();
+  const int64_t grid = (rows * (pitch / 8) + 255) / 256;
+  vl_split_kernel<<<(unsigned)(grid < most ? grid : most), 256, 0, p.st>>>(src, rows, p.D, pitch, parts);
+  DYNCONV_CHECK_LAUNCH("vl_split_kernel");
+  return DYNCONV_OK;
+}
+
 // Rows of hidden (a group) that stay in L2 while the vocabulary is swept over them: half of it.
-int row_group(int64_t D) {
-  const int64_t g = ((int64_t)64 << 20) / (kM * D * 2);
+int row_group(int64_t row_bytes) {
+  const int64_t g = ((int64_t)64 << 20) / (kM * row_bytes);
   return g < 1 ? 1 : (int)(g < 4096 ? g : 4096);
+}
+
+int blocks_of(int64_t n) { return (int)((n + kKB - 1) / kKB); }
+
+template <bool SPLIT>
+int fwd(const Problem& all) {
+  const int64_t words = SPLIT ? words_at_once(all.D, all.V) : all.V, ld = SPLIT ? part_pitch(all.D) : all.D;
+  int s;
+  for (int64_t r0 = 0; r0 < all.N; r0 += kRowsAtOnce) {
+    Problem p = rows_from(all, r0, SPLIT ? 4 : 2);
+    if (SPLIT && (s = split_launch(p, (const float*)p.hidden, p.N, p.hidden_parts))) return s;
+    CUtensorMap a;
+    if ((s = matrix_map<SPLIT>(&a, SPLIT ? p.hidden_parts : p.hidden, p.D, p.N, ld, kHalfM, p.N * ld))) return s;
+    TcGemm g{};
+    g.M = p.N, g.k_blocks = blocks_of(p.D), g.z = 1, g.group = row_group(p.D * (SPLIT ? 2 * kSplitParts : 2));
+    for (int64_t v0 = 0; v0 < p.V; v0 += words) {  // (words: all, or a multiple of a tile's)
+      g.N = p.V - v0 < words ? p.V - v0 : words, g.col0 = v0;
+      if (SPLIT && (r0 == 0 || words < p.V) &&
+          (s = split_launch(p, (const float*)p.weight + v0 * p.D, g.N, p.weight_parts)))
+        return s;
+      CUtensorMap b;
+      if ((s = matrix_map<SPLIT>(&b, SPLIT ? p.weight_parts : p.weight, p.D, g.N, ld, kHalfB, g.N * ld))) return s;
+      Problem tiles = p;
+      tiles.part += v0 / kHalf * p.N;
+      s = SPLIT || g.k_blocks <= kChain
+              ? launch<kTcForward, false, false, SPLIT>(a, b, a, g, tiles, "vl_tc_kernel (forward)")
+              : launch<kTcForwardLong, false, false, false>(a, b, a, g, tiles, "vl_tc_kernel (forward)");
+      if (s) return s;
+    }
+    if ((s = merge_launch(p, (p.V + kN - 1) / kN * 2))) return s;
+  }
+  return total_launch(all);
+}
+
+template <bool SPLIT>
+int bwd(const Problem& p, const Plan& pl) {
+  constexpr int kType = SPLIT ? DYNCONV_DTYPE_F32 : DYNCONV_DTYPE_BF16, kElem = SPLIT ? 4 : 2;
+  const int64_t ld = SPLIT ? part_pitch(p.D) : p.D;
+  // shares of an inner dimension: each has a block, or a chain, at least
+  const auto shares = [](int z, int blocks) {
+    const int most = SPLIT ? (blocks + kSplitChain - 1) / kSplitChain : blocks;
+    return z < most ? z : most;
+  };
+  const auto vec = [&](const void* q) { return SPLIT && p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  int s;
+  if (SPLIT && (s = split_launch(p, (const float*)p.hidden, p.N, p.hidden_parts))) return s;
+  const void* hidden = SPLIT ? p.hidden_parts : p.hidden;
+  CUtensorMap hk, hm;
+  if ((s = matrix_map<SPLIT>(&hk, hidden, p.D, p.N, ld, kHalfM, p.N * ld))) return s;
+  if ((s = matrix_map<SPLIT>(&hm, hidden, p.D, p.N, ld, 64, p.N * ld))) return s;
+  for (int64_t v0 = 0; v0 < p.V; v0 += pl.piece) {
+    const int64_t vp = p.V - v0 < pl.piece ? p.V - v0 : pl.piece;
+    const void* w = (const char*)p.weight + v0 * p.D * kElem;
+    if (SPLIT) {
+      if ((s = split_launch(p, (const float*)w, vp, p.weight_parts))) return s;
+      w = p.weight_parts;
+    }
+    // maps of exactly this piece: what lies beyond it reads as zero
+    CUtensorMap wk, wm, pk, pm, po;
+    if ((s = matrix_map<SPLIT>(&wk, w, p.D, vp, ld, kHalfB, vp * ld))) return s;
+    if ((s = matrix_map<SPLIT>(&wm, w, p.D, vp, ld, 64, vp * ld))) return s;
+    if ((s = matrix_map<SPLIT>(&pk, p.piece, vp, p.N, pl.pitch, kHalfM, p.N * pl.pitch))) return s;
+    if ((s = matrix_map<SPLIT>(&pm, p.piece, vp, p.N, pl.pitch, 64, p.N * pl.pitch))) return s;
+    if ((s = matrix_map<SPLIT>(&po, p.piece, vp, p.N, pl.pitch, 32, p.N * pl.pitch))) return s;
+    TcGemm g{};
+    g.M = p.N, g.N = vp, g.k_blocks = blocks_of(p.D), g.z = 1, g.group = row_group(p.D * (SPLIT ? 2 * kSplitParts : 2));
+    g.col0 = v0;
+    if ((s = launch<kTcGrad, false, false, SPLIT>(hk, wk, po, g, p, "vl_tc_kernel (logits' gradient)"))) return s;
+    if (p.dweight) {
+      void* dw = (char*)p.dweight + v0 * p.D * kElem;
+      TcGemm gw{};
+      gw.M = vp, gw.N = p.D, gw.k_blocks = blocks_of(p.N), gw.group = 1, gw.out_ld = p.D;
+      gw.z = shares(pl.z_w, gw.k_blocks);
+      gw.out = p.acc_w, gw.vec = vec(p.acc_w);
+      if (pl.z_w == 1 && !SPLIT) {
+        CUtensorMap wo;
+        if ((s = matrix_map<false>(&wo, dw, p.D, vp, p.D, 32))) return s;
+        if ((s = launch<kTcStore, true, true, false>(pm, hm, wo, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
+      } else {
+        if (pl.z_w == 1) gw.result = dw, gw.vec = vec(dw);
+        if ((s = launch<kTcAdd, true, true, SPLIT>(pm, hm, pm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
+        if (pl.z_w > 1 && (s = finish_launch(p, p.acc_w, gw.z, vp * p.D, dw, kType))) return s;
+      }
+    }
+    if (p.dhidden) {
+      TcGemm gh{};
+      gh.M = p.N, gh.N = p.D, gh.k_blocks = blocks_of(vp), gh.group = 1;
+      gh.z = shares(pl.z_h, gh.k_blocks);  // the first piece fills every share; a short last one may not
+      gh.out = p.acc_h, gh.out_ld = p.D, gh.add = v0 > 0;
+      gh.result = pl.z_h == 1 && v0 + vp == p.V ? p.dhidden : nullptr;
+      gh.vec = vec(p.acc_h) && (!gh.result || vec(gh.result));
+      if ((s = launch<kTcAdd, false, true, SPLIT>(pk, wm, pk, gh, p, "vl_tc_kernel (hidden gradient)"))) return s;
+    }
+  }
+  if (!p.dhidden || pl.z_h == 1) return DYNCONV_OK;
+  return finish_launch(p, p.acc_h, pl.z_h, p.N * p.D, p.dhidden, kType);
 }
 
 }  // namespace
 
 bool tc_supported(const Problem& p, int dtype) {
-  if (dtype != DYNCONV_DTYPE_BF16 || p.D % 8 != 0) return false;
+  if (dtype == DYNCONV_DTYPE_F32) return true;  // (its operands are copies)
+  if (p.D % 8 != 0) return false;
   const void* ptrs[] = {p.hidden, p.weight, p.dhidden, p.dweight, p.piece};
   for (const void* q : ptrs)
     if (reinterpret_cast<uintptr_t>(q) & 15) return false;
   return true;
 }
 
-int tc_fwd(const Problem& all) {
-  CUtensorMap a, b;
-  int s;
-  if ((s = matrix_map(&b, all.weight, all.D, all.V, all.D, kHalfB))) return s;
-  for (int64_t r0 = 0; r0 < all.N; r0 += kRowsAtOnce) {
-    const Problem p = rows_from(all, r0, 2);
-    if ((s = matrix_map(&a, p.hidden, p.D, p.N, p.D, kHalfM))) return s;
-    TcGemm g{};
-    g.M = p.N, g.N = p.V, g.k_blocks = (int)((p.D + kKB - 1) / kKB), g.z = 1, g.group = row_group(p.D);
-    s = g.k_blocks <= kChain ? launch<kTcForward, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)")
-                             : launch<kTcForwardLong, false, false>(a, b, a, g, p, "vl_tc_kernel (forward)");
-    if (s || (s = merge_launch(p, (p.V + kN - 1) / kN * 2))) return s;
-  }
-  return total_launch(all);
-}
+int tc_fwd(const Problem& p, int dtype) { return dtype == DYNCONV_DTYPE_F32 ? fwd<true>(p) : fwd<false>(p); }
 
-int tc_bwd(const Problem& p, const Plan& pl) {
-  int s;
-  CUtensorMap hk, hm;
-  if ((s = matrix_map(&hk, p.hidden, p.D, p.N, p.D, kHalfM))) return s;
-  if ((s = matrix_map(&hm, p.hidden, p.D, p.N, p.D, 64))) return s;
-  const int d_blocks = (int)((p.D + kKB - 1) / kKB);
-  for (int64_t v0 = 0; v0 < p.V; v0 += pl.piece) {
-    const int64_t vp = p.V - v0 < pl.piece ? p.V - v0 : pl.piece;
-    const __nv_bfloat16* w = (const __nv_bfloat16*)p.weight + v0 * p.D;
-    // maps of exactly this piece: what lies beyond it reads as zero
-    CUtensorMap wk, wm, pk, pm, po;
-    if ((s = matrix_map(&wk, w, p.D, vp, p.D, kHalfB))) return s;
-    if ((s = matrix_map(&wm, w, p.D, vp, p.D, 64))) return s;
-    if ((s = matrix_map(&pk, p.piece, vp, p.N, pl.pitch, kHalfM))) return s;
-    if ((s = matrix_map(&pm, p.piece, vp, p.N, pl.pitch, 64))) return s;
-    if ((s = matrix_map(&po, p.piece, vp, p.N, pl.pitch, 32))) return s;
-    TcGemm g{};
-    g.M = p.N, g.N = vp, g.k_blocks = d_blocks, g.z = 1, g.group = row_group(p.D);
-    g.col0 = v0;
-    if ((s = launch<kTcGrad, false, false>(hk, wk, po, g, p, "vl_tc_kernel (logits' gradient)"))) return s;
-    if (p.dweight) {
-      __nv_bfloat16* dw = (__nv_bfloat16*)p.dweight + v0 * p.D;
-      TcGemm gw{};
-      gw.M = vp, gw.N = p.D, gw.k_blocks = (int)((p.N + kKB - 1) / kKB), gw.z = pl.z_w, gw.group = 1, gw.out_ld = p.D;
-      if (pl.z_w == 1) {
-        CUtensorMap wo;
-        if ((s = matrix_map(&wo, dw, p.D, vp, p.D, 32))) return s;
-        if ((s = launch<kTcStore, true, true>(pm, hm, wo, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
-      } else {
-        gw.out = p.acc_w;
-        if ((s = launch<kTcAdd, true, true>(pm, hm, pm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
-        if ((s = finish_launch(p, p.acc_w, pl.z_w, vp * p.D, dw, DYNCONV_DTYPE_BF16))) return s;
-      }
-    }
-    if (p.dhidden) {
-      TcGemm gh{};
-      gh.M = p.N, gh.N = p.D, gh.k_blocks = (int)((vp + kKB - 1) / kKB), gh.group = 1;
-      // the first piece fills every share; a short last one may have fewer blocks than shares
-      gh.z = pl.z_h < gh.k_blocks ? pl.z_h : gh.k_blocks;
-      gh.out = p.acc_h, gh.out_ld = p.D, gh.add = v0 > 0;
-      gh.result = pl.z_h == 1 && v0 + vp == p.V ? p.dhidden : nullptr;
-      if ((s = launch<kTcAdd, false, true>(pk, wm, pk, gh, p, "vl_tc_kernel (hidden gradient)"))) return s;
-    }
-  }
-  if (!p.dhidden || pl.z_h == 1) return DYNCONV_OK;
-  return finish_launch(p, p.acc_h, pl.z_h, p.N * p.D, p.dhidden, DYNCONV_DTYPE_BF16);
+int tc_bwd(const Problem& p, const Plan& pl, int dtype) {
+  return dtype == DYNCONV_DTYPE_F32 ? bwd<true>(p, pl) : bwd<false>(p, pl);
 }
 
 }  // namespace vl

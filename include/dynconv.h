@@ -313,6 +313,9 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
  *   reduction: 0 none (loss [N]), 1 sum, 2 mean over the rows that count (loss [1]; NaN
  *   when none does).  loss, lse [N] and stats [2] are float32; lse and stats are kept for
  *   the backward (stats: sum of the rows' losses, number of rows that count).
+ * float32 tensors are multiplied as three bf16 parts each, which the workspaces hold (6
+ * bytes per number of hidden, and of at most 512 MB of parts of weight): these workspaces
+ * are 16-byte aligned (DYNCONV_ERR_ALIGN).
  * N <= 2^30, V <= 4194304. */
 size_t dynconv_vocab_loss_fwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype);
 int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t* target,
@@ -321,7 +324,8 @@ int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t
                            int dtype, void* stream);
 /* Gradients for dloss ([N] or [1] float32, as loss).  dhidden [N,D] or dweight [V,D] may be
  * NULL (not wanted).  The logits' gradient is rounded to `dtype` before its two products
- * (bf16 tensor-core operands), which accumulate in float32; no atomics. */
+ * (bf16 tensor-core operands; for float32 three bf16 parts that hold all of it), which
+ * accumulate in float32; no atomics. */
 size_t dynconv_vocab_loss_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype,
                                               int want_dhidden, int want_dweight);
 int dynconv_vocab_loss_bwd(const void* hidden, const void* weight, const int64_t* target,

@@ -250,6 +250,62 @@ def test_same_bits_again_and_other_stream():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("N,D,V", [(300, 256, 600), (130, 320, 700), (700, 1000, 900), (1021, 256, 4999), (40, 2048, 300), (2000, 129, 257)])
+def test_fp32_keeps_its_digits(N, D, V):
+    """fp32 tensors are multiplied as three bf16 parts: 24 digits, of whose products those below
+    2^-23 are left out (2^-22 of a sum, for three of them), in tensor-core sums of 256 that lose
+    at most 2^-30 each time (2^-22), added up in fp32 (2^-24 for each 256).  Logits of up to 8 are
+    then off by 8 * 2^-21 = 2^-18 and exp() by that factor; the gradients' own sums add 2^-21
+    each: below 2^-17, where two parts, or bf16, would not come."""
+    h, w, t = make(N, D, V, torch.float32, seed=D)
+    own = [x.detach().requires_grad_() for x in (h, w)]
+    loss = linear_cross_entropy(*own, t)
+    loss.backward()
+    check_device(loss)
+    rl, rh, rw = definition(h, w, t, torch.tensor(1.0, device="cuda"), "mean")
+    got = (rel(loss, rl), rel(own[0].grad, rh), rel(own[1].grad, rw))
+    assert max(got) <= 2.0**-17, got
+
+
+def test_fp32_unaligned_and_odd_widths():
+    """The parts are copies of their own: any base and any width, the same result."""
+    shift = lambda x: torch.cat([x.new_zeros(1), x.flatten()])[1:].view(x.shape)  # noqa: E731
+    for D in (64, 66, 67):
+        h, w, t = make(200, D, 500, torch.float32)
+        for a, b in zip(check(h, w, t), check(shift(h), shift(w), t)):
+            assert torch.equal(a, b)
+
+
+def test_fp32_vocabulary_larger_than_its_parts_at_once():
+    """512 MB of parts hold 10752 words of 8192 channels."""
+    check(*make(40, 8192, 11000, torch.float32), loss_tol=2 * LOSS)
+
+
+def test_fp32_extremes():
+    """Numbers that would round to infinity in bf16 stay finite; NaN and infinite rows are NaN, and
+    ignored ones count for nothing in the loss."""
+    h, w, t = make(80, 64, 300, torch.float32, ignored=0.0)
+    h, w = h.clone(), w.clone()
+    h[:, 5] = 1e-30
+    w[:, 5] = 0.0
+    w[7, 5] = torch.finfo(torch.float32).max  # a logit of 3.4e8 in every row
+    rows = linear_cross_entropy(h, w, torch.full_like(t, 8), reduction="none")
+    want, _, _ = definition(h, w, torch.full_like(t, 8), torch.ones(80, device="cuda"), "none")
+    assert rel(rows, want) <= LOSS
+    w[7, 5] = 0.0
+    h[3, 3], h[4, 3], h[5, 3] = float("nan"), float("inf"), float("-inf")
+    rows = linear_cross_entropy(h, w, t, reduction="none")
+    assert rows[3:6].isnan().all() and rows.isnan().sum() == 3
+    t[3:6] = IGNORE
+    assert linear_cross_entropy(h, w, t).isfinite()
+
+
+def test_fp32_same_bits_again():
+    h, w, t = make(300, 136, 3000, torch.float32)
+    for a, b in zip(check(h, w, t), check(h, w, t)):
+        assert torch.equal(a, b)
+
+
 def test_refusals():
     h, w, t = make(10, 64, 50, torch.bfloat16)
     good = dict(hidden=h, weight=w, target=t)

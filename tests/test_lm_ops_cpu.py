@@ -8,7 +8,7 @@ import torch
 import dynamic_conv1d_b200 as dc
 from dynamic_conv1d_b200 import _lib
 
-SHAPE, UNSUPPORTED, WORKSPACE, ARGUMENT = 1, 3, 6, 7
+SHAPE, ALIGN, UNSUPPORTED, WORKSPACE, ARGUMENT = 1, 2, 3, 6, 7
 
 
 def test_step_validation():
@@ -59,6 +59,23 @@ def test_loss_validation():
     n = lib.dynconv_vocab_loss_bwd_workspace_bytes(65536, 1024, 131072, 0, 0, 1)
     assert 0 < n <= (1 << 30)
     assert lib.dynconv_vocab_loss_bwd_workspace_bytes(0, 64, 100, 0, 1, 1) == 0
+
+
+def test_loss_workspace_of_fp32_parts():
+    lib = _lib.load()
+    N, D, V = 4096, 2048, 131072
+    parts = 6 * N * D + (512 << 20)  # of hidden, and of as many words as 512 MB hold
+    n = lib.dynconv_vocab_loss_fwd_workspace_bytes(N, D, V, 1)
+    assert parts - (8 << 20) < n <= parts + 8 * N * (V // 64 + 2) + (1 << 20)
+    n = lib.dynconv_vocab_loss_bwd_workspace_bytes(N, D, V, 1, 1, 1)
+    assert 0 < n < 6 * N * D + (2 << 30)
+    # a vocabulary too wide for 1024 words of it in 512 MB still has a workspace
+    assert lib.dynconv_vocab_loss_fwd_workspace_bytes(1, 1 << 20, 5000, 1) >= 6 * 1024 << 20
+    # an unaligned workspace is refused before any launch
+    args = [256, 256, 256, 256, 256, 256, 264, 1 << 30, 4, 64, 100, -100, 2]
+    assert lib.dynconv_vocab_loss_fwd(*args, 1, None) == ALIGN
+    args = [256, 256, 256, 256, 256, 256, 256, 256, 264, 1 << 30, 4, 64, 100, -100, 2]
+    assert lib.dynconv_vocab_loss_bwd(*args, 1, None) == ALIGN
 
 
 def test_python_refuses_cpu_tensors():
