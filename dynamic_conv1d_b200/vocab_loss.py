@@ -4,7 +4,8 @@ logits (libdynconv's ``dynconv_vocab_loss_fwd`` / ``dynconv_vocab_loss_bwd``).
 The forward reads the hidden states and the vocabulary's weight once and keeps one float32
 per token (the logarithm of the sum of exponentials).  The backward computes the logits
 again, one piece of the vocabulary at a time, into a buffer that holds that piece's
-gradient only.
+gradient only.  float32 tensors are multiplied as three bfloat16 parts each, to float32
+accuracy.
 """
 from __future__ import annotations
 
