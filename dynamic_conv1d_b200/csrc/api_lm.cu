@@ -112,21 +112,24 @@ int check_loss(int64_t N, int64_t D, int64_t V, int reduction, int dtype) {
   return DYNCONV_OK;
 }
 
+bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
+
 struct LossBackwardBytes {
-  size_t piece, acc_h, acc_w, hidden_parts, weight_parts;
-  size_t total() const { return piece + acc_h + acc_w + hidden_parts + weight_parts; }
+  size_t piece, acc_h, acc_w, hidden_copy, weight_copy;
+  size_t total() const { return piece + acc_h + acc_w + hidden_copy + weight_copy; }
 };
 
 LossBackwardBytes loss_backward_bytes(const vl::Plan& pl, int64_t N, int64_t D, int dtype, int want_hidden,
                                       int want_weight) {
-  const bool split = dtype == DYNCONV_DTYPE_F32;
-  const size_t elem = split ? 2 * vl::kSplitParts : 2;
+  const bool copy = vl::copied(D, dtype);
+  const size_t elem = 2 * vl::parts_of(dtype);
+  const int64_t ld = copy ? vl::copy_pitch(D) : D;
   LossBackwardBytes b;
-  b.hidden_parts = split ? align_up(vl::part_bytes(N, D)) : 0;
-  b.weight_parts = split ? align_up(vl::part_bytes(pl.piece, D)) : 0;
+  b.hidden_copy = copy ? align_up(vl::copy_bytes(N, D, dtype)) : 0;
+  b.weight_copy = copy ? align_up(vl::copy_bytes(pl.piece, D, dtype)) : 0;
   b.piece = align_up((size_t)N * pl.pitch * elem);
-  b.acc_h = want_hidden ? align_up((size_t)pl.z_h * N * D * sizeof(float)) : 0;
-  b.acc_w = want_weight && pl.z_w > 1 ? align_up((size_t)pl.z_w * pl.piece * D * sizeof(float)) : 0;
+  b.acc_h = want_hidden ? align_up((size_t)pl.z_h * N * ld * sizeof(float)) : 0;
+  b.acc_w = want_weight && (pl.z_w > 1 || (copy && dtype == DYNCONV_DTYPE_BF16)) ? align_up((size_t)pl.z_w * pl.piece * ld * sizeof(float)) : 0;
   return b;
 }
 
@@ -236,11 +239,11 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
 
 size_t dynconv_vocab_loss_fwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype) {
   if (check_loss(N, D, V, 0, dtype)) return 0;
-  const int64_t tiles = (V + vl::kNarrowestTile - 1) / vl::kNarrowestTile + 2;  // enough for either path
+  const int64_t tiles = (V + vl::kTileColumns - 1) / vl::kTileColumns + 1;  // (an even number is written)
   const int64_t rows = std::min(N, vl::kRowsAtOnce);
   size_t n = align_up((size_t)tiles * rows * sizeof(float2)) + align_up((size_t)N * sizeof(float));
-  if (dtype == DYNCONV_DTYPE_F32)
-    n += align_up(vl::part_bytes(rows, D)) + align_up(vl::part_bytes(vl::words_at_once(D, V), D));
+  if (vl::copied(D, dtype))
+    n += align_up(vl::copy_bytes(rows, D, dtype)) + align_up(vl::copy_bytes(vl::words_at_once(D, V, dtype), D, dtype));
   return n;
 }
 
@@ -262,17 +265,18 @@ int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t
   const size_t need = dynconv_vocab_loss_fwd_workspace_bytes(N, D, V, dtype);
   if (!workspace || workspace_bytes < need)
     return set_error(DYNCONV_ERR_WORKSPACE, "vocab_loss_fwd: workspace %zu < %zu bytes", workspace_bytes, need);
-  if (dtype == DYNCONV_DTYPE_F32 && (reinterpret_cast<uintptr_t>(workspace) & 15))
-    return set_error(DYNCONV_ERR_ALIGN, "vocab_loss_fwd: workspace not 16-byte aligned");
+  if (misaligned(workspace) ||
+      (!vl::copied(D, dtype) && (misaligned(hidden) || misaligned(weight))))
+    return set_error(DYNCONV_ERR_ALIGN, "vocab_loss_fwd: workspace or bf16 tensor not 16-byte aligned");
   p.tgt = (float*)workspace;
   p.part = (float2*)((char*)workspace + align_up((size_t)N * sizeof(float)));
-  if (dtype == DYNCONV_DTYPE_F32) {  // (the parts of the tensors end the workspace)
-    const size_t words = align_up(vl::part_bytes(vl::words_at_once(D, V), D));
-    p.weight_parts = (__nv_bfloat16*)((char*)workspace + need - words);
-    p.hidden_parts =
-        (__nv_bfloat16*)((char*)p.weight_parts - align_up(vl::part_bytes(std::min(N, vl::kRowsAtOnce), D)));
+  if (vl::copied(D, dtype)) {  // (the copies end the workspace)
+    const size_t words = align_up(vl::copy_bytes(vl::words_at_once(D, V, dtype), D, dtype));
+    const size_t rows = align_up(vl::copy_bytes(std::min(N, vl::kRowsAtOnce), D, dtype));
+    p.weight_copy = (__nv_bfloat16*)((char*)workspace + need - words);
+    p.hidden_copy = (__nv_bfloat16*)((char*)workspace + need - words - rows);
   }
-  return vl::tc_supported(p, dtype) ? vl::tc_fwd(p, dtype) : vl::simple_fwd(p);
+  return vl::forward(p, dtype);
 }
 
 size_t dynconv_vocab_loss_bwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int want_dhidden,
@@ -303,18 +307,18 @@ int dynconv_vocab_loss_bwd(const void* hidden, const void* weight, const int64_t
   p.lse = const_cast<float*>(lse), p.stats = const_cast<float*>(stats), p.dloss = dloss;
   p.dhidden = dhidden, p.dweight = dweight, p.st = st;
   p.piece = workspace;
-  const bool tc = vl::tc_supported(p, dtype);
   const vl::Plan pl = vl::plan(N, D, V, dtype);
   const LossBackwardBytes b = loss_backward_bytes(pl, N, D, dtype, dhidden != nullptr, dweight != nullptr);
   if (!workspace || workspace_bytes < b.total())
     return set_error(DYNCONV_ERR_WORKSPACE, "vocab_loss_bwd: workspace %zu < %zu bytes", workspace_bytes, b.total());
-  if (dtype == DYNCONV_DTYPE_F32 && (reinterpret_cast<uintptr_t>(workspace) & 15))
-    return set_error(DYNCONV_ERR_ALIGN, "vocab_loss_bwd: workspace not 16-byte aligned");
+  if (misaligned(workspace) ||
+      (!vl::copied(D, dtype) && (misaligned(hidden) || misaligned(weight) || misaligned(dhidden) || misaligned(dweight))))
+    return set_error(DYNCONV_ERR_ALIGN, "vocab_loss_bwd: workspace or bf16 tensor not 16-byte aligned");
   p.acc_h = (float*)((char*)workspace + b.piece);
   p.acc_w = (float*)((char*)workspace + b.piece + b.acc_h);
-  p.hidden_parts = (__nv_bfloat16*)((char*)workspace + b.piece + b.acc_h + b.acc_w);
-  p.weight_parts = (__nv_bfloat16*)((char*)p.hidden_parts + b.hidden_parts);
-  return tc ? vl::tc_bwd(p, pl, dtype) : vl::simple_bwd(p, pl);
+  p.hidden_copy = (__nv_bfloat16*)((char*)workspace + b.piece + b.acc_h + b.acc_w);
+  p.weight_copy = (__nv_bfloat16*)((char*)p.hidden_copy + b.hidden_copy);
+  return vl::backward(p, pl, dtype);
 }
 
 }  // extern "C"

@@ -12,8 +12,8 @@
 // per row (no reduction) the factors differ and are part of dl.
 // Forward: one matrix product whose epilogue keeps, of each tile, every row's maximum and
 // sum of exponentials (fp32); a second kernel merges the tiles.  Backward, piece of the
-// vocabulary by piece: the product again, with dl rounded to the tensors' type into a
-// piece buffer, then its two products.  dhidden accumulates in fp32 over the pieces.
+// vocabulary by piece: the product again, with dl in bf16 (three parts of it for fp32
+// tensors) into a piece buffer, then its two products.  dhidden accumulates in fp32 over the pieces.
 #pragma once
 
 #include "common.cuh"
@@ -43,12 +43,12 @@ struct Problem {
   const float* dloss;       // [N] (kNone) or [1]
   void* dhidden;            // [N, D] or null
   void* dweight;            // [V, D] or null
-  void* piece;              // [N, pitch]: dl of one piece of the vocabulary
-  float* acc_h;             // [z_h][N][D] fp32
-  float* acc_w;             // [z_w][piece rows][D] fp32, z_w > 1
-  // fp32 tensors, either way: three bf16 parts of each (pitch part_pitch(D))
-  __nv_bfloat16* hidden_parts;  // [3][N or rows at once][pitch]
-  __nv_bfloat16* weight_parts;  // [3][words at once][pitch]
+  void* piece;              // [parts][N][pitch]: dl of one piece of the vocabulary
+  float* acc_h;             // [z_h][N][D] fp32; rows of copy_pitch(D) where operands are copies
+  float* acc_w;             // [z_w][piece rows][D] fp32 likewise, where dweight is not written at once
+  // either way, where operands are copies
+  __nv_bfloat16* hidden_copy;  // [parts][N or rows at once][copy_pitch]
+  __nv_bfloat16* weight_copy;  // [parts][words at once][copy_pitch]
   cudaStream_t st;
 };
 
@@ -75,24 +75,27 @@ __device__ __forceinline__ float result_factor(const Problem& p) {
 // The forward takes this many rows at a time: it bounds the tiles' partial sums in the workspace
 // (8 bytes for each row and tile), and the weight is read again once per 32768 rows only.
 constexpr int64_t kRowsAtOnce = 32768;
-constexpr int kNarrowestTile = 64;  // columns of the vocabulary in one forward tile, at least
+constexpr int kTileColumns = 128;  // of the vocabulary: the forward keeps a (maximum, sum) for each
 
-// fp32 tensors on the tensor cores: x = x0 + x1 + x2, each part the rest rounded to bf16 (8
-// digits each: the three hold all 24), and a product of two such numbers is the six products of
-// parts whose indices add up to at most two; the three left out are below 2^-23 of it.
-constexpr int kSplitParts = 3, kSplitProducts = 6;
-// The tensor core's accumulation truncates (vocab_loss_tc.cu): 4 blocks of 64 inner elements
-// are summed there, and these sums in fp32 registers.
-constexpr int kSplitChain = 4;
-inline int64_t part_pitch(int64_t D) { return (D + 7) / 8 * 8; }
-inline size_t part_bytes(int64_t rows, int64_t D) { return (size_t)kSplitParts * 2 * rows * part_pitch(D); }
-// Words of the vocabulary whose parts are kept at once: at most 512 MB of them.
-inline int64_t words_at_once(int64_t D, int64_t V) {
-  const int64_t most = ((int64_t)512 << 20) / (2 * kSplitParts * part_pitch(D)) / 256 * 256;
+// The products run on bf16 operands that TMA can address.  fp32 tensors are copied as three bf16
+// parts: x = x0 + x1 + x2, each part the rest rounded to bf16 (8 digits each: the three hold all
+// 24), and a product of two such numbers is the six products of parts whose indices add up to at
+// most two; the three left out are below 2^-23 of it.  bf16 tensors whose rows are no multiple of
+// 16 bytes are copied as they are, with padded rows ("one part").
+inline bool copied(int64_t D, int dtype) { return dtype == DYNCONV_DTYPE_F32 || D % 8 != 0; }
+inline int parts_of(int dtype) { return dtype == DYNCONV_DTYPE_F32 ? 3 : 1; }
+__host__ __device__ constexpr int products_of(int parts) { return parts == 3 ? 6 : 1; }
+// The tensor core's accumulation truncates (vocab_loss_tc.cu): of copied operands, 4 blocks of 64
+// inner elements are summed there, and these sums in fp32 registers.
+constexpr int kCopyChain = 4;
+inline int64_t copy_pitch(int64_t D) { return (D + 7) / 8 * 8; }
+inline size_t copy_bytes(int64_t rows, int64_t D, int dtype) { return (size_t)parts_of(dtype) * 2 * rows * copy_pitch(D); }
+// Words of the vocabulary that are copied at once: at most 512 MB of copies.
+inline int64_t words_at_once(int64_t D, int64_t V, int dtype) {
+  const int64_t most = ((int64_t)512 << 20) / (int64_t)copy_bytes(1, D, dtype) / 256 * 256;
   return most < 1024 ? (V < 1024 ? V : 1024) : most < V ? most : V;
 }
 
-bool tc_supported(const Problem& p, int dtype);
 Plan plan(int64_t N, int64_t D, int64_t V, int dtype);
 int merge_launch(const Problem& rows, int64_t tiles);  // the rows' losses from their tiles
 int total_launch(const Problem& p);                    // their sum and number
@@ -105,13 +108,11 @@ inline Problem rows_from(const Problem& p, int64_t r0, int64_t elem) {
   if (p.reduction == kNone) r.loss += r0;
   return r;
 }
-// out[i] = result_factor * the sum of n-element parts, in part order, rounded to dtype
-int finish_launch(const Problem& p, const float* parts, int n_parts, int64_t n, void* out, int dtype);
+// out [rows][D] = result_factor * the sum of n_parts [rows][ld], in their order, rounded to dtype
+int finish_launch(const Problem& p, const float* parts, int n_parts, int64_t rows, int64_t ld, void* out, int dtype);
 
-int simple_fwd(const Problem& p);
-int simple_bwd(const Problem& p, const Plan& pl);
-int tc_fwd(const Problem& p, int dtype);
-int tc_bwd(const Problem& p, const Plan& pl, int dtype);
+int forward(const Problem& p, int dtype);
+int backward(const Problem& p, const Plan& pl, int dtype);
 
 }  // namespace vl
 }  // namespace dynconv

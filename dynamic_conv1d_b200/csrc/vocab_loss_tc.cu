@@ -1,5 +1,5 @@
-// vocab_loss_tc.cu -- the vocabulary loss on the tensor cores: bf16 tensors, and fp32 ones in three
-// bf16 parts.
+// vocab_loss_tc.cu -- the vocabulary loss's products, on the tensor cores: of bf16 tensors in place, of
+// fp32 ones as three bf16 parts, of bf16 rows that TMA cannot address as padded copies.
 //
 // One persistent kernel computes out(m, n) = sum_k A(m, k) B(n, k) for all four products;
 // only the operands' majors and the epilogue differ:
@@ -26,17 +26,17 @@
 // burst rate; back to back under the power limit the pass takes 10.6 ms (1.27 PFLOP/s; that
 // library product sustains 1.38).
 //
-// fp32 tensors (SPLIT) go through the same kernel: a small kernel writes each tensor as three bf16
-// parts (bound by HBM: 4 bytes read and 6 written for each number), the inner dimension is walked
-// once for each of six products of parts, and dl leaves the epilogue as parts too.  The sums of
-// 256 inner elements' products are added up in registers (the tensor core's sums alone would be
-// off by more than fp32's rounding).  Products at 1/6 of the bf16 rate are 3.5 times what the
-// fp32 units could do at their best.  Whole passes, forward and backward (B200; in brackets the CUDA
-// cores' tiles that did this before): 1021 tokens x 256 channels over 4999 words 35 + 103 us (90 + 233),
-// 1021 x 1024 x 8000 93 + 269 us (400 + 1226), 4096 x 2048 x 65536 5.0 + 16.2 ms (20.8 + 71.1):
-// 1.25 PFLOP/s of bf16 products.  Few rows gain only over large vocabularies, as the tensors are
-// written anew: one row of 256 x 4999 25 + 61 us (19 + 40), of 2048 x 65536 0.83 + 1.27 ms (0.63 +
-// 1.52), 32 rows of the latter 0.59 + 1.12 (0.65 + 1.67).
+// Copied operands (PARTS) go through the same kernel.  fp32: a small kernel writes each tensor as
+// three bf16 parts, the inner dimension is walked once for each of six products of parts, and dl
+// leaves the epilogue as parts too.  The sums of 256 inner elements' products are added up in
+// registers (the tensor core's sums alone would be off by more than fp32's rounding).  Products at
+// 1/6 of the bf16 rate are 3.5 times what the fp32 units could do at their best.  Whole passes, forward
+// and backward (B200; in brackets fp32 products on the CUDA cores, in tiles of 128 x 128): 1021 tokens x
+// 256 channels over 4999 words 35 + 101 us (90 + 233), 1021 x 1024 x 8000 93 + 269 us (400 + 1226), 4096 x
+// 2048 x 65536 5.0 + 16.2 ms (20.8 + 71.1): 1.25 PFLOP/s of bf16 products.  Few rows gain only over
+// large vocabularies, as the tensors are written anew: one row of 256 x 4999 25 + 61 us (19 + 40), of
+// 2048 x 65536 0.83 + 1.27 ms (0.63 + 1.52), 32 rows of the latter 0.59 + 1.12 (0.65 + 1.67).  bf16, 1021
+// x 257 x 4999: 118 us of kernels (430).
 #include "vocab_loss.cuh"
 
 namespace dynconv {
@@ -61,15 +61,11 @@ static_assert(kSmem <= 232448 - 1024, "shared memory of one CTA");
 constexpr int kChain = 32;
 constexpr int kHalf = kN / 2;  // columns of one epilogue warp; a forward tile's partials are per half
 
-// fp32 tensors in three bf16 parts (SPLIT): in blocks of 64 inner elements by product, kSplitChain
-// blocks' six products at a time, the smallest products first.
-constexpr int kSplitBlocks = kSplitChain * kSplitProducts;
-
 enum TcMode { kTcForward, kTcForwardLong, kTcGrad, kTcAdd, kTcStore };
 
 struct TcGemm {
   int64_t M, N;        // extents of the output
-  int k_blocks;        // 64-element blocks of the inner dimension (SPLIT: of each product)
+  int k_blocks;        // 64-element blocks of the inner dimension (COPIED: of each product of parts)
   int m_tiles, n_tiles, z;
   int group;           // m tiles that share a sweep over n: consecutive tiles walk a group's rows first
   int64_t col0;        // kTcGrad: first vocabulary column
@@ -77,14 +73,14 @@ struct TcGemm {
   int64_t out_ld;
   int add;             // kTcAdd: add to what is there
   void* result;        // kTcAdd: not null: the last sums, in the tensors' type
-  int vec;             // SPLIT kTcAdd: rows of out and result may be written 16 bytes at a time
+  int vec;             // COPIED kTcAdd: rows of result may be written 16 bytes at a time
 };
 
 struct Tile {
   int m, n, z, kb0, kb1;
 };
 
-template <bool SPLIT>
+template <int PARTS>
 __device__ __forceinline__ Tile tile_at(const TcGemm& g, int t) {
   Tile r;
   const int plane = g.m_tiles * g.n_tiles;
@@ -95,10 +91,11 @@ __device__ __forceinline__ Tile tile_at(const TcGemm& g, int t) {
   const int rows = min(g.group, g.m_tiles - grp * g.group);
   r.n = t / rows;
   r.m = grp * g.group + (t - r.n * rows);
-  if constexpr (SPLIT) {  // whole chains
-    const int64_t chains = (g.k_blocks + kSplitChain - 1) / kSplitChain;
-    r.kb0 = (int)(chains * r.z / g.z) * kSplitBlocks;
-    r.kb1 = min((int)(chains * (r.z + 1) / g.z) * kSplitBlocks, g.k_blocks * kSplitProducts);
+  if constexpr (PARTS > 0) {  // whole chains
+    const int64_t chains = (g.k_blocks + kCopyChain - 1) / kCopyChain;
+    constexpr int products = products_of(PARTS);
+    r.kb0 = (int)(chains * r.z / g.z) * kCopyChain * products;
+    r.kb1 = min((int)(chains * (r.z + 1) / g.z) * kCopyChain, g.k_blocks) * products;
   } else {
     r.kb0 = (int)((int64_t)g.k_blocks * r.z / g.z);
     r.kb1 = (int)((int64_t)g.k_blocks * (r.z + 1) / g.z);
@@ -106,16 +103,17 @@ __device__ __forceinline__ Tile tile_at(const TcGemm& g, int t) {
   return r;
 }
 
-// SPLIT: what the kb-th block of products multiplies.
-struct SplitBlock {
+// What the kb-th block of products of three parts multiplies: kCopyChain blocks' six products at a
+// time, the smallest products first.
+struct CopyBlock {
   int block, a, b;  // 64 inner elements, parts of A and B
 };
 
-__device__ __forceinline__ SplitBlock split_block(int k_blocks, int kb) {
-  const int chain = kb / kSplitBlocks, r = kb - chain * kSplitBlocks;
-  const int blocks = min(kSplitChain, k_blocks - chain * kSplitChain), product = r / blocks;
+__device__ __forceinline__ CopyBlock copy_block(int k_blocks, int kb) {
+  const int chain = kb / (kCopyChain * 6), r = kb - chain * kCopyChain * 6;
+  const int blocks = min(kCopyChain, k_blocks - chain * kCopyChain), product = r / blocks;
   // parts (0,2), (1,1), (2,0), (0,1), (1,0), (0,0)
-  return {chain * kSplitChain + r - product * blocks, 0x010210 >> (4 * product) & 3, 0x001012 >> (4 * product) & 3};
+  return {chain * kCopyChain + r - product * blocks, 0x010210 >> (4 * product) & 3, 0x001012 >> (4 * product) & 3};
 }
 
 // ---- a CTA pair: addresses in the first CTA, products over both
@@ -149,7 +147,7 @@ __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map,
       : "memory");
 }
 
-// The same from one of the parts of an fp32 tensor.
+// The same from one of a copy's parts.
 __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int part) {
   asm volatile(
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
@@ -208,62 +206,77 @@ __device__ __forceinline__ uint32_t take_part(float2& x) {
   return p;
 }
 
-// An fp32 matrix as its three parts.
-__global__ void __launch_bounds__(256) vl_split_kernel(const float* __restrict__ src, int64_t rows, int64_t D,
-                                                       int64_t pitch, __nv_bfloat16* __restrict__ parts) {
+// A matrix as its parts: fp32 as three, bf16 as it is; rows padded with zeros.
+template <typename In>
+__global__ void __launch_bounds__(256) vl_copy_kernel(const In* __restrict__ src, int64_t rows, int64_t D, int64_t pitch,
+                                                      __nv_bfloat16* __restrict__ copy) {
   const int64_t per = pitch / 8, n = rows * per, plane = rows * pitch;
   const bool vec = D % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t row = i / per, c = (i - row * per) * 8;
-    const float* s = src + row * D + c;
-    float2 v[4];
-    if (vec) {
-      const float4 lo = reinterpret_cast<const float4*>(s)[0], hi = reinterpret_cast<const float4*>(s)[1];
-      v[0] = make_float2(lo.x, lo.y), v[1] = make_float2(lo.z, lo.w);
-      v[2] = make_float2(hi.x, hi.y), v[3] = make_float2(hi.z, hi.w);
+    const In* s = src + row * D + c;
+    __nv_bfloat16* to = copy + row * pitch + c;
+    if constexpr (sizeof(In) == 2) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = c + j < D ? reinterpret_cast<const uint16_t*>(s)[j] : 0;
+      *reinterpret_cast<uint4*>(to) = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
     } else {
+      float2 v[4];
+      if (vec) {
+        const float4 lo = reinterpret_cast<const float4*>(s)[0], hi = reinterpret_cast<const float4*>(s)[1];
+        v[0] = make_float2(lo.x, lo.y), v[1] = make_float2(lo.z, lo.w);
+        v[2] = make_float2(hi.x, hi.y), v[3] = make_float2(hi.z, hi.w);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        v[j] = make_float2(c + 2 * j < D ? s[2 * j] : 0.f, c + 2 * j + 1 < D ? s[2 * j + 1] : 0.f);
+        for (int j = 0; j < 4; ++j)
+          v[j] = make_float2(c + 2 * j < D ? s[2 * j] : 0.f, c + 2 * j + 1 < D ? s[2 * j + 1] : 0.f);
+      }
+      // the first part is cut to bf16's range: a number close to fp32's largest stays finite, an
+      // infinity or a NaN becomes a NaN in the parts that follow
+      constexpr float kLargest = 3.38953139e38f;
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float2 cut = make_float2(fminf(fmaxf(v[j].x, -kLargest), kLargest), fminf(fmaxf(v[j].y, -kLargest), kLargest));
+        const float2 over = make_float2(v[j].x - cut.x, v[j].y - cut.y);  // zero, but for those
+        w[j] = take_part(cut);
+        v[j] = add2(cut, over);
+      }
+      *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+      for (int k = 1; k < 3; ++k)
+        *reinterpret_cast<uint4*>(to + k * plane) = make_uint4(take_part(v[0]), take_part(v[1]), take_part(v[2]), take_part(v[3]));
     }
-    // the first part is cut to bf16's range: a number close to fp32's largest stays finite, an
-    // infinity or a NaN becomes a NaN in the parts that follow
-    constexpr float kLargest = 3.38953139e38f;
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float2 cut = make_float2(fminf(fmaxf(v[j].x, -kLargest), kLargest), fminf(fmaxf(v[j].y, -kLargest), kLargest));
-      const float2 over = make_float2(v[j].x - cut.x, v[j].y - cut.y);  // zero, but for those
-      w[j] = take_part(cut);
-      v[j] = add2(cut, over);
-    }
-    __nv_bfloat16* to = parts + row * pitch + c;
-    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-#pragma unroll
-    for (int k = 1; k < kSplitParts; ++k)
-      *reinterpret_cast<uint4*>(to + k * plane) = make_uint4(take_part(v[0]), take_part(v[1]), take_part(v[2]), take_part(v[3]));
   }
 }
 
-// 16 columns of a row of fp32 sums, added up over pieces; the last ones are the result in fp32.
+// COPIED: 16 columns of a row of the fp32 sums (rows padded to whole 16 bytes), added up over pieces;
+// the last ones are the result in fp32.
 __device__ __forceinline__ void add_columns(const TcGemm& g, const float (&v)[16], int64_t row, int64_t col, int z,
                                             float factor) {
-  const float* o = (const float*)g.out + ((int64_t)z * g.M + row) * g.out_ld + col;
-  float* to = g.result ? (float*)g.result + row * g.out_ld + col : const_cast<float*>(o);
-  const float f = g.result ? factor : 1.f;
+  float* o = (float*)g.out + ((int64_t)z * g.M + row) * g.out_ld + col;
+  float* r = (float*)g.result + row * g.N + col;
 #pragma unroll
   for (int j = 0; j < 16; j += 4) {
-    if (g.vec && col + j < g.N) {  // (N is a multiple of four)
-      float4 u = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-      if (g.add) {
-        const float4 w = *reinterpret_cast<const float4*>(o + j);
-        u.x += w.x, u.y += w.y, u.z += w.z, u.w += w.w;
-      }
-      *reinterpret_cast<float4*>(to + j) = make_float4(u.x * f, u.y * f, u.z * f, u.w * f);
+    if (col + j >= g.N) break;
+    float4 u = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    if (g.add) {
+      const float4 w = *reinterpret_cast<const float4*>(o + j);
+      u.x += w.x, u.y += w.y, u.z += w.z, u.w += w.w;
+    }
+    if (!g.result) {
+      *reinterpret_cast<float4*>(o + j) = u;
+      continue;
+    }
+    u.x *= factor, u.y *= factor, u.z *= factor, u.w *= factor;
+    if (g.vec) {
+      *reinterpret_cast<float4*>(r + j) = u;
     } else {
-#pragma unroll
-      for (int i = j; i < j + 4; ++i)
-        if (col + i < g.N) to[i] = (v[i] + (g.add ? o[i] : 0.f)) * f;
+      r[j] = u.x;
+      if (col + j + 1 < g.N) r[j + 1] = u.y;
+      if (col + j + 2 < g.N) r[j + 2] = u.z;
+      if (col + j + 3 < g.N) r[j + 3] = u.w;
     }
   }
 }
@@ -305,13 +318,14 @@ __device__ __forceinline__ void stage_columns(uint8_t* tile, int row, int half, 
   }
 }
 
-template <int MODE, bool A_MN, bool B_MN, bool SPLIT>
+template <int MODE, bool A_MN, bool B_MN, int PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     vl_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                  const __grid_constant__ CUtensorMap omap, const __grid_constant__ TcGemm g, const __grid_constant__ Problem p) {
+  constexpr bool COPIED = PARTS > 0;
   constexpr bool kForward = MODE == kTcForward || MODE == kTcForwardLong;
-  constexpr bool kChained = MODE == kTcForwardLong || SPLIT;  // sums of kBlocks blocks are added up in registers
-  constexpr int kBlocks = SPLIT ? kSplitBlocks : kChain;
+  constexpr bool kChained = MODE == kTcForwardLong || COPIED;  // sums of kBlocks blocks are added up in registers
+  constexpr int kBlocks = COPIED ? kCopyChain * products_of(PARTS) : kChain;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
   // full and acce are used in the first CTA only; empty and accf in both
@@ -349,7 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       int it = 0;
       bool dead = false;
       for (int i = pair; i < n_tiles && !dead; i += pairs) {
-        const Tile t = tile_at<SPLIT>(g, i);
+        const Tile t = tile_at<PARTS>(g, i);
         const int m0 = t.m * kM + rank * kHalfM, n0 = t.n * kN + rank * kHalfB;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
           const int s = it % kStages;
@@ -363,25 +377,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           // the first CTA announces both CTAs' bytes (the other's may land before: the phase
           // still waits for this arrival)
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * kStageBytes);
-          SplitBlock sp{kb, 0, 0};
-          if constexpr (SPLIT) sp = split_block(g.k_blocks, kb);
+          CopyBlock cb{kb, 0, 0};
+          if constexpr (PARTS == 3) cb = copy_block(g.k_blocks, kb);
           auto load = [&](uint8_t* dst, const CUtensorMap* map, int c0, int c1, int part) {
-            if constexpr (SPLIT)
+            if constexpr (COPIED)
               tma_load_pair(dst, map, full, c0, c1, part);
             else
               tma_load_pair(dst, map, full, c0, c1);
           };
           if constexpr (A_MN) {
 #pragma unroll
-            for (int j = 0; j < kHalfM / 64; ++j) load(a + j * kAtom, &amap, m0 + j * 64, sp.block * kKB, sp.a);
+            for (int j = 0; j < kHalfM / 64; ++j) load(a + j * kAtom, &amap, m0 + j * 64, cb.block * kKB, cb.a);
           } else {
-            load(a, &amap, sp.block * kKB, m0, sp.a);
+            load(a, &amap, cb.block * kKB, m0, cb.a);
           }
           if constexpr (B_MN) {
 #pragma unroll
-            for (int j = 0; j < kHalfB / 64; ++j) load(b + j * kAtom, &bmap, n0 + j * 64, sp.block * kKB, sp.b);
+            for (int j = 0; j < kHalfB / 64; ++j) load(b + j * kAtom, &bmap, n0 + j * 64, cb.block * kKB, cb.b);
           } else {
-            load(b, &bmap, sp.block * kKB, n0, sp.b);
+            load(b, &bmap, cb.block * kKB, n0, cb.b);
           }
         }
       }
@@ -400,7 +414,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       int it = 0, n = 0;
       bool dead = false;
       for (int i = pair; i < n_tiles && !dead; i += pairs, ++n) {
-        const Tile t = tile_at<SPLIT>(g, i);
+        const Tile t = tile_at<PARTS>(g, i);
         int a = n & 1, first = t.kb0;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
           if (kb == t.kb0 || (kChained && kb - first == kBlocks)) {
@@ -442,7 +456,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     const float factor = MODE == kTcAdd || MODE == kTcStore ? result_factor(p) : 1.f;
     const uint32_t freed[2] = {in_first_cta(&acce_bar[0]), in_first_cta(&acce_bar[1])};
     for (int i = pair; i < n_tiles; i += pairs, ++n) {
-      const Tile t = tile_at<SPLIT>(g, i);
+      const Tile t = tile_at<PARTS>(g, i);
       int a = n & 1;
       const int64_t row = (int64_t)t.m * kM + rank * kHalfM + q * 32 + lane;
       const int64_t col0 = (int64_t)t.n * kN + half * kHalf;
@@ -458,9 +472,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      float chained[kChained ? kHalf : 1];  // the sums of the chains before the last (SPLIT: of all)
+      float chained[kChained ? kHalf : 1];  // the sums of the chains before the last (COPIED: of all)
       if constexpr (kChained) {
-        const int chains = (t.kb1 - t.kb0 + kBlocks - 1) / kBlocks, early = SPLIT ? chains : chains - 1;
+        const int chains = (t.kb1 - t.kb0 + kBlocks - 1) / kBlocks, early = COPIED ? chains : chains - 1;
 #pragma unroll
         for (int j = 0; j < kHalf; ++j) chained[j] = 0.f;
 #pragma unroll 1
@@ -483,10 +497,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           __syncwarp();
           if (lane == 0) arrive_in_first_cta(freed[a]);
         }
-        if constexpr (SPLIT) --n;
+        if constexpr (COPIED) --n;
         a = n & 1;
       }
-      if constexpr (!SPLIT) {
+      if constexpr (!COPIED) {
         if (!dead) dead = !mbar_wait(&accf_bar[a], (n >> 1) & 1, kErrWaitEpilogue, &abort_flag);
         tc_fence_after();
       }
@@ -500,7 +514,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 #pragma unroll (kChained ? kHalf / kStep : 1)
         for (int c = 0; c < kHalf; c += kStep) {
           float v[kStep];
-          if constexpr (SPLIT) {
+          if constexpr (COPIED) {
 #pragma unroll
             for (int j = 0; j < kStep; ++j) v[j] = chained[c + j];
           } else if constexpr (kChained) {
@@ -544,11 +558,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             }
           } else if constexpr (MODE == kTcAdd) {
             if (row_in) add_columns(g, v, row, col0 + c, t.z, factor);
-          } else if constexpr (SPLIT) {
+          } else if constexpr (COPIED) {
             logits_gradient(v, f, lse2, target - g.col0 - (col0 + c));
 #pragma unroll
             for (int j = 0; j < kStep; ++j) chained[c + j] = v[j];
-            // 64 columns at a time, part by part, through the staged tile (1021 x 256 x 4999: 102 us for the
+            // 64 columns at a time, part by part, through the staged tile (fp32, 1021 x 256 x 4999: 102 us for the
             // backward, where 16-byte stores from each row's thread take 114)
             if ((c + kStep) % 64 == 0) {
               uint8_t* tile = smem + kStages * kStageBytes + (warp - 2) * kStageOut;
@@ -557,7 +571,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 #pragma unroll
               for (int j = 0; j < 32; ++j) pr[j] = make_float2(chained[from + 2 * j], chained[from + 2 * j + 1]);
 #pragma unroll
-              for (int k = 0; k < kSplitParts; ++k) {
+              for (int k = 0; k < PARTS; ++k) {
                 if (lane == 0) bulk_wait_group_read<0>();
                 __syncwarp();
 #pragma unroll
@@ -601,7 +615,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           if (row_in) p.part[((int64_t)t.n * 2 + half) * g.M + row] = make_float2(m2, sum);
         }
       }
-      if constexpr (!SPLIT) {  // (SPLIT has given its accumulators back one by one)
+      if constexpr (!COPIED) {  // (COPIED has given its accumulators back one by one)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_in_first_cta(freed[a]);
@@ -617,17 +631,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
-// A row-major [rows][cols] bf16 matrix as boxes of 64 columns x box_rows rows, 128-byte swizzle; with
-// PARTS, the three parts of an fp32 one.
-template <bool PARTS>
-int matrix_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows, int64_t plane = 0) {
-  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, kSplitParts};
-  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
+// A row-major [rows][cols] bf16 matrix as boxes of 64 columns x box_rows rows, 128-byte swizzle; of a
+// copy, its parts one behind the other (0: no copy).
+int matrix_map(CUtensorMap* map, int parts, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows) {
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)parts};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(rows * ld) * 2};
   const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
-  return encode_tensor_map_bf16(map, base, PARTS ? 3 : 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  return encode_tensor_map_bf16(map, base, parts ? 3 : 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int MODE, bool A_MN, bool B_MN, bool SPLIT>
+template <int MODE, bool A_MN, bool B_MN, int PARTS>
 int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, TcGemm g, const Problem& p, const char* what) {
   const int64_t mt = (g.M + kM - 1) / kM, nt = (g.N + kN - 1) / kN;
   if (mt * nt * g.z > INT32_MAX) return set_error(DYNCONV_ERR_SHAPE, "%s: too many tiles", what);
@@ -636,55 +649,64 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& o, TcG
   const int tiles = g.m_tiles * g.n_tiles * g.z, most = sm_count() / 2;
   const int grid = 2 * (tiles < most ? tiles : most);
   cudaError_t e =
-      cudaFuncSetAttribute(vl_tc_kernel<MODE, A_MN, B_MN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      cudaFuncSetAttribute(vl_tc_kernel<MODE, A_MN, B_MN, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return cuda_status(e, "cudaFuncSetAttribute(vl_tc)");
   }
-  vl_tc_kernel<MODE, A_MN, B_MN, SPLIT><<<grid, kTcThreads, kSmem, p.st>>>(a, b, o, g, p);
+  vl_tc_kernel<MODE, A_MN, B_MN, PARTS><<<grid, kTcThreads, kSmem, p.st>>>(a, b, o, g, p);
   DYNCONV_CHECK_LAUNCH(what);
   return DYNCONV_OK;
 }
 
-int split_launch(const Problem& p, const float* src, int64_t rows, __nv_bfloat16* parts) {
-  const int64_t pitch = part_pitch(p.D), most = 16 * (int64_t)sm_count();
-  const int64_t grid = (rows * (pitch / 8) + 255) / 256;
-  vl_split_kernel<<<(unsigned)(grid < most ? grid : most), 256, 0, p.st>>>(src, rows, p.D, pitch, parts);
-  DYNCONV_CHECK_LAUNCH("vl_split_kernel");
+int copy_launch(const Problem& p, const void* src, int64_t rows, int dtype, __nv_bfloat16* copy) {
+  const int64_t pitch = copy_pitch(p.D), most = 16 * (int64_t)sm_count();
+  int64_t grid = (rows * (pitch / 8) + 255) / 256;
+  if (grid > most) grid = most;
+  if (dtype == DYNCONV_DTYPE_F32)
+    vl_copy_kernel<<<(unsigned)grid, 256, 0, p.st>>>((const float*)src, rows, p.D, pitch, copy);
+  else
+    vl_copy_kernel<<<(unsigned)grid, 256, 0, p.st>>>((const __nv_bfloat16*)src, rows, p.D, pitch, copy);
+  DYNCONV_CHECK_LAUNCH("vl_copy_kernel");
   return DYNCONV_OK;
 }
 
 // Rows of hidden (a group) that stay in L2 while the vocabulary is swept over them: half of it.
-int row_group(int64_t row_bytes) {
-  const int64_t g = ((int64_t)64 << 20) / (kM * row_bytes);
+int row_group(int64_t D, int dtype) {
+  const int64_t g = ((int64_t)64 << 20) / (kM * (int64_t)copy_bytes(1, D, dtype));
   return g < 1 ? 1 : (int)(g < 4096 ? g : 4096);
 }
 
 int blocks_of(int64_t n) { return (int)((n + kKB - 1) / kKB); }
 
-template <bool SPLIT>
-int fwd(const Problem& all) {
-  const int64_t words = SPLIT ? words_at_once(all.D, all.V) : all.V, ld = SPLIT ? part_pitch(all.D) : all.D;
+template <int PARTS>
+int fwd(const Problem& all, int dtype) {
+  constexpr bool COPIED = PARTS > 0;
+  const int64_t words = COPIED ? words_at_once(all.D, all.V, dtype) : all.V, ld = COPIED ? copy_pitch(all.D) : all.D;
+  const int64_t elem = dtype == DYNCONV_DTYPE_F32 ? 4 : 2;
   int s;
   for (int64_t r0 = 0; r0 < all.N; r0 += kRowsAtOnce) {
-    Problem p = rows_from(all, r0, SPLIT ? 4 : 2);
-    if (SPLIT && (s = split_launch(p, (const float*)p.hidden, p.N, p.hidden_parts))) return s;
+    const Problem p = rows_from(all, r0, elem);
+    if (COPIED && (s = copy_launch(p, p.hidden, p.N, dtype, p.hidden_copy))) return s;
     CUtensorMap a;
-    if ((s = matrix_map<SPLIT>(&a, SPLIT ? p.hidden_parts : p.hidden, p.D, p.N, ld, kHalfM, p.N * ld))) return s;
+    if ((s = matrix_map(&a, PARTS, COPIED ? p.hidden_copy : p.hidden, p.D, p.N, ld, kHalfM))) return s;
     TcGemm g{};
-    g.M = p.N, g.k_blocks = blocks_of(p.D), g.z = 1, g.group = row_group(p.D * (SPLIT ? 2 * kSplitParts : 2));
+    g.M = p.N, g.k_blocks = blocks_of(p.D), g.z = 1, g.group = row_group(p.D, dtype);
     for (int64_t v0 = 0; v0 < p.V; v0 += words) {  // (words: all, or a multiple of a tile's)
+      const void* w = p.weight;
       g.N = p.V - v0 < words ? p.V - v0 : words, g.col0 = v0;
-      if (SPLIT && (r0 == 0 || words < p.V) &&
-          (s = split_launch(p, (const float*)p.weight + v0 * p.D, g.N, p.weight_parts)))
-        return s;
+      if constexpr (COPIED) {
+        if (r0 == 0 || words < p.V)
+          if ((s = copy_launch(p, (const char*)w + v0 * p.D * elem, g.N, dtype, p.weight_copy))) return s;
+        w = p.weight_copy;
+      }
       CUtensorMap b;
-      if ((s = matrix_map<SPLIT>(&b, SPLIT ? p.weight_parts : p.weight, p.D, g.N, ld, kHalfB, g.N * ld))) return s;
+      if ((s = matrix_map(&b, PARTS, w, p.D, g.N, ld, kHalfB))) return s;
       Problem tiles = p;
       tiles.part += v0 / kHalf * p.N;
-      s = SPLIT || g.k_blocks <= kChain
-              ? launch<kTcForward, false, false, SPLIT>(a, b, a, g, tiles, "vl_tc_kernel (forward)")
-              : launch<kTcForwardLong, false, false, false>(a, b, a, g, tiles, "vl_tc_kernel (forward)");
+      s = COPIED || g.k_blocks <= kChain
+              ? launch<kTcForward, false, false, PARTS>(a, b, a, g, tiles, "vl_tc_kernel (forward)")
+              : launch<kTcForwardLong, false, false, 0>(a, b, a, g, tiles, "vl_tc_kernel (forward)");
       if (s) return s;
     }
     if ((s = merge_launch(p, (p.V + kN - 1) / kN * 2))) return s;
@@ -692,85 +714,86 @@ int fwd(const Problem& all) {
   return total_launch(all);
 }
 
-template <bool SPLIT>
-int bwd(const Problem& p, const Plan& pl) {
-  constexpr int kType = SPLIT ? DYNCONV_DTYPE_F32 : DYNCONV_DTYPE_BF16, kElem = SPLIT ? 4 : 2;
-  const int64_t ld = SPLIT ? part_pitch(p.D) : p.D;
+template <int PARTS>
+int bwd(const Problem& p, const Plan& pl, int dtype) {
+  constexpr bool COPIED = PARTS > 0;
+  const int64_t ld = COPIED ? copy_pitch(p.D) : p.D, elem = dtype == DYNCONV_DTYPE_F32 ? 4 : 2;
   // shares of an inner dimension: each has a block, or a chain, at least
   const auto shares = [](int z, int blocks) {
-    const int most = SPLIT ? (blocks + kSplitChain - 1) / kSplitChain : blocks;
+    const int most = COPIED ? (blocks + kCopyChain - 1) / kCopyChain : blocks;
     return z < most ? z : most;
   };
-  const auto vec = [&](const void* q) { return SPLIT && p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  const auto vec = [&](const void* q) { return COPIED && p.D % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  // the products' sums are the result itself (fp32, or bf16 rows of whole 16 bytes)
+  const bool direct = !COPIED || dtype == DYNCONV_DTYPE_F32;
   int s;
-  if (SPLIT && (s = split_launch(p, (const float*)p.hidden, p.N, p.hidden_parts))) return s;
-  const void* hidden = SPLIT ? p.hidden_parts : p.hidden;
+  const void* hidden = p.hidden;
+  if constexpr (COPIED) {
+    if ((s = copy_launch(p, hidden, p.N, dtype, p.hidden_copy))) return s;
+    hidden = p.hidden_copy;
+  }
   CUtensorMap hk, hm;
-  if ((s = matrix_map<SPLIT>(&hk, hidden, p.D, p.N, ld, kHalfM, p.N * ld))) return s;
-  if ((s = matrix_map<SPLIT>(&hm, hidden, p.D, p.N, ld, 64, p.N * ld))) return s;
+  if ((s = matrix_map(&hk, PARTS, hidden, p.D, p.N, ld, kHalfM))) return s;
+  if ((s = matrix_map(&hm, PARTS, hidden, p.D, p.N, ld, 64))) return s;
   for (int64_t v0 = 0; v0 < p.V; v0 += pl.piece) {
     const int64_t vp = p.V - v0 < pl.piece ? p.V - v0 : pl.piece;
-    const void* w = (const char*)p.weight + v0 * p.D * kElem;
-    if (SPLIT) {
-      if ((s = split_launch(p, (const float*)w, vp, p.weight_parts))) return s;
-      w = p.weight_parts;
+    const void* w = (const char*)p.weight + v0 * p.D * elem;
+    if constexpr (COPIED) {
+      if ((s = copy_launch(p, w, vp, dtype, p.weight_copy))) return s;
+      w = p.weight_copy;
     }
     // maps of exactly this piece: what lies beyond it reads as zero
     CUtensorMap wk, wm, pk, pm, po;
-    if ((s = matrix_map<SPLIT>(&wk, w, p.D, vp, ld, kHalfB, vp * ld))) return s;
-    if ((s = matrix_map<SPLIT>(&wm, w, p.D, vp, ld, 64, vp * ld))) return s;
-    if ((s = matrix_map<SPLIT>(&pk, p.piece, vp, p.N, pl.pitch, kHalfM, p.N * pl.pitch))) return s;
-    if ((s = matrix_map<SPLIT>(&pm, p.piece, vp, p.N, pl.pitch, 64, p.N * pl.pitch))) return s;
-    if ((s = matrix_map<SPLIT>(&po, p.piece, vp, p.N, pl.pitch, 32, p.N * pl.pitch))) return s;
+    if ((s = matrix_map(&wk, PARTS, w, p.D, vp, ld, kHalfB))) return s;
+    if ((s = matrix_map(&wm, PARTS, w, p.D, vp, ld, 64))) return s;
+    if ((s = matrix_map(&pk, PARTS, p.piece, vp, p.N, pl.pitch, kHalfM))) return s;
+    if ((s = matrix_map(&pm, PARTS, p.piece, vp, p.N, pl.pitch, 64))) return s;
+    if ((s = matrix_map(&po, PARTS, p.piece, vp, p.N, pl.pitch, 32))) return s;
     TcGemm g{};
-    g.M = p.N, g.N = vp, g.k_blocks = blocks_of(p.D), g.z = 1, g.group = row_group(p.D * (SPLIT ? 2 * kSplitParts : 2));
+    g.M = p.N, g.N = vp, g.k_blocks = blocks_of(p.D), g.z = 1, g.group = row_group(p.D, dtype);
     g.col0 = v0;
-    if ((s = launch<kTcGrad, false, false, SPLIT>(hk, wk, po, g, p, "vl_tc_kernel (logits' gradient)"))) return s;
+    if ((s = launch<kTcGrad, false, false, PARTS>(hk, wk, po, g, p, "vl_tc_kernel (logits' gradient)"))) return s;
     if (p.dweight) {
-      void* dw = (char*)p.dweight + v0 * p.D * kElem;
+      void* dw = (char*)p.dweight + v0 * p.D * elem;
+      const bool finish = pl.z_w > 1 || !direct;
       TcGemm gw{};
-      gw.M = vp, gw.N = p.D, gw.k_blocks = blocks_of(p.N), gw.group = 1, gw.out_ld = p.D;
+      gw.M = vp, gw.N = p.D, gw.k_blocks = blocks_of(p.N), gw.group = 1, gw.out_ld = ld;
       gw.z = shares(pl.z_w, gw.k_blocks);
-      gw.out = p.acc_w, gw.vec = vec(p.acc_w);
-      if (pl.z_w == 1 && !SPLIT) {
+      gw.out = p.acc_w;
+      if (!COPIED && !finish) {
         CUtensorMap wo;
-        if ((s = matrix_map<false>(&wo, dw, p.D, vp, p.D, 32))) return s;
-        if ((s = launch<kTcStore, true, true, false>(pm, hm, wo, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
+        if ((s = matrix_map(&wo, 0, dw, p.D, vp, p.D, 32))) return s;
+        if ((s = launch<kTcStore, true, true, 0>(pm, hm, wo, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
       } else {
-        if (pl.z_w == 1) gw.result = dw, gw.vec = vec(dw);
-        if ((s = launch<kTcAdd, true, true, SPLIT>(pm, hm, pm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
-        if (pl.z_w > 1 && (s = finish_launch(p, p.acc_w, gw.z, vp * p.D, dw, kType))) return s;
+        if (!finish) gw.result = dw, gw.vec = vec(dw);
+        if ((s = launch<kTcAdd, true, true, PARTS>(pm, hm, pm, gw, p, "vl_tc_kernel (weight gradient)"))) return s;
+        if (finish && (s = finish_launch(p, p.acc_w, gw.z, vp, ld, dw, dtype))) return s;
       }
     }
     if (p.dhidden) {
       TcGemm gh{};
       gh.M = p.N, gh.N = p.D, gh.k_blocks = blocks_of(vp), gh.group = 1;
       gh.z = shares(pl.z_h, gh.k_blocks);  // the first piece fills every share; a short last one may not
-      gh.out = p.acc_h, gh.out_ld = p.D, gh.add = v0 > 0;
-      gh.result = pl.z_h == 1 && v0 + vp == p.V ? p.dhidden : nullptr;
-      gh.vec = vec(p.acc_h) && (!gh.result || vec(gh.result));
-      if ((s = launch<kTcAdd, false, true, SPLIT>(pk, wm, pk, gh, p, "vl_tc_kernel (hidden gradient)"))) return s;
+      gh.out = p.acc_h, gh.out_ld = ld, gh.add = v0 > 0;
+      gh.result = direct && pl.z_h == 1 && v0 + vp == p.V ? p.dhidden : nullptr;
+      gh.vec = vec(gh.result);
+      if ((s = launch<kTcAdd, false, true, PARTS>(pk, wm, pk, gh, p, "vl_tc_kernel (hidden gradient)"))) return s;
     }
   }
-  if (!p.dhidden || pl.z_h == 1) return DYNCONV_OK;
-  return finish_launch(p, p.acc_h, pl.z_h, p.N * p.D, p.dhidden, kType);
+  if (!p.dhidden || (direct && pl.z_h == 1)) return DYNCONV_OK;
+  return finish_launch(p, p.acc_h, pl.z_h, p.N, ld, p.dhidden, dtype);
 }
 
 }  // namespace
 
-bool tc_supported(const Problem& p, int dtype) {
-  if (dtype == DYNCONV_DTYPE_F32) return true;  // (its operands are copies)
-  if (p.D % 8 != 0) return false;
-  const void* ptrs[] = {p.hidden, p.weight, p.dhidden, p.dweight, p.piece};
-  for (const void* q : ptrs)
-    if (reinterpret_cast<uintptr_t>(q) & 15) return false;
-  return true;
+int forward(const Problem& p, int dtype) {
+  if (!copied(p.D, dtype)) return fwd<0>(p, dtype);
+  return parts_of(dtype) == 3 ? fwd<3>(p, dtype) : fwd<1>(p, dtype);
 }
 
-int tc_fwd(const Problem& p, int dtype) { return dtype == DYNCONV_DTYPE_F32 ? fwd<true>(p) : fwd<false>(p); }
-
-int tc_bwd(const Problem& p, const Plan& pl, int dtype) {
-  return dtype == DYNCONV_DTYPE_F32 ? bwd<true>(p, pl) : bwd<false>(p, pl);
+int backward(const Problem& p, const Plan& pl, int dtype) {
+  if (!copied(p.D, dtype)) return bwd<0>(p, pl, dtype);
+  return parts_of(dtype) == 3 ? bwd<3>(p, pl, dtype) : bwd<1>(p, pl, dtype);
 }
 
 }  // namespace vl

@@ -16,6 +16,12 @@ from . import _lib
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
+def _aligned(t):
+    """t at a 16-byte boundary, where its rows of bfloat16 are whole multiples of 16 bytes (the
+    library then reads them in place)."""
+    return t.clone() if t.dtype == torch.bfloat16 and t.shape[1] % 8 == 0 and t.data_ptr() % 16 else t
+
+
 class _LinearCrossEntropyFn(torch.autograd.Function):
     @staticmethod
     @_lib.on_device
@@ -24,7 +30,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         V = weight.shape[0]
         lib = _lib.load()
         code = _lib.dtype_code(hidden.dtype)
-        w = weight if weight.dtype == hidden.dtype else weight.to(hidden.dtype)
+        hidden, w = _aligned(hidden), _aligned(weight if weight.dtype == hidden.dtype else weight.to(hidden.dtype))
         loss = torch.empty((N,) if reduction == 0 else (), device=hidden.device, dtype=torch.float32)
         kept = torch.empty(N + 2, device=hidden.device, dtype=torch.float32)  # stats, lse
         n = lib.dynconv_vocab_loss_fwd_workspace_bytes(N, D, V, code)

@@ -123,7 +123,7 @@ def test_long_inner_dimensions():
 
 
 def test_unaligned_tensors():
-    """Views that TMA cannot address take the CUDA-core products, cut the same way."""
+    """Views that begin off 16 bytes: read through aligned copies."""
     N, D, V = 200, 64, 500
     h, w, t = make(N, D, V, torch.bfloat16)
     shift = lambda x: torch.cat([x.new_zeros(1), x.flatten()])[1:].view(x.shape)  # noqa: E731
@@ -265,6 +265,12 @@ def test_fp32_keeps_its_digits(N, D, V):
     rl, rh, rw = definition(h, w, t, torch.tensor(1.0, device="cuda"), "mean")
     got = (rel(loss, rl), rel(own[0].grad, rh), rel(own[1].grad, rw))
     assert max(got) <= 2.0**-17, got
+
+
+@pytest.mark.parametrize("N,D,V", [(1021, 257, 4999), (130, 2051, 300), (17000, 12, 9001), (40, 30, 30000), (1, 1, 1)])
+def test_bf16_widths_off_16_bytes(N, D, V):
+    """Rows that are no multiple of 16 bytes are copied with padding."""
+    check(*make(N, D, V, torch.bfloat16, seed=D))
 
 
 def test_fp32_unaligned_and_odd_widths():

@@ -71,7 +71,18 @@ def test_loss_workspace_of_fp32_parts():
     assert 0 < n < 6 * N * D + (2 << 30)
     # a vocabulary too wide for 1024 words of it in 512 MB still has a workspace
     assert lib.dynconv_vocab_loss_fwd_workspace_bytes(1, 1 << 20, 5000, 1) >= 6 * 1024 << 20
-    # an unaligned workspace is refused before any launch
+    # bf16 rows of whole 16 bytes are read in place, others are copied
+    assert lib.dynconv_vocab_loss_fwd_workspace_bytes(N, 2048, 1000, 0) < 2 << 20
+    assert lib.dynconv_vocab_loss_fwd_workspace_bytes(N, 2049, 1000, 0) >= 2 * 2056 * (N + 1000)
+    # an unaligned workspace, or an unaligned tensor that is used in place, is refused before any launch
+    for k in (0, 1):
+        args = [256, 256, 256, 256, 256, 256, 256, 1 << 30, 4, 64, 100, -100, 2]
+        args[k] = 264
+        assert lib.dynconv_vocab_loss_fwd(*args, 0, None) == ALIGN
+    for k in (0, 1, 6, 7):
+        args = [256, 256, 256, 256, 256, 256, 256, 256, 256, 1 << 30, 4, 64, 100, -100, 2]
+        args[k] = 264
+        assert lib.dynconv_vocab_loss_bwd(*args, 0, None) == ALIGN
     args = [256, 256, 256, 256, 256, 256, 264, 1 << 30, 4, 64, 100, -100, 2]
     assert lib.dynconv_vocab_loss_fwd(*args, 1, None) == ALIGN
     args = [256, 256, 256, 256, 256, 256, 256, 256, 264, 1 << 30, 4, 64, 100, -100, 2]
