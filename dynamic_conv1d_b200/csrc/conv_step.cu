@@ -16,7 +16,9 @@
 // Measured (B200, graph replay): one row of 3 x 2048 channels at rank 15 2.3 us, a launch's time; 512
 // such rows 9.2 us; 256 rows of 3 x 4096 at rank 31 13.4 us with the tensors in L2 and 18.5 us
 // from HBM, where their 53 MB take 8.2 us: bound by the latency of a block's phases (slots, then
-// caches; U's tile; products; stores) at 20 warps per SM.  Headwise, 64 rows of 2048: 2.5 us.
+// caches; U's tile; products; stores) at 20 warps per SM.  W = 8: 256 rows of 3 x 2048 at rank 15 9.6 us,
+// 512 rows of 3 x 4096 at rank 31 51 us (30 and 191 on the CUDA cores, which keep the widest filters
+// with more than 47 ranks).  Headwise, 64 rows of 2048: 2.5 us.
 #include "common.cuh"
 
 namespace dynconv {
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(32 * W) lr_step_few_kernel(const T* __restrict
   store_vec<T, VEC>(y + b * C + c, out);
 }
 
-// bf16, W <= 4, whole 16-byte groups of channels: the taps are a small matrix product (rows x ranks
+// bf16, whole 16-byte groups of channels: the taps are a small matrix product (rows x ranks
 // by ranks x channels), 2 R operations for each byte of the batch: on the CUDA cores 53 us for
 // 256 rows of 3 x 4096 channels at R = 31, so it goes to the tensor cores.  mma.sync is the
 // fitting form here: a warp's 16 x 32 outputs are consumed in registers by the convolution
@@ -218,6 +220,13 @@ __global__ void __launch_bounds__(32 * W) lr_step_few_kernel(const T* __restrict
 // 16-byte access per row and tensor.  (64 channels and 128 or 256 rows per block measured
 // 10 to 25% longer.)
 constexpr int kMmaRows = 64, kMmaCh = 32, kMmaThreads = 128;
+// us[w][k / 2][position] = channels' (U[k], U[k + 1]) pairs: B fragments are single words.
+// Row pitch 40 words: the four k rows that a fragment load touches lie 8 banks apart.
+constexpr int kPitch = 40;
+// Shared memory of the tiles of U and z: wide filters with many ranks do not fit.
+constexpr bool mma_fits(int W, int KS) {
+  return (W * KS * 8 * kPitch + (KS == 1 ? 4 : 64) * (KS * 8 + 4)) * 4 <= 48 * 1024;
+}
 
 __device__ __forceinline__ void mma_16n8k16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -237,17 +246,15 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
 }
 
 template <int W, int KS>
-__global__ void __launch_bounds__(kMmaThreads, KS == 1 ? 6 : 5) lr_step_mma_kernel(const __nv_bfloat16* __restrict__ x,
+__global__ void __launch_bounds__(kMmaThreads, W > 4 ? 3 : KS == 1 ? 6 : 5) lr_step_mma_kernel(const __nv_bfloat16* __restrict__ x,
                                                           const __nv_bfloat16* __restrict__ z,
                                                           const __nv_bfloat16* __restrict__ U,
                                                           const __nv_bfloat16* __restrict__ sw, __nv_bfloat16* cache,
                                                           __nv_bfloat16* __restrict__ y, const void* __restrict__ slots,
                                                           int slot_bytes, int64_t B, int64_t n_rows, int64_t D, int R,
                                                           int G, int residual) {
-  // us[w][k / 2][position] = channels' (U[k], U[k + 1]) pairs: B fragments are single words.
-  // Row pitch 40 words: the four k rows that a fragment load touches lie 8 banks apart.
-  constexpr int kPitch = 40, K2 = KS * 8;
-  __shared__ uint32_t us[W * K2 * kPitch];  // at most 25 KB
+  constexpr int K2 = KS * 8;
+  __shared__ uint32_t us[W * K2 * kPitch];
   __shared__ uint32_t zs[4][KS == 1 ? 1 : 16][K2 + 4];  // each warp's rows of z (pitch: 8 rows meet no bank twice)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t C = (int64_t)G * D;
@@ -454,15 +461,18 @@ int lr_mma_go(const StepArgs& a) {
   return DYNCONV_OK;
 }
 
+int mma_steps(const StepArgs& a) { return (a.R + (a.sw ? 1 : 0) + 15) / 16; }  // ranks, the static filter's among them
+
 template <int W>
 int lr_mma(const StepArgs& a) {
-  switch ((a.R + (a.sw ? 1 : 0) + 15) / 16) {  // ranks, the static filter's among them
-    case 1: return lr_mma_go<W, 1>(a);
-    case 2: return lr_mma_go<W, 2>(a);
-    case 3: return lr_mma_go<W, 3>(a);
-    case 4: return lr_mma_go<W, 4>(a);
-    default: return lr_mma_go<W, 5>(a);
-  }
+  const int ks = mma_steps(a);
+  if (ks == 1) return lr_mma_go<W, 1>(a);
+  if (ks == 2) return lr_mma_go<W, 2>(a);
+  if constexpr (mma_fits(W, 4))
+    if (ks == 4) return lr_mma_go<W, 4>(a);
+  if constexpr (mma_fits(W, 5))
+    if (ks == 5) return lr_mma_go<W, 5>(a);
+  return lr_mma_go<W, 3>(a);
 }
 
 bool aligned_octets(const StepArgs& a) {
@@ -475,8 +485,8 @@ bool aligned_octets(const StepArgs& a) {
 
 template <typename T, int W>
 int lr_pick(const StepArgs& a, bool pairs) {
-  if constexpr (sizeof(T) == 2 && W <= 4)
-    if (aligned_octets(a)) return lr_mma<W>(a);
+  if constexpr (sizeof(T) == 2)
+    if (aligned_octets(a) && mma_fits(W, mma_steps(a))) return lr_mma<W>(a);
   if (a.B < kFewRows) return pairs ? lr_few<T, W, 2>(a) : lr_few<T, W, 1>(a);
   return pairs ? lr_many<T, W, 2>(a) : lr_many<T, W, 1>(a);
 }

@@ -102,6 +102,21 @@ def test_headwise(dtype, static, B, H, hs, W):
     assert torch.equal(c, torch.cat([cache, x[:, None]], 1)[:, 1:])
 
 
+@pytest.mark.parametrize("W", [1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("R", [1, 15, 16, 31, 33, 47, 50, 64])
+def test_lowrank_widths_and_ranks(W, R):
+    """Every width with every number of 16-rank steps, whole octets of channels, rows beyond a block."""
+    B, G, D = 70, 2, 40
+    x, z, U, cache, sw = make(B, G, D, R, W, torch.bfloat16, seed=R + W)
+    for s in (sw, None):
+        c = cache.clone()
+        y = lowrank_dynamic_convolution_grouped_step(x, z, U, c, s, residual=True)
+        ref = [None if t is None else t.double() for t in (x, z, U, cache, s)]
+        ry, rc = lowrank_definition(*ref, True)
+        terms, _ = lowrank_definition(*(None if t is None else t.abs() for t in ref), True)
+        assert near(y, ry, terms) and torch.equal(c.double(), rc)
+
+
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 def test_slots(index):
     B, G, D, R, W, n = 6, 2, 64, 7, 4, 9
