@@ -26,9 +26,13 @@ namespace dynconv {
 namespace {
 
 constexpr int kThreads = 128;
-// Below this many rows the CUDA-core path runs a block per row with its taps in parallel: 2.5 to 3
-// us for 1 to 6 rows of 3 x 2048 channels in fp32, where blocks of eight rows take 7.7 us up to 32.
-constexpr int kFewRows = 32;
+// The CUDA-core path runs a block per row with its taps in parallel up to this many rows, as long as
+// the rows' loads of U (G D / VEC x R W for each) stay below this number; blocks of eight rows read U
+// an eighth as often but take longer to start.  Measured per row / in eights, fp32 (us): 3 x 2048 at rank
+// 15, W = 4: 1 row 2.5 / 6.0, 16 5.2 / 7.8, 32 8.1 / 7.9, 64 14.0 / 8.5; 3 x 4096 at rank 31, W = 8: 1 row 3.7 /
+// 10.1, 4 7.7 / 11.1, 8 13.2 / 13.0, 20 29 / 13.6; 512 at rank 7: 64 rows 2.8 / 5.8.
+constexpr int kFewRows = 64;
+constexpr int64_t kFewLoads = 6 << 20;
 
 __device__ __forceinline__ int64_t slot_of(const void* slots, int slot_bytes, int b) {
   if (!slots) return b;
@@ -487,7 +491,8 @@ template <typename T, int W>
 int lr_pick(const StepArgs& a, bool pairs) {
   if constexpr (sizeof(T) == 2)
     if (aligned_octets(a) && mma_fits(W, mma_steps(a))) return lr_mma<W>(a);
-  if (a.B < kFewRows) return pairs ? lr_few<T, W, 2>(a) : lr_few<T, W, 1>(a);
+  const int64_t loads = a.G * a.D / (pairs ? 2 : 1) * a.R * W;
+  if (a.B <= kFewRows && a.B * loads <= kFewLoads) return pairs ? lr_few<T, W, 2>(a) : lr_few<T, W, 1>(a);
   return pairs ? lr_many<T, W, 2>(a) : lr_many<T, W, 1>(a);
 }
 
