@@ -123,7 +123,7 @@ def on_device(fn):
 
     @functools.wraps(fn)
     def wrapper(ctx, first, *args):
-        with torch.cuda.device(first.device):
+        with device_of(first):
             return fn(ctx, first, *args)
 
     return wrapper

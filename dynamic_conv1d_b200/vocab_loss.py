@@ -101,7 +101,8 @@ def linear_cross_entropy(
     assert weight.shape[1] == hidden.shape[-1]
     assert target.device == hidden.device and target.dtype == torch.int64 and target.shape == hidden.shape[:-1]
     assert reduction in _REDUCTIONS, f"reduction must be one of {tuple(_REDUCTIONS)}"
+    if hidden.dim() != 2:  # (a view is one more node of the graph)
+        hidden = hidden.view(-1, hidden.shape[-1])
     loss = _LinearCrossEntropyFn.apply(
-        hidden.view(-1, hidden.shape[-1]), weight, target.reshape(-1).contiguous(), int(ignore_index),
-        _REDUCTIONS[reduction])
+        hidden, weight, target.reshape(-1).contiguous(), int(ignore_index), _REDUCTIONS[reduction])
     return loss.view(target.shape) if reduction == "none" else loss
