@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(32 * W) lr_step_few_kernel(const T* __restrict
       }
   }
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) part[w][lane * VEC + e] = tap[e] * past[e];
+  for (int e = 0; e < VEC; ++e) part[w][lane * VEC + e] = live ? tap[e] * past[e] : 0.f;  // (z of a padding row may be anything)
   if (in && live && w > 0) store_vec<T, VEC>(cr + (int64_t)(W - 1 - w) * C, next);
   __syncthreads();
   if (w != 0 || !in) return;

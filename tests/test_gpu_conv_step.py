@@ -198,3 +198,30 @@ def test_refusals():
         lowrank_dynamic_convolution_step(x9, z9, U9[0], c9, s9[0])
     with pytest.raises(AssertionError):
         headwise_dynamic_convolution_step(x, torch.zeros(2, 5, 4, device="cuda").bfloat16(), cache)
+
+
+@pytest.mark.parametrize("dtype,B,D", [(torch.float32, 6, 64), (torch.float32, 70, 64), (torch.float32, 6, 33), (torch.bfloat16, 6, 33),
+                                       (torch.bfloat16, 70, 33), (torch.bfloat16, 6, 64)])
+def test_padding_rows_of_anything(dtype, B, D):
+    """Rows whose slot lies outside the pool give zeros whatever their inputs hold, in every form of the
+    step, and the other rows do not see them."""
+    G, R, W, n = 2, 7, 4, 80
+    x, z, U, pool, sw = make(B, G, D, R, W, dtype, n=n)
+    slots = torch.arange(B, device="cuda", dtype=torch.int32)
+    padding = [1, 4, B - 1]
+    live = [i for i in range(B) if i not in padding]
+    slots[padding] = torch.tensor([-1, n, -5], device="cuda", dtype=torch.int32)
+    w = torch.randn(B, 4 if D % 4 == 0 else 3, W, device="cuda").to(dtype)
+    D_hw = G * D
+    want_pool, want_hw_pool = pool.clone(), pool.clone()
+    want = lowrank_dynamic_convolution_grouped_step(x, z, U, want_pool, sw, residual=True, slots=slots)
+    want_hw = headwise_dynamic_convolution_step(x, w, want_hw_pool, sw.reshape(W, D_hw), residual=True, slots=slots)
+    for bad in (float("nan"), float("inf")):
+        xb, zb, wb = x.clone(), z.clone(), w.clone()
+        xb[padding], zb[padding], wb[padding] = bad, bad, bad
+        c, ch = pool.clone(), pool.clone()
+        y = lowrank_dynamic_convolution_grouped_step(xb, zb, U, c, sw, residual=True, slots=slots)
+        yh = headwise_dynamic_convolution_step(xb, wb, ch, sw.reshape(W, D_hw), residual=True, slots=slots)
+        for got, ref in ((y, want), (yh, want_hw)):
+            assert got[padding].count_nonzero() == 0 and torch.equal(got[live], ref[live])
+        assert torch.equal(c, want_pool) and torch.equal(ch, want_hw_pool)
