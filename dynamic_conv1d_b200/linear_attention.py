@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .step import _refuse_gradient, _slots
@@ -261,4 +262,5 @@ def decay_linear_attention_step(
         if status:
             _lib.check(status)
         _lib.after_call(o)
+    increment_version(state)  # (a backward that kept the state before this step raises)
     return o

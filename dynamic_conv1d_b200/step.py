@@ -8,11 +8,13 @@ W-1 inputs, and each step takes one token per sequence, updating the cache in pl
     cache = convolution_cache(x, W)
     y_t = lowrank_dynamic_convolution_step(x_t, z_t, U, cache, static_w, residual=True)
 
-The steps have no gradient (generating text needs none) and refuse inputs that ask for one.
+The steps have no gradient (generating text needs none) and refuse inputs that ask for one.  They
+count as updates in place of the cache: a backward that kept it before a step raises.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -108,7 +110,7 @@ def _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, G):
         assert static_w.shape == ((W, D) if U.dim() == 2 else (G, W, D))
         if static_w.dtype != dtype:
             static_w = static_w.to(dtype)
-    if torch.is_grad_enabled() and (x.requires_grad or z.requires_grad or U.requires_grad
+    if torch.is_grad_enabled() and (x.requires_grad or z.requires_grad or U.requires_grad or cache.requires_grad
                                     or (static_w is not None and static_w.requires_grad)):
         _refuse_gradient()
     code = _lib.dtype_code(dtype)
@@ -126,6 +128,7 @@ def _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, G):
         if status:
             _lib.check(status)
         _lib.after_call(y)
+    increment_version(cache)
     return y
 
 
@@ -152,7 +155,7 @@ def headwise_dynamic_convolution_step(
         assert static_w.get_device() == dev and static_w.is_contiguous()
         assert static_w.dtype == dtype
         assert static_w.shape == (W, D)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or cache.requires_grad
                                     or (static_w is not None and static_w.requires_grad)):
         _refuse_gradient()
     code = _lib.dtype_code(dtype)
@@ -167,4 +170,5 @@ def headwise_dynamic_convolution_step(
         if status:
             _lib.check(status)
         _lib.after_call(y)
+    increment_version(cache)
     return y

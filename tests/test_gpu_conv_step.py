@@ -225,3 +225,24 @@ def test_padding_rows_of_anything(dtype, B, D):
         for got, ref in ((y, want), (yh, want_hw)):
             assert got[padding].count_nonzero() == 0 and torch.equal(got[live], ref[live])
         assert torch.equal(c, want_pool) and torch.equal(ch, want_hw_pool)
+
+
+def test_updates_in_place_are_seen_by_autograd():
+    """A cache that autograd has kept cannot be stepped unnoticed, and one that asks for a gradient is refused."""
+    x, z, U, cache, sw = make(2, 1, 64, 7, 4, torch.bfloat16)
+    w = torch.randn(2, 8, 4, device="cuda").bfloat16()
+    steps = (lambda c: lowrank_dynamic_convolution_step(x, z, U[0], c, sw[0]), lambda c: headwise_dynamic_convolution_step(x, w, c))
+    for step in steps:
+        c, p = cache.clone(), torch.ones((), device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        kept = (c * p).sum()
+        step(c)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.backward()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            step(cache.clone().requires_grad_())
+        with torch.no_grad():
+            step(cache.clone().requires_grad_())
+        with torch.inference_mode():
+            inside = cache.clone()
+            step(inside)
+        step(inside)  # (inference tensors have no counter, and may be stepped anywhere)

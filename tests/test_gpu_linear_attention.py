@@ -393,3 +393,21 @@ def test_refusals():
                 dict(slots=torch.zeros(3, device="cuda", dtype=torch.int32)), dict(q=q[:, 0].clone().requires_grad_())):
         with pytest.raises((AssertionError, RuntimeError)):
             decay_linear_attention_step(**(step | bad))
+
+
+# ------------------------------------------------------------------------------ autograd
+
+
+def test_updates_in_place_are_seen_by_autograd():
+    """A step on a state that a prompt's backward still needs is an error, not another gradient."""
+    q, k, v, do, S0, _, ld = inputs(2, 20, 2, 64, 64, torch.bfloat16)
+    S = S0.clone()
+    o = decay_linear_attention(q.requires_grad_(), k, v, ld, S)
+    with torch.no_grad():
+        decay_linear_attention_step(q[:, 0], k[:, 0], v[:, 0], S, ld)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.backward(do)
+    with torch.inference_mode():
+        inside = S0.clone()
+        decay_linear_attention_step(q[:, 0], k[:, 0], v[:, 0], inside, ld)
+    assert torch.equal(inside, S)
