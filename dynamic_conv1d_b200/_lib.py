@@ -129,6 +129,40 @@ def on_device(fn):
     return wrapper
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """Gradients as they are; differentiating them is an error."""
+
+    @staticmethod
+    def forward(ctx, *grads):
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("this operator's gradients cannot be differentiated again (create_graph=True)")
+
+
+def differentiable_once(backward):
+    """Decorator of a Function's backward whose kernels autograd does not see.  Under create_graph=True
+    its gradients would come back as constants and a penalty on them would be left out without a word;
+    here differentiating them raises.  (torch's once_differentiable does so only where the upstream gradient
+    asks for a gradient itself, but these depend on the saved inputs too.)"""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *upstream):
+        with torch.no_grad():
+            grads = backward(ctx, *upstream)
+        if not torch.is_grad_enabled():
+            return grads
+        there = [i for i, g in enumerate(grads) if g is not None]
+        marked = _NoSecondDerivative.apply(*(grads[i].requires_grad_() for i in there))
+        out = [None] * len(grads)
+        for i, g in zip(there, marked):
+            out[i] = g
+        return tuple(out)
+
+    return wrapper
+
+
 _same_device = contextlib.nullcontext()
 # the bindings under torch.cuda.current_device / current_stream, without the Python objects, for
 # calls whose kernels take a few microseconds

@@ -88,6 +88,7 @@ class _DecayLinearAttentionFn(torch.autograd.Function):
         return o, s1
 
     @staticmethod
+    @_lib.differentiable_once
     def backward(ctx, do, ds1):
         q, k, v, log_decay, s0 = ctx.saved_tensors
         B, T, H, dk = q.shape
@@ -122,6 +123,7 @@ class _FusedDecayLinearAttentionFn(torch.autograd.Function):
         return o, s1
 
     @staticmethod
+    @_lib.differentiable_once
     def backward(ctx, do, ds1):
         qkv, log_decay, s0 = ctx.saved_tensors
         B, T, C = qkv.shape
@@ -177,7 +179,7 @@ def decay_linear_attention(
         return_state:  also return the state after the last token, [B, H, dk, dv] float32.
 
     Returns:
-        o [B, T, H, dv], or (o, state).  Differentiable in q, k, v and initial_state.
+        o [B, T, H, dv], or (o, state).  Differentiable (once) in q, k, v and initial_state.
     """
     dev = q.get_device()  # (-1 on the CPU)
     assert dev >= 0 and k.get_device() == dev and v.get_device() == dev

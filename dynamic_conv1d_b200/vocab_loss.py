@@ -48,6 +48,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @_lib.differentiable_once
     @_lib.on_device
     def backward(ctx, dloss):
         hidden, w, target, kept = ctx.saved_tensors
@@ -92,7 +93,7 @@ def linear_cross_entropy(
         reduction:    "mean" over the rows that count (NaN when none does), "sum", or "none".
 
     Returns:
-        the loss in float32: a scalar, or of target's shape for "none".  Differentiable in
+        the loss in float32: a scalar, or of target's shape for "none".  Differentiable (once) in
         hidden and weight.  Under ``data_parallel()`` both the mean and weight's gradient
         are this rank's own, as for any other parameter of the model around the ops.
     """

@@ -411,3 +411,18 @@ def test_updates_in_place_are_seen_by_autograd():
         inside = S0.clone()
         decay_linear_attention_step(q[:, 0], k[:, 0], v[:, 0], inside, ld)
     assert torch.equal(inside, S)
+
+
+def test_no_second_derivative():
+    """The gradients are no functions of the inputs to autograd: differentiating them is an error, not a
+    constant."""
+    q, k, v, do, S0, _, ld = inputs(1, 40, 2, 64, 64, torch.float32)
+    x = torch.stack([q, k, v], 2).reshape(1, 40, 3 * 2 * 64).requires_grad_()
+    q.requires_grad_()
+    for leaf, run in ((q, lambda: decay_linear_attention(q, k, v, ld, S0)), (x, lambda: decay_linear_attention_fused(x, ld))):
+        o = run()
+        (g,) = torch.autograd.grad(o, leaf, do.view_as(o), create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (leaf.sum() + g.square().sum()).backward()
+        (g1,) = torch.autograd.grad(run(), leaf, do.view_as(o))
+        assert torch.equal(g, g1)

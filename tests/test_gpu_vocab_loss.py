@@ -319,3 +319,16 @@ def test_refusals():
                 dict(target=t[:5]), dict(target=t.int()), dict(target=t.cpu()), dict(reduction="max")):
         with pytest.raises((AssertionError, TypeError, RuntimeError)):
             linear_cross_entropy(**(good | bad))
+
+
+def test_no_second_derivative():
+    """The gradients are no functions of the inputs to autograd: differentiating them is an error, not a
+    constant."""
+    h, w, t = make(20, 64, 50, torch.float32)
+    h.requires_grad_()
+    loss = linear_cross_entropy(h, w, t)
+    (g,) = torch.autograd.grad(loss, h, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        (h.sum() + g.square().sum()).backward()
+    (g1,) = torch.autograd.grad(linear_cross_entropy(h, w, t), h)
+    assert torch.equal(g, g1)

@@ -120,3 +120,32 @@ def test_layer_arguments():
         dc.ConvolvedLinearAttention(64, 4, R=14)
     m = dc.ConvolvedLinearAttention(64, 4).to(torch.bfloat16)
     assert m.log_decay.dtype == torch.float32 and (m.log_decay < 0).all()
+
+
+def test_gradients_that_cannot_be_differentiated():
+    """The mark on a backward whose kernels autograd does not see: ordinary gradients as they are, an error
+    for a second derivative whether or not the upstream gradient asks for one."""
+
+    class Cube(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, unused):
+            ctx.save_for_backward(x)
+            return x**3
+
+        @staticmethod
+        @_lib.differentiable_once
+        def backward(ctx, d):
+            return 3 * ctx.saved_tensors[0]**2 * d, None
+
+    x = torch.tensor([1.0, 2.0], requires_grad=True)
+    y = Cube.apply(x, None)
+    y.sum().backward(retain_graph=True)
+    assert x.grad.tolist() == [3.0, 12.0] and not x.grad.requires_grad
+    for loss in (y.sum(), y.square().sum()):
+        (g,) = torch.autograd.grad(loss, x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (x.sum() + g.sum()).backward()
+    (g,) = torch.autograd.grad(Cube.apply(2 * x, None).sum(), x, create_graph=True)  # (through an operator of torch's)
+    assert g.tolist() == [24.0, 96.0]
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        g.sum().backward()
