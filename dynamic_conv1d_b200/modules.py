@@ -145,14 +145,18 @@ class ConvolvedLinearAttention(nn.Module):
         self.qkv = nn.Linear(d_model, 3 * d_model, bias=False)
         self.conv = QKVLowRankDynamicShortConvolution(d_model, R, W)
         self.out = nn.Linear(d_model, d_model, bias=False)
-        # float32 whatever the parameters' type: not a buffer, which .to(dtype) would round
-        self._log_decay = torch.log1p(-torch.exp2(-torch.linspace(5, 12, n_heads, dtype=torch.float64))).float()
+        self._log_decay = None
 
     @property
     def log_decay(self) -> torch.Tensor:
+        """[n_heads] float32 on the parameters' device whatever their type: not a buffer, which .to(dtype)
+        would round.  Made where it is first used, from the number of heads alone: on the CPU, so that
+        every device has the same bits, and outside inference mode, whose tensors no backward may keep."""
         device = self.qkv.weight.device
-        if self._log_decay.device != device:
-            self._log_decay = self._log_decay.to(device)
+        if self._log_decay is None or self._log_decay.device != device:
+            with torch.inference_mode(False):
+                e = torch.linspace(5, 12, self.n_heads, dtype=torch.float64, device="cpu")
+                self._log_decay = torch.log1p(-torch.exp2(-e)).float().to(device)
         return self._log_decay
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

@@ -96,3 +96,16 @@ def test_example_learns_and_generates(capsys):
     first, last, right = lm.main(["--steps", "200"])
     assert first > 5.0  # about log(500): the model starts ignorant
     assert last < 1.5 and right > 0.8
+
+
+def test_training_after_evaluation_in_inference_mode():
+    """The layer's first use on a device may be under inference mode."""
+    x = torch.randn(2, 40, 256, device="cuda").bfloat16()
+    m = layer()
+    want = layer()(x)
+    with torch.inference_mode():
+        y, cache = m.prompt(x)
+        m.step(x[:, 0], cache)
+    assert torch.equal(y, want)
+    m(x).float().square().mean().backward()
+    assert all(p.grad is not None and p.grad.isfinite().all() for p in m.parameters())

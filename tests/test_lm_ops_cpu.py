@@ -2,6 +2,8 @@
 touching the GPU, size their workspaces, and their Python forms refuse what they cannot do."""
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 
@@ -149,3 +151,27 @@ def test_gradients_that_cannot_be_differentiated():
     assert g.tolist() == [24.0, 96.0]
     with pytest.raises(RuntimeError, match="differentiated again"):
         g.sum().backward()
+
+
+def test_layer_decays_wherever_they_are_first_used():
+    """The decays of a layer are the same constants whichever context asks first: an evaluation under
+    inference mode before training, or a layer that was built without storage."""
+    want = dc.ConvolvedLinearAttention(64, 4).log_decay
+    exact = torch.log1p(-torch.exp2(-torch.linspace(5, 12, 4, dtype=torch.float64)))
+    assert torch.equal(want, exact.float())
+    m = dc.ConvolvedLinearAttention(64, 4)
+    m.to("meta")
+    with torch.inference_mode():
+        assert m.log_decay.device.type == "meta" and not m.log_decay.is_inference()
+    p = torch.ones(4, device="meta", requires_grad=True)
+    (p * m.log_decay).sum().backward()  # (an inference tensor cannot be kept for this)
+    with torch.device("meta"):
+        m = dc.ConvolvedLinearAttention(64, 4)
+    assert m.log_decay.device.type == "meta"
+    m.to_empty(device="cpu")
+    assert torch.equal(m.log_decay, want)
+    with torch.inference_mode():
+        m = dc.ConvolvedLinearAttention(64, 4)
+    assert torch.equal(m.log_decay, want) and not m.log_decay.is_inference()
+    m = copy.deepcopy(dc.ConvolvedLinearAttention(64, 4).to("meta"))
+    assert m.log_decay.device.type == "meta" and m.to_empty(device="cpu").log_decay.equal(want)
