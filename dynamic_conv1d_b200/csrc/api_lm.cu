@@ -125,7 +125,7 @@ LossBackwardBytes loss_backward_bytes(const vl::Plan& pl, int64_t N, int64_t D, 
   const size_t elem = 2 * vl::parts_of(dtype);
   const int64_t ld = copy ? vl::copy_pitch(D) : D;
   LossBackwardBytes b;
-  b.hidden_copy = copy ? align_up(vl::copy_bytes(N, D, dtype)) : 0;
+  b.hidden_copy = copy || want_weight ? align_up(vl::copy_bytes(N, D, dtype)) : 0;
   b.weight_copy = copy ? align_up(vl::copy_bytes(pl.piece, D, dtype)) : 0;
   b.piece = align_up((size_t)N * pl.pitch * elem);
   b.acc_h = want_hidden ? align_up((size_t)pl.z_h * N * ld * sizeof(float)) : 0;

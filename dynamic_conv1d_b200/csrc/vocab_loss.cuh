@@ -47,7 +47,7 @@ struct Problem {
   float* acc_h;             // [z_h][N][D] fp32; rows of copy_pitch(D) where operands are copies
   float* acc_w;             // [z_w][piece rows][D] fp32 likewise, where dweight is not written at once
   // either way, where operands are copies
-  __nv_bfloat16* hidden_copy;  // [parts][N or rows at once][copy_pitch]
+  __nv_bfloat16* hidden_copy;  // [parts][N or rows at once][copy_pitch]; for dweight always
   __nv_bfloat16* weight_copy;  // [parts][words at once][copy_pitch]
   cudaStream_t st;
 };

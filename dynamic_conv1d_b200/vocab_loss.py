@@ -88,8 +88,8 @@ def linear_cross_entropy(
         hidden:       [..., D] (bfloat16 or float32, CUDA, contiguous).
         weight:       [V, D], contiguous; cast to hidden's dtype when it has another one.
         target:       [...] int64, the index of each row's word.  Rows whose target is
-                      ``ignore_index`` count for nothing.  Any other target outside 0..V-1
-                      makes the loss NaN (and gives that row no gradient).
+                      ``ignore_index`` count for nothing, whatever they hold.  Any other target
+                      outside 0..V-1 makes the loss NaN (and gives that row no gradient).
         reduction:    "mean" over the rows that count (NaN when none does), "sum", or "none".
 
     Returns:

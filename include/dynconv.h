@@ -309,14 +309,16 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
  * computed in pieces of the vocabulary without the [N,V] logits in memory (no reference
  * counterpart; the loss of a language model built on the convolutions).
  *   target [N] int64.  A row whose target is ignore_index counts for nothing; any other
- *   target outside [0,V) makes the loss NaN and contributes no gradient.
+ *   target outside [0,V) makes the loss NaN and contributes no gradient.  The hidden states of
+ *   either may hold anything.
  *   reduction: 0 none (loss [N]), 1 sum, 2 mean over the rows that count (loss [1]; NaN
  *   when none does).  loss, lse [N] and stats [2] are float32; lse and stats are kept for
  *   the backward (stats: sum of the rows' losses, number of rows that count).
  * float32 tensors are multiplied as three bf16 parts each, and bf16 ones whose D is no multiple
  * of 8 as padded copies: the workspaces hold those (of weight at most 512 MB at a time).
  * Workspaces are 16-byte aligned, and so are bf16 tensors with D a multiple of 8, which are
- * read and written in place (DYNCONV_ERR_ALIGN).
+ * read and written in place (DYNCONV_ERR_ALIGN; for dweight the workspace holds a copy of hidden
+ * without the rows that do not count).
  * N <= 2^30, V <= 4194304. */
 size_t dynconv_vocab_loss_fwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype);
 int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t* target,

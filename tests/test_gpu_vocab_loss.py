@@ -332,3 +332,34 @@ def test_no_second_derivative():
         (h.sum() + g.square().sum()).backward()
     (g1,) = torch.autograd.grad(linear_cross_entropy(h, w, t), h)
     assert torch.equal(g, g1)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("D", [64, 65, 512])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_rows_that_count_for_nothing_may_hold_anything(dtype, bad, D, reduction):
+    """Hidden states of ignored rows, and of rows whose target is no word, reach neither gradient."""
+    h, w, t = make(300, D, 700, dtype)
+    ignored = (t == IGNORE).nonzero()[:, 0]
+    up = torch.randn(300, device="cuda") if reduction == "none" else torch.tensor(1.0, device="cuda")
+
+    def grads(h, t, need_h=True):
+        own = [h.detach().requires_grad_(need_h), w.detach().requires_grad_()]
+        loss = linear_cross_entropy(*own, t, reduction=reduction)
+        loss.backward(up)
+        check_device(loss)
+        return loss.detach(), own[0].grad, own[1].grad
+
+    hb = h.clone()
+    hb[ignored] = bad
+    want, got = grads(h, t), grads(hb, t)
+    for a, b in zip(want, got):
+        assert b.isfinite().all() and torch.equal(a, b)
+    assert got[1][ignored].count_nonzero() == 0
+    assert torch.equal(grads(hb, t, False)[2], want[2])
+    t = t.clone()
+    t[ignored[::2]] = 700  # no word either: the loss says so, the gradients leave it out
+    _, _, rw = grads(h, t)
+    _, gh, gw = grads(hb, t)
+    assert gh.isfinite().all() and torch.equal(gw, rw)
