@@ -18,8 +18,8 @@ __global__ void __launch_bounds__(256) vl_merge_kernel(const Problem p, int64_t 
   if (n < p.N) {
     for (int64_t i = w; i < tiles; i += 8) {
       const float2 v = p.part[i * p.N + n];
-      const float m2 = fmaxf(mx, v.x);
-      if (m2 == -INFINITY) continue;  // nothing finite so far: exp(-inf) adds nothing
+      const float m2 = max_nan(mx, v.x);
+      if (m2 == -INFINITY) continue;  // only words of minus infinity so far: exp(-inf) adds nothing
       sum = sum * exp2f(mx - m2) + v.y * exp2f(v.x - m2);
       mx = m2;
     }
@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(256) vl_merge_kernel(const Problem p, int64_t 
   if (w != 0 || n >= p.N) return;
   for (int i = 1; i < 8; ++i) {
     const float2 v = part[i][lane];
-    const float m2 = fmaxf(mx, v.x);
+    const float m2 = max_nan(mx, v.x);
     if (m2 == -INFINITY) continue;
     sum = sum * exp2f(mx - m2) + v.y * exp2f(v.x - m2);
     mx = m2;

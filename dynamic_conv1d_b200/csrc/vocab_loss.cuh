@@ -59,6 +59,13 @@ struct Plan {
   int z_h, z_w;
 };
 
+// The larger of two numbers; NaN if either is (fmaxf would drop it, and with it a row's NaN logits).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // A row's factor within dl: 0 where the target is ignored or outside the vocabulary.
 __device__ __forceinline__ float row_factor(const Problem& p, int64_t n, int64_t t) {
   if (t == p.ignore || t < 0 || t >= p.V) return 0.f;

@@ -543,16 +543,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             float mx = -INFINITY;
             if (left >= kStep) {
 #pragma unroll
-              for (int j = 0; j < kStep; ++j) mx = fmaxf(mx, v[j]);
+              for (int j = 0; j < kStep; ++j) mx = max_nan(mx, v[j]);
             } else {
 #pragma unroll
               for (int j = 0; j < kStep; ++j) {
                 if (j >= left) v[j] = -INFINITY;
-                mx = fmaxf(mx, v[j]);
+                mx = max_nan(mx, v[j]);
               }
             }
-            const float m_new = fmaxf(m2, mx * kLog2e);
-            if (m_new > -INFINITY) {
+            const float m_new = max_nan(m2, mx * kLog2e);
+            if (m_new != -INFINITY) {  // (a NaN goes into the sum)
               float s0 = 0.f, s1 = 0.f;
 #pragma unroll
               for (int j = 0; j < kStep; j += 2) {

@@ -363,3 +363,37 @@ def test_rows_that_count_for_nothing_may_hold_anything(dtype, bad, D, reduction)
     _, _, rw = grads(h, t)
     _, gh, gw = grads(hb, t)
     assert gh.isfinite().all() and torch.equal(gw, rw)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("D", [64, 65, 2056])
+@pytest.mark.parametrize("first,count", [(0, 1), (0, 16), (0, 32), (0, 128), (128, 128), (256, 256), (300, 1), (320, 80), (0, 400)])
+def test_words_that_are_nan(dtype, D, first, count):
+    """One NaN among a row's logits makes its loss NaN, whichever words have it."""
+    h, w, t = make(150, D, 400, dtype, ignored=0.0)
+    w = w.clone()
+    w[first:first + count] = float("nan")
+    t = torch.where((t >= first) & (t < first + count), torch.full_like(t, 200 if first != 128 else 50), t)
+    assert linear_cross_entropy(h, w, t, reduction="none").isnan().all()
+    assert linear_cross_entropy(h, w, t).isnan()
+
+
+@pytest.mark.parametrize("D", [8, 9, 2056])
+@pytest.mark.parametrize("first,count", [(0, 1), (0, 32), (0, 128), (256, 256), (320, 80)])
+def test_words_that_are_excluded(D, first, count):
+    """Logits of minus infinity take their words out of the sum; a row with nothing else, or with plus
+    infinity, has no loss."""
+    h, w, t = make(150, D, 400, torch.bfloat16, ignored=0.0)
+    h[:, 0], w = 1.0, w.clone()
+    w[first:first + count, 0] = -float("inf")
+    t = torch.where((t >= first) & (t < first + count), torch.full_like(t, 200), t)
+    keep = [v for v in range(400) if not first <= v < first + count]
+    own = [x.detach().requires_grad_() for x in (h, w)]
+    rows = linear_cross_entropy(*own, t, reduction="none")
+    l = h.double() @ w[keep].double().T
+    lt = (h.double() * w[t].double()).sum(1)
+    assert rel(rows, torch.logsumexp(l, 1) - lt) <= 2 * LOSS
+    w[0, 0] = float("inf")
+    assert linear_cross_entropy(h, w, t, reduction="none").isnan().all()
+    w[:, 0] = -float("inf")
+    assert linear_cross_entropy(h, w, t, reduction="none").isnan().all()
