@@ -103,12 +103,13 @@ int la_run(la::Params& p, int dtype, void* ws, size_t ws_bytes, cudaStream_t st)
 
 int check_loss(int64_t N, int64_t D, int64_t V, int reduction, int dtype) {
   int s;
+  reduction &= ~vl::kKeepRows;
   if ((s = check_dtype(dtype))) return s;
   if (N < 0 || D < 1 || V < 1 || N > (1 << 30) || D > INT32_MAX / 16 || V > (int64_t)1 << 22)
     return set_error(DYNCONV_ERR_SHAPE, "vocabulary loss: bad sizes N=%lld D=%lld V=%lld", (long long)N, (long long)D,
                      (long long)V);
   if (reduction < vl::kNone || reduction > vl::kMean)
-    return set_error(DYNCONV_ERR_ARGUMENT, "vocabulary loss: reduction %d (none=0, sum=1, mean=2)", reduction);
+    return set_error(DYNCONV_ERR_ARGUMENT, "vocabulary loss: reduction %d (none=0, sum=1, mean=2; +4: lse and the rows' losses)", reduction);
   return DYNCONV_OK;
 }
 
@@ -254,12 +255,14 @@ int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t
   cudaStream_t st = (cudaStream_t)stream;
   if ((s = op_entry(st))) return s;
   if ((s = check_loss(N, D, V, reduction, dtype))) return s;
+  const bool keep = reduction & vl::kKeepRows;
+  reduction &= ~vl::kKeepRows;
   if (!stats || (!loss && (N > 0 || reduction != vl::kNone)))
     return set_error(DYNCONV_ERR_ARGUMENT, "vocab_loss_fwd: null loss or stats");
   vl::Problem p{};
   p.hidden = hidden, p.weight = weight, p.target = target;
   p.N = N, p.D = D, p.V = V, p.ignore = ignore_index, p.reduction = reduction;
-  p.lse = lse, p.loss = loss, p.stats = stats, p.st = st;
+  p.lse = lse, p.row_loss = keep && lse ? lse + N : nullptr, p.loss = loss, p.stats = stats, p.st = st;
   if (N == 0) return vl::total_launch(p);
   if (!hidden || !weight || !target || !lse) return set_error(DYNCONV_ERR_ARGUMENT, "vocab_loss_fwd: null tensor");
   const size_t need = dynconv_vocab_loss_fwd_workspace_bytes(N, D, V, dtype);
@@ -303,7 +306,8 @@ int dynconv_vocab_loss_bwd(const void* hidden, const void* weight, const int64_t
     return set_error(DYNCONV_ERR_ARGUMENT, "vocab_loss_bwd: null tensor");
   vl::Problem p{};
   p.hidden = hidden, p.weight = weight, p.target = target;
-  p.N = N, p.D = D, p.V = V, p.ignore = ignore_index, p.reduction = reduction;
+  p.N = N, p.D = D, p.V = V, p.ignore = ignore_index, p.reduction = reduction & ~vl::kKeepRows;
+  p.row_loss = reduction & vl::kKeepRows ? const_cast<float*>(lse) + N : nullptr;
   p.lse = const_cast<float*>(lse), p.stats = const_cast<float*>(stats), p.dloss = dloss;
   p.dhidden = dhidden, p.dweight = dweight, p.st = st;
   p.piece = workspace;

@@ -8,6 +8,14 @@ namespace vl {
 
 namespace {
 
+// Adds a tile's (maximum, sum) to a row's.
+__device__ __forceinline__ void merge(float& mx, float& sum, float2 v) {
+  const float m2 = max_nan(mx, v.x);
+  if (m2 == -INFINITY) return;  // only words of minus infinity so far: exp(-inf) adds nothing
+  sum = sum * exp2f(mx - m2) + v.y * exp2f(v.x - m2);
+  mx = m2;
+}
+
 // Merges the tiles' (maximum, sum) of 32 rows per CTA: lane = row, warps take every eighth
 // tile; then the rows' losses.
 __global__ void __launch_bounds__(256) vl_merge_kernel(const Problem p, int64_t tiles) {
@@ -15,31 +23,29 @@ __global__ void __launch_bounds__(256) vl_merge_kernel(const Problem p, int64_t 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t n = (int64_t)blockIdx.x * 32 + lane;
   float mx = -INFINITY, sum = 0.f;
-  if (n < p.N) {
-    for (int64_t i = w; i < tiles; i += 8) {
-      const float2 v = p.part[i * p.N + n];
-      const float m2 = max_nan(mx, v.x);
-      if (m2 == -INFINITY) continue;  // only words of minus infinity so far: exp(-inf) adds nothing
-      sum = sum * exp2f(mx - m2) + v.y * exp2f(v.x - m2);
-      mx = m2;
-    }
-  }
+  if (n < p.N)
+    for (int64_t i = w; i < tiles; i += 8) merge(mx, sum, p.part[i * p.N + n]);
   part[w][lane] = make_float2(mx, sum);
   __syncthreads();
   if (w != 0 || n >= p.N) return;
-  for (int i = 1; i < 8; ++i) {
-    const float2 v = part[i][lane];
-    const float m2 = max_nan(mx, v.x);
-    if (m2 == -INFINITY) continue;
-    sum = sum * exp2f(mx - m2) + v.y * exp2f(v.x - m2);
-    mx = m2;
-  }
-  const float lse = (float)(((double)mx + (double)log2f(sum)) * 0.6931471805599453);
-  p.lse[n] = lse;
+  for (int i = 1; i < 8; ++i) merge(mx, sum, part[i][lane]);
+  const double others = ((double)mx + (double)log2f(sum)) / (double)kLog2e;  // (the constant that scaled them)
   const int64_t t = p.target[n];
+  const bool word = t >= 0 && t < p.V;
   // an ignored row adds nothing; a target outside the vocabulary makes the loss NaN
-  float row = 0.f;
-  if (t != p.ignore) row = (t >= 0 && t < p.V) ? lse - p.tgt[n] : __int_as_float(0x7fc00000);
+  const float nan = __int_as_float(0x7fc00000);
+  float row = nan;
+  float lse = (float)others;
+  if (word) {
+    const float tgt = p.tgt[n];
+    const double l = tgt == INFINITY ? (double)nan : (double)tgt;  // (inf - inf: no softmax)
+    const double d = others - l, top = d > 0.0 ? others : l, rest = (double)log1pf(expf((float)-fabs(d)));
+    row = (float)((top - l) + rest);
+    lse = (float)(top + rest);
+  }
+  p.lse[n] = lse;
+  if (p.row_loss) p.row_loss[n] = row;
+  if (t == p.ignore) row = 0.f;
   if (p.reduction == kNone)
     p.loss[n] = row;
   else

@@ -3,15 +3,18 @@
 // Softmax cross entropy of hidden [N, D] against a vocabulary weight [V, D] without the
 // logits [N, V] in memory.  With l = hidden weight^T:
 //     lse_n = log sum_v exp(l_nv),  loss_n = lse_n - l_{n,t_n}
-//     dl_nv = (exp(l_nv - lse_n) - [v = t_n]) * g_n
+//     dl_nv = (exp(l_nv - lse_n) - [v = t_n]) * g_n, for the target itself expm1(-loss_n) * g_n
 //     dhidden = dl weight,  dweight = dl^T hidden
 // The factors g_n are dloss (sum) or dloss / count (mean) of every row that counts: they multiply
 // the finished products in fp32, and the operand dl is exp(l - lse) - [v = t] alone, so that
 // its largest entry, near -1, is not rounded together with a factor that is the same for every
 // row (one bf16 rounding of the factor moved both gradients by up to 2^-8).  With one dloss
 // per row (no reduction) the factors differ and are part of dl.
-// Forward: one matrix product whose epilogue keeps, of each tile, every row's maximum and
-// sum of exponentials (fp32); a second kernel merges the tiles.  Backward, piece of the
+// Forward: one matrix product whose epilogue keeps, of each tile, every row's maximum and sum of
+// exponentials (fp32) over all words but the target; a second kernel merges the tiles.  With lse' over
+// the others, loss = log(1 + exp(lse' - l_t)) and lse = l_t + loss: a row that its target dominates keeps
+// the digits of a small loss, which a sum with the target's own 1 in it, or a difference of lse and
+// l_t, would lose.  For the same reason the backward gets lse and the rows' losses.  Backward, piece of the
 // vocabulary by piece: the product again, with dl in bf16 (three parts of it for fp32
 // tensors) into a piece buffer, then its two products.  dhidden accumulates in fp32 over the pieces.
 #pragma once
@@ -24,6 +27,7 @@ namespace vl {
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum Reduction { kNone = 0, kSum = 1, kMean = 2 };
+constexpr int kKeepRows = 4;  // added to the reduction by callers whose lse has [2][N] numbers
 
 struct Problem {
   const void* hidden;       // [N, D]
@@ -34,10 +38,11 @@ struct Problem {
   int reduction;
   // forward
   float* lse;               // [N]
+  float* row_loss;          // [N], or null: not kept
   float* loss;              // [N] (kNone) or [1]
   float* stats;             // [2]: sum of the rows' losses, number of rows that count
-  float2* part;             // [tiles][rows at once]: of a tile's row, m = max * log2(e) rounded, and
-                            // sum of 2^(l * log2(e) - m)
+  float2* part;             // [tiles][rows at once]: of a tile's row, without the target's word,
+                            // m = max * log2(e) rounded, and sum of 2^(l * log2(e) - m)
   float* tgt;               // [N]: the target's logit
   // backward
   const float* dloss;       // [N] (kNone) or [1]
@@ -112,6 +117,7 @@ inline Problem rows_from(const Problem& p, int64_t r0, int64_t elem) {
   r.N = p.N - r0 < kRowsAtOnce ? p.N - r0 : kRowsAtOnce;
   r.hidden = (const char*)p.hidden + r0 * p.D * elem;
   r.target += r0, r.lse += r0, r.tgt += r0;
+  if (p.row_loss) r.row_loss += r0;
   if (p.reduction == kNone) r.loss += r0;
   return r;
 }

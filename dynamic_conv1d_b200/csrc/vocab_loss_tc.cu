@@ -53,7 +53,7 @@ constexpr uint32_t kABytes = kHalfM * kKB * 2, kBBytes = kHalfB * kKB * 2, kStag
 constexpr uint32_t kAtom = 64 * kKB * 2;  // one 64 x 64 box
 constexpr uint32_t kStageOut = 32 * 128;  // an epilogue warp's 32 rows x 64 columns of bf16, staged for a TMA store
 constexpr int kSmem = kStages * (int)kStageBytes + kEpiWarps * (int)kStageOut + 1024;
-static_assert(kSmem <= 232448 - 1024, "shared memory of one CTA");
+static_assert(kSmem <= 232448 - 2048, "shared memory of one CTA");
 // The tensor core's accumulation truncates: a sum of 4096 products came out 3.8e-6 of itself too
 // small, which the loss's 32 bits would show (1.1e-6 of it).  Where the inner dimension is longer
 // than kChain blocks (2048 products), the forward sums that many at a time and adds those sums
@@ -187,15 +187,27 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
-// dl of n columns, in place.  f: the row's factor, at: the target's column among them.
+// v[at].  (Selected by masks: an indexed read would put v into local memory.)
 template <int n>
-__device__ __forceinline__ void logits_gradient(float (&v)[n], float f, float lse2, int64_t at) {
+__device__ __forceinline__ float pick(const float (&v)[n], int at) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int j = 0; j < n; ++j) bits |= __float_as_uint(v[j]) & -(uint32_t)(j == at);
+  return __uint_as_float(bits);
+}
+
+// dl of n columns, in place.  f: the row's factor, at: the target's column among them, own: its gradient (null
+// where the row's loss was not kept).  lse2 = lse * log2(e), rounded: an error of 2^-24 lse in each exponent, as the
+// logits themselves have.
+template <int n>
+__device__ __forceinline__ void logits_gradient(float (&v)[n], float f, float lse2, int at, const float* own) {
 #pragma unroll
   for (int j = 0; j < n; ++j) v[j] = f != 0.f ? ex2(fmaf(v[j], kLog2e, -lse2)) * f : 0.f;  // (an ignored row's NaN stays out)
   if (at >= 0 && at < n) {
+    const float g = own ? *own : pick(v, at) - f;
 #pragma unroll
     for (int j = 0; j < n; ++j)
-      if (j == at) v[j] -= f;
+      if (j == at) v[j] = g;
   }
 }
 
@@ -344,6 +356,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   __shared__ uint64_t full_bar[kStages], empty_bar[kStages], accf_bar[2], acce_bar[2], drain_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
+  // kTcGrad: each row's dl at its target, needed by one column of it (in a register it cost the fp32 backward
+  // 2 us of 102 at 1021 x 256 x 4999: beside 128 sums there is none left)
+  __shared__ float target_dl[MODE == kTcGrad ? kEpiWarps : 1][32];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int n_tiles = g.m_tiles * g.n_tiles * g.z;
   const int rank = (int)cta_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -481,6 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
           if (row_in) {
             f = row_factor(p, row, target);
             lse2 = p.lse[row] * kLog2e;
+            if (p.row_loss) target_dl[warp - 2][lane] = f != 0.f ? f * expm1f(-p.row_loss[row]) : 0.f;
           }
         }
       }
@@ -539,6 +555,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             tmem_ld_wait();
           }
           if constexpr (kForward) {
+            if (mine >= c && mine < c + kStep) {  // the target's logit leaves the others' sum
+              p.tgt[row] = pick(v, mine - c);
+#pragma unroll
+              for (int j = 0; j < kStep; ++j)
+                if (j == mine - c) v[j] = -INFINITY;
+            }
             const int left = there - c;
             float mx = -INFINITY;
             if (left >= kStep) {
@@ -562,16 +584,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
               sum = fmaf(sum, ex2(m2 - m_new), s0 + s1);
               m2 = m_new;
             }
-            if (mine >= c && mine < c + kStep) {
-              uint32_t bits = 0;  // (selected by masks: an indexed read would put v into local memory)
-#pragma unroll
-              for (int j = 0; j < kStep; ++j) bits |= __float_as_uint(v[j]) & -(uint32_t)(j == mine - c);
-              p.tgt[row] = __uint_as_float(bits);
-            }
           } else if constexpr (MODE == kTcAdd) {
             if (row_in) add_columns(g, v, row, col0 + c, t.z, factor);
           } else if constexpr (COPIED) {
-            logits_gradient(v, f, lse2, target - g.col0 - (col0 + c));
+            logits_gradient(v, f, lse2, mine - c, p.row_loss ? &target_dl[warp - 2][lane] : nullptr);
 #pragma unroll
             for (int j = 0; j < kStep; ++j) chained[c + j] = v[j];
             // 64 columns at a time, part by part, through the staged tile (fp32, 1021 x 256 x 4999: 102 us for the
@@ -607,7 +623,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
               __syncwarp();
             }
             if constexpr (MODE == kTcGrad) {
-              logits_gradient(v, f, lse2, target - g.col0 - (col0 + c));
+              logits_gradient(v, f, lse2, mine - c, p.row_loss ? &target_dl[warp - 2][lane] : nullptr);
             } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] *= factor;

@@ -1,8 +1,8 @@
 """Softmax cross entropy over a large vocabulary, in pieces of it, without keeping the
 logits (libdynconv's ``dynconv_vocab_loss_fwd`` / ``dynconv_vocab_loss_bwd``).
 
-The forward reads the hidden states and the vocabulary's weight once and keeps one float32
-per token (the logarithm of the sum of exponentials).  The backward computes the logits
+The forward reads the hidden states and the vocabulary's weight once and keeps two float32
+per token (the logarithm of the sum of exponentials, and the token's loss).  The backward computes the logits
 again, one piece of the vocabulary at a time, into a buffer that holds that piece's
 gradient only.  float32 tensors are multiplied as three bfloat16 parts each, to float32
 accuracy.
@@ -14,6 +14,7 @@ import torch
 from . import _lib
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_KEEP_ROWS = 4  # added to the reduction for the library
 
 
 def _aligned(t):
@@ -32,14 +33,14 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         code = _lib.dtype_code(hidden.dtype)
         hidden, w = _aligned(hidden), _aligned(weight if weight.dtype == hidden.dtype else weight.to(hidden.dtype))
         loss = torch.empty((N,) if reduction == 0 else (), device=hidden.device, dtype=torch.float32)
-        kept = torch.empty(N + 2, device=hidden.device, dtype=torch.float32)  # stats, lse
+        kept = torch.empty(2 * N + 2, device=hidden.device, dtype=torch.float32)  # stats, lse, the rows' losses
         n = lib.dynconv_vocab_loss_fwd_workspace_bytes(N, D, V, code)
         ws = torch.empty(max(n, 1), device=hidden.device, dtype=torch.uint8)
         _lib.check(
             lib.dynconv_vocab_loss_fwd(
                 hidden.data_ptr(), w.data_ptr(), target.data_ptr(), loss.data_ptr(), kept.data_ptr() + 8,
-                kept.data_ptr(), ws.data_ptr(), ws.numel(), N, D, V, ignore_index, reduction, code,
-                _lib.raw_stream(hidden),
+                kept.data_ptr(), ws.data_ptr(), ws.numel(), N, D, V, ignore_index, reduction + _KEEP_ROWS,
+                code, _lib.raw_stream(hidden),
             )
         )
         _lib.after_call(loss)
@@ -66,7 +67,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
             lib.dynconv_vocab_loss_bwd(
                 hidden.data_ptr(), w.data_ptr(), target.data_ptr(), kept.data_ptr() + 8, kept.data_ptr(),
                 dloss.data_ptr(), None if dh is None else dh.data_ptr(), None if dw is None else dw.data_ptr(),
-                ws.data_ptr(), ws.numel(), N, D, V, ignore_index, reduction, code, _lib.raw_stream(hidden),
+                ws.data_ptr(), ws.numel(), N, D, V, ignore_index, reduction + _KEEP_ROWS, code, _lib.raw_stream(hidden),
             )
         )
         _lib.after_call(hidden)

@@ -314,12 +314,16 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
  *   reduction: 0 none (loss [N]), 1 sum, 2 mean over the rows that count (loss [1]; NaN
  *   when none does).  loss, lse [N] and stats [2] are float32; lse and stats are kept for
  *   the backward (stats: sum of the rows' losses, number of rows that count).
+ *   reduction + DYNCONV_LOSS_KEEP_ROWS, in both calls: lse is [2][N], the second N numbers being the
+ *   rows' losses.  Without them the gradient at a row's target is a difference with lse, off by 2^-24
+ *   of lse, which a row whose loss is as small does not bear; the loss has its digits either way.
  * float32 tensors are multiplied as three bf16 parts each, and bf16 ones whose D is no multiple
  * of 8 as padded copies: the workspaces hold those (of weight at most 512 MB at a time).
  * Workspaces are 16-byte aligned, and so are bf16 tensors with D a multiple of 8, which are
  * read and written in place (DYNCONV_ERR_ALIGN; for dweight the workspace holds a copy of hidden
  * without the rows that do not count).
  * N <= 2^30, V <= 4194304. */
+#define DYNCONV_LOSS_KEEP_ROWS 4
 size_t dynconv_vocab_loss_fwd_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype);
 int dynconv_vocab_loss_fwd(const void* hidden, const void* weight, const int64_t* target,
                            float* loss, float* lse, float* stats, void* workspace, size_t workspace_bytes,

@@ -12,10 +12,12 @@ Tolerances (relative 2-norm):
 """
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
-from dynamic_conv1d_b200 import check_device, linear_cross_entropy
+from dynamic_conv1d_b200 import _lib, check_device, linear_cross_entropy
 
 pytestmark = pytest.mark.gpu
 
@@ -397,3 +399,80 @@ def test_words_that_are_excluded(D, first, count):
     assert linear_cross_entropy(h, w, t, reduction="none").isnan().all()
     w[:, 0] = -float("inf")
     assert linear_cross_entropy(h, w, t, reduction="none").isnan().all()
+
+
+def dominated(c, D, V, dtype):
+    """Rows whose target's logit is c + r_t, all others being r_v in [-3, 3]: exact in every product and sum
+    (c and r are multiples of 1/32, below 128).  Returns (hidden, weight, target, loss in 64 bits)."""
+    N = len(c)
+    g = torch.Generator(device="cuda").manual_seed(N)
+    r = (torch.randn(V, device="cuda", generator=g).clamp(-3, 3) * 32).round() / 32
+    t = torch.randperm(V, device="cuda", generator=g)[:N]
+    h, w = torch.zeros(N, D, device="cuda"), torch.zeros(V, D, device="cuda")
+    i = torch.arange(N, device="cuda")
+    h[i, i], w[t, i] = torch.tensor(c, device="cuda"), 1.0
+    h[:, N], w[:, N] = 1.0, r
+    l = h.double() @ w.double().T
+    d = l - l.gather(1, t[:, None])
+    d[i, t] = -math.inf
+    return h.to(dtype), w.to(dtype), t, torch.log1p(d.exp().sum(1))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("D", [16, 17])
+@pytest.mark.parametrize("V", [500, 50000])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_rows_dominated_by_their_target(dtype, D, V, reduction):
+    """A confident row's loss and gradient keep their digits, row by row: they are what the other words
+    add, not a difference of two large numbers.
+
+    Each other word's exponent, below 128, is rounded to 2^-18 (2^-18.5 of the word's share) and its
+    factor log2(e) is off by 2^-26 (2^-20), exp() by 2^-22, and up to 100 sums by 2^-24 each (2^-17.3): 1e-5
+    together.  In fp32 the gradient's products add 2^-20; in bf16 it is rounded twice (2^-8 each)."""
+    c = [0.0, 4.0, 10.0, 14.0, 18.0, 22.0, 25.0, 32.0, 60.0]
+    h, w, t, want = dominated(c, D, V, dtype)
+    own = [x.requires_grad_() for x in (h, w)]
+    loss = linear_cross_entropy(*own, t, reduction=reduction)
+    up = torch.linspace(1, 2, len(c), device="cuda") if reduction == "none" else torch.tensor(1.0, device="cuda")
+    loss.backward(up)
+    check_device(loss)
+    ref = {"none": want, "sum": want.sum(), "mean": want.mean()}[reduction]
+    assert ((loss.detach().double() - ref).abs() <= 1e-5 * ref).all()
+    # channel n is in row n's target alone: its gradients are the target's own
+    n = torch.arange(len(c), device="cuda")
+    dl = torch.expm1(-want) * (up.double() if reduction == "none" else 1.0 / (len(c) if reduction == "mean" else 1))
+    tol = 1.1e-5 if dtype == torch.float32 else 2.0**-7
+    dh = own[0].grad[n, n].double()
+    assert ((dh - dl).abs() <= tol * dl.abs()).all(), (dh / dl - 1)
+    dw, to = own[1].grad[t, n].double(), dl * torch.tensor(c, device="cuda")
+    assert ((dw - to).abs() <= tol * to.abs()).all(), (dw / to - 1)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_equal_logits(dtype):
+    """Many words share the maximum: log(V), and a gradient of 1/V (2^-22: log1p of an exact sum)."""
+    for V in (1, 2, 31, 128, 129, 5000):
+        h, w = torch.ones(3, 16, device="cuda", dtype=dtype), torch.full((V, 16), 0.5, device="cuda", dtype=dtype)
+        rows = linear_cross_entropy(h, w, torch.tensor([0, V // 2, V - 1], device="cuda"), reduction="none")
+        assert ((rows.double() - math.log(V)).abs() <= 2.0**-22 * math.log(V)).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_callers_that_keep_lse_alone(dtype):
+    """The library without DYNCONV_LOSS_KEEP_ROWS: lse has N numbers and none is written behind them; the
+    same loss, and gradients that differ by lse's rounding only."""
+    N, D, V = 130, 64, 300
+    h, w, t = make(N, D, V, dtype)
+    rl, rh, rw = check(h, w, t)
+    lib, code = _lib.load(), _lib.dtype_code(dtype)
+    stats, lse, loss = torch.empty(2, device="cuda"), torch.full((N + 8,), 7.0, device="cuda"), torch.empty((), device="cuda")
+    dh, dw, up = torch.empty_like(h), torch.empty_like(w), torch.ones((), device="cuda")
+    n = max(lib.dynconv_vocab_loss_fwd_workspace_bytes(N, D, V, code), lib.dynconv_vocab_loss_bwd_workspace_bytes(N, D, V, code, 1, 1))
+    ws = torch.empty(n, device="cuda", dtype=torch.uint8)
+    tail = (ws.data_ptr(), n, N, D, V, IGNORE, 2, code, _lib.raw_stream(h))
+    _lib.check(lib.dynconv_vocab_loss_fwd(*(x.data_ptr() for x in (h, w, t, loss, lse, stats)), *tail))
+    _lib.check(lib.dynconv_vocab_loss_bwd(*(x.data_ptr() for x in (h, w, t, lse, stats, up, dh, dw)), *tail))
+    check_device(h)
+    assert torch.equal(loss, rl) and (lse[N:] == 7.0).all()
+    assert rel(lse[:N], torch.logsumexp(h.double() @ w.double().T, 1)) <= LOSS
+    assert rel(dh, rh) <= GRAD[dtype] and rel(dw, rw) <= GRAD[dtype]
