@@ -56,12 +56,15 @@ constexpr int kSmem = kStages * (int)kStageBytes + kEpiWarps * (int)kStageOut + 
 static_assert(kSmem <= 232448 - 2048, "shared memory of one CTA");
 // The tensor core's accumulation truncates: a sum of 4096 products came out 3.8e-6 of itself too
 // small, which the loss's 32 bits would show (1.1e-6 of it).  Where the inner dimension is longer
-// than kChain blocks (2048 products), the forward sums that many at a time and adds those sums
-// up in registers (kTcForwardLong; a form of its own, as it needs 128 registers more).
+// than kChain blocks (2048 products), the logits are summed that many at a time and those sums added
+// up in registers (the long modes; forms of their own, as they need 128 registers more).  The backward does as
+// the forward, bit for bit: dl is the difference of a logit and the forward's sums, and where a row's target
+// dominates it, dl is smaller than what the two ways of adding differ by.  The gradients' own sums are not
+// broken up: over 16384 tokens they lose 2^-16, and are rounded to 2^-8.
 constexpr int kChain = 32;
 constexpr int kHalf = kN / 2;  // columns of one epilogue warp; a forward tile's partials are per half
 
-enum TcMode { kTcForward, kTcForwardLong, kTcGrad, kTcAdd, kTcStore };
+enum TcMode { kTcForward, kTcForwardLong, kTcGrad, kTcGradLong, kTcAdd, kTcStore };
 
 struct TcGemm {
   int64_t M, N;        // extents of the output
@@ -332,13 +335,14 @@ __device__ __forceinline__ void add_columns(const TcGemm& g, const float (&v)[32
   }
 }
 
-// 32 columns of a row, rounded into half of the warp's staged tile (128-byte swizzle).
-__device__ __forceinline__ void stage_columns(uint8_t* tile, int row, int half, const float (&v)[32]) {
+// n columns of a row from column c on, rounded into the warp's staged tile (128-byte swizzle).
+template <int n>
+__device__ __forceinline__ void stage_columns(uint8_t* tile, int row, int c, const float (&v)[n]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < n / 8; ++j) {
     const uint4 u = make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
                                pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-    *reinterpret_cast<uint4*>(tile + row * 128 + (((half * 4 + j) ^ (row & 7)) << 4)) = u;
+    *reinterpret_cast<uint4*>(tile + row * 128 + (((c / 8 + j) ^ (row & 7)) << 4)) = u;
   }
 }
 
@@ -348,7 +352,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
                  const __grid_constant__ CUtensorMap omap, const __grid_constant__ TcGemm g, const __grid_constant__ Problem p) {
   constexpr bool COPIED = PARTS > 0;
   constexpr bool kForward = MODE == kTcForward || MODE == kTcForwardLong;
-  constexpr bool kChained = MODE == kTcForwardLong || COPIED;  // sums of kBlocks blocks are added up in registers
+  constexpr bool kGrad = MODE == kTcGrad || MODE == kTcGradLong;
+  constexpr bool kChained = MODE == kTcForwardLong || MODE == kTcGradLong || COPIED;  // sums of kBlocks blocks are added up in registers
   constexpr int kBlocks = COPIED ? kCopyChain * products_of(PARTS) : kChain;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
@@ -356,9 +361,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   __shared__ uint64_t full_bar[kStages], empty_bar[kStages], accf_bar[2], acce_bar[2], drain_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  // kTcGrad: each row's dl at its target, needed by one column of it (in a register it cost the fp32 backward
+  // kGrad: each row's dl at its target, needed by one column of it (in a register it cost the fp32 backward
   // 2 us of 102 at 1021 x 256 x 4999: beside 128 sums there is none left)
-  __shared__ float target_dl[MODE == kTcGrad ? kEpiWarps : 1][32];
+  __shared__ float target_dl[kGrad ? kEpiWarps : 1][32];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int n_tiles = g.m_tiles * g.n_tiles * g.z;
   const int rank = (int)cta_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -490,9 +495,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       const bool row_in = row < g.M;
       float f = 0.f, lse2 = 0.f;
       int64_t target = -1;
-      if constexpr (kForward || MODE == kTcGrad) {
+      if constexpr (kForward || kGrad) {
         if (row_in) target = p.target[row];
-        if constexpr (MODE == kTcGrad) {
+        if constexpr (kGrad) {
           if (row_in) {
             f = row_factor(p, row, target);
             lse2 = p.lse[row] * kLog2e;
@@ -618,22 +623,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             // bf16: 64 columns at a time through the warp's staged tile and a TMA store, which
             // leaves out what lies beyond the matrix
             uint8_t* tile = smem + kStages * kStageBytes + (warp - 2) * kStageOut;
-            if ((c & 32) == 0) {
+            if (c % 64 == 0) {
               if (lane == 0) bulk_wait_group_read<0>();
               __syncwarp();
             }
-            if constexpr (MODE == kTcGrad) {
+            if constexpr (kGrad) {
               logits_gradient(v, f, lse2, mine - c, p.row_loss ? &target_dl[warp - 2][lane] : nullptr);
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= factor;
+              for (int j = 0; j < kStep; ++j) v[j] *= factor;
             }
-            stage_columns(tile, lane, (c >> 5) & 1, v);
-            if (c & 32) {
+            stage_columns(tile, lane, c % 64, v);
+            if ((c + kStep) % 64 == 0) {
               fence_proxy_async_smem();
               __syncwarp();
               if (lane == 0) {
-                tma_store_2d(&omap, tile, (int)(col0 + c - 32), t.m * kM + rank * kHalfM + q * 32);
+                tma_store_2d(&omap, tile, (int)(col0 + c + kStep - 64), t.m * kM + rank * kHalfM + q * 32);
                 bulk_commit_group();
               }
             }
@@ -649,7 +654,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         if (lane == 0) arrive_in_first_cta(freed[a]);
       }
     }
-    if constexpr (MODE == kTcGrad || MODE == kTcStore) {
+    if constexpr (kGrad || MODE == kTcStore) {
       if (lane == 0) bulk_wait_group_read<0>();  // (shared memory may go once it has been read)
     }
   }
@@ -783,7 +788,10 @@ int bwd(const Problem& p, const Plan& pl, int dtype) {
     TcGemm g{};
     g.M = p.N, g.N = vp, g.k_blocks = blocks_of(p.D), g.z = 1, g.group = row_group(p.D, dtype);
     g.col0 = v0;
-    if ((s = launch<kTcGrad, false, false, PARTS>(hk, wk, po, g, p, "vl_tc_kernel (logits' gradient)"))) return s;
+    s = COPIED || g.k_blocks <= kChain
+            ? launch<kTcGrad, false, false, PARTS>(hk, wk, po, g, p, "vl_tc_kernel (logits' gradient)")
+            : launch<kTcGradLong, false, false, 0>(hk, wk, po, g, p, "vl_tc_kernel (logits' gradient)");
+    if (s) return s;
     if (p.dweight) {
       void* dw = (char*)p.dweight + v0 * p.D * elem;
       const bool finish = pl.z_w > 1 || !direct;

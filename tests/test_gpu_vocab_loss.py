@@ -476,3 +476,68 @@ def test_callers_that_keep_lse_alone(dtype):
     assert torch.equal(loss, rl) and (lse[N:] == 7.0).all()
     assert rel(lse[:N], torch.logsumexp(h.double() @ w.double().T, 1)) <= LOSS
     assert rel(dh, rh) <= GRAD[dtype] and rel(dw, rw) <= GRAD[dtype]
+
+
+def long_rows(D, signed):
+    """Rows whose targets have logits of 5 to 40, among 300 words of about one (all h positive: and among the
+    other rows' targets)."""
+    N, V = 12, 300
+    g = torch.Generator(device="cuda").manual_seed(D)
+    h = torch.rand(N, D, device="cuda", generator=g).add_(0.5)
+    if signed:
+        h = torch.where(torch.rand(N, D, device="cuda", generator=g) < 0.5, -h, h)
+    h = h.bfloat16()
+    w = (torch.randn(V, D, device="cuda", generator=g) * D**-0.5).bfloat16()
+    t = torch.randperm(V, device="cuda", generator=g)[:N]
+    size = torch.tensor([5.0, 10.0, 20.0, 40.0], device="cuda").repeat(3)
+    w[t] = (h.float() * (size / h.float().square().sum(1))[:, None]).bfloat16()
+    return h, w, t, size
+
+
+@pytest.mark.parametrize("signed", [False, True])
+@pytest.mark.parametrize("D", [2056, 4096, 5000])
+def test_rows_of_long_sums(D, signed):
+    """Loss and gradient row by row where a logit has more than 2048 products (bf16).
+
+    A logit of 40 is a sum whose products the tensor core truncates, by 2^-30 of the sum for each of
+    2048: 8e-5, and so is every word's share.  dl is rounded by 2^-8 of each entry, the result by 2^-8."""
+    h, w, t, _ = long_rows(D, signed)
+    l = h.double() @ w.double().T
+    i = torch.arange(len(t), device="cuda")
+    share = (l - l.gather(1, t[:, None])).exp()
+    share[i, t] = 0.0
+    want = torch.log1p(share.sum(1))
+    dl = share * torch.exp(-want)[:, None]
+    dl[i, t] = torch.expm1(-want)
+    own = h.requires_grad_()
+    rows = linear_cross_entropy(own, w, t, reduction="none")
+    rows.sum().backward()
+    assert ((rows.detach().double() - want).abs() <= 2e-4 * want).all(), rows.detach().double() / want - 1
+    ref = dl @ w.double()
+    size = lambda x: torch.linalg.vector_norm(x.double(), dim=1)  # noqa: E731
+    err, terms = size(own.grad.double() - ref), dl.abs() @ size(w)
+    assert (err <= (2.0**-8 + 2e-4) * terms + 2.0**-8 * size(ref)).all(), err / terms
+
+
+@pytest.mark.parametrize("D", [64, 2048, 2056, 4096, 8192])
+def test_forward_and_backward_add_up_alike(D):
+    """A gradient without the rows' losses is a difference of the backward's logit and the forward's sums:
+    the logits are the same bits in both, so what is left at the target of a row that it has to itself is
+    the rounding of lse, twice (2^-24 of it each), of the exponent and of exp(): less than 4 * 2^-24 of lse."""
+    h, w, t, size = long_rows(D, True)
+    w = w * 0.01
+    w[t] *= 100
+    N, V = len(t), w.shape[0]
+    lib = _lib.load()
+    stats, lse, loss = torch.empty(2, device="cuda"), torch.empty(N, device="cuda"), torch.empty((), device="cuda")
+    dh, up = torch.empty_like(h), torch.ones((), device="cuda")
+    n = max(lib.dynconv_vocab_loss_fwd_workspace_bytes(N, D, V, 0), lib.dynconv_vocab_loss_bwd_workspace_bytes(N, D, V, 0, 1, 0))
+    ws = torch.empty(n, device="cuda", dtype=torch.uint8)
+    tail = (ws.data_ptr(), n, N, D, V, IGNORE, 1, 0, _lib.raw_stream(h))
+    _lib.check(lib.dynconv_vocab_loss_fwd(*(x.data_ptr() for x in (h, w, t, loss, lse, stats)), *tail))
+    _lib.check(lib.dynconv_vocab_loss_bwd(*(x.data_ptr() for x in (h, w, t, lse, stats, up, dh)), None, *tail))
+    check_device(h)
+    # the largest logits: the other words have exp(-40) of the row, below fp32's rounding of the rest
+    big = size == 40
+    along = (dh.double() * w[t].double()).sum(1) / w[t].double().square().sum(1)  # dl at the target
+    assert (along[big].abs() <= 4 * 2.0**-24 * 40).all(), along
