@@ -23,8 +23,16 @@ __global__ void __launch_bounds__(256) vl_merge_kernel(const Problem p, int64_t 
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t n = (int64_t)blockIdx.x * 32 + lane;
   float mx = -INFINITY, sum = 0.f;
-  if (n < p.N)
-    for (int64_t i = w; i < tiles; i += 8) merge(mx, sum, p.part[i * p.N + n]);
+  if (n < p.N) {
+    constexpr int kFly = 4;  // tiles under way before the first is used
+    for (int64_t i = w; i < tiles; i += 8 * kFly) {
+      float2 v[kFly];
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) v[k] = i + 8 * k < tiles ? p.part[(i + 8 * k) * p.N + n] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) merge(mx, sum, v[k]);
+    }
+  }
   part[w][lane] = make_float2(mx, sum);
   __syncthreads();
   if (w != 0 || n >= p.N) return;
