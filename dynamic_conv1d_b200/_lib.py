@@ -149,10 +149,10 @@ def differentiable_once(backward):
 
     @functools.wraps(backward)
     def wrapper(ctx, *upstream):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *upstream)
         with torch.no_grad():
             grads = backward(ctx, *upstream)
-        if not torch.is_grad_enabled():
-            return grads
         there = [i for i, g in enumerate(grads) if g is not None]
         marked = _NoSecondDerivative.apply(*(grads[i].requires_grad_() for i in there))
         out = [None] * len(grads)
