@@ -15,10 +15,13 @@
 //
 // Measured (B200, graph replay): one row of 3 x 2048 channels at rank 15 2.3 us, a launch's time; 512
 // such rows 9.2 us; 256 rows of 3 x 4096 at rank 31 13.4 us with the tensors in L2 and 18.5 us
-// from HBM, where their 53 MB take 8.2 us: bound by the latency of a block's phases (slots, then
-// caches; U's tile; products; stores) at 20 warps per SM.  W = 8: 256 rows of 3 x 2048 at rank 15 9.6 us,
+// from HBM, where their 53 MB take 8.2 us.  What holds it there is the schedule: 1536 blocks at five per SM are
+// 2.08 rounds, the third for 56 of them, and a block goes through its phases (slots, then
+// caches; U's tile; products; stores) one after the other with only four others to fill the gaps.  W = 8: 256 rows of 3 x 2048 at rank 15 9.6 us,
 // 512 rows of 3 x 4096 at rank 31 51 us (30 and 191 on the CUDA cores, which keep the widest filters
-// with more than 47 ranks).  Headwise, 64 rows of 2048: 2.5 us.
+// with more than 47 ranks).  fp32 stays on the CUDA cores: 256 rows of 3 x 4096 at rank 31 52 us, W = 8 and 512
+// rows 195 us (floors 16 and 64).  Headwise, 64 rows of 2048: 2.4 us; 512 rows of 8192 channels from HBM 20 us in
+// bf16 (10.3 at the copy rate), 24.5 us in fp32 (20.8).
 #include "common.cuh"
 
 namespace dynconv {

@@ -36,8 +36,10 @@ __device__ __forceinline__ void dot4(float& acc, const float4& a, const float4& 
 // Everything is fp32; each output is rounded once.  Every product runs along a dense dimension of
 // both operands (w and the state are kept transposed), four elements per shared-memory read, and
 // a thread owns 2 x 2 scores and outputs or 2 x 4 elements of the state.  Bound by the latency of a
-// chunk's four phases: 2 x 512 tokens, 4 heads of 64 in fp32 take 24 us forward and 55 us backward
-// (B200), cut into segments of one to two chunks.
+// chunk's four phases: 2 x 512 tokens, 4 heads of 64 in fp32 take 24 us forward and 57 us backward
+// (B200), cut into segments of one to two chunks.  Longer ones are far from the bytes' time: 4 x 4096
+// tokens, 16 heads of 128 in fp32 2.4 and 6.4 ms (82 and 144 us), 8 heads of 256 in bf16 3.9 and 10.2 ms (41
+// and 72 us).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) la_simple_kernel(const __grid_constant__ Params p, int n_slices,
                                                              int state_only) {

@@ -19,11 +19,15 @@
 // so that while the scores groups mask chunk i and write the outputs of chunk i-1, the pipe has
 // KV and O2 of chunk i and O1 and Sc of the next.
 //
-// What bounds it: shared memory.  At 128 x 128 about 400 KB pass through it per chunk and CTA (80 KB
-// brought in, 224 KB of operands, W' 48, S 16, outputs 32), 3100 cycles at 128 bytes each; a
-// chunk takes 3000 to 3700 (tensor pipe 46% active, issue slots 50%).  Slices of 64 columns read x
-// and y once each for the two halves of w; 128 columns would not fit two chunks of tiles into
-// shared memory, and would leave half as many chains.
+// What bounds it: no unit by itself.  A chunk takes 3000 to 3700 cycles at 128 x 128, of which the tensor
+// pipe is active 46%, issue slots 50% and, by ncu's L1 / shared counter, shared memory 54%; warps
+// wait mostly for TMEM and for one another's barriers: the phases of a chunk hang on each other and
+// one CTA per SM has no other chain to fill the gaps.  (Counted at the port, with the products' operand
+// reads and TMA's writes, about 400 KB pass per chunk and CTA: 80 KB brought in, 224 KB of operands, W' 48, S 16,
+// outputs 32, 3100 cycles at 128 bytes.  The counter does not show that much; whether it sees operand
+// reads is not documented.)  Slices of 64 columns read x and y once each for the two halves of w, and compute the
+// scores twice; 128 columns in one CTA would not fit two chunks of tiles into shared memory.  A CTA pair
+// over 128 columns (cta_group::2, as the vocabulary loss has) has not been built.
 // Measured (B200, 16 heads of 128, bf16): forward of 4 x 4096 tokens 64 us, 4.2 TB/s of its 268 MB
 // (41 us at the copy rate); its backward, three roles in one launch, 188 us (384 chains on 148
 // SMs are three rounds of one per SM where 2.6 would do); 65536 tokens with a state in and out

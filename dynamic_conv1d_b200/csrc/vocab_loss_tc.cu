@@ -23,7 +23,7 @@
 // What bounds it: the tensor cores at the clock that the power limit leaves (pipe 88 to 92% active).
 // 16384 tokens x 2048 channels over 50001 words (B200, bf16): forward 2.2 ms, logits again 2.3,
 // weight gradient 2.15, hidden gradient 2.1 ms: 1.5 PFLOP/s each, 94% of a library product's
-// burst rate; back to back under the power limit the pass takes 10.6 ms (1.27 PFLOP/s; that
+// burst rate; back to back under the power limit the pass takes 10.8 ms (1.25 PFLOP/s; that
 // library product sustains 1.38).
 //
 // Copied operands (PARTS) go through the same kernel.  fp32: a small kernel writes each tensor as
@@ -32,11 +32,13 @@
 // registers (the tensor core's sums alone would be off by more than fp32's rounding).  Products at
 // 1/6 of the bf16 rate are 3.5 times what the fp32 units could do at their best.  Whole passes, forward
 // and backward (B200; in brackets fp32 products on the CUDA cores, in tiles of 128 x 128): 1021 tokens x
-// 256 channels over 4999 words 35 + 101 us (90 + 233), 1021 x 1024 x 8000 93 + 269 us (400 + 1226), 4096 x
+// 256 channels over 4999 words 34 + 102 us (90 + 233), 1021 x 1024 x 8000 93 + 269 us (400 + 1226), 4096 x
 // 2048 x 65536 5.0 + 16.2 ms (20.8 + 71.1): 1.25 PFLOP/s of bf16 products.  Few rows gain only over
 // large vocabularies, as the tensors are written anew: one row of 256 x 4999 25 + 61 us (19 + 40), of
-// 2048 x 65536 0.83 + 1.27 ms (0.63 + 1.52), 32 rows of the latter 0.59 + 1.12 (0.65 + 1.67).  bf16, 1021
-// x 257 x 4999: 118 us of kernels (430).
+// 2048 x 65536 0.83 + 1.27 ms (0.63 + 1.52), 32 rows of the latter 0.59 + 1.12 (0.65 + 1.67).  Elementary torch
+// operations are faster there: whole calls of one row of 2048 x 9000 188 us against 360 here, of 2048 x 20000 240
+// against 706; from about 64 rows on, or over 4999 words of 256, they are not.  bf16, 1021 x 257 x 4999: 118 us of
+// kernels (430).
 #include "vocab_loss.cuh"
 
 namespace dynconv {

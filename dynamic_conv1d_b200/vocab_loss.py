@@ -87,7 +87,8 @@ def linear_cross_entropy(
 
     Args:
         hidden:       [..., D] (bfloat16 or float32, CUDA, contiguous).
-        weight:       [V, D], contiguous; cast to hidden's dtype when it has another one.
+        weight:       [V, D], contiguous; cast to hidden's dtype when it has another one (its
+                      gradient is then rounded to that dtype before it is cast back).
         target:       [...] int64, the index of each row's word.  Rows whose target is
                       ``ignore_index`` count for nothing, whatever they hold.  Any other target
                       outside 0..V-1 makes the loss NaN (and gives that row no gradient).
