@@ -17,7 +17,8 @@ import math
 import pytest
 import torch
 
-from dynamic_conv1d_b200 import _lib, check_device, linear_cross_entropy
+from dynamic_conv1d_b200 import _lib
+from dynamic_conv1d_b200 import check_device, linear_cross_entropy
 
 pytestmark = pytest.mark.gpu
 
@@ -541,3 +542,12 @@ def test_forward_and_backward_add_up_alike(D):
     big = size == 40
     along = (dh.double() * w[t].double()).sum(1) / w[t].double().square().sum(1)  # dl at the target
     assert (along[big].abs() <= 4 * 2.0**-24 * 40).all(), along
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("D", [64, 65])
+def test_hidden_gradient_alone_with_ignored_rows_of_anything(dtype, D):
+    h, w, t = make(300, D, 700, dtype)
+    hb = torch.where((t == IGNORE)[:, None], torch.full_like(h, float("nan")), h)
+    want, got = (torch.autograd.grad(linear_cross_entropy(x.requires_grad_(), w, t), x)[0] for x in (h, hb))
+    assert torch.equal(got, want) and got[t == IGNORE].count_nonzero() == 0
