@@ -7,6 +7,8 @@ hand-written sm_100a CUDA kernels (see ``include/dynconv.h``).  So are the opera
 them in a language model:
 
     decay_linear_attention[_fused]        linear attention with a decay for each head
+    gated_delta_rule                      the same with learned decays and corrections per token
+    gated_rms_norm, residual_rms_norm     norms fused with a gate, with the residual stream
     linear_cross_entropy                  the loss over a large vocabulary, without logits
     *_step, convolution_cache             one token at a time, on caches updated in place
 
@@ -17,6 +19,7 @@ DYNCONV_ERR_TIMEOUT).  Call it once per training step (or set DYNCONV_SYNC_CHECK
 / ``set_sync_checks(True)`` to check after every call while debugging).
 """
 from ._lib import DynconvError, check_device, set_sync_checks
+from .gated_delta import gated_delta_rule, gated_delta_rule_step
 from .headwise import headwise_dynamic_convolution
 from .linear_attention import decay_linear_attention, decay_linear_attention_fused, decay_linear_attention_step
 from .lowrank import lowrank_dynamic_convolution, lowrank_dynamic_convolution_grouped
@@ -26,6 +29,7 @@ from .modules import (
     LowRankDynamicShortConvolution,
     QKVLowRankDynamicShortConvolution,
 )
+from .norm import gated_rms_norm, residual_rms_norm
 from .parallel import data_parallel, shard_rows
 from .sequence_parallel import headwise_dynamic_convolution_sp, lowrank_dynamic_convolution_sp
 from .step import (
@@ -47,6 +51,10 @@ __all__ = [
     "decay_linear_attention",
     "decay_linear_attention_fused",
     "decay_linear_attention_step",
+    "gated_delta_rule",
+    "gated_delta_rule_step",
+    "gated_rms_norm",
+    "residual_rms_norm",
     "linear_cross_entropy",
     "LowRankDynamicShortConvolution",
     "QKVLowRankDynamicShortConvolution",

@@ -56,6 +56,19 @@ _SIGNATURES = {
     "dynconv_la_fwd": (_c_int, [_c_vp] * 8 + [_c_vp, _c_size] + [_c_i64] * 5 + [ctypes.c_float, _c_int, _c_vp]),
     "dynconv_la_bwd": (_c_int, [_c_vp] * 12 + [_c_vp, _c_size] + [_c_i64] * 5 + [ctypes.c_float, _c_int, _c_vp]),
     "dynconv_la_step": (_c_int, [_c_vp] * 7 + [_c_int, _c_vp] + [_c_i64] * 5 + [ctypes.c_float, _c_int, _c_vp]),
+    "dynconv_delta_kept_bytes": (_c_size, [_c_i64] * 5 + [_c_int]),
+    "dynconv_delta_fwd": (_c_int, [_c_vp] * 9 + [_c_size, _c_vp, _c_vp, _c_size] + [_c_i64] * 5 + [ctypes.c_float, _c_int, _c_vp]),
+    "dynconv_delta_workspace_bytes": (_c_size, [_c_i64] * 5 + [_c_int] * 2),
+    "dynconv_delta_bwd": (_c_int, [_c_vp] * 5 + [_c_size] + [_c_vp] * 10 + [_c_size] + [_c_i64] * 5
+                          + [ctypes.c_float, _c_int, _c_vp]),
+    "dynconv_delta_step": (_c_int, [_c_vp] * 8 + [_c_int, _c_vp] + [_c_i64] * 5 + [ctypes.c_float, _c_int, _c_vp]),
+    "dynconv_norm_workspace_bytes": (_c_size, [_c_i64]),
+    "dynconv_gated_norm_fwd": (_c_int, [_c_vp] * 5 + [_c_i64] * 3 + [ctypes.c_float] * 2 + [_c_int, _c_vp]),
+    "dynconv_gated_norm_bwd": (_c_int, [_c_vp] * 9 + [_c_size] + [_c_i64] * 3 + [ctypes.c_float] * 2 + [_c_int, _c_vp]),
+    "dynconv_residual_norm_fwd": (_c_int, [_c_vp] * 4 + [ctypes.c_float] + [_c_vp] * 2 + [_c_i64] * 2
+                                  + [ctypes.c_float, _c_int, _c_vp]),
+    "dynconv_residual_norm_bwd": (_c_int, [_c_vp] * 4 + [ctypes.c_float] + [_c_vp] * 7 + [_c_size] + [_c_i64] * 2
+                                  + [ctypes.c_float, _c_int, _c_vp]),
     "dynconv_vocab_loss_fwd_workspace_bytes": (_c_size, [_c_i64] * 3 + [_c_int]),
     "dynconv_vocab_loss_fwd": (_c_int, [_c_vp] * 7 + [_c_size] + [_c_i64] * 4 + [_c_int, _c_int, _c_vp]),
     "dynconv_vocab_loss_bwd_workspace_bytes": (_c_size, [_c_i64] * 3 + [_c_int] * 3),

@@ -88,12 +88,20 @@ int sm_count() {
   return n;
 }
 
+unsigned int dr_prep_error_word();
+unsigned int dr_fwd_error_word();
+unsigned int dr_bwd_error_word();
+unsigned int dr_grad_error_word();
 unsigned int lr_tc_error_word();
 unsigned int lr_bwd_tm_error_word();
 unsigned int hw_tma_error_word();
 unsigned int selftest_error_word();
 unsigned int vl_tc_error_word();
 unsigned int la_tc_error_word();
+int dr_prep_error_word_wire(unsigned int* host_word);
+int dr_fwd_error_word_wire(unsigned int* host_word);
+int dr_bwd_error_word_wire(unsigned int* host_word);
+int dr_grad_error_word_wire(unsigned int* host_word);
 int lr_tc_error_word_wire(unsigned int* host_word);
 int lr_bwd_tm_error_word_wire(unsigned int* host_word);
 int hw_tma_error_word_wire(unsigned int* host_word);
@@ -212,7 +220,8 @@ void wire_host_error_word(cudaStream_t st) {
   unsigned int* mine = static_cast<unsigned int*>(dp) + dev;
   if (lr_tc_error_word_wire(mine) || lr_bwd_tm_error_word_wire(mine) || hw_tma_error_word_wire(mine) ||
       selftest_error_word_wire(mine) || vl_tc_error_word_wire(mine) ||
-      la_tc_error_word_wire(mine)) {
+      la_tc_error_word_wire(mine) || dr_prep_error_word_wire(mine) || dr_fwd_error_word_wire(mine) ||
+      dr_bwd_error_word_wire(mine) || dr_grad_error_word_wire(mine)) {
     cudaGetLastError();
     return;
   }
@@ -237,6 +246,10 @@ int report_earlier_timeout(cudaStream_t st) {
     (void)hw_tma_error_word();
     (void)vl_tc_error_word();
     (void)la_tc_error_word();
+    (void)dr_bwd_error_word();
+    (void)dr_grad_error_word();
+    (void)dr_fwd_error_word();
+    (void)dr_prep_error_word();
   }
   return set_error(DYNCONV_ERR_TIMEOUT,
                    "a kernel launched earlier on device %d gave up a bounded wait (site %u): the outputs of that "
@@ -296,9 +309,11 @@ int dynconv_check_device(void* stream) {
   }
   // every word is read (and so cleared) before the first non-zero one is reported
   const unsigned int words[] = {lr_tc_error_word(), lr_bwd_tm_error_word(), selftest_error_word(),
-                                hw_tma_error_word(), vl_tc_error_word(), la_tc_error_word()};
+                                hw_tma_error_word(), vl_tc_error_word(), la_tc_error_word(),
+                                dr_prep_error_word(), dr_fwd_error_word(), dr_bwd_error_word(), dr_grad_error_word()};
   static const char* const kFile[] = {"lowrank forward", "lowrank backward", "self-test", "headwise",
-                                      "vocabulary loss", "linear attention"};
+                                      "vocabulary loss", "linear attention", "gated delta rule, chunks",
+                                      "gated delta rule, forward", "gated delta rule, backward", "gated delta rule, gradients"};
   for (unsigned int v : words)
     if (v == 0xFFFFFFFFu) return set_error(DYNCONV_ERR_CUDA, "could not read the device error word");
   for (size_t i = 0; i < sizeof(words) / sizeof(words[0]); ++i)

@@ -1,0 +1,182 @@
+// delta_chain.cuh -- the frame of the two chain kernels of the gated delta rule (formulas: delta_rule.cuh).
+//
+// A CTA walks the chunks of one (batch row, head) for `teams` slices of 16 of v's columns.  A team of W warps holds
+// a slice of the state, transposed: warp w keeps 16 x (128 / W) of it in registers, fp32, in the accumulators' layout,
+// and works out 16 x (C / W) of what belongs to tokens.  What the others need of a warp's numbers
+// goes through shared memory as bf16 parts in the layout of first operands, 16 bytes per lane.  One more
+// warp brings the next chunks' tiles by TMA into two or three stages.  (16-byte asynchronous copies by threads, of
+// one warp or four, took longer than a chunk's products: 10 to 20 bytes per cycle and SM.)
+//
+// Why teams: one warp per slice, its numbers all in registers, took 7400 cycles for a chunk of 64 tokens
+// and 128 x 128 states, four times what its matrix instructions need: every instruction waited for the one
+// before.  More warps hide that, and where there are few chains they bring idle quarters of the SM to bear.
+#pragma once
+
+#include "delta_rule.cuh"
+
+namespace dynconv {
+namespace dr {
+
+struct Plan {
+  int teams, stages;
+  int o_vectors;
+};
+
+template <typename G, int W>
+struct Chain {
+  static constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks;
+  static constexpr int TB = NB / W;          // token blocks of a warp
+  static constexpr int NT = 16 / W;          // its 8-column tiles of the state
+  static constexpr int PU = PX == 1 ? 2 : 3;  // parts of what the backward is given
+  using E = typename G::T;
+
+  static constexpr int kKq = PX * G::kTile * 2;  // bytes
+  static constexpr int kV = C * 16 * (int)sizeof(E);  // of a team: [C tokens][16 columns]
+  static constexpr int kT = G::kLower * NP * 512, kP = G::kLower * PP * 512, kGates = sizeof(Gates<C>);
+  static constexpr int kState = 8 * NP * 512, kBlock = NB * NP * 512;  // a team's buffers
+  static constexpr int kTeam = kState + 3 * kBlock;
+  static __host__ __device__ constexpr int stage_bytes(int teams) {
+    return (2 * kKq + teams * kV + kT + kP + kGates + 1023) / 1024 * 1024;
+  }
+  static constexpr int smem_bytes(int teams, int stages) { return 1024 + stages * stage_bytes(teams) + teams * kTeam; }
+
+  struct Stage {
+    uint8_t* at;
+    int teams;
+    __device__ __forceinline__ uint32_t k() const { return smem_u32(at); }
+    __device__ __forceinline__ uint32_t q() const { return smem_u32(at) + kKq; }
+    __device__ __forceinline__ E* v(int team) const { return (E*)(at + 2 * kKq + team * kV); }
+    __device__ __forceinline__ uint4* t() const { return (uint4*)(at + 2 * kKq + teams * kV); }
+    __device__ __forceinline__ uint4* p() const { return t() + kT / 16; }
+    __device__ __forceinline__ Gates<C>& gates() const { return *(Gates<C>*)(p() + kP / 16); }
+  };
+
+  struct Bars {
+    uint64_t full[3], empty[3];
+    int abort_flag;
+  };
+
+  // A warp's token block b and the team's barrier.
+  static __device__ __forceinline__ int token_block(int w, int b) { return b == 0 ? w : NB - 1 - w; }
+  static __device__ __forceinline__ void team_sync(int team) {
+    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(32 * W) : "memory");
+  }
+  // The barrier with "and" of `ok`: a team whose wait gave up leaves as a whole.
+  static __device__ __forceinline__ bool team_all(int team, bool ok) {
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.and.pred p, %2, %3, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(all)
+                 : "r"((uint32_t)ok), "r"(team + 1), "n"(32 * W)
+                 : "memory");
+    return all != 0;
+  }
+  static __device__ __forceinline__ int live_teams(const Plan& plan, int dv, int first_col) {
+    return min(plan.teams, (dv - first_col + 15) / 16);
+  }
+  static __device__ __forceinline__ void init(Bars& bars, int live) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < 3; ++i) mbar_init(&bars.full[i], 1), mbar_init(&bars.empty[i], live * W);
+      bars.abort_flag = 0;
+      fence_barrier_init();
+    }
+    __syncthreads();
+  }
+
+  // The producer's walk, one thread of it (BACK: from the last chunk to the first).
+  template <bool BACK>
+  static __device__ __forceinline__ void produce(uint8_t* smem, Bars& bars, const Plan& plan, const Maps& maps, const Prepared& pre, int b,
+                                                 int h, int64_t bh, int chunks, int dk, int dv, int first_col) {
+    const int bytes = stage_bytes(plan.teams), halves = dk > 64 ? 2 : 1, live = live_teams(plan, dv, first_col), slices = (dv + 15) / 16;
+    const uint32_t half = C * 128, all = 2 * PX * halves * half + live * kV + kT + kP + kGates;
+    int n = 0, s = 0, round = 0;
+    for (; n < chunks; ++n) {
+      if (round > 0 && !mbar_wait(&bars.empty[s], (round - 1) & 1, kErrWaitProducer, &bars.abort_flag)) break;
+      const Stage st{smem + s * bytes, plan.teams};
+      uint8_t *const k = st.at, *const q = st.at + kKq;
+      const int c = BACK ? chunks - 1 - n : n;
+      const int64_t at = bh * chunks + c;
+      uint64_t* const bar = &bars.full[s];
+      mbar_arrive_expect_tx(bar, all);
+      if (pre.k) {
+        for (int i = 0; i < PX; ++i) {
+          const int64_t from = (at * PX + i) * halves * (C * 64);
+          bulk_load(k + i * G::kTile * 2, pre.k + from, halves * half, bar);
+          bulk_load(q + i * G::kTile * 2, pre.q + from, halves * half, bar);
+        }
+      } else {
+        for (int d = 0; d < halves; ++d) {
+          tma_load_4d(k + d * half, &maps.k, bar, 64 * d, h, c * C, b, policy_evict_normal());
+          tma_load_4d(q + d * half, &maps.q, bar, 64 * d, h, c * C, b, policy_evict_normal());
+        }
+      }
+      for (int t = 0; t < live; ++t) {
+        if (pre.v)
+          bulk_load(st.v(t), (const E*)pre.v + (at * slices + first_col / 16 + t) * (C * 16), kV, bar);
+        else
+          tma_load_4d(st.v(t), &maps.v, bar, (first_col + 16 * t) * (int)(sizeof(E) / 2), h, c * C, b, policy_evict_normal());
+      }
+      bulk_load(st.t(), pre.t + at * (kT / 16), kT, bar);
+      bulk_load(st.p(), pre.p + at * (kP / 16), kP, bar);
+      bulk_load(&st.gates(), (const uint8_t*)pre.gates + at * kGates, kGates, bar);
+      if (++s == plan.stages) s = 0, ++round;
+    }
+    if (n < chunks)  // gave up: what is in flight lands before the shared memory goes
+      for (int i = max(0, n - plan.stages); i < n; ++i) mbar_drain(&bars.full[i % plan.stages], (i / plan.stages) & 1);
+  }
+
+  // The first row (last: one more than the last) of a [C] x [16] tile that holds a number that is not finite; C (0)
+  // where there is none.  One warp.
+  static __device__ __noinline__ int bad_row(const E* tile, bool last) {
+    int bad = last ? 0 : C;
+    for (int r = threadIdx.x & 31; r < C; r += 32)
+      for (int d = 0; d < 16; ++d)
+        if (!(fabsf(Elem<E>::to_f(tile[r * 16 + d])) < INFINITY)) bad = last ? max(bad, r + 1) : min(bad, r);
+    return last ? __reduce_max_sync(0xffffffffu, bad) : __reduce_min_sync(0xffffffffu, bad);
+  }
+
+  // A first operand's parts to and from a team's buffer.
+  template <int N>
+  static __device__ __forceinline__ void put(uint4* to, const uint32_t (&a)[N][4]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i * 32 + (threadIdx.x & 31)] = make_uint4(a[i][0], a[i][1], a[i][2], a[i][3]);
+  }
+  template <int N>
+  static __device__ __forceinline__ void get(const uint4* from, uint32_t (&a)[N][4]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint4 u = from[i * 32 + (threadIdx.x & 31)];
+      a[i][0] = u.x, a[i][1] = u.y, a[i][2] = u.z, a[i][3] = u.w;
+    }
+  }
+  // The same for the backward, as four matrices of 128 bytes.
+  static __device__ __forceinline__ void keep(__nv_bfloat16* to, const uint32_t (&a)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ((uint32_t*)to)[e * 32 + (threadIdx.x & 31)] = a[e];
+  }
+};
+
+template <typename G>
+int chain_maps(Maps* maps, const Prepared& pre, const View& k, const View& q, const View& v, int B, int64_t T, int H, int dk, int dv) {
+  int s = DYNCONV_OK;
+  if (!pre.k && ((s = view_map(&maps->k, k, B, T, H, dk, 2, 64, G::C)) || (s = view_map(&maps->q, q, B, T, H, dk, 2, 64, G::C)))) return s;
+  if (!pre.v) s = view_map(&maps->v, v, B, T, H, dv, sizeof(typename G::T), 16, G::C);
+  return s;
+}
+
+// CTAs of as few teams as let all slices run at once, each then having more of its SM's matrix units and shared
+// memory; four warps for a team then, and two where the SMs are full anyway: the shared operands are
+// read half as often.
+template <typename G, int W>
+Plan plan_of(int64_t bh, int dv) {
+  using Ch = Chain<G, W>;
+  constexpr int kMost = 227 * 1024 - 1024;  // (barriers)
+  const int slices = (dv + 15) / 16;
+  Plan p{};
+  p.teams = 1;
+  while (p.teams < 4 && Ch::smem_bytes(2 * p.teams, 2) <= kMost && bh * ((slices + p.teams - 1) / p.teams) > sm_count()) p.teams *= 2;
+  p.stages = Ch::smem_bytes(p.teams, 3) <= kMost ? 3 : 2;
+  return p;
+}
+
+}  // namespace dr
+}  // namespace dynconv

@@ -1,0 +1,375 @@
+// delta_rule_fwd.cu -- the gated delta rule over whole sequences: the chain over the chunks (formulas:
+// delta_rule.cuh; how the warps share the work: delta_chain.cuh).
+#include "delta_chain.cuh"
+
+namespace dynconv {
+namespace dr {
+namespace {
+
+// 16 rows x 16 columns, staged in shared memory, to the output.
+template <typename E>
+__device__ __noinline__ void store_slow(const E* tile, E* to, int64_t step, int rows, int cols) {
+  for (int i = threadIdx.x & 31; i < 16 * rows; i += 32)
+    if (i % 16 < cols) to[i / 16 * step + i % 16] = tile[i];
+}
+
+template <typename G, int W, bool SAVE>
+__global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __grid_constant__ Maps maps, Plan plan) {
+  using Ch = Chain<G, W>;
+  using E = typename G::T;
+  constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks, TB = Ch::TB, NT = Ch::NT, PU = Ch::PU;
+  constexpr int PS = PX == 1 ? 1 : 3;  // parts of the state in the outputs' product
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ typename Ch::Bars bars;
+  uint8_t* const smem = align_smem_1024(smem_raw);
+  const int64_t bh = blockIdx.y, b = bh / p.H, h = bh % p.H;
+  const int chunks = (int)((p.T + C - 1) / C), n_k16 = (p.dk + 15) / 16, first_col = blockIdx.x * plan.teams * 16;
+  const int warp = warp_index(), l = threadIdx.x & 31, row = l >> 2, col = 2 * (l & 3);
+  Ch::init(bars, Ch::live_teams(plan, p.dv, first_col));
+  if (warp == plan.teams * W) {
+    if (l == 0) Ch::template produce<false>(smem, bars, plan, maps, p.pre, (int)b, (int)h, bh, chunks, p.dk, p.dv, first_col);
+    return;
+  }
+  const int team = warp / W, w = (warp + team) % W;  // (turned, so that the last tokens' warps fall on different schedulers)
+  const int d0 = first_col + 16 * team, slices = (p.dv + 15) / 16, slice = d0 / 16;
+  if (d0 >= p.dv) return;
+  const int bytes = Ch::stage_bytes(plan.teams);
+  uint4* const state = (uint4*)(smem + plan.stages * bytes + team * Ch::kTeam);
+  uint4 *const part_r = state + Ch::kState / 16, *const part_u = part_r + Ch::kBlock / 16, *const part_s = part_u + Ch::kBlock / 16;
+  const KeyLane across(false);
+  const int v_across = lane_offset(16, false);
+  uint32_t down[NT / 2];  // this warp's columns of K, 16 at a time
+  {
+    const KeyLane lane(true);
+#pragma unroll
+    for (int m = 0; m < NT / 2; ++m) {
+      const int kk = w * NT / 2 + m;
+      down[m] = (NT == 8 || !(w & 1) ? lane.off[m] : lane.off[m + 2]) + (kk >> 2) * (C * 128);
+    }
+  }
+
+  float S[NT][4];  // S^T: rows d0 + row (+ 8), columns 8 (w NT + n) + col (+ 1) of dk
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = d0 + row + 8 * (e >> 1), k = 8 * (w * NT + n) + col + (e & 1);
+      S[n][e] = p.s_in && d < p.dv && k < p.dk ? p.s_in[(bh * p.dk + k) * p.dv + d] : 0.f;
+    }
+  // the state before chunk c to the team, and to the backward
+  auto publish = [&](int c) {
+#pragma unroll
+    for (int m = 0; m < NT / 2; ++m) {
+      const int kk = w * NT / 2 + m;
+      uint32_t a[NP][4];
+      operand<NP>(S[2 * m], S[2 * m + 1], a);
+      Ch::put(state + kk * NP * 32, a);
+      if constexpr (SAVE) {
+        if (kk < n_k16 && c < chunks)
+#pragma unroll
+          for (int i = 0; i < PS; ++i)
+            Ch::keep(p.states + ((((i * (int64_t)p.B * p.H + bh) * chunks + c) * slices + slice) * n_k16 + kk) * 256, a[i]);
+      }
+    }
+  };
+  publish(0);
+
+  for (int c = 0, stage = 0, parity = 0; c < chunks; ++c) {
+    if (!Ch::team_all(team, mbar_wait(&bars.full[stage], parity, kErrWaitMma, &bars.abort_flag))) return;
+    const typename Ch::Stage s{smem + stage * bytes, plan.teams};
+    const Gates<C>& gate = s.gates();
+    int bad = gate.bad;
+    // (K S0)^T and (Q S0)^T; the operands of the next 16 of dk are asked for before the products of these
+    float Z[TB][2][4], O[TB][2][4];
+    {
+      constexpr int L = TB == 1 ? 2 : 1;  // (two token blocks are enough independent work, and the registers they leave)
+      float z[TB][L][2][4], o[TB][L][2][4];
+#pragma unroll
+      for (int t = 0; t < TB; ++t)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int i = 0; i < L; ++i) zero(z[t][i][m]), zero(o[t][i][m]);
+      uint32_t a[2][NP][4], f[2][TB][PX][4], g[2][TB][PX][4];
+      auto fetch = [&](int kk, uint32_t(&a)[NP][4], uint32_t(&f)[TB][PX][4], uint32_t(&g)[TB][PX][4]) {
+        Ch::template get<NP>(state + kk * NP * 32, a);
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+          const uint32_t at = across.at<C>(Ch::token_block(w, t), kk);
+#pragma unroll
+          for (int i = 0; i < PX; ++i) {
+            ldsm(f[t][i], s.k() + at + i * G::kTile * 2);
+            ldsm(g[t][i], s.q() + at + i * G::kTile * 2);
+          }
+        }
+      };
+      fetch(0, a[0], f[0], g[0]);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        if (kk >= n_k16) continue;
+        if (kk + 1 < n_k16) fetch(kk + 1, a[(kk + 1) & 1], f[(kk + 1) & 1], g[(kk + 1) & 1]);
+        uint32_t a_o[PS][4];
+#pragma unroll
+        for (int i = 0; i < PS; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a_o[i][e] = a[kk & 1][i][e];
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+          mma_levels<NP, PX, NP, L>(z[t], a[kk & 1], f[kk & 1][t]);
+          mma_levels<PS, PX, PS, L>(o[t], a_o, g[kk & 1][t]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < TB; ++t) sum_levels<L>(Z[t], z[t]), sum_levels<L>(O[t], o[t]);
+    }
+    // (V - e^b K S0)^T in Z's place, O scaled
+    E* const v_tile = s.v(team);
+    float odd = 0.f;  // NaN if a value is not finite
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      const int t0 = 16 * Ch::token_block(w, t);
+      float v[2][4];
+      if constexpr (sizeof(E) == 2) {
+        uint32_t f[4];
+        ldsm_t(f, smem_u32(v_tile + t0 * 16 + v_across));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i >> 1][2 * (i & 1)] = low(f[i]), v[i >> 1][2 * (i & 1) + 1] = high(f[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[i >> 2][i & 3] = v_tile[(t0 + 8 * (i >> 2) + col + (i & 1)) * 16 + row + 8 * ((i >> 1) & 1)];
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const float2 eb = *reinterpret_cast<const float2*>(gate.e + t0 + 8 * m + col);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          odd = fmaf(v[m][e], 0.f, odd);
+          Z[t][m][e] = fmaf(-(e & 1 ? eb.y : eb.x), Z[t][m][e], v[m][e]);
+          O[t][m][e] *= p.scale * (e & 1 ? eb.y : eb.x);
+        }
+      }
+    }
+    const bool odd_here = __any_sync(0xffffffffu, !(odd == 0.f));
+    if (bad < C || odd_here) {  // (rare)
+      // What is not finite must not meet the zeros of T and P: values from the first bad token on count as zero.
+      bad = min(bad, Ch::bad_row(v_tile, false));
+#pragma unroll
+      for (int t = 0; t < TB; ++t)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * Ch::token_block(w, t) + 8 * m + col + (e & 1) >= bad) Z[t][m][e] = O[t][m][e] = 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      uint32_t a[NP][4];
+      operand<NP>(Z[t][0], Z[t][1], a);
+      Ch::put(part_r + Ch::token_block(w, t) * NP * 32, a);
+    }
+    // (another warp's tokens may be the bad ones)
+    if (!Ch::team_all(team, !odd_here)) bad = min(bad, Ch::bad_row(v_tile, false));
+    // r^T = (V - e^b K S0)^T T^T, U = beta r
+    float U[TB][2][4];
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      const int blk = Ch::token_block(w, t);
+      {
+        float u[NP][2][4];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) zero(u[i][0]), zero(u[i][1]);
+        uint32_t a[2][NP][4], f[2][NP][4];
+        const uint4* const t_at = s.t() + lower(blk, 0) * NP * 32;
+        Ch::template get<NP>(part_r, a[0]);
+        Ch::template get<NP>(t_at, f[0]);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          if (j > blk) continue;
+          if (j < blk) {
+            Ch::template get<NP>(part_r + (j + 1) * NP * 32, a[(j + 1) & 1]);
+            Ch::template get<NP>(t_at + (j + 1) * NP * 32, f[(j + 1) & 1]);
+          }
+          mma_levels<NP, NP, NP, NP>(u, a[j & 1], f[j & 1]);
+        }
+        sum_levels<NP>(U[t], u);
+      }
+      if constexpr (SAVE) {
+        uint32_t a[PU][4];
+        operand<PU>(U[t][0], U[t][1], a);
+#pragma unroll
+        for (int i = 0; i < PU; ++i)
+          Ch::keep(p.rest + ((((i * (int64_t)p.B * p.H + bh) * chunks + c) * slices + slice) * NB + blk) * 256, a[i]);
+      }
+      float x[2][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const float2 beta = *reinterpret_cast<const float2*>(gate.beta + 16 * blk + 8 * m + col);
+        const float2 out = *reinterpret_cast<const float2*>(gate.out + 16 * blk + 8 * m + col);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          U[t][m][e] *= e & 1 ? beta.y : beta.x;
+          x[m][e] = U[t][m][e] * (e & 1 ? out.y : out.x);
+        }
+      }
+      uint32_t a[NP][4];
+      operand<NP>(x[0], x[1], a);
+      Ch::put(part_s + blk * NP * 32, a);
+      uint32_t a_u[PU][4];
+      operand<PU>(U[t][0], U[t][1], a_u);
+      Ch::put(part_u + blk * PU * 32, a_u);
+    }
+    Ch::team_sync(team);
+    // S^T <- e^(b_C) S^T + (e^(b_C - b) U)^T K, each chunk's sum by itself first: the instruction's own
+    // additions are cut off, not rounded
+    const float total = gate.total;
+#pragma unroll
+    for (int n = 0; n < NT; n += 4) {
+      if (8 * (w * NT + n) >= 16 * n_k16) continue;
+      float x[4][4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) zero(x[m]);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        uint32_t a[NP][4];
+        Ch::template get<NP>(part_s + j * NP * 32, a);
+#pragma unroll
+        for (int m = 0; m < 4; m += 2) {
+          uint32_t f[PX][4];
+#pragma unroll
+          for (int i = 0; i < PX; ++i)
+            ldsm_t(f[i], s.k() + 2 * i * G::kTile + j * 2048 + down[(n + m) / 2]);
+          mma_parts<NP, PX, NP>(x[m], x[m + 1], a, f);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[n + m][e] = bad < C ? NAN : fmaf(total, S[n + m][e], x[m][e]);
+    }
+    // (the state's readers of this chunk passed the barriers above)
+    publish(c + 1);
+    // O^T += U^T P^T
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      const int blk = Ch::token_block(w, t);
+      {
+        float o[PU][2][4];
+#pragma unroll
+        for (int i = 0; i < PU; ++i) zero(o[i][0]), zero(o[i][1]);
+        uint32_t a[2][PU][4], f[2][PP][4];
+        const uint4* const p_at = s.p() + lower(blk, 0) * PP * 32;
+        Ch::template get<PU>(part_u, a[0]);
+        Ch::template get<PP>(p_at, f[0]);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          if (j > blk) continue;
+          if (j < blk) {
+            Ch::template get<PU>(part_u + (j + 1) * PU * 32, a[(j + 1) & 1]);
+            Ch::template get<PP>(p_at + (j + 1) * PP * 32, f[(j + 1) & 1]);
+          }
+          mma_levels<PU, PP, PU, PU>(o, a[j & 1], f[j & 1]);
+        }
+        float x[2][4];
+        sum_levels<PU>(x, o);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) O[t][m][e] += x[m][e];
+      }
+      if (bad < C) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * blk + 8 * m + col + (e & 1) >= bad) O[t][m][e] = NAN;
+      }
+      // through v's tile, of which nobody else needs these tokens and columns any more
+      const int64_t t0 = (int64_t)c * C + 16 * blk;
+      const int rows = (int)(p.T - t0 < 16 ? p.T - t0 : 16);
+      E* const to = (E*)p.o.p + b * p.o.sb + h * p.o.sh + t0 * p.o.st + d0;
+      E* const stage_o = v_tile + 16 * blk * 16;
+      if constexpr (sizeof(E) == 2) {
+        stsm_t(smem_u32(stage_o + v_across), pack(O[t][0][0], O[t][0][1]), pack(O[t][0][2], O[t][0][3]),
+               pack(O[t][1][0], O[t][1][1]), pack(O[t][1][2], O[t][1][3]));
+        __syncwarp();
+        if (plan.o_vectors) {
+          const int r = l >> 1, d = (l & 1) * 8;
+          if (r < rows && d0 + d < p.dv) *reinterpret_cast<uint4*>(to + r * p.o.st + d) = *reinterpret_cast<const uint4*>(stage_o + r * 16 + d);
+        } else {
+          store_slow(stage_o, to, p.o.st, rows, p.dv - d0);
+        }
+      } else {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 8 * m + col + (e & 1), d = row + 8 * (e >> 1);
+            if (r < rows && d0 + d < p.dv) to[r * p.o.st + d] = O[t][m][e];
+          }
+      }
+    }
+    if constexpr (sizeof(E) == 2) fence_proxy_async_smem();  // (the outputs went through the tile that is loaded again)
+    __syncwarp();
+    if (l == 0) mbar_arrive(&bars.empty[stage]);
+    if (++stage == plan.stages) stage = 0, parity ^= 1;
+  }
+  if (p.s_out) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = d0 + row + 8 * (e >> 1), k = 8 * (w * NT + n) + col + (e & 1);
+        if (d < p.dv && k < p.dk) p.s_out[(bh * p.dk + k) * p.dv + d] = S[n][e];
+      }
+  }
+}
+
+template <typename G, int W, bool SAVE>
+int go(const Forward& p, Plan plan, cudaStream_t st) {
+  using Ch = Chain<G, W>;
+  int s;
+  const int slices = (p.dv + 15) / 16;
+  plan.o_vectors = vectors_of(p.o, p.dv, sizeof(typename G::T));
+  const int smem = Ch::smem_bytes(plan.teams, plan.stages);
+  const cudaError_t e = cudaFuncSetAttribute(delta_fwd_kernel<G, W, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_status(e, "cudaFuncSetAttribute(delta_fwd)");
+  }
+  Maps maps{};
+  if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.v, p.B, p.T, p.H, p.dk, p.dv))) return s;
+  const dim3 grid((unsigned)((slices + plan.teams - 1) / plan.teams), (unsigned)(p.B * p.H));
+  delta_fwd_kernel<G, W, SAVE><<<grid, 32 * (plan.teams * W + 1), smem, st>>>(p, maps, plan);
+  DYNCONV_CHECK_LAUNCH("delta_fwd_kernel");
+  return DYNCONV_OK;
+}
+
+template <typename G, bool SAVE>
+int pick(const Forward& p, cudaStream_t st) {
+  const int64_t bh = (int64_t)p.B * p.H;
+  if constexpr (G::kBlocks == 4) {
+    const Plan four = plan_of<G, 4>(bh, p.dv);
+    if (four.teams <= 2) return go<G, 4, SAVE>(p, four, st);
+  }
+  return go<G, 2, SAVE>(p, plan_of<G, 2>(bh, p.dv), st);
+}
+
+}  // namespace
+
+// bf16 chains hold their numbers as two parts (16 digits: the outputs' own rounding is 8), as three where
+// the state after the last token goes back to the caller, who gets it in fp32.
+int forward_launch(const Forward& p, int dtype, cudaStream_t st) {
+  const bool save = p.states != nullptr, exact = p.s_out != nullptr;
+  const int s = prep_launch(p.pre, p.k, p.q, p.v, p.g, p.beta, p.B, p.H, p.T, p.dk, p.dv, p.scale, dtype, exact, false, st);
+  if (s) return s;
+  if (dtype == DYNCONV_DTYPE_F32) return save ? pick<CfgF32, true>(p, st) : pick<CfgF32, false>(p, st);
+  if (exact) return save ? pick<CfgBf16<true, false>, true>(p, st) : pick<CfgBf16<true, false>, false>(p, st);
+  return save ? pick<CfgBf16<false, false>, true>(p, st) : pick<CfgBf16<false, false>, false>(p, st);
+}
+
+}  // namespace dr
+
+DYNCONV_DEFINE_ERROR_ACCESSOR(dr_fwd_error_word)
+
+}  // namespace dynconv

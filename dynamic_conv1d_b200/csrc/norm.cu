@@ -1,0 +1,463 @@
+// norm.cu -- root-mean-square norms fused with what stands next to them in a layer.
+//
+// Gated norm (after a block, one row per head):
+//     r = rsqrt(mean(x^2) + eps),  y = scale * x r * w * silu(g)           (w, g optional)
+//     dn = scale * dy w silu(g),   dx = r (dn - x r^2 mean(dn x))
+//     dw = sum_rows scale * dy x r silu(g),  dg = scale * dy x r w silu'(g)
+// Residual norm (between two blocks):
+//     h = residual + s * x,  r = rsqrt(mean(h^2) + eps),  y = h r * w      (s a number or one per channel)
+//     dt = dh + r (dy w - h r^2 mean(dy w h)),  dresidual = dt,  dx = s dt
+//     dw = sum_rows dy h r,  ds = sum_rows dt x
+// Both sums that a backward row needs (of squares and of dn x) are of its inputs, so one pass over
+// the row gives them and nothing is kept from the forward but h, which the caller has anyway.
+//
+// Bound by HBM: a row is read once into registers (up to 16 numbers per thread) and written once; sums
+// are fp32.  A row belongs to 8..32 lanes of a warp, or to a whole CTA of 256 to 1024 threads above
+// 512 channels.  The sums over rows stay in the threads that own their columns; the CTAs'
+// partial rows are added up in a fixed order by a second launch, so results do not change from
+// run to run.
+#include "common.cuh"
+#include "norm.cuh"
+
+namespace dynconv {
+namespace norm {
+namespace {
+
+constexpr int kPerThread = 16;  // numbers of a row per thread, at most (32 spilled: the backward holds four tensors' and two sums)
+
+// A thread's share of a row, as stored.
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T)) Vec {
+  T e[VEC];
+};
+
+// Sums a and b over the TPR threads of a row, in every one of them.
+template <int TPR>
+__device__ __forceinline__ float2 row_sum(float2 v, int& flip) {
+  constexpr int kIn = TPR < 32 ? TPR : 32;
+#pragma unroll
+  for (int d = kIn / 2; d > 0; d >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, d);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, d);
+  }
+  if constexpr (TPR > 32) {
+    constexpr int kWarps = TPR / 32;
+    __shared__ float2 part[2][kWarps];  // (alternating: one barrier for each row)
+    if ((threadIdx.x & 31) == 0) part[flip][threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = part[flip][0];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) v.x += part[flip][i].x, v.y += part[flip][i].y;
+    flip ^= 1;
+  }
+  return v;
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
+
+// Threads of a CTA for a row of TPR threads.
+__host__ __device__ constexpr int cta(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// The sums over this CTA's rows: thread (row group, lane) holds N_ACC columns; groups are added in
+// order through shared memory and the result is the CTA's row of `part`.
+template <int TPR, int VEC, int NV>
+__device__ __forceinline__ void store_sums(const float (&acc)[NV * VEC], float* part, int D) {
+  constexpr int kGroups = cta(TPR) / TPR;
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  if constexpr (kGroups == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int c = (i * TPR + lane) * VEC + e;
+        if (c < D) part[c] = acc[i * VEC + e];
+      }
+  } else {
+    __shared__ float sh[kGroups][TPR * 4 + 1];
+#pragma unroll
+    for (int j = 0; j < NV * VEC; j += 4) {  // four numbers of each thread at a time
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e < NV * VEC) sh[group][lane * 4 + e] = acc[j + e];
+      __syncthreads();
+      for (int t = threadIdx.x; t < TPR * 4; t += cta(TPR)) {
+        const int k = j + t % 4;  // the number's index in its thread
+        const int c = (k / VEC * TPR + t / 4) * VEC + k % VEC;
+        if (k < NV * VEC && c < D) {
+          float s = sh[0][t];
+          for (int g = 1; g < kGroups; ++g) s += sh[g][t];
+          part[c] = s;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
+  using V = Vec<T, VEC>;
+  constexpr int kRows = cta(TPR) / TPR;
+  const int lane = threadIdx.x % TPR;
+  int flip = 0;
+  const int64_t rows = p.N * p.G;
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
+    const int64_t row = r0 + threadIdx.x / TPR;
+    const bool in = row < rows;
+    const int64_t n = in ? row / p.G : 0, g = in ? row % p.G : 0;
+    const T* x = (const T*)p.x + n * p.x_outer + g * p.x_inner;
+    const T* z = (const T*)p.gate + n * p.gate_outer + g * p.gate_inner;
+    V xv[NV], zv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (in && c < p.D) {
+        xv[i] = *reinterpret_cast<const V*>(x + c);
+        if (p.gate) zv[i] = *reinterpret_cast<const V*>(z + c);
+      }
+    }
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (in && (i * TPR + lane) * VEC < p.D)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float v = Elem<T>::to_f(xv[i].e[e]);
+          s.x = fmaf(v, v, s.x);
+        }
+    const float r = p.scale * rsqrtf(row_sum<TPR>(s, flip).x / p.D + p.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (!in || c >= p.D) continue;
+      V w{}, y;
+      if (p.weight) w = *reinterpret_cast<const V*>((const T*)p.weight + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        float v = Elem<T>::to_f(xv[i].e[e]) * r;
+        if (p.weight) v *= Elem<T>::to_f(w.e[e]);
+        if (p.gate) {
+          const float zf = Elem<T>::to_f(zv[i].e[e]);
+          v *= zf * sigmoid(zf);
+        }
+        y.e[e] = Elem<T>::from_f(v);
+      }
+      *reinterpret_cast<V*>((T*)p.y + row * p.D + c) = y;
+    }
+  }
+}
+
+template <typename T, int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(cta(TPR)) gated_bwd_kernel(Gated p) {
+  using V = Vec<T, VEC>;
+  constexpr int kRows = cta(TPR) / TPR;
+  const int lane = threadIdx.x % TPR;
+  int flip = 0;
+  const int64_t rows = p.N * p.G;
+  float acc[NV * VEC];
+#pragma unroll
+  for (int i = 0; i < NV * VEC; ++i) acc[i] = 0.f;
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
+    const int64_t row = r0 + threadIdx.x / TPR;
+    const bool in = row < rows;
+    const int64_t n = in ? row / p.G : 0, g = in ? row % p.G : 0;
+    const T* x = (const T*)p.x + n * p.x_outer + g * p.x_inner;
+    const T* z = (const T*)p.gate + n * p.gate_outer + g * p.gate_inner;
+    const T* dy = (const T*)p.dy + row * p.D;
+    V xv[NV], zv[NV], dv[NV], wv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (in && c < p.D) {
+        xv[i] = *reinterpret_cast<const V*>(x + c);
+        dv[i] = *reinterpret_cast<const V*>(dy + c);
+        if (p.gate) zv[i] = *reinterpret_cast<const V*>(z + c);
+        if (p.weight) wv[i] = *reinterpret_cast<const V*>((const T*)p.weight + c);
+      }
+    }
+    // dn = scale * dy w silu(g) is made twice: a second copy of the row would not stay in registers
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (in && (i * TPR + lane) * VEC < p.D)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float v = Elem<T>::to_f(xv[i].e[e]);
+          float dn = p.scale * Elem<T>::to_f(dv[i].e[e]);
+          if (p.weight) dn *= Elem<T>::to_f(wv[i].e[e]);
+          if (p.gate) {
+            const float zf = Elem<T>::to_f(zv[i].e[e]);
+            dn *= zf * sigmoid(zf);
+          }
+          s.x = fmaf(v, v, s.x);
+          s.y = fmaf(dn, v, s.y);
+        }
+    s = row_sum<TPR>(s, flip);
+    const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (!in || c >= p.D) continue;
+      V dx, dz;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float v = Elem<T>::to_f(xv[i].e[e]), d = p.scale * Elem<T>::to_f(dv[i].e[e]);
+        const float w = p.weight ? Elem<T>::to_f(wv[i].e[e]) : 1.f;
+        float silu = 1.f, slope = 0.f;
+        if (p.gate) {
+          const float zf = Elem<T>::to_f(zv[i].e[e]), sg = sigmoid(zf);
+          silu = zf * sg;
+          slope = sg * (1.f + zf * (1.f - sg));
+        }
+        dx.e[e] = Elem<T>::from_f(r * (d * w * silu - v * m));
+        const float dn = d * v * r;
+        if (p.gate) dz.e[e] = Elem<T>::from_f(dn * w * slope);
+        acc[i * VEC + e] = fmaf(dn, silu, acc[i * VEC + e]);
+      }
+      if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
+      if (p.dgate) *reinterpret_cast<V*>((T*)p.dgate + row * p.D + c) = dz;
+    }
+  }
+  if (p.part) store_sums<TPR, VEC, NV>(acc, p.part + (int64_t)blockIdx.x * p.D, p.D);
+}
+
+template <typename T, int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
+  using V = Vec<T, VEC>;
+  constexpr int kRows = cta(TPR) / TPR;
+  const int lane = threadIdx.x % TPR;
+  int flip = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < p.N; r0 += (int64_t)gridDim.x * kRows) {
+    const int64_t row = r0 + threadIdx.x / TPR;
+    const bool in = row < p.N;
+    V xv[NV], rv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (in && c < p.D) {
+        xv[i] = *reinterpret_cast<const V*>((const T*)p.x + row * p.D + c);
+        rv[i] = *reinterpret_cast<const V*>((const T*)p.residual + row * p.D + c);
+      }
+    }
+    float h[NV * VEC];  // unrounded: y is the norm of the sum itself
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (!in || c >= p.D) continue;
+      V sv{}, hv;
+      if (p.scale) sv = *reinterpret_cast<const V*>((const T*)p.scale + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float f = p.scale ? Elem<T>::to_f(sv.e[e]) : p.factor;
+        const float v = fmaf(f, Elem<T>::to_f(xv[i].e[e]), Elem<T>::to_f(rv[i].e[e]));
+        h[i * VEC + e] = v;
+        hv.e[e] = Elem<T>::from_f(v);
+        s.x = fmaf(v, v, s.x);
+      }
+      *reinterpret_cast<V*>((T*)p.h + row * p.D + c) = hv;
+    }
+    const float r = rsqrtf(row_sum<TPR>(s, flip).x / p.D + p.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (!in || c >= p.D) continue;
+      const V w = *reinterpret_cast<const V*>((const T*)p.weight + c);
+      V y;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y.e[e] = Elem<T>::from_f(h[i * VEC + e] * r * Elem<T>::to_f(w.e[e]));
+      *reinterpret_cast<V*>((T*)p.y + row * p.D + c) = y;
+    }
+  }
+}
+
+template <typename T, int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(cta(TPR)) residual_bwd_kernel(Residual p) {
+  using V = Vec<T, VEC>;
+  constexpr int kRows = cta(TPR) / TPR;
+  const int lane = threadIdx.x % TPR;
+  int flip = 0;
+  float acc_w[NV * VEC], acc_s[NV * VEC];
+#pragma unroll
+  for (int i = 0; i < NV * VEC; ++i) acc_w[i] = acc_s[i] = 0.f;
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < p.N; r0 += (int64_t)gridDim.x * kRows) {
+    const int64_t row = r0 + threadIdx.x / TPR;
+    const bool in = row < p.N;
+    V hv[NV], dv[NV], uv[NV], xv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (in && c < p.D) {
+        hv[i] = *reinterpret_cast<const V*>((const T*)p.h + row * p.D + c);
+        dv[i] = p.dy ? *reinterpret_cast<const V*>((const T*)p.dy + row * p.D + c) : V{};
+        uv[i] = p.dh ? *reinterpret_cast<const V*>((const T*)p.dh + row * p.D + c) : V{};
+        if (p.part_s) xv[i] = *reinterpret_cast<const V*>((const T*)p.x + row * p.D + c);
+      }
+    }
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (!in || c >= p.D) continue;
+      const V w = *reinterpret_cast<const V*>((const T*)p.weight + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float v = Elem<T>::to_f(hv[i].e[e]);
+        s.x = fmaf(v, v, s.x);
+        s.y = fmaf(Elem<T>::to_f(dv[i].e[e]) * Elem<T>::to_f(w.e[e]), v, s.y);
+      }
+    }
+    s = row_sum<TPR>(s, flip);
+    const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (!in || c >= p.D) continue;
+      const V w = *reinterpret_cast<const V*>((const T*)p.weight + c);
+      V sv{}, dt, dx;
+      if (p.scale) sv = *reinterpret_cast<const V*>((const T*)p.scale + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float v = Elem<T>::to_f(hv[i].e[e]), d = Elem<T>::to_f(dv[i].e[e]);
+        const float t = fmaf(r, fmaf(d, Elem<T>::to_f(w.e[e]), -v * m), Elem<T>::to_f(uv[i].e[e]));
+        dt.e[e] = Elem<T>::from_f(t);
+        dx.e[e] = Elem<T>::from_f(t * (p.scale ? Elem<T>::to_f(sv.e[e]) : p.factor));
+        acc_w[i * VEC + e] = fmaf(d, v * r, acc_w[i * VEC + e]);
+        if (p.part_s) acc_s[i * VEC + e] = fmaf(t, Elem<T>::to_f(xv[i].e[e]), acc_s[i * VEC + e]);
+      }
+      if (p.dresidual) *reinterpret_cast<V*>((T*)p.dresidual + row * p.D + c) = dt;
+      if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
+    }
+  }
+  if (p.part_w) store_sums<TPR, VEC, NV>(acc_w, p.part_w + (int64_t)blockIdx.x * p.D, p.D);
+  if (p.part_s) store_sums<TPR, VEC, NV>(acc_s, p.part_s + (int64_t)blockIdx.x * p.D, p.D);
+}
+
+// out[c] = sum over the CTAs' partial rows.  32 columns per CTA; 32 threads of a column take every
+// 32nd row and are added in order.  (One thread per column would read 600 rows one after another.)
+template <typename T>
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part_a, T* __restrict__ out_a,
+                                                          const float* __restrict__ part_b, T* __restrict__ out_b,
+                                                          int P, int D) {
+  __shared__ float sh[32][33];
+  const float* part = blockIdx.y ? part_b : part_a;
+  T* out = blockIdx.y ? out_b : out_a;
+  const int c = blockIdx.x * 32 + threadIdx.x % 32, r = threadIdx.x / 32;
+  float s = 0.f;
+  if (c < D)
+#pragma unroll 4
+    for (int i = r; i < P; i += 32) s += part[(int64_t)i * D + c];
+  sh[r][threadIdx.x % 32] = s;
+  __syncthreads();
+  if (r == 0 && c < D) {
+    s = sh[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) s += sh[i][threadIdx.x];
+    out[c] = Elem<T>::from_f(s);
+  }
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// CTAs of a launch: as many as run at once (2048 threads of an SM; backward half of that), no more than there is work for.
+int64_t grid_of(int64_t rows, int tpr, bool backward) {
+  const int64_t want = (rows * tpr + cta(tpr) - 1) / cta(tpr);
+  const int64_t most = (int64_t)sm_count() * (backward ? 1024 : 2048) / cta(tpr);
+  return want < most ? want : most;
+}
+
+// Threads of a row: the fewest that hold it at VEC x NV numbers each, where narrow rows take one
+// vector each (more rows in flight), up to a warp, and wide ones a CTA.
+template <typename T, int VEC, typename F>
+int pick(int64_t D, F&& go) {
+  constexpr int kNV = kPerThread / VEC;
+  constexpr int kOne = VEC > 1 ? 1 : 4;  // vectors per thread of a narrow row
+  if (D <= 8 * VEC * kOne) return go.template operator()<T, VEC, 8, kOne>();
+  if (D <= 16 * VEC * kOne) return go.template operator()<T, VEC, 16, kOne>();
+  if (D <= 32 * VEC * kOne) return go.template operator()<T, VEC, 32, kOne>();
+  if (D <= 32 * kPerThread) return go.template operator()<T, VEC, 32, kNV>();
+  if (D <= 256 * kPerThread / 2) return go.template operator()<T, VEC, 256, kNV / 2>();
+  if (D <= 256 * kPerThread) return go.template operator()<T, VEC, 256, kNV>();
+  if (D <= 512 * kPerThread) return go.template operator()<T, VEC, 512, kNV>();
+  return go.template operator()<T, VEC, 1024, kNV>();
+}
+
+struct GatedGo {
+  const Gated& p;
+  bool backward;
+  cudaStream_t st;
+  template <typename T, int VEC, int TPR, int NV>
+  int operator()() const {
+    Gated q = p;
+    const int64_t g = grid_of(q.N * q.G, TPR, backward);
+    if (!backward) {
+      gated_fwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+      DYNCONV_CHECK_LAUNCH("gated_fwd_kernel");
+      return DYNCONV_OK;
+    }
+    gated_bwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+    DYNCONV_CHECK_LAUNCH("gated_bwd_kernel");
+    if (q.part) {
+      column_sum_kernel<T><<<(unsigned)((q.D + 31) / 32), 1024, 0, st>>>(q.part, (T*)q.dweight, nullptr, nullptr, (int)g, q.D);
+      DYNCONV_CHECK_LAUNCH("column_sum_kernel");
+    }
+    return DYNCONV_OK;
+  }
+};
+
+struct ResidualGo {
+  const Residual& p;
+  bool backward;
+  cudaStream_t st;
+  template <typename T, int VEC, int TPR, int NV>
+  int operator()() const {
+    Residual q = p;
+    const int64_t g = grid_of(q.N, TPR, backward);
+    if (!backward) {
+      residual_fwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+      DYNCONV_CHECK_LAUNCH("residual_fwd_kernel");
+      return DYNCONV_OK;
+    }
+    residual_bwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+    DYNCONV_CHECK_LAUNCH("residual_bwd_kernel");
+    if (q.part_w || q.part_s) {
+      const float *a = q.part_w, *b = q.part_s;
+      T *oa = (T*)q.dweight, *ob = (T*)q.dscale;
+      if (!a) a = b, oa = ob;
+      const dim3 grid((unsigned)((q.D + 31) / 32), q.part_w && q.part_s ? 2 : 1);
+      column_sum_kernel<T><<<grid, 1024, 0, st>>>(a, oa, b, ob, (int)g, q.D);
+      DYNCONV_CHECK_LAUNCH("column_sum_kernel");
+    }
+    return DYNCONV_OK;
+  }
+};
+
+template <typename Go>
+int dispatch(int64_t D, int dtype, bool vectors, const Go& go) {
+  if (dtype == DYNCONV_DTYPE_BF16)
+    return vectors ? pick<__nv_bfloat16, 8>(D, go) : pick<__nv_bfloat16, 1>(D, go);
+  return vectors ? pick<float, 4>(D, go) : pick<float, 1>(D, go);
+}
+
+}  // namespace
+
+// Rows of partial sums that a backward may write.
+int64_t partial_rows() { return (int64_t)sm_count() * 4; }
+
+int gated_launch(const Gated& p, int dtype, bool backward, cudaStream_t st) {
+  const int per = dtype == DYNCONV_DTYPE_BF16 ? 8 : 4;
+  const bool strides = p.x_outer % per == 0 && p.x_inner % per == 0 && (!p.gate || (p.gate_outer % per == 0 && p.gate_inner % per == 0));
+  const bool vectors = p.D % per == 0 && strides && aligned(p.x) && aligned(p.weight) && aligned(p.gate) && aligned(p.y) &&
+                       aligned(p.dy) && aligned(p.dx) && aligned(p.dgate);
+  return dispatch(p.D, dtype, vectors, GatedGo{p, backward, st});
+}
+
+int residual_launch(const Residual& p, int dtype, bool backward, cudaStream_t st) {
+  const int per = dtype == DYNCONV_DTYPE_BF16 ? 8 : 4;
+  const bool vectors = p.D % per == 0 && aligned(p.x) && aligned(p.residual) && aligned(p.weight) && aligned(p.scale) &&
+                       aligned(p.y) && aligned(p.h) && aligned(p.dy) && aligned(p.dh) && aligned(p.dx) && aligned(p.dresidual);
+  return dispatch(p.D, dtype, vectors, ResidualGo{p, backward, st});
+}
+
+}  // namespace norm
+}  // namespace dynconv

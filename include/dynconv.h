@@ -303,6 +303,68 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
                     int64_t B, int64_t n_rows, int64_t H, int64_t dk, int64_t dv, float scale,
                     int dtype, void* stream);
 
+/* ------------------------------------------------------- the gated delta rule */
+
+/* A state that forgets by a factor of its own for each token and corrects what it holds for
+ * the token's key (no reference counterpart; it consumes the convolved queries, keys and values):
+ *     S_t = a_t S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - a_t S_{t-1}^T k_t),  o_t = scale S_t^T q_t,
+ *     a_t = exp(log_decay_t)
+ *   q, k [B,T,H,dk], v, o [B,T,H,dv], log_decay, beta [B,T,H] in `dtype`, dense in the last
+ *   dimension of four, any other strides: `strides` holds the element strides of batch, time and
+ *   head for q, k, v, log_decay, beta, o (18 numbers).  log_decay <= 0 (-inf forgets at once).
+ *   initial_state (NULL = zero), final_state (NULL = not wanted): [B,H,dk,dv] float32.
+ *   kept (NULL = no backward to come): dynconv_delta_kept_bytes bytes, 16-byte aligned, for
+ *   dynconv_delta_bwd: the states at every 64th token (float32 tensors: 32nd) and each token's
+ *   v_t - a_t S_{t-1}^T k_t.
+ * The workspace and kept are 16-byte aligned, and so are bf16 (float32) tensors whose width is a multiple of 8 (4),
+ * rows and all (DYNCONV_ERR_ALIGN); other widths are read through copies in the workspace.
+ * dk in 1..128, dv in 1..256, B*H <= 65535, T <= 2^30.  T = 0 copies the state.  A token that holds a
+ * number that is not finite makes its head's outputs from it on NaN, and none before it. */
+size_t dynconv_delta_kept_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype);
+size_t dynconv_delta_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype, int backward);
+int dynconv_delta_fwd(const void* q, const void* k, const void* v, const void* log_decay, const void* beta,
+                      const float* initial_state, void* o, float* final_state, void* kept, size_t kept_bytes,
+                      const int64_t* strides, void* workspace, size_t workspace_bytes, int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, float scale,
+                      int dtype, void* stream);
+/* Gradients for upstream d_o and d_final_state (NULL = zero).  `strides`: batch, time and head for
+ * q, k, log_decay, beta, d_o, dq, d_k, d_v, d_log_decay, d_beta (30 numbers).  d_initial_state may be
+ * NULL.  Alignment as above, for q, k and d_o. */
+int dynconv_delta_bwd(const void* q, const void* k, const void* log_decay, const void* beta, const void* kept,
+                      size_t kept_bytes, const void* d_o, const float* d_final_state, void* dq, void* d_k, void* d_v,
+                      void* d_log_decay, void* d_beta, float* d_initial_state, const int64_t* strides,
+                      void* workspace, size_t workspace_bytes,
+                      int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, float scale, int dtype, void* stream);
+/* One token for B sequences: q, k [B,H,dk], v [B,H,dv], log_decay, beta [B,H] (`strides`: batch and
+ * head of the five, 10 numbers), o [B,H,dv] dense, state [n_rows,H,dk,dv] float32 updated in place;
+ * slots as for dynconv_lr_step. */
+int dynconv_delta_step(const void* q, const void* k, const void* v, const void* log_decay, const void* beta,
+                       float* state, void* o, const void* slots, int slot_bytes, const int64_t* strides,
+                       int64_t B, int64_t n_rows, int64_t H, int64_t dk, int64_t dv, float scale, int dtype, void* stream);
+
+/* -------------------------------------------------------------------- norms */
+
+/* y = scale * x rsqrt(mean(x^2) + eps) * weight * silu(gate) over rows of D numbers, 1..16384 (no
+ * reference counterpart).  weight [D] and gate may be NULL (one).  Rows (n, g), n < N and g < G: x and gate
+ * at n * outer + g * inner (`strides`, in elements: outer and inner of x, then of gate), y dense. */
+size_t dynconv_norm_workspace_bytes(int64_t D);
+int dynconv_gated_norm_fwd(const void* x, const void* weight, const void* gate, void* y, const int64_t* strides,
+                           int64_t N, int64_t G, int64_t D, float eps, float scale, int dtype, void* stream);
+/* Gradients for dy [N,G,D], dense; dx, dgate [N,G,D] dense and dweight [D] may be NULL (not wanted).  The
+ * workspace (dynconv_norm_workspace_bytes, 16-byte aligned) is for dweight. */
+int dynconv_gated_norm_bwd(const void* x, const void* weight, const void* gate, const void* dy, void* dx,
+                           void* dweight, void* dgate, const int64_t* strides, void* workspace, size_t workspace_bytes,
+                           int64_t N, int64_t G, int64_t D, float eps, float scale, int dtype, void* stream);
+/* h = residual + s x and y = h rsqrt(mean(h^2) + eps) * weight (of the unrounded h) for dense rows
+ * x, residual, y, h [N,D]; s is scale [D], or `factor` where scale is NULL. */
+int dynconv_residual_norm_fwd(const void* x, const void* residual, const void* weight, const void* scale, float factor,
+                              void* y, void* h, int64_t N, int64_t D, float eps, int dtype, void* stream);
+/* Gradients for dy and dh (NULL = zero) from h; x is read for dscale alone.  dx, dresidual [N,D], dweight
+ * and dscale [D] may be NULL.  Workspace: dynconv_norm_workspace_bytes for each of dweight and dscale. */
+int dynconv_residual_norm_bwd(const void* h, const void* x, const void* weight, const void* scale, float factor,
+                              const void* dy, const void* dh, void* dx, void* dresidual, void* dweight, void* dscale,
+                              void* workspace, size_t workspace_bytes, int64_t N, int64_t D, float eps, int dtype,
+                              void* stream);
+
 /* ------------------------------------------------------------ vocabulary loss */
 
 /* Softmax cross entropy of hidden [N,D] against weight [V,D] (logits = hidden weight^T),
