@@ -3,8 +3,9 @@
 // A CTA walks the chunks of one (batch row, head) for `teams` slices of 16 of v's columns.  A team of W warps holds
 // a slice of the state, transposed: warp w keeps 16 x (128 / W) of it in registers, fp32, in the accumulators' layout,
 // and works out 16 x (C / W) of what belongs to tokens.  What the others need of a warp's numbers
-// goes through shared memory as bf16 parts in the layout of first operands, 16 bytes per lane.  One more
-// warp brings the next chunks' tiles by TMA into two or three stages.  (16-byte asynchronous copies by threads, of
+// goes through shared memory as bf16 parts in the layout of first operands, 16 bytes per lane.  One thread,
+// of a warp of its own or, where the chains' warps take all registers, of the first team, brings the next chunks' tiles
+// by TMA into two or three stages.  (16-byte asynchronous copies by threads, of
 // one warp or four, took longer than a chunk's products: 10 to 20 bytes per cycle and SM.)
 //
 // Why teams: one warp per slice, its numbers all in registers, took 7400 cycles for a chunk of 64 tokens
@@ -20,20 +21,24 @@ namespace dr {
 struct Plan {
   int teams, stages;
   int o_vectors;
+  int own_warp;  // the producer has one
 };
 
-template <typename G, int W>
+// KK: pieces of 16 of dk that are worked on, 4 or 8 (behind dk there are zeros).
+template <typename G, int W, int KK_>
 struct Chain {
   static constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks;
   static constexpr int TB = NB / W;          // token blocks of a warp
-  static constexpr int NT = 16 / W;          // its 8-column tiles of the state
+  static constexpr int KK = KK_, NT = 2 * KK / W;  // a warp's 8-column tiles of the state
   static constexpr int PU = PX == 1 ? 2 : 3;  // parts of what the backward is given
   using E = typename G::T;
+  static constexpr int kMostTeams = NP == 2 ? 4 : 2;  // (three parts: the registers of 8 warps, and shared memory)
+  static constexpr int kMostThreads = 32 * W * kMostTeams;
 
   static constexpr int kKq = PX * G::kTile * 2;  // bytes
   static constexpr int kV = C * 16 * (int)sizeof(E);  // of a team: [C tokens][16 columns]
   static constexpr int kT = G::kLower * NP * 512, kP = G::kLower * PP * 512, kGates = sizeof(Gates<C>);
-  static constexpr int kState = 8 * NP * 512, kBlock = NB * NP * 512;  // a team's buffers
+  static constexpr int kState = KK * NP * 512, kBlock = NB * NP * 512;  // a team's buffers
   static constexpr int kTeam = kState + 3 * kBlock;
   static __host__ __device__ constexpr int stage_bytes(int teams) {
     return (2 * kKq + teams * kV + kT + kP + kGates + 1023) / 1024 * 1024;
@@ -82,20 +87,25 @@ struct Chain {
     __syncthreads();
   }
 
-  // The producer's walk, one thread of it (BACK: from the last chunk to the first).
-  template <bool BACK>
-  static __device__ __forceinline__ void produce(uint8_t* smem, Bars& bars, const Plan& plan, const Maps& maps, const Prepared& pre, int b,
-                                                 int h, int64_t bh, int chunks, int dk, int dv, int first_col) {
-    const int bytes = stage_bytes(plan.teams), halves = dk > 64 ? 2 : 1, live = live_teams(plan, dv, first_col), slices = (dv + 15) / 16;
-    const uint32_t half = C * 128, all = 2 * PX * halves * half + live * kV + kT + kP + kGates;
-    int n = 0, s = 0, round = 0;
-    for (; n < chunks; ++n) {
-      if (round > 0 && !mbar_wait(&bars.empty[s], (round - 1) & 1, kErrWaitProducer, &bars.abort_flag)) break;
-      const Stage st{smem + s * bytes, plan.teams};
+  // One thread asks for the tiles of the n-th chunk in the order of the walk (BACK: from the last chunk to the first).
+  struct Producer {
+    uint8_t* smem;
+    Bars& bars;
+    const Plan& plan;
+    const Maps& maps;
+    const Prepared& pre;
+    int b, h, chunks, dk, dv, first_col;
+    int64_t bh;
+
+    template <bool BACK>
+    __device__ __forceinline__ void load(int n, int stage) const {
+      const int halves = dk > 64 ? 2 : 1, live = live_teams(plan, dv, first_col), slices = (dv + 15) / 16;
+      const uint32_t half = C * 128, all = 2 * PX * halves * half + live * kV + kT + kP + kGates;
+      const Stage st{smem + stage * stage_bytes(plan.teams), plan.teams};
       uint8_t *const k = st.at, *const q = st.at + kKq;
       const int c = BACK ? chunks - 1 - n : n;
       const int64_t at = bh * chunks + c;
-      uint64_t* const bar = &bars.full[s];
+      uint64_t* const bar = &bars.full[stage];
       mbar_arrive_expect_tx(bar, all);
       if (pre.k) {
         for (int i = 0; i < PX; ++i) {
@@ -118,11 +128,33 @@ struct Chain {
       bulk_load(st.t(), pre.t + at * (kT / 16), kT, bar);
       bulk_load(st.p(), pre.p + at * (kP / 16), kP, bar);
       bulk_load(&st.gates(), (const uint8_t*)pre.gates + at * kGates, kGates, bar);
-      if (++s == plan.stages) s = 0, ++round;
     }
-    if (n < chunks)  // gave up: what is in flight lands before the shared memory goes
-      for (int i = max(0, n - plan.stages); i < n; ++i) mbar_drain(&bars.full[i % plan.stages], (i / plan.stages) & 1);
-  }
+    template <bool BACK>
+    __device__ __forceinline__ void start() const {
+      for (int n = 0; n < plan.stages && n < chunks; ++n) load<BACK>(n, n);
+    }
+    // In the n-th chunk, n > 0: refills the stage of the chunk before it, once all warps are done with it.
+    template <bool BACK>
+    __device__ __forceinline__ void refill(int n) const {
+      const int next = n - 1 + plan.stages, stage = (n - 1) % plan.stages, round = (n - 1) / plan.stages;
+      if (next < chunks && mbar_wait(&bars.empty[stage], round & 1, kErrWaitProducer, &bars.abort_flag)) load<BACK>(next, stage);
+    }
+    // The walk of a producer with a warp of its own.
+    template <bool BACK>
+    __device__ __forceinline__ void walk() const {
+      int n = 0;
+      for (; n < chunks; ++n) {
+        const int stage = n % plan.stages, round = n / plan.stages;
+        if (round > 0 && !mbar_wait(&bars.empty[stage], (round - 1) & 1, kErrWaitProducer, &bars.abort_flag)) break;
+        load<BACK>(n, stage);
+      }
+      if (n < chunks) drain(max(0, n - plan.stages), n);
+    }
+    // The wait for chunk n gave up: what is in flight lands before the shared memory goes.
+    __device__ __forceinline__ void drain(int n, int end) const {
+      for (int i = n; i < end && i < chunks; ++i) mbar_drain(&bars.full[i % plan.stages], (i / plan.stages) & 1);
+    }
+  };
 
   // The first row (last: one more than the last) of a [C] x [16] tile that holds a number that is not finite; C (0)
   // where there is none.  One warp.
@@ -164,17 +196,17 @@ int chain_maps(Maps* maps, const Prepared& pre, const View& k, const View& q, co
 }
 
 // CTAs of as few teams as let all slices run at once, each then having more of its SM's matrix units and shared
-// memory; four warps for a team then, and two where the SMs are full anyway: the shared operands are
-// read half as often.
-template <typename G, int W>
+// memory.
+template <typename Ch>
 Plan plan_of(int64_t bh, int dv) {
-  using Ch = Chain<G, W>;
   constexpr int kMost = 227 * 1024 - 1024;  // (barriers)
   const int slices = (dv + 15) / 16;
   Plan p{};
   p.teams = 1;
-  while (p.teams < 4 && Ch::smem_bytes(2 * p.teams, 2) <= kMost && bh * ((slices + p.teams - 1) / p.teams) > sm_count()) p.teams *= 2;
+  while (2 * p.teams <= Ch::kMostTeams && Ch::smem_bytes(2 * p.teams, 2) <= kMost && bh * ((slices + p.teams - 1) / p.teams) > sm_count())
+    p.teams *= 2;
   p.stages = Ch::smem_bytes(p.teams, 3) <= kMost ? 3 : 2;
+  p.own_warp = p.teams < Ch::kMostTeams;
   return p;
 }
 

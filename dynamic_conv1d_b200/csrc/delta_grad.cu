@@ -3,7 +3,7 @@
 //
 // A CTA of eight warps takes one (batch row, head, chunk) after another.  v's columns come in slabs, the next one by TMA
 // while this one is worked on.  A warp has 16 tokens and, of dk, a half (a quarter with chunks of 32): it sums
-// dO S0^T, r dS1^T and dU S0^T over the slabs, and the first warps of each 16 tokens the triangles dO r^T and dU r^T.
+// dO S0^T, r dS1^T and dU S0^T over the slabs, and some blocks of the triangles dO r^T and dU r^T.
 // These become W and N, which go through shared memory into the products with K and Q; their products with
 // Q K^T and K K^T, entry by entry, are what the log decays' gradients are sums of.  Row sums and column sums
 // of the same numbers are taken, so what has to cancel does.
@@ -13,33 +13,35 @@ namespace dynconv {
 namespace dr {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 
-template <int PX_, int C_>
+// KK: 16-column pieces of dk, 4 or 8 (columns behind dk are zeros in the tiles of K and Q, and read as zeros from states)
+template <int PX_, int C_, int KK_>
 struct Grad {
-  static constexpr int PX = PX_, C = C_, NB = C / 16, kGroups = 8 / NB, kCols = kMaxKey / kGroups;  // a warp's columns of dk
+  static constexpr int PX = PX_, C = C_, NB = C / 16, kGroups = kWarps / NB, KK = KK_, NT = 2 * KK / kGroups;  // a warp's 8-column tiles of dk
+  // a group of warps has every kGroups / 2-th block column of one of the triangles
+  static constexpr int kStep = kGroups / 2, kBlocks = NB > kStep ? NB / kStep : 1;
   static constexpr int PU = PX == 1 ? 2 : 3, PS = PX == 1 ? 1 : 3;  // parts of r and dU, of the states
   static constexpr int kSlab = PX == 1 ? 4 : 2;                     // slices of 16 columns of v
   static constexpr int kTile = C * kMaxKey, kSquare = C + 8;
   using E = typename std::conditional<PX_ == 1, __nv_bfloat16, float>::type;
   static constexpr int kDo = C * 16 * (int)sizeof(E), kU = NB * 512;  // bytes of a slice: of dO, of one part of r or dU
-  static constexpr int kS = 8 * 512;                                  // of one part of a state, at most
+  static constexpr int kS = KK * 512;                                 // of one part of a state, at most
   static constexpr int kSlabBytes = kSlab * (kDo + 2 * PU * kU + 2 * PS * kS);
   static constexpr int kKq = 2 * PX * kTile * 2, kWn = 2 * PX * C * kSquare * 2;
   static constexpr int kBytes = 1024 + 2 * kSlabBytes + kKq + kWn;
-  struct Slab {
-    uint8_t* at;
-    __device__ __forceinline__ E* d_o(int slice) const { return (E*)(at + slice * kDo); }
-    __device__ __forceinline__ uint8_t* r(int part, int slice) const { return at + kSlab * kDo + (part * kSlab + slice) * kU; }
-    __device__ __forceinline__ uint8_t* du(int part, int slice) const { return r(PU, 0) + (part * kSlab + slice) * kU; }
-    __device__ __forceinline__ uint8_t* s0(int part, int slice) const { return r(2 * PU, 0) + (part * kSlab + slice) * kS; }
-    __device__ __forceinline__ uint8_t* ds(int part, int slice) const { return s0(PS, 0) + (part * kSlab + slice) * kS; }
-  };
+  // where a slab's parts begin, the parts of each kSlab slices apart
+  static constexpr uint32_t kR = kSlab * kDo, kDu = kR + PU * kSlab * kU, kS0 = kDu + PU * kSlab * kU, kDs = kS0 + PS * kSlab * kS;
 };
 
-// A 16 x 16 block kept as four matrices of 128 bytes, transposed: as second operand {0,1},{2,3}; as first {0,2,1,3}.
-__device__ __forceinline__ void turned(uint32_t (&f)[4], const uint8_t* block) { ldsm_t(f, smem_u32(block) + (threadIdx.x & 31) * 16); }
-__device__ __forceinline__ void first(uint32_t (&a)[4], const uint32_t (&f)[4]) { a[0] = f[0], a[1] = f[2], a[2] = f[1], a[3] = f[3]; }
+// A 16 x 16 block kept as four matrices of 128 bytes is read transposed, as second operand, or as first, whose
+// middle two matrices are the other way about.
+// So are a lane's offsets in it.
+__device__ __forceinline__ uint32_t second_lane() { return (threadIdx.x & 31) * 16; }
+__device__ __forceinline__ uint32_t first_lane() {
+  const int l = threadIdx.x & 31;
+  return ((l >> 4 & 1) + (l >> 2 & 2)) * 128 + (l & 7) * 16;
+}
 
 template <typename E>
 __device__ __forceinline__ void store2(E* to, float x, float y, int n, bool pairs) {
@@ -54,50 +56,57 @@ __device__ __forceinline__ void store2(E* to, float x, float y, int n, bool pair
 template <typename R>
 __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, const __grid_constant__ Maps maps, int64_t items, int pairs) {
   constexpr int PX = R::PX, C = R::C, NB = R::NB, PU = R::PU, PS = R::PS, kSlab = R::kSlab, kSquare = R::kSquare;
-  constexpr int NT = R::kCols / 8, KX = PX > PS ? PX : PS, KS = PU > PS ? PU : PS;
+  constexpr int NT = R::NT, KK = R::KK, KX = PX > PS ? PX : PS, KS = PU > PS ? PU : PS;
   using E = typename R::E;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t slab_full[2], kq_full;
   __shared__ int abort_flag;
   __shared__ Gates<C> gate;
-  __shared__ float row_sum[2][C], col_sum[2][NB][C], from_state[R::kGroups][C], to_state[R::kGroups][C], inner[8];
+  __shared__ float row_sum[R::kGroups][C], col_sum[2][NB][C], from_state[R::kGroups][C], to_state[R::kGroups][C], inner[kWarps];
   uint8_t* const smem = align_smem_1024(smem_raw);
   uint8_t *const k_tile = smem, *const q_tile = smem + R::kKq / 2, *const slabs = smem + R::kKq;
   __nv_bfloat16 *const W = (__nv_bfloat16*)(slabs + 2 * R::kSlabBytes), *const N = W + PX * C * kSquare;
   const int tid = threadIdx.x, l = tid & 31, warp = warp_index(), row = l >> 2, col = 2 * (l & 3);
   const int group = warp / NB, rb = group & 1 ? NB - 1 - warp % NB : warp % NB;  // (the triangle's long rows on different schedulers)
   const int chunks = (int)((p.T + C - 1) / C), n_k16 = (p.dk + 15) / 16, slices = (p.dv + 15) / 16, n_slabs = (slices + kSlab - 1) / kSlab;
-  const int halves = p.dk > 64 ? 2 : 1;
+  constexpr int halves = KK / 4;
   const int64_t all = (int64_t)p.B * p.H * chunks;
   if (tid == 0) {
     mbar_init(&slab_full[0], 1), mbar_init(&slab_full[1], 1), mbar_init(&kq_full, 1);
     abort_flag = 0;
     fence_barrier_init();
   }
+  if (n_k16 < KK) {  // pieces of the states that no load writes
+    for (int i = tid; i < 2 * R::kSlabBytes / 16; i += kThreads) ((uint4*)slabs)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+  }
   __syncthreads();
   // (one thread)
   auto load_slab = [&](int64_t item, int slab, int at) {
     const int64_t bh = item / chunks;
     const int c = (int)(item % chunks), first = slab * kSlab, n = min(kSlab, slices - first);
-    const typename R::Slab s{slabs + at * R::kSlabBytes};
+    uint8_t* const s = slabs + at * R::kSlabBytes;
     uint64_t* const bar = &slab_full[at];
     const uint32_t state = n * n_k16 * 512;
     mbar_arrive_expect_tx(bar, n * (R::kDo + 2 * PU * R::kU) + 2 * PS * state);
     for (int i = 0; i < n; ++i) {
       if (p.pre.v)
-        bulk_load(s.d_o(i), (const E*)p.pre.v + (item * slices + first + i) * (C * 16), R::kDo, bar);
+        bulk_load(s + i * R::kDo, (const E*)p.pre.v + (item * slices + first + i) * (C * 16), R::kDo, bar);
       else
-        tma_load_4d(s.d_o(i), &maps.v, bar, (first + i) * 16 * (int)(sizeof(E) / 2), (int)(bh % p.H), c * C, (int)(bh / p.H), policy_evict_normal());
+        tma_load_4d(s + i * R::kDo, &maps.v, bar, (first + i) * 16 * (int)(sizeof(E) / 2), (int)(bh % p.H), c * C, (int)(bh / p.H), policy_evict_normal());
     }
     for (int i = 0; i < PU; ++i) {
       const int64_t from = ((i * all + item) * slices + first) * (R::kU / 2);
-      bulk_load(s.r(i, 0), p.rest + from, n * R::kU, bar);
-      bulk_load(s.du(i, 0), p.du + from, n * R::kU, bar);
+      bulk_load(s + R::kR + i * kSlab * R::kU, p.rest + from, n * R::kU, bar);
+      bulk_load(s + R::kDu + i * kSlab * R::kU, p.du + from, n * R::kU, bar);
     }
     for (int i = 0; i < PS; ++i) {
       const int64_t from = ((i * all + item) * slices + first) * n_k16 * 256;
-      bulk_load(s.s0(i, 0), p.states + from, state, bar);
-      bulk_load(s.ds(i, 0), p.dstates + from, state, bar);
+      for (int v = 0; v < (n_k16 == KK ? 1 : n); ++v) {  // (slices lie KK pieces apart)
+        const uint32_t one = n_k16 == KK ? state : n_k16 * 512;
+        bulk_load(s + R::kS0 + (i * kSlab + v) * R::kS, p.states + from + v * n_k16 * 256, one, bar);
+        bulk_load(s + R::kDs + (i * kSlab + v) * R::kS, p.dstates + from + v * n_k16 * 256, one, bar);
+      }
     }
   };
   auto load_kq = [&](int64_t item) {
@@ -120,6 +129,12 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
   const KeyLane key_across(false), key_down(true);
   const int s_down = lane_offset(kSquare, true), s_across = lane_offset(kSquare, false), o_down = lane_offset(16, true);
   const int kk0 = group * NT / 2;  // its first 16 columns of dk
+  uint32_t own_down[NT / 2];
+#pragma unroll
+  for (int m = 0; m < NT / 2; ++m) {
+    const int kk = kk0 + m;
+    own_down[m] = key_swizzle((l & 7) + 8 * (l >> 3 & 1), (2 * kk & 7) + (l >> 4)) + (kk >> 2) * (C * 128);
+  }
 
   int64_t item = blockIdx.x;
   if (item >= items) return;
@@ -130,13 +145,18 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
     const int c = (int)(item % chunks);
     const int64_t t0 = (int64_t)c * C;
     const int rows = (int)(p.T - t0 < C ? p.T - t0 : C);
+    E* const dv_at = (E*)p.dv_.p + b * p.dv_.sb + h * p.dv_.sh + t0 * p.dv_.st;
+    float beta_own[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) beta_own[i] = ((const Gates<C>*)p.pre.gates)[item].beta[16 * rb + row + 8 * i];
     float dq[NT][4], kr[NT][4], ku[NT][4];  // dO S0^T, r dS1^T, dU S0^T
-    float X[NB][2][4];                      // groups 0 and 1: dO r^T, dU r^T, blocks j <= rb
-    float dot = 0.f;
+    float X[R::kBlocks][2][4];              // blocks of dO r^T (even groups) or dU r^T
+    float dot[2][4];                        // its diagonals add up to <dS1, S0>
 #pragma unroll
     for (int n = 0; n < NT; ++n) zero(dq[n]), zero(kr[n]), zero(ku[n]);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) zero(X[j][0]), zero(X[j][1]);
+    for (int j = 0; j < R::kBlocks; ++j) zero(X[j][0]), zero(X[j][1]);
+    zero(dot[0]), zero(dot[1]);
     for (int slab = 0; slab < n_slabs; ++slab, ++n_loaded) {
       const int at = n_loaded & 1;
       if (!__syncthreads_and(mbar_wait(&slab_full[at], (n_loaded >> 1) & 1, kErrWaitMma, &abort_flag))) {
@@ -157,83 +177,94 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
         const uint4* g = (const uint4*)p.pre.gates + item * (sizeof(Gates<C>) / 16);
         for (int i = tid; i < (int)sizeof(Gates<C>) / 16; i += kThreads) ((uint4*)&gate)[i] = g[i];
       }
-      const typename R::Slab s{slabs + at * R::kSlabBytes};
       const int n = min(kSlab, slices - slab * kSlab);
-      for (int v = 0; v < n; ++v) {
-        uint32_t dO[PX][4], r[PU][4], u[PU][4];
+      const uint32_t base = smem_u32(slabs) + at * R::kSlabBytes;
+      uint32_t a_do = base + 2 * (16 * rb * 16 + o_down), a_r = base + R::kR + rb * 512 + first_lane(), b_r = base + R::kR + (group >> 1) * 512 + second_lane();
+      uint32_t b_s = base + R::kS0 + kk0 * 512 + second_lane();
+#pragma unroll 1
+      for (int v = 0; v < n; ++v, a_do += R::kDo, a_r += R::kU, b_r += R::kU, b_s += R::kS) {
+        uint32_t dO[PX][4], r[PU][4], u[PU][4], f[NT / 2][PS][4], x[R::kBlocks][PU][4];
         if constexpr (PX == 1) {
-          ldsm(dO[0], smem_u32(s.d_o(v) + 16 * rb * 16 + o_down));
+          ldsm(dO[0], a_do);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 f = *reinterpret_cast<const float2*>(s.d_o(v) + (16 * rb + row + 8 * (e & 1)) * 16 + 8 * (e >> 1) + col);
+            const float2 t = *reinterpret_cast<const float2*>(slabs + at * R::kSlabBytes + v * R::kDo + 4 * ((16 * rb + row + 8 * (e & 1)) * 16 + 8 * (e >> 1) + col));
             uint32_t part[PX];
-            split<PX>(f.x, f.y, part);
+            split<PX>(t.x, t.y, part);
 #pragma unroll
             for (int i = 0; i < PX; ++i) dO[i][e] = part[i];
           }
         }
 #pragma unroll
-        for (int i = 0; i < PU; ++i) {
-          uint32_t f[4];
-          turned(f, s.r(i, v) + rb * 512);
-          first(r[i], f);
-          turned(f, s.du(i, v) + rb * 512);
-          first(u[i], f);
-        }
+        for (int i = 0; i < PU; ++i) ldsm_t(u[i], a_r + R::kDu - R::kR + i * kSlab * R::kU);
 #pragma unroll
-        for (int m = 0; m < NT / 2; ++m) {
-          if (kk0 + m >= n_k16) continue;
-          uint32_t f[PS][4], g[PS][4];
+        for (int m = 0; m < NT / 2; ++m)
 #pragma unroll
-          for (int i = 0; i < PS; ++i) {
-            turned(f[i], s.s0(i, 0) + (v * n_k16 + kk0 + m) * 512);
-            turned(g[i], s.ds(i, 0) + (v * n_k16 + kk0 + m) * 512);
-          }
-          mma_parts<PX, PS, KX>(dq[2 * m], dq[2 * m + 1], dO, f);
-          mma_parts<PU, PS, KS>(ku[2 * m], ku[2 * m + 1], u, f);
-          mma_parts<PU, PS, KS>(kr[2 * m], kr[2 * m + 1], r, g);
-          // <dS1, S0>, each pair of matrices by one of the warps that read it
-          if ((v + m) % NB == rb) {
+          for (int i = 0; i < PS; ++i) ldsm_t(f[m][i], b_s + m * 512 + i * kSlab * R::kS);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float x = 0.f, y = 0.f, x1 = 0.f, y1 = 0.f;
+        for (int i = 0; i < PU; ++i) ldsm_t(r[i], a_r + i * kSlab * R::kU);
 #pragma unroll
-              for (int i = PS - 1; i >= 0; --i) x += low(f[i][e]), x1 += high(f[i][e]), y += low(g[i][e]), y1 += high(g[i][e]);
-              dot = fmaf(x, y, fmaf(x1, y1, dot));
-            }
-          }
-        }
-        if (group < 2) {
+        for (int m = 0; m < NT / 2; ++m) mma_parts<PX, PS, KX>(dq[2 * m], dq[2 * m + 1], dO, f[m]);
+        // (all tiles' products of one pair of parts, then of the next: none waits for the one before)
 #pragma unroll
-          for (int j = 0; j < NB; ++j) {
-            if (j > rb) continue;
-            uint32_t f[PU][4];
+        for (int t = KS - 1; t >= 0; --t)
 #pragma unroll
-            for (int i = 0; i < PU; ++i) turned(f[i], s.r(i, v) + j * 512);
-            if (group == 0)
-              mma_parts<PX, PU, PU>(X[j][0], X[j][1], dO, f);
-            else
-              mma_parts<PU, PU, PU>(X[j][0], X[j][1], u, f);
+          for (int i = 0; i < PU; ++i)
+#pragma unroll
+            for (int m = 0; m < NT / 2; ++m)
+              if (t - i >= 0 && t - i < PS) {
+                mma(ku[2 * m], u[i], f[m][t - i][0], f[m][t - i][1]);
+                mma(ku[2 * m + 1], u[i], f[m][t - i][2], f[m][t - i][3]);
+              }
+        uint32_t g[NT / 2][PS][4];
+#pragma unroll
+        for (int m = 0; m < NT / 2; ++m)
+#pragma unroll
+          for (int i = 0; i < PS; ++i) ldsm_t(g[m][i], b_s + R::kDs - R::kS0 + m * 512 + i * kSlab * R::kS);
+#pragma unroll
+        for (int c = 0; c < R::kBlocks; ++c)
+          if ((group >> 1) + c * R::kStep <= rb)
+#pragma unroll
+            for (int i = 0; i < PU; ++i) ldsm_t(x[c][i], b_r + c * R::kStep * 512 + i * kSlab * R::kU);
+        // <dS1, S0>: the trace of a product; each piece by one of the warps that read it
+        if ((v & (NB - 1)) == rb) {
+#pragma unroll
+          for (int m = 0; m < NT / 2; ++m) {
+            uint32_t t[PS][4];
+#pragma unroll
+            for (int i = 0; i < PS; ++i) t[i][0] = f[m][i][0], t[i][1] = f[m][i][2], t[i][2] = f[m][i][1], t[i][3] = f[m][i][3];
+            mma_parts<PS, PS, PS>(dot[0], dot[1], t, g[m]);
           }
         }
-        if (group == (R::kGroups == 2 ? 0 : 2) + (v & 1)) {
+#pragma unroll
+        for (int t = KS - 1; t >= 0; --t)
+#pragma unroll
+          for (int i = 0; i < PU; ++i)
+#pragma unroll
+            for (int m = 0; m < NT / 2; ++m)
+              if (t - i >= 0 && t - i < PS) {
+                mma(kr[2 * m], r[i], g[m][t - i][0], g[m][t - i][1]);
+                mma(kr[2 * m + 1], r[i], g[m][t - i][2], g[m][t - i][3]);
+              }
+#pragma unroll
+        for (int c = 0; c < R::kBlocks; ++c) {
+          if ((group >> 1) + c * R::kStep > rb) continue;
+          if (group & 1)
+            mma_parts<PU, PU, PU>(X[c][0], X[c][1], u, x[c]);
+          else
+            mma_parts<PX, PU, PU>(X[c][0], X[c][1], dO, x[c]);
+        }
+        if (group == (v & (R::kGroups - 1))) {
           // dV = beta dU
-          float x[4][2];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e][0] = x[e][1] = 0.f;
-#pragma unroll
-            for (int i = PU - 1; i >= 0; --i) x[e][0] += low(u[i][e]), x[e][1] += high(u[i][e]);
-          }
-          const float* beta = ((const Gates<C>*)p.pre.gates)[item].beta;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int t = 16 * rb + row + 8 * (e & 1), d = (slab * kSlab + v) * 16 + 8 * (e >> 1) + col;
-            if (t < rows) {
-              const float f = beta[t];
-              store2((E*)p.dv_.p + b * p.dv_.sb + h * p.dv_.sh + (t0 + t) * p.dv_.st + d, x[e][0] * f, x[e][1] * f, p.dv - d, pairs & 1);
-            }
+            float x0 = low(u[PU - 1][e]), x1 = high(u[PU - 1][e]);
+#pragma unroll
+            for (int i = PU - 2; i >= 0; --i) x0 += low(u[i][e]), x1 += high(u[i][e]);
+            const float beta = e & 1 ? beta_own[1] : beta_own[0];
+            if (t < rows) store2(dv_at + (int64_t)t * p.dv_.st + d, x0 * beta, x1 * beta, p.dv - d, pairs & 1);
           }
         }
       }
@@ -244,30 +275,32 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       return;
     }
     const uint32_t k_at = smem_u32(k_tile), q_at = smem_u32(q_tile);
-    if (group < 2) {
-      float Y[NB][2][4];
+    {
+      const bool is_n = group & 1;
+      float Y[R::kBlocks][2][4];
 #pragma unroll
-      for (int j = 0; j < NB; ++j) zero(Y[j][0]), zero(Y[j][1]);
-      const uint32_t a_at = group == 0 ? q_at : k_at;
+      for (int n = 0; n < R::kBlocks; ++n) zero(Y[n][0]), zero(Y[n][1]);
+      const uint32_t a_at = is_n ? k_at : q_at;
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        if (kk >= n_k16) continue;
+      for (int kk = 0; kk < KK; ++kk) {
         uint32_t a[PX][4];
 #pragma unroll
         for (int i = 0; i < PX; ++i) ldsm(a[i], a_at + 2 * i * R::kTile + key_down.at<C>(rb, kk));
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
+        for (int n = 0; n < R::kBlocks; ++n) {
+          const int j = (group >> 1) + n * R::kStep;
           if (j > rb) continue;
           uint32_t f[PX][4];
 #pragma unroll
           for (int i = 0; i < PX; ++i) ldsm(f[i], k_at + 2 * i * R::kTile + key_across.at<C>(j, kk));
-          mma_parts<PX, PX, PX>(Y[j][0], Y[j][1], a, f);
+          mma_parts<PX, PX, PX>(Y[n][0], Y[n][1], a, f);
         }
       }
-      __nv_bfloat16* const out = group == 0 ? W : N;
+      __nv_bfloat16* const out = is_n ? N : W;
       float sums[2] = {0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
+      for (int jn = 0; jn < R::kBlocks; ++jn) {
+        const int j = (group >> 1) + jn * R::kStep;
         if (j > rb) continue;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -278,20 +311,20 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int r = 16 * rb + row + 8 * half;
-            const float f = group == 0 ? p.scale : -gate.beta[r];
-            float x = X[j][n][2 * half], y = X[j][n][2 * half + 1];
-            if (group == 1 && (cc == r || cc + 1 == r) && r < rows)
+            const float f = is_n ? -gate.beta[r] : p.scale;
+            float x = X[jn][n][2 * half], y = X[jn][n][2 * half + 1];
+            if (is_n && (cc == r || cc + 1 == r) && r < rows)
               ((E*)p.dbeta.p)[b * p.dbeta.sb + h * p.dbeta.sh + (t0 + r) * p.dbeta.st] = Elem<E>::from_f(cc == r ? x : y);
             x *= f * beta.x * exp2_fast((gate.hi[r] - hi.x) + (gate.lo[r] - lo.x));
             y *= f * beta.y * exp2_fast((gate.hi[r] - hi.y) + (gate.lo[r] - lo.y));
-            const int last = group == 0 ? r : r - 1;
+            const int last = is_n ? r - 1 : r;
             x = cc <= last ? x : 0.f, y = cc < last ? y : 0.f;
             uint32_t part[PX];
             split<PX>(x, y, part);
 #pragma unroll
             for (int i = 0; i < PX; ++i) *reinterpret_cast<uint32_t*>(out + i * C * kSquare + r * kSquare + cc) = part[i];
             // (a token's own term does not depend on the decays)
-            const float mx = cc < r ? x * Y[j][n][2 * half] : 0.f, my = cc + 1 < r ? y * Y[j][n][2 * half + 1] : 0.f;
+            const float mx = cc < r ? x * Y[jn][n][2 * half] : 0.f, my = cc + 1 < r ? y * Y[jn][n][2 * half + 1] : 0.f;
             sums[half] += mx + my;
             below[0] += mx, below[1] += my;
           }
@@ -300,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
             below[0] += __shfl_xor_sync(0xffffffffu, below[0], d);
             below[1] += __shfl_xor_sync(0xffffffffu, below[1], d);
           }
-          if (row == 0) col_sum[group][rb][cc] = below[0], col_sum[group][rb][cc + 1] = below[1];
+          if (row == 0) col_sum[is_n][rb][cc] = below[0], col_sum[is_n][rb][cc + 1] = below[1];
         }
       }
 #pragma unroll
@@ -310,9 +343,17 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
         if ((l & 3) == 0) row_sum[group][16 * rb + row + 8 * half] = sums[half];
       }
     }
+    {
+      float x = 0.f;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    if (l == 0) inner[warp] = dot;
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (row + 8 * (e >> 1) == 8 * n + col + (e & 1)) x += dot[n][e];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+      if (l == 0) inner[warp] = x;
+    }
     // the states' parts, scaled, and what the decays get from them
     {
       float from[2] = {0.f, 0.f}, to[2] = {0.f, 0.f};
@@ -322,15 +363,17 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
         const float fq = p.scale * gate.e[r], fr = gate.out[r] * gate.beta[r], fu = -gate.beta[r] * gate.e[r];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          if (kk0 + n / 2 >= n_k16) continue;
           const int kk = kk0 + n / 2, piece = (2 * kk + (n & 1)) & 7;
           const uint32_t at = (kk >> 2) * (C * 128) + 2048 * rb + key_swizzle(row + 8 * half, piece) + 2 * col;
-          float qx = 0.f, qy = 0.f, kx = 0.f, ky = 0.f;
+          float qx, qy, kx, ky;
 #pragma unroll
           for (int i = PX - 1; i >= 0; --i) {
             const uint32_t uq = *reinterpret_cast<const uint32_t*>(q_tile + 2 * i * R::kTile + at);
             const uint32_t uk = *reinterpret_cast<const uint32_t*>(k_tile + 2 * i * R::kTile + at);
-            qx += low(uq), qy += high(uq), kx += low(uk), ky += high(uk);
+            if (i == PX - 1)
+              qx = low(uq), qy = high(uq), kx = low(uk), ky = high(uk);
+            else
+              qx += low(uq), qy += high(uq), kx += low(uk), ky += high(uk);
           }
           float &q0 = dq[n][2 * half], &q1 = dq[n][2 * half + 1], &r0 = kr[n][2 * half], &r1 = kr[n][2 * half + 1];
           const float u0 = ku[n][2 * half] * fu, u1 = ku[n][2 * half + 1] * fu;
@@ -347,24 +390,23 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       }
     }
     __syncthreads();
-    if (warp == 7) {
+    if (warp == kWarps - 1) {
       // dlog_decay: sums of tokens from t on, and before t
       constexpr int M = C / 32;
       float a[M], e[M];
 #pragma unroll
       for (int i = 0; i < M; ++i) {
         const int t = l * M + i;
-        a[i] = row_sum[0][t] + row_sum[1][t];
-        e[i] = 0.f;
+        a[i] = e[i] = 0.f;
         float below = 0.f;
         for (int j = t / 16; j < NB; ++j) below += col_sum[0][j][t] + col_sum[1][j][t];
         a[i] -= below;
 #pragma unroll
-        for (int g = 0; g < R::kGroups; ++g) a[i] += from_state[g][t], e[i] += to_state[g][t];
+        for (int g = 0; g < R::kGroups; ++g) a[i] += row_sum[g][t] + from_state[g][t], e[i] += to_state[g][t];
       }
       float total = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) total += inner[i];
+      for (int i = 0; i < kWarps; ++i) total += inner[i];
       total *= gate.total;
 #pragma unroll
       for (int i = M - 2; i >= 0; --i) a[i] += a[i + 1];
@@ -407,9 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       }
 #pragma unroll
       for (int m = 0; m < NT / 2; ++m) {
-        if (kk0 + m >= n_k16) continue;
         uint32_t f[PX][4], g[PX][4];
-        const uint32_t at = key_down.at<C>(j, (kk0 + m) & 7);
+        const uint32_t at = own_down[m] + j * 2048;
 #pragma unroll
         for (int i = 0; i < PX; ++i) {
           ldsm_t(f[i], k_at + 2 * i * R::kTile + at);
@@ -425,15 +466,17 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
         }
       }
     }
+    E* const dq_at = (E*)p.dq.p + b * p.dq.sb + h * p.dq.sh + t0 * p.dq.st + 8 * group * NT + col;
+    E* const dk_at = (E*)p.dk_.p + b * p.dk_.sb + h * p.dk_.sh + t0 * p.dk_.st + 8 * group * NT + col;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int d = 8 * (group * NT + n) + col;
+    for (int half = 0; half < 2; ++half) {
+      const int t = 16 * rb + row + 8 * half;
+      if (t >= rows) continue;
+      E *const to_q = dq_at + (int64_t)t * p.dq.st, *const to_k = dk_at + (int64_t)t * p.dk_.st;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int t = 16 * rb + row + 8 * half;
-        if (t >= rows) continue;
-        store2((E*)p.dq.p + b * p.dq.sb + h * p.dq.sh + (t0 + t) * p.dq.st + d, dq[n][2 * half], dq[n][2 * half + 1], p.dk - d, pairs & 2);
-        store2((E*)p.dk_.p + b * p.dk_.sb + h * p.dk_.sh + (t0 + t) * p.dk_.st + d, kr[n][2 * half], kr[n][2 * half + 1], p.dk - d, pairs & 2);
+      for (int n = 0; n < NT; ++n) {
+        store2(to_q + 8 * n, dq[n][2 * half], dq[n][2 * half + 1], p.dk - (8 * (group * NT + n) + col), pairs & 2);
+        store2(to_k + 8 * n, kr[n][2 * half], kr[n][2 * half + 1], p.dk - (8 * (group * NT + n) + col), pairs & 2);
       }
     }
   }
@@ -467,7 +510,8 @@ int go(const Backward& p, cudaStream_t st) {
 }  // namespace
 
 int grad_launch(const Backward& p, int dtype, cudaStream_t st) {
-  return dtype == DYNCONV_DTYPE_F32 ? go<Grad<3, 32>>(p, st) : go<Grad<1, 64>>(p, st);
+  if (p.dk <= 64) return dtype == DYNCONV_DTYPE_F32 ? go<Grad<3, 32, 4>>(p, st) : go<Grad<1, 64, 4>>(p, st);
+  return dtype == DYNCONV_DTYPE_F32 ? go<Grad<3, 32, 8>>(p, st) : go<Grad<1, 64, 8>>(p, st);
 }
 
 }  // namespace dr

@@ -164,91 +164,117 @@ struct Inverse {
   }
 };
 
-// A = L beta (backward: beta L; into t and diag) and P of a chunk from its K and Q.  Row block i of either has
-// i + 1 blocks of 16 x 16.  Of four row blocks, warp 0 takes A's first and last, warp 1 the two between them, warps 2 and 3
-// the same of P: five blocks each, of which the first is of the first row block and the last three of
-// the second.  (Of two row blocks, warp 0 takes A's and warp 2 P's.)
-// Without BACK, `bad` becomes the first token whose key is not finite: its square shows it.
-template <typename G, bool BACK>
-__device__ __forceinline__ void make_scores(uint32_t k, uint32_t q, Gates<G::C>& s, float scale, int n_k16, __nv_bfloat16* t,
-                                            float* diag, __nv_bfloat16* p_out) {
-  constexpr int C = G::C, kS = G::kSquare, kPart = C * kS, PX = G::PX, NB = G::kBlocks, kUnits = NB == 4 ? 5 : 3;
-  const int w = warp_index(), l = threadIdx.x & 31, row = l >> 2, col = 2 * (l & 3);
-  if (NB == 2 && (w & 1)) return;
-  const bool is_p = w >= 2;
-  const int i0 = NB == 4 ? w & 1 : 0, i1 = NB - 1 - i0;  // the row blocks
+// A = L beta (backward: beta L) and P of a chunk from its K and Q.  Row block i of either has i + 1 blocks of
+// 16 x 16.  Of four row blocks, warp 0 takes A's first and last, warp 1 the two between them, warps 2 and 3 the same of P:
+// five blocks each, of which the first is of the first row block and the last three of the second.
+// (Of two row blocks, warp 0 takes A's and warp 2 P's.)
+template <typename G>
+struct Scores {
+  static constexpr int C = G::C, kS = G::kSquare, kPart = C * kS, PX = G::PX, NB = G::kBlocks, kUnits = NB == 4 ? 5 : 3;
   float X[kUnits][2][4];
+  int w, row, col, i0, i1;
+  bool is_p;
+
+  __device__ __forceinline__ Scores() {
+    const int l = threadIdx.x & 31;
+    w = warp_index(), row = l >> 2, col = 2 * (l & 3);
+    is_p = w >= 2;
+    i0 = NB == 4 ? w & 1 : 0, i1 = NB - 1 - i0;  // the row blocks
+  }
+  __device__ __forceinline__ bool idle() const { return NB == 2 && (w & 1); }
+  __device__ __forceinline__ int block_of(int u) const { return u <= i0 ? u : u - i0 - 1; }
+
+  __device__ __forceinline__ void products(uint32_t k, uint32_t q, int n_k16) {
+    if (idle()) return;
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) zero(X[u][0]), zero(X[u][1]);
-  const KeyLane across(false), down(true);
-  const uint32_t a_at = is_p ? q : k;
-  auto block_of = [&](int u) { return u <= i0 ? u : u - i0 - 1; };
+    for (int u = 0; u < kUnits; ++u) zero(X[u][0]), zero(X[u][1]);
+    const KeyLane across(false), down(true);
+    const uint32_t a_at = is_p ? q : k;
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk) {
-    if (kk >= n_k16) continue;
-    uint32_t a0[PX][4], a1[PX][4], am[PX][4];
+    for (int kk = 0; kk < 8; ++kk) {
+      if (kk >= n_k16) continue;
+      uint32_t a0[PX][4], a1[PX][4], am[PX][4];
 #pragma unroll
-    for (int i = 0; i < PX; ++i) {
-      ldsm(a0[i], a_at + 2 * i * G::kTile + down.at<C>(i0, kk));
-      ldsm(a1[i], a_at + 2 * i * G::kTile + down.at<C>(i1, kk));
+      for (int i = 0; i < PX; ++i) {
+        ldsm(a0[i], a_at + 2 * i * G::kTile + down.at<C>(i0, kk));
+        ldsm(a1[i], a_at + 2 * i * G::kTile + down.at<C>(i1, kk));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) am[i][e] = i0 ? a0[i][e] : a1[i][e];
-    }
+        for (int e = 0; e < 4; ++e) am[i][e] = i0 ? a0[i][e] : a1[i][e];
+      }
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      uint32_t b[PX][4];
+      for (int u = 0; u < kUnits; ++u) {
+        uint32_t b[PX][4];
 #pragma unroll
-      for (int i = 0; i < PX; ++i) ldsm(b[i], k + 2 * i * G::kTile + across.at<C>(block_of(u), kk));
-      if (u == 0)
-        mma_parts<PX, PX, PX>(X[u][0], X[u][1], a0, b);
-      else if (u == 1)
-        mma_parts<PX, PX, PX>(X[u][0], X[u][1], am, b);
-      else
-        mma_parts<PX, PX, PX>(X[u][0], X[u][1], a1, b);
+        for (int i = 0; i < PX; ++i) ldsm(b[i], k + 2 * i * G::kTile + across.at<C>(block_of(u), kk));
+        if (u == 0)
+          mma_parts<PX, PX, PX>(X[u][0], X[u][1], a0, b);
+        else if (u == 1)
+          mma_parts<PX, PX, PX>(X[u][0], X[u][1], am, b);
+        else
+          mma_parts<PX, PX, PX>(X[u][0], X[u][1], a1, b);
+      }
     }
   }
+
+  // The first token whose key is not finite: its square shows it.
+  __device__ __forceinline__ void find_bad(int* bad) const {
+    if (idle() || is_p) return;
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    const int i = u <= i0 ? i0 : i1, j = block_of(u);
+    for (int u = 0; u < kUnits; ++u) {
+      const int i = u <= i0 ? i0 : i1;
+      if (block_of(u) != i) continue;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = 16 * i + row + 8 * half, last = is_p ? r : r - 1;  // the last column that counts
-      const float hi_r = s.hi[r], lo_r = s.lo[r], beta_r = is_p ? scale : s.beta[r];
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int c = 16 * j + 8 * n + col;
-        const float2 hi = *reinterpret_cast<const float2*>(s.hi + c), lo = *reinterpret_cast<const float2*>(s.lo + c);
-        const float2 beta = *reinterpret_cast<const float2*>(s.beta + c);
-        float x = X[u][n][2 * half], y = X[u][n][2 * half + 1];
-        if constexpr (!BACK) {
-          if (!is_p && ((c == r && !(x < INFINITY)) || (c + 1 == r && !(y < INFINITY)))) atomicMin(&s.bad, r);
-        }
-        x *= (BACK || is_p ? beta_r : beta.x) * exp2_fast((hi_r - hi.x) + (lo_r - lo.x));
-        y *= (BACK || is_p ? beta_r : beta.y) * exp2_fast((hi_r - hi.y) + (lo_r - lo.y));
-        x = c <= last ? x : 0.f, y = c < last ? y : 0.f;
-        if (is_p) {
-          uint32_t p[G::PP];
-          split<G::PP>(x, y, p);
+        for (int e = 0; e < 4; ++e)
+          if (row + 8 * (e >> 1) == 8 * n + col + (e & 1) && !(X[u][n][e] < INFINITY)) atomicMin(bad, 16 * i + row + 8 * (e >> 1));
+    }
+  }
+
+  template <bool BACK>
+  __device__ __forceinline__ void write(const Gates<C>& s, float scale, __nv_bfloat16* t, float* diag, __nv_bfloat16* p_out) const {
+    if (idle()) return;
 #pragma unroll
-          for (int e = 0; e < G::PP; ++e) *reinterpret_cast<uint32_t*>(p_out + e * kPart + r * kS + c) = p[e];
-        } else if (j == i) {
-          *reinterpret_cast<float2*>(diag + i * 256 + (row + 8 * half) * 16 + 8 * n + col) = make_float2(x, y);
-        } else {
-          uint32_t p[G::NP];
-          split<G::NP>(x, y, p);
+    for (int u = 0; u < kUnits; ++u) {
+      const int i = u <= i0 ? i0 : i1, j = block_of(u);
 #pragma unroll
-          for (int e = 0; e < G::NP; ++e)
-            *reinterpret_cast<uint32_t*>(t + e * kPart + (16 * j + row + 8 * half) * kS + 16 * i + 8 * n + col) = p[e];
+      for (int half = 0; half < 2; ++half) {
+        const int r = 16 * i + row + 8 * half, last = is_p ? r : r - 1;  // the last column that counts
+        const float hi_r = s.hi[r], lo_r = s.lo[r], beta_r = is_p ? scale : s.beta[r];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int c = 16 * j + 8 * n + col;
+          const float2 hi = *reinterpret_cast<const float2*>(s.hi + c), lo = *reinterpret_cast<const float2*>(s.lo + c);
+          const float2 beta = *reinterpret_cast<const float2*>(s.beta + c);
+          float x = X[u][n][2 * half], y = X[u][n][2 * half + 1];
+          x *= (BACK || is_p ? beta_r : beta.x) * exp2_fast((hi_r - hi.x) + (lo_r - lo.x));
+          y *= (BACK || is_p ? beta_r : beta.y) * exp2_fast((hi_r - hi.y) + (lo_r - lo.y));
+          x = c <= last ? x : 0.f, y = c < last ? y : 0.f;
+          if (is_p) {
+            uint32_t p[G::PP];
+            split<G::PP>(x, y, p);
+#pragma unroll
+            for (int e = 0; e < G::PP; ++e) *reinterpret_cast<uint32_t*>(p_out + e * kPart + r * kS + c) = p[e];
+          } else if (j == i) {
+            *reinterpret_cast<float2*>(diag + i * 256 + (row + 8 * half) * 16 + 8 * n + col) = make_float2(x, y);
+          } else {
+            uint32_t p[G::NP];
+            split<G::NP>(x, y, p);
+#pragma unroll
+            for (int e = 0; e < G::NP; ++e)
+              *reinterpret_cast<uint32_t*>(t + e * kPart + (16 * j + row + 8 * half) * kS + 16 * i + 8 * n + col) = p[e];
+          }
         }
       }
     }
   }
-}
+};
 
 template <typename G>
 struct PrepSmem {
   static constexpr int kT = G::NP * G::C * G::kSquare, kP = G::PP * G::C * G::kSquare;  // elements
-  static constexpr size_t kBytes = 1024 + 2 * (size_t)(2 * G::PX * G::kTile + kT + kP) + G::kBlocks * 1024 + sizeof(Gates<G::C>);
+  static constexpr int kKq = 2 * G::PX * G::kTile, kSpace = kT + kP > kKq ? kT + kP : kKq;  // T and P take K's and Q's place
+  static constexpr size_t kBytes = 1024 + 2 * (size_t)kSpace + G::kBlocks * 1024 + sizeof(Gates<G::C>);
 };
 
 template <typename G, bool BACK>
@@ -261,8 +287,8 @@ __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const
   uint8_t* const smem = align_smem_1024(smem_raw);
   using E = typename G::T;
   uint8_t *const ks = smem, *const qs = ks + 2 * PX * G::kTile;
-  __nv_bfloat16 *const t = (__nv_bfloat16*)(qs + 2 * PX * G::kTile), *const p = t + PrepSmem<G>::kT;
-  float* const diag = (float*)(p + PrepSmem<G>::kP);
+  __nv_bfloat16 *const t = (__nv_bfloat16*)ks, *const p = t + PrepSmem<G>::kT;
+  float* const diag = (float*)(smem + 2 * PrepSmem<G>::kSpace);
   Gates<C>& s = *(Gates<C>*)(diag + NB * 256);
   const int tid = threadIdx.x, lane = tid & 31, w = warp_index(), n_k16 = (dk + 15) / 16, halves = dk > 64 ? 2 : 1;
   const int64_t bh = blockIdx.y, b = bh / H, h = bh % H, chunk = blockIdx.x, t0 = chunk * C, at = bh * gridDim.x + chunk;
@@ -298,22 +324,27 @@ __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const
     if (tid == 0) mbar_drain(&full, 0);
     return;
   }
-  for (bool cleared = BACK;; cleared = true) {
-    make_scores<G, BACK>(smem_u32(ks), smem_u32(qs), s, scale, n_k16, t, diag, p);
-    __syncthreads();
+  Scores<G> scores;
+  scores.products(smem_u32(ks), smem_u32(qs), n_k16);
+  if constexpr (!BACK) scores.find_bad(&s.bad);
+  __syncthreads();
+  if constexpr (!BACK) {
     // Products with a masked zero would carry what is not finite to earlier tokens: keys and gates from the
     // first bad token on are zeroed, and the chains make NaN of what depends on them.  (rare)
     const int bad = s.bad;
-    if (cleared || bad >= C) break;
-    for (int i = tid; i < PX * halves * C * 32; i += kThreads)
-      if (i / 32 % C >= bad) ((uint32_t*)ks)[i / (halves * C * 32) * (G::kTile / 2) + i % (halves * C * 32)] = 0;
-    if (tid >= bad && tid < C) {
-      s.beta[tid] = 0.f;
-      s.hi[tid] = bad > 0 ? s.hi[bad - 1] : 0.f, s.lo[tid] = bad > 0 ? s.lo[bad - 1] : 0.f;
-      s.e[tid] = bad > 0 ? s.e[bad - 1] : 1.f;
+    if (bad < C) {
+      for (int i = tid; i < PX * halves * C * 32; i += kThreads)
+        if (i / 32 % C >= bad) ((uint32_t*)ks)[i / (halves * C * 32) * (G::kTile / 2) + i % (halves * C * 32)] = 0;
+      if (tid >= bad && tid < C) {
+        s.beta[tid] = 0.f;
+        s.hi[tid] = bad > 0 ? s.hi[bad - 1] : 0.f, s.lo[tid] = bad > 0 ? s.lo[bad - 1] : 0.f;
+        s.e[tid] = bad > 0 ? s.e[bad - 1] : 1.f;
+      }
+      if (tid < C) s.out[tid] = 0.f;  // (the state after the chunk is NaN)
+      __syncthreads();
+      scores.products(smem_u32(ks), smem_u32(qs), n_k16);
+      __syncthreads();
     }
-    if (tid < C) s.out[tid] = 0.f;  // (the state after the chunk is NaN)
-    __syncthreads();
   }
   // gates and copies
   for (int i = tid; i < (int)sizeof(Gates<C>) / 16; i += kThreads)
@@ -324,7 +355,9 @@ __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const
       ((uint4*)to.k)[at * (PX * halves * C * 8) + i] = ((const uint4*)ks)[from];
       ((uint4*)to.q)[at * (PX * halves * C * 8) + i] = ((const uint4*)qs)[from];
     }
+    __syncthreads();
   }
+  scores.template write<BACK>(s, scale, t, diag, p);
   if (to.v) {
     const int dv16 = (dv + 15) / 16 * 16;
     const E* from = (const E*)v.p + b * v.sb + h * v.sh + t0 * v.st;
@@ -333,6 +366,7 @@ __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const
       ((E*)to.v)[at * (C * dv16) + i] = r < rows && c < dv ? from[r * v.st + c] : Elem<E>::from_f(0.f);
     }
   }
+  __syncthreads();
   Inverse<G>::run(t, diag);
   // blocks (i, j), j <= i, as second operands: of a product with the transpose, or (BACK) with the matrix itself
   const int turn = lane_offset(G::kSquare, BACK);

@@ -7,9 +7,9 @@ namespace dynconv {
 namespace dr {
 namespace {
 
-template <typename G, int W>
-__global__ void __launch_bounds__(288, 1) delta_bwd_kernel(Backward p, const __grid_constant__ Maps maps, Plan plan) {
-  using Ch = Chain<G, W>;
+template <typename G, int W, int KK>
+__global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_kernel(Backward p, const __grid_constant__ Maps maps, Plan plan) {
+  using Ch = Chain<G, W, KK>;
   using E = typename G::T;
   constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks, TB = Ch::TB, NT = Ch::NT, PU = Ch::PU;
   constexpr int PS = PX == 1 ? 1 : 3, KX = PX > PP ? PX : PP;
@@ -20,10 +20,13 @@ __global__ void __launch_bounds__(288, 1) delta_bwd_kernel(Backward p, const __g
   const int chunks = (int)((p.T + C - 1) / C), n_k16 = (p.dk + 15) / 16, first_col = blockIdx.x * plan.teams * 16;
   const int warp = warp_index(), l = threadIdx.x & 31, row = l >> 2, col = 2 * (l & 3);
   Ch::init(bars, Ch::live_teams(plan, p.dv, first_col));
+  const typename Ch::Producer producer{smem, bars, plan, maps, p.pre, (int)b, (int)h, chunks, p.dk, p.dv, first_col, bh};
   if (warp == plan.teams * W) {
-    if (l == 0) Ch::template produce<true>(smem, bars, plan, maps, p.pre, (int)b, (int)h, bh, chunks, p.dk, p.dv, first_col);
+    if (l == 0) producer.template walk<true>();
     return;
   }
+  const bool produces = threadIdx.x == 0 && !plan.own_warp;
+  if (produces) producer.template start<true>();
   const int team = warp / W, w = (warp + team) % W;
   const int d0 = first_col + 16 * team, slices = (p.dv + 15) / 16, slice = d0 / 16;
   if (d0 >= p.dv) return;
@@ -38,7 +41,11 @@ __global__ void __launch_bounds__(288, 1) delta_bwd_kernel(Backward p, const __g
 #pragma unroll
     for (int m = 0; m < NT / 2; ++m) {
       const int kk = w * NT / 2 + m;
-      down[m] = (NT == 8 || !(w & 1) ? lane.off[m] : lane.off[m + 2]) + (kk >> 2) * (C * 128);
+      uint32_t off = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i == (kk & 3)) off = lane.off[i];
+      down[m] = off + (kk >> 2) * (C * 128);
     }
   }
 
@@ -67,7 +74,10 @@ __global__ void __launch_bounds__(288, 1) delta_bwd_kernel(Backward p, const __g
   publish(chunks - 1);
 
   for (int c = chunks - 1, stage = 0, parity = 0; c >= 0; --c) {
-    if (!Ch::team_all(team, mbar_wait(&bars.full[stage], parity, kErrWaitMma, &bars.abort_flag))) return;
+    if (!Ch::team_all(team, mbar_wait(&bars.full[stage], parity, kErrWaitMma, &bars.abort_flag))) {
+      if (produces) producer.drain(chunks - 1 - c, chunks - 1 - c + plan.stages);
+      return;
+    }
     const typename Ch::Stage s{smem + stage * bytes, plan.teams};
     const Gates<C>& gate = s.gates();
     // dO^T of the slice as first operands
@@ -126,9 +136,8 @@ __global__ void __launch_bounds__(288, 1) delta_bwd_kernel(Backward p, const __g
       };
       fetch(0, a[0], f[0]);
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        if (kk >= n_k16) continue;
-        if (kk + 1 < n_k16) fetch(kk + 1, a[(kk + 1) & 1], f[(kk + 1) & 1]);
+      for (int kk = 0; kk < KK; ++kk) {
+        if (kk + 1 < KK) fetch(kk + 1, a[(kk + 1) & 1], f[(kk + 1) & 1]);
 #pragma unroll
         for (int t = 0; t < TB; ++t) mma_levels<NP, PX, NP, L>(z[t], a[kk & 1], f[kk & 1][t]);
       }
@@ -177,6 +186,7 @@ __global__ void __launch_bounds__(288, 1) delta_bwd_kernel(Backward p, const __g
       operand<NP>(scaled[0], scaled[1], a);
       Ch::put(part_o + blk * NP * 32, a);
     }
+    if (produces && c < chunks - 1) producer.template refill<true>(chunks - 1 - c);
     Ch::team_sync(team);
     // dU^T = x^T T
 #pragma unroll
@@ -220,19 +230,19 @@ __global__ void __launch_bounds__(288, 1) delta_bwd_kernel(Backward p, const __g
     Ch::team_sync(team);
     // dS0^T = e^(b_C) dS1^T + (scale e^b dO)^T Q - (beta e^b dU)^T K
     const float total = gate.total;
+    constexpr int NX = NT < 4 ? NT : 4;
 #pragma unroll
-    for (int n = 0; n < NT; n += 4) {
-      if (8 * (w * NT + n) >= 16 * n_k16) continue;
-      float x[4][4];
+    for (int n = 0; n < NT; n += NX) {
+      float x[NX][4];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) zero(x[m]);
+      for (int m = 0; m < NX; ++m) zero(x[m]);
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         uint32_t a[NP][4], g[NP][4];
         Ch::template get<NP>(part_o + j * NP * 32, a);
         Ch::template get<NP>(part_u + j * NP * 32, g);
 #pragma unroll
-        for (int m = 0; m < 4; m += 2) {
+        for (int m = 0; m < NX; m += 2) {
           uint32_t f[PX][4], k[PX][4];
 #pragma unroll
           for (int i = 0; i < PX; ++i) {
@@ -245,7 +255,7 @@ __global__ void __launch_bounds__(288, 1) delta_bwd_kernel(Backward p, const __g
         }
       }
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int m = 0; m < NX; ++m)
 #pragma unroll
         for (int e = 0; e < 4; ++e) S[n + m][e] = bad > 0 ? NAN : fmaf(total, S[n + m][e], x[m][e]);
     }
@@ -265,12 +275,12 @@ __global__ void __launch_bounds__(288, 1) delta_bwd_kernel(Backward p, const __g
   }
 }
 
-template <typename G, int W>
+template <typename G, int W, int KK>
 int go(const Backward& p, const Plan& plan, cudaStream_t st) {
-  using Ch = Chain<G, W>;
+  using Ch = Chain<G, W, KK>;
   int s;
   const int slices = (p.dv + 15) / 16, smem = Ch::smem_bytes(plan.teams, plan.stages);
-  const cudaError_t e = cudaFuncSetAttribute(delta_bwd_kernel<G, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = cudaFuncSetAttribute(delta_bwd_kernel<G, W, KK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return cuda_status(e, "cudaFuncSetAttribute(delta_bwd)");
@@ -278,7 +288,7 @@ int go(const Backward& p, const Plan& plan, cudaStream_t st) {
   Maps maps{};
   if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.d_o, p.B, p.T, p.H, p.dk, p.dv))) return s;
   const dim3 grid((unsigned)((slices + plan.teams - 1) / plan.teams), (unsigned)(p.B * p.H));
-  delta_bwd_kernel<G, W><<<grid, 32 * (plan.teams * W + 1), smem, st>>>(p, maps, plan);
+  delta_bwd_kernel<G, W, KK><<<grid, 32 * (plan.teams * W + plan.own_warp), smem, st>>>(p, maps, plan);
   DYNCONV_CHECK_LAUNCH("delta_bwd_kernel");
   return DYNCONV_OK;
 }
@@ -286,11 +296,9 @@ int go(const Backward& p, const Plan& plan, cudaStream_t st) {
 template <typename G>
 int pick(const Backward& p, cudaStream_t st) {
   const int64_t bh = (int64_t)p.B * p.H;
-  if constexpr (G::kBlocks == 4) {
-    const Plan four = plan_of<G, 4>(bh, p.dv);
-    if (four.teams <= 2) return go<G, 4>(p, four, st);
-  }
-  return go<G, 2>(p, plan_of<G, 2>(bh, p.dv), st);
+  constexpr int W = G::kBlocks;  // one block of 16 tokens for each warp
+  if (p.dk <= 64) return go<G, W, 4>(p, plan_of<Chain<G, W, 4>>(bh, p.dv), st);
+  return go<G, W, 8>(p, plan_of<Chain<G, W, 8>>(bh, p.dv), st);
 }
 
 }  // namespace

@@ -13,9 +13,9 @@ __device__ __noinline__ void store_slow(const E* tile, E* to, int64_t step, int 
     if (i % 16 < cols) to[i / 16 * step + i % 16] = tile[i];
 }
 
-template <typename G, int W, bool SAVE>
-__global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __grid_constant__ Maps maps, Plan plan) {
-  using Ch = Chain<G, W>;
+template <typename G, int W, int KK, bool SAVE>
+__global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_kernel(Forward p, const __grid_constant__ Maps maps, Plan plan) {
+  using Ch = Chain<G, W, KK>;
   using E = typename G::T;
   constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks, TB = Ch::TB, NT = Ch::NT, PU = Ch::PU;
   constexpr int PS = PX == 1 ? 1 : 3;  // parts of the state in the outputs' product
@@ -26,10 +26,13 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
   const int chunks = (int)((p.T + C - 1) / C), n_k16 = (p.dk + 15) / 16, first_col = blockIdx.x * plan.teams * 16;
   const int warp = warp_index(), l = threadIdx.x & 31, row = l >> 2, col = 2 * (l & 3);
   Ch::init(bars, Ch::live_teams(plan, p.dv, first_col));
+  const typename Ch::Producer producer{smem, bars, plan, maps, p.pre, (int)b, (int)h, chunks, p.dk, p.dv, first_col, bh};
   if (warp == plan.teams * W) {
-    if (l == 0) Ch::template produce<false>(smem, bars, plan, maps, p.pre, (int)b, (int)h, bh, chunks, p.dk, p.dv, first_col);
+    if (l == 0) producer.template walk<false>();
     return;
   }
+  const bool produces = threadIdx.x == 0 && !plan.own_warp;
+  if (produces) producer.template start<false>();
   const int team = warp / W, w = (warp + team) % W;  // (turned, so that the last tokens' warps fall on different schedulers)
   const int d0 = first_col + 16 * team, slices = (p.dv + 15) / 16, slice = d0 / 16;
   if (d0 >= p.dv) return;
@@ -44,7 +47,11 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
 #pragma unroll
     for (int m = 0; m < NT / 2; ++m) {
       const int kk = w * NT / 2 + m;
-      down[m] = (NT == 8 || !(w & 1) ? lane.off[m] : lane.off[m + 2]) + (kk >> 2) * (C * 128);
+      uint32_t off = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i == (kk & 3)) off = lane.off[i];
+      down[m] = off + (kk >> 2) * (C * 128);
     }
   }
 
@@ -75,7 +82,10 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
   publish(0);
 
   for (int c = 0, stage = 0, parity = 0; c < chunks; ++c) {
-    if (!Ch::team_all(team, mbar_wait(&bars.full[stage], parity, kErrWaitMma, &bars.abort_flag))) return;
+    if (!Ch::team_all(team, mbar_wait(&bars.full[stage], parity, kErrWaitMma, &bars.abort_flag))) {
+      if (produces) producer.drain(c, c + plan.stages);
+      return;
+    }
     const typename Ch::Stage s{smem + stage * bytes, plan.teams};
     const Gates<C>& gate = s.gates();
     int bad = gate.bad;
@@ -105,9 +115,8 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
       };
       fetch(0, a[0], f[0], g[0]);
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        if (kk >= n_k16) continue;
-        if (kk + 1 < n_k16) fetch(kk + 1, a[(kk + 1) & 1], f[(kk + 1) & 1], g[(kk + 1) & 1]);
+      for (int kk = 0; kk < KK; ++kk) {
+        if (kk + 1 < KK) fetch(kk + 1, a[(kk + 1) & 1], f[(kk + 1) & 1], g[(kk + 1) & 1]);
         uint32_t a_o[PS][4];
 #pragma unroll
         for (int i = 0; i < PS; ++i)
@@ -169,6 +178,7 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
       Ch::put(part_r + Ch::token_block(w, t) * NP * 32, a);
     }
     // (another warp's tokens may be the bad ones)
+    if (produces && c > 0) producer.template refill<false>(c);
     if (!Ch::team_all(team, !odd_here)) bad = min(bad, Ch::bad_row(v_tile, false));
     // r^T = (V - e^b K S0)^T T^T, U = beta r
     float U[TB][2][4];
@@ -179,18 +189,14 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
         float u[NP][2][4];
 #pragma unroll
         for (int i = 0; i < NP; ++i) zero(u[i][0]), zero(u[i][1]);
-        uint32_t a[2][NP][4], f[2][NP][4];
         const uint4* const t_at = s.t() + lower(blk, 0) * NP * 32;
-        Ch::template get<NP>(part_r, a[0]);
-        Ch::template get<NP>(t_at, f[0]);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           if (j > blk) continue;
-          if (j < blk) {
-            Ch::template get<NP>(part_r + (j + 1) * NP * 32, a[(j + 1) & 1]);
-            Ch::template get<NP>(t_at + (j + 1) * NP * 32, f[(j + 1) & 1]);
-          }
-          mma_levels<NP, NP, NP, NP>(u, a[j & 1], f[j & 1]);
+          uint32_t a[NP][4], f[NP][4];
+          Ch::template get<NP>(part_r + j * NP * 32, a);
+          Ch::template get<NP>(t_at + j * NP * 32, f);
+          mma_levels<NP, NP, NP, NP>(u, a, f);
         }
         sum_levels<NP>(U[t], u);
       }
@@ -223,18 +229,18 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
     // S^T <- e^(b_C) S^T + (e^(b_C - b) U)^T K, each chunk's sum by itself first: the instruction's own
     // additions are cut off, not rounded
     const float total = gate.total;
+    constexpr int NX = NT < 4 ? NT : 4;
 #pragma unroll
-    for (int n = 0; n < NT; n += 4) {
-      if (8 * (w * NT + n) >= 16 * n_k16) continue;
-      float x[4][4];
+    for (int n = 0; n < NT; n += NX) {
+      float x[NX][4];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) zero(x[m]);
+      for (int m = 0; m < NX; ++m) zero(x[m]);
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         uint32_t a[NP][4];
         Ch::template get<NP>(part_s + j * NP * 32, a);
 #pragma unroll
-        for (int m = 0; m < 4; m += 2) {
+        for (int m = 0; m < NX; m += 2) {
           uint32_t f[PX][4];
 #pragma unroll
           for (int i = 0; i < PX; ++i)
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
         }
       }
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int m = 0; m < NX; ++m)
 #pragma unroll
         for (int e = 0; e < 4; ++e) S[n + m][e] = bad < C ? NAN : fmaf(total, S[n + m][e], x[m][e]);
     }
@@ -257,18 +263,14 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
         float o[PU][2][4];
 #pragma unroll
         for (int i = 0; i < PU; ++i) zero(o[i][0]), zero(o[i][1]);
-        uint32_t a[2][PU][4], f[2][PP][4];
         const uint4* const p_at = s.p() + lower(blk, 0) * PP * 32;
-        Ch::template get<PU>(part_u, a[0]);
-        Ch::template get<PP>(p_at, f[0]);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           if (j > blk) continue;
-          if (j < blk) {
-            Ch::template get<PU>(part_u + (j + 1) * PU * 32, a[(j + 1) & 1]);
-            Ch::template get<PP>(p_at + (j + 1) * PP * 32, f[(j + 1) & 1]);
-          }
-          mma_levels<PU, PP, PU, PU>(o, a[j & 1], f[j & 1]);
+          uint32_t a[PU][4], f[PP][4];
+          Ch::template get<PU>(part_u + j * PU * 32, a);
+          Ch::template get<PP>(p_at + j * PP * 32, f);
+          mma_levels<PU, PP, PU, PU>(o, a, f);
         }
         float x[2][4];
         sum_levels<PU>(x, o);
@@ -325,14 +327,14 @@ __global__ void __launch_bounds__(288, 1) delta_fwd_kernel(Forward p, const __gr
   }
 }
 
-template <typename G, int W, bool SAVE>
+template <typename G, int W, int KK, bool SAVE>
 int go(const Forward& p, Plan plan, cudaStream_t st) {
-  using Ch = Chain<G, W>;
+  using Ch = Chain<G, W, KK>;
   int s;
   const int slices = (p.dv + 15) / 16;
   plan.o_vectors = vectors_of(p.o, p.dv, sizeof(typename G::T));
   const int smem = Ch::smem_bytes(plan.teams, plan.stages);
-  const cudaError_t e = cudaFuncSetAttribute(delta_fwd_kernel<G, W, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = cudaFuncSetAttribute(delta_fwd_kernel<G, W, KK, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return cuda_status(e, "cudaFuncSetAttribute(delta_fwd)");
@@ -340,7 +342,7 @@ int go(const Forward& p, Plan plan, cudaStream_t st) {
   Maps maps{};
   if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.v, p.B, p.T, p.H, p.dk, p.dv))) return s;
   const dim3 grid((unsigned)((slices + plan.teams - 1) / plan.teams), (unsigned)(p.B * p.H));
-  delta_fwd_kernel<G, W, SAVE><<<grid, 32 * (plan.teams * W + 1), smem, st>>>(p, maps, plan);
+  delta_fwd_kernel<G, W, KK, SAVE><<<grid, 32 * (plan.teams * W + plan.own_warp), smem, st>>>(p, maps, plan);
   DYNCONV_CHECK_LAUNCH("delta_fwd_kernel");
   return DYNCONV_OK;
 }
@@ -348,11 +350,9 @@ int go(const Forward& p, Plan plan, cudaStream_t st) {
 template <typename G, bool SAVE>
 int pick(const Forward& p, cudaStream_t st) {
   const int64_t bh = (int64_t)p.B * p.H;
-  if constexpr (G::kBlocks == 4) {
-    const Plan four = plan_of<G, 4>(bh, p.dv);
-    if (four.teams <= 2) return go<G, 4, SAVE>(p, four, st);
-  }
-  return go<G, 2, SAVE>(p, plan_of<G, 2>(bh, p.dv), st);
+  constexpr int W = G::kBlocks;  // one block of 16 tokens for each warp
+  if (p.dk <= 64) return go<G, W, 4, SAVE>(p, plan_of<Chain<G, W, 4>>(bh, p.dv), st);
+  return go<G, W, 8, SAVE>(p, plan_of<Chain<G, W, 8>>(bh, p.dv), st);
 }
 
 }  // namespace
