@@ -36,7 +36,7 @@ struct Chain {
   static constexpr int kMostThreads = 32 * W * kMostTeams;
 
   static constexpr int kKq = PX * G::kTile * 2;  // bytes
-  static constexpr int kV = C * 16 * (int)sizeof(E);  // of a team: [C tokens][16 columns]
+  static constexpr int kRow = 16 * (int)sizeof(E), kV = C * kRow;  // of a team's columns: the tile is [C tokens][teams * 16]
   static constexpr int kT = G::kLower * NP * 512, kP = G::kLower * PP * 512, kGates = sizeof(Gates<C>);
   static constexpr int kState = KK * NP * 512, kBlock = NB * NP * 512;  // a team's buffers
   static constexpr int kTeam = kState + 3 * kBlock;
@@ -50,7 +50,14 @@ struct Chain {
     int teams;
     __device__ __forceinline__ uint32_t k() const { return smem_u32(at); }
     __device__ __forceinline__ uint32_t q() const { return smem_u32(at) + kKq; }
-    __device__ __forceinline__ E* v(int team) const { return (E*)(at + 2 * kKq + team * kV); }
+    __device__ __forceinline__ uint8_t* v() const { return at + 2 * kKq; }
+    // a token's 16-byte piece of a team's columns
+    __device__ __forceinline__ uint8_t* v(int team, int r, int piece) const {
+      return v() + row_swizzle(teams * kRow, r, team * (kRow / 16) + piece);
+    }
+    __device__ __forceinline__ E& value(int team, int r, int d) const {
+      return ((E*)v(team, r, d / (16 / (int)sizeof(E))))[d % (16 / (int)sizeof(E))];
+    }
     __device__ __forceinline__ uint4* t() const { return (uint4*)(at + 2 * kKq + teams * kV); }
     __device__ __forceinline__ uint4* p() const { return t() + kT / 16; }
     __device__ __forceinline__ Gates<C>& gates() const { return *(Gates<C>*)(p() + kP / 16); }
@@ -99,8 +106,8 @@ struct Chain {
 
     template <bool BACK>
     __device__ __forceinline__ void load(int n, int stage) const {
-      const int halves = dk > 64 ? 2 : 1, live = live_teams(plan, dv, first_col), slices = (dv + 15) / 16;
-      const uint32_t half = C * 128, all = 2 * PX * halves * half + live * kV + kT + kP + kGates;
+      const int halves = dk > 64 ? 2 : 1;
+      const uint32_t half = C * 128, all = 2 * PX * halves * half + plan.teams * kV + kT + kP + kGates;
       const Stage st{smem + stage * stage_bytes(plan.teams), plan.teams};
       uint8_t *const k = st.at, *const q = st.at + kKq;
       const int c = BACK ? chunks - 1 - n : n;
@@ -119,12 +126,7 @@ struct Chain {
           tma_load_4d(q + d * half, &maps.q, bar, 64 * d, h, c * C, b, policy_evict_normal());
         }
       }
-      for (int t = 0; t < live; ++t) {
-        if (pre.v)
-          bulk_load(st.v(t), (const E*)pre.v + (at * slices + first_col / 16 + t) * (C * 16), kV, bar);
-        else
-          tma_load_4d(st.v(t), &maps.v, bar, (first_col + 16 * t) * (int)(sizeof(E) / 2), h, c * C, b, policy_evict_normal());
-      }
+      tma_load_4d(st.v(), &maps.v, bar, first_col * (int)(sizeof(E) / 2), h, c * C, b, policy_evict_normal());
       bulk_load(st.t(), pre.t + at * (kT / 16), kT, bar);
       bulk_load(st.p(), pre.p + at * (kP / 16), kP, bar);
       bulk_load(&st.gates(), (const uint8_t*)pre.gates + at * kGates, kGates, bar);
@@ -156,13 +158,13 @@ struct Chain {
     }
   };
 
-  // The first row (last: one more than the last) of a [C] x [16] tile that holds a number that is not finite; C (0)
+  // The first row (last: one more than the last) of a team's columns that holds a number that is not finite; C (0)
   // where there is none.  One warp.
-  static __device__ __noinline__ int bad_row(const E* tile, bool last) {
+  static __device__ __noinline__ int bad_row(Stage s, int team, bool last) {
     int bad = last ? 0 : C;
     for (int r = threadIdx.x & 31; r < C; r += 32)
       for (int d = 0; d < 16; ++d)
-        if (!(fabsf(Elem<E>::to_f(tile[r * 16 + d])) < INFINITY)) bad = last ? max(bad, r + 1) : min(bad, r);
+        if (!(fabsf(Elem<E>::to_f(s.value(team, r, d))) < INFINITY)) bad = last ? max(bad, r + 1) : min(bad, r);
     return last ? __reduce_max_sync(0xffffffffu, bad) : __reduce_min_sync(0xffffffffu, bad);
   }
 
@@ -188,11 +190,10 @@ struct Chain {
 };
 
 template <typename G>
-int chain_maps(Maps* maps, const Prepared& pre, const View& k, const View& q, const View& v, int B, int64_t T, int H, int dk, int dv) {
+int chain_maps(Maps* maps, const Prepared& pre, const View& k, const View& q, const View& v, int B, int64_t T, int H, int dk, int dv, int teams) {
   int s = DYNCONV_OK;
   if (!pre.k && ((s = view_map(&maps->k, k, B, T, H, dk, 2, 64, G::C)) || (s = view_map(&maps->q, q, B, T, H, dk, 2, 64, G::C)))) return s;
-  if (!pre.v) s = view_map(&maps->v, v, B, T, H, dv, sizeof(typename G::T), 16, G::C);
-  return s;
+  return value_map(&maps->v, pre, v, B, T, H, dv, sizeof(typename G::T), 16 * teams, G::C);
 }
 
 // CTAs of as few teams as let all slices run at once, each then having more of its SM's matrix units and shared

@@ -25,7 +25,9 @@ struct Grad {
   static constexpr int kSlab = PX == 1 ? 4 : 2;                     // slices of 16 columns of v
   static constexpr int kTile = C * kMaxKey, kSquare = C + 8;
   using E = typename std::conditional<PX_ == 1, __nv_bfloat16, float>::type;
-  static constexpr int kDo = C * 16 * (int)sizeof(E), kU = NB * 512;  // bytes of a slice: of dO, of one part of r or dU
+  static constexpr int kRow = 16 * (int)sizeof(E), kDo = C * kRow, kU = NB * 512;  // bytes of a slice: of dO (tile: [C][kSlab * 16]), of one
+                                                                                   // part of r or dU
+  static_assert(kSlab * kRow == 128, "a tile of dO has rows of 128 bytes");
   static constexpr int kS = KK * 512;                                 // of one part of a state, at most
   static constexpr int kSlabBytes = kSlab * (kDo + 2 * PU * kU + 2 * PS * kS);
   static constexpr int kKq = 2 * PX * kTile * 2, kWn = 2 * PX * C * kSquare * 2;
@@ -88,13 +90,8 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
     uint8_t* const s = slabs + at * R::kSlabBytes;
     uint64_t* const bar = &slab_full[at];
     const uint32_t state = n * n_k16 * 512;
-    mbar_arrive_expect_tx(bar, n * (R::kDo + 2 * PU * R::kU) + 2 * PS * state);
-    for (int i = 0; i < n; ++i) {
-      if (p.pre.v)
-        bulk_load(s + i * R::kDo, (const E*)p.pre.v + (item * slices + first + i) * (C * 16), R::kDo, bar);
-      else
-        tma_load_4d(s + i * R::kDo, &maps.v, bar, (first + i) * 16 * (int)(sizeof(E) / 2), (int)(bh % p.H), c * C, (int)(bh / p.H), policy_evict_normal());
-    }
+    mbar_arrive_expect_tx(bar, kSlab * R::kDo + n * 2 * PU * R::kU + 2 * PS * state);
+    tma_load_4d(s, &maps.v, bar, first * 16 * (int)(sizeof(E) / 2), (int)(bh % p.H), c * C, (int)(bh / p.H), policy_evict_normal());
     for (int i = 0; i < PU; ++i) {
       const int64_t from = ((i * all + item) * slices + first) * (R::kU / 2);
       bulk_load(s + R::kR + i * kSlab * R::kU, p.rest + from, n * R::kU, bar);
@@ -127,7 +124,8 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
     }
   };
   const KeyLane key_across(false), key_down(true);
-  const int s_down = lane_offset(kSquare, true), s_across = lane_offset(kSquare, false), o_down = lane_offset(16, true);
+  const int s_down = lane_offset(kSquare, true), s_across = lane_offset(kSquare, false);
+  const int o_row = 16 * rb + (l & 15);  // a lane's row of dO's tile as first operand; its piece is l / 16
   const int kk0 = group * NT / 2;  // its first 16 columns of dk
   uint32_t own_down[NT / 2];
 #pragma unroll
@@ -179,17 +177,17 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       }
       const int n = min(kSlab, slices - slab * kSlab);
       const uint32_t base = smem_u32(slabs) + at * R::kSlabBytes;
-      uint32_t a_do = base + 2 * (16 * rb * 16 + o_down), a_r = base + R::kR + rb * 512 + first_lane(), b_r = base + R::kR + (group >> 1) * 512 + second_lane();
+      uint32_t a_r = base + R::kR + rb * 512 + first_lane(), b_r = base + R::kR + (group >> 1) * 512 + second_lane();
       uint32_t b_s = base + R::kS0 + kk0 * 512 + second_lane();
 #pragma unroll 1
-      for (int v = 0; v < n; ++v, a_do += R::kDo, a_r += R::kU, b_r += R::kU, b_s += R::kS) {
+      for (int v = 0; v < n; ++v, a_r += R::kU, b_r += R::kU, b_s += R::kS) {
         uint32_t dO[PX][4], r[PU][4], u[PU][4], f[NT / 2][PS][4], x[R::kBlocks][PU][4];
         if constexpr (PX == 1) {
-          ldsm(dO[0], a_do);
+          ldsm(dO[0], base + row_swizzle(128, o_row, 2 * v + (l >> 4)));
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 t = *reinterpret_cast<const float2*>(slabs + at * R::kSlabBytes + v * R::kDo + 4 * ((16 * rb + row + 8 * (e & 1)) * 16 + 8 * (e >> 1) + col));
+            const float2 t = *reinterpret_cast<const float2*>(slabs + at * R::kSlabBytes + row_swizzle(128, 16 * rb + row + 8 * (e & 1), 4 * v + 2 * (e >> 1) + (col >> 2)) + 4 * (col & 3));
             uint32_t part[PX];
             split<PX>(t.x, t.y, part);
 #pragma unroll
@@ -399,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
         const int t = l * M + i;
         a[i] = e[i] = 0.f;
         float below = 0.f;
-        for (int j = t / 16; j < NB; ++j) below += col_sum[0][j][t] + col_sum[1][j][t];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) below += j >= t / 16 ? col_sum[0][j][t] + col_sum[1][j][t] : 0.f;
         a[i] -= below;
 #pragma unroll
         for (int g = 0; g < R::kGroups; ++g) a[i] += row_sum[g][t] + from_state[g][t], e[i] += to_state[g][t];
@@ -466,25 +465,43 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
         }
       }
     }
-    E* const dq_at = (E*)p.dq.p + b * p.dq.sb + h * p.dq.sh + t0 * p.dq.st + 8 * group * NT + col;
-    E* const dk_at = (E*)p.dk_.p + b * p.dk_.sb + h * p.dk_.sh + t0 * p.dk_.st + 8 * group * NT + col;
+    // bf16: two lanes exchange halves of two tiles, so that each stores four columns of one
+    E* const dq_at = (E*)p.dq.p + b * p.dq.sb + h * p.dq.sh + t0 * p.dq.st;
+    E* const dk_at = (E*)p.dk_.p + b * p.dk_.sb + h * p.dk_.sh + t0 * p.dk_.st;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int t = 16 * rb + row + 8 * half;
-      if (t >= rows) continue;
       E *const to_q = dq_at + (int64_t)t * p.dq.st, *const to_k = dk_at + (int64_t)t * p.dk_.st;
+      if (sizeof(E) == 2 && (pairs & 4)) {
+        const int odd = l & 1;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        store2(to_q + 8 * n, dq[n][2 * half], dq[n][2 * half + 1], p.dk - (8 * (group * NT + n) + col), pairs & 2);
-        store2(to_k + 8 * n, kr[n][2 * half], kr[n][2 * half + 1], p.dk - (8 * (group * NT + n) + col), pairs & 2);
+        for (int n = 0; n < NT; n += 2) {
+          const int d = 8 * (group * NT + n + odd) + col - 2 * odd;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float(&x)[4] = i ? kr[n] : dq[n];
+            const float(&y)[4] = i ? kr[n + 1] : dq[n + 1];
+            const uint32_t mine = pack(x[2 * half], x[2 * half + 1]), next = pack(y[2 * half], y[2 * half + 1]);
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? mine : next, 1);
+            if (t < rows && d < p.dk)
+              *reinterpret_cast<uint2*>((i ? to_k : to_q) + d) = odd ? make_uint2(got, next) : make_uint2(mine, got);
+          }
+        }
+      } else if (t < rows) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int d = 8 * (group * NT + n) + col;
+          store2(to_q + d, dq[n][2 * half], dq[n][2 * half + 1], p.dk - d, pairs & 2);
+          store2(to_k + d, kr[n][2 * half], kr[n][2 * half + 1], p.dk - d, pairs & 2);
+        }
       }
     }
   }
 }
 
-// Rows whose pairs of bf16 can be written at once.
-bool even(const View& v, int width) {
-  return width % 2 == 0 && v.sb % 2 == 0 && v.st % 2 == 0 && v.sh % 2 == 0 && (reinterpret_cast<uintptr_t>(v.p) & 3) == 0;
+// Rows whose numbers can be written n at a time.
+bool whole(const View& v, int width, int n) {
+  return width % n == 0 && v.sb % n == 0 && v.st % n == 0 && v.sh % n == 0 && (reinterpret_cast<uintptr_t>(v.p) & (2 * n - 1)) == 0;
 }
 
 template <typename R>
@@ -498,9 +515,10 @@ int go(const Backward& p, cudaStream_t st) {
   int s;
   if (!p.pre.k && ((s = view_map(&maps.k, p.k, p.B, p.T, p.H, p.dk, 2, 64, R::C)) || (s = view_map(&maps.q, p.q, p.B, p.T, p.H, p.dk, 2, 64, R::C))))
     return s;
-  if (!p.pre.v && (s = view_map(&maps.v, p.d_o, p.B, p.T, p.H, p.dv, sizeof(typename R::E), 16, R::C))) return s;
+  if ((s = value_map(&maps.v, p.pre, p.d_o, p.B, p.T, p.H, p.dv, sizeof(typename R::E), 16 * R::kSlab, R::C))) return s;
   const int64_t items = (int64_t)p.B * p.H * ((p.T + R::C - 1) / R::C);
-  const int pairs = (even(p.dv_, p.dv) ? 1 : 0) | (even(p.dq, p.dk) && even(p.dk_, p.dk) ? 2 : 0);
+  const int pairs = (whole(p.dv_, p.dv, 2) ? 1 : 0) | (whole(p.dq, p.dk, 2) && whole(p.dk_, p.dk, 2) ? 2 : 0) |
+                    (whole(p.dq, p.dk, 4) && whole(p.dk_, p.dk, 4) ? 4 : 0);
   const unsigned grid = (unsigned)(items < sm_count() ? items : sm_count());
   delta_grad_kernel<R><<<grid, kThreads, R::kBytes, st>>>(p, maps, items, pairs);
   DYNCONV_CHECK_LAUNCH("delta_grad_kernel");

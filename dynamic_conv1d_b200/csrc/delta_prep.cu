@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const
     const int dv16 = (dv + 15) / 16 * 16;
     const E* from = (const E*)v.p + b * v.sb + h * v.sh + t0 * v.st;
     for (int i = tid; i < C * dv16; i += kThreads) {
-      const int r = i / 16 % C, c = i / (16 * C) * 16 + i % 16;
+      const int r = i / dv16, c = i % dv16;
       ((E*)to.v)[at * (C * dv16) + i] = r < rows && c < dv ? from[r * v.st + c] : Elem<E>::from_f(0.f);
     }
   }

@@ -51,7 +51,7 @@ struct View {
 // j <= i, of 16 x 16, [B*H][chunks][blocks][parts][512 bytes] in the order in which a warp reads them as second
 // operands; the gates; and copies of k, q and v where the chains cannot have them from tensor maps: k and q as
 // tiles of their parts as they lie in shared memory [B*H][chunks][parts][halves][C][64], v as
-// [B*H][chunks][dv16 / 16][C][16] (dk16, dv16: dk and dv up to multiples of 16).
+// [B*H][chunks * C][dv16] (dv16: dv up to a multiple of 16).
 struct Prepared {
   uint4 *t, *p;
   void* gates;
@@ -314,15 +314,31 @@ inline bool mappable(const View& v, int64_t B, int64_t T, int64_t H, int elem) {
     if (n[i] > 1 && (s[i] <= 0 || s[i] * elem % 16 != 0 || s[i] * elem >= ((int64_t)1 << 40))) return false;
   return true;
 }
-// Tiles of `rows` tokens and 64 (with the swizzle above) or 16 columns of a [B, T, H, width] tensor; fp32 as pairs
-// of 16-bit numbers.
+// A tile of rows of 32, 64 or 128 bytes as a tensor map with the swizzle of that width leaves it: where the 16-byte piece of a
+// row lies.  (32: no swizzle.)
+__device__ __forceinline__ uint32_t row_swizzle(int row_bytes, int r, int piece) {
+  const int turn = row_bytes == 128 ? r & 7 : row_bytes == 64 ? (r >> 1) & 3 : 0;
+  return r * row_bytes + ((piece ^ turn) << 4);
+}
+// Tiles of `rows` tokens and `cols` columns (32, 64 or 128 bytes) of a [B, T, H, width] tensor, swizzled as above; fp32
+// as pairs of 16-bit numbers.
 inline int view_map(CUtensorMap* map, const View& v, int64_t B, int64_t T, int64_t H, int width, int elem, int cols, int rows) {
   const int per = elem / 2;
   const cuuint64_t dims[4] = {(cuuint64_t)(width * per), (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
   const cuuint64_t strides[3] = {(cuuint64_t)(H > 1 ? v.sh * elem : 16), (cuuint64_t)(T > 1 ? v.st * elem : 16),
                                  (cuuint64_t)(B > 1 ? v.sb * elem : 16)};
   const cuuint32_t box[4] = {(cuuint32_t)(cols * per), 1, (cuuint32_t)rows, 1};
-  return encode_tensor_map_bf16(map, v.p, 4, dims, strides, box, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+  const int bytes = cols * elem;
+  return encode_tensor_map_bf16(map, v.p, 4, dims, strides, box,
+                                bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                              : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+// The same of v or dO, from the tensor or from its copy.
+inline int value_map(CUtensorMap* map, const Prepared& pre, const View& v, int64_t B, int64_t T, int64_t H, int dv, int elem, int cols, int C) {
+  if (!pre.v) return view_map(map, v, B, T, H, dv, elem, cols, C);
+  const int64_t dv16 = (dv + 15) / 16 * 16, all = (T + C - 1) / C * C;
+  return view_map(map, View{pre.v, H * all * dv16, dv16, all * dv16}, B, all, H, (int)dv16, elem, cols, C);
 }
 struct Maps {
   CUtensorMap k, q, v;  // (v: or dO)

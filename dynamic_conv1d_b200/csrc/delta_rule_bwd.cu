@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
   uint4* const state = (uint4*)(smem + plan.stages * bytes + team * Ch::kTeam);
   uint4 *const part_x = state + Ch::kState / 16, *const part_o = part_x + Ch::kBlock / 16, *const part_u = part_o + Ch::kBlock / 16;
   const KeyLane across(false);
-  const int v_across = lane_offset(16, false);
+  const int v_row = (l & 7) + 8 * (l >> 4), v_piece = l >> 3 & 1;
   uint32_t down[NT / 2];  // this warp's columns of K and Q, 16 at a time
   {
     const KeyLane lane(true);
@@ -86,14 +86,14 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       if constexpr (sizeof(E) == 2) {
-        ldsm_t(dO[j][0], smem_u32(s.v(team) + 16 * j * 16 + v_across));
+        ldsm_t(dO[j][0], smem_u32(s.v(team, 16 * j + v_row, v_piece)));
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd = fmaf(low(dO[j][0][e]), 0.f, fmaf(high(dO[j][0][e]), 0.f, odd));
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const E* at = s.v(team) + (16 * j + 8 * (e >> 1) + col) * 16 + row + 8 * (e & 1);
-          const float x = at[0], y = at[16];
+          const int t = 16 * j + 8 * (e >> 1) + col, d = row + 8 * (e & 1);
+          const float x = s.value(team, t, d), y = s.value(team, t + 1, d);
           odd = fmaf(x, 0.f, fmaf(y, 0.f, odd));
           uint32_t part[PX];
           split<PX>(x, y, part);
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
     }
     int bad = 0;  // tokens up to the last one of dO that is not finite
     if (__any_sync(0xffffffffu, !(odd == 0.f))) {  // (rare) must not meet the zeros of P: counts as zero, and makes NaN at the end
-      bad = Ch::bad_row(s.v(team), true);
+      bad = Ch::bad_row(s, team, true);
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -286,7 +286,7 @@ int go(const Backward& p, const Plan& plan, cudaStream_t st) {
     return cuda_status(e, "cudaFuncSetAttribute(delta_bwd)");
   }
   Maps maps{};
-  if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.d_o, p.B, p.T, p.H, p.dk, p.dv))) return s;
+  if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.d_o, p.B, p.T, p.H, p.dk, p.dv, plan.teams))) return s;
   const dim3 grid((unsigned)((slices + plan.teams - 1) / plan.teams), (unsigned)(p.B * p.H));
   delta_bwd_kernel<G, W, KK><<<grid, 32 * (plan.teams * W + plan.own_warp), smem, st>>>(p, maps, plan);
   DYNCONV_CHECK_LAUNCH("delta_bwd_kernel");

@@ -6,13 +6,6 @@ namespace dynconv {
 namespace dr {
 namespace {
 
-// 16 rows x 16 columns, staged in shared memory, to the output.
-template <typename E>
-__device__ __noinline__ void store_slow(const E* tile, E* to, int64_t step, int rows, int cols) {
-  for (int i = threadIdx.x & 31; i < 16 * rows; i += 32)
-    if (i % 16 < cols) to[i / 16 * step + i % 16] = tile[i];
-}
-
 template <typename G, int W, int KK, bool SAVE>
 __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_kernel(Forward p, const __grid_constant__ Maps maps, Plan plan) {
   using Ch = Chain<G, W, KK>;
@@ -40,7 +33,8 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
   uint4* const state = (uint4*)(smem + plan.stages * bytes + team * Ch::kTeam);
   uint4 *const part_r = state + Ch::kState / 16, *const part_u = part_r + Ch::kBlock / 16, *const part_s = part_u + Ch::kBlock / 16;
   const KeyLane across(false);
-  const int v_across = lane_offset(16, false);
+  // (the row and piece of a lane in transposed reads and writes of a team's bf16 columns, 16 tokens at a time)
+  const int v_row = (l & 7) + 8 * (l >> 4), v_piece = l >> 3 & 1;
   uint32_t down[NT / 2];  // this warp's columns of K, 16 at a time
   {
     const KeyLane lane(true);
@@ -132,7 +126,6 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
       for (int t = 0; t < TB; ++t) sum_levels<L>(Z[t], z[t]), sum_levels<L>(O[t], o[t]);
     }
     // (V - e^b K S0)^T in Z's place, O scaled
-    E* const v_tile = s.v(team);
     float odd = 0.f;  // NaN if a value is not finite
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
@@ -140,13 +133,13 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
       float v[2][4];
       if constexpr (sizeof(E) == 2) {
         uint32_t f[4];
-        ldsm_t(f, smem_u32(v_tile + t0 * 16 + v_across));
+        ldsm_t(f, smem_u32(s.v(team, t0 + v_row, v_piece)));
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i >> 1][2 * (i & 1)] = low(f[i]), v[i >> 1][2 * (i & 1) + 1] = high(f[i]);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          v[i >> 2][i & 3] = v_tile[(t0 + 8 * (i >> 2) + col + (i & 1)) * 16 + row + 8 * ((i >> 1) & 1)];
+          v[i >> 2][i & 3] = s.value(team, t0 + 8 * (i >> 2) + col + (i & 1), row + 8 * ((i >> 1) & 1));
       }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -162,7 +155,7 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
     const bool odd_here = __any_sync(0xffffffffu, !(odd == 0.f));
     if (bad < C || odd_here) {  // (rare)
       // What is not finite must not meet the zeros of T and P: values from the first bad token on count as zero.
-      bad = min(bad, Ch::bad_row(v_tile, false));
+      bad = min(bad, Ch::bad_row(s, team, false));
 #pragma unroll
       for (int t = 0; t < TB; ++t)
 #pragma unroll
@@ -179,7 +172,7 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
     }
     // (another warp's tokens may be the bad ones)
     if (produces && c > 0) producer.template refill<false>(c);
-    if (!Ch::team_all(team, !odd_here)) bad = min(bad, Ch::bad_row(v_tile, false));
+    if (!Ch::team_all(team, !odd_here)) bad = min(bad, Ch::bad_row(s, team, false));
     // r^T = (V - e^b K S0)^T T^T, U = beta r
     float U[TB][2][4];
 #pragma unroll
@@ -290,16 +283,16 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
       const int64_t t0 = (int64_t)c * C + 16 * blk;
       const int rows = (int)(p.T - t0 < 16 ? p.T - t0 : 16);
       E* const to = (E*)p.o.p + b * p.o.sb + h * p.o.sh + t0 * p.o.st + d0;
-      E* const stage_o = v_tile + 16 * blk * 16;
       if constexpr (sizeof(E) == 2) {
-        stsm_t(smem_u32(stage_o + v_across), pack(O[t][0][0], O[t][0][1]), pack(O[t][0][2], O[t][0][3]),
+        stsm_t(smem_u32(s.v(team, 16 * blk + v_row, v_piece)), pack(O[t][0][0], O[t][0][1]), pack(O[t][0][2], O[t][0][3]),
                pack(O[t][1][0], O[t][1][1]), pack(O[t][1][2], O[t][1][3]));
         __syncwarp();
         if (plan.o_vectors) {
           const int r = l >> 1, d = (l & 1) * 8;
-          if (r < rows && d0 + d < p.dv) *reinterpret_cast<uint4*>(to + r * p.o.st + d) = *reinterpret_cast<const uint4*>(stage_o + r * 16 + d);
+          if (r < rows && d0 + d < p.dv) *reinterpret_cast<uint4*>(to + r * p.o.st + d) = *reinterpret_cast<const uint4*>(s.v(team, 16 * blk + r, l & 1));
         } else {
-          store_slow(stage_o, to, p.o.st, rows, p.dv - d0);
+          for (int i = l; i < 16 * rows; i += 32)
+            if (d0 + i % 16 < p.dv) to[i / 16 * p.o.st + i % 16] = s.value(team, 16 * blk + i / 16, i % 16);
         }
       } else {
 #pragma unroll
@@ -340,7 +333,7 @@ int go(const Forward& p, Plan plan, cudaStream_t st) {
     return cuda_status(e, "cudaFuncSetAttribute(delta_fwd)");
   }
   Maps maps{};
-  if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.v, p.B, p.T, p.H, p.dk, p.dv))) return s;
+  if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.v, p.B, p.T, p.H, p.dk, p.dv, plan.teams))) return s;
   const dim3 grid((unsigned)((slices + plan.teams - 1) / plan.teams), (unsigned)(p.B * p.H));
   delta_fwd_kernel<G, W, KK, SAVE><<<grid, 32 * (plan.teams * W + plan.own_warp), smem, st>>>(p, maps, plan);
   DYNCONV_CHECK_LAUNCH("delta_fwd_kernel");
