@@ -45,18 +45,27 @@ __device__ __forceinline__ uint32_t first_lane() {
   return ((l >> 4 & 1) + (l >> 2 & 2)) * 128 + (l & 7) * 16;
 }
 
+// (out of line: the kernel has to stay in the instruction cache)
+template <typename E>
+__device__ __noinline__ void store2_slow(E* to, float x, float y, int n) {
+  if (n > 0) to[0] = Elem<E>::from_f(x);
+  if (n > 1) to[1] = Elem<E>::from_f(y);
+}
 template <typename E>
 __device__ __forceinline__ void store2(E* to, float x, float y, int n, bool pairs) {
-  if (sizeof(E) == 2 && pairs) {
-    if (n > 0) *reinterpret_cast<uint32_t*>(to) = pack(x, y);
+  if (pairs) {
+    if (n <= 0) return;
+    if constexpr (sizeof(E) == 2)
+      *reinterpret_cast<uint32_t*>(to) = pack(x, y);
+    else
+      *reinterpret_cast<float2*>(to) = make_float2(x, y);
   } else {
-    if (n > 0) to[0] = Elem<E>::from_f(x);
-    if (n > 1) to[1] = Elem<E>::from_f(y);
+    store2_slow(to, x, y, n);
   }
 }
 
 template <typename R>
-__global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, const __grid_constant__ Maps maps, int64_t items, int pairs) {
+__global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, const __grid_constant__ Maps maps, int items, int pairs) {
   constexpr int PX = R::PX, C = R::C, NB = R::NB, PU = R::PU, PS = R::PS, kSlab = R::kSlab, kSquare = R::kSquare;
   constexpr int NT = R::NT, KK = R::KK, KX = PX > PS ? PX : PS, KS = PU > PS ? PU : PS;
   using E = typename R::E;
@@ -84,21 +93,31 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
   }
   __syncthreads();
   // (one thread)
-  auto load_slab = [&](int64_t item, int slab, int at) {
-    const int64_t bh = item / chunks;
-    const int c = (int)(item % chunks), first = slab * kSlab, n = min(kSlab, slices - first);
+  // Items count heads first, then chunks: neighbouring SMs read neighbouring heads of the same tokens, whole pages of DRAM.
+  auto place = [&](int item, int& b, int& h, int& c) {
+    h = item % p.H;
+    c = item / p.H % chunks, b = item / p.H / chunks;
+    return (int64_t)(b * p.H + h) * chunks + c;  // among what the chains left
+  };
+  auto load_slab = [&](int nth, int slab, int at) {
+    int b, h, c;
+    const int64_t item = place(nth, b, h, c);
+    const int first = slab * kSlab, n = min(kSlab, slices - first);
     uint8_t* const s = slabs + at * R::kSlabBytes;
     uint64_t* const bar = &slab_full[at];
     const uint32_t state = n * n_k16 * 512;
     mbar_arrive_expect_tx(bar, kSlab * R::kDo + n * 2 * PU * R::kU + 2 * PS * state);
-    tma_load_4d(s, &maps.v, bar, first * 16 * (int)(sizeof(E) / 2), (int)(bh % p.H), c * C, (int)(bh / p.H), policy_evict_normal());
+    tma_load_4d(s, &maps.v, bar, first * 16 * (int)(sizeof(E) / 2), h, c * C, b, policy_evict_normal());
+#pragma unroll 1
     for (int i = 0; i < PU; ++i) {
       const int64_t from = ((i * all + item) * slices + first) * (R::kU / 2);
       bulk_load(s + R::kR + i * kSlab * R::kU, p.rest + from, n * R::kU, bar);
       bulk_load(s + R::kDu + i * kSlab * R::kU, p.du + from, n * R::kU, bar);
     }
+#pragma unroll 1
     for (int i = 0; i < PS; ++i) {
       const int64_t from = ((i * all + item) * slices + first) * n_k16 * 256;
+#pragma unroll 1
       for (int v = 0; v < (n_k16 == KK ? 1 : n); ++v) {  // (slices lie KK pieces apart)
         const uint32_t one = n_k16 == KK ? state : n_k16 * 512;
         bulk_load(s + R::kS0 + (i * kSlab + v) * R::kS, p.states + from + v * n_k16 * 256, one, bar);
@@ -106,9 +125,9 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       }
     }
   };
-  auto load_kq = [&](int64_t item) {
-    const int64_t bh = item / chunks;
-    const int c = (int)(item % chunks);
+  auto load_kq = [&](int nth) {
+    int b, h, c;
+    const int64_t item = place(nth, b, h, c);
     mbar_arrive_expect_tx(&kq_full, 2 * PX * halves * C * 128);
     if (p.pre.k) {
       for (int i = 0; i < PX; ++i) {
@@ -118,8 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       }
     } else {
       for (int d = 0; d < halves; ++d) {
-        tma_load_4d(k_tile + d * C * 128, &maps.k, &kq_full, 64 * d, (int)(bh % p.H), c * C, (int)(bh / p.H), policy_evict_normal());
-        tma_load_4d(q_tile + d * C * 128, &maps.q, &kq_full, 64 * d, (int)(bh % p.H), c * C, (int)(bh / p.H), policy_evict_normal());
+        tma_load_4d(k_tile + d * C * 128, &maps.k, &kq_full, 64 * d, h, c * C, b, policy_evict_normal());
+        tma_load_4d(q_tile + d * C * 128, &maps.q, &kq_full, 64 * d, h, c * C, b, policy_evict_normal());
       }
     }
   };
@@ -134,13 +153,10 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
     own_down[m] = key_swizzle((l & 7) + 8 * (l >> 3 & 1), (2 * kk & 7) + (l >> 4)) + (kk >> 2) * (C * 128);
   }
 
-  int64_t item = blockIdx.x;
-  if (item >= items) return;
-  int n_loaded = 0;  // slabs so far
-  if (tid == 0) load_slab(item, 0, 0);
-  for (int done = 0; item < items; item += gridDim.x, ++done) {
-    const int64_t bh = item / chunks, b = bh / p.H, h = bh % p.H;
-    const int c = (int)(item % chunks);
+  int n_loaded = -1;  // slabs worked on (-1: before the first one's load)
+  for (int nth = blockIdx.x, done = 0; nth < items; nth += gridDim.x, ++done) {
+    int b_, h_, c;
+    const int64_t item = place(nth, b_, h_, c), b = b_, h = h_;
     const int64_t t0 = (int64_t)c * C;
     const int rows = (int)(p.T - t0 < C ? p.T - t0 : C);
     E* const dv_at = (E*)p.dv_.p + b * p.dv_.sb + h * p.dv_.sh + t0 * p.dv_.st;
@@ -155,9 +171,9 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
 #pragma unroll
     for (int j = 0; j < R::kBlocks; ++j) zero(X[j][0]), zero(X[j][1]);
     zero(dot[0]), zero(dot[1]);
-    for (int slab = 0; slab < n_slabs; ++slab, ++n_loaded) {
+    for (int slab = n_loaded < 0 ? -1 : 0; slab < n_slabs; ++slab, ++n_loaded) {
       const int at = n_loaded & 1;
-      if (!__syncthreads_and(mbar_wait(&slab_full[at], (n_loaded >> 1) & 1, kErrWaitMma, &abort_flag))) {
+      if (n_loaded >= 0 && !__syncthreads_and(mbar_wait(&slab_full[at], (n_loaded >> 1) & 1, kErrWaitMma, &abort_flag))) {
         if (tid == 0) {  // (what is in flight lands before the shared memory goes)
           mbar_drain(&slab_full[at], (n_loaded >> 1) & 1);
           if (slab > 0) mbar_drain(&kq_full, done & 1);
@@ -165,12 +181,11 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
         return;
       }
       if (tid == 0) {  // (everybody is done with the other slab, and with the keys of the item before)
-        if (slab == 0) load_kq(item);
-        if (slab + 1 < n_slabs)
-          load_slab(item, slab + 1, at ^ 1);
-        else if (item + gridDim.x < items)
-          load_slab(item + gridDim.x, 0, at ^ 1);
+        if (slab == 0) load_kq(nth);
+        const int next = slab + 1 < n_slabs ? nth : nth + (int)gridDim.x;
+        if (next < items) load_slab(next, slab + 1 < n_slabs ? slab + 1 : 0, at ^ 1);
       }
+      if (slab < 0) continue;
       if (slab == 0) {
         const uint4* g = (const uint4*)p.pre.gates + item * (sizeof(Gates<C>) / 16);
         for (int i = tid; i < (int)sizeof(Gates<C>) / 16; i += kThreads) ((uint4*)&gate)[i] = g[i];
@@ -279,23 +294,31 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
 #pragma unroll
       for (int n = 0; n < R::kBlocks; ++n) zero(Y[n][0]), zero(Y[n][1]);
       const uint32_t a_at = is_n ? k_at : q_at;
+#pragma unroll 1
+      for (int hf = 0; hf < halves; ++hf)
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        uint32_t a[PX][4];
+        for (int kk = 0; kk < 4; ++kk) {
+          uint32_t a[PX][4];
 #pragma unroll
-        for (int i = 0; i < PX; ++i) ldsm(a[i], a_at + 2 * i * R::kTile + key_down.at<C>(rb, kk));
+          for (int i = 0; i < PX; ++i) ldsm(a[i], a_at + hf * (C * 128) + 2 * i * R::kTile + key_down.at<C>(rb, kk));
 #pragma unroll
-        for (int n = 0; n < R::kBlocks; ++n) {
-          const int j = (group >> 1) + n * R::kStep;
-          if (j > rb) continue;
-          uint32_t f[PX][4];
+          for (int n = 0; n < R::kBlocks; ++n) {
+            const int j = (group >> 1) + n * R::kStep;
+            if (j > rb) continue;
+            uint32_t f[PX][4];
 #pragma unroll
-          for (int i = 0; i < PX; ++i) ldsm(f[i], k_at + 2 * i * R::kTile + key_across.at<C>(j, kk));
-          mma_parts<PX, PX, PX>(Y[n][0], Y[n][1], a, f);
+            for (int i = 0; i < PX; ++i) ldsm(f[i], k_at + hf * (C * 128) + 2 * i * R::kTile + key_across.at<C>(j, kk));
+            mma_parts<PX, PX, PX>(Y[n][0], Y[n][1], a, f);
+          }
         }
+      // the gates, for all blocks before the first is written: loads do not pass stores
+      float f_r[2], hi_r[2], lo_r[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = 16 * rb + row + 8 * half;
+        f_r[half] = is_n ? -gate.beta[r] : p.scale, hi_r[half] = gate.hi[r], lo_r[half] = gate.lo[r];
       }
-      __nv_bfloat16* const out = is_n ? N : W;
-      float sums[2] = {0.f, 0.f};
+      float sums[2] = {0.f, 0.f}, below[R::kBlocks][2][2], own[2] = {0.f, 0.f};
 #pragma unroll
       for (int jn = 0; jn < R::kBlocks; ++jn) {
         const int j = (group >> 1) + jn * R::kStep;
@@ -305,33 +328,58 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
           const int cc = 16 * j + 8 * n + col;
           const float2 hi = *reinterpret_cast<const float2*>(gate.hi + cc), lo = *reinterpret_cast<const float2*>(gate.lo + cc);
           const float2 beta = *reinterpret_cast<const float2*>(gate.beta + cc);
-          float below[2] = {0.f, 0.f};
+          below[jn][n][0] = below[jn][n][1] = 0.f;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int r = 16 * rb + row + 8 * half;
-            const float f = is_n ? -gate.beta[r] : p.scale;
-            float x = X[jn][n][2 * half], y = X[jn][n][2 * half + 1];
-            if (is_n && (cc == r || cc + 1 == r) && r < rows)
-              ((E*)p.dbeta.p)[b * p.dbeta.sb + h * p.dbeta.sh + (t0 + r) * p.dbeta.st] = Elem<E>::from_f(cc == r ? x : y);
-            x *= f * beta.x * exp2_fast((gate.hi[r] - hi.x) + (gate.lo[r] - lo.x));
-            y *= f * beta.y * exp2_fast((gate.hi[r] - hi.y) + (gate.lo[r] - lo.y));
+            float &x = X[jn][n][2 * half], &y = X[jn][n][2 * half + 1];
+            own[half] = cc == r ? x : cc + 1 == r ? y : own[half];
+            x *= f_r[half] * beta.x * exp2_fast((hi_r[half] - hi.x) + (lo_r[half] - lo.x));
+            y *= f_r[half] * beta.y * exp2_fast((hi_r[half] - hi.y) + (lo_r[half] - lo.y));
             const int last = is_n ? r - 1 : r;
             x = cc <= last ? x : 0.f, y = cc < last ? y : 0.f;
-            uint32_t part[PX];
-            split<PX>(x, y, part);
-#pragma unroll
-            for (int i = 0; i < PX; ++i) *reinterpret_cast<uint32_t*>(out + i * C * kSquare + r * kSquare + cc) = part[i];
             // (a token's own term does not depend on the decays)
             const float mx = cc < r ? x * Y[jn][n][2 * half] : 0.f, my = cc + 1 < r ? y * Y[jn][n][2 * half + 1] : 0.f;
             sums[half] += mx + my;
-            below[0] += mx, below[1] += my;
+            below[jn][n][0] += mx, below[jn][n][1] += my;
           }
+        }
+      }
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            below[0] += __shfl_xor_sync(0xffffffffu, below[0], d);
-            below[1] += __shfl_xor_sync(0xffffffffu, below[1], d);
+      for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+        for (int jn = 0; jn < R::kBlocks; ++jn)
+          if ((group >> 1) + jn * R::kStep <= rb)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              below[jn][n][0] += __shfl_xor_sync(0xffffffffu, below[jn][n][0], d);
+              below[jn][n][1] += __shfl_xor_sync(0xffffffffu, below[jn][n][1], d);
+            }
+      __nv_bfloat16* const out = (is_n ? N : W) + (16 * rb + row) * kSquare + col;
+#pragma unroll
+      for (int jn = 0; jn < R::kBlocks; ++jn) {
+        const int j = (group >> 1) + jn * R::kStep;
+        if (j > rb) continue;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int cc = 16 * j + 8 * n;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t part[PX];
+            split<PX>(X[jn][n][2 * half], X[jn][n][2 * half + 1], part);
+#pragma unroll
+            for (int i = 0; i < PX; ++i) *reinterpret_cast<uint32_t*>(out + i * C * kSquare + 8 * half * kSquare + cc) = part[i];
           }
-          if (row == 0) col_sum[is_n][rb][cc] = below[0], col_sum[is_n][rb][cc + 1] = below[1];
+          if (row == 0) *reinterpret_cast<float2*>(&col_sum[is_n][rb][cc + col]) = make_float2(below[jn][n][0], below[jn][n][1]);
+        }
+      }
+      // dbeta: the diagonal of dU r^T
+      if (is_n && (rb - (group >> 1)) % R::kStep == 0 && rb >= (group >> 1)) {
+        E* const db = (E*)p.dbeta.p + b * p.dbeta.sb + h * p.dbeta.sh + t0 * p.dbeta.st;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int r = 16 * rb + row + 8 * half, c = (row + 8 * half) & 7;  // (the lane that holds column r)
+          if ((c >> 1) == (l & 3) && r < rows) db[r * p.dbeta.st] = Elem<E>::from_f(own[half]);
         }
       }
 #pragma unroll
@@ -431,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       }
     }
     // dQ += W K, dK += W^T Q + (N + N^T) K
-#pragma unroll
+#pragma unroll 1
     for (int j = 0; j < NB; ++j) {
       uint32_t wa[PX][4], na[PX][4], wt[PX][4], nt[PX][4];
 #pragma unroll
@@ -500,8 +548,8 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
 }
 
 // Rows whose numbers can be written n at a time.
-bool whole(const View& v, int width, int n) {
-  return width % n == 0 && v.sb % n == 0 && v.st % n == 0 && v.sh % n == 0 && (reinterpret_cast<uintptr_t>(v.p) & (2 * n - 1)) == 0;
+bool whole(const View& v, int width, int n, int elem) {
+  return width % n == 0 && v.sb % n == 0 && v.st % n == 0 && v.sh % n == 0 && (reinterpret_cast<uintptr_t>(v.p) & (n * elem - 1)) == 0;
 }
 
 template <typename R>
@@ -517,10 +565,12 @@ int go(const Backward& p, cudaStream_t st) {
     return s;
   if ((s = value_map(&maps.v, p.pre, p.d_o, p.B, p.T, p.H, p.dv, sizeof(typename R::E), 16 * R::kSlab, R::C))) return s;
   const int64_t items = (int64_t)p.B * p.H * ((p.T + R::C - 1) / R::C);
-  const int pairs = (whole(p.dv_, p.dv, 2) ? 1 : 0) | (whole(p.dq, p.dk, 2) && whole(p.dk_, p.dk, 2) ? 2 : 0) |
-                    (whole(p.dq, p.dk, 4) && whole(p.dk_, p.dk, 4) ? 4 : 0);
+  if (items > INT32_MAX - 65536) return set_error(DYNCONV_ERR_SHAPE, "gated delta rule: B*H*T too large");
+  const int elem = sizeof(typename R::E);
+  const int pairs = (whole(p.dv_, p.dv, 2, elem) ? 1 : 0) | (whole(p.dq, p.dk, 2, elem) && whole(p.dk_, p.dk, 2, elem) ? 2 : 0) |
+                    (whole(p.dq, p.dk, 4, elem) && whole(p.dk_, p.dk, 4, elem) ? 4 : 0);
   const unsigned grid = (unsigned)(items < sm_count() ? items : sm_count());
-  delta_grad_kernel<R><<<grid, kThreads, R::kBytes, st>>>(p, maps, items, pairs);
+  delta_grad_kernel<R><<<grid, kThreads, R::kBytes, st>>>(p, maps, (int)items, pairs);
   DYNCONV_CHECK_LAUNCH("delta_grad_kernel");
   return DYNCONV_OK;
 }

@@ -231,41 +231,69 @@ struct Scores {
     }
   }
 
+  // Applies the gates, all blocks before the first is written: loads do not pass stores.
   template <bool BACK>
-  __device__ __forceinline__ void write(const Gates<C>& s, float scale, __nv_bfloat16* t, float* diag, __nv_bfloat16* p_out) const {
+  __device__ __forceinline__ void scale(const Gates<C>& s, float scale) {
     if (idle()) return;
+    float hi_r[2][2], lo_r[2][2], beta_r[2][2];  // of the two row blocks
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = 16 * (b ? i1 : i0) + row + 8 * half;
+        hi_r[b][half] = s.hi[r], lo_r[b][half] = s.lo[r], beta_r[b][half] = is_p ? scale : s.beta[r];
+      }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       const int i = u <= i0 ? i0 : i1, j = block_of(u);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = 16 * i + row + 8 * half, last = is_p ? r : r - 1;  // the last column that counts
-        const float hi_r = s.hi[r], lo_r = s.lo[r], beta_r = is_p ? scale : s.beta[r];
+      for (int n = 0; n < 2; ++n) {
+        const int c = 16 * j + 8 * n + col;
+        const float2 hi = *reinterpret_cast<const float2*>(s.hi + c), lo = *reinterpret_cast<const float2*>(s.lo + c);
+        const float2 beta = *reinterpret_cast<const float2*>(s.beta + c);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int r = 16 * i + row + 8 * half, last = is_p ? r : r - 1;  // the last column that counts
+          // (block 0 is of the first row block, blocks from 2 on of the second)
+          const bool b1 = u >= 2 || (u == 1 && i0 == 0);
+          const float h = b1 ? hi_r[1][half] : hi_r[0][half], l = b1 ? lo_r[1][half] : lo_r[0][half];
+          const float f = b1 ? beta_r[1][half] : beta_r[0][half];
+          float &x = X[u][n][2 * half], &y = X[u][n][2 * half + 1];
+          x *= (BACK || is_p ? f : beta.x) * exp2_fast((h - hi.x) + (l - lo.x));
+          y *= (BACK || is_p ? f : beta.y) * exp2_fast((h - hi.y) + (l - lo.y));
+          x = c <= last ? x : 0.f, y = c < last ? y : 0.f;
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void write(__nv_bfloat16* t, float* diag, __nv_bfloat16* p_out) const {
+    if (idle()) return;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int i = u <= i0 ? i0 : i1, j = block_of(u);
+      __nv_bfloat16* const to = is_p ? p_out + (16 * i + row) * kS + 16 * j + col : t + (16 * j + row) * kS + 16 * i + col;
+      float* const to_diag = diag + i * 256 + row * 16 + col;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const int c = 16 * j + 8 * n + col;
-          const float2 hi = *reinterpret_cast<const float2*>(s.hi + c), lo = *reinterpret_cast<const float2*>(s.lo + c);
-          const float2 beta = *reinterpret_cast<const float2*>(s.beta + c);
-          float x = X[u][n][2 * half], y = X[u][n][2 * half + 1];
-          x *= (BACK || is_p ? beta_r : beta.x) * exp2_fast((hi_r - hi.x) + (lo_r - lo.x));
-          y *= (BACK || is_p ? beta_r : beta.y) * exp2_fast((hi_r - hi.y) + (lo_r - lo.y));
-          x = c <= last ? x : 0.f, y = c < last ? y : 0.f;
+          const float x = X[u][n][2 * half], y = X[u][n][2 * half + 1];
+          const int at = 8 * half * kS + 8 * n;
           if (is_p) {
             uint32_t p[G::PP];
             split<G::PP>(x, y, p);
 #pragma unroll
-            for (int e = 0; e < G::PP; ++e) *reinterpret_cast<uint32_t*>(p_out + e * kPart + r * kS + c) = p[e];
+            for (int e = 0; e < G::PP; ++e) *reinterpret_cast<uint32_t*>(to + e * kPart + at) = p[e];
           } else if (j == i) {
-            *reinterpret_cast<float2*>(diag + i * 256 + (row + 8 * half) * 16 + 8 * n + col) = make_float2(x, y);
+            *reinterpret_cast<float2*>(to_diag + 8 * half * 16 + 8 * n) = make_float2(x, y);
           } else {
             uint32_t p[G::NP];
             split<G::NP>(x, y, p);
 #pragma unroll
-            for (int e = 0; e < G::NP; ++e)
-              *reinterpret_cast<uint32_t*>(t + e * kPart + (16 * j + row + 8 * half) * kS + 16 * i + 8 * n + col) = p[e];
+            for (int e = 0; e < G::NP; ++e) *reinterpret_cast<uint32_t*>(to + e * kPart + at) = p[e];
           }
         }
-      }
     }
   }
 };
@@ -291,7 +319,9 @@ __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const
   float* const diag = (float*)(smem + 2 * PrepSmem<G>::kSpace);
   Gates<C>& s = *(Gates<C>*)(diag + NB * 256);
   const int tid = threadIdx.x, lane = tid & 31, w = warp_index(), n_k16 = (dk + 15) / 16, halves = dk > 64 ? 2 : 1;
-  const int64_t bh = blockIdx.y, b = bh / H, h = bh % H, chunk = blockIdx.x, t0 = chunk * C, at = bh * gridDim.x + chunk;
+  // (heads first: CTAs that run together read neighbouring heads of the same tokens, whole pages of DRAM)
+  const int64_t h = blockIdx.x % H, chunk = blockIdx.x / H, b = blockIdx.y, bh = b * H + h, t0 = chunk * C;
+  const int64_t at = bh * ((T + C - 1) / C) + chunk;
   const int rows = (int)(T - t0 < C ? T - t0 : C);
   if (to.k) {
 #pragma unroll 1
@@ -357,7 +387,8 @@ __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const
     }
     __syncthreads();
   }
-  scores.template write<BACK>(s, scale, t, diag, p);
+  scores.template scale<BACK>(s, scale);
+  scores.write(t, diag, p);
   if (to.v) {
     const int dv16 = (dv + 15) / 16 * 16;
     const E* from = (const E*)v.p + b * v.sb + h * v.sh + t0 * v.st;
@@ -403,7 +434,9 @@ int go(const Prepared& to, const View& k, const View& q, const View& v, const Vi
     int s;
     if ((s = view_map(&maps.k, k, B, T, H, dk, 2, 64, G::C)) || (s = view_map(&maps.q, q, B, T, H, dk, 2, 64, G::C))) return s;
   }
-  const dim3 grid((unsigned)((T + G::C - 1) / G::C), (unsigned)(B * H));
+  const int64_t blocks = (T + G::C - 1) / G::C * H;
+  if (blocks > INT32_MAX) return set_error(DYNCONV_ERR_SHAPE, "gated delta rule: H*T too large");
+  const dim3 grid((unsigned)blocks, (unsigned)B);
   delta_prep_kernel<G, BACK><<<grid, kThreads, PrepSmem<G>::kBytes, st>>>(to, maps, k, q, v, g, beta, H, T, dk, dv, scale);
   DYNCONV_CHECK_LAUNCH("delta_prep_kernel");
   return DYNCONV_OK;
