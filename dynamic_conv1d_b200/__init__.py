@@ -24,10 +24,12 @@ from .headwise import headwise_dynamic_convolution
 from .linear_attention import decay_linear_attention, decay_linear_attention_fused, decay_linear_attention_step
 from .lowrank import lowrank_dynamic_convolution, lowrank_dynamic_convolution_grouped
 from .modules import (
+    ConvolvedGatedDelta,
     ConvolvedLinearAttention,
     LayerCache,
     LowRankDynamicShortConvolution,
     QKVLowRankDynamicShortConvolution,
+    ResidualRMSNorm,
 )
 from .norm import gated_rms_norm, residual_rms_norm
 from .parallel import data_parallel, shard_rows
@@ -59,6 +61,8 @@ __all__ = [
     "LowRankDynamicShortConvolution",
     "QKVLowRankDynamicShortConvolution",
     "ConvolvedLinearAttention",
+    "ConvolvedGatedDelta",
+    "ResidualRMSNorm",
     "LayerCache",
     "data_parallel",
     "lowrank_dynamic_convolution_sp",

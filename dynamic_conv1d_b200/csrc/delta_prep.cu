@@ -456,7 +456,7 @@ size_t prepared_bytes(Prepared* p, void* base, int64_t B, int64_t T, int64_t H, 
   };
   Prepared out{};
   out.t = (uint4*)take(n * pairs * 3 * 512);  // (two parts or three: three fit either)
-  out.p = (uint4*)take(n * pairs * (f32 ? 3 : back ? 2 : 1) * 512);
+  out.p = (uint4*)take(n * pairs * (f32 ? 3 : 2) * 512);
   out.gates = take(n * (f32 ? sizeof(Gates<32>) : sizeof(Gates<64>)));
   if (packs_keys(dk, dtype)) {
     out.k = (__nv_bfloat16*)take(n * (f32 ? 3 : 1) * C * dk64 * 2);

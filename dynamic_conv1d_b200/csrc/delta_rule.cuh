@@ -270,9 +270,9 @@ struct Cfg {
   static constexpr int kSquare = C + 8;   // pitch of a C x C matrix
   static constexpr int kTile = C * kMaxKey;  // elements of one part of K or Q
 };
-// P has one part in the forward (its product is rounded to bf16 next) and two in the backward.
+// P has two parts in bf16 too: with one, the outputs were 2.5e-3 off in the root mean square, where their own rounding is 1.65e-3.
 template <bool EXACT, bool BACK>
-using CfgBf16 = Cfg<1, EXACT ? 3 : 2, BACK ? 2 : 1, 64>;
+using CfgBf16 = Cfg<1, EXACT ? 3 : 2, 2, 64>;
 using CfgF32 = Cfg<3, 3, 3, 32>;
 __host__ __device__ constexpr int lower(int i, int j) { return i * (i + 1) / 2 + j; }
 

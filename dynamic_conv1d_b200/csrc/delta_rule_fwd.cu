@@ -244,7 +244,11 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
 #pragma unroll
       for (int m = 0; m < NX; ++m)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) S[n + m][e] = bad < C ? NAN : fmaf(total, S[n + m][e], x[m][e]);
+        for (int e = 0; e < 4; ++e) S[n + m][e] = fmaf(total, S[n + m][e], x[m][e]);
+    }
+    if (bad < C) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) S[n][0] = S[n][1] = S[n][2] = S[n][3] = NAN;
     }
     // (the state's readers of this chunk passed the barriers above)
     publish(c + 1);

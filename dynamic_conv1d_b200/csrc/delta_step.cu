@@ -16,7 +16,7 @@ namespace {
 constexpr int kThreads = 256, kSlice = 32;
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) delta_step_kernel(Step p) {
+__global__ void __launch_bounds__(kThreads, 5) delta_step_kernel(Step p) {
   constexpr int kLanes = kSlice / VEC;           // threads across a row
   constexpr int kGroups = kThreads / kLanes;     // rows at a time
   constexpr int kRows = kMaxKey / kGroups;       // rows per thread

@@ -53,7 +53,8 @@ __device__ __forceinline__ float2 row_sum(float2 v, int& flip) {
   return v;
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
+// (the quick exponential is off by 2^-21 + 2^-23 |z|; silu of -inf is NaN, as -inf * 0 is)
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 
 // Threads of a CTA for a row of TPR threads.
 __host__ __device__ constexpr int cta(int tpr) { return tpr < 256 ? 256 : tpr; }
@@ -94,241 +95,304 @@ __device__ __forceinline__ void store_sums(const float (&acc)[NV * VEC], float* 
   }
 }
 
+// A thread's columns of a weight: held over all rows where its share of a row is small, else read again for each.
 template <typename T, int VEC, int TPR, int NV>
-__global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
+struct Columns {
   using V = Vec<T, VEC>;
-  constexpr int kRows = cta(TPR) / TPR;
-  const int lane = threadIdx.x % TPR;
-  int flip = 0;
-  const int64_t rows = p.N * p.G;
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
-    const int64_t row = r0 + threadIdx.x / TPR;
-    const bool in = row < rows;
-    const int64_t n = in ? row / p.G : 0, g = in ? row % p.G : 0;
-    const T* x = (const T*)p.x + n * p.x_outer + g * p.x_inner;
-    const T* z = (const T*)p.gate + n * p.gate_outer + g * p.gate_inner;
-    V xv[NV], zv[NV];
+  static constexpr bool kHeld = VEC * NV <= 8;
+  V held[kHeld ? NV : 1];
+  const T* at;
+  __device__ __forceinline__ Columns(const void* p, int lane, int D) : at((const T*)p + lane * VEC) {
+    if constexpr (kHeld) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (in && c < p.D) {
-        xv[i] = *reinterpret_cast<const V*>(x + c);
-        if (p.gate) zv[i] = *reinterpret_cast<const V*>(z + c);
-      }
+      for (int i = 0; i < NV; ++i)
+        if (p && (i * TPR + lane) * VEC < D) held[i] = *reinterpret_cast<const V*>(at + i * TPR * VEC);
     }
-    float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (in && (i * TPR + lane) * VEC < p.D)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float v = Elem<T>::to_f(xv[i].e[e]);
-          s.x = fmaf(v, v, s.x);
-        }
-    const float r = p.scale * rsqrtf(row_sum<TPR>(s, flip).x / p.D + p.eps);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (!in || c >= p.D) continue;
-      V w{}, y;
-      if (p.weight) w = *reinterpret_cast<const V*>((const T*)p.weight + c);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float v = Elem<T>::to_f(xv[i].e[e]) * r;
-        if (p.weight) v *= Elem<T>::to_f(w.e[e]);
-        if (p.gate) {
-          const float zf = Elem<T>::to_f(zv[i].e[e]);
-          v *= zf * sigmoid(zf);
-        }
-        y.e[e] = Elem<T>::from_f(v);
-      }
-      *reinterpret_cast<V*>((T*)p.y + row * p.D + c) = y;
+  }
+  __device__ __forceinline__ V operator[](int i) const {
+    if constexpr (kHeld) return held[i];
+    return *reinterpret_cast<const V*>(at + i * TPR * VEC);
+  }
+};
+
+// Whether a thread's share of a row is small enough to have the next row's loads under way meanwhile.
+constexpr bool ahead(int vec, int nv) { return vec * nv <= 8; }
+
+// Walks this CTA's rows: load(row, buffer) for each, the next one's before the work on the present one.
+template <typename Buf, int TPR, bool AHEAD, typename Load, typename Work>
+__device__ __forceinline__ void walk(int64_t rows, Load&& load, Work&& work) {
+  constexpr int kRows = cta(TPR) / TPR;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR, first = (int64_t)blockIdx.x * kRows;
+  Buf now;
+  if (AHEAD && first < rows) load(row, now);
+  for (; first < rows; first += step, row += step) {
+    if constexpr (AHEAD) {
+      Buf next;
+      if (first + step < rows) load(row + step, next);
+      work(row, now);
+      now = next;
+    } else {
+      load(row, now);
+      work(row, now);
     }
   }
 }
 
 template <typename T, int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
+  using V = Vec<T, VEC>;
+  struct Buf {
+    V x[NV], z[NV];
+  };
+  const int lane = threadIdx.x % TPR;
+  int flip = 0;
+  const int64_t rows = p.N * p.G;
+  const Columns<T, VEC, TPR, NV> w(p.weight, lane, p.D);
+  walk<Buf, TPR, ahead(VEC, NV)>(
+      rows,
+      [&](int64_t row, Buf& a) {
+        const int64_t n = p.G == 1 ? row : row / p.G, g = row - n * p.G;
+        const T* x = (const T*)p.x + n * p.x_outer + g * p.x_inner;
+        const T* z = (const T*)p.gate + n * p.gate_outer + g * p.gate_inner;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + lane) * VEC;
+          if (row < rows && c < p.D) {
+            a.x[i] = *reinterpret_cast<const V*>(x + c);
+            if (p.gate) a.z[i] = *reinterpret_cast<const V*>(z + c);
+          }
+        }
+      },
+      [&](int64_t row, const Buf& a) {
+        const bool in = row < rows;
+        float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (in && (i * TPR + lane) * VEC < p.D)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const float v = Elem<T>::to_f(a.x[i].e[e]);
+              s.x = fmaf(v, v, s.x);
+            }
+        const float r = p.scale * rsqrtf(row_sum<TPR>(s, flip).x / p.D + p.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + lane) * VEC;
+          if (!in || c >= p.D) continue;
+          V y;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            float v = Elem<T>::to_f(a.x[i].e[e]) * r;
+            if (p.weight) v *= Elem<T>::to_f(w[i].e[e]);
+            if (p.gate) {
+              const float zf = Elem<T>::to_f(a.z[i].e[e]);
+              v *= zf * sigmoid(zf);
+            }
+            y.e[e] = Elem<T>::from_f(v);
+          }
+          *reinterpret_cast<V*>((T*)p.y + row * p.D + c) = y;
+        }
+      });
+}
+
+template <typename T, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR)) gated_bwd_kernel(Gated p) {
   using V = Vec<T, VEC>;
-  constexpr int kRows = cta(TPR) / TPR;
+  struct Buf {
+    V x[NV], z[NV], d[NV];
+  };
   const int lane = threadIdx.x % TPR;
   int flip = 0;
   const int64_t rows = p.N * p.G;
   float acc[NV * VEC];
+  const Columns<T, VEC, TPR, NV> w(p.weight, lane, p.D);
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc[i] = 0.f;
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
-    const int64_t row = r0 + threadIdx.x / TPR;
-    const bool in = row < rows;
-    const int64_t n = in ? row / p.G : 0, g = in ? row % p.G : 0;
-    const T* x = (const T*)p.x + n * p.x_outer + g * p.x_inner;
-    const T* z = (const T*)p.gate + n * p.gate_outer + g * p.gate_inner;
-    const T* dy = (const T*)p.dy + row * p.D;
-    V xv[NV], zv[NV], dv[NV], wv[NV];
+  walk<Buf, TPR, ahead(VEC, NV)>(
+      rows,
+      [&](int64_t row, Buf& a) {
+        const int64_t n = p.G == 1 ? row : row / p.G, g = row - n * p.G;
+        const T* x = (const T*)p.x + n * p.x_outer + g * p.x_inner;
+        const T* z = (const T*)p.gate + n * p.gate_outer + g * p.gate_inner;
+        const T* dy = (const T*)p.dy + row * p.D;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (in && c < p.D) {
-        xv[i] = *reinterpret_cast<const V*>(x + c);
-        dv[i] = *reinterpret_cast<const V*>(dy + c);
-        if (p.gate) zv[i] = *reinterpret_cast<const V*>(z + c);
-        if (p.weight) wv[i] = *reinterpret_cast<const V*>((const T*)p.weight + c);
-      }
-    }
-    // dn = scale * dy w silu(g) is made twice: a second copy of the row would not stay in registers
-    float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (in && (i * TPR + lane) * VEC < p.D)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float v = Elem<T>::to_f(xv[i].e[e]);
-          float dn = p.scale * Elem<T>::to_f(dv[i].e[e]);
-          if (p.weight) dn *= Elem<T>::to_f(wv[i].e[e]);
-          if (p.gate) {
-            const float zf = Elem<T>::to_f(zv[i].e[e]);
-            dn *= zf * sigmoid(zf);
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + lane) * VEC;
+          if (row < rows && c < p.D) {
+            a.x[i] = *reinterpret_cast<const V*>(x + c);
+            a.d[i] = *reinterpret_cast<const V*>(dy + c);
+            if (p.gate) a.z[i] = *reinterpret_cast<const V*>(z + c);
           }
-          s.x = fmaf(v, v, s.x);
-          s.y = fmaf(dn, v, s.y);
         }
-    s = row_sum<TPR>(s, flip);
-    const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
+      },
+      [&](int64_t row, const Buf& a) {
+        const bool in = row < rows;
+        // a narrow row's gates stay in registers between the sums and the gradients; a wide one's are made twice
+        constexpr bool kKeep = ahead(VEC, NV);
+        float sg[kKeep ? NV * VEC : 1];
+        float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (!in || c >= p.D) continue;
-      V dx, dz;
+        for (int i = 0; i < NV; ++i)
+          if (in && (i * TPR + lane) * VEC < p.D)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float v = Elem<T>::to_f(xv[i].e[e]), d = p.scale * Elem<T>::to_f(dv[i].e[e]);
-        const float w = p.weight ? Elem<T>::to_f(wv[i].e[e]) : 1.f;
-        float silu = 1.f, slope = 0.f;
-        if (p.gate) {
-          const float zf = Elem<T>::to_f(zv[i].e[e]), sg = sigmoid(zf);
-          silu = zf * sg;
-          slope = sg * (1.f + zf * (1.f - sg));
+            for (int e = 0; e < VEC; ++e) {
+              const float v = Elem<T>::to_f(a.x[i].e[e]);
+              float dn = Elem<T>::to_f(a.d[i].e[e]);
+              if (p.weight) dn *= Elem<T>::to_f(w[i].e[e]);
+              if (p.gate) {
+                const float zf = Elem<T>::to_f(a.z[i].e[e]), g = sigmoid(zf);
+                if constexpr (kKeep) sg[i * VEC + e] = g;
+                dn *= zf * g;
+              }
+              s.x = fmaf(v, v, s.x);
+              s.y = fmaf(dn, v, s.y);
+            }
+        s = row_sum<TPR>(s, flip);
+        const float r = rsqrtf(s.x / p.D + p.eps), rs = p.scale * r, m = s.y / p.D * r * r;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + lane) * VEC;
+          if (!in || c >= p.D) continue;
+          V dx, dz;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float v = Elem<T>::to_f(a.x[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
+            const float dw = p.weight ? d * Elem<T>::to_f(w[i].e[e]) : d, vr = v * rs;
+            if (p.gate) {
+              const float zf = Elem<T>::to_f(a.z[i].e[e]);
+              float g;
+              if constexpr (kKeep)
+                g = sg[i * VEC + e];
+              else
+                g = sigmoid(zf);
+              const float silu = zf * g;
+              dx.e[e] = Elem<T>::from_f(rs * fmaf(dw, silu, -v * m));
+              dz.e[e] = Elem<T>::from_f(dw * vr * (g + silu * (1.f - g)));
+              acc[i * VEC + e] = fmaf(d * vr, silu, acc[i * VEC + e]);
+            } else {
+              dx.e[e] = Elem<T>::from_f(rs * fmaf(-v, m, dw));
+              acc[i * VEC + e] = fmaf(d, vr, acc[i * VEC + e]);
+            }
+          }
+          if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
+          if (p.dgate) *reinterpret_cast<V*>((T*)p.dgate + row * p.D + c) = dz;
         }
-        dx.e[e] = Elem<T>::from_f(r * (d * w * silu - v * m));
-        const float dn = d * v * r;
-        if (p.gate) dz.e[e] = Elem<T>::from_f(dn * w * slope);
-        acc[i * VEC + e] = fmaf(dn, silu, acc[i * VEC + e]);
-      }
-      if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
-      if (p.dgate) *reinterpret_cast<V*>((T*)p.dgate + row * p.D + c) = dz;
-    }
-  }
+      });
   if (p.part) store_sums<TPR, VEC, NV>(acc, p.part + (int64_t)blockIdx.x * p.D, p.D);
 }
 
 template <typename T, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
   using V = Vec<T, VEC>;
-  constexpr int kRows = cta(TPR) / TPR;
+  struct Buf {
+    V x[NV], r[NV];
+  };
   const int lane = threadIdx.x % TPR;
   int flip = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < p.N; r0 += (int64_t)gridDim.x * kRows) {
-    const int64_t row = r0 + threadIdx.x / TPR;
-    const bool in = row < p.N;
-    V xv[NV], rv[NV];
+  const Columns<T, VEC, TPR, NV> w(p.weight, lane, p.D), sc(p.scale, lane, p.D);
+  walk<Buf, TPR, ahead(VEC, NV)>(
+      p.N,
+      [&](int64_t row, Buf& a) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (in && c < p.D) {
-        xv[i] = *reinterpret_cast<const V*>((const T*)p.x + row * p.D + c);
-        rv[i] = *reinterpret_cast<const V*>((const T*)p.residual + row * p.D + c);
-      }
-    }
-    float h[NV * VEC];  // unrounded: y is the norm of the sum itself
-    float2 s = make_float2(0.f, 0.f);
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + lane) * VEC;
+          if (row < p.N && c < p.D) {
+            a.x[i] = *reinterpret_cast<const V*>((const T*)p.x + row * p.D + c);
+            a.r[i] = *reinterpret_cast<const V*>((const T*)p.residual + row * p.D + c);
+          }
+        }
+      },
+      [&](int64_t row, const Buf& a) {
+        const bool in = row < p.N;
+        float h[NV * VEC];  // unrounded: y is the norm of the sum itself
+        float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (!in || c >= p.D) continue;
-      V sv{}, hv;
-      if (p.scale) sv = *reinterpret_cast<const V*>((const T*)p.scale + c);
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + lane) * VEC;
+          if (!in || c >= p.D) continue;
+          V hv;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float f = p.scale ? Elem<T>::to_f(sv.e[e]) : p.factor;
-        const float v = fmaf(f, Elem<T>::to_f(xv[i].e[e]), Elem<T>::to_f(rv[i].e[e]));
-        h[i * VEC + e] = v;
-        hv.e[e] = Elem<T>::from_f(v);
-        s.x = fmaf(v, v, s.x);
-      }
-      *reinterpret_cast<V*>((T*)p.h + row * p.D + c) = hv;
-    }
-    const float r = rsqrtf(row_sum<TPR>(s, flip).x / p.D + p.eps);
+          for (int e = 0; e < VEC; ++e) {
+            const float f = p.scale ? Elem<T>::to_f(sc[i].e[e]) : p.factor;
+            const float v = fmaf(f, Elem<T>::to_f(a.x[i].e[e]), Elem<T>::to_f(a.r[i].e[e]));
+            h[i * VEC + e] = v;
+            hv.e[e] = Elem<T>::from_f(v);
+            s.x = fmaf(v, v, s.x);
+          }
+          *reinterpret_cast<V*>((T*)p.h + row * p.D + c) = hv;
+        }
+        const float r = rsqrtf(row_sum<TPR>(s, flip).x / p.D + p.eps);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (!in || c >= p.D) continue;
-      const V w = *reinterpret_cast<const V*>((const T*)p.weight + c);
-      V y;
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + lane) * VEC;
+          if (!in || c >= p.D) continue;
+          V y;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) y.e[e] = Elem<T>::from_f(h[i * VEC + e] * r * Elem<T>::to_f(w.e[e]));
-      *reinterpret_cast<V*>((T*)p.y + row * p.D + c) = y;
-    }
-  }
+          for (int e = 0; e < VEC; ++e) y.e[e] = Elem<T>::from_f(h[i * VEC + e] * r * Elem<T>::to_f(w[i].e[e]));
+          *reinterpret_cast<V*>((T*)p.y + row * p.D + c) = y;
+        }
+      });
 }
 
 template <typename T, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR)) residual_bwd_kernel(Residual p) {
   using V = Vec<T, VEC>;
-  constexpr int kRows = cta(TPR) / TPR;
+  struct Buf {
+    V h[NV], d[NV], u[NV], x[NV];
+  };
   const int lane = threadIdx.x % TPR;
   int flip = 0;
   float acc_w[NV * VEC], acc_s[NV * VEC];
+  const Columns<T, VEC, TPR, NV> w(p.weight, lane, p.D), sc(p.scale, lane, p.D);
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc_w[i] = acc_s[i] = 0.f;
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < p.N; r0 += (int64_t)gridDim.x * kRows) {
-    const int64_t row = r0 + threadIdx.x / TPR;
-    const bool in = row < p.N;
-    V hv[NV], dv[NV], uv[NV], xv[NV];
+  walk<Buf, TPR, ahead(VEC, NV)>(
+      p.N,
+      [&](int64_t row, Buf& a) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (in && c < p.D) {
-        hv[i] = *reinterpret_cast<const V*>((const T*)p.h + row * p.D + c);
-        dv[i] = p.dy ? *reinterpret_cast<const V*>((const T*)p.dy + row * p.D + c) : V{};
-        uv[i] = p.dh ? *reinterpret_cast<const V*>((const T*)p.dh + row * p.D + c) : V{};
-        if (p.part_s) xv[i] = *reinterpret_cast<const V*>((const T*)p.x + row * p.D + c);
-      }
-    }
-    float2 s = make_float2(0.f, 0.f);
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + lane) * VEC;
+          if (row < p.N && c < p.D) {
+            a.h[i] = *reinterpret_cast<const V*>((const T*)p.h + row * p.D + c);
+            a.d[i] = p.dy ? *reinterpret_cast<const V*>((const T*)p.dy + row * p.D + c) : V{};
+            a.u[i] = p.dh ? *reinterpret_cast<const V*>((const T*)p.dh + row * p.D + c) : V{};
+            if (p.part_s) a.x[i] = *reinterpret_cast<const V*>((const T*)p.x + row * p.D + c);
+          }
+        }
+      },
+      [&](int64_t row, const Buf& a) {
+        const bool in = row < p.N;
+        float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (!in || c >= p.D) continue;
-      const V w = *reinterpret_cast<const V*>((const T*)p.weight + c);
+        for (int i = 0; i < NV; ++i)
+          if (in && (i * TPR + lane) * VEC < p.D)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float v = Elem<T>::to_f(hv[i].e[e]);
-        s.x = fmaf(v, v, s.x);
-        s.y = fmaf(Elem<T>::to_f(dv[i].e[e]) * Elem<T>::to_f(w.e[e]), v, s.y);
-      }
-    }
-    s = row_sum<TPR>(s, flip);
-    const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
+            for (int e = 0; e < VEC; ++e) {
+              const float v = Elem<T>::to_f(a.h[i].e[e]);
+              s.x = fmaf(v, v, s.x);
+              s.y = fmaf(Elem<T>::to_f(a.d[i].e[e]) * Elem<T>::to_f(w[i].e[e]), v, s.y);
+            }
+        s = row_sum<TPR>(s, flip);
+        const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (!in || c >= p.D) continue;
-      const V w = *reinterpret_cast<const V*>((const T*)p.weight + c);
-      V sv{}, dt, dx;
-      if (p.scale) sv = *reinterpret_cast<const V*>((const T*)p.scale + c);
+        for (int i = 0; i < NV; ++i) {
+          const int c = (i * TPR + lane) * VEC;
+          if (!in || c >= p.D) continue;
+          V dt, dx;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float v = Elem<T>::to_f(hv[i].e[e]), d = Elem<T>::to_f(dv[i].e[e]);
-        const float t = fmaf(r, fmaf(d, Elem<T>::to_f(w.e[e]), -v * m), Elem<T>::to_f(uv[i].e[e]));
-        dt.e[e] = Elem<T>::from_f(t);
-        dx.e[e] = Elem<T>::from_f(t * (p.scale ? Elem<T>::to_f(sv.e[e]) : p.factor));
-        acc_w[i * VEC + e] = fmaf(d, v * r, acc_w[i * VEC + e]);
-        if (p.part_s) acc_s[i * VEC + e] = fmaf(t, Elem<T>::to_f(xv[i].e[e]), acc_s[i * VEC + e]);
-      }
-      if (p.dresidual) *reinterpret_cast<V*>((T*)p.dresidual + row * p.D + c) = dt;
-      if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
-    }
-  }
+          for (int e = 0; e < VEC; ++e) {
+            const float v = Elem<T>::to_f(a.h[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
+            const float t = fmaf(r, fmaf(d, Elem<T>::to_f(w[i].e[e]), -v * m), Elem<T>::to_f(a.u[i].e[e]));
+            dt.e[e] = Elem<T>::from_f(t);
+            dx.e[e] = Elem<T>::from_f(t * (p.scale ? Elem<T>::to_f(sc[i].e[e]) : p.factor));
+            acc_w[i * VEC + e] = fmaf(d, v * r, acc_w[i * VEC + e]);
+            if (p.part_s) acc_s[i * VEC + e] = fmaf(t, Elem<T>::to_f(a.x[i].e[e]), acc_s[i * VEC + e]);
+          }
+          if (p.dresidual) *reinterpret_cast<V*>((T*)p.dresidual + row * p.D + c) = dt;
+          if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
+        }
+      });
   if (p.part_w) store_sums<TPR, VEC, NV>(acc_w, p.part_w + (int64_t)blockIdx.x * p.D, p.D);
   if (p.part_s) store_sums<TPR, VEC, NV>(acc_s, p.part_s + (int64_t)blockIdx.x * p.D, p.D);
 }
@@ -357,7 +421,14 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restric
   }
 }
 
-bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// The most numbers that can be read at once: the pointers (or-ed addresses) and strides (or-ed) decide.
+int vec_of(uintptr_t addresses, int64_t strides, int dtype) {
+  const int elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4;
+  for (int n : {16 / elem, 2})
+    if (addresses % (n * elem) == 0 && strides % n == 0) return n;
+  return 1;
+}
+uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 // CTAs of a launch: as many as run at once (2048 threads of an SM; backward half of that), no more than there is work for.
 int64_t grid_of(int64_t rows, int tpr, bool backward) {
@@ -371,7 +442,7 @@ int64_t grid_of(int64_t rows, int tpr, bool backward) {
 template <typename T, int VEC, typename F>
 int pick(int64_t D, F&& go) {
   constexpr int kNV = kPerThread / VEC;
-  constexpr int kOne = VEC > 1 ? 1 : 4;  // vectors per thread of a narrow row
+  constexpr int kOne = VEC >= 4 ? 1 : 4 / VEC;  // vectors per thread of a narrow row
   if (D <= 8 * VEC * kOne) return go.template operator()<T, VEC, 8, kOne>();
   if (D <= 16 * VEC * kOne) return go.template operator()<T, VEC, 16, kOne>();
   if (D <= 32 * VEC * kOne) return go.template operator()<T, VEC, 32, kOne>();
@@ -432,11 +503,12 @@ struct ResidualGo {
   }
 };
 
+// vec: numbers that can be read at once, a 16-byte vector of them, two or one.
 template <typename Go>
-int dispatch(int64_t D, int dtype, bool vectors, const Go& go) {
+int dispatch(int64_t D, int dtype, int vec, const Go& go) {
   if (dtype == DYNCONV_DTYPE_BF16)
-    return vectors ? pick<__nv_bfloat16, 8>(D, go) : pick<__nv_bfloat16, 1>(D, go);
-  return vectors ? pick<float, 4>(D, go) : pick<float, 1>(D, go);
+    return vec == 8 ? pick<__nv_bfloat16, 8>(D, go) : vec == 2 ? pick<__nv_bfloat16, 2>(D, go) : pick<__nv_bfloat16, 1>(D, go);
+  return vec == 4 ? pick<float, 4>(D, go) : vec == 2 ? pick<float, 2>(D, go) : pick<float, 1>(D, go);
 }
 
 }  // namespace
@@ -445,18 +517,15 @@ int dispatch(int64_t D, int dtype, bool vectors, const Go& go) {
 int64_t partial_rows() { return (int64_t)sm_count() * 4; }
 
 int gated_launch(const Gated& p, int dtype, bool backward, cudaStream_t st) {
-  const int per = dtype == DYNCONV_DTYPE_BF16 ? 8 : 4;
-  const bool strides = p.x_outer % per == 0 && p.x_inner % per == 0 && (!p.gate || (p.gate_outer % per == 0 && p.gate_inner % per == 0));
-  const bool vectors = p.D % per == 0 && strides && aligned(p.x) && aligned(p.weight) && aligned(p.gate) && aligned(p.y) &&
-                       aligned(p.dy) && aligned(p.dx) && aligned(p.dgate);
-  return dispatch(p.D, dtype, vectors, GatedGo{p, backward, st});
+  const int64_t strides = p.D | p.x_outer | p.x_inner | (p.gate ? p.gate_outer | p.gate_inner : 0);
+  const uintptr_t all = bits(p.x) | bits(p.weight) | bits(p.gate) | bits(p.y) | bits(p.dy) | bits(p.dx) | bits(p.dgate);
+  return dispatch(p.D, dtype, vec_of(all, strides, dtype), GatedGo{p, backward, st});
 }
 
 int residual_launch(const Residual& p, int dtype, bool backward, cudaStream_t st) {
-  const int per = dtype == DYNCONV_DTYPE_BF16 ? 8 : 4;
-  const bool vectors = p.D % per == 0 && aligned(p.x) && aligned(p.residual) && aligned(p.weight) && aligned(p.scale) &&
-                       aligned(p.y) && aligned(p.h) && aligned(p.dy) && aligned(p.dh) && aligned(p.dx) && aligned(p.dresidual);
-  return dispatch(p.D, dtype, vectors, ResidualGo{p, backward, st});
+  const uintptr_t all = bits(p.x) | bits(p.residual) | bits(p.weight) | bits(p.scale) | bits(p.y) | bits(p.h) | bits(p.dy) | bits(p.dh) |
+                        bits(p.dx) | bits(p.dresidual);
+  return dispatch(p.D, dtype, vec_of(all, p.D, dtype), ResidualGo{p, backward, st});
 }
 
 }  // namespace norm

@@ -15,7 +15,8 @@ convolutions as one grouped kernel launch per direction.
 
 ``ConvolvedLinearAttention`` is an attention layer on top of it: the three convolved
 streams mixed by linear attention with a decay for each head, for training and prompts,
-and its single-token form for generating text.
+and its single-token form for generating text.  ``ConvolvedGatedDelta`` is its sibling on the gated
+delta rule, with learned decays and a gated norm, and ``ResidualRMSNorm`` stands between two blocks.
 
 proj_in is an ordinary GEMM (cuBLAS through ``torch.nn.functional.linear``): z
 needs a dot product over all d_model channels for each token, while a
@@ -29,8 +30,10 @@ from dataclasses import dataclass
 import torch
 from torch import nn
 
+from .gated_delta import gated_delta_rule, gated_delta_rule_step
 from .linear_attention import decay_linear_attention_fused, decay_linear_attention_step
 from .lowrank import lowrank_dynamic_convolution, lowrank_dynamic_convolution_grouped
+from .norm import gated_rms_norm, residual_rms_norm
 from .step import convolution_cache, lowrank_dynamic_convolution_grouped_step
 
 
@@ -118,7 +121,7 @@ class QKVLowRankDynamicShortConvolution(nn.Module):
 
 @dataclass
 class LayerCache:
-    """What one ``ConvolvedLinearAttention`` layer keeps of its sequences between tokens."""
+    """What one ``ConvolvedLinearAttention`` or ``ConvolvedGatedDelta`` layer keeps of its sequences between tokens."""
 
     conv: torch.Tensor  # [n, W-1, 3*d_model]: the last inputs of the convolutions
     state: torch.Tensor  # [n, H, d, d] float32: the attention's state
@@ -175,3 +178,77 @@ class ConvolvedLinearAttention(nn.Module):
         q, k, v = y.view(B, 3, H, self.d_model // H).unbind(1)
         o = decay_linear_attention_step(q, k, v, cache.state, self.log_decay, slots=slots)
         return self.out(o.view(B, self.d_model))
+
+
+class ConvolvedGatedDelta(nn.Module):
+    """A layer on the gated delta rule: one fused projection of queries, keys and values, the grouped
+    low-rank dynamic convolution of its three thirds, queries and keys of length one, the rule with
+    decays and rates that come from the input, a norm of each head's output under a gate, and an
+    output projection.
+
+    The decay of head h is exp(-exp(A_log[h]) softplus(a + dt_bias[h])), its rate sigmoid(b), with a and b
+    linear in the input.  ``forward``, ``prompt`` and ``step`` are those of ``ConvolvedLinearAttention``.
+    A head has at most 128 channels.
+    """
+
+    def __init__(self, d_model: int, n_heads: int, R: int = 15, W: int = 4):
+        super().__init__()
+        if d_model % n_heads != 0:
+            raise ValueError("d_model must be divisible by n_heads")
+        if d_model // n_heads > 128:
+            raise ValueError("a head must have at most 128 channels")
+        self.d_model, self.n_heads, self.d_head, self.W = d_model, n_heads, d_model // n_heads, W
+        self.qkv = nn.Linear(d_model, 3 * d_model, bias=False)
+        self.conv = QKVLowRankDynamicShortConvolution(d_model, R, W)
+        self.gates = nn.Linear(d_model, 2 * n_heads, bias=False)
+        # decay rates of 1 to 16 over the heads, steps of about 0.001 to 0.1
+        self.A_log = nn.Parameter(torch.linspace(1, 16, n_heads).log())
+        steps = torch.exp(torch.rand(n_heads) * math.log(100.0) + math.log(1e-3))
+        self.dt_bias = nn.Parameter(steps + torch.log(-torch.expm1(-steps)))  # (softplus gives the steps)
+        self.gate = nn.Linear(d_model, d_model, bias=False)
+        self.norm = nn.Parameter(torch.ones(self.d_head))
+        self.out = nn.Linear(d_model, d_model, bias=False)
+
+    def _gates(self, x: torch.Tensor):
+        """log decays and rates, [..., n_heads] in x's dtype; the decays are worked out in float32."""
+        a, b = self.gates(x).split(self.n_heads, -1)
+        g = -torch.exp(self.A_log.float()) * torch.nn.functional.softplus(a.float() + self.dt_bias.float())
+        return g.to(x.dtype), torch.sigmoid(b)
+
+    def _heads(self, y: torch.Tensor):
+        """Queries and keys of length one, and values, [..., n_heads, d_head], of the convolved [..., 3*d_model]."""
+        qk, v = y.split([2 * self.d_model, self.d_model], -1)
+        qk = gated_rms_norm(qk.unflatten(-1, (2 * self.n_heads, self.d_head)), scale=self.d_head**-0.5)
+        q, k = qk.split(self.n_heads, -2)
+        return q, k, v.unflatten(-1, (self.n_heads, self.d_head))
+
+    def _finish(self, o: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+        return self.out(gated_rms_norm(o, self.norm, self.gate(x).view(o.shape)).flatten(-2))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self._finish(gated_delta_rule(*self._heads(self.conv.forward_fused(self.qkv(x), x)), *self._gates(x)), x)
+
+    def prompt(self, x: torch.Tensor) -> tuple[torch.Tensor, LayerCache]:
+        qkv = self.qkv(x)
+        o, state = gated_delta_rule(*self._heads(self.conv.forward_fused(qkv, x)), *self._gates(x), return_state=True)
+        return self._finish(o, x), LayerCache(convolution_cache(qkv, self.W), state, self.conv.stacked())
+
+    def step(self, x: torch.Tensor, cache: LayerCache, slots: torch.Tensor | None = None) -> torch.Tensor:
+        q, k, v = self._heads(self.conv.step(self.qkv(x), x, cache.conv, cache.stacked, slots))
+        o = gated_delta_rule_step(q, k, v, cache.state, *self._gates(x), slots=slots)
+        return self._finish(o, x)
+
+
+class ResidualRMSNorm(nn.Module):
+    """Between two blocks: adds the one's output to the residual stream, times a learned scale per channel
+    where ``layer_scale`` is given (its initial value), and normalises the sum for the other.
+    forward(x, residual) returns (normalised, residual stream)."""
+
+    def __init__(self, d_model: int, layer_scale: float | None = None, eps: float = 1e-6):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(d_model))
+        self.scale = None if layer_scale is None else nn.Parameter(torch.full((d_model,), float(layer_scale)))
+        self.eps = eps
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor):
+        return residual_rms_norm(x, residual, self.weight, 1.0 if self.scale is None else self.scale, self.eps)

@@ -1,6 +1,7 @@
-"""A small language model on convolved linear attention: trained, then continued token by token.
+"""A small language model on convolved linear attention, or (--layer delta) on the gated delta rule: trained, then
+continued token by token.
 
-    python examples/linear_attention_lm.py [--steps 200] [--generate 24]
+    python examples/linear_attention_lm.py [--steps 200] [--generate 24] [--layer delta]
 
 Each training sequence repeats a short random word over and over, so a model that has learned
 to look back a word's length predicts everything after the first repetition.  Training
@@ -19,7 +20,7 @@ from torch import nn
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from dynamic_conv1d_b200 import ConvolvedLinearAttention, linear_cross_entropy  # noqa: E402
+from dynamic_conv1d_b200 import ConvolvedGatedDelta, ConvolvedLinearAttention, ResidualRMSNorm, linear_cross_entropy  # noqa: E402
 
 
 class Block(nn.Module):
@@ -43,12 +44,37 @@ class Block(nn.Module):
         return x + self.mlp(self.norm2(x))
 
 
+class DeltaBlock(nn.Module):
+    """The same on the gated delta rule, the second norm fused with the residual stream before it."""
+
+    def __init__(self, d_model: int, n_heads: int):
+        super().__init__()
+        self.norm1, self.norm2 = nn.RMSNorm(d_model), ResidualRMSNorm(d_model)
+        self.attn = ConvolvedGatedDelta(d_model, n_heads)
+        self.mlp = nn.Sequential(nn.Linear(d_model, 4 * d_model, bias=False), nn.SiLU(), nn.Linear(4 * d_model, d_model, bias=False))
+
+    def _rest(self, y, x):
+        y, x = self.norm2(y, x)
+        return x + self.mlp(y)
+
+    def forward(self, x):
+        return self._rest(self.attn(self.norm1(x)), x)
+
+    def prompt(self, x):
+        y, cache = self.attn.prompt(self.norm1(x))
+        return self._rest(y, x), cache
+
+    def step(self, x, cache):
+        return self._rest(self.attn.step(self.norm1(x), cache), x)
+
+
 class LanguageModel(nn.Module):
-    def __init__(self, vocab: int, d_model: int = 256, n_heads: int = 4, n_layers: int = 2):
+    def __init__(self, vocab: int, d_model: int = 256, n_heads: int = 4, n_layers: int = 2, layer: str = "linear"):
         super().__init__()
         self.embed = nn.Embedding(vocab, d_model)
         nn.init.normal_(self.embed.weight, std=d_model**-0.5)
-        self.blocks = nn.ModuleList(Block(d_model, n_heads) for _ in range(n_layers))
+        block = DeltaBlock if layer == "delta" else Block
+        self.blocks = nn.ModuleList(block(d_model, n_heads) for _ in range(n_layers))
         self.norm = nn.RMSNorm(d_model)
         self.scale = d_model**0.5
 
@@ -92,11 +118,12 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--vocab", type=int, default=500)
     ap.add_argument("--generate", type=int, default=24)
+    ap.add_argument("--layer", choices=("linear", "delta"), default="linear")
     a = ap.parse_args(argv)
     device = torch.device("cuda")
     torch.manual_seed(0)
     g = torch.Generator(device=device).manual_seed(1)
-    model = LanguageModel(a.vocab).to(device, torch.bfloat16)
+    model = LanguageModel(a.vocab, layer=a.layer).to(device, torch.bfloat16)
     opt = torch.optim.AdamW(model.parameters(), lr=2e-3, weight_decay=0.0)
     first = last = None
     for i in range(a.steps):

@@ -97,3 +97,17 @@ def test_python_refuses_cpu_tensors():
         dc.gated_rms_norm(t)
     with pytest.raises(AssertionError):
         dc.residual_rms_norm(t, t, t[0, 0, 0])
+
+
+def test_layer_arguments():
+    with pytest.raises(ValueError):
+        dc.ConvolvedGatedDelta(100, 3)
+    with pytest.raises(ValueError):
+        dc.ConvolvedGatedDelta(256, 1)
+    with pytest.raises(ValueError):
+        dc.ConvolvedGatedDelta(64, 2, R=16)
+    m = dc.ConvolvedGatedDelta(64, 2)
+    # the steps that the bias stands for lie between 0.001 and 0.1
+    steps = torch.nn.functional.softplus(m.dt_bias)
+    assert ((steps > 9e-4) & (steps < 0.11)).all()
+    assert dc.ResidualRMSNorm(8).scale is None and dc.ResidualRMSNorm(8, layer_scale=0.5).scale.shape == (8,)
