@@ -45,6 +45,20 @@ __device__ __forceinline__ uint32_t first_lane() {
   return ((l >> 4 & 1) + (l >> 2 & 2)) * 128 + (l & 7) * 16;
 }
 
+// c0, c1 += a b.  fp32: the sum by itself first, since the instruction's own additions are cut off, not rounded, and dk
+// is a sum of some fifty of them.
+template <int NA, int NB, int KEEP, bool ROUND>
+__device__ __forceinline__ void add_parts(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
+  if constexpr (ROUND) {
+    float x[2][4];
+    zero(x[0]), zero(x[1]);
+    mma_parts<NA, NB, KEEP>(x[0], x[1], a, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c0[e] += x[0][e], c1[e] += x[1][e];
+  } else {
+    mma_parts<NA, NB, KEEP>(c0, c1, a, b);
+  }
+}
 // (out of line: the kernel has to stay in the instruction cache)
 template <typename E>
 __device__ __noinline__ void store2_slow(E* to, float x, float y, int n) {
@@ -67,6 +81,7 @@ __device__ __forceinline__ void store2(E* to, float x, float y, int n, bool pair
 template <typename R>
 __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, const __grid_constant__ Maps maps, int items, int pairs) {
   constexpr int PX = R::PX, C = R::C, NB = R::NB, PU = R::PU, PS = R::PS, kSlab = R::kSlab, kSquare = R::kSquare;
+  constexpr bool kRound = PX > 1;
   constexpr int NT = R::NT, KK = R::KK, KX = PX > PS ? PX : PS, KS = PU > PS ? PU : PS;
   using E = typename R::E;
   extern __shared__ uint8_t smem_raw[];
@@ -218,18 +233,23 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
 #pragma unroll
         for (int i = 0; i < PU; ++i) ldsm_t(r[i], a_r + i * kSlab * R::kU);
 #pragma unroll
-        for (int m = 0; m < NT / 2; ++m) mma_parts<PX, PS, KX>(dq[2 * m], dq[2 * m + 1], dO, f[m]);
+        for (int m = 0; m < NT / 2; ++m) add_parts<PX, PS, KX, kRound>(dq[2 * m], dq[2 * m + 1], dO, f[m]);
         // (all tiles' products of one pair of parts, then of the next: none waits for the one before)
+        if constexpr (kRound) {
 #pragma unroll
-        for (int t = KS - 1; t >= 0; --t)
+          for (int m = 0; m < NT / 2; ++m) add_parts<PU, PS, KS, true>(ku[2 * m], ku[2 * m + 1], u, f[m]);
+        } else {
 #pragma unroll
-          for (int i = 0; i < PU; ++i)
+          for (int t = KS - 1; t >= 0; --t)
 #pragma unroll
-            for (int m = 0; m < NT / 2; ++m)
-              if (t - i >= 0 && t - i < PS) {
-                mma(ku[2 * m], u[i], f[m][t - i][0], f[m][t - i][1]);
-                mma(ku[2 * m + 1], u[i], f[m][t - i][2], f[m][t - i][3]);
-              }
+            for (int i = 0; i < PU; ++i)
+#pragma unroll
+              for (int m = 0; m < NT / 2; ++m)
+                if (t - i >= 0 && t - i < PS) {
+                  mma(ku[2 * m], u[i], f[m][t - i][0], f[m][t - i][1]);
+                  mma(ku[2 * m + 1], u[i], f[m][t - i][2], f[m][t - i][3]);
+                }
+        }
         uint32_t g[NT / 2][PS][4];
 #pragma unroll
         for (int m = 0; m < NT / 2; ++m)
@@ -250,23 +270,28 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
             mma_parts<PS, PS, PS>(dot[0], dot[1], t, g[m]);
           }
         }
+        if constexpr (kRound) {
 #pragma unroll
-        for (int t = KS - 1; t >= 0; --t)
+          for (int m = 0; m < NT / 2; ++m) add_parts<PU, PS, KS, true>(kr[2 * m], kr[2 * m + 1], r, g[m]);
+        } else {
 #pragma unroll
-          for (int i = 0; i < PU; ++i)
+          for (int t = KS - 1; t >= 0; --t)
 #pragma unroll
-            for (int m = 0; m < NT / 2; ++m)
-              if (t - i >= 0 && t - i < PS) {
-                mma(kr[2 * m], r[i], g[m][t - i][0], g[m][t - i][1]);
-                mma(kr[2 * m + 1], r[i], g[m][t - i][2], g[m][t - i][3]);
-              }
+            for (int i = 0; i < PU; ++i)
+#pragma unroll
+              for (int m = 0; m < NT / 2; ++m)
+                if (t - i >= 0 && t - i < PS) {
+                  mma(kr[2 * m], r[i], g[m][t - i][0], g[m][t - i][1]);
+                  mma(kr[2 * m + 1], r[i], g[m][t - i][2], g[m][t - i][3]);
+                }
+        }
 #pragma unroll
         for (int c = 0; c < R::kBlocks; ++c) {
           if ((group >> 1) + c * R::kStep > rb) continue;
           if (group & 1)
-            mma_parts<PU, PU, PU>(X[c][0], X[c][1], u, x[c]);
+            add_parts<PU, PU, PU, kRound>(X[c][0], X[c][1], u, x[c]);
           else
-            mma_parts<PX, PU, PU>(X[c][0], X[c][1], dO, x[c]);
+            add_parts<PX, PU, PU, kRound>(X[c][0], X[c][1], dO, x[c]);
         }
         if (group == (v & (R::kGroups - 1))) {
           // dV = beta dU
@@ -504,12 +529,12 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
           if (j >= rb) ldsm_t(g[i], q_at + 2 * i * R::kTile + at);
         }
         if (j <= rb) {
-          mma_parts<PX, PX, PX>(dq[2 * m], dq[2 * m + 1], wa, f);
-          mma_parts<PX, PX, PX>(kr[2 * m], kr[2 * m + 1], na, f);
+          add_parts<PX, PX, PX, kRound>(dq[2 * m], dq[2 * m + 1], wa, f);
+          add_parts<PX, PX, PX, kRound>(kr[2 * m], kr[2 * m + 1], na, f);
         }
         if (j >= rb) {
-          mma_parts<PX, PX, PX>(kr[2 * m], kr[2 * m + 1], nt, f);
-          mma_parts<PX, PX, PX>(kr[2 * m], kr[2 * m + 1], wt, g);
+          add_parts<PX, PX, PX, kRound>(kr[2 * m], kr[2 * m + 1], nt, f);
+          add_parts<PX, PX, PX, kRound>(kr[2 * m], kr[2 * m + 1], wt, g);
         }
       }
     }

@@ -4,19 +4,19 @@
 // old state gives both S_old^T k and S_old^T q, one exchange through shared memory adds them up, and
 // the state is written from registers.
 //
-// Bound by HBM: 8 dk dv bytes per row and head.  Slices of 32 columns, so that one row of 16 heads of
-// 128 x 128 already fills 64 SMs; a thread holds up to 16 numbers of the state, all loaded before the
-// first is used.
+// Bound by HBM: 8 dk dv bytes per row and head.  Slices of 16 columns, so that one row of 16 heads of
+// 128 x 128 already fills 128 SMs, and many small CTAs, whose loads, exchanges and stores overlap; a thread
+// holds up to 16 numbers of the state, all loaded before the first is used.
 #include "delta_rule.cuh"
 
 namespace dynconv {
 namespace dr {
 namespace {
 
-constexpr int kThreads = 256, kSlice = 32;
+constexpr int kThreads = 128, kSlice = 16;
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, 5) delta_step_kernel(Step p) {
+__global__ void __launch_bounds__(kThreads, 10) delta_step_kernel(Step p) {
   constexpr int kLanes = kSlice / VEC;           // threads across a row
   constexpr int kGroups = kThreads / kLanes;     // rows at a time
   constexpr int kRows = kMaxKey / kGroups;       // rows per thread

@@ -118,6 +118,14 @@ struct Columns {
 // Whether a thread's share of a row is small enough to have the next row's loads under way meanwhile.
 constexpr bool ahead(int vec, int nv) { return vec * nv <= 8; }
 
+// CTAs of a backward that an SM runs at once.  Narrow rows: 512 threads of 100 to 114 registers, the next row under way
+// (gated, 16384 x 16 x 128: 74 us, and 79 at 80 registers and 768 threads; residual, 16384 x 2048: 108 us, 148 so, and
+// 123 with 1024 threads of 64 registers and one row at a time).
+__host__ __device__ constexpr int backward_ctas(int tpr) {
+  const int n = (cta(tpr) > 512 ? 1024 : 512) / cta(tpr);
+  return n < 1 ? 1 : n;
+}
+
 // Walks this CTA's rows: load(row, buffer) for each, the next one's before the work on the present one.
 template <typename Buf, int TPR, bool AHEAD, typename Load, typename Work>
 __device__ __forceinline__ void walk(int64_t rows, Load&& load, Work&& work) {
@@ -197,7 +205,7 @@ __global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
 }
 
 template <typename T, int VEC, int TPR, int NV>
-__global__ void __launch_bounds__(cta(TPR)) gated_bwd_kernel(Gated p) {
+__global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) gated_bwd_kernel(Gated p) {
   using V = Vec<T, VEC>;
   struct Buf {
     V x[NV], z[NV], d[NV];
@@ -336,7 +344,7 @@ __global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
 }
 
 template <typename T, int VEC, int TPR, int NV>
-__global__ void __launch_bounds__(cta(TPR)) residual_bwd_kernel(Residual p) {
+__global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_kernel(Residual p) {
   using V = Vec<T, VEC>;
   struct Buf {
     V h[NV], d[NV], u[NV], x[NV];
@@ -430,10 +438,10 @@ int vec_of(uintptr_t addresses, int64_t strides, int dtype) {
 }
 uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
-// CTAs of a launch: as many as run at once (2048 threads of an SM; backward half of that), no more than there is work for.
-int64_t grid_of(int64_t rows, int tpr, bool backward) {
+// CTAs of a launch: as many as run at once, no more than there is work for.
+int64_t grid_of(int64_t rows, int tpr, int per_sm) {
   const int64_t want = (rows * tpr + cta(tpr) - 1) / cta(tpr);
-  const int64_t most = (int64_t)sm_count() * (backward ? 1024 : 2048) / cta(tpr);
+  const int64_t most = (int64_t)sm_count() * per_sm;
   return want < most ? want : most;
 }
 
@@ -460,7 +468,7 @@ struct GatedGo {
   template <typename T, int VEC, int TPR, int NV>
   int operator()() const {
     Gated q = p;
-    const int64_t g = grid_of(q.N * q.G, TPR, backward);
+    const int64_t g = grid_of(q.N * q.G, TPR, backward ? backward_ctas(TPR) : 2048 / cta(TPR));
     if (!backward) {
       gated_fwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
       DYNCONV_CHECK_LAUNCH("gated_fwd_kernel");
@@ -483,7 +491,7 @@ struct ResidualGo {
   template <typename T, int VEC, int TPR, int NV>
   int operator()() const {
     Residual q = p;
-    const int64_t g = grid_of(q.N, TPR, backward);
+    const int64_t g = grid_of(q.N, TPR, backward ? backward_ctas(TPR) : 2048 / cta(TPR));
     if (!backward) {
       residual_fwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
       DYNCONV_CHECK_LAUNCH("residual_fwd_kernel");
