@@ -144,10 +144,11 @@ def gated_delta_rule(
         return_state:  also return the state after the last token, [B, H, dk, dv] float32.
 
     Returns:
-        o [B, T, H, dv], or (o, state).  Differentiable (once) in all tensors.  A token that holds a
-        number that is not finite makes its head's outputs from it on NaN and none before it.
-        With gradients the call keeps the state at every 64th token (float32: 32nd) and two numbers of
-        v's dtype (float32: one and a half) for each of v.
+        o [B, T, H, dv], or (o, state).  Differentiable (once) in all tensors.  What is not finite in
+        one token reaches no earlier token's output; from it on the head's are NaN (from a value: at
+        least its own columns').
+        With gradients the call keeps the state at every 64th token (float32: 32nd) in that type's digits and
+        four bytes (float32: six) for each number of v.
     """
     dev = q.get_device()  # (-1 on the CPU)
     assert dev >= 0 and k.get_device() == dev and v.get_device() == dev
