@@ -4,9 +4,11 @@
 // a slice of the state, transposed: warp w keeps 16 x (128 / W) of it in registers, fp32, in the accumulators' layout,
 // and works out 16 x (C / W) of what belongs to tokens.  What the others need of a warp's numbers
 // goes through shared memory as bf16 parts in the layout of first operands, 16 bytes per lane.  One thread,
-// of a warp of its own or, where the chains' warps take all registers, of the first team, brings the next chunks' tiles
-// by TMA into two or three stages.  (16-byte asynchronous copies by threads, of
-// one warp or four, took longer than a chunk's products: 10 to 20 bytes per cycle and SM.)
+// of a warp of its own or, where the chains' warps take all registers, of the first team's warp with the fewest blocks
+// of T, right behind a barrier of the team (before it, the whole team waited for the copies' start: 296 and 270 us
+// against 278 and 264 us for the chains at 4 x 4096 tokens, 16 heads of 128 x 128), brings the next chunks' tiles
+// by TMA into two or three stages.  (16-byte asynchronous copies by threads, of one warp or four, took longer than a
+// chunk's products: 10 to 20 bytes per cycle and SM.  Asking for the chunk after next into L2 as well: 316 and 319 us.)
 //
 // Why teams: one warp per slice, its numbers all in registers, took 7400 cycles for a chunk of 64 tokens
 // and 128 x 128 states, four times what its matrix instructions need: every instruction waited for the one

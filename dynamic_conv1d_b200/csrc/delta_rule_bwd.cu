@@ -25,11 +25,11 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
     if (l == 0) producer.template walk<true>();
     return;
   }
-  const bool produces = threadIdx.x == 0 && !plan.own_warp;
-  if (produces) producer.template start<true>();
   const int team = warp / W, w = (warp + team) % W;
   const int d0 = first_col + 16 * team, slices = (p.dv + 15) / 16, slice = d0 / 16;
   if (d0 >= p.dv) return;
+  const bool produces = !plan.own_warp && team == 0 && w == W - 1 && l == 0;  // (of the warp with the fewest blocks of T)
+  if (produces) producer.template start<true>();
   const int bytes = Ch::stage_bytes(plan.teams);
   uint4* const state = (uint4*)(smem + plan.stages * bytes + team * Ch::kTeam);
   uint4 *const part_x = state + Ch::kState / 16, *const part_o = part_x + Ch::kBlock / 16, *const part_u = part_o + Ch::kBlock / 16;
@@ -186,8 +186,8 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
       operand<NP>(scaled[0], scaled[1], a);
       Ch::put(part_o + blk * NP * 32, a);
     }
-    if (produces && c < chunks - 1) producer.template refill<true>(chunks - 1 - c);
     Ch::team_sync(team);
+    if (produces && c < chunks - 1) producer.template refill<true>(chunks - 1 - c);
     // dU^T = x^T T
 #pragma unroll
     for (int t = 0; t < TB; ++t) {

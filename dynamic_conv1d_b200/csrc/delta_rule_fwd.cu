@@ -24,11 +24,11 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
     if (l == 0) producer.template walk<false>();
     return;
   }
-  const bool produces = threadIdx.x == 0 && !plan.own_warp;
-  if (produces) producer.template start<false>();
   const int team = warp / W, w = (warp + team) % W;  // (turned, so that the last tokens' warps fall on different schedulers)
   const int d0 = first_col + 16 * team, slices = (p.dv + 15) / 16, slice = d0 / 16;
   if (d0 >= p.dv) return;
+  const bool produces = !plan.own_warp && team == 0 && w == 0 && l == 0;  // (of the warp with the fewest blocks of T)
+  if (produces) producer.template start<false>();
   const int bytes = Ch::stage_bytes(plan.teams);
   uint4* const state = (uint4*)(smem + plan.stages * bytes + team * Ch::kTeam);
   uint4 *const part_r = state + Ch::kState / 16, *const part_u = part_r + Ch::kBlock / 16, *const part_s = part_u + Ch::kBlock / 16;
@@ -171,8 +171,8 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
       Ch::put(part_r + Ch::token_block(w, t) * NP * 32, a);
     }
     // (another warp's tokens may be the bad ones)
-    if (produces && c > 0) producer.template refill<false>(c);
     if (!Ch::team_all(team, !odd_here)) bad = min(bad, Ch::bad_row(s, team, false));
+    if (produces && c > 0) producer.template refill<false>(c);
     // r^T = (V - e^b K S0)^T T^T, U = beta r
     float U[TB][2][4];
 #pragma unroll
