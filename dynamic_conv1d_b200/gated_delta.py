@@ -198,14 +198,16 @@ def gated_delta_rule_step(
     _check_gates(log_decay, beta, q, (B, H))
     n = _check_state(state, dev, None, H, dk, dv)
     assert slots is not None or n >= B
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state, log_decay, beta)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad
+                                    or log_decay.requires_grad or beta.requires_grad):
         _refuse_gradient()
     code = _lib.dtype_code(q.dtype)
     q, k, v = _dense(q), _dense(k), _dense(v)
     sp, sb = (None, 0) if slots is None else _slots(slots, B, dev)
-    o = torch.empty((B, H, dv), device=q.device, dtype=q.dtype)
-    strides = _Strides[10](*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *log_decay.stride(), *beta.stride())
+    (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
+    strides = _Strides[10](qb, qh, kb, kh, vb, vh, *log_decay.stride(), *beta.stride())
     with _lib.device_of(q):
+        o = v.new_empty((B, H, dv))
         status = _lib.load().dynconv_delta_step(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), o.data_ptr(), sp, sb,
             strides, B, n, H, dk, dv, dk**-0.5 if scale is None else float(scale), code, _lib.raw_stream(q))

@@ -44,6 +44,9 @@ def _rows(t: torch.Tensor):
 
 def _pair(x, gate):
     """x and gate over the same split of their rows: (x, gate, N, G, strides)."""
+    if x.is_contiguous() and (gate is None or gate.is_contiguous()):
+        D = x.shape[-1]
+        return x, gate, x.numel() // D if D else 0, 1, _Strides4(D, 0, D, 0)
     x, n, g, xo, xi = _rows(x)
     if gate is None:
         return x, None, n, g, _Strides4(xo, xi, 0, 0)
@@ -69,7 +72,7 @@ def _gated_forward(x, weight, gate, eps, scale):
     lib = _lib.load()
     code = _lib.dtype_code(x.dtype)
     with _lib.device_of(x):
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        y = x.new_empty(x.shape)
         status = lib.dynconv_gated_norm_fwd(x.data_ptr(), _ptr(weight), _ptr(gate), y.data_ptr(), strides, n, g, x.shape[-1],
                                             eps, scale, code, _lib.raw_stream(x))
         if status:
@@ -96,8 +99,8 @@ class _GatedRmsNormFn(torch.autograd.Function):
         with _lib.device_of(x):
             dy = dy.contiguous()
             want_x, want_w, want_g = ctx.needs_input_grad[:3]
-            new = lambda: torch.empty(x.shape, device=x.device, dtype=x.dtype)  # noqa: E731
-            dx, dg = new() if want_x else None, new() if want_g else None
+            dx = x.new_empty(x.shape) if want_x else None
+            dg = x.new_empty(x.shape) if want_g else None
             dw = torch.empty_like(weight) if want_w else None
             ws, nbytes = _sum_workspace(lib, x, x.shape[-1], 1) if want_w else (None, 0)
             status = lib.dynconv_gated_norm_bwd(
