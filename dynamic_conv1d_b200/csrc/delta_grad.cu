@@ -7,6 +7,10 @@
 // These become W and N, which go through shared memory into the products with K and Q; their products with
 // Q K^T and K K^T, entry by entry, are what the log decays' gradients are sums of.  Row sums and column sums
 // of the same numbers are taken, so what has to cancel does.
+//
+// 4 x 4096 tokens, 16 heads of 128 x 128: 440 us for 0.9 GB, bound by its instructions (eight warps of up to 255 registers,
+// a CTA to an SM: issue 32%, matrix units 34%, DRAM 24%); sixteen warps of half as much each took 460 us.
+// Items go heads first, since the heads of the same tokens share what they read.
 #include "delta_rule.cuh"
 
 namespace dynconv {

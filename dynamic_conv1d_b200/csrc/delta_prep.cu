@@ -1,6 +1,12 @@
 // delta_prep.cu -- what the chunks of the gated delta rule need before their state is known: the gates, and
 // from K and Q the triangular matrices T and P (formulas: delta_rule.cuh).  A CTA of four warps per
-// chunk and head.
+// chunk and head, heads of the same tokens side by side, since they share the rows of K and Q that a fused projection
+// lays out together; five CTAs on an SM, so that one's products fill the other's barriers.  Apart from the chains,
+// because T needs nothing of them: as helper warps of a chain's CTA the same work held up the chain (440 against
+// 360 us for the forward).
+//
+// 4 x 4096 tokens, 16 heads of 128: 63 us for 134 MB read and 90 MB written; bound by its barriers and by the
+// instructions that split numbers into parts (issue 46%, DRAM 25%), not by memory.  32768 tokens with three parts: 145 us.
 #include "delta_rule.cuh"
 
 namespace dynconv {

@@ -1,6 +1,9 @@
 // delta_rule_bwd.cu -- the gradients' chain of the gated delta rule: dS of every chunk and dU, from the last chunk to the
 // first (formulas: delta_rule.cuh; how the warps share the work: delta_chain.cuh).  The gradients themselves
 // follow from these chunk by chunk (delta_grad.cu).
+//
+// Bound as the forward's chain is, each chunk being P^T dO and K dS, then T^T x, then the products with Q and K that
+// the state takes: 264 us for 4 x 4096 tokens, 16 heads of 128 x 128 (matrix units 52% active, issue 45%).
 #include "delta_chain.cuh"
 
 namespace dynconv {

@@ -1,5 +1,10 @@
 // delta_rule_fwd.cu -- the gated delta rule over whole sequences: the chain over the chunks (formulas:
 // delta_rule.cuh; how the warps share the work: delta_chain.cuh).
+//
+// Bound by the chunks' order: each is three products in a row, K S0 and Q S0, then T x, then P U and K^T U.  4 x 4096 tokens, 16
+// heads of 128 x 128, states kept: 278 us, 4.3 us for 64 tokens of four teams (matrix units 45% active, issue 43%:
+// warps wait for shared memory and for the instruction before).  One row of 32768 tokens, a team to a CTA and an
+// exact state: 1.05 ms, 2.05 us a chunk.
 #include "delta_chain.cuh"
 
 namespace dynconv {
