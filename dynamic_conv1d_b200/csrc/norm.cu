@@ -12,10 +12,13 @@
 // the row gives them and nothing is kept from the forward but h, which the caller has anyway.
 //
 // Bound by HBM: a row is read once into registers (up to 16 numbers per thread) and written once; sums
-// are fp32.  A row belongs to 8..32 lanes of a warp, or to a whole CTA of 256 to 1024 threads above
+// are fp32.  A row belongs to 8..32 lanes of a warp, or to a whole CTA of 128 to 1024 threads above
 // 512 channels.  The sums over rows stay in the threads that own their columns; the CTAs'
 // partial rows are added up in a fixed order by a second launch, so results do not change from
 // run to run.
+//
+// 16384 rows of 2048 in bf16: residual norm 50 us forward (5.4 TB/s), 65 us back (6.2 TB/s); 16384 x 16 rows of 128:
+// gated norm 41 us forward (4.9 TB/s), 74 us back (4.5 TB/s: its instructions, issue 75%).
 #include "common.cuh"
 #include "norm.cuh"
 
@@ -57,7 +60,7 @@ __device__ __forceinline__ float2 row_sum(float2 v, int& flip) {
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 
 // Threads of a CTA for a row of TPR threads.
-__host__ __device__ constexpr int cta(int tpr) { return tpr < 256 ? 256 : tpr; }
+__host__ __device__ constexpr int cta(int tpr) { return tpr <= 32 ? 256 : tpr; }
 
 // The sums over this CTA's rows: thread (row group, lane) holds N_ACC columns; groups are added in
 // order through shared memory and the result is the CTA's row of `part`.
@@ -118,9 +121,8 @@ struct Columns {
 // Whether a thread's share of a row is small enough to have the next row's loads under way meanwhile.
 constexpr bool ahead(int vec, int nv) { return vec * nv <= 8; }
 
-// CTAs of a backward that an SM runs at once.  Narrow rows: 512 threads of 100 to 114 registers, the next row under way
-// (gated, 16384 x 16 x 128: 74 us, and 79 at 80 registers and 768 threads; residual, 16384 x 2048: 108 us, 148 so, and
-// 123 with 1024 threads of 64 registers and one row at a time).
+// CTAs of a backward that an SM runs at once.  Narrow rows: 512 threads of 100 to 128 registers, the next rows under way
+// (gated, 16384 x 16 x 128: 74 us, and 79 at 80 registers and 768 threads).
 __host__ __device__ constexpr int backward_ctas(int tpr) {
   const int n = (cta(tpr) > 512 ? 1024 : 512) / cta(tpr);
   return n < 1 ? 1 : n;
@@ -144,6 +146,28 @@ __device__ __forceinline__ void walk(int64_t rows, Load&& load, Work&& work) {
       load(row, now);
       work(row, now);
     }
+  }
+}
+
+// The same with the rows to come in shared memory: each thread copies its own pieces of 16 bytes asynchronously and reads
+// them back itself, so nothing but its own copies has to be waited for, and rows under way cost no registers.
+// start(row, slot) asks for a row's pieces, work(row, slot) has them.
+template <int TPR, int STAGES, typename Start, typename Work>
+__device__ __forceinline__ void walk_ring(int64_t rows, Start&& start, Work&& work) {
+  constexpr int kRows = cta(TPR) / TPR;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR, first = (int64_t)blockIdx.x * kRows;
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    start(row + i * step, i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  for (int slot = 0; first < rows; first += step, row += step) {
+    start(row + (STAGES - 1) * step, slot == 0 ? STAGES - 1 : slot - 1);  // (the slot that the row before this one had)
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    work(row, slot);
+    slot = slot == STAGES - 1 ? 0 : slot + 1;
   }
 }
 
@@ -343,64 +367,110 @@ __global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
       });
 }
 
+// The backward's rows in shared memory: four tensors' pieces for each thread, as many rows as the CTAs' shares of an SM's
+// shared memory hold, at most four; none (0) where a piece is not 16 bytes or two rows do not fit.  Of 2-byte
+// types alone: 16384 x 2048 in bf16 takes 65 us so and 105 us with one row ahead in registers (3 CTAs on an SM instead
+// of 2: 74 us); of 4-byte types the registers' row is enough already, 62 us for 8192 x 2048 and 66 us with the ring.
+template <typename T, int VEC, int TPR, int NV>
+struct Ring {
+  static constexpr int kSlot = 4 * NV * cta(TPR) * 16, kFit = 208 * 1024 / backward_ctas(TPR) / kSlot;
+  static constexpr int kStages = sizeof(T) != 2 || VEC != 8 || kFit < 2 ? 0 : kFit < 4 ? kFit : 4;
+  static constexpr int kBytes = kStages * kSlot;
+};
+
 template <typename T, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_kernel(Residual p) {
   using V = Vec<T, VEC>;
+  using R = Ring<T, VEC, TPR, NV>;
   struct Buf {
     V h[NV], d[NV], u[NV], x[NV];
   };
+  extern __shared__ __align__(16) uint8_t ring[];
   const int lane = threadIdx.x % TPR;
   int flip = 0;
   float acc_w[NV * VEC], acc_s[NV * VEC];
   const Columns<T, VEC, TPR, NV> w(p.weight, lane, p.D), sc(p.scale, lane, p.D);
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc_w[i] = acc_s[i] = 0.f;
-  walk<Buf, TPR, ahead(VEC, NV)>(
-      p.N,
-      [&](int64_t row, Buf& a) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int c = (i * TPR + lane) * VEC;
-          if (row < p.N && c < p.D) {
-            a.h[i] = *reinterpret_cast<const V*>((const T*)p.h + row * p.D + c);
-            a.d[i] = p.dy ? *reinterpret_cast<const V*>((const T*)p.dy + row * p.D + c) : V{};
-            a.u[i] = p.dh ? *reinterpret_cast<const V*>((const T*)p.dh + row * p.D + c) : V{};
-            if (p.part_s) a.x[i] = *reinterpret_cast<const V*>((const T*)p.x + row * p.D + c);
-          }
-        }
-      },
-      [&](int64_t row, const Buf& a) {
-        const bool in = row < p.N;
-        float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (in && (i * TPR + lane) * VEC < p.D)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const float v = Elem<T>::to_f(a.h[i].e[e]);
-              s.x = fmaf(v, v, s.x);
-              s.y = fmaf(Elem<T>::to_f(a.d[i].e[e]) * Elem<T>::to_f(w[i].e[e]), v, s.y);
+  auto work = [&](int64_t row, const Buf& a) {
+            const bool in = row < p.N;
+            float2 s = make_float2(0.f, 0.f);
+    #pragma unroll
+            for (int i = 0; i < NV; ++i)
+              if (in && (i * TPR + lane) * VEC < p.D)
+    #pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                  const float v = Elem<T>::to_f(a.h[i].e[e]);
+                  s.x = fmaf(v, v, s.x);
+                  s.y = fmaf(Elem<T>::to_f(a.d[i].e[e]) * Elem<T>::to_f(w[i].e[e]), v, s.y);
+                }
+            s = row_sum<TPR>(s, flip);
+            const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
+    #pragma unroll
+            for (int i = 0; i < NV; ++i) {
+              const int c = (i * TPR + lane) * VEC;
+              if (!in || c >= p.D) continue;
+              V dt, dx;
+    #pragma unroll
+              for (int e = 0; e < VEC; ++e) {
+                const float v = Elem<T>::to_f(a.h[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
+                const float t = fmaf(r, fmaf(d, Elem<T>::to_f(w[i].e[e]), -v * m), Elem<T>::to_f(a.u[i].e[e]));
+                dt.e[e] = Elem<T>::from_f(t);
+                dx.e[e] = Elem<T>::from_f(t * (p.scale ? Elem<T>::to_f(sc[i].e[e]) : p.factor));
+                acc_w[i * VEC + e] = fmaf(d, v * r, acc_w[i * VEC + e]);
+                if (p.part_s) acc_s[i * VEC + e] = fmaf(t, Elem<T>::to_f(a.x[i].e[e]), acc_s[i * VEC + e]);
+              }
+              if (p.dresidual) *reinterpret_cast<V*>((T*)p.dresidual + row * p.D + c) = dt;
+              if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
             }
-        s = row_sum<TPR>(s, flip);
-        const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
+  };
+  if constexpr (R::kStages > 0) {
+    auto at = [&](int slot, int tensor, int i) { return ring + slot * R::kSlot + ((tensor * NV + i) * cta(TPR) + threadIdx.x) * 16; };
+    auto copy = [&](int slot, int tensor, int i, const void* from, int64_t n) {
+      if (from)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(at(slot, tensor, i))), "l"((const T*)from + n) : "memory");
+    };
+    walk_ring<TPR, R::kStages>(
+        p.N,
+        [&](int64_t row, int slot) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int c = (i * TPR + lane) * VEC;
-          if (!in || c >= p.D) continue;
-          V dt, dx;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float v = Elem<T>::to_f(a.h[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
-            const float t = fmaf(r, fmaf(d, Elem<T>::to_f(w[i].e[e]), -v * m), Elem<T>::to_f(a.u[i].e[e]));
-            dt.e[e] = Elem<T>::from_f(t);
-            dx.e[e] = Elem<T>::from_f(t * (p.scale ? Elem<T>::to_f(sc[i].e[e]) : p.factor));
-            acc_w[i * VEC + e] = fmaf(d, v * r, acc_w[i * VEC + e]);
-            if (p.part_s) acc_s[i * VEC + e] = fmaf(t, Elem<T>::to_f(a.x[i].e[e]), acc_s[i * VEC + e]);
+          for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + lane) * VEC;
+            if (row < p.N && c < p.D) {
+              const int64_t n = row * p.D + c;
+              copy(slot, 0, i, p.h, n), copy(slot, 1, i, p.dy, n), copy(slot, 2, i, p.dh, n);
+              copy(slot, 3, i, p.part_s ? p.x : nullptr, n);
+            }
           }
-          if (p.dresidual) *reinterpret_cast<V*>((T*)p.dresidual + row * p.D + c) = dt;
-          if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
-        }
-      });
+        },
+        [&](int64_t row, int slot) {
+          Buf a;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            a.h[i] = *reinterpret_cast<const V*>(at(slot, 0, i));
+            a.d[i] = p.dy ? *reinterpret_cast<const V*>(at(slot, 1, i)) : V{};
+            a.u[i] = p.dh ? *reinterpret_cast<const V*>(at(slot, 2, i)) : V{};
+            a.x[i] = *reinterpret_cast<const V*>(at(slot, 3, i));
+          }
+          work(row, a);
+        });
+  } else {
+    walk<Buf, TPR, ahead(VEC, NV)>(
+        p.N,
+        [&](int64_t row, Buf& a) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + lane) * VEC;
+            if (row < p.N && c < p.D) {
+              a.h[i] = *reinterpret_cast<const V*>((const T*)p.h + row * p.D + c);
+              a.d[i] = p.dy ? *reinterpret_cast<const V*>((const T*)p.dy + row * p.D + c) : V{};
+              a.u[i] = p.dh ? *reinterpret_cast<const V*>((const T*)p.dh + row * p.D + c) : V{};
+              if (p.part_s) a.x[i] = *reinterpret_cast<const V*>((const T*)p.x + row * p.D + c);
+            }
+          }
+        },
+        work);
+  }
   if (p.part_w) store_sums<TPR, VEC, NV>(acc_w, p.part_w + (int64_t)blockIdx.x * p.D, p.D);
   if (p.part_s) store_sums<TPR, VEC, NV>(acc_s, p.part_s + (int64_t)blockIdx.x * p.D, p.D);
 }
@@ -446,7 +516,9 @@ int64_t grid_of(int64_t rows, int tpr, int per_sm) {
 }
 
 // Threads of a row: the fewest that hold it at VEC x NV numbers each, where narrow rows take one
-// vector each (more rows in flight), up to a warp, and wide ones a CTA.
+// vector each (more rows in flight), up to a warp, and wide ones a CTA.  Rows of 513 to 4096 numbers have 8 of them in
+// a thread: 32768 rows of 1024 in bf16 take 48 us forward and 71 us back with 128 threads (72 and 89 us with 256, half
+// of them idle), 8192 rows of 4096 61 and 74 us with 512 (56 and 93 us with 256 of 16 numbers).
 template <typename T, int VEC, typename F>
 int pick(int64_t D, F&& go) {
   constexpr int kNV = kPerThread / VEC;
@@ -455,8 +527,9 @@ int pick(int64_t D, F&& go) {
   if (D <= 16 * VEC * kOne) return go.template operator()<T, VEC, 16, kOne>();
   if (D <= 32 * VEC * kOne) return go.template operator()<T, VEC, 32, kOne>();
   if (D <= 32 * kPerThread) return go.template operator()<T, VEC, 32, kNV>();
+  if (D <= 128 * kPerThread / 2) return go.template operator()<T, VEC, 128, kNV / 2>();
   if (D <= 256 * kPerThread / 2) return go.template operator()<T, VEC, 256, kNV / 2>();
-  if (D <= 256 * kPerThread) return go.template operator()<T, VEC, 256, kNV>();
+  if (D <= 512 * kPerThread / 2) return go.template operator()<T, VEC, 512, kNV / 2>();
   if (D <= 512 * kPerThread) return go.template operator()<T, VEC, 512, kNV>();
   return go.template operator()<T, VEC, 1024, kNV>();
 }
@@ -491,13 +564,21 @@ struct ResidualGo {
   template <typename T, int VEC, int TPR, int NV>
   int operator()() const {
     Residual q = p;
+    using R = Ring<T, VEC, TPR, NV>;
     const int64_t g = grid_of(q.N, TPR, backward ? backward_ctas(TPR) : 2048 / cta(TPR));
     if (!backward) {
       residual_fwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
       DYNCONV_CHECK_LAUNCH("residual_fwd_kernel");
       return DYNCONV_OK;
     }
-    residual_bwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+    if (R::kBytes) {
+      const cudaError_t e = cudaFuncSetAttribute(residual_bwd_kernel<T, VEC, TPR, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_status(e, "cudaFuncSetAttribute(residual_bwd)");
+      }
+    }
+    residual_bwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), R::kBytes, st>>>(q);
     DYNCONV_CHECK_LAUNCH("residual_bwd_kernel");
     if (q.part_w || q.part_s) {
       const float *a = q.part_w, *b = q.part_s;

@@ -206,3 +206,21 @@ def test_refusals():
     (g,) = torch.autograd.grad(gated_rms_norm(a).sum(), a, create_graph=True)
     with pytest.raises(RuntimeError, match="cannot be differentiated again"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("which", ["both", "y", "h"])
+@pytest.mark.parametrize("N,D", [(48001, 64), (9001, 520), (5003, 1024), (2502, 2048), (1203, 4096), (907, 8192)])
+def test_residual_rows_in_turn(N, D, which):
+    """So many rows that a CTA's places in shared memory are used several times over, with one upstream gradient or both."""
+    x, r, dy, dh = (rnd(N, D, dtype=BF16, seed=i) for i in range(4))
+    w, s = 1 + rnd(D, dtype=BF16, seed=5) / 4, 0.5 + rnd(D, dtype=BF16, seed=6) / 8
+    own, ref = [t.detach().requires_grad_() for t in (x, r, w, s)], [t.detach().double().requires_grad_() for t in (x, r, w, s)]
+    y, h = residual_rms_norm(*own, eps=1e-6)
+    ry, rh = residual(*ref, 1e-6)
+    outs, ups = {"both": ([0, 1], (dy, dh)), "y": ([0], (dy,)), "h": ([1], (dh,))}[which]
+    leaves = [i for i in range(4) if which != "h" or i != 2]  # (h does not depend on the weight)
+    got = torch.autograd.grad([(y, h)[i] for i in outs], [own[i] for i in leaves], ups)
+    want = torch.autograd.grad([(ry, rh)[i] for i in outs], [ref[i] for i in leaves], [u.double() for u in ups])
+    for i, a, b in zip(leaves, got, want):
+        # (a CTA adds 48001 / 9472 to 907 / 148 rows one after another, column sums of at most 592 follow: rounding to bf16 counts alone)
+        assert rel(a, b) <= SUM_TOL[BF16], "xrws"[i]
