@@ -58,6 +58,17 @@ int check_dtype(int dtype);
 // Counts kernel launches (dynconv_launch_count) -- call once per launch.
 void note_launch(int n = 1);
 
+// Lets `kern` be launched with up to `bytes` of dynamic shared memory.  The limit belongs to the function, for all
+// threads of the process: every call for a kernel gives the same number, the most that any launch of it takes.  (With
+// each launch's own need, another thread's smaller one could lower the limit between this call and the launch.)
+template <typename K>
+int allow_shared(K* kern, int bytes, const char* what) {
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) return DYNCONV_OK;
+  cudaGetLastError();  // do not leave the failure pending for the next launch check
+  return cuda_status(e, what);
+}
+
 #define DYNCONV_CHECK_LAUNCH(what)                                  \
   do {                                                              \
     cudaError_t e__ = cudaGetLastError();                           \

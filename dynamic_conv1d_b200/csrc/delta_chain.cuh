@@ -46,6 +46,8 @@ struct Chain {
     return (2 * kKq + teams * kV + kT + kP + kGates + 1023) / 1024 * 1024;
   }
   static constexpr int smem_bytes(int teams, int stages) { return 1024 + stages * stage_bytes(teams) + teams * kTeam; }
+  static constexpr int kMostBytes = 227 * 1024 - 1024;  // of any plan (the rest: barriers)
+  static_assert(smem_bytes(1, 2) <= kMostBytes, "the smallest plan");
 
   struct Stage {
     uint8_t* at;
@@ -202,13 +204,12 @@ int chain_maps(Maps* maps, const Prepared& pre, const View& k, const View& q, co
 // memory.
 template <typename Ch>
 Plan plan_of(int64_t bh, int dv) {
-  constexpr int kMost = 227 * 1024 - 1024;  // (barriers)
   const int slices = (dv + 15) / 16;
   Plan p{};
   p.teams = 1;
-  while (2 * p.teams <= Ch::kMostTeams && Ch::smem_bytes(2 * p.teams, 2) <= kMost && bh * ((slices + p.teams - 1) / p.teams) > sm_count())
+  while (2 * p.teams <= Ch::kMostTeams && Ch::smem_bytes(2 * p.teams, 2) <= Ch::kMostBytes && bh * ((slices + p.teams - 1) / p.teams) > sm_count())
     p.teams *= 2;
-  p.stages = Ch::smem_bytes(p.teams, 3) <= kMost ? 3 : 2;
+  p.stages = Ch::smem_bytes(p.teams, 3) <= Ch::kMostBytes ? 3 : 2;
   p.own_warp = p.teams < Ch::kMostTeams;
   return p;
 }

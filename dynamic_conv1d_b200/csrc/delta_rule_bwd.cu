@@ -287,11 +287,7 @@ int go(const Backward& p, const Plan& plan, cudaStream_t st) {
   using Ch = Chain<G, W, KK>;
   int s;
   const int slices = (p.dv + 15) / 16, smem = Ch::smem_bytes(plan.teams, plan.stages);
-  const cudaError_t e = cudaFuncSetAttribute(delta_bwd_kernel<G, W, KK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return cuda_status(e, "cudaFuncSetAttribute(delta_bwd)");
-  }
+  if ((s = allow_shared(delta_bwd_kernel<G, W, KK>, Ch::kMostBytes, "cudaFuncSetAttribute(delta_bwd)"))) return s;
   Maps maps{};
   if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.d_o, p.B, p.T, p.H, p.dk, p.dv, plan.teams))) return s;
   const dim3 grid((unsigned)((slices + plan.teams - 1) / plan.teams), (unsigned)(p.B * p.H));

@@ -336,11 +336,7 @@ int go(const Forward& p, Plan plan, cudaStream_t st) {
   const int slices = (p.dv + 15) / 16;
   plan.o_vectors = vectors_of(p.o, p.dv, sizeof(typename G::T));
   const int smem = Ch::smem_bytes(plan.teams, plan.stages);
-  const cudaError_t e = cudaFuncSetAttribute(delta_fwd_kernel<G, W, KK, SAVE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return cuda_status(e, "cudaFuncSetAttribute(delta_fwd)");
-  }
+  if ((s = allow_shared(delta_fwd_kernel<G, W, KK, SAVE>, Ch::kMostBytes, "cudaFuncSetAttribute(delta_fwd)"))) return s;
   Maps maps{};
   if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.v, p.B, p.T, p.H, p.dk, p.dv, plan.teams))) return s;
   const dim3 grid((unsigned)((slices + plan.teams - 1) / plan.teams), (unsigned)(p.B * p.H));

@@ -416,11 +416,8 @@ int simple_go(const Params& p, cudaStream_t st) {
     dw = p.role[r].dw > dw ? p.role[r].dw : dw;
   }
   const size_t smem = simple_smem_floats(dx) * sizeof(float);
-  cudaError_t e = cudaFuncSetAttribute(la_simple_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return cuda_status(e, "cudaFuncSetAttribute(la_simple)");
-  }
+  constexpr int kMost = (int)(simple_smem_floats(kMaxDim) * sizeof(float));
+  if (int s = allow_shared(la_simple_kernel<T>, kMost, "cudaFuncSetAttribute(la_simple)")) return s;
   const int n_slices = (dw + kSlice - 1) / kSlice;
   const int64_t blocks = (int64_t)p.n_roles * p.n_seg * p.B * p.H * n_slices;
   if (blocks > INT32_MAX) return set_error(DYNCONV_ERR_SHAPE, "linear attention: B*H too large");

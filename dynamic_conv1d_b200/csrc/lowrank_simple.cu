@@ -282,24 +282,25 @@ int64_t lr_simple_partial_rows(int64_t B, int64_t T) { return (B * T + kDuChunk 
 
 namespace {
 
+// Floats of shared memory of the two tiled kernels.
+constexpr size_t kx_floats(int W, int Rk) { return (size_t)Rk * W * kKxCh + (size_t)(kKxTok + W - 1) * Rk; }
+constexpr size_t dz_floats(int W, int R) {
+  return (size_t)((R + 7) / 8 * 8 + 4) * W * kDzCh + (size_t)W * kDzTok * kDzPad + (size_t)kDzTok * kDzPad +
+         (size_t)(kDzTok + W - 1) * kDzPad + (size_t)8 * kDzTok * 8;
+}
+// A launch of `floats`, of `most` at the widest rank, needs leave for more than 48 KB.
 template <typename K>
-int set_smem(K kern, size_t bytes, const char* what) {
-  if (bytes <= 48 * 1024) return DYNCONV_OK;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return cuda_status(e, what);
-  }
-  return DYNCONV_OK;
+int set_smem(K* kern, size_t floats, size_t most, const char* what) {
+  return floats * sizeof(float) <= 48 * 1024 ? DYNCONV_OK : allow_shared(kern, (int)(most * sizeof(float)), what);
 }
 
 template <typename E, bool DX, int W>
 int launch_kx_w(const void* xin, const void* z, const void* U, const void* sw, void* out, int64_t B, int64_t Tlen,
                 int64_t D, int R, int Rk, int residual, cudaStream_t st) {
   const int64_t ntok = B * Tlen;
-  const size_t smem = ((size_t)Rk * W * kKxCh + (size_t)(kKxTok + W - 1) * Rk) * sizeof(float);
+  const size_t smem = kx_floats(W, Rk) * sizeof(float);
   auto kern = lr_kx_tiled_kernel<E, DX, W>;
-  if (int s = set_smem(kern, smem, "cudaFuncSetAttribute(lr_kx_tiled)")) return s;
+  if (int s = set_smem(kern, kx_floats(W, Rk), kx_floats(W, kMaxRk), "cudaFuncSetAttribute(lr_kx_tiled)")) return s;
   dim3 grid((unsigned)((D + kKxCh - 1) / kKxCh), (unsigned)((ntok + kKxTok - 1) / kKxTok));
   kern<<<grid, 256, smem, st>>>((const E*)xin, (const E*)z, (const E*)U, (const E*)sw, (E*)out, ntok, (int)Tlen, (int)D,
                                 R, Rk, residual);
@@ -327,11 +328,9 @@ template <typename E, int W>
 int launch_dz_w(const void* x, const void* U, const void* dy, void* dz, int64_t B, int64_t Tlen, int64_t D, int R,
                 cudaStream_t st) {
   const int64_t ntok = B * Tlen;
-  const size_t smem = ((size_t)((R + 7) / 8 * 8 + 4) * W * kDzCh + (size_t)W * kDzTok * kDzPad +
-                       (size_t)kDzTok * kDzPad + (size_t)(kDzTok + W - 1) * kDzPad + (size_t)8 * kDzTok * 8) *
-                      sizeof(float);
+  const size_t smem = dz_floats(W, R) * sizeof(float);
   auto kern = lr_dz_tiled_kernel<E, W>;
-  if (int s = set_smem(kern, smem, "cudaFuncSetAttribute(lr_dz_tiled)")) return s;
+  if (int s = set_smem(kern, dz_floats(W, R), dz_floats(W, kMaxRk), "cudaFuncSetAttribute(lr_dz_tiled)")) return s;
   kern<<<(unsigned)((ntok + kDzTok - 1) / kDzTok), 256, smem, st>>>((const E*)x, (const E*)U, (const E*)dy, (E*)dz,
                                                                     ntok, (int)Tlen, (int)D, R);
   DYNCONV_CHECK_LAUNCH("lr_dz_tiled_kernel");
