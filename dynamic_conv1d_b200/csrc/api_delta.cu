@@ -10,7 +10,14 @@
 namespace dynconv {
 namespace {
 
-constexpr int64_t kMaxRows = 65535;  // batch rows of a step, B*H of a sequence (grid limits)
+constexpr int64_t kMaxRows = 65535;  // grid limits: batch rows and heads of a step, their product in a sequence
+
+int check_widths(int64_t dk, int64_t dv) {
+  if (dk < 1 || dk > dr::kMaxKey || dv < 1 || dv > dr::kMaxValue)
+    return set_error(DYNCONV_ERR_UNSUPPORTED, "gated delta rule: dk=%lld (1..%d), dv=%lld (1..%d)", (long long)dk, dr::kMaxKey,
+                     (long long)dv, dr::kMaxValue);
+  return DYNCONV_OK;
+}
 
 int check_rule(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype) {
   int s;
@@ -18,10 +25,7 @@ int check_rule(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtyp
   if (B < 0 || T < 0 || H <= 0 || H > kMaxRows || B * H > kMaxRows || T > (1 << 30))
     return set_error(DYNCONV_ERR_SHAPE, "gated delta rule: bad sizes B=%lld T=%lld H=%lld", (long long)B, (long long)T,
                      (long long)H);
-  if (dk < 1 || dk > dr::kMaxKey || dv < 1 || dv > dr::kMaxValue)
-    return set_error(DYNCONV_ERR_UNSUPPORTED, "gated delta rule: dk=%lld (1..%d), dv=%lld (1..%d)", (long long)dk, dr::kMaxKey,
-                     (long long)dv, dr::kMaxValue);
-  return DYNCONV_OK;
+  return check_widths(dk, dv);
 }
 
 dr::View view(const void* p, const int64_t* strides, int i) {
@@ -71,7 +75,10 @@ int dynconv_delta_step(const void* q, const void* k, const void* v, const void* 
                        int64_t H, int64_t dk, int64_t dv, float scale, int dtype, void* stream) {
   int s;
   if ((s = op_entry((cudaStream_t)stream))) return s;
-  if ((s = check_rule(B, 1, H, dk, dv, dtype))) return s;
+  if ((s = check_dtype(dtype))) return s;
+  if (B < 0 || B > kMaxRows || H <= 0 || H > kMaxRows)
+    return set_error(DYNCONV_ERR_SHAPE, "delta_step: bad sizes B=%lld H=%lld", (long long)B, (long long)H);
+  if ((s = check_widths(dk, dv))) return s;
   if (slots && slot_bytes != 4 && slot_bytes != 8)
     return set_error(DYNCONV_ERR_ARGUMENT, "delta_step: slots of %d bytes (expected 4 or 8)", slot_bytes);
   if (n_rows < 0 || (!slots && n_rows < B))

@@ -136,6 +136,7 @@ def gated_delta_rule(
         q, k:          [B, T, H, dk] (bfloat16 or float32, CUDA; any strides of batch, time and
                        head, so views of a fused projection are read in place).  dk <= 128.  Keys
                        are meant to have a length of at most one (``gated_rms_norm`` gives them it).
+                       B * H <= 65535.
         v:             [B, T, H, dv], dv <= 256.
         log_decay:     [B, T, H] in q's dtype, the logarithm of each token's decay, <= 0.
         beta:          [B, T, H] in q's dtype, the share of the value that is replaced.
@@ -181,6 +182,7 @@ def gated_delta_rule_step(
 
     Args:
         q, k:            [B, H, dk], v: [B, H, dv] (bfloat16 or float32; views of a fused row will do).
+                         B and H up to 65535 each.
         state:           [n, H, dk, dv] float32, contiguous; updated in place.
         log_decay, beta: [B, H] in q's dtype.
         slots:           [B] int32 or int64, each sequence's row of the state, none twice; rows

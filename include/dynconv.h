@@ -318,7 +318,7 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
  *   v_t - a_t S_{t-1}^T k_t.
  * The workspace and kept are 16-byte aligned, and so are bf16 (float32) tensors whose width is a multiple of 8 (4),
  * rows and all (DYNCONV_ERR_ALIGN); other widths are read through copies in the workspace.
- * dk in 1..128, dv in 1..256, B*H <= 65535, T <= 2^30.  T = 0 copies the state.  What is not finite in one
+ * dk in 1..128, dv in 1..256, B*H <= 65535 (the step: below), T <= 2^30.  T = 0 copies the state.  What is not finite in one
  * token reaches no earlier token's output; from it on the head's are NaN (from a value: at least its own columns'). */
 size_t dynconv_delta_kept_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype);
 size_t dynconv_delta_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype, int backward);
@@ -336,7 +336,7 @@ int dynconv_delta_bwd(const void* q, const void* k, const void* log_decay, const
                       int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, float scale, int dtype, void* stream);
 /* One token for B sequences: q, k [B,H,dk], v [B,H,dv], log_decay, beta [B,H] (`strides`: batch and
  * head of the five, 10 numbers), o [B,H,dv] dense, state [n_rows,H,dk,dv] float32 updated in place;
- * slots as for dynconv_lr_step. */
+ * slots as for dynconv_lr_step.  B and H up to 65535 each. */
 int dynconv_delta_step(const void* q, const void* k, const void* v, const void* log_decay, const void* beta,
                        float* state, void* o, const void* slots, int slot_bytes, const int64_t* strides,
                        int64_t B, int64_t n_rows, int64_t H, int64_t dk, int64_t dv, float scale, int dtype, void* stream);

@@ -111,3 +111,11 @@ def test_layer_arguments():
     steps = torch.nn.functional.softplus(m.dt_bias)
     assert ((steps > 9e-4) & (steps < 0.11)).all()
     assert dc.ResidualRMSNorm(8).scale is None and dc.ResidualRMSNorm(8, layer_scale=0.5).scale.shape == (8,)
+
+
+def test_step_sizes():
+    """A step's sequences and heads are bounded each by itself: their product is no dimension of its grid."""
+    lib = _lib.load()
+    step = lambda B, H: lib.dynconv_delta_step(*([None] * 7), None, 0, None, B, B, H, 64, 64, 1.0, 0, None)  # noqa: E731
+    assert step(2048, 33) == ARGUMENT and step(65535, 65535) == ARGUMENT  # (past the sizes: no tensors)
+    assert step(65536, 1) == SHAPE and step(1, 65536) == SHAPE and step(1, 0) == SHAPE and step(-1, 2) == SHAPE
