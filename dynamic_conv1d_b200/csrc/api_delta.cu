@@ -22,7 +22,7 @@ int check_widths(int64_t dk, int64_t dv) {
 int check_rule(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype) {
   int s;
   if ((s = check_dtype(dtype))) return s;
-  if (B < 0 || T < 0 || H <= 0 || H > kMaxRows || B * H > kMaxRows || T > (1 << 30))
+  if (B < 0 || B > kMaxRows || T < 0 || H <= 0 || H > kMaxRows || B * H > kMaxRows || T > (1 << 30))
     return set_error(DYNCONV_ERR_SHAPE, "gated delta rule: bad sizes B=%lld T=%lld H=%lld", (long long)B, (long long)T,
                      (long long)H);
   return check_widths(dk, dv);

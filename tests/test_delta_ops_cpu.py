@@ -119,3 +119,10 @@ def test_step_sizes():
     step = lambda B, H: lib.dynconv_delta_step(*([None] * 7), None, 0, None, B, B, H, 64, 64, 1.0, 0, None)  # noqa: E731
     assert step(2048, 33) == ARGUMENT and step(65535, 65535) == ARGUMENT  # (past the sizes: no tensors)
     assert step(65536, 1) == SHAPE and step(1, 65536) == SHAPE and step(1, 0) == SHAPE and step(-1, 2) == SHAPE
+
+
+def test_sizes_whose_product_overflows():
+    lib = _lib.load()
+    for B, H in ((1 << 62, 4), (1 << 48, 1 << 16), (1 << 61, 8)):
+        assert lib.dynconv_delta_fwd(*([None] * 9), 0, None, None, 0, B, 1, H, 64, 64, 1.0, 0, None) == SHAPE
+        assert lib.dynconv_delta_kept_bytes(B, 1, H, 64, 64, 0) == 0
