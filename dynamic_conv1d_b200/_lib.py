@@ -13,6 +13,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdynconv.so")
@@ -174,6 +175,17 @@ def differentiable_once(backward):
         return tuple(out)
 
     return wrapper
+
+
+_is_tracing = torch._C._is_tracing if hasattr(torch._C, "_is_tracing") else torch.jit.is_tracing
+
+
+def watched() -> bool:
+    """Whether somebody watches a call who asks for no gradient: inside a level of forward-mode differentiation,
+    whose tangents a direct call of the library would drop, or under torch.jit.trace, which would record the
+    allocation of the outputs alone.  Such calls go through their autograd Function, which refuses tangents and is
+    recorded as a whole, or are refused."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 or _is_tracing()
 
 
 _same_device = contextlib.nullcontext()

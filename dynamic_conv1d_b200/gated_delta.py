@@ -19,7 +19,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib
 from .linear_attention import _check_state, _dense, _ptr
-from .step import _refuse_gradient, _slots
+from .step import _refuse_gradient, _refuse_watched, _slots
 
 _Strides = {n: ctypes.c_int64 * n for n in (10, 18, 30)}
 
@@ -55,6 +55,8 @@ def _forward(q, k, v, log_decay, beta, initial_state, scale, want_state, keep):
     q, k, v = _rows(q), _rows(k), _rows(v)
     B, T, H, dk = q.shape
     dv = v.shape[-1]
+    if scale is None:
+        scale = dk**-0.5
     lib = _lib.load()
     code = _lib.dtype_code(q.dtype)
     with _lib.device_of(q):
@@ -72,13 +74,13 @@ def _forward(q, k, v, log_decay, beta, initial_state, scale, want_state, keep):
         if status:
             _lib.check(status)
         _lib.after_call(o)
-    return o, s1, q, k, kept
+    return o, s1, q, k, kept, scale
 
 
 class _GatedDeltaRuleFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, beta, initial_state, scale, want_state):
-        o, s1, q, k, kept = _forward(q, k, v, log_decay, beta, initial_state, scale, want_state, True)
+        o, s1, q, k, kept, scale = _forward(q, k, v, log_decay, beta, initial_state, scale, want_state, True)
         ctx.save_for_backward(q, k, log_decay, beta, kept)
         ctx.args = (scale, v.shape[-1], initial_state is not None)
         ctx.set_materialize_grads(False)
@@ -159,9 +161,9 @@ def gated_delta_rule(
     _check_gates(log_decay, beta, q, (B, T, H))
     if initial_state is not None:
         _check_state(initial_state, dev, B, H, dk, v.shape[-1])
-    scale = dk**-0.5 if scale is None else float(scale)
+    scale = None if scale is None else float(scale)
     args = (q, k, v, log_decay, beta, initial_state)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)) or _lib.watched():
         o, s1 = _GatedDeltaRuleFn.apply(*args, scale, bool(return_state))
     else:
         o, s1 = _forward(*args, scale, return_state, False)[:2]
@@ -203,6 +205,8 @@ def gated_delta_rule_step(
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad
                                     or log_decay.requires_grad or beta.requires_grad):
         _refuse_gradient()
+    if _lib.watched():
+        _refuse_watched(q, k, v, state, log_decay, beta)
     code = _lib.dtype_code(q.dtype)
     q, k, v = _dense(q), _dense(k), _dense(v)
     sp, sb = (None, 0) if slots is None else _slots(slots, B, dev)

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from .step import _refuse_gradient, _slots
+from .step import _refuse_gradient, _refuse_watched, _slots
 
 _Strides = {n: ctypes.c_int64 * n for n in (6, 12, 21)}
 
@@ -249,6 +249,8 @@ def decay_linear_attention_step(
     assert slots is not None or n >= B
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         _refuse_gradient()
+    if _lib.watched():
+        _refuse_watched(q, k, v, state)
     code = _lib.dtype_code(q.dtype)
     (qb, qh, qd), (kb, kh, kd), (vb, vh, vd) = q.stride(), k.stride(), v.stride()
     if (qd != 1 and dk > 1) or (kd != 1 and dk > 1) or (vd != 1 and dv > 1):

@@ -141,8 +141,8 @@ def gated_rms_norm(
     if gate is not None:
         assert gate.get_device() == x.get_device() and gate.shape == x.shape and gate.dtype == x.dtype
     eps, scale = float(eps), float(scale)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (gate is not None and gate.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                     or (gate is not None and gate.requires_grad))) or _lib.watched():
         return _GatedRmsNormFn.apply(x, weight, gate, eps, scale)
     return _gated_forward(x, weight, gate, eps, scale)
 
@@ -227,6 +227,6 @@ def residual_rms_norm(
     else:
         scale, factor = None, float(scale)
     args = (x, residual, weight, scale)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)) or _lib.watched():
         return _ResidualRmsNormFn.apply(*args, factor, float(eps))
     return _residual_forward(*args, factor, float(eps))

@@ -23,6 +23,14 @@ def _refuse_gradient():
     raise RuntimeError("a single-token step has no gradient: call it under torch.no_grad()")
 
 
+def _refuse_watched(*tensors):
+    """For a call that is watched (``_lib.watched``): it may go on where no tensor has a tangent and no trace is taken."""
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _refuse_gradient()
+    if torch.jit.is_tracing():
+        raise RuntimeError("a single-token step cannot be traced: the trace would not hold what the step updates")
+
+
 def _slots(slots: torch.Tensor, B: int, dev: int):
     """(pointer, bytes of an index) of a slot table on device `dev`."""
     assert slots.get_device() == dev and slots.is_contiguous() and slots.shape == (B,)
@@ -113,6 +121,8 @@ def _lowrank_step(x, z, U, cache, static_w, residual, slots, R, WD, G):
     if torch.is_grad_enabled() and (x.requires_grad or z.requires_grad or U.requires_grad or cache.requires_grad
                                     or (static_w is not None and static_w.requires_grad)):
         _refuse_gradient()
+    if _lib.watched():
+        _refuse_watched(x, z, U, cache, static_w)
     code = _lib.dtype_code(dtype)
     # parameters of another dtype are cast for the call, as by the whole-sequence op
     if z.dtype != dtype:
@@ -158,6 +168,8 @@ def headwise_dynamic_convolution_step(
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or cache.requires_grad
                                     or (static_w is not None and static_w.requires_grad)):
         _refuse_gradient()
+    if _lib.watched():
+        _refuse_watched(x, weight, cache, static_w)
     code = _lib.dtype_code(dtype)
     if weight.dtype != dtype or not weight.is_contiguous():
         weight = weight.to(dtype=dtype).contiguous()
