@@ -57,10 +57,17 @@ int check_norm(int64_t rows, int64_t D, int dtype) {
   return DYNCONV_OK;
 }
 
+// Takes DYNCONV_WEIGHTS_F32 out of `dtype`.
+bool take_w32(int& dtype) {
+  const bool w32 = dtype >= 0 && (dtype & DYNCONV_WEIGHTS_F32);
+  if (w32) dtype -= DYNCONV_WEIGHTS_F32;
+  return w32;
+}
+
 // The gradient of a weight that no row contributes to.
-int zero_sum(void* p, int64_t D, int dtype, cudaStream_t st) {
+int zero_sum(void* p, int64_t D, int dtype, bool w32, cudaStream_t st) {
   if (!p) return DYNCONV_OK;
-  return cuda_status(cudaMemsetAsync(p, 0, D * (dtype == DYNCONV_DTYPE_BF16 ? 2 : 4), st), "norm: gradient of no rows");
+  return cuda_status(cudaMemsetAsync(p, 0, D * (dtype == DYNCONV_DTYPE_BF16 && !w32 ? 2 : 4), st), "norm: gradient of no rows");
 }
 
 }  // namespace
@@ -179,6 +186,7 @@ size_t dynconv_norm_workspace_bytes(int64_t D) {
 int dynconv_gated_norm_fwd(const void* x, const void* weight, const void* gate, void* y, const int64_t* strides, int64_t N,
                            int64_t G, int64_t D, float eps, float scale, int dtype, void* stream) {
   int s;
+  const bool w32 = take_w32(dtype);
   if ((s = op_entry((cudaStream_t)stream))) return s;
   if (N < 0 || G < 0 || (G > 0 && N > ((int64_t)1 << 40) / G)) return set_error(DYNCONV_ERR_SHAPE, "gated_norm: bad sizes N=%lld G=%lld", (long long)N, (long long)G);
   if ((s = check_norm(N * G, D, dtype))) return s;
@@ -188,7 +196,7 @@ int dynconv_gated_norm_fwd(const void* x, const void* weight, const void* gate, 
   p.x = x, p.weight = weight, p.gate = gate, p.y = y;
   p.x_outer = strides[0], p.x_inner = strides[1], p.gate_outer = strides[2], p.gate_inner = strides[3];
   p.N = N, p.G = G, p.D = (int)D, p.eps = eps, p.scale = scale;
-  return norm::gated_launch(p, dtype, false, (cudaStream_t)stream);
+  return norm::gated_launch(p, dtype, w32, false, (cudaStream_t)stream);
 }
 
 int dynconv_gated_norm_bwd(const void* x, const void* weight, const void* gate, const void* dy, void* dx, void* dweight,
@@ -196,10 +204,11 @@ int dynconv_gated_norm_bwd(const void* x, const void* weight, const void* gate, 
                            int64_t D, float eps, float scale, int dtype, void* stream) {
   int s;
   cudaStream_t st = (cudaStream_t)stream;
+  const bool w32 = take_w32(dtype);
   if ((s = op_entry(st))) return s;
   if (N < 0 || G < 0 || (G > 0 && N > ((int64_t)1 << 40) / G)) return set_error(DYNCONV_ERR_SHAPE, "gated_norm: bad sizes N=%lld G=%lld", (long long)N, (long long)G);
   if ((s = check_norm(N * G, D, dtype))) return s;
-  if (N * G == 0) return zero_sum(dweight, D, dtype, st);
+  if (N * G == 0) return zero_sum(dweight, D, dtype, w32, st);
   if (!x || !dy || !strides || (dweight && !weight) || (dgate && !gate)) return set_error(DYNCONV_ERR_ARGUMENT, "gated_norm: null tensor");
   if (dweight && (!workspace || workspace_bytes < dynconv_norm_workspace_bytes(D)))
     return set_error(DYNCONV_ERR_WORKSPACE, "gated_norm: workspace %zu < %zu bytes", workspace_bytes, dynconv_norm_workspace_bytes(D));
@@ -208,12 +217,13 @@ int dynconv_gated_norm_bwd(const void* x, const void* weight, const void* gate, 
   p.part = dweight ? (float*)workspace : nullptr;
   p.x_outer = strides[0], p.x_inner = strides[1], p.gate_outer = strides[2], p.gate_inner = strides[3];
   p.N = N, p.G = G, p.D = (int)D, p.eps = eps, p.scale = scale;
-  return norm::gated_launch(p, dtype, true, st);
+  return norm::gated_launch(p, dtype, w32, true, st);
 }
 
 int dynconv_residual_norm_fwd(const void* x, const void* residual, const void* weight, const void* scale, float factor, void* y,
                               void* h, int64_t N, int64_t D, float eps, int dtype, void* stream) {
   int s;
+  const bool w32 = take_w32(dtype);
   if ((s = op_entry((cudaStream_t)stream))) return s;
   if ((s = check_norm(N, D, dtype))) return s;
   if (N == 0) return DYNCONV_OK;
@@ -221,7 +231,7 @@ int dynconv_residual_norm_fwd(const void* x, const void* residual, const void* w
   norm::Residual p{};
   p.x = x, p.residual = residual, p.weight = weight, p.scale = scale, p.factor = factor, p.y = y, p.h = h;
   p.N = N, p.D = (int)D, p.eps = eps;
-  return norm::residual_launch(p, dtype, false, (cudaStream_t)stream);
+  return norm::residual_launch(p, dtype, w32, false, (cudaStream_t)stream);
 }
 
 int dynconv_residual_norm_bwd(const void* h, const void* x, const void* weight, const void* scale, float factor, const void* dy,
@@ -229,11 +239,12 @@ int dynconv_residual_norm_bwd(const void* h, const void* x, const void* weight, 
                               size_t workspace_bytes, int64_t N, int64_t D, float eps, int dtype, void* stream) {
   int s;
   cudaStream_t st = (cudaStream_t)stream;
+  const bool w32 = take_w32(dtype);
   if ((s = op_entry(st))) return s;
   if ((s = check_norm(N, D, dtype))) return s;
   if (N == 0) {
-    if ((s = zero_sum(dweight, D, dtype, st))) return s;
-    return zero_sum(dscale, D, dtype, st);
+    if ((s = zero_sum(dweight, D, dtype, w32, st))) return s;
+    return zero_sum(dscale, D, dtype, w32, st);
   }
   if (!h || !weight || (dscale && (!x || !scale))) return set_error(DYNCONV_ERR_ARGUMENT, "residual_norm: null tensor");
   const size_t one = dynconv_norm_workspace_bytes(D), need = one * ((dweight != nullptr) + (dscale != nullptr));
@@ -245,7 +256,7 @@ int dynconv_residual_norm_bwd(const void* h, const void* x, const void* weight, 
   p.part_w = dweight ? (float*)workspace : nullptr;
   p.part_s = dscale ? (float*)((char*)workspace + (dweight ? one : 0)) : nullptr;
   p.N = N, p.D = (int)D, p.eps = eps;
-  return norm::residual_launch(p, dtype, true, st);
+  return norm::residual_launch(p, dtype, w32, true, st);
 }
 
 }  // extern "C"

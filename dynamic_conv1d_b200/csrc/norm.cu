@@ -28,9 +28,9 @@ namespace {
 
 constexpr int kPerThread = 16;  // numbers of a row per thread, at most (32 spilled: the backward holds four tensors' and two sums)
 
-// A thread's share of a row, as stored.
+// A thread's share of a row, as stored.  (A float32 weight's eight numbers beside a row in bf16 are two pieces of 16 bytes.)
 template <typename T, int VEC>
-struct alignas(VEC * sizeof(T)) Vec {
+struct alignas(VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) Vec {
   T e[VEC];
 };
 
@@ -98,14 +98,15 @@ __device__ __forceinline__ void store_sums(const float (&acc)[NV * VEC], float* 
   }
 }
 
-// A thread's columns of a weight: held over all rows where its share of a row is small, else read again for each.
-template <typename T, int VEC, int TPR, int NV>
+// A thread's columns of a weight: held over all rows where its share of a row is small, else read again for each.  A
+// weight has the row's type or float32, which keeps the digits of a master weight and of its gradient's sum.
+template <typename W, int VEC, int TPR, int NV>
 struct Columns {
-  using V = Vec<T, VEC>;
+  using V = Vec<W, VEC>;
   static constexpr bool kHeld = VEC * NV <= 8;
   V held[kHeld ? NV : 1];
-  const T* at;
-  __device__ __forceinline__ Columns(const void* p, int lane, int D) : at((const T*)p + lane * VEC) {
+  const W* at;
+  __device__ __forceinline__ Columns(const void* p, int lane, int D) : at((const W*)p + lane * VEC) {
     if constexpr (kHeld) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -171,7 +172,7 @@ __device__ __forceinline__ void walk_ring(int64_t rows, Start&& start, Work&& wo
   }
 }
 
-template <typename T, int VEC, int TPR, int NV>
+template <typename T, typename W, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
   using V = Vec<T, VEC>;
   struct Buf {
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
   const int lane = threadIdx.x % TPR;
   int flip = 0;
   const int64_t rows = p.N * p.G;
-  const Columns<T, VEC, TPR, NV> w(p.weight, lane, p.D);
+  const Columns<W, VEC, TPR, NV> w(p.weight, lane, p.D);
   walk<Buf, TPR, ahead(VEC, NV)>(
       rows,
       [&](int64_t row, Buf& a) {
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             float v = Elem<T>::to_f(a.x[i].e[e]) * r;
-            if (p.weight) v *= Elem<T>::to_f(w[i].e[e]);
+            if (p.weight) v *= Elem<W>::to_f(w[i].e[e]);
             if (p.gate) {
               const float zf = Elem<T>::to_f(a.z[i].e[e]);
               v *= zf * sigmoid(zf);
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
       });
 }
 
-template <typename T, int VEC, int TPR, int NV>
+template <typename T, typename W, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) gated_bwd_kernel(Gated p) {
   using V = Vec<T, VEC>;
   struct Buf {
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) gated_bwd_kernel
   int flip = 0;
   const int64_t rows = p.N * p.G;
   float acc[NV * VEC];
-  const Columns<T, VEC, TPR, NV> w(p.weight, lane, p.D);
+  const Columns<W, VEC, TPR, NV> w(p.weight, lane, p.D);
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc[i] = 0.f;
   walk<Buf, TPR, ahead(VEC, NV)>(
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) gated_bwd_kernel
             for (int e = 0; e < VEC; ++e) {
               const float v = Elem<T>::to_f(a.x[i].e[e]);
               float dn = Elem<T>::to_f(a.d[i].e[e]);
-              if (p.weight) dn *= Elem<T>::to_f(w[i].e[e]);
+              if (p.weight) dn *= Elem<W>::to_f(w[i].e[e]);
               if (p.gate) {
                 const float zf = Elem<T>::to_f(a.z[i].e[e]), g = sigmoid(zf);
                 if constexpr (kKeep) sg[i * VEC + e] = g;
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) gated_bwd_kernel
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             const float v = Elem<T>::to_f(a.x[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
-            const float dw = p.weight ? d * Elem<T>::to_f(w[i].e[e]) : d, vr = v * rs;
+            const float dw = p.weight ? d * Elem<W>::to_f(w[i].e[e]) : d, vr = v * rs;
             if (p.gate) {
               const float zf = Elem<T>::to_f(a.z[i].e[e]);
               float g;
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) gated_bwd_kernel
   if (p.part) store_sums<TPR, VEC, NV>(acc, p.part + (int64_t)blockIdx.x * p.D, p.D);
 }
 
-template <typename T, int VEC, int TPR, int NV>
+template <typename T, typename W, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
   using V = Vec<T, VEC>;
   struct Buf {
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
   };
   const int lane = threadIdx.x % TPR;
   int flip = 0;
-  const Columns<T, VEC, TPR, NV> w(p.weight, lane, p.D), sc(p.scale, lane, p.D);
+  const Columns<W, VEC, TPR, NV> w(p.weight, lane, p.D), sc(p.scale, lane, p.D);
   walk<Buf, TPR, ahead(VEC, NV)>(
       p.N,
       [&](int64_t row, Buf& a) {
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
           V hv;
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            const float f = p.scale ? Elem<T>::to_f(sc[i].e[e]) : p.factor;
+            const float f = p.scale ? Elem<W>::to_f(sc[i].e[e]) : p.factor;
             const float v = fmaf(f, Elem<T>::to_f(a.x[i].e[e]), Elem<T>::to_f(a.r[i].e[e]));
             h[i * VEC + e] = v;
             hv.e[e] = Elem<T>::from_f(v);
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
           if (!in || c >= p.D) continue;
           V y;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) y.e[e] = Elem<T>::from_f(h[i * VEC + e] * r * Elem<T>::to_f(w[i].e[e]));
+          for (int e = 0; e < VEC; ++e) y.e[e] = Elem<T>::from_f(h[i * VEC + e] * r * Elem<W>::to_f(w[i].e[e]));
           *reinterpret_cast<V*>((T*)p.y + row * p.D + c) = y;
         }
       });
@@ -378,7 +379,7 @@ struct Ring {
   static constexpr int kBytes = kStages * kSlot;
 };
 
-template <typename T, int VEC, int TPR, int NV>
+template <typename T, typename W, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_kernel(Residual p) {
   using V = Vec<T, VEC>;
   using R = Ring<T, VEC, TPR, NV>;
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_ker
   const int lane = threadIdx.x % TPR;
   int flip = 0;
   float acc_w[NV * VEC], acc_s[NV * VEC];
-  const Columns<T, VEC, TPR, NV> w(p.weight, lane, p.D), sc(p.scale, lane, p.D);
+  const Columns<W, VEC, TPR, NV> w(p.weight, lane, p.D), sc(p.scale, lane, p.D);
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc_w[i] = acc_s[i] = 0.f;
   auto work = [&](int64_t row, const Buf& a) {
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_ker
                 for (int e = 0; e < VEC; ++e) {
                   const float v = Elem<T>::to_f(a.h[i].e[e]);
                   s.x = fmaf(v, v, s.x);
-                  s.y = fmaf(Elem<T>::to_f(a.d[i].e[e]) * Elem<T>::to_f(w[i].e[e]), v, s.y);
+                  s.y = fmaf(Elem<T>::to_f(a.d[i].e[e]) * Elem<W>::to_f(w[i].e[e]), v, s.y);
                 }
             s = row_sum<TPR>(s, flip);
             const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
@@ -414,9 +415,9 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_ker
     #pragma unroll
               for (int e = 0; e < VEC; ++e) {
                 const float v = Elem<T>::to_f(a.h[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
-                const float t = fmaf(r, fmaf(d, Elem<T>::to_f(w[i].e[e]), -v * m), Elem<T>::to_f(a.u[i].e[e]));
+                const float t = fmaf(r, fmaf(d, Elem<W>::to_f(w[i].e[e]), -v * m), Elem<T>::to_f(a.u[i].e[e]));
                 dt.e[e] = Elem<T>::from_f(t);
-                dx.e[e] = Elem<T>::from_f(t * (p.scale ? Elem<T>::to_f(sc[i].e[e]) : p.factor));
+                dx.e[e] = Elem<T>::from_f(t * (p.scale ? Elem<W>::to_f(sc[i].e[e]) : p.factor));
                 acc_w[i * VEC + e] = fmaf(d, v * r, acc_w[i * VEC + e]);
                 if (p.part_s) acc_s[i * VEC + e] = fmaf(t, Elem<T>::to_f(a.x[i].e[e]), acc_s[i * VEC + e]);
               }
@@ -499,11 +500,12 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restric
   }
 }
 
-// The most numbers that can be read at once: the pointers (or-ed addresses) and strides (or-ed) decide.
-int vec_of(uintptr_t addresses, int64_t strides, int dtype) {
-  const int elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4;
+// The most numbers that can be read at once: the pointers (or-ed addresses; of the weights, of their own type, apart) and
+// strides (or-ed) decide.
+int vec_of(uintptr_t addresses, uintptr_t weights, int64_t strides, int dtype, bool w32) {
+  const int elem = dtype == DYNCONV_DTYPE_BF16 ? 2 : 4, w_elem = w32 ? 4 : elem;
   for (int n : {16 / elem, 2})
-    if (addresses % (n * elem) == 0 && strides % n == 0) return n;
+    if (addresses % (n * elem) == 0 && weights % (n * w_elem < 16 ? n * w_elem : 16) == 0 && strides % n == 0) return n;
   return 1;
 }
 uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
@@ -519,38 +521,38 @@ int64_t grid_of(int64_t rows, int tpr, int per_sm) {
 // vector each (more rows in flight), up to a warp, and wide ones a CTA.  Rows of 513 to 4096 numbers have 8 of them in
 // a thread: 32768 rows of 1024 in bf16 take 48 us forward and 71 us back with 128 threads (72 and 89 us with 256, half
 // of them idle), 8192 rows of 4096 61 and 74 us with 512 (56 and 93 us with 256 of 16 numbers).
-template <typename T, int VEC, typename F>
+template <typename T, typename W, int VEC, typename F>
 int pick(int64_t D, F&& go) {
   constexpr int kNV = kPerThread / VEC;
   constexpr int kOne = VEC >= 4 ? 1 : 4 / VEC;  // vectors per thread of a narrow row
-  if (D <= 8 * VEC * kOne) return go.template operator()<T, VEC, 8, kOne>();
-  if (D <= 16 * VEC * kOne) return go.template operator()<T, VEC, 16, kOne>();
-  if (D <= 32 * VEC * kOne) return go.template operator()<T, VEC, 32, kOne>();
-  if (D <= 32 * kPerThread) return go.template operator()<T, VEC, 32, kNV>();
-  if (D <= 128 * kPerThread / 2) return go.template operator()<T, VEC, 128, kNV / 2>();
-  if (D <= 256 * kPerThread / 2) return go.template operator()<T, VEC, 256, kNV / 2>();
-  if (D <= 512 * kPerThread / 2) return go.template operator()<T, VEC, 512, kNV / 2>();
-  if (D <= 512 * kPerThread) return go.template operator()<T, VEC, 512, kNV>();
-  return go.template operator()<T, VEC, 1024, kNV>();
+  if (D <= 8 * VEC * kOne) return go.template operator()<T, W, VEC, 8, kOne>();
+  if (D <= 16 * VEC * kOne) return go.template operator()<T, W, VEC, 16, kOne>();
+  if (D <= 32 * VEC * kOne) return go.template operator()<T, W, VEC, 32, kOne>();
+  if (D <= 32 * kPerThread) return go.template operator()<T, W, VEC, 32, kNV>();
+  if (D <= 128 * kPerThread / 2) return go.template operator()<T, W, VEC, 128, kNV / 2>();
+  if (D <= 256 * kPerThread / 2) return go.template operator()<T, W, VEC, 256, kNV / 2>();
+  if (D <= 512 * kPerThread / 2) return go.template operator()<T, W, VEC, 512, kNV / 2>();
+  if (D <= 512 * kPerThread) return go.template operator()<T, W, VEC, 512, kNV>();
+  return go.template operator()<T, W, VEC, 1024, kNV>();
 }
 
 struct GatedGo {
   const Gated& p;
   bool backward;
   cudaStream_t st;
-  template <typename T, int VEC, int TPR, int NV>
+  template <typename T, typename W, int VEC, int TPR, int NV>
   int operator()() const {
     Gated q = p;
     const int64_t g = grid_of(q.N * q.G, TPR, backward ? backward_ctas(TPR) : 2048 / cta(TPR));
     if (!backward) {
-      gated_fwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+      gated_fwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
       DYNCONV_CHECK_LAUNCH("gated_fwd_kernel");
       return DYNCONV_OK;
     }
-    gated_bwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+    gated_bwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
     DYNCONV_CHECK_LAUNCH("gated_bwd_kernel");
     if (q.part) {
-      column_sum_kernel<T><<<(unsigned)((q.D + 31) / 32), 1024, 0, st>>>(q.part, (T*)q.dweight, nullptr, nullptr, (int)g, q.D);
+      column_sum_kernel<W><<<(unsigned)((q.D + 31) / 32), 1024, 0, st>>>(q.part, (W*)q.dweight, nullptr, nullptr, (int)g, q.D);
       DYNCONV_CHECK_LAUNCH("column_sum_kernel");
     }
     return DYNCONV_OK;
@@ -561,31 +563,31 @@ struct ResidualGo {
   const Residual& p;
   bool backward;
   cudaStream_t st;
-  template <typename T, int VEC, int TPR, int NV>
+  template <typename T, typename W, int VEC, int TPR, int NV>
   int operator()() const {
     Residual q = p;
     using R = Ring<T, VEC, TPR, NV>;
     const int64_t g = grid_of(q.N, TPR, backward ? backward_ctas(TPR) : 2048 / cta(TPR));
     if (!backward) {
-      residual_fwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+      residual_fwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
       DYNCONV_CHECK_LAUNCH("residual_fwd_kernel");
       return DYNCONV_OK;
     }
     if (R::kBytes) {
-      const cudaError_t e = cudaFuncSetAttribute(residual_bwd_kernel<T, VEC, TPR, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
+      const cudaError_t e = cudaFuncSetAttribute(residual_bwd_kernel<T, W, VEC, TPR, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
       if (e != cudaSuccess) {
         cudaGetLastError();
         return cuda_status(e, "cudaFuncSetAttribute(residual_bwd)");
       }
     }
-    residual_bwd_kernel<T, VEC, TPR, NV><<<(unsigned)g, cta(TPR), R::kBytes, st>>>(q);
+    residual_bwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), R::kBytes, st>>>(q);
     DYNCONV_CHECK_LAUNCH("residual_bwd_kernel");
     if (q.part_w || q.part_s) {
       const float *a = q.part_w, *b = q.part_s;
-      T *oa = (T*)q.dweight, *ob = (T*)q.dscale;
+      W *oa = (W*)q.dweight, *ob = (W*)q.dscale;
       if (!a) a = b, oa = ob;
       const dim3 grid((unsigned)((q.D + 31) / 32), q.part_w && q.part_s ? 2 : 1);
-      column_sum_kernel<T><<<grid, 1024, 0, st>>>(a, oa, b, ob, (int)g, q.D);
+      column_sum_kernel<W><<<grid, 1024, 0, st>>>(a, oa, b, ob, (int)g, q.D);
       DYNCONV_CHECK_LAUNCH("column_sum_kernel");
     }
     return DYNCONV_OK;
@@ -593,11 +595,15 @@ struct ResidualGo {
 };
 
 // vec: numbers that can be read at once, a 16-byte vector of them, two or one.
+template <typename T, typename W, typename Go>
+int with_vec(int64_t D, int vec, const Go& go) {
+  constexpr int kVec = 16 / (int)sizeof(T);
+  return vec == kVec ? pick<T, W, kVec>(D, go) : vec == 2 ? pick<T, W, 2>(D, go) : pick<T, W, 1>(D, go);
+}
 template <typename Go>
-int dispatch(int64_t D, int dtype, int vec, const Go& go) {
-  if (dtype == DYNCONV_DTYPE_BF16)
-    return vec == 8 ? pick<__nv_bfloat16, 8>(D, go) : vec == 2 ? pick<__nv_bfloat16, 2>(D, go) : pick<__nv_bfloat16, 1>(D, go);
-  return vec == 4 ? pick<float, 4>(D, go) : vec == 2 ? pick<float, 2>(D, go) : pick<float, 1>(D, go);
+int dispatch(int64_t D, int dtype, bool w32, int vec, const Go& go) {
+  if (dtype != DYNCONV_DTYPE_BF16) return with_vec<float, float>(D, vec, go);
+  return w32 ? with_vec<__nv_bfloat16, float>(D, vec, go) : with_vec<__nv_bfloat16, __nv_bfloat16>(D, vec, go);
 }
 
 }  // namespace
@@ -605,16 +611,15 @@ int dispatch(int64_t D, int dtype, int vec, const Go& go) {
 // Rows of partial sums that a backward may write.
 int64_t partial_rows() { return (int64_t)sm_count() * 4; }
 
-int gated_launch(const Gated& p, int dtype, bool backward, cudaStream_t st) {
+int gated_launch(const Gated& p, int dtype, bool w32, bool backward, cudaStream_t st) {
   const int64_t strides = p.D | p.x_outer | p.x_inner | (p.gate ? p.gate_outer | p.gate_inner : 0);
-  const uintptr_t all = bits(p.x) | bits(p.weight) | bits(p.gate) | bits(p.y) | bits(p.dy) | bits(p.dx) | bits(p.dgate);
-  return dispatch(p.D, dtype, vec_of(all, strides, dtype), GatedGo{p, backward, st});
+  const uintptr_t all = bits(p.x) | bits(p.gate) | bits(p.y) | bits(p.dy) | bits(p.dx) | bits(p.dgate);
+  return dispatch(p.D, dtype, w32, vec_of(all, bits(p.weight), strides, dtype, w32), GatedGo{p, backward, st});
 }
 
-int residual_launch(const Residual& p, int dtype, bool backward, cudaStream_t st) {
-  const uintptr_t all = bits(p.x) | bits(p.residual) | bits(p.weight) | bits(p.scale) | bits(p.y) | bits(p.h) | bits(p.dy) | bits(p.dh) |
-                        bits(p.dx) | bits(p.dresidual);
-  return dispatch(p.D, dtype, vec_of(all, p.D, dtype), ResidualGo{p, backward, st});
+int residual_launch(const Residual& p, int dtype, bool w32, bool backward, cudaStream_t st) {
+  const uintptr_t all = bits(p.x) | bits(p.residual) | bits(p.y) | bits(p.h) | bits(p.dy) | bits(p.dh) | bits(p.dx) | bits(p.dresidual);
+  return dispatch(p.D, dtype, w32, vec_of(all, bits(p.weight) | bits(p.scale), p.D, dtype, w32), ResidualGo{p, backward, st});
 }
 
 }  // namespace norm

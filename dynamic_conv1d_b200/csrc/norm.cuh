@@ -33,8 +33,9 @@ struct Residual {
 };
 
 int64_t partial_rows();
-int gated_launch(const Gated& p, int dtype, bool backward, cudaStream_t st);
-int residual_launch(const Residual& p, int dtype, bool backward, cudaStream_t st);
+// w32: weight and scale, and their gradients, are float32 whatever the rows' type.
+int gated_launch(const Gated& p, int dtype, bool w32, bool backward, cudaStream_t st);
+int residual_launch(const Residual& p, int dtype, bool w32, bool backward, cudaStream_t st);
 
 }  // namespace norm
 }  // namespace dynconv

@@ -4,7 +4,7 @@
 ``gated_rms_norm`` normalises rows under a gate, one row per head; without weight and gate it is
 the normalisation of queries and keys.  ``residual_rms_norm`` adds a block's output to the residual
 stream and gives the next block its norm.  Sums are float32; the sums over rows behind the gradients
-of weights are added in a fixed order.
+of weights are added in a fixed order.  Weights may be float32 beside bfloat16 rows, and so are their gradients then.
 """
 from __future__ import annotations
 
@@ -67,6 +67,10 @@ def _sum_workspace(lib, like, D, sums):
     return (torch.empty(n, device=like.device, dtype=torch.uint8), n) if n else (None, 0)
 
 
+def _weights_code(weight, like):
+    return 0 if weight is None or weight.dtype == like.dtype else _lib.WEIGHTS_F32
+
+
 def _gated_forward(x, weight, gate, eps, scale):
     x, gate, n, g, strides = _pair(x, gate)
     lib = _lib.load()
@@ -74,7 +78,7 @@ def _gated_forward(x, weight, gate, eps, scale):
     with _lib.device_of(x):
         y = x.new_empty(x.shape)
         status = lib.dynconv_gated_norm_fwd(x.data_ptr(), _ptr(weight), _ptr(gate), y.data_ptr(), strides, n, g, x.shape[-1],
-                                            eps, scale, code, _lib.raw_stream(x))
+                                            eps, scale, code + _weights_code(weight, x), _lib.raw_stream(x))
         if status:
             _lib.check(status)
         _lib.after_call(y)
@@ -105,7 +109,7 @@ class _GatedRmsNormFn(torch.autograd.Function):
             ws, nbytes = _sum_workspace(lib, x, x.shape[-1], 1) if want_w else (None, 0)
             status = lib.dynconv_gated_norm_bwd(
                 x.data_ptr(), _ptr(weight), _ptr(gate), dy.data_ptr(), _ptr(dx), _ptr(dw), _ptr(dg), strides, _ptr(ws), nbytes,
-                n, g, x.shape[-1], eps, scale, code, _lib.raw_stream(x))
+                n, g, x.shape[-1], eps, scale, code + _weights_code(weight, x), _lib.raw_stream(x))
             if status:
                 _lib.check(status)
             _lib.after_call(x)
@@ -114,7 +118,7 @@ class _GatedRmsNormFn(torch.autograd.Function):
 
 def _check_weight(weight, x, name="weight"):
     assert weight.get_device() == x.get_device() and weight.is_contiguous() and weight.shape == x.shape[-1:], f"{name} must be [{x.shape[-1]}]"
-    return weight if weight.dtype == x.dtype else weight.to(x.dtype)
+    return weight if weight.dtype == x.dtype else weight.float()
 
 
 def gated_rms_norm(
@@ -128,7 +132,7 @@ def gated_rms_norm(
 
     Args:
         x:      [..., D] (bfloat16 or float32, CUDA), D <= 16384; views of a fused projection are read in place.
-        weight: [D] or None; cast to x's dtype when it has another one.
+        weight: [D] or None, in x's dtype or float32 (its gradient likewise); cast to float32 when it has another one.
         gate:   of x's shape and dtype, or None.
         scale:  a number; D**-0.5 without weight and gate gives rows of length one.
 
@@ -155,7 +159,7 @@ def _residual_forward(x, residual, weight, scale, factor, eps):
         y, h = torch.empty_like(x), torch.empty_like(x)
         status = lib.dynconv_residual_norm_fwd(
             x.data_ptr(), residual.data_ptr(), weight.data_ptr(), _ptr(scale), factor, y.data_ptr(), h.data_ptr(),
-            x.numel() // D if D else 0, D, eps, code, _lib.raw_stream(x))
+            x.numel() // D if D else 0, D, eps, code + _weights_code(weight, x), _lib.raw_stream(x))
         if status:
             _lib.check(status)
         _lib.after_call(y)
@@ -191,7 +195,8 @@ class _ResidualRmsNormFn(torch.autograd.Function):
             ws, nbytes = _sum_workspace(lib, h, D, int(want_w) + int(want_s))
             status = lib.dynconv_residual_norm_bwd(
                 h.data_ptr(), _ptr(x), weight.data_ptr(), _ptr(scale), factor, _ptr(dy), _ptr(dh), _ptr(dx), _ptr(dr), _ptr(dw),
-                _ptr(ds), _ptr(ws), nbytes, h.numel() // D if D else 0, D, eps, code, _lib.raw_stream(h))
+                _ptr(ds), _ptr(ws), nbytes, h.numel() // D if D else 0, D, eps, code + _weights_code(weight, h),
+                _lib.raw_stream(h))
             if status:
                 _lib.check(status)
             _lib.after_call(h)
@@ -211,7 +216,8 @@ def residual_rms_norm(
 
     Args:
         x, residual: [..., D] (bfloat16 or float32, CUDA, contiguous), D <= 16384.
-        weight:      [D]; scale: a number, or [D].  Cast to x's dtype when they have another one.
+        weight:      [D]; scale: a number, or [D].  In x's dtype or float32 (their gradients likewise); cast to
+                     float32 when one has another, or when the other is float32.
 
     Returns:
         (y, h), both of x's shape; y is the norm of the sum before it is rounded to x's dtype.
@@ -224,6 +230,8 @@ def residual_rms_norm(
     factor = 1.0
     if isinstance(scale, torch.Tensor):
         scale = _check_weight(scale, x, "scale")
+        if scale.dtype != weight.dtype:
+            weight, scale = weight.float(), scale.float()
     else:
         scale, factor = None, float(scale)
     args = (x, residual, weight, scale)

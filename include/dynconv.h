@@ -345,7 +345,10 @@ int dynconv_delta_step(const void* q, const void* k, const void* v, const void* 
 
 /* y = scale * x rsqrt(mean(x^2) + eps) * weight * silu(gate) over rows of D numbers, 1..16384 (no
  * reference counterpart).  weight [D] and gate may be NULL (one).  Rows (n, g), n < N and g < G: x and gate
- * at n * outer + g * inner (`strides`, in elements: outer and inner of x, then of gate), y dense. */
+ * at n * outer + g * inner (`strides`, in elements: outer and inner of x, then of gate), y dense.
+ * dtype + DYNCONV_WEIGHTS_F32, in the calls of both norms and directions alike: weight and scale, and their
+ * gradients, are float32 whatever the rows' type. */
+#define DYNCONV_WEIGHTS_F32 256
 size_t dynconv_norm_workspace_bytes(int64_t D);
 int dynconv_gated_norm_fwd(const void* x, const void* weight, const void* gate, void* y, const int64_t* strides,
                            int64_t N, int64_t G, int64_t D, float eps, float scale, int dtype, void* stream);

@@ -126,3 +126,13 @@ def test_sizes_whose_product_overflows():
     for B, H in ((1 << 62, 4), (1 << 48, 1 << 16), (1 << 61, 8)):
         assert lib.dynconv_delta_fwd(*([None] * 9), 0, None, None, 0, B, 1, H, 64, 64, 1.0, 0, None) == SHAPE
         assert lib.dynconv_delta_kept_bytes(B, 1, H, 64, 64, 0) == 0
+
+
+def test_float32_weights_flag():
+    """Beside either type; what is no type stays none with it."""
+    lib = _lib.load()
+    for dtype, want in ((256, ARGUMENT), (257, ARGUMENT), (258, UNSUPPORTED), (512, UNSUPPORTED), (-256, UNSUPPORTED), (-1, UNSUPPORTED)):
+        assert lib.dynconv_gated_norm_fwd(*([None] * 5), 1, 1, 64, 1e-6, 1.0, dtype, None) == want
+        assert lib.dynconv_gated_norm_bwd(*([None] * 9), 0, 1, 1, 64, 1e-6, 1.0, dtype, None) == want
+        assert lib.dynconv_residual_norm_fwd(*([None] * 4), 1.0, None, None, 1, 64, 1e-6, dtype, None) == want
+        assert lib.dynconv_residual_norm_bwd(*([None] * 4), 1.0, *([None] * 7), 0, 1, 64, 1e-6, dtype, None) == want
