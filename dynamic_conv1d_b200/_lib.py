@@ -20,7 +20,8 @@ LIB_PATH = os.path.join(_HERE, "libdynconv.so")
 
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
-WEIGHTS_F32 = 256  # added to the dtype: the norms' weights and scales are float32
+# added to the dtype: the norms' weights and scales, the gated delta rule's log decays and rates are float32
+WEIGHTS_F32 = GATES_F32 = 256
 _TORCH_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32}
 
 _c_i64 = ctypes.c_int64

@@ -12,6 +12,14 @@ namespace {
 
 constexpr int64_t kMaxRows = 65535;  // grid limits: batch rows and heads of a step, their product in a sequence
 
+// Takes DYNCONV_GATES_F32 or DYNCONV_WEIGHTS_F32, the same number, out of `dtype`.
+static_assert(DYNCONV_GATES_F32 == DYNCONV_WEIGHTS_F32, "one flag");
+bool take_f32(int& dtype) {
+  const bool there = dtype >= 0 && (dtype & DYNCONV_GATES_F32);
+  if (there) dtype -= DYNCONV_GATES_F32;
+  return there;
+}
+
 int check_widths(int64_t dk, int64_t dv) {
   if (dk < 1 || dk > dr::kMaxKey || dv < 1 || dv > dr::kMaxValue)
     return set_error(DYNCONV_ERR_UNSUPPORTED, "gated delta rule: dk=%lld (1..%d), dv=%lld (1..%d)", (long long)dk, dr::kMaxKey,
@@ -57,13 +65,6 @@ int check_norm(int64_t rows, int64_t D, int dtype) {
   return DYNCONV_OK;
 }
 
-// Takes DYNCONV_WEIGHTS_F32 out of `dtype`.
-bool take_w32(int& dtype) {
-  const bool w32 = dtype >= 0 && (dtype & DYNCONV_WEIGHTS_F32);
-  if (w32) dtype -= DYNCONV_WEIGHTS_F32;
-  return w32;
-}
-
 // The gradient of a weight that no row contributes to.
 int zero_sum(void* p, int64_t D, int dtype, bool w32, cudaStream_t st) {
   if (!p) return DYNCONV_OK;
@@ -81,6 +82,7 @@ int dynconv_delta_step(const void* q, const void* k, const void* v, const void* 
                        void* o, const void* slots, int slot_bytes, const int64_t* strides, int64_t B, int64_t n_rows,
                        int64_t H, int64_t dk, int64_t dv, float scale, int dtype, void* stream) {
   int s;
+  const bool gates32 = take_f32(dtype);
   if ((s = op_entry((cudaStream_t)stream))) return s;
   if ((s = check_dtype(dtype))) return s;
   if (B < 0 || B > kMaxRows || H <= 0 || H > kMaxRows)
@@ -97,18 +99,20 @@ int dynconv_delta_step(const void* q, const void* k, const void* v, const void* 
   dr::View* views[5] = {&p.q, &p.k, &p.v, &p.g, &p.beta};
   const void* at[5] = {q, k, v, log_decay, beta};
   for (int i = 0; i < 5; ++i) *views[i] = dr::View{at[i], strides[2 * i], 0, strides[2 * i + 1]};
-  p.o = o, p.state = state, p.slots = slots, p.slot_bytes = slot_bytes;
+  p.gates32 = gates32, p.o = o, p.state = state, p.slots = slots, p.slot_bytes = slot_bytes;
   p.B = B, p.n_rows = n_rows, p.H = (int)H, p.dk = (int)dk, p.dv = (int)dv, p.scale = scale;
   return dr::step_launch(p, dtype, (cudaStream_t)stream);
 }
 
 size_t dynconv_delta_kept_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype) {
+  take_f32(dtype);
   if (check_rule(B, T, H, dk, dv, dtype) || B * T == 0) return 0;
   const dr::Kept n = dr::kept_bytes(B, T, H, dk, dv, dtype);
   return n.states + n.rest;  // (both are multiples of 512)
 }
 
 size_t dynconv_delta_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype, int backward) {
+  take_f32(dtype);
   if (check_rule(B, T, H, dk, dv, dtype) || B * T == 0) return 0;
   return dr::prepared_bytes(nullptr, nullptr, B, T, H, dk, dv, dtype, backward != 0) +
          (backward ? dynconv_delta_kept_bytes(B, T, H, dk, dv, dtype) : 0);
@@ -120,6 +124,7 @@ int dynconv_delta_fwd(const void* q, const void* k, const void* v, const void* l
                       int64_t dv, float scale, int dtype, void* stream) {
   int s;
   cudaStream_t st = (cudaStream_t)stream;
+  const bool gates32 = take_f32(dtype);
   if ((s = op_entry(st))) return s;
   if ((s = check_rule(B, T, H, dk, dv, dtype))) return s;
   if (B * T == 0) return pass_state(initial_state, final_state, B * H * dk * dv, st);
@@ -139,7 +144,7 @@ int dynconv_delta_fwd(const void* q, const void* k, const void* v, const void* l
       (s = check_rows("delta_fwd", p.v, B, T, H, dv, dtype)))
     return s;
   dr::prepared_bytes(&p.pre, workspace, B, T, H, dk, dv, dtype, false);
-  p.s_in = initial_state, p.s_out = final_state;
+  p.gates32 = gates32, p.s_in = initial_state, p.s_out = final_state;
   if (kept) p.states = (__nv_bfloat16*)kept, p.rest = (__nv_bfloat16*)((char*)kept + n.states);
   p.B = (int)B, p.H = (int)H, p.dk = (int)dk, p.dv = (int)dv, p.T = T, p.scale = scale;
   return dr::forward_launch(p, dtype, st);
@@ -152,6 +157,7 @@ int dynconv_delta_bwd(const void* q, const void* k, const void* log_decay, const
                       void* stream) {
   int s;
   cudaStream_t st = (cudaStream_t)stream;
+  const bool gates32 = take_f32(dtype);
   if ((s = op_entry(st))) return s;
   if ((s = check_rule(B, T, H, dk, dv, dtype))) return s;
   if (B * T == 0) return pass_state(d_final_state, d_initial_state, B * H * dk * dv, st);
@@ -174,7 +180,7 @@ int dynconv_delta_bwd(const void* q, const void* k, const void* log_decay, const
     return s;
   dr::prepared_bytes(&p.pre, workspace, B, T, H, dk, dv, dtype, true);
   p.dstates = (__nv_bfloat16*)((char*)workspace + pre), p.du = (__nv_bfloat16*)((char*)workspace + pre + n.states);
-  p.ds_out = d_final_state, p.ds_in = d_initial_state;
+  p.gates32 = gates32, p.ds_out = d_final_state, p.ds_in = d_initial_state;
   p.B = (int)B, p.H = (int)H, p.dk = (int)dk, p.dv = (int)dv, p.T = T, p.scale = scale;
   return dr::backward_launch(p, dtype, st);
 }
@@ -186,7 +192,7 @@ size_t dynconv_norm_workspace_bytes(int64_t D) {
 int dynconv_gated_norm_fwd(const void* x, const void* weight, const void* gate, void* y, const int64_t* strides, int64_t N,
                            int64_t G, int64_t D, float eps, float scale, int dtype, void* stream) {
   int s;
-  const bool w32 = take_w32(dtype);
+  const bool w32 = take_f32(dtype);
   if ((s = op_entry((cudaStream_t)stream))) return s;
   if (N < 0 || G < 0 || (G > 0 && N > ((int64_t)1 << 40) / G)) return set_error(DYNCONV_ERR_SHAPE, "gated_norm: bad sizes N=%lld G=%lld", (long long)N, (long long)G);
   if ((s = check_norm(N * G, D, dtype))) return s;
@@ -204,7 +210,7 @@ int dynconv_gated_norm_bwd(const void* x, const void* weight, const void* gate, 
                            int64_t D, float eps, float scale, int dtype, void* stream) {
   int s;
   cudaStream_t st = (cudaStream_t)stream;
-  const bool w32 = take_w32(dtype);
+  const bool w32 = take_f32(dtype);
   if ((s = op_entry(st))) return s;
   if (N < 0 || G < 0 || (G > 0 && N > ((int64_t)1 << 40) / G)) return set_error(DYNCONV_ERR_SHAPE, "gated_norm: bad sizes N=%lld G=%lld", (long long)N, (long long)G);
   if ((s = check_norm(N * G, D, dtype))) return s;
@@ -223,7 +229,7 @@ int dynconv_gated_norm_bwd(const void* x, const void* weight, const void* gate, 
 int dynconv_residual_norm_fwd(const void* x, const void* residual, const void* weight, const void* scale, float factor, void* y,
                               void* h, int64_t N, int64_t D, float eps, int dtype, void* stream) {
   int s;
-  const bool w32 = take_w32(dtype);
+  const bool w32 = take_f32(dtype);
   if ((s = op_entry((cudaStream_t)stream))) return s;
   if ((s = check_norm(N, D, dtype))) return s;
   if (N == 0) return DYNCONV_OK;
@@ -239,7 +245,7 @@ int dynconv_residual_norm_bwd(const void* h, const void* x, const void* weight, 
                               size_t workspace_bytes, int64_t N, int64_t D, float eps, int dtype, void* stream) {
   int s;
   cudaStream_t st = (cudaStream_t)stream;
-  const bool w32 = take_w32(dtype);
+  const bool w32 = take_f32(dtype);
   if ((s = op_entry(st))) return s;
   if ((s = check_norm(N, D, dtype))) return s;
   if (N == 0) {

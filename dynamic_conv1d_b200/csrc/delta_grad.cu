@@ -404,11 +404,11 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       }
       // dbeta: the diagonal of dU r^T
       if (is_n && (rb - (group >> 1)) % R::kStep == 0 && rb >= (group >> 1)) {
-        E* const db = (E*)p.dbeta.p + b * p.dbeta.sb + h * p.dbeta.sh + t0 * p.dbeta.st;
+        const int64_t db = b * p.dbeta.sb + h * p.dbeta.sh + t0 * p.dbeta.st;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int r = 16 * rb + row + 8 * half, c = (row + 8 * half) & 7;  // (the lane that holds column r)
-          if ((c >> 1) == (l & 3) && r < rows) db[r * p.dbeta.st] = Elem<E>::from_f(own[half]);
+          if ((c >> 1) == (l & 3) && r < rows) put_gate<E>(p.dbeta, db + r * p.dbeta.st, own[half], p.gates32);
         }
       }
 #pragma unroll
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       for (int i = 0; i < M; ++i) {
         const int t = l * M + i;
         const float x = total + a[i] + (l < 31 ? later : 0.f) + earlier;
-        if (t < rows) ((E*)p.dg.p)[b * p.dg.sb + h * p.dg.sh + (t0 + t) * p.dg.st] = Elem<E>::from_f(x);
+        if (t < rows) put_gate<E>(p.dg, b * p.dg.sb + h * p.dg.sh + (t0 + t) * p.dg.st, x, p.gates32);
         earlier += e[i];
       }
     }

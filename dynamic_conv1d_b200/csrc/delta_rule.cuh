@@ -61,6 +61,7 @@ struct Prepared {
 
 struct Forward {
   View q, k, v, g, beta, o;   // g: log_decay
+  int gates32;                // g and beta are float32 (else of the tensors' type)
   const float* s_in;          // [B*H][dk][dv] or null (zero)
   float* s_out;               // or null (not wanted)
   // for the backward (null: not wanted), transposed and as 8 x 8 matrices of 128 bytes: the states before the
@@ -76,6 +77,7 @@ struct Forward {
 // One token: q, k, v, g, beta without a time stride.
 struct Step {
   View q, k, v, g, beta;
+  int gates32;
   void* o;
   float* state;
   const void* slots;
@@ -88,6 +90,7 @@ struct Step {
 struct Backward {
   View q, k, g, beta, d_o;
   View dq, dk_, dv_, dg, dbeta;         // written
+  int gates32;                          // so g, beta, dg and dbeta
   const __nv_bfloat16 *states, *rest;   // of the forward
   __nv_bfloat16 *dstates, *du;          // dS1 of the chunks and dU, laid out like them
   const float* ds_out;                  // gradient of the state after the last token, or null
@@ -120,7 +123,7 @@ inline Kept kept_bytes(int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, 
 // Carves the workspace of `Prepared` (at `base`, which may be null); its bytes.
 size_t prepared_bytes(Prepared* p, void* base, int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv, int dtype, bool back);
 // Chains whose state goes back to the caller hold their numbers as three parts (`exact`), as fp32 ones do.
-int prep_launch(const Prepared& to, const View& k, const View& q, const View& v, const View& g, const View& beta, int B, int H,
+int prep_launch(const Prepared& to, const View& k, const View& q, const View& v, const View& g, const View& beta, int gates32, int B, int H,
                 int64_t T, int dk, int dv, float scale, int dtype, bool exact, bool back, cudaStream_t st);
 
 // ---------------------------------------------------------------- matrix instructions
@@ -275,6 +278,20 @@ template <bool EXACT, bool BACK>
 using CfgBf16 = Cfg<1, EXACT ? 3 : 2, 2, 64>;
 using CfgF32 = Cfg<3, 3, 3, 32>;
 __host__ __device__ constexpr int lower(int i, int j) { return i * (i + 1) / 2 + j; }
+
+// A token's log decay or rate, or the gradient of one: float32, or of the tensors' type.  (It is worked with as a sum of two floats
+// anyway, so float32 costs nothing but its bytes, and log decays of long memories need its digits.)
+template <typename E>
+__device__ __forceinline__ float gate_at(const View& v, int64_t at, int gates32) {
+  return gates32 ? ((const float*)v.p)[at] : Elem<E>::to_f(((const E*)v.p)[at]);
+}
+template <typename E>
+__device__ __forceinline__ void put_gate(const View& v, int64_t at, float x, int gates32) {
+  if (gates32)
+    ((float*)v.p)[at] = x;
+  else
+    ((E*)v.p)[at] = Elem<E>::from_f(x);
+}
 
 // Gates of a chunk, as the chains read them.
 template <int C>

@@ -309,7 +309,7 @@ int pick(const Backward& p, cudaStream_t st) {
 // Three parts where the gradient of the first state goes back to the caller, as in the forward.
 int backward_launch(const Backward& p, int dtype, cudaStream_t st) {
   const bool exact = p.ds_in != nullptr;
-  int s = prep_launch(p.pre, p.k, p.q, p.d_o, p.g, p.beta, p.B, p.H, p.T, p.dk, p.dv, p.scale, dtype, exact, true, st);
+  int s = prep_launch(p.pre, p.k, p.q, p.d_o, p.g, p.beta, p.gates32, p.B, p.H, p.T, p.dk, p.dv, p.scale, dtype, exact, true, st);
   if (s) return s;
   s = dtype == DYNCONV_DTYPE_F32 ? pick<CfgF32>(p, st) : exact ? pick<CfgBf16<true, true>>(p, st) : pick<CfgBf16<false, true>>(p, st);
   return s ? s : grad_launch(p, dtype, st);

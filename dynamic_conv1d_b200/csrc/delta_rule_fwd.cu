@@ -359,7 +359,7 @@ int pick(const Forward& p, cudaStream_t st) {
 // the state after the last token goes back to the caller, who gets it in fp32.
 int forward_launch(const Forward& p, int dtype, cudaStream_t st) {
   const bool save = p.states != nullptr, exact = p.s_out != nullptr;
-  const int s = prep_launch(p.pre, p.k, p.q, p.v, p.g, p.beta, p.B, p.H, p.T, p.dk, p.dv, p.scale, dtype, exact, false, st);
+  const int s = prep_launch(p.pre, p.k, p.q, p.v, p.g, p.beta, p.gates32, p.B, p.H, p.T, p.dk, p.dv, p.scale, dtype, exact, false, st);
   if (s) return s;
   if (dtype == DYNCONV_DTYPE_F32) return save ? pick<CfgF32, true>(p, st) : pick<CfgF32, false>(p, st);
   if (exact) return save ? pick<CfgBf16<true, false>, true>(p, st) : pick<CfgBf16<true, false>, false>(p, st);

@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(kThreads, ctas(VEC)) delta_step_kernel(Step p)
   const T* q = (const T*)p.q.p + b * p.q.sb + h * p.q.sh;
   const T* k = (const T*)p.k.p + b * p.k.sb + h * p.k.sh;
   const T* v = (const T*)p.v.p + b * p.v.sb + h * p.v.sh;
-  const float g = Elem<T>::to_f(((const T*)p.g.p)[b * p.g.sb + h * p.g.sh]);
-  const float beta = Elem<T>::to_f(((const T*)p.beta.p)[b * p.beta.sb + h * p.beta.sh]);
+  const float g = gate_at<T>(p.g, b * p.g.sb + h * p.g.sh, p.gates32);
+  const float beta = gate_at<T>(p.beta, b * p.beta.sb + h * p.beta.sh, p.gates32);
   float vv[VEC], kq = 0.f;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) vv[e] = c + e < p.dv ? Elem<T>::to_f(v[c + e]) : 0.f;

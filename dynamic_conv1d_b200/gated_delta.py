@@ -51,6 +51,11 @@ def _workspace(lib, like, B, T, H, dk, dv, code, backward):
     return torch.empty(n, device=like.device, dtype=torch.uint8)
 
 
+def _code(q, log_decay):
+    code = _lib.dtype_code(q.dtype)
+    return code if log_decay.dtype == q.dtype else code + _lib.GATES_F32
+
+
 def _forward(q, k, v, log_decay, beta, initial_state, scale, want_state, keep):
     q, k, v = _rows(q), _rows(k), _rows(v)
     B, T, H, dk = q.shape
@@ -58,7 +63,7 @@ def _forward(q, k, v, log_decay, beta, initial_state, scale, want_state, keep):
     if scale is None:
         scale = dk**-0.5
     lib = _lib.load()
-    code = _lib.dtype_code(q.dtype)
+    code = _code(q, log_decay)
     with _lib.device_of(q):
         o = torch.empty((B, T, H, dv), device=q.device, dtype=q.dtype)
         s1 = torch.empty((B, H, dk, dv), device=q.device, dtype=torch.float32) if want_state else None
@@ -93,13 +98,14 @@ class _GatedDeltaRuleFn(torch.autograd.Function):
         scale, dv, has_state = ctx.args
         B, T, H, dk = q.shape
         lib = _lib.load()
-        code = _lib.dtype_code(q.dtype)
+        code = _code(q, log_decay)
         with _lib.device_of(q):
             do = torch.zeros((B, T, H, dv), device=q.device, dtype=q.dtype) if do is None else _rows(do.to(q.dtype))
             if ds1 is not None:
                 ds1 = ds1.to(torch.float32).contiguous()
-            new = lambda *shape: torch.empty(shape, device=q.device, dtype=q.dtype)  # noqa: E731
-            dq, dk_, dv_, dg, db = new(B, T, H, dk), new(B, T, H, dk), new(B, T, H, dv), new(B, T, H), new(B, T, H)
+            new = lambda like, *shape: torch.empty(shape, device=q.device, dtype=like.dtype)  # noqa: E731
+            dq, dk_, dv_ = new(q, B, T, H, dk), new(q, B, T, H, dk), new(q, B, T, H, dv)
+            dg, db = new(log_decay, B, T, H), new(beta, B, T, H)
             ds0 = None
             if has_state and ctx.needs_input_grad[5]:
                 ds0 = torch.empty((B, H, dk, dv), device=q.device, dtype=torch.float32)
@@ -118,7 +124,7 @@ class _GatedDeltaRuleFn(torch.autograd.Function):
 def _check_gates(log_decay, beta, like, shape):
     dev = like.get_device()
     assert log_decay.get_device() == dev and beta.get_device() == dev
-    assert log_decay.dtype == like.dtype and beta.dtype == like.dtype
+    assert log_decay.dtype == beta.dtype and (beta.dtype == like.dtype or beta.dtype == torch.float32)
     assert log_decay.shape == shape and beta.shape == shape, f"log_decay and beta must be {list(shape)}"
 
 
@@ -140,8 +146,8 @@ def gated_delta_rule(
                        are meant to have a length of at most one (``gated_rms_norm`` gives them it).
                        B * H <= 65535.
         v:             [B, T, H, dv], dv <= 256.
-        log_decay:     [B, T, H] in q's dtype, the logarithm of each token's decay, <= 0.
-        beta:          [B, T, H] in q's dtype, the share of the value that is replaced.
+        log_decay:     [B, T, H] in q's dtype or float32, the logarithm of each token's decay, <= 0.
+        beta:          [B, T, H] in log_decay's dtype, the share of the value that is replaced.
         initial_state: [B, H, dk, dv] float32, the state before the first token (None: zero).
         scale:         factor of the queries; dk**-0.5 by default.
         return_state:  also return the state after the last token, [B, H, dk, dv] float32.
@@ -186,7 +192,7 @@ def gated_delta_rule_step(
         q, k:            [B, H, dk], v: [B, H, dv] (bfloat16 or float32; views of a fused row will do).
                          B and H up to 65535 each.
         state:           [n, H, dk, dv] float32, contiguous; updated in place.
-        log_decay, beta: [B, H] in q's dtype.
+        log_decay, beta: [B, H], both in q's dtype or both float32.
         slots:           [B] int32 or int64, each sequence's row of the state, none twice; rows
                          outside 0..n-1 touch no state and give zeros.  None: row b (n >= B).
 
@@ -207,7 +213,7 @@ def gated_delta_rule_step(
         _refuse_gradient()
     if _lib.watched():
         _refuse_watched(q, k, v, state, log_decay, beta)
-    code = _lib.dtype_code(q.dtype)
+    code = _code(q, log_decay)
     q, k, v = _dense(q), _dense(k), _dense(v)
     sp, sb = (None, 0) if slots is None else _slots(slots, B, dev)
     (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()

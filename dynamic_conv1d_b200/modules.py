@@ -210,10 +210,10 @@ class ConvolvedGatedDelta(nn.Module):
         self.out = nn.Linear(d_model, d_model, bias=False)
 
     def _gates(self, x: torch.Tensor):
-        """log decays and rates, [..., n_heads] in x's dtype; the decays are worked out in float32."""
+        """log decays and rates, [..., n_heads] float32 (a long memory's decay is lost between two numbers of bf16)."""
         a, b = self.gates(x).split(self.n_heads, -1)
         g = -torch.exp(self.A_log.float()) * torch.nn.functional.softplus(a.float() + self.dt_bias.float())
-        return g.to(x.dtype), torch.sigmoid(b)
+        return g, torch.sigmoid(b.float())
 
     def _heads(self, y: torch.Tensor):
         """Queries and keys of length one, and values, [..., n_heads, d_head], of the convolved [..., 3*d_model]."""

@@ -136,3 +136,16 @@ def test_float32_weights_flag():
         assert lib.dynconv_gated_norm_bwd(*([None] * 9), 0, 1, 1, 64, 1e-6, 1.0, dtype, None) == want
         assert lib.dynconv_residual_norm_fwd(*([None] * 4), 1.0, None, None, 1, 64, 1e-6, dtype, None) == want
         assert lib.dynconv_residual_norm_bwd(*([None] * 4), 1.0, *([None] * 7), 0, 1, 64, 1e-6, dtype, None) == want
+
+
+def test_float32_gates_flag():
+    lib = _lib.load()
+    for dtype, want in ((256, ARGUMENT), (257, ARGUMENT), (258, UNSUPPORTED), (512, UNSUPPORTED), (-256, UNSUPPORTED)):
+        assert lib.dynconv_delta_fwd(*([None] * 9), 0, None, None, 0, 1, 4, 2, 64, 64, 1.0, dtype, None) == want
+        assert lib.dynconv_delta_bwd(*([None] * 5), 0, *([None] * 10), 0, 1, 4, 2, 64, 64, 1.0, dtype, None) == want
+        assert lib.dynconv_delta_step(*([None] * 7), None, 0, None, 1, 1, 2, 64, 64, 1.0, dtype, None) == want
+    # what the rule keeps and works in does not depend on the gates' type
+    for dtype in (0, 1):
+        assert lib.dynconv_delta_kept_bytes(1, 100, 2, 64, 64, dtype + 256) == lib.dynconv_delta_kept_bytes(1, 100, 2, 64, 64, dtype) > 0
+        for back in (0, 1):
+            assert lib.dynconv_delta_workspace_bytes(1, 100, 2, 64, 64, dtype + 256, back) == lib.dynconv_delta_workspace_bytes(1, 100, 2, 64, 64, dtype, back)
