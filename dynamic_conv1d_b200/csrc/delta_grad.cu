@@ -82,7 +82,7 @@ __device__ __forceinline__ void store2(E* to, float x, float y, int n, bool pair
   }
 }
 
-template <typename R>
+template <typename R, typename GT>
 __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, const __grid_constant__ Maps maps, int items, int pairs) {
   constexpr int PX = R::PX, C = R::C, NB = R::NB, PU = R::PU, PS = R::PS, kSlab = R::kSlab, kSquare = R::kSquare;
   constexpr bool kRound = PX > 1;
@@ -404,11 +404,11 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       }
       // dbeta: the diagonal of dU r^T
       if (is_n && (rb - (group >> 1)) % R::kStep == 0 && rb >= (group >> 1)) {
-        const int64_t db = b * p.dbeta.sb + h * p.dbeta.sh + t0 * p.dbeta.st;
+        GT* const db = (GT*)p.dbeta.p + b * p.dbeta.sb + h * p.dbeta.sh + t0 * p.dbeta.st;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int r = 16 * rb + row + 8 * half, c = (row + 8 * half) & 7;  // (the lane that holds column r)
-          if ((c >> 1) == (l & 3) && r < rows) put_gate<E>(p.dbeta, db + r * p.dbeta.st, own[half], p.gates32);
+          if ((c >> 1) == (l & 3) && r < rows) db[r * p.dbeta.st] = Elem<GT>::from_f(own[half]);
         }
       }
 #pragma unroll
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) delta_grad_kernel(Backward p, con
       for (int i = 0; i < M; ++i) {
         const int t = l * M + i;
         const float x = total + a[i] + (l < 31 ? later : 0.f) + earlier;
-        if (t < rows) put_gate<E>(p.dg, b * p.dg.sb + h * p.dg.sh + (t0 + t) * p.dg.st, x, p.gates32);
+        if (t < rows) ((GT*)p.dg.p)[b * p.dg.sb + h * p.dg.sh + (t0 + t) * p.dg.st] = Elem<GT>::from_f(x);
         earlier += e[i];
       }
     }
@@ -581,9 +581,9 @@ bool whole(const View& v, int width, int n, int elem) {
   return width % n == 0 && v.sb % n == 0 && v.st % n == 0 && v.sh % n == 0 && (reinterpret_cast<uintptr_t>(v.p) & (n * elem - 1)) == 0;
 }
 
-template <typename R>
-int go(const Backward& p, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(delta_grad_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
+template <typename R, typename GT>
+int launch(const Backward& p, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(delta_grad_kernel<R, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return cuda_status(e, "cudaFuncSetAttribute(delta_grad)");
@@ -599,9 +599,13 @@ int go(const Backward& p, cudaStream_t st) {
   const int pairs = (whole(p.dv_, p.dv, 2, elem) ? 1 : 0) | (whole(p.dq, p.dk, 2, elem) && whole(p.dk_, p.dk, 2, elem) ? 2 : 0) |
                     (whole(p.dq, p.dk, 4, elem) && whole(p.dk_, p.dk, 4, elem) ? 4 : 0);
   const unsigned grid = (unsigned)(items < sm_count() ? items : sm_count());
-  delta_grad_kernel<R><<<grid, kThreads, R::kBytes, st>>>(p, maps, (int)items, pairs);
+  delta_grad_kernel<R, GT><<<grid, kThreads, R::kBytes, st>>>(p, maps, (int)items, pairs);
   DYNCONV_CHECK_LAUNCH("delta_grad_kernel");
   return DYNCONV_OK;
+}
+template <typename R>
+int go(const Backward& p, cudaStream_t st) {
+  return p.gates32 ? launch<R, float>(p, st) : launch<R, typename R::E>(p, st);
 }
 
 }  // namespace

@@ -311,9 +311,9 @@ struct PrepSmem {
   static constexpr size_t kBytes = 1024 + 2 * (size_t)kSpace + G::kBlocks * 1024 + sizeof(Gates<G::C>);
 };
 
-template <typename G, bool BACK>
+template <typename G, bool BACK, typename GT>
 __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const __grid_constant__ Maps maps, View k, View q, View v, View g,
-                                                              View beta, int gates32, int H, int64_t T, int dk, int dv, float scale) {
+                                                              View beta, int H, int64_t T, int dk, int dv, float scale) {
   constexpr int C = G::C, PX = G::PX, NB = G::kBlocks;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full;
@@ -350,8 +350,8 @@ __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const
 #pragma unroll
     for (int i = 0; i < C / 32; ++i) {  // (zeros behind the last token)
       const int r = lane * (C / 32) + i;
-      own.g[i] = r < rows ? gate_at<E>(g, b * g.sb + h * g.sh + (t0 + r) * g.st, gates32) : 0.f;
-      own.beta[i] = r < rows ? gate_at<E>(beta, b * beta.sb + h * beta.sh + (t0 + r) * beta.st, gates32) : 0.f;
+      own.g[i] = r < rows ? Elem<GT>::to_f(((const GT*)g.p)[b * g.sb + h * g.sh + (t0 + r) * g.st]) : 0.f;
+      own.beta[i] = r < rows ? Elem<GT>::to_f(((const GT*)beta.p)[b * beta.sb + h * beta.sh + (t0 + r) * beta.st]) : 0.f;
     }
     make_gates<C>(s, own, !BACK);
   }
@@ -427,10 +427,10 @@ __global__ void __launch_bounds__(kThreads) delta_prep_kernel(Prepared to, const
   }
 }
 
-template <typename G, bool BACK>
-int go(const Prepared& to, const View& k, const View& q, const View& v, const View& g, const View& beta, int gates32, int B, int H, int64_t T, int dk,
-       int dv, float scale, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(delta_prep_kernel<G, BACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrepSmem<G>::kBytes);
+template <typename G, bool BACK, typename GT>
+int launch(const Prepared& to, const View& k, const View& q, const View& v, const View& g, const View& beta, int B, int H, int64_t T, int dk,
+           int dv, float scale, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(delta_prep_kernel<G, BACK, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrepSmem<G>::kBytes);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return cuda_status(e, "cudaFuncSetAttribute(delta_prep)");
@@ -443,9 +443,16 @@ int go(const Prepared& to, const View& k, const View& q, const View& v, const Vi
   const int64_t blocks = (T + G::C - 1) / G::C * H;
   if (blocks > INT32_MAX) return set_error(DYNCONV_ERR_SHAPE, "gated delta rule: H*T too large");
   const dim3 grid((unsigned)blocks, (unsigned)B);
-  delta_prep_kernel<G, BACK><<<grid, kThreads, PrepSmem<G>::kBytes, st>>>(to, maps, k, q, v, g, beta, gates32, H, T, dk, dv, scale);
+  delta_prep_kernel<G, BACK, GT><<<grid, kThreads, PrepSmem<G>::kBytes, st>>>(to, maps, k, q, v, g, beta, H, T, dk, dv, scale);
   DYNCONV_CHECK_LAUNCH("delta_prep_kernel");
   return DYNCONV_OK;
+}
+
+template <typename G, bool BACK>
+int go(const Prepared& to, const View& k, const View& q, const View& v, const View& g, const View& beta, int gates32, int B, int H, int64_t T,
+       int dk, int dv, float scale, cudaStream_t st) {
+  return gates32 ? launch<G, BACK, float>(to, k, q, v, g, beta, B, H, T, dk, dv, scale, st)
+                 : launch<G, BACK, typename G::T>(to, k, q, v, g, beta, B, H, T, dk, dv, scale, st);
 }
 
 }  // namespace

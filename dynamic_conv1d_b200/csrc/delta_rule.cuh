@@ -61,7 +61,8 @@ struct Prepared {
 
 struct Forward {
   View q, k, v, g, beta, o;   // g: log_decay
-  int gates32;                // g and beta are float32 (else of the tensors' type)
+  int gates32;                // g and beta are float32 (else of the tensors' type; kernels take their type, GT: a branch on
+                              // it cost the preparation 5 us of 61, each load waited for before the next)
   const float* s_in;          // [B*H][dk][dv] or null (zero)
   float* s_out;               // or null (not wanted)
   // for the backward (null: not wanted), transposed and as 8 x 8 matrices of 128 bytes: the states before the
@@ -278,20 +279,6 @@ template <bool EXACT, bool BACK>
 using CfgBf16 = Cfg<1, EXACT ? 3 : 2, 2, 64>;
 using CfgF32 = Cfg<3, 3, 3, 32>;
 __host__ __device__ constexpr int lower(int i, int j) { return i * (i + 1) / 2 + j; }
-
-// A token's log decay or rate, or the gradient of one: float32, or of the tensors' type.  (It is worked with as a sum of two floats
-// anyway, so float32 costs nothing but its bytes, and log decays of long memories need its digits.)
-template <typename E>
-__device__ __forceinline__ float gate_at(const View& v, int64_t at, int gates32) {
-  return gates32 ? ((const float*)v.p)[at] : Elem<E>::to_f(((const E*)v.p)[at]);
-}
-template <typename E>
-__device__ __forceinline__ void put_gate(const View& v, int64_t at, float x, int gates32) {
-  if (gates32)
-    ((float*)v.p)[at] = x;
-  else
-    ((E*)v.p)[at] = Elem<E>::from_f(x);
-}
 
 // Gates of a chunk, as the chains read them.
 template <int C>

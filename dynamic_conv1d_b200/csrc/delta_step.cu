@@ -23,7 +23,7 @@ __host__ __device__ constexpr int slice(int keys) { return 16 * kMaxKey / keys; 
 // CTAs per SM, with a few registers spilled (9 and 8 without: 97 and 113 us in the first and third case above)
 __host__ __device__ constexpr int ctas(int vec) { return vec == 4 ? 10 : 9; }
 
-template <typename T, int VEC, int KEYS>
+template <typename T, typename GT, int VEC, int KEYS>
 __global__ void __launch_bounds__(kThreads, ctas(VEC)) delta_step_kernel(Step p) {
   constexpr int kSlice = slice(KEYS);
   constexpr int kLanes = kSlice / VEC;           // threads across a row
@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(kThreads, ctas(VEC)) delta_step_kernel(Step p)
   const T* q = (const T*)p.q.p + b * p.q.sb + h * p.q.sh;
   const T* k = (const T*)p.k.p + b * p.k.sb + h * p.k.sh;
   const T* v = (const T*)p.v.p + b * p.v.sb + h * p.v.sh;
-  const float g = gate_at<T>(p.g, b * p.g.sb + h * p.g.sh, p.gates32);
-  const float beta = gate_at<T>(p.beta, b * p.beta.sb + h * p.beta.sh, p.gates32);
+  const float g = Elem<GT>::to_f(((const GT*)p.g.p)[b * p.g.sb + h * p.g.sh]);
+  const float beta = Elem<GT>::to_f(((const GT*)p.beta.p)[b * p.beta.sb + h * p.beta.sh]);
   float vv[VEC], kq = 0.f;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) vv[e] = c + e < p.dv ? Elem<T>::to_f(v[c + e]) : 0.f;
@@ -140,18 +140,18 @@ __global__ void __launch_bounds__(kThreads, ctas(VEC)) delta_step_kernel(Step p)
   }
 }
 
-template <typename T, int VEC, int KEYS>
+template <typename T, typename GT, int VEC, int KEYS>
 void launch(const Step& p, cudaStream_t st) {
   const dim3 grid((unsigned)((p.dv + slice(KEYS) - 1) / slice(KEYS)), (unsigned)p.H, (unsigned)p.B);
-  delta_step_kernel<T, VEC, KEYS><<<grid, kThreads, 0, st>>>(p);
+  delta_step_kernel<T, GT, VEC, KEYS><<<grid, kThreads, 0, st>>>(p);
 }
 
-template <typename T>
+template <typename T, typename GT>
 int go(const Step& p, cudaStream_t st) {
   if (p.dv % 4 == 0 && (reinterpret_cast<uintptr_t>(p.state) & 15) == 0)
-    p.dk <= 64 ? launch<T, 4, 64>(p, st) : launch<T, 4, kMaxKey>(p, st);
+    p.dk <= 64 ? launch<T, GT, 4, 64>(p, st) : launch<T, GT, 4, kMaxKey>(p, st);
   else
-    p.dk <= 64 ? launch<T, 1, 64>(p, st) : launch<T, 1, kMaxKey>(p, st);
+    p.dk <= 64 ? launch<T, GT, 1, 64>(p, st) : launch<T, GT, 1, kMaxKey>(p, st);
   DYNCONV_CHECK_LAUNCH("delta_step_kernel");
   return DYNCONV_OK;
 }
@@ -159,7 +159,8 @@ int go(const Step& p, cudaStream_t st) {
 }  // namespace
 
 int step_launch(const Step& p, int dtype, cudaStream_t st) {
-  return dtype == DYNCONV_DTYPE_BF16 ? go<__nv_bfloat16>(p, st) : go<float>(p, st);
+  if (dtype != DYNCONV_DTYPE_BF16) return go<float, float>(p, st);
+  return p.gates32 ? go<__nv_bfloat16, float>(p, st) : go<__nv_bfloat16, __nv_bfloat16>(p, st);
 }
 
 }  // namespace dr
