@@ -1,8 +1,8 @@
 // delta_chain.cuh -- the frame of the two chain kernels of the gated delta rule (formulas: delta_rule.cuh).
 //
-// A CTA walks the chunks of one (batch row, head) for `teams` slices of 16 of v's columns.  A team of W warps holds
-// a slice of the state, transposed: warp w keeps 16 x (128 / W) of it in registers, fp32, in the accumulators' layout,
-// and works out 16 x (C / W) of what belongs to tokens.  What the others need of a warp's numbers
+// A CTA walks the chunks of one (batch row, head) for `teams` slices of 16 of v's columns.  A team of W warps, one for each 16
+// tokens of a chunk, holds a slice of the state, transposed: warp w keeps 16 x (128 / W) of it in registers, fp32, in the
+// accumulators' layout, and works out what belongs to the tokens from 16 w on.  What the others need of a warp's numbers
 // goes through shared memory as bf16 parts in the layout of first operands, 16 bytes per lane.  One thread,
 // of a warp of its own or, where the chains' warps take all registers, of the first team's warp with the fewest blocks
 // of T, right behind a barrier of the team (before it, the whole team waited for the copies' start: 296 and 270 us
@@ -27,10 +27,10 @@ struct Plan {
 };
 
 // KK: pieces of 16 of dk that are worked on, 4 or 8 (behind dk there are zeros).
-template <typename G, int W, int KK_>
+template <typename G, int KK_>
 struct Chain {
   static constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks;
-  static constexpr int TB = NB / W;          // token blocks of a warp
+  static constexpr int W = NB;                     // warps of a team, one for each block of 16 tokens
   static constexpr int KK = KK_, NT = 2 * KK / W;  // a warp's 8-column tiles of the state
   static constexpr int PU = PX == 1 ? 2 : 3;  // parts of what the backward is given
   using E = typename G::T;
@@ -72,8 +72,7 @@ struct Chain {
     int abort_flag;
   };
 
-  // A warp's token block b and the team's barrier.
-  static __device__ __forceinline__ int token_block(int w, int b) { return b == 0 ? w : NB - 1 - w; }
+  // The team's barrier.
   static __device__ __forceinline__ void team_sync(int team) {
     asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(32 * W) : "memory");
   }

@@ -10,11 +10,11 @@ namespace dynconv {
 namespace dr {
 namespace {
 
-template <typename G, int W, int KK>
-__global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_kernel(Backward p, const __grid_constant__ Maps maps, Plan plan) {
-  using Ch = Chain<G, W, KK>;
+template <typename G, int KK>
+__global__ void __launch_bounds__(Chain<G, KK>::kMostThreads, 1) delta_bwd_kernel(Backward p, const __grid_constant__ Maps maps, Plan plan) {
+  using Ch = Chain<G, KK>;
   using E = typename G::T;
-  constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks, TB = Ch::TB, NT = Ch::NT, PU = Ch::PU;
+  constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks, NT = Ch::NT, PU = Ch::PU;
   constexpr int PS = PX == 1 ? 1 : 3, KX = PX > PP ? PX : PP;
   extern __shared__ uint8_t smem_raw[];
   __shared__ typename Ch::Bars bars;
@@ -24,14 +24,14 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
   const int warp = warp_index(), l = threadIdx.x & 31, row = l >> 2, col = 2 * (l & 3);
   Ch::init(bars, Ch::live_teams(plan, p.dv, first_col));
   const typename Ch::Producer producer{smem, bars, plan, maps, p.pre, (int)b, (int)h, chunks, p.dk, p.dv, first_col, bh};
-  if (warp == plan.teams * W) {
+  if (warp == plan.teams * Ch::W) {
     if (l == 0) producer.template walk<true>();
     return;
   }
-  const int team = warp / W, w = (warp + team) % W;
+  const int team = warp / Ch::W, w = (warp + team) % Ch::W;
   const int d0 = first_col + 16 * team, slices = (p.dv + 15) / 16, slice = d0 / 16;
   if (d0 >= p.dv) return;
-  const bool produces = !plan.own_warp && team == 0 && w == W - 1 && l == 0;  // (of the warp with the fewest blocks of T)
+  const bool produces = !plan.own_warp && team == 0 && w == Ch::W - 1 && l == 0;  // (of the warp with the fewest blocks of T)
   if (produces) producer.template start<true>();
   const int bytes = Ch::stage_bytes(plan.teams);
   uint4* const state = (uint4*)(smem + plan.stages * bytes + team * Ch::kTeam);
@@ -119,46 +119,38 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
           }
     }
     // (K dS1)^T
-    float Z[TB][2][4];
+    float Z[2][4];
     {
-      constexpr int L = TB == 1 ? 2 : 1;
-      float z[TB][L][2][4];
+      constexpr int L = 2;
+      float z[L][2][4];
 #pragma unroll
-      for (int t = 0; t < TB; ++t)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int i = 0; i < L; ++i) zero(z[t][i][m]);
-      uint32_t a[2][NP][4], f[2][TB][PX][4];
-      auto fetch = [&](int kk, uint32_t(&a)[NP][4], uint32_t(&f)[TB][PX][4]) {
+        for (int i = 0; i < L; ++i) zero(z[i][m]);
+      uint32_t a[2][NP][4], f[2][PX][4];
+      auto fetch = [&](int kk, uint32_t(&a)[NP][4], uint32_t(&f)[PX][4]) {
         Ch::template get<NP>(state + kk * NP * 32, a);
 #pragma unroll
-        for (int t = 0; t < TB; ++t)
-#pragma unroll
-          for (int i = 0; i < PX; ++i) ldsm(f[t][i], s.k() + across.at<C>(Ch::token_block(w, t), kk) + i * G::kTile * 2);
+        for (int i = 0; i < PX; ++i) ldsm(f[i], s.k() + across.at<C>(w, kk) + i * G::kTile * 2);
       };
       fetch(0, a[0], f[0]);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         if (kk + 1 < KK) fetch(kk + 1, a[(kk + 1) & 1], f[(kk + 1) & 1]);
-#pragma unroll
-        for (int t = 0; t < TB; ++t) mma_levels<NP, PX, NP, L>(z[t], a[kk & 1], f[kk & 1][t]);
+        mma_levels<NP, PX, NP, L>(z, a[kk & 1], f[kk & 1]);
       }
-#pragma unroll
-      for (int t = 0; t < TB; ++t) sum_levels<L>(Z[t], z[t]);
+      sum_levels<L>(Z, z);
     }
     // what reaches U from outside its own chunk's corrections: P^T dO + e^(b_C - b) K dS1, transposed
-#pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      const int blk = Ch::token_block(w, t);
+    {
       float x[KX][2][4];
 #pragma unroll
       for (int i = 0; i < KX; ++i) zero(x[i][0]), zero(x[i][1]);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        if (i < blk) continue;
+        if (i < w) continue;
         uint32_t f[PP][4];
-        Ch::template get<PP>(s.p() + lower(i, blk) * PP * 32, f);
+        Ch::template get<PP>(s.p() + lower(i, w) * PP * 32, f);
         mma_levels<PX, PP, KX, KX>(x, dO[i], f);
       }
       float y[2][4];
@@ -166,18 +158,18 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
       float scaled[2][4];  // scale e^b dO of these tokens
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const float2 out = *reinterpret_cast<const float2*>(gate.out + 16 * blk + 8 * m + col);
-        const float2 eb = *reinterpret_cast<const float2*>(gate.e + 16 * blk + 8 * m + col);
+        const float2 out = *reinterpret_cast<const float2*>(gate.out + 16 * w + 8 * m + col);
+        const float2 eb = *reinterpret_cast<const float2*>(gate.e + 16 * w + 8 * m + col);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          y[m][e] = fmaf(e & 1 ? out.y : out.x, Z[t][m][e], y[m][e]);
+          y[m][e] = fmaf(e & 1 ? out.y : out.x, Z[m][e], y[m][e]);
           float v = 0.f;
 #pragma unroll
           for (int i = PX - 1; i >= 0; --i) {
             uint32_t u = 0;
 #pragma unroll
             for (int j = 0; j < NB; ++j)
-              if (j == blk) u = dO[j][i][2 * m + (e >> 1)];
+              if (j == w) u = dO[j][i][2 * m + (e >> 1)];
             v += e & 1 ? high(u) : low(u);
           }
           scaled[m][e] = v * (p.scale * (e & 1 ? eb.y : eb.x));
@@ -185,50 +177,48 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
       }
       uint32_t a[NP][4];
       operand<NP>(y[0], y[1], a);
-      Ch::put(part_x + blk * NP * 32, a);
+      Ch::put(part_x + w * NP * 32, a);
       operand<NP>(scaled[0], scaled[1], a);
-      Ch::put(part_o + blk * NP * 32, a);
+      Ch::put(part_o + w * NP * 32, a);
     }
     Ch::team_sync(team);
     if (produces && c < chunks - 1) producer.template refill<true>(chunks - 1 - c);
     // dU^T = x^T T
-#pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      const int blk = Ch::token_block(w, t);
+    {
       float u[NP][2][4], U[2][4];
 #pragma unroll
       for (int i = 0; i < NP; ++i) zero(u[i][0]), zero(u[i][1]);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        if (i < blk) continue;
+        if (i < w) continue;
         uint32_t a[NP][4], f[NP][4];
         Ch::template get<NP>(part_x + i * NP * 32, a);
-        Ch::template get<NP>(s.t() + lower(i, blk) * NP * 32, f);
+        Ch::template get<NP>(s.t() + lower(i, w) * NP * 32, f);
         mma_levels<NP, NP, NP, NP>(u, a, f);
       }
       sum_levels<NP>(U, u);
-      if (bad > 16 * blk) {
+      if (bad > 16 * w) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (16 * blk + 8 * m + col + (e & 1) < bad) U[m][e] = NAN;
+            if (16 * w + 8 * m + col + (e & 1) < bad) U[m][e] = NAN;
       }
       uint32_t a_u[PU][4];
       operand<PU>(U[0], U[1], a_u);
 #pragma unroll
       for (int i = 0; i < PU; ++i)
-        Ch::keep(p.du + ((((i * (int64_t)p.B * p.H + bh) * chunks + c) * slices + slice) * NB + blk) * 256, a_u[i]);
+        Ch::keep(p.du + ((((i * (int64_t)p.B * p.H + bh) * chunks + c) * slices + slice) * NB + w) * 256, a_u[i]);
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const float2 beta = *reinterpret_cast<const float2*>(gate.beta + 16 * blk + 8 * m + col);
-        const float2 eb = *reinterpret_cast<const float2*>(gate.e + 16 * blk + 8 * m + col);
+        const float2 beta = *reinterpret_cast<const float2*>(gate.beta + 16 * w + 8 * m + col);
+        const float2 eb = *reinterpret_cast<const float2*>(gate.e + 16 * w + 8 * m + col);
 #pragma unroll
         for (int e = 0; e < 4; ++e) U[m][e] *= -(e & 1 ? beta.y * eb.y : beta.x * eb.x);
       }
       uint32_t a[NP][4];
       operand<NP>(U[0], U[1], a);
-      Ch::put(part_u + blk * NP * 32, a);
+      Ch::put(part_u + w * NP * 32, a);
     }
     Ch::team_sync(team);
     // dS0^T = e^(b_C) dS1^T + (scale e^b dO)^T Q - (beta e^b dU)^T K
@@ -282,16 +272,16 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_bwd_ke
   }
 }
 
-template <typename G, int W, int KK>
+template <typename G, int KK>
 int go(const Backward& p, const Plan& plan, cudaStream_t st) {
-  using Ch = Chain<G, W, KK>;
+  using Ch = Chain<G, KK>;
   int s;
   const int slices = (p.dv + 15) / 16, smem = Ch::smem_bytes(plan.teams, plan.stages);
-  if ((s = allow_shared(delta_bwd_kernel<G, W, KK>, Ch::kMostBytes, "cudaFuncSetAttribute(delta_bwd)"))) return s;
+  if ((s = allow_shared(delta_bwd_kernel<G, KK>, Ch::kMostBytes, "cudaFuncSetAttribute(delta_bwd)"))) return s;
   Maps maps{};
   if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.d_o, p.B, p.T, p.H, p.dk, p.dv, plan.teams))) return s;
   const dim3 grid((unsigned)((slices + plan.teams - 1) / plan.teams), (unsigned)(p.B * p.H));
-  delta_bwd_kernel<G, W, KK><<<grid, 32 * (plan.teams * W + plan.own_warp), smem, st>>>(p, maps, plan);
+  delta_bwd_kernel<G, KK><<<grid, 32 * (plan.teams * Ch::W + plan.own_warp), smem, st>>>(p, maps, plan);
   DYNCONV_CHECK_LAUNCH("delta_bwd_kernel");
   return DYNCONV_OK;
 }
@@ -299,9 +289,8 @@ int go(const Backward& p, const Plan& plan, cudaStream_t st) {
 template <typename G>
 int pick(const Backward& p, cudaStream_t st) {
   const int64_t bh = (int64_t)p.B * p.H;
-  constexpr int W = G::kBlocks;  // one block of 16 tokens for each warp
-  if (p.dk <= 64) return go<G, W, 4>(p, plan_of<Chain<G, W, 4>>(bh, p.dv), st);
-  return go<G, W, 8>(p, plan_of<Chain<G, W, 8>>(bh, p.dv), st);
+  if (p.dk <= 64) return go<G, 4>(p, plan_of<Chain<G, 4>>(bh, p.dv), st);
+  return go<G, 8>(p, plan_of<Chain<G, 8>>(bh, p.dv), st);
 }
 
 }  // namespace

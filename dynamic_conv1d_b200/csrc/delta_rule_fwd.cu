@@ -11,11 +11,11 @@ namespace dynconv {
 namespace dr {
 namespace {
 
-template <typename G, int W, int KK, bool SAVE>
-__global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_kernel(Forward p, const __grid_constant__ Maps maps, Plan plan) {
-  using Ch = Chain<G, W, KK>;
+template <typename G, int KK, bool SAVE>
+__global__ void __launch_bounds__(Chain<G, KK>::kMostThreads, 1) delta_fwd_kernel(Forward p, const __grid_constant__ Maps maps, Plan plan) {
+  using Ch = Chain<G, KK>;
   using E = typename G::T;
-  constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks, TB = Ch::TB, NT = Ch::NT, PU = Ch::PU;
+  constexpr int C = G::C, NP = G::NP, PX = G::PX, PP = G::PP, NB = G::kBlocks, NT = Ch::NT, PU = Ch::PU;
   constexpr int PS = PX == 1 ? 1 : 3;  // parts of the state in the outputs' product
   extern __shared__ uint8_t smem_raw[];
   __shared__ typename Ch::Bars bars;
@@ -25,11 +25,11 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
   const int warp = warp_index(), l = threadIdx.x & 31, row = l >> 2, col = 2 * (l & 3);
   Ch::init(bars, Ch::live_teams(plan, p.dv, first_col));
   const typename Ch::Producer producer{smem, bars, plan, maps, p.pre, (int)b, (int)h, chunks, p.dk, p.dv, first_col, bh};
-  if (warp == plan.teams * W) {
+  if (warp == plan.teams * Ch::W) {
     if (l == 0) producer.template walk<false>();
     return;
   }
-  const int team = warp / W, w = (warp + team) % W;  // (turned, so that the last tokens' warps fall on different schedulers)
+  const int team = warp / Ch::W, w = (warp + team) % Ch::W;  // (turned, so that the last tokens' warps fall on different schedulers)
   const int d0 = first_col + 16 * team, slices = (p.dv + 15) / 16, slice = d0 / 16;
   if (d0 >= p.dv) return;
   const bool produces = !plan.own_warp && team == 0 && w == 0 && l == 0;  // (of the warp with the fewest blocks of T)
@@ -89,27 +89,22 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
     const Gates<C>& gate = s.gates();
     int bad = gate.bad;
     // (K S0)^T and (Q S0)^T; the operands of the next 16 of dk are asked for before the products of these
-    float Z[TB][2][4], O[TB][2][4];
+    float Z[2][4], O[2][4];
     {
-      constexpr int L = TB == 1 ? 2 : 1;  // (two token blocks are enough independent work, and the registers they leave)
-      float z[TB][L][2][4], o[TB][L][2][4];
+      constexpr int L = 2;
+      float z[L][2][4], o[L][2][4];
 #pragma unroll
-      for (int t = 0; t < TB; ++t)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int i = 0; i < L; ++i) zero(z[t][i][m]), zero(o[t][i][m]);
-      uint32_t a[2][NP][4], f[2][TB][PX][4], g[2][TB][PX][4];
-      auto fetch = [&](int kk, uint32_t(&a)[NP][4], uint32_t(&f)[TB][PX][4], uint32_t(&g)[TB][PX][4]) {
+        for (int i = 0; i < L; ++i) zero(z[i][m]), zero(o[i][m]);
+      uint32_t a[2][NP][4], f[2][PX][4], g[2][PX][4];
+      auto fetch = [&](int kk, uint32_t(&a)[NP][4], uint32_t(&f)[PX][4], uint32_t(&g)[PX][4]) {
         Ch::template get<NP>(state + kk * NP * 32, a);
+        const uint32_t at = across.at<C>(w, kk);
 #pragma unroll
-        for (int t = 0; t < TB; ++t) {
-          const uint32_t at = across.at<C>(Ch::token_block(w, t), kk);
-#pragma unroll
-          for (int i = 0; i < PX; ++i) {
-            ldsm(f[t][i], s.k() + at + i * G::kTile * 2);
-            ldsm(g[t][i], s.q() + at + i * G::kTile * 2);
-          }
+        for (int i = 0; i < PX; ++i) {
+          ldsm(f[i], s.k() + at + i * G::kTile * 2);
+          ldsm(g[i], s.q() + at + i * G::kTile * 2);
         }
       };
       fetch(0, a[0], f[0], g[0]);
@@ -121,39 +116,33 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
         for (int i = 0; i < PS; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) a_o[i][e] = a[kk & 1][i][e];
-#pragma unroll
-        for (int t = 0; t < TB; ++t) {
-          mma_levels<NP, PX, NP, L>(z[t], a[kk & 1], f[kk & 1][t]);
-          mma_levels<PS, PX, PS, L>(o[t], a_o, g[kk & 1][t]);
-        }
+        mma_levels<NP, PX, NP, L>(z, a[kk & 1], f[kk & 1]);
+        mma_levels<PS, PX, PS, L>(o, a_o, g[kk & 1]);
       }
-#pragma unroll
-      for (int t = 0; t < TB; ++t) sum_levels<L>(Z[t], z[t]), sum_levels<L>(O[t], o[t]);
+      sum_levels<L>(Z, z), sum_levels<L>(O, o);
     }
     // (V - e^b K S0)^T in Z's place, O scaled
     float odd = 0.f;  // NaN if a value is not finite
-#pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      const int t0 = 16 * Ch::token_block(w, t);
+    {
       float v[2][4];
       if constexpr (sizeof(E) == 2) {
         uint32_t f[4];
-        ldsm_t(f, smem_u32(s.v(team, t0 + v_row, v_piece)));
+        ldsm_t(f, smem_u32(s.v(team, 16 * w + v_row, v_piece)));
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i >> 1][2 * (i & 1)] = low(f[i]), v[i >> 1][2 * (i & 1) + 1] = high(f[i]);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          v[i >> 2][i & 3] = s.value(team, t0 + 8 * (i >> 2) + col + (i & 1), row + 8 * ((i >> 1) & 1));
+          v[i >> 2][i & 3] = s.value(team, 16 * w + 8 * (i >> 2) + col + (i & 1), row + 8 * ((i >> 1) & 1));
       }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const float2 eb = *reinterpret_cast<const float2*>(gate.e + t0 + 8 * m + col);
+        const float2 eb = *reinterpret_cast<const float2*>(gate.e + 16 * w + 8 * m + col);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           odd = fmaf(v[m][e], 0.f, odd);
-          Z[t][m][e] = fmaf(-(e & 1 ? eb.y : eb.x), Z[t][m][e], v[m][e]);
-          O[t][m][e] *= p.scale * (e & 1 ? eb.y : eb.x);
+          Z[m][e] = fmaf(-(e & 1 ? eb.y : eb.x), Z[m][e], v[m][e]);
+          O[m][e] *= p.scale * (e & 1 ? eb.y : eb.x);
         }
       }
     }
@@ -162,66 +151,59 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
       // What is not finite must not meet the zeros of T and P: values from the first bad token on count as zero.
       bad = min(bad, Ch::bad_row(s, team, false));
 #pragma unroll
-      for (int t = 0; t < TB; ++t)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (16 * Ch::token_block(w, t) + 8 * m + col + (e & 1) >= bad) Z[t][m][e] = O[t][m][e] = 0.f;
+        for (int e = 0; e < 4; ++e)
+          if (16 * w + 8 * m + col + (e & 1) >= bad) Z[m][e] = O[m][e] = 0.f;
     }
-#pragma unroll
-    for (int t = 0; t < TB; ++t) {
+    {
       uint32_t a[NP][4];
-      operand<NP>(Z[t][0], Z[t][1], a);
-      Ch::put(part_r + Ch::token_block(w, t) * NP * 32, a);
+      operand<NP>(Z[0], Z[1], a);
+      Ch::put(part_r + w * NP * 32, a);
     }
     // (another warp's tokens may be the bad ones)
     if (!Ch::team_all(team, !odd_here)) bad = min(bad, Ch::bad_row(s, team, false));
     if (produces && c > 0) producer.template refill<false>(c);
     // r^T = (V - e^b K S0)^T T^T, U = beta r
-    float U[TB][2][4];
+    float U[2][4];
+    {
+      float u[NP][2][4];
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      const int blk = Ch::token_block(w, t);
-      {
-        float u[NP][2][4];
+      for (int i = 0; i < NP; ++i) zero(u[i][0]), zero(u[i][1]);
+      const uint4* const t_at = s.t() + lower(w, 0) * NP * 32;
 #pragma unroll
-        for (int i = 0; i < NP; ++i) zero(u[i][0]), zero(u[i][1]);
-        const uint4* const t_at = s.t() + lower(blk, 0) * NP * 32;
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          if (j > blk) continue;
-          uint32_t a[NP][4], f[NP][4];
-          Ch::template get<NP>(part_r + j * NP * 32, a);
-          Ch::template get<NP>(t_at + j * NP * 32, f);
-          mma_levels<NP, NP, NP, NP>(u, a, f);
-        }
-        sum_levels<NP>(U[t], u);
+      for (int j = 0; j < NB; ++j) {
+        if (j > w) continue;
+        uint32_t a[NP][4], f[NP][4];
+        Ch::template get<NP>(part_r + j * NP * 32, a);
+        Ch::template get<NP>(t_at + j * NP * 32, f);
+        mma_levels<NP, NP, NP, NP>(u, a, f);
       }
+      sum_levels<NP>(U, u);
       if constexpr (SAVE) {
         uint32_t a[PU][4];
-        operand<PU>(U[t][0], U[t][1], a);
+        operand<PU>(U[0], U[1], a);
 #pragma unroll
         for (int i = 0; i < PU; ++i)
-          Ch::keep(p.rest + ((((i * (int64_t)p.B * p.H + bh) * chunks + c) * slices + slice) * NB + blk) * 256, a[i]);
+          Ch::keep(p.rest + ((((i * (int64_t)p.B * p.H + bh) * chunks + c) * slices + slice) * NB + w) * 256, a[i]);
       }
       float x[2][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const float2 beta = *reinterpret_cast<const float2*>(gate.beta + 16 * blk + 8 * m + col);
-        const float2 out = *reinterpret_cast<const float2*>(gate.out + 16 * blk + 8 * m + col);
+        const float2 beta = *reinterpret_cast<const float2*>(gate.beta + 16 * w + 8 * m + col);
+        const float2 out = *reinterpret_cast<const float2*>(gate.out + 16 * w + 8 * m + col);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          U[t][m][e] *= e & 1 ? beta.y : beta.x;
-          x[m][e] = U[t][m][e] * (e & 1 ? out.y : out.x);
+          U[m][e] *= e & 1 ? beta.y : beta.x;
+          x[m][e] = U[m][e] * (e & 1 ? out.y : out.x);
         }
       }
       uint32_t a[NP][4];
       operand<NP>(x[0], x[1], a);
-      Ch::put(part_s + blk * NP * 32, a);
+      Ch::put(part_s + w * NP * 32, a);
       uint32_t a_u[PU][4];
-      operand<PU>(U[t][0], U[t][1], a_u);
-      Ch::put(part_u + blk * PU * 32, a_u);
+      operand<PU>(U[0], U[1], a_u);
+      Ch::put(part_u + w * PU * 32, a_u);
     }
     Ch::team_sync(team);
     // S^T <- e^(b_C) S^T + (e^(b_C - b) U)^T K, each chunk's sum by itself first: the instruction's own
@@ -258,50 +240,46 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
     // (the state's readers of this chunk passed the barriers above)
     publish(c + 1);
     // O^T += U^T P^T
+    {
+      float o[PU][2][4];
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      const int blk = Ch::token_block(w, t);
-      {
-        float o[PU][2][4];
+      for (int i = 0; i < PU; ++i) zero(o[i][0]), zero(o[i][1]);
+      const uint4* const p_at = s.p() + lower(w, 0) * PP * 32;
 #pragma unroll
-        for (int i = 0; i < PU; ++i) zero(o[i][0]), zero(o[i][1]);
-        const uint4* const p_at = s.p() + lower(blk, 0) * PP * 32;
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          if (j > blk) continue;
-          uint32_t a[PU][4], f[PP][4];
-          Ch::template get<PU>(part_u + j * PU * 32, a);
-          Ch::template get<PP>(p_at + j * PP * 32, f);
-          mma_levels<PU, PP, PU, PU>(o, a, f);
-        }
-        float x[2][4];
-        sum_levels<PU>(x, o);
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) O[t][m][e] += x[m][e];
+      for (int j = 0; j < NB; ++j) {
+        if (j > w) continue;
+        uint32_t a[PU][4], f[PP][4];
+        Ch::template get<PU>(part_u + j * PU * 32, a);
+        Ch::template get<PP>(p_at + j * PP * 32, f);
+        mma_levels<PU, PP, PU, PU>(o, a, f);
       }
+      float x[2][4];
+      sum_levels<PU>(x, o);
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[m][e] += x[m][e];
       if (bad < C) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (16 * blk + 8 * m + col + (e & 1) >= bad) O[t][m][e] = NAN;
+            if (16 * w + 8 * m + col + (e & 1) >= bad) O[m][e] = NAN;
       }
       // through v's tile, of which nobody else needs these tokens and columns any more
-      const int64_t t0 = (int64_t)c * C + 16 * blk;
+      const int64_t t0 = (int64_t)c * C + 16 * w;
       const int rows = (int)(p.T - t0 < 16 ? p.T - t0 : 16);
       E* const to = (E*)p.o.p + b * p.o.sb + h * p.o.sh + t0 * p.o.st + d0;
       if constexpr (sizeof(E) == 2) {
-        stsm_t(smem_u32(s.v(team, 16 * blk + v_row, v_piece)), pack(O[t][0][0], O[t][0][1]), pack(O[t][0][2], O[t][0][3]),
-               pack(O[t][1][0], O[t][1][1]), pack(O[t][1][2], O[t][1][3]));
+        stsm_t(smem_u32(s.v(team, 16 * w + v_row, v_piece)), pack(O[0][0], O[0][1]), pack(O[0][2], O[0][3]),
+               pack(O[1][0], O[1][1]), pack(O[1][2], O[1][3]));
         __syncwarp();
         if (plan.o_vectors) {
           const int r = l >> 1, d = (l & 1) * 8;
-          if (r < rows && d0 + d < p.dv) *reinterpret_cast<uint4*>(to + r * p.o.st + d) = *reinterpret_cast<const uint4*>(s.v(team, 16 * blk + r, l & 1));
+          if (r < rows && d0 + d < p.dv) *reinterpret_cast<uint4*>(to + r * p.o.st + d) = *reinterpret_cast<const uint4*>(s.v(team, 16 * w + r, l & 1));
         } else {
           for (int i = l; i < 16 * rows; i += 32)
-            if (d0 + i % 16 < p.dv) to[i / 16 * p.o.st + i % 16] = s.value(team, 16 * blk + i / 16, i % 16);
+            if (d0 + i % 16 < p.dv) to[i / 16 * p.o.st + i % 16] = s.value(team, 16 * w + i / 16, i % 16);
         }
       } else {
 #pragma unroll
@@ -309,7 +287,7 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 8 * m + col + (e & 1), d = row + 8 * (e >> 1);
-            if (r < rows && d0 + d < p.dv) to[r * p.o.st + d] = O[t][m][e];
+            if (r < rows && d0 + d < p.dv) to[r * p.o.st + d] = O[m][e];
           }
       }
     }
@@ -329,18 +307,18 @@ __global__ void __launch_bounds__(Chain<G, W, KK>::kMostThreads, 1) delta_fwd_ke
   }
 }
 
-template <typename G, int W, int KK, bool SAVE>
+template <typename G, int KK, bool SAVE>
 int go(const Forward& p, Plan plan, cudaStream_t st) {
-  using Ch = Chain<G, W, KK>;
+  using Ch = Chain<G, KK>;
   int s;
   const int slices = (p.dv + 15) / 16;
   plan.o_vectors = vectors_of(p.o, p.dv, sizeof(typename G::T));
   const int smem = Ch::smem_bytes(plan.teams, plan.stages);
-  if ((s = allow_shared(delta_fwd_kernel<G, W, KK, SAVE>, Ch::kMostBytes, "cudaFuncSetAttribute(delta_fwd)"))) return s;
+  if ((s = allow_shared(delta_fwd_kernel<G, KK, SAVE>, Ch::kMostBytes, "cudaFuncSetAttribute(delta_fwd)"))) return s;
   Maps maps{};
   if ((s = chain_maps<G>(&maps, p.pre, p.k, p.q, p.v, p.B, p.T, p.H, p.dk, p.dv, plan.teams))) return s;
   const dim3 grid((unsigned)((slices + plan.teams - 1) / plan.teams), (unsigned)(p.B * p.H));
-  delta_fwd_kernel<G, W, KK, SAVE><<<grid, 32 * (plan.teams * W + plan.own_warp), smem, st>>>(p, maps, plan);
+  delta_fwd_kernel<G, KK, SAVE><<<grid, 32 * (plan.teams * Ch::W + plan.own_warp), smem, st>>>(p, maps, plan);
   DYNCONV_CHECK_LAUNCH("delta_fwd_kernel");
   return DYNCONV_OK;
 }
@@ -348,9 +326,8 @@ int go(const Forward& p, Plan plan, cudaStream_t st) {
 template <typename G, bool SAVE>
 int pick(const Forward& p, cudaStream_t st) {
   const int64_t bh = (int64_t)p.B * p.H;
-  constexpr int W = G::kBlocks;  // one block of 16 tokens for each warp
-  if (p.dk <= 64) return go<G, W, 4, SAVE>(p, plan_of<Chain<G, W, 4>>(bh, p.dv), st);
-  return go<G, W, 8, SAVE>(p, plan_of<Chain<G, W, 8>>(bh, p.dv), st);
+  if (p.dk <= 64) return go<G, 4, SAVE>(p, plan_of<Chain<G, 4>>(bh, p.dv), st);
+  return go<G, 8, SAVE>(p, plan_of<Chain<G, 8>>(bh, p.dv), st);
 }
 
 }  // namespace
