@@ -200,13 +200,14 @@ int chain_maps(Maps* maps, const Prepared& pre, const View& k, const View& q, co
 }
 
 // CTAs of as few teams as let all slices run at once, each then having more of its SM's matrix units and shared
-// memory.
+// memory; and of no more than there are slices, since a team without columns would only take the copies' own warp and
+// a stage (200 chains of 2048 tokens, 64 x 16: 211 us with four teams, 193 with the one that has columns).
 template <typename Ch>
 Plan plan_of(int64_t bh, int dv) {
   const int slices = (dv + 15) / 16;
   Plan p{};
   p.teams = 1;
-  while (2 * p.teams <= Ch::kMostTeams && Ch::smem_bytes(2 * p.teams, 2) <= Ch::kMostBytes && bh * ((slices + p.teams - 1) / p.teams) > sm_count())
+  while (2 * p.teams <= Ch::kMostTeams && p.teams < slices && Ch::smem_bytes(2 * p.teams, 2) <= Ch::kMostBytes && bh * ((slices + p.teams - 1) / p.teams) > sm_count())
     p.teams *= 2;
   p.stages = Ch::smem_bytes(p.teams, 3) <= Ch::kMostBytes ? 3 : 2;
   p.own_warp = p.teams < Ch::kMostTeams;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from dynamic_conv1d_b200 import check_device, gated_delta_rule_step
-from test_gpu_gated_delta import BF16, F32, F32_TOL, STEP, inputs, recurrence, rel
+from test_gpu_gated_delta import BF16, F32, F32_TOL, STEP, check, inputs, recurrence, rel
 
 pytestmark = pytest.mark.gpu
 
@@ -19,3 +19,10 @@ def test_step_of_more_heads_than_a_grid_dimension(dtype):
     ro, rS = recurrence(*(t[:, None].double() for t in ts), S0.double(), 8**-0.5)
     check_device(o)
     assert rel(o, ro[:, 0]) <= (2 * STEP if dtype == BF16 else F32_TOL) and rel(S, rS) <= F32_TOL
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dk,dv", [(64, 16), (128, 16), (128, 32), (64, 48)])
+def test_few_columns_of_many_chains(dtype, dk, dv):
+    """Fewer slices of 16 columns than the teams that so many chains would have."""
+    check(*inputs(4, 130, 50, dk, dv, dtype, seed=dv), states=dv != 32)
