@@ -99,23 +99,50 @@ __device__ __forceinline__ void store_sums(const float (&acc)[NV * VEC], float* 
 }
 
 // A thread's columns of a weight: held over all rows where its share of a row is small, else read again for each.  A
-// weight has the row's type or float32, which keeps the digits of a master weight and of its gradient's sum.
-template <typename W, int VEC, int TPR, int NV>
+// weight has the row's type or float32, which keeps the digits of a master weight and of its gradient's sum.  float32
+// beside rows in bf16 lies in shared memory, each thread's own columns where it alone reads them, but for the small shares of a
+// backward (HOLD).  Residual norm, forward and back: 4096 x 8192 66 and 79 us so, 87 and 147 us read again for each row; 8192 x
+// 4096 48 and 86 us so, 59 and 73 us held.
+template <typename T, typename W, int VEC, int TPR, int NV, bool HOLD>
 struct Columns {
   using V = Vec<W, VEC>;
-  static constexpr bool kHeld = VEC * NV <= 8;
+  static constexpr bool kSmall = VEC * NV <= 8, kStashed = sizeof(W) != sizeof(T) && !(HOLD && kSmall), kHeld = !kStashed && kSmall;
+  static constexpr int kPiece = VEC < 4 ? VEC : 4;  // numbers of a float32 vector that are read at once
+  static constexpr int kBytes = kStashed ? NV * VEC * (int)sizeof(W) * cta(TPR) : 0;
+  using Piece = Vec<W, kPiece>;
   V held[kHeld ? NV : 1];
   const W* at;
-  __device__ __forceinline__ Columns(const void* p, int lane, int D) : at((const W*)p + lane * VEC) {
-    if constexpr (kHeld) {
+  Piece* own;
+  __device__ __forceinline__ Columns(const void* p, int lane, int D, uint8_t* room) : at((const W*)p + lane * VEC), own((Piece*)room + threadIdx.x) {
+    if constexpr (kHeld || kStashed) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (p && (i * TPR + lane) * VEC < D) held[i] = *reinterpret_cast<const V*>(at + i * TPR * VEC);
+        if (p && (i * TPR + lane) * VEC < D) {
+          if constexpr (kHeld) {
+            held[i] = *reinterpret_cast<const V*>(at + i * TPR * VEC);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC / kPiece; ++j)
+              own[(i * (VEC / kPiece) + j) * cta(TPR)] = *reinterpret_cast<const Piece*>(at + i * TPR * VEC + j * kPiece);
+          }
+        }
     }
   }
   __device__ __forceinline__ V operator[](int i) const {
-    if constexpr (kHeld) return held[i];
-    return *reinterpret_cast<const V*>(at + i * TPR * VEC);
+    if constexpr (kHeld) {
+      return held[i];
+    } else if constexpr (kStashed) {
+      V v;
+#pragma unroll
+      for (int j = 0; j < VEC / kPiece; ++j) {
+        const Piece x = own[(i * (VEC / kPiece) + j) * cta(TPR)];
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) v.e[j * kPiece + e] = x.e[e];
+      }
+      return v;
+    } else {
+      return *reinterpret_cast<const V*>(at + i * TPR * VEC);
+    }
   }
 };
 
@@ -172,6 +199,39 @@ __device__ __forceinline__ void walk_ring(int64_t rows, Start&& start, Work&& wo
   }
 }
 
+// The backward's rows in shared memory: a piece of each of N tensors for each thread, as many rows as the CTAs' shares of an SM's
+// shared memory hold beside float32 weights, at most four; none (0) where a piece is not 16 bytes or two rows do not fit.  Of 2-byte
+// types alone: residual norm, 16384 x 2048 in bf16, takes 65 us so and 105 us with one row ahead in registers (3 CTAs on an SM instead
+// of 2: 74 us); of 4-byte types the registers' row is enough already, 62 us for 8192 x 2048 and 66 us with the ring.
+template <typename T, int VEC, int TPR, int NV, int N, int WEIGHTS>
+struct Ring {
+  static constexpr int kSlot = N * NV * cta(TPR) * 16, kFit = (208 * 1024 / backward_ctas(TPR) - WEIGHTS) / kSlot;
+  static constexpr int kStages = sizeof(T) != 2 || VEC != 8 || kFit < 2 ? 0 : kFit < 4 ? kFit : 4;
+  static constexpr int kBytes = kStages * kSlot;
+  // Where a thread's piece i of a tensor lies, and its copy from n numbers behind `from` (null: none).
+  static __device__ __forceinline__ uint8_t* at(uint8_t* ring, int slot, int tensor, int i) {
+    return ring + slot * kSlot + ((tensor * NV + i) * cta(TPR) + threadIdx.x) * 16;
+  }
+  static __device__ __forceinline__ void copy(uint8_t* ring, int slot, int tensor, int i, const void* from, int64_t n) {
+    if (from)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(at(ring, slot, tensor, i))), "l"((const T*)from + n) : "memory");
+  }
+};
+// Those of the two norms.  The gated norm's rows lie in the registers of the bf16 kernel anyway; beside a float32 weight the
+// compiler waits for the next row too early (16384 x 16 x 128: 91 us, 72 us with the ring and with a bf16 weight).
+template <typename T, typename W, int VEC, int TPR, int NV>
+struct GatedBack {
+  using Cols = Columns<T, W, VEC, TPR, NV, true>;
+  using R = Ring<T, VEC, TPR, NV, 3, Cols::kBytes>;
+  static constexpr bool kRing = R::kStages > 0 && sizeof(W) != sizeof(T);
+  static constexpr int kRingBytes = kRing ? R::kBytes : 0;
+};
+template <typename T, typename W, int VEC, int TPR, int NV>
+struct ResidualBack {
+  using Cols = Columns<T, W, VEC, TPR, NV, true>;
+  using R = Ring<T, VEC, TPR, NV, 4, 2 * Cols::kBytes>;
+};
+
 template <typename T, typename W, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
   using V = Vec<T, VEC>;
@@ -181,7 +241,8 @@ __global__ void __launch_bounds__(cta(TPR)) gated_fwd_kernel(Gated p) {
   const int lane = threadIdx.x % TPR;
   int flip = 0;
   const int64_t rows = p.N * p.G;
-  const Columns<W, VEC, TPR, NV> w(p.weight, lane, p.D);
+  extern __shared__ __align__(16) uint8_t room[];
+  const Columns<T, W, VEC, TPR, NV, false> w(p.weight, lane, p.D, room);
   walk<Buf, TPR, ahead(VEC, NV)>(
       rows,
       [&](int64_t row, Buf& a) {
@@ -239,27 +300,13 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) gated_bwd_kernel
   int flip = 0;
   const int64_t rows = p.N * p.G;
   float acc[NV * VEC];
-  const Columns<W, VEC, TPR, NV> w(p.weight, lane, p.D);
+  using B = GatedBack<T, W, VEC, TPR, NV>;
+  using R = typename B::R;
+  extern __shared__ __align__(16) uint8_t room[];
+  const typename B::Cols w(p.weight, lane, p.D, room + B::kRingBytes);
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc[i] = 0.f;
-  walk<Buf, TPR, ahead(VEC, NV)>(
-      rows,
-      [&](int64_t row, Buf& a) {
-        const int64_t n = p.G == 1 ? row : row / p.G, g = row - n * p.G;
-        const T* x = (const T*)p.x + n * p.x_outer + g * p.x_inner;
-        const T* z = (const T*)p.gate + n * p.gate_outer + g * p.gate_inner;
-        const T* dy = (const T*)p.dy + row * p.D;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int c = (i * TPR + lane) * VEC;
-          if (row < rows && c < p.D) {
-            a.x[i] = *reinterpret_cast<const V*>(x + c);
-            a.d[i] = *reinterpret_cast<const V*>(dy + c);
-            if (p.gate) a.z[i] = *reinterpret_cast<const V*>(z + c);
-          }
-        }
-      },
-      [&](int64_t row, const Buf& a) {
+  auto work = [&](int64_t row, const Buf& a) {
         const bool in = row < rows;
         // a narrow row's gates stay in registers between the sums and the gradients; a wide one's are made twice
         constexpr bool kKeep = ahead(VEC, NV);
@@ -311,7 +358,52 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) gated_bwd_kernel
           if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
           if (p.dgate) *reinterpret_cast<V*>((T*)p.dgate + row * p.D + c) = dz;
         }
-      });
+      };
+  if constexpr (B::kRing) {
+    walk_ring<TPR, R::kStages>(
+        rows,
+        [&](int64_t row, int slot) {
+          const int64_t n = p.G == 1 ? row : row / p.G, g = row - n * p.G;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + lane) * VEC;
+            if (row < rows && c < p.D) {
+              R::copy(room, slot, 0, i, p.x, n * p.x_outer + g * p.x_inner + c);
+              R::copy(room, slot, 1, i, p.dy, row * p.D + c);
+              R::copy(room, slot, 2, i, p.gate, n * p.gate_outer + g * p.gate_inner + c);
+            }
+          }
+        },
+        [&](int64_t row, int slot) {
+          Buf a;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            a.x[i] = *reinterpret_cast<const V*>(R::at(room, slot, 0, i));
+            a.d[i] = *reinterpret_cast<const V*>(R::at(room, slot, 1, i));
+            if (p.gate) a.z[i] = *reinterpret_cast<const V*>(R::at(room, slot, 2, i));
+          }
+          work(row, a);
+        });
+  } else {
+    walk<Buf, TPR, ahead(VEC, NV)>(
+        rows,
+        [&](int64_t row, Buf& a) {
+          const int64_t n = p.G == 1 ? row : row / p.G, g = row - n * p.G;
+          const T* x = (const T*)p.x + n * p.x_outer + g * p.x_inner;
+          const T* z = (const T*)p.gate + n * p.gate_outer + g * p.gate_inner;
+          const T* dy = (const T*)p.dy + row * p.D;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + lane) * VEC;
+            if (row < rows && c < p.D) {
+              a.x[i] = *reinterpret_cast<const V*>(x + c);
+              a.d[i] = *reinterpret_cast<const V*>(dy + c);
+              if (p.gate) a.z[i] = *reinterpret_cast<const V*>(z + c);
+            }
+          }
+        },
+        work);
+  }
   if (p.part) store_sums<TPR, VEC, NV>(acc, p.part + (int64_t)blockIdx.x * p.D, p.D);
 }
 
@@ -323,7 +415,9 @@ __global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
   };
   const int lane = threadIdx.x % TPR;
   int flip = 0;
-  const Columns<W, VEC, TPR, NV> w(p.weight, lane, p.D), sc(p.scale, lane, p.D);
+  using Cols = Columns<T, W, VEC, TPR, NV, false>;
+  extern __shared__ __align__(16) uint8_t room[];
+  const Cols w(p.weight, lane, p.D, room), sc(p.scale, lane, p.D, room + Cols::kBytes);
   walk<Buf, TPR, ahead(VEC, NV)>(
       p.N,
       [&](int64_t row, Buf& a) {
@@ -368,21 +462,11 @@ __global__ void __launch_bounds__(cta(TPR)) residual_fwd_kernel(Residual p) {
       });
 }
 
-// The backward's rows in shared memory: four tensors' pieces for each thread, as many rows as the CTAs' shares of an SM's
-// shared memory hold, at most four; none (0) where a piece is not 16 bytes or two rows do not fit.  Of 2-byte
-// types alone: 16384 x 2048 in bf16 takes 65 us so and 105 us with one row ahead in registers (3 CTAs on an SM instead
-// of 2: 74 us); of 4-byte types the registers' row is enough already, 62 us for 8192 x 2048 and 66 us with the ring.
-template <typename T, int VEC, int TPR, int NV>
-struct Ring {
-  static constexpr int kSlot = 4 * NV * cta(TPR) * 16, kFit = 208 * 1024 / backward_ctas(TPR) / kSlot;
-  static constexpr int kStages = sizeof(T) != 2 || VEC != 8 || kFit < 2 ? 0 : kFit < 4 ? kFit : 4;
-  static constexpr int kBytes = kStages * kSlot;
-};
-
 template <typename T, typename W, int VEC, int TPR, int NV>
 __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_kernel(Residual p) {
   using V = Vec<T, VEC>;
-  using R = Ring<T, VEC, TPR, NV>;
+  using R = typename ResidualBack<T, W, VEC, TPR, NV>::R;
+  using Cols = typename ResidualBack<T, W, VEC, TPR, NV>::Cols;
   struct Buf {
     V h[NV], d[NV], u[NV], x[NV];
   };
@@ -390,7 +474,7 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_ker
   const int lane = threadIdx.x % TPR;
   int flip = 0;
   float acc_w[NV * VEC], acc_s[NV * VEC];
-  const Columns<W, VEC, TPR, NV> w(p.weight, lane, p.D), sc(p.scale, lane, p.D);
+  const Cols w(p.weight, lane, p.D, ring + R::kBytes), sc(p.scale, lane, p.D, ring + R::kBytes + Cols::kBytes);
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc_w[i] = acc_s[i] = 0.f;
   auto work = [&](int64_t row, const Buf& a) {
@@ -426,11 +510,6 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_ker
             }
   };
   if constexpr (R::kStages > 0) {
-    auto at = [&](int slot, int tensor, int i) { return ring + slot * R::kSlot + ((tensor * NV + i) * cta(TPR) + threadIdx.x) * 16; };
-    auto copy = [&](int slot, int tensor, int i, const void* from, int64_t n) {
-      if (from)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(at(slot, tensor, i))), "l"((const T*)from + n) : "memory");
-    };
     walk_ring<TPR, R::kStages>(
         p.N,
         [&](int64_t row, int slot) {
@@ -439,8 +518,8 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_ker
             const int c = (i * TPR + lane) * VEC;
             if (row < p.N && c < p.D) {
               const int64_t n = row * p.D + c;
-              copy(slot, 0, i, p.h, n), copy(slot, 1, i, p.dy, n), copy(slot, 2, i, p.dh, n);
-              copy(slot, 3, i, p.part_s ? p.x : nullptr, n);
+              R::copy(ring, slot, 0, i, p.h, n), R::copy(ring, slot, 1, i, p.dy, n), R::copy(ring, slot, 2, i, p.dh, n);
+              R::copy(ring, slot, 3, i, p.part_s ? p.x : nullptr, n);
             }
           }
         },
@@ -448,10 +527,10 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_ker
           Buf a;
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
-            a.h[i] = *reinterpret_cast<const V*>(at(slot, 0, i));
-            a.d[i] = p.dy ? *reinterpret_cast<const V*>(at(slot, 1, i)) : V{};
-            a.u[i] = p.dh ? *reinterpret_cast<const V*>(at(slot, 2, i)) : V{};
-            a.x[i] = *reinterpret_cast<const V*>(at(slot, 3, i));
+            a.h[i] = *reinterpret_cast<const V*>(R::at(ring, slot, 0, i));
+            a.d[i] = p.dy ? *reinterpret_cast<const V*>(R::at(ring, slot, 1, i)) : V{};
+            a.u[i] = p.dh ? *reinterpret_cast<const V*>(R::at(ring, slot, 2, i)) : V{};
+            a.x[i] = *reinterpret_cast<const V*>(R::at(ring, slot, 3, i));
           }
           work(row, a);
         });
@@ -536,6 +615,12 @@ int pick(int64_t D, F&& go) {
   return go.template operator()<T, W, VEC, 1024, kNV>();
 }
 
+// (static shared memory counts too, so any bytes at all are asked for)
+template <typename K>
+int room(K* kern, int bytes) {
+  return bytes == 0 ? DYNCONV_OK : allow_shared(kern, bytes, "cudaFuncSetAttribute(norm)");
+}
+
 struct GatedGo {
   const Gated& p;
   bool backward;
@@ -543,13 +628,17 @@ struct GatedGo {
   template <typename T, typename W, int VEC, int TPR, int NV>
   int operator()() const {
     Gated q = p;
+    constexpr int kRoom = Columns<T, W, VEC, TPR, NV, false>::kBytes;
+    using B = GatedBack<T, W, VEC, TPR, NV>;
     const int64_t g = grid_of(q.N * q.G, TPR, backward ? backward_ctas(TPR) : 2048 / cta(TPR));
     if (!backward) {
-      gated_fwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+      if (int s = room(gated_fwd_kernel<T, W, VEC, TPR, NV>, kRoom)) return s;
+      gated_fwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), q.weight ? kRoom : 0, st>>>(q);
       DYNCONV_CHECK_LAUNCH("gated_fwd_kernel");
       return DYNCONV_OK;
     }
-    gated_bwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+    if (int s = room(gated_bwd_kernel<T, W, VEC, TPR, NV>, B::kRingBytes + B::Cols::kBytes)) return s;
+    gated_bwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), B::kRingBytes + (q.weight ? B::Cols::kBytes : 0), st>>>(q);
     DYNCONV_CHECK_LAUNCH("gated_bwd_kernel");
     if (q.part) {
       column_sum_kernel<W><<<(unsigned)((q.D + 31) / 32), 1024, 0, st>>>(q.part, (W*)q.dweight, nullptr, nullptr, (int)g, q.D);
@@ -566,21 +655,18 @@ struct ResidualGo {
   template <typename T, typename W, int VEC, int TPR, int NV>
   int operator()() const {
     Residual q = p;
-    using R = Ring<T, VEC, TPR, NV>;
+    using B = ResidualBack<T, W, VEC, TPR, NV>;
+    constexpr int kRoom = Columns<T, W, VEC, TPR, NV, false>::kBytes;
+    const int weights = q.scale ? 2 : 1;
     const int64_t g = grid_of(q.N, TPR, backward ? backward_ctas(TPR) : 2048 / cta(TPR));
     if (!backward) {
-      residual_fwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), 0, st>>>(q);
+      if (int s = room(residual_fwd_kernel<T, W, VEC, TPR, NV>, 2 * kRoom)) return s;
+      residual_fwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), weights * kRoom, st>>>(q);
       DYNCONV_CHECK_LAUNCH("residual_fwd_kernel");
       return DYNCONV_OK;
     }
-    if (R::kBytes) {
-      const cudaError_t e = cudaFuncSetAttribute(residual_bwd_kernel<T, W, VEC, TPR, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::kBytes);
-      if (e != cudaSuccess) {
-        cudaGetLastError();
-        return cuda_status(e, "cudaFuncSetAttribute(residual_bwd)");
-      }
-    }
-    residual_bwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), R::kBytes, st>>>(q);
+    if (int s = room(residual_bwd_kernel<T, W, VEC, TPR, NV>, B::R::kBytes + 2 * B::Cols::kBytes)) return s;
+    residual_bwd_kernel<T, W, VEC, TPR, NV><<<(unsigned)g, cta(TPR), B::R::kBytes + weights * B::Cols::kBytes, st>>>(q);
     DYNCONV_CHECK_LAUNCH("residual_bwd_kernel");
     if (q.part_w || q.part_s) {
       const float *a = q.part_w, *b = q.part_s;

@@ -78,6 +78,31 @@ def test_residual(D, scale):
         assert own[3].grad.dtype == BF16 and rel(own[3].grad, (t * x.double()).sum(0)) <= 2 * STEP
 
 
+@pytest.mark.parametrize("N,D", [(80003, 64), (30001, 128), (9001, 520), (5003, 1024), (2502, 2048), (1203, 4096), (907, 8192), (331, 16384)])
+def test_rows_in_turn(N, D):
+    """So many rows that a CTA takes several, and its places in shared memory are used several times over.  Sums of up to
+    80003 products, over at most 34 rows of a thread and 592 CTAs: under 256 additions of 2^-24 in a row."""
+    x, z, dy, dh = (rnd(N, D, dtype=BF16, seed=i) for i in range(4))
+    w, s = weights(D, 5), weights(D, 7) / 2
+    wide = torch.cat([x, z], -1)  # (rows of two tensors side by side)
+    own, ref = [t.detach().requires_grad_() for t in (wide, w)], [t.detach().double().requires_grad_() for t in (x, w, z)]
+    gated_rms_norm(own[0][:, :D], own[1], own[0][:, D:]).backward(dy)
+    gated(*ref, 1e-6, 1.0).backward(dy.double())
+    for a, b in ((own[0].grad[:, :D], ref[0].grad), (own[0].grad[:, D:], ref[2].grad)):
+        assert rel(a, b) <= 2 * STEP
+    assert rel(own[1].grad, ref[1].grad) <= 256 * 2.0**-24
+    own = [t.detach().requires_grad_() for t in (x, z, w, s)]
+    y, h = residual_rms_norm(*own)
+    torch.autograd.backward([y, h], [dy, dh])
+    hd, wd = h.detach().double(), w.double()
+    n = torch.rsqrt(hd.square().mean(-1, keepdim=True) + 1e-6)
+    g = dy.double() * wd
+    t = dh.double() + n * (g - hd * n.square() * (g * hd).mean(-1, keepdim=True))
+    assert rel(own[1].grad, t) <= 2 * STEP and rel(own[0].grad, t * s.double()) <= 2 * STEP
+    assert rel(own[2].grad, (dy.double() * hd * n).sum(0)) <= 256 * 2.0**-24
+    assert rel(own[3].grad, (t * x.double()).sum(0)) <= 256 * 2.0**-24
+
+
 def test_weights_off_16_bytes_and_casts():
     """A float32 weight at any address; one of another type is cast to float32; bf16 beside bf16 stays as it was."""
     x, r, w = rnd(9, 64, dtype=BF16), rnd(9, 64, dtype=BF16, seed=1), weights(64, 2)
