@@ -180,6 +180,7 @@ def differentiable_once(backward):
 
 
 _is_tracing = torch._C._is_tracing if hasattr(torch._C, "_is_tracing") else torch.jit.is_tracing
+_says_level = hasattr(forward_ad, "_current_level")
 
 
 def watched() -> bool:
@@ -187,7 +188,7 @@ def watched() -> bool:
     whose tangents a direct call of the library would drop, or under torch.jit.trace, which would record the
     allocation of the outputs alone.  Such calls go through their autograd Function, which refuses tangents and is
     recorded as a whole, or are refused."""
-    return getattr(forward_ad, "_current_level", 0) >= 0 or _is_tracing()
+    return not _says_level or forward_ad._current_level >= 0 or _is_tracing()
 
 
 _same_device = contextlib.nullcontext()

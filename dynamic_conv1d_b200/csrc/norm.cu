@@ -307,58 +307,58 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) gated_bwd_kernel
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc[i] = 0.f;
   auto work = [&](int64_t row, const Buf& a) {
-        const bool in = row < rows;
-        // a narrow row's gates stay in registers between the sums and the gradients; a wide one's are made twice
-        constexpr bool kKeep = ahead(VEC, NV);
-        float sg[kKeep ? NV * VEC : 1];
-        float2 s = make_float2(0.f, 0.f);
+    const bool in = row < rows;
+    // a narrow row's gates stay in registers between the sums and the gradients; a wide one's are made twice
+    constexpr bool kKeep = ahead(VEC, NV);
+    float sg[kKeep ? NV * VEC : 1];
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (in && (i * TPR + lane) * VEC < p.D)
+    for (int i = 0; i < NV; ++i)
+      if (in && (i * TPR + lane) * VEC < p.D)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const float v = Elem<T>::to_f(a.x[i].e[e]);
-              float dn = Elem<T>::to_f(a.d[i].e[e]);
-              if (p.weight) dn *= Elem<W>::to_f(w[i].e[e]);
-              if (p.gate) {
-                const float zf = Elem<T>::to_f(a.z[i].e[e]), g = sigmoid(zf);
-                if constexpr (kKeep) sg[i * VEC + e] = g;
-                dn *= zf * g;
-              }
-              s.x = fmaf(v, v, s.x);
-              s.y = fmaf(dn, v, s.y);
-            }
-        s = row_sum<TPR>(s, flip);
-        const float r = rsqrtf(s.x / p.D + p.eps), rs = p.scale * r, m = s.y / p.D * r * r;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int c = (i * TPR + lane) * VEC;
-          if (!in || c >= p.D) continue;
-          V dx, dz;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float v = Elem<T>::to_f(a.x[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
-            const float dw = p.weight ? d * Elem<W>::to_f(w[i].e[e]) : d, vr = v * rs;
-            if (p.gate) {
-              const float zf = Elem<T>::to_f(a.z[i].e[e]);
-              float g;
-              if constexpr (kKeep)
-                g = sg[i * VEC + e];
-              else
-                g = sigmoid(zf);
-              const float silu = zf * g;
-              dx.e[e] = Elem<T>::from_f(rs * fmaf(dw, silu, -v * m));
-              dz.e[e] = Elem<T>::from_f(dw * vr * (g + silu * (1.f - g)));
-              acc[i * VEC + e] = fmaf(d * vr, silu, acc[i * VEC + e]);
-            } else {
-              dx.e[e] = Elem<T>::from_f(rs * fmaf(-v, m, dw));
-              acc[i * VEC + e] = fmaf(d, vr, acc[i * VEC + e]);
-            }
+        for (int e = 0; e < VEC; ++e) {
+          const float v = Elem<T>::to_f(a.x[i].e[e]);
+          float dn = Elem<T>::to_f(a.d[i].e[e]);
+          if (p.weight) dn *= Elem<W>::to_f(w[i].e[e]);
+          if (p.gate) {
+            const float zf = Elem<T>::to_f(a.z[i].e[e]), g = sigmoid(zf);
+            if constexpr (kKeep) sg[i * VEC + e] = g;
+            dn *= zf * g;
           }
-          if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
-          if (p.dgate) *reinterpret_cast<V*>((T*)p.dgate + row * p.D + c) = dz;
+          s.x = fmaf(v, v, s.x);
+          s.y = fmaf(dn, v, s.y);
         }
-      };
+    s = row_sum<TPR>(s, flip);
+    const float r = rsqrtf(s.x / p.D + p.eps), rs = p.scale * r, m = s.y / p.D * r * r;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (!in || c >= p.D) continue;
+      V dx, dz;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float v = Elem<T>::to_f(a.x[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
+        const float dw = p.weight ? d * Elem<W>::to_f(w[i].e[e]) : d, vr = v * rs;
+        if (p.gate) {
+          const float zf = Elem<T>::to_f(a.z[i].e[e]);
+          float g;
+          if constexpr (kKeep)
+            g = sg[i * VEC + e];
+          else
+            g = sigmoid(zf);
+          const float silu = zf * g;
+          dx.e[e] = Elem<T>::from_f(rs * fmaf(dw, silu, -v * m));
+          dz.e[e] = Elem<T>::from_f(dw * vr * (g + silu * (1.f - g)));
+          acc[i * VEC + e] = fmaf(d * vr, silu, acc[i * VEC + e]);
+        } else {
+          dx.e[e] = Elem<T>::from_f(rs * fmaf(-v, m, dw));
+          acc[i * VEC + e] = fmaf(d, vr, acc[i * VEC + e]);
+        }
+      }
+      if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
+      if (p.dgate) *reinterpret_cast<V*>((T*)p.dgate + row * p.D + c) = dz;
+    }
+  };
   if constexpr (B::kRing) {
     walk_ring<TPR, R::kStages>(
         rows,
@@ -478,36 +478,36 @@ __global__ void __launch_bounds__(cta(TPR), backward_ctas(TPR)) residual_bwd_ker
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc_w[i] = acc_s[i] = 0.f;
   auto work = [&](int64_t row, const Buf& a) {
-            const bool in = row < p.N;
-            float2 s = make_float2(0.f, 0.f);
-    #pragma unroll
-            for (int i = 0; i < NV; ++i)
-              if (in && (i * TPR + lane) * VEC < p.D)
-    #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                  const float v = Elem<T>::to_f(a.h[i].e[e]);
-                  s.x = fmaf(v, v, s.x);
-                  s.y = fmaf(Elem<T>::to_f(a.d[i].e[e]) * Elem<W>::to_f(w[i].e[e]), v, s.y);
-                }
-            s = row_sum<TPR>(s, flip);
-            const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
-    #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-              const int c = (i * TPR + lane) * VEC;
-              if (!in || c >= p.D) continue;
-              V dt, dx;
-    #pragma unroll
-              for (int e = 0; e < VEC; ++e) {
-                const float v = Elem<T>::to_f(a.h[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
-                const float t = fmaf(r, fmaf(d, Elem<W>::to_f(w[i].e[e]), -v * m), Elem<T>::to_f(a.u[i].e[e]));
-                dt.e[e] = Elem<T>::from_f(t);
-                dx.e[e] = Elem<T>::from_f(t * (p.scale ? Elem<W>::to_f(sc[i].e[e]) : p.factor));
-                acc_w[i * VEC + e] = fmaf(d, v * r, acc_w[i * VEC + e]);
-                if (p.part_s) acc_s[i * VEC + e] = fmaf(t, Elem<T>::to_f(a.x[i].e[e]), acc_s[i * VEC + e]);
-              }
-              if (p.dresidual) *reinterpret_cast<V*>((T*)p.dresidual + row * p.D + c) = dt;
-              if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
-            }
+    const bool in = row < p.N;
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (in && (i * TPR + lane) * VEC < p.D)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float v = Elem<T>::to_f(a.h[i].e[e]);
+          s.x = fmaf(v, v, s.x);
+          s.y = fmaf(Elem<T>::to_f(a.d[i].e[e]) * Elem<W>::to_f(w[i].e[e]), v, s.y);
+        }
+    s = row_sum<TPR>(s, flip);
+    const float r = rsqrtf(s.x / p.D + p.eps), m = s.y / p.D * r * r;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * VEC;
+      if (!in || c >= p.D) continue;
+      V dt, dx;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float v = Elem<T>::to_f(a.h[i].e[e]), d = Elem<T>::to_f(a.d[i].e[e]);
+        const float t = fmaf(r, fmaf(d, Elem<W>::to_f(w[i].e[e]), -v * m), Elem<T>::to_f(a.u[i].e[e]));
+        dt.e[e] = Elem<T>::from_f(t);
+        dx.e[e] = Elem<T>::from_f(t * (p.scale ? Elem<W>::to_f(sc[i].e[e]) : p.factor));
+        acc_w[i * VEC + e] = fmaf(d, v * r, acc_w[i * VEC + e]);
+        if (p.part_s) acc_s[i * VEC + e] = fmaf(t, Elem<T>::to_f(a.x[i].e[e]), acc_s[i * VEC + e]);
+      }
+      if (p.dresidual) *reinterpret_cast<V*>((T*)p.dresidual + row * p.D + c) = dt;
+      if (p.dx) *reinterpret_cast<V*>((T*)p.dx + row * p.D + c) = dx;
+    }
   };
   if constexpr (R::kStages > 0) {
     walk_ring<TPR, R::kStages>(

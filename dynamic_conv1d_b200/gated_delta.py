@@ -122,9 +122,9 @@ class _GatedDeltaRuleFn(torch.autograd.Function):
 
 
 def _check_gates(log_decay, beta, like, shape):
-    dev = like.get_device()
+    dev, dtype = like.get_device(), log_decay.dtype
     assert log_decay.get_device() == dev and beta.get_device() == dev
-    assert log_decay.dtype == beta.dtype and (beta.dtype == like.dtype or beta.dtype == torch.float32)
+    assert dtype == beta.dtype and (dtype == like.dtype or dtype == torch.float32)
     assert log_decay.shape == shape and beta.shape == shape, f"log_decay and beta must be {list(shape)}"
 
 

@@ -67,18 +67,19 @@ def _sum_workspace(lib, like, D, sums):
     return (torch.empty(n, device=like.device, dtype=torch.uint8), n) if n else (None, 0)
 
 
-def _weights_code(weight, like):
-    return 0 if weight is None or weight.dtype == like.dtype else _lib.WEIGHTS_F32
+def _code(like, weight):
+    code = _lib.dtype_code(like.dtype)
+    return code if weight is None or weight.dtype == like.dtype else code + _lib.WEIGHTS_F32
 
 
 def _gated_forward(x, weight, gate, eps, scale):
     x, gate, n, g, strides = _pair(x, gate)
     lib = _lib.load()
-    code = _lib.dtype_code(x.dtype)
+    code = _code(x, weight)
     with _lib.device_of(x):
         y = x.new_empty(x.shape)
         status = lib.dynconv_gated_norm_fwd(x.data_ptr(), _ptr(weight), _ptr(gate), y.data_ptr(), strides, n, g, x.shape[-1],
-                                            eps, scale, code + _weights_code(weight, x), _lib.raw_stream(x))
+                                            eps, scale, code, _lib.raw_stream(x))
         if status:
             _lib.check(status)
         _lib.after_call(y)
@@ -99,7 +100,7 @@ class _GatedRmsNormFn(torch.autograd.Function):
         eps, scale = ctx.args
         x, gate, n, g, strides = _pair(x, gate)
         lib = _lib.load()
-        code = _lib.dtype_code(x.dtype)
+        code = _code(x, weight)
         with _lib.device_of(x):
             dy = dy.contiguous()
             want_x, want_w, want_g = ctx.needs_input_grad[:3]
@@ -109,7 +110,7 @@ class _GatedRmsNormFn(torch.autograd.Function):
             ws, nbytes = _sum_workspace(lib, x, x.shape[-1], 1) if want_w else (None, 0)
             status = lib.dynconv_gated_norm_bwd(
                 x.data_ptr(), _ptr(weight), _ptr(gate), dy.data_ptr(), _ptr(dx), _ptr(dw), _ptr(dg), strides, _ptr(ws), nbytes,
-                n, g, x.shape[-1], eps, scale, code + _weights_code(weight, x), _lib.raw_stream(x))
+                n, g, x.shape[-1], eps, scale, code, _lib.raw_stream(x))
             if status:
                 _lib.check(status)
             _lib.after_call(x)
@@ -153,13 +154,13 @@ def gated_rms_norm(
 
 def _residual_forward(x, residual, weight, scale, factor, eps):
     lib = _lib.load()
-    code = _lib.dtype_code(x.dtype)
+    code = _code(x, weight)
     D = x.shape[-1]
     with _lib.device_of(x):
         y, h = torch.empty_like(x), torch.empty_like(x)
         status = lib.dynconv_residual_norm_fwd(
             x.data_ptr(), residual.data_ptr(), weight.data_ptr(), _ptr(scale), factor, y.data_ptr(), h.data_ptr(),
-            x.numel() // D if D else 0, D, eps, code + _weights_code(weight, x), _lib.raw_stream(x))
+            x.numel() // D if D else 0, D, eps, code, _lib.raw_stream(x))
         if status:
             _lib.check(status)
         _lib.after_call(y)
@@ -183,7 +184,7 @@ class _ResidualRmsNormFn(torch.autograd.Function):
         factor, eps = ctx.args
         D = h.shape[-1]
         lib = _lib.load()
-        code = _lib.dtype_code(h.dtype)
+        code = _code(h, weight)
         with _lib.device_of(h):
             dy = None if dy is None else dy.contiguous()
             dh = None if dh is None else dh.contiguous()
@@ -195,7 +196,7 @@ class _ResidualRmsNormFn(torch.autograd.Function):
             ws, nbytes = _sum_workspace(lib, h, D, int(want_w) + int(want_s))
             status = lib.dynconv_residual_norm_bwd(
                 h.data_ptr(), _ptr(x), weight.data_ptr(), _ptr(scale), factor, _ptr(dy), _ptr(dh), _ptr(dx), _ptr(dr), _ptr(dw),
-                _ptr(ds), _ptr(ws), nbytes, h.numel() // D if D else 0, D, eps, code + _weights_code(weight, h),
+                _ptr(ds), _ptr(ws), nbytes, h.numel() // D if D else 0, D, eps, code,
                 _lib.raw_stream(h))
             if status:
                 _lib.check(status)
