@@ -8,8 +8,9 @@
 // Q K^T and K K^T, entry by entry, are what the log decays' gradients are sums of.  Row sums and column sums
 // of the same numbers are taken, so what has to cancel does.
 //
-// 4 x 4096 tokens, 16 heads of 128 x 128: 440 us for 0.9 GB, bound by its instructions (eight warps of up to 255 registers,
-// a CTA to an SM: issue 32%, matrix units 34%, DRAM 24%); sixteen warps of half as much each took 460 us.
+// 4 x 4096 tokens, 16 heads of 128 x 128: 440 us for 0.9 GB.  No unit is near its limit (issue 32%, matrix units 34%, shared memory
+// 41%, DRAM 24%): eight warps of 255 registers, all that an SM holds, wait for their own instructions, and spill 260 bytes (none
+// with dk <= 64 or in fp32); sixteen warps of half as much each took 460 us.
 // Items go heads first, since the heads of the same tokens share what they read.
 #include "delta_rule.cuh"
 

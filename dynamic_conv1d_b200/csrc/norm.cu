@@ -9,16 +9,21 @@
 //     dt = dh + r (dy w - h r^2 mean(dy w h)),  dresidual = dt,  dx = s dt
 //     dw = sum_rows dy h r,  ds = sum_rows dt x
 // Both sums that a backward row needs (of squares and of dn x) are of its inputs, so one pass over
-// the row gives them and nothing is kept from the forward but h, which the caller has anyway.
+// the row gives them and nothing is kept from the forward but h, which the caller has anyway.  That h is rounded to the
+// rows' type, where y came from the sum itself: in bf16 dw is off by 2.3e-3 of its length, of which its own rounding is 1.6e-3;
+// dx, dresidual and ds show nothing of it.  (The sum itself would have to be made again, from x and residual: two tensors for one.)
 //
-// Bound by HBM: a row is read once into registers (up to 16 numbers per thread) and written once; sums
-// are fp32.  A row belongs to 8..32 lanes of a warp, or to a whole CTA of 128 to 1024 threads above
+// A row is read once into registers (up to 16 numbers per thread) and written once; sums are fp32.  A row belongs to 8..32 lanes of a warp, or to a whole CTA of 128 to 1024 threads above
 // 512 channels.  The sums over rows stay in the threads that own their columns; the CTAs'
 // partial rows are added up in a fixed order by a second launch, so results do not change from
 // run to run.
 //
-// 16384 rows of 2048 in bf16: residual norm 50 us forward (5.4 TB/s), 65 us back (6.2 TB/s); 16384 x 16 rows of 128:
-// gated norm 41 us forward (4.9 TB/s), 74 us back (4.5 TB/s: its instructions, issue 75%).
+// The residual norm is bound by HBM: 16384 rows of 2048 in bf16 take 49 us forward (5.4 TB/s) and 66 us back (6.1 TB/s), in fp32 86
+// and 120 us (6.2 and 6.7 TB/s); 8192 x 4096 in bf16 59 and 73 us (one CTA of 512 threads is all an SM holds of the forward).
+// The gated norm by its instructions: 16384 x 16 rows of 128 in bf16 take 40 us forward (issue 77%, DRAM 50%) and 73 us
+// back (issue 75%, DRAM 49%), in fp32 74 and 147 us.  Rows of more than 8192 numbers belong to 1024 threads of 64 registers: no
+// next row is under way and the backward spills (76 to 736 bytes); 2048 x 16384 in bf16: residual norm 60 and 222 us, gated
+// norm 62 and 253 us; 509 x 8190 in fp32: residual norm 20 and 27 us.
 #include "common.cuh"
 #include "norm.cuh"
 
@@ -589,7 +594,8 @@ int vec_of(uintptr_t addresses, uintptr_t weights, int64_t strides, int dtype, b
 }
 uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
-// CTAs of a launch: as many as run at once, no more than there is work for.
+// CTAs of a launch: per_sm for each SM (a backward's run at once; of a forward's 2048 threads the registers let three
+// eighths to a half do so, the others follow), no more than there is work for.
 int64_t grid_of(int64_t rows, int tpr, int per_sm) {
   const int64_t want = (rows * tpr + cta(tpr) - 1) / cta(tpr);
   const int64_t most = (int64_t)sm_count() * per_sm;

@@ -155,7 +155,7 @@ def gated_delta_rule(
     Returns:
         o [B, T, H, dv], or (o, state).  Differentiable (once) in all tensors.  What is not finite in
         one token reaches no earlier token's output; from it on the head's are NaN (from a value: at
-        least its own columns').
+        least its own columns'; a query is its own token's alone).
         With gradients the call keeps the state at every 64th token (float32: 32nd) in that type's digits and
         four bytes (float32: six) for each number of v.
     """

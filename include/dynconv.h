@@ -319,7 +319,8 @@ int dynconv_la_step(const void* q, const void* k, const void* v, float* state, c
  * The workspace and kept are 16-byte aligned, and so are bf16 (float32) tensors whose width is a multiple of 8 (4),
  * rows and all (DYNCONV_ERR_ALIGN); other widths are read through copies in the workspace.
  * dk in 1..128, dv in 1..256, B*H <= 65535 (the step: below), T <= 2^30.  T = 0 copies the state.  What is not finite in one
- * token reaches no earlier token's output; from it on the head's are NaN (from a value: at least its own columns').
+ * token reaches no earlier token's output; from it on the head's are NaN (from a value: at least its own columns'; a
+ * query is its own token's alone).
  * dtype + DYNCONV_GATES_F32, in any of these calls: log_decay and beta, and their gradients, are float32 whatever the
  * tensors' type. */
 #define DYNCONV_GATES_F32 256
